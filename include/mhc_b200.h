@@ -221,6 +221,144 @@ int mhc_pre_bwd(const void *x, int x_dtype, int64_t T, int n, int C,
                 void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Training step: causal attention over packed sequences                     */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * out[i,h] = sum_j P[i,j] v[j,h'],  P[i,:] = softmax over the visible j of scale q[i,h] . k[j,h']
+ *
+ * for T tokens, H query heads of size D (up to 128), Hk key / value heads, h' =
+ * h / (H / Hk).  Token i sees the tokens j <= i of its own sequence.  The
+ * sequences: cu_seqlens != NULL: sequence b is the tokens [cu_seqlens[b],
+ * cu_seqlens[b+1]), b < batch (device int32, non-decreasing; sequences may be
+ * empty, and tokens before the first and after the last belong to none: their
+ * out is 0 and what their q, k, v hold, NaN included, touches no other token);
+ * NULL: sequences of seqlen tokens each, T a multiple of it.
+ *
+ * q, k, v: element (t, h, d) at t * strides[0] + h * strides[1] + d (q), strides
+ * [2], [3] (k), [4], [5] (v); host array of 6, in elements.  out is (T, H, D)
+ * contiguous in `dtype`.  For mhc_attn_bwd: lse (H, T) fp32, log2 of the row's sum
+ * of exp2(scale log2(e) score), +inf for a row that sees nothing; out_lo (NULL:
+ * not wanted), laid out like out, what the rounding of out left over, in `dtype`.
+ *
+ * Replaces: scaled_dot_product_attention in Attention.forward
+ * (model/model_minimind.py:220-250).
+ */
+int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t T, int H, int Hk, int D,
+                 const int64_t *strides, const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale,
+                 void *out, void *out_lo, float *lse, void *stream);
+
+/* Bytes of scratch `mhc_attn_bwd` needs. */
+size_t mhc_attn_bwd_workspace(int64_t T, int H);
+
+/*
+ * Gradients of mhc_attn_fwd from out, out_lo (or NULL), lse and dout (T, H, D) contiguous:
+ * dq (T, H, D), dk and dv (T, Hk, D) contiguous, each summed in fp32 in a fixed
+ * order (no atomics), the heads of a group included.
+ */
+int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo,
+                 const void *dout, const float *lse, int dtype, int64_t T, int H, int Hk, int D, const int64_t *strides,
+                 const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale, void *dq, void *dk,
+                 void *dv, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Training step: top-k router with its balance loss                         */
+/* ------------------------------------------------------------------------ */
+
+/* Bytes of scratch `mhc_route_fwd` needs (on the device the call will run on). */
+size_t mhc_route_fwd_workspace(int64_t T, int E);
+
+/*
+ * Router of a mixture of E experts over T tokens, logits (T, E) in `dtype` with
+ * rows `row_stride` elements apart:
+ *
+ *   p            = softmax(logits) per token                         (fp32)
+ *   experts[t,j] = index of the j-th largest logit, j < k; the lower index first
+ *                  among equals, NaN above everything
+ *   weights[t,j] = p[t, experts[t,j]] / (sum_j p[t, experts[t,j]] + 1e-20)
+ *   counts[e]    = number of (t, j) with experts[t,j] == e
+ *   loss         = coef * E * sum_e (counts[e] / T) * mean_t p[t,e]
+ *
+ * weights and experts are (T, k) contiguous.  A row of -inf only has p = 0.
+ * 1 <= E <= 512, 1 <= k <= E.  T == 0: counts and loss are set to 0.
+ * Deterministic (fixed-order sums, no atomics).
+ *
+ * Replaces: the router of the reference's MOEFeedForward
+ * (model/model_minimind.py:262-293), a softmax, a top-k, the renormalisation and
+ * the one-hot mean of the auxiliary loss.
+ */
+int mhc_route_fwd(const void *logits, int dtype, int64_t T, int E, int64_t row_stride, int k, float coef,
+                  float *weights, int64_t *experts, int64_t *counts, float *loss,
+                  void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradient of mhc_route_fwd: dlogits (T, E) contiguous in `dtype`, 16-byte
+ * aligned, from dweights (T, k) fp32 and dloss (one fp32 on the device); either
+ * may be NULL (zero).  The counts are constants, as in the reference's loss.
+ */
+int mhc_route_bwd(const void *logits, int dtype, int64_t T, int E, int64_t row_stride, int k, float coef,
+                  const float *weights, const int64_t *experts, const int64_t *counts,
+                  const float *dweights, const float *dloss, void *dlogits, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Training step: AdamW over many tensors                                    */
+/* ------------------------------------------------------------------------ */
+
+/* One tensor of mhc_grad_norm / mhc_adamw_step: n values, contiguous.  exp_avg /
+ * exp_avg_sq are fp32 (state_bits 32; the scales are ignored) or int8 / uint8
+ * codes with ceil(n / 256) fp32 scales each (state_bits 8).  step counts the
+ * tensor's updates, this one included, from 1.  mhc_grad_norm reads grad, n and
+ * grad_dtype only. */
+typedef struct {
+  void *param;
+  const void *grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  int64_t n;
+  int64_t step;
+  int32_t param_dtype, grad_dtype;
+} mhc_adamw_tensor;
+
+/* Bytes of the workspace `mhc_grad_norm` fills (on the device the call will run on). */
+size_t mhc_grad_norm_workspace(void);
+
+/*
+ * Sums of squares of all gradients, as fp64 partials in `workspace` for
+ * mhc_adamw_step; accumulate != 0 adds to what an earlier call left there
+ * (several groups of tensors under one norm).  Deterministic.  The tensors'
+ * table is a host array; it is copied into the launches' arguments.
+ */
+int mhc_grad_norm(const mhc_adamw_tensor *tensors, int count, int accumulate, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/*
+ * One step of Adam with decoupled weight decay, in place, over `count` tensors (a
+ * host array; it is copied into the launches' arguments and may be freed on
+ * return), t = the tensor's step:
+ *
+ *   g = grad * min(1, max_norm / (|grads| + 1e-6))     (max_norm > 0; else g = grad)
+ *   m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ *
+ * in fp32, rounded once to the parameter's type.  |grads| is the root of the
+ * partials mhc_grad_norm left in norm_workspace; norm_out (device fp32 or NULL)
+ * receives it.  state_bits 8: the moments are read from and rounded to 8-bit
+ * codes, 256 values to a scale (the step uses the unrounded ones):
+ * m = (c/127)^2 sign(c) scale, v = (c/255)^4 scale, scale = the block's largest
+ * magnitude; v > 0 keeps a code >= 1.
+ *
+ * No counterpart in the reference's own code: its trainers call
+ * torch.optim.AdamW and clip_grad_norm_ (trainer/train_pretrain.py:45-52, 146).
+ */
+int mhc_adamw_step(const mhc_adamw_tensor *tensors, int count, int state_bits, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, double max_norm,
+                   const void *norm_workspace, float *norm_out, void *stream);
+
+/* The n values that 8-bit codes stand for, as fp32: is_signed selects exp_avg's
+ * form (int8) or exp_avg_sq's (uint8). */
+int mhc_adamw_unpack(const void *codes, int is_signed, const float *scales, float *out, int64_t n, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Stand-alone Sinkhorn-Knopp                                                */
 /* ------------------------------------------------------------------------ */
 

@@ -1,0 +1,559 @@
+// AdamW over many tensors in one launch, moments in fp32 or in 8 bits.
+//
+//   g' = g * clip                     clip = min(1, max_norm / (||g|| + 1e-6)), or 1
+//   m' = b1 m + (1 - b1) g'           v' = b2 v + ((1 - b2) g') g'
+//   p' = p (1 - lr wd) - (lr / (1 - b1^t)) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// Every value is touched once, so the kernel is bound by HBM: 28 bytes a value
+// with fp32 parameters, gradients and moments, 16 with 8-bit moments.  The
+// tensors' table travels as a kernel argument (up to 31 KB), so a step needs no
+// copy to the device, no table kept between calls and one launch for up to
+// MAX_TENSORS tensors.
+//
+// 8-bit moments: 256 consecutive values share one fp32 scale, the largest
+// magnitude among them.  m = (c / 127)^2 * sign * scale with c = round(127
+// sqrt(|m| / scale)): the squared spacing keeps small momenta (down to 6e-5 of
+// the largest) apart.  v = (c / 255)^4 * scale with c = round(255 (v /
+// scale)^(1/4)): a step divides by sqrt(v), whose spacing is then quadratic, and
+// a code of zero is kept for v = 0 (anything above it takes at least 1), since a
+// v rounded to zero would divide by eps.  The step itself uses the fp32 m' and
+// v'; only what is stored is rounded.  A block with a non-finite moment gets the
+// non-finite scale and so reads back as NaN, as fp32 moments would.
+// The arithmetic uses single IEEE operations (no contraction, no approximate
+// division or root): a value next to the edge between two codes then falls on
+// the same side wherever the formula is evaluated in fp32.
+//
+// A warp owns one block of 256 values at a time, a lane 4 + 4 of them (16-byte
+// accesses in fp32, 8-byte in 16-bit types, 4-byte for codes), so the block's
+// largest magnitude is one warp reduction.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "mhc_b200.h"
+#include "mhc_device.cuh"
+#include "mhc_dispatch.cuh"
+#include "mhc_kernels.h"
+
+namespace mhc {
+namespace adamw {
+
+constexpr int QB = 256;             // values per 8-bit block, per warp step
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int CHUNK = QB * WARPS * 2;  // values of one tensor a block takes at a time
+constexpr int MAX_TENSORS = 440;    // 72 bytes each: the largest table a launch's 32,764 bytes of arguments carry
+constexpr int FEW_TENSORS = 24;
+
+struct Entry {
+  void *p;
+  const void *g;
+  void *m, *v;
+  float *ms, *vs;
+  int64_t n;
+  int first_chunk;
+  uint8_t pdt, gdt, vec, pad;
+  float rbc2, step_size;  // 1 / sqrt(1 - b2^t), lr / (1 - b1^t) at the tensor's own step t
+};
+static_assert(sizeof(Entry) == 72, "table entry");
+
+template <int N>
+struct Table {
+  Entry t[N];
+  int count, chunks;
+};
+
+struct Scalars {
+  float b1, c1, b2, c2, eps, keep;  // c = 1 - b, keep = 1 - lr wd
+  float max_norm;
+  const double *partials;  // squared-norm partials, or null: no clipping
+  int npartials;
+  float *norm_out;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// 4 consecutive values of a runtime-typed tensor, at value index i
+__device__ __forceinline__ void load4(const void *p, int dt, int64_t i, float (&o)[4]) {
+  if (dt == MHC_F32) {
+    const float4 r = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i));
+    o[0] = r.x; o[1] = r.y; o[2] = r.z; o[3] = r.w;
+  } else {
+    const uint2 r = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i));
+    if (dt == MHC_BF16) {
+      o[0] = __uint_as_float(r.x << 16); o[1] = __uint_as_float(r.x & 0xffff0000u);
+      o[2] = __uint_as_float(r.y << 16); o[3] = __uint_as_float(r.y & 0xffff0000u);
+    } else {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&r.x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
+      o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
+    }
+  }
+}
+__device__ __forceinline__ void store4(void *p, int dt, int64_t i, const float (&v)[4]) {
+  if (dt == MHC_F32) {
+    __stcs(reinterpret_cast<float4 *>(static_cast<float *>(p) + i), make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+    uint2 r;
+    if (dt == MHC_BF16) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      r.x = *reinterpret_cast<const uint32_t *>(&a);
+      r.y = *reinterpret_cast<const uint32_t *>(&b);
+    } else {
+      const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+      r.x = *reinterpret_cast<const uint32_t *>(&a);
+      r.y = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    __stcs(reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + i), r);
+  }
+}
+
+// The values a lane holds of its warp's block: value index base + idx(e),
+// e < 8; two runs of four.
+__device__ __forceinline__ int lane_value(int lane, int e) { return (e >> 2) * 128 + lane * 4 + (e & 3); }
+
+__device__ __forceinline__ void load8(const void *p, int dt, int64_t base, int64_t n, bool whole, int lane,
+                                      float (&o)[8]) {
+  if (whole) {
+    float a[4], b[4];
+    load4(p, dt, base + lane * 4, a);
+    load4(p, dt, base + 128 + lane * 4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { o[e] = a[e]; o[4 + e] = b[e]; }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = base + lane_value(lane, e);
+      o[e] = i < n ? load_dyn(p, dt, i) : 0.f;
+    }
+  }
+}
+__device__ __forceinline__ void store8(void *p, int dt, int64_t base, int64_t n, bool whole, int lane,
+                                       const float (&v)[8]) {
+  if (whole) {
+    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+    store4(p, dt, base + lane * 4, a);
+    store4(p, dt, base + 128 + lane * 4, b);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = base + lane_value(lane, e);
+      if (i < n) store_dyn(p, dt, i, v[e]);
+    }
+  }
+}
+
+// 8-bit codes of a lane as integers (signed for m, unsigned for v)
+template <bool SIGNED>
+__device__ __forceinline__ void load_codes(const void *p, int64_t base, int64_t n, bool whole, int lane, float (&o)[8]) {
+  const uint8_t *q = static_cast<const uint8_t *>(p);
+  if (whole) {
+    const uint32_t w[2] = {__ldcs(reinterpret_cast<const uint32_t *>(q + base + lane * 4)),
+                           __ldcs(reinterpret_cast<const uint32_t *>(q + base + 128 + lane * 4))};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = (w[e >> 2] >> (8 * (e & 3))) & 0xffu;
+      o[e] = SIGNED ? (float)(int)(int8_t)b : (float)b;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = base + lane_value(lane, e);
+      const uint8_t b = i < n ? q[i] : 0;
+      o[e] = SIGNED ? (float)(int)(int8_t)b : (float)b;
+    }
+  }
+}
+__device__ __forceinline__ void store_codes(void *p, int64_t base, int64_t n, bool whole, int lane, const int (&c)[8]) {
+  uint8_t *q = static_cast<uint8_t *>(p);
+  if (whole) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w |= ((uint32_t)c[h * 4 + e] & 0xffu) << (8 * e);
+      __stcs(reinterpret_cast<uint32_t *>(q + base + h * 128 + lane * 4), w);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = base + lane_value(lane, e);
+      if (i < n) q[i] = (uint8_t)c[e];
+    }
+  }
+}
+
+__device__ __forceinline__ float unpack_m(float c, float scale) {
+  return __fmul_rn(__fmul_rn(c * fabsf(c), scale), (float)(1.0 / 16129.0));
+}
+__device__ __forceinline__ float unpack_v(float c, float scale) {
+  const float cc = c * c;  // an integer up to 65025: exact
+  return __fmul_rn(__fmul_rn(__fmul_rn(__fmul_rn(cc, scale), (float)(1.0 / 65025.0)), cc), (float)(1.0 / 65025.0));
+}
+__device__ __forceinline__ int pack_m(float m, float safe) {
+  const float r = rintf(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), safe)), 127.f));
+  return __float2int_rn(m < 0.f ? -r : r);  // NaN converts to 0
+}
+__device__ __forceinline__ int pack_v(float v, float safe) {
+  const int c = __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, safe))), 255.f));
+  return v > 0.f && c < 1 ? 1 : c;
+}
+
+// table entry of a chunk: the last one whose first chunk is not above it
+template <int N>
+__device__ __forceinline__ int entry_of(const Table<N> &tab, int chunk) {
+  int lo = 0, hi = tab.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.t[mid].first_chunk <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Clip factor from the partial sums, each block for itself: the same sum in the
+// same order everywhere.
+__device__ __forceinline__ float clip_factor(const Scalars &s) {
+  __shared__ double sh[WARPS];
+  double a = 0.0;
+  for (int i = threadIdx.x; i < s.npartials; i += THREADS) a += s.partials[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) t += sh[w];
+  const float norm = (float)sqrt(t);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && s.norm_out) *s.norm_out = norm;
+  const float f = __fdiv_rn(s.max_norm, __fadd_rn(norm, 1e-6f));
+  return f < 1.f ? f : (f >= 1.f ? 1.f : f);  // NaN stays NaN
+}
+
+template <int N, bool Q8>
+__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Table<N> tab, const Scalars s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float clip = 1.f;
+  if (s.partials) clip = clip_factor(s);
+  for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
+    const int ei = entry_of(tab, chunk);
+    const Entry &t = tab.t[ei];
+    const int64_t first = (int64_t)(chunk - t.first_chunk) * CHUNK;
+#pragma unroll
+    for (int it = 0; it < CHUNK / (QB * WARPS); ++it) {
+      const int64_t base = first + (int64_t)(it * WARPS + warp) * QB;
+      if (base >= t.n) break;
+      const bool whole = t.vec && base + QB <= t.n;
+      float p[8], g[8], m[8], v[8];
+      load8(t.p, t.pdt, base, t.n, whole, lane, p);
+      load8(t.g, t.gdt, base, t.n, whole, lane, g);
+      if constexpr (Q8) {
+        const float sm = t.ms[base / QB], sv = t.vs[base / QB];
+        load_codes<true>(t.m, base, t.n, whole, lane, m);
+        load_codes<false>(t.v, base, t.n, whole, lane, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          m[e] = unpack_m(m[e], sm);
+          v[e] = unpack_v(v[e], sv);
+        }
+      } else {
+        load8(t.m, MHC_F32, base, t.n, whole, lane, m);
+        load8(t.v, MHC_F32, base, t.n, whole, lane, v);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float gr = s.partials ? __fmul_rn(g[e], clip) : g[e];
+        m[e] = __fadd_rn(__fmul_rn(m[e], s.b1), __fmul_rn(gr, s.c1));
+        v[e] = __fadd_rn(__fmul_rn(v[e], s.b2), __fmul_rn(__fmul_rn(gr, s.c2), gr));
+        const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v[e]), t.rbc2), s.eps);
+        p[e] = __fsub_rn(__fmul_rn(p[e], s.keep), __fmul_rn(__fdiv_rn(m[e], denom), t.step_size));
+      }
+      store8(t.p, t.pdt, base, t.n, whole, lane, p);
+      if constexpr (Q8) {
+        float am = 0.f, av = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          am = max_nan(am, fabsf(m[e]));
+          av = max_nan(av, v[e]);
+        }
+        am = warp_max_nan(am);
+        av = warp_max_nan(av);
+        if (lane == 0) {
+          t.ms[base / QB] = am;
+          t.vs[base / QB] = av;
+        }
+        // an empty block divides by one; every code is then zero
+        const float dm = am > 0.f ? am : 1.f, dv = av > 0.f ? av : 1.f;
+        int cm[8], cv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          cm[e] = pack_m(m[e], dm);
+          cv[e] = pack_v(v[e], dv);
+        }
+        store_codes(t.m, base, t.n, whole, lane, cm);
+        store_codes(t.v, base, t.n, whole, lane, cv);
+      } else {
+        store8(t.m, MHC_F32, base, t.n, whole, lane, m);
+        store8(t.v, MHC_F32, base, t.n, whole, lane, v);
+      }
+    }
+  }
+}
+
+// Squared norm of all gradients: one partial a block, summed in a fixed order by
+// whoever reads them.  fp32 within a lane's few values, fp64 from there on.
+template <int N>
+__global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constant__ Table<N> tab, double *partials,
+                                                            int accumulate) {
+  __shared__ double sh[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double total = 0.0;
+  for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
+    const int ei = entry_of(tab, chunk);
+    const Entry &t = tab.t[ei];
+    const int64_t first = (int64_t)(chunk - t.first_chunk) * CHUNK;
+    float a = 0.f;
+#pragma unroll
+    for (int it = 0; it < CHUNK / (QB * WARPS); ++it) {
+      const int64_t base = first + (int64_t)(it * WARPS + warp) * QB;
+      if (base >= t.n) break;
+      float g[8];
+      load8(t.g, t.gdt, base, t.n, t.vec && base + QB <= t.n, lane, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = fmaf(g[e], g[e], a);
+    }
+    total += (double)a;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) sh[warp] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double r = accumulate ? partials[blockIdx.x] : 0.0;
+    for (int w = 0; w < WARPS; ++w) r += sh[w];
+    partials[blockIdx.x] = r;
+  }
+}
+
+// The values 8-bit moments stand for.
+template <bool SIGNED>
+__global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *codes, const float *scales, float *out,
+                                                         int64_t n, int vec) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t blocks = (n + QB - 1) / QB;
+  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < blocks; b += (int64_t)gridDim.x * WARPS) {
+    const int64_t base = b * QB;
+    const bool whole = vec && base + QB <= n;
+    const float s = scales[b];
+    float c[8];
+    load_codes<SIGNED>(codes, base, n, whole, lane, c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = SIGNED ? unpack_m(c[e], s) : unpack_v(c[e], s);
+    store8(out, MHC_F32, base, n, whole, lane, c);
+  }
+}
+
+constexpr int NORM_BLOCKS_PER_SM = 4;
+
+// Fills tables of up to N tensors and launches each of them: launch(table, first).
+template <int N, typename F>
+static cudaError_t for_tables(const mhc_adamw_tensor *ts, int count, int state_bits, double lr, double beta1,
+                              double beta2, F &&launch) {
+  bool first = true;
+  int64_t step = 0;
+  float rbc2 = 0.f, step_size = 0.f;
+  for (int at = 0; at < count;) {
+    Table<N> tab;
+    tab.count = 0;
+    int64_t chunks = 0;
+    while (at < count && tab.count < N) {
+      const mhc_adamw_tensor &t = ts[at];
+      const int64_t c = (t.n + CHUNK - 1) / CHUNK;
+      if (chunks + c > (int64_t)1 << 30) break;  // never the table's first: n is at most 2^40
+      ++at;
+      if (t.n == 0) continue;
+      if (t.step != step) {
+        step = t.step;
+        rbc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+        step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+      }
+      Entry &e = tab.t[tab.count++];
+      e.p = t.param;
+      e.g = t.grad;
+      e.m = t.exp_avg;
+      e.v = t.exp_avg_sq;
+      e.ms = t.exp_avg_scale;
+      e.vs = t.exp_avg_sq_scale;
+      e.n = t.n;
+      e.first_chunk = (int)chunks;
+      e.pdt = (uint8_t)t.param_dtype;
+      e.gdt = (uint8_t)t.grad_dtype;
+      // whether blocks of 4 values may be read and written at once
+      const uintptr_t pa = t.param_dtype == MHC_F32 ? 15 : 7, ga = t.grad_dtype == MHC_F32 ? 15 : 7;
+      const uintptr_t sa = state_bits == 8 ? 3 : 15;
+      e.vec = !((uintptr_t)t.param & pa) && !((uintptr_t)t.grad & ga) && !((uintptr_t)t.exp_avg & sa) &&
+              !((uintptr_t)t.exp_avg_sq & sa);
+      e.pad = 0;
+      e.rbc2 = rbc2;
+      e.step_size = step_size;
+      chunks += c;
+    }
+    if (tab.count == 0) continue;
+    tab.chunks = (int)chunks;
+    launch(tab, first);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    first = false;
+  }
+  return cudaSuccess;
+}
+
+template <int N>
+static cudaError_t run_norm(const mhc_adamw_tensor *ts, int count, int accumulate, double *partials, int grid,
+                            cudaStream_t stream) {
+  return for_tables<N>(ts, count, 32, 0.0, 0.0, 0.0, [&](const Table<N> &tab, bool first) {
+    // every block writes its partial, so the grid does not shrink with the work
+    grad_norm_kernel<N><<<grid, THREADS, 0, stream>>>(tab, partials, first ? accumulate : 1);
+  });
+}
+
+template <int N, bool Q8>
+static cudaError_t run_step(const mhc_adamw_tensor *ts, int count, double lr, double beta1, double beta2, const Scalars &s,
+                            int sms, cudaStream_t stream) {
+  return for_tables<N>(ts, count, Q8 ? 8 : 32, lr, beta1, beta2, [&](const Table<N> &tab, bool) {
+    const int cap = sms * 8;
+    adamw_kernel<N, Q8><<<tab.chunks < cap ? tab.chunks : cap, THREADS, 0, stream>>>(tab, s);
+  });
+}
+
+static int sm_count_or_default() {
+  const int v = device_sm_count();
+  return v > 0 ? v : 148;
+}
+
+}  // namespace adamw
+}  // namespace mhc
+
+using namespace mhc;
+
+// tensors with values; < 0: a status code
+static int64_t check_tensors(const char *who, const mhc_adamw_tensor *ts, int count, int state_bits, bool grads_only) {
+  if (count < 0) return fail(MHC_ERR_SHAPE, "%s: count %d", who, count);
+  if (count > 0 && !ts) return fail(MHC_ERR_NULL, "%s: tensors is NULL", who);
+  const bool q8 = state_bits == 8;
+  int64_t live = 0;
+  for (int i = 0; i < count; ++i) {
+    const mhc_adamw_tensor &t = ts[i];
+    if (t.n < 0 || t.n > (int64_t)1 << 40) return fail(MHC_ERR_SHAPE, "%s: tensor %d has %lld values", who, i, (long long)t.n);
+    if (t.n == 0) continue;
+    ++live;
+    const bool types = (grads_only || t.param_dtype == MHC_F32 || t.param_dtype == MHC_BF16 || t.param_dtype == MHC_F16) &&
+                       (t.grad_dtype == MHC_F32 || t.grad_dtype == MHC_BF16 || t.grad_dtype == MHC_F16);
+    if (!types) return fail(MHC_ERR_DTYPE, "%s: tensor %d: bad dtype code", who, i);
+    const uintptr_t ga = t.grad_dtype == MHC_F32 ? 3 : 1;
+    if (!t.grad) return fail(MHC_ERR_NULL, "%s: tensor %d: grad is NULL", who, i);
+    if ((uintptr_t)t.grad & ga) return fail(MHC_ERR_ALIGN, "%s: tensor %d is not aligned to its elements", who, i);
+    if (grads_only) continue;
+    if (t.step < 1) return fail(MHC_ERR_SHAPE, "%s: tensor %d: steps count from 1 (got %lld)", who, i, (long long)t.step);
+    if (!t.param || !t.exp_avg || !t.exp_avg_sq || (q8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
+      return fail(MHC_ERR_NULL, "%s: tensor %d: required pointer is NULL", who, i);
+    const uintptr_t pa = t.param_dtype == MHC_F32 ? 3 : 1, sa = q8 ? 0 : 3;
+    if (((uintptr_t)t.param & pa) || (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & sa) ||
+        (q8 && (((uintptr_t)t.exp_avg_scale | (uintptr_t)t.exp_avg_sq_scale) & 3)))
+      return fail(MHC_ERR_ALIGN, "%s: tensor %d is not aligned to its elements", who, i);
+  }
+  return live;
+}
+
+extern "C" {
+
+size_t mhc_grad_norm_workspace(void) {
+  return (size_t)adamw::sm_count_or_default() * adamw::NORM_BLOCKS_PER_SM * sizeof(double);
+}
+
+int mhc_grad_norm(const mhc_adamw_tensor *tensors, int count, int accumulate, void *workspace, size_t workspace_bytes,
+                  void *stream) {
+  clear_error();
+  const int64_t live = check_tensors("mhc_grad_norm", tensors, count, 32, true);
+  if (live < 0) return (int)live;
+  const size_t need = mhc_grad_norm_workspace();
+  if (!workspace || workspace_bytes < need)
+    return fail(MHC_ERR_WORKSPACE, "mhc_grad_norm: workspace %zu < %zu bytes", workspace_bytes, need);
+  if ((uintptr_t)workspace & 7) return fail(MHC_ERR_ALIGN, "mhc_grad_norm: workspace is not 8-byte aligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (live == 0)
+    return accumulate ? MHC_OK : cuda_status(cudaMemsetAsync(workspace, 0, need, st), "mhc_grad_norm");
+  const int grid = adamw::sm_count_or_default() * adamw::NORM_BLOCKS_PER_SM;
+  double *pw = static_cast<double *>(workspace);
+  return cuda_status(live <= adamw::FEW_TENSORS
+                         ? adamw::run_norm<adamw::FEW_TENSORS>(tensors, count, accumulate, pw, grid, st)
+                         : adamw::run_norm<adamw::MAX_TENSORS>(tensors, count, accumulate, pw, grid, st),
+                     "mhc_grad_norm");
+}
+
+int mhc_adamw_step(const mhc_adamw_tensor *tensors, int count, int state_bits, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, double max_norm, const void *norm_workspace, float *norm_out,
+                   void *stream) {
+  clear_error();
+  if (state_bits != 8 && state_bits != 32)
+    return fail(MHC_ERR_UNSUPPORTED, "mhc_adamw_step: state_bits must be 8 or 32 (got %d)", state_bits);
+  if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) ||
+      !(beta2 >= 0.0 && beta2 < 1.0))
+    return fail(MHC_ERR_SHAPE, "mhc_adamw_step: lr, eps, weight_decay >= 0 and betas in [0, 1) are wanted");
+  const int64_t live = check_tensors("mhc_adamw_step", tensors, count, state_bits, false);
+  if (live < 0) return (int)live;
+  if (max_norm > 0.0 && (!norm_workspace || ((uintptr_t)norm_workspace & 7)))
+    return fail(MHC_ERR_WORKSPACE, "mhc_adamw_step: clipping needs the workspace that mhc_grad_norm filled");
+  if (live == 0) return MHC_OK;
+  const int sms = adamw::sm_count_or_default();
+  adamw::Scalars s;
+  s.b1 = (float)beta1;
+  s.c1 = (float)(1.0 - beta1);
+  s.b2 = (float)beta2;
+  s.c2 = (float)(1.0 - beta2);
+  s.eps = (float)eps;
+  s.keep = (float)(1.0 - lr * weight_decay);
+  s.max_norm = (float)max_norm;
+  s.partials = max_norm > 0.0 ? static_cast<const double *>(norm_workspace) : nullptr;
+  s.npartials = sms * adamw::NORM_BLOCKS_PER_SM;
+  s.norm_out = s.partials ? norm_out : nullptr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  constexpr int F = adamw::FEW_TENSORS, M = adamw::MAX_TENSORS;
+  cudaError_t e;
+  if (live <= F)
+    e = state_bits == 8 ? adamw::run_step<F, true>(tensors, count, lr, beta1, beta2, s, sms, st)
+                        : adamw::run_step<F, false>(tensors, count, lr, beta1, beta2, s, sms, st);
+  else
+    e = state_bits == 8 ? adamw::run_step<M, true>(tensors, count, lr, beta1, beta2, s, sms, st)
+                        : adamw::run_step<M, false>(tensors, count, lr, beta1, beta2, s, sms, st);
+  return cuda_status(e, "mhc_adamw_step");
+}
+
+int mhc_adamw_unpack(const void *codes, int is_signed, const float *scales, float *out, int64_t n, void *stream) {
+  clear_error();
+  if (n < 0 || n > (int64_t)1 << 40) return fail(MHC_ERR_SHAPE, "mhc_adamw_unpack: %lld values", (long long)n);
+  if (n == 0) return MHC_OK;
+  if (!codes || !scales || !out) return fail(MHC_ERR_NULL, "mhc_adamw_unpack: required pointer is NULL");
+  if (((uintptr_t)scales & 3) || ((uintptr_t)out & 3)) return fail(MHC_ERR_ALIGN, "mhc_adamw_unpack: scales / out misaligned");
+  const int vec = !((uintptr_t)codes & 3) && !((uintptr_t)out & 15);
+  const int64_t blocks = (n + adamw::QB - 1) / adamw::QB;
+  const unsigned grid = grid_for(blocks, adamw::WARPS, device_sm_count(), 8);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const uint8_t *c = static_cast<const uint8_t *>(codes);
+  if (is_signed)
+    adamw::unpack_kernel<true><<<grid, adamw::THREADS, 0, st>>>(c, scales, out, n, vec);
+  else
+    adamw::unpack_kernel<false><<<grid, adamw::THREADS, 0, st>>>(c, scales, out, n, vec);
+  return cuda_status(cudaGetLastError(), "mhc_adamw_unpack");
+}
+
+}  // extern "C"

@@ -1,0 +1,459 @@
+// Causal attention over packed sequences, forward and backward, on CUDA cores:
+// every type, every head size up to 128, any token and head strides.
+//
+//   O_i  = sum_j P_ij V_j,   P_ij = exp(scale q_i . k_j - L_i),   start(i) <= j <= i
+//   D_i  = dO_i . O_i,       dS_ij = P_ij (dO_i . V_j - D_i)
+//   dQ_i = scale sum_j dS_ij K_j
+//   dK_j = scale sum_{h in group, i} dS_ij Q_i,   dV_j = sum_{h in group, i} P_ij dO_i
+//
+// fp32 throughout.  A block of 16 x 16 threads owns 64 rows and walks tiles of 64
+// columns; a thread holds a 4 x 4 piece of the scores and 4 rows x D / 16 columns
+// of the result in registers, the operands are staged as fp32 in shared memory.
+// Forward: one pass with the running maximum and sum.  Backward: the scores again
+// from the saved L, in two kernels of the same form (a block owns 64 queries and
+// sums dQ, or 64 keys and sums dK and dV over the heads that share them), so
+// every gradient is a sum in a fixed order.  The FFMA pipe and its shared-memory
+// operands bound it; fp32 inputs have no tensor-core form of this accuracy.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <initializer_list>
+#include <mutex>
+
+#include "mhc_attn.cuh"
+#include "mhc_b200.h"
+#include "mhc_device.cuh"
+#include "mhc_dispatch.cuh"
+#include "mhc_kernels.h"
+
+namespace mhc {
+namespace attn {
+
+constexpr int TILE = 64;
+constexpr int THREADS = 256;
+constexpr int PP = TILE + 4;  // pitch of a score tile
+
+// 64 rows of one head as fp32 into shared memory, zero outside of the packed
+// range and past column D
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t ts, int row0, int D, Span range) {
+  for (int e = threadIdx.x; e < TILE * DP; e += THREADS) {
+    const int r = e / DP, c = e - r * DP;
+    const int t = row0 + r;
+    dst[r * (DP + 4) + c] = t >= range.start && t < range.end && c < D ? to_f(src[(int64_t)t * ts + c]) : 0.f;
+  }
+}
+
+// s[i][j] = sum_d A[ty*4+i][d] B[tx+16j][d]
+template <int DP>
+__device__ __forceinline__ void scores(const float *A, const float *B, int ty, int tx, float (&s)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(A + (ty * 4 + i) * (DP + 4) + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4 *>(B + (tx + 16 * j) * (DP + 4) + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+        s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+        s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+        s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+      }
+  }
+}
+
+// acc[i][2c..2c+1] += sum_kk W[ty*4+i][kk] B[kk][2 tx + 32 c ..]
+template <int DP>
+__device__ __forceinline__ void accumulate(const float *W, const float *B, int ty, int tx, float (&acc)[4][DP / 16]) {
+#pragma unroll 2
+  for (int kk = 0; kk < TILE; kk += 4) {
+    float4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4 *>(W + (ty * 4 + i) * PP + kk);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float2 b[DP / 32];
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) b[c] = *reinterpret_cast<const float2 *>(B + (kk + u) * (DP + 4) + 2 * tx + 32 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float wi = u == 0 ? w[i].x : (u == 1 ? w[i].y : (u == 2 ? w[i].z : w[i].w));
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          acc[i][2 * c] = fmaf(wi, b[c].x, acc[i][2 * c]);
+          acc[i][2 * c + 1] = fmaf(wi, b[c].y, acc[i][2 * c + 1]);
+        }
+      }
+    }
+  }
+}
+
+// lo != null: what the rounding to T left over, itself in T
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, int64_t T_, int D, int ty, int tx,
+                                           const float (&acc)[4][DP / 16], const float (&mul)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = row0 + ty * 4 + i;
+    if (t >= T_) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int col = 2 * tx + 32 * (c / 2) + (c & 1);
+      if (col < D) {
+        const float v = acc[i][c] * mul[i];
+        const T r = from_f<T>(v);
+        dst[(int64_t)t * ts + col] = r;
+        if (lo) lo[(int64_t)t * ts + col] = from_f<T>(v - to_f(r));
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a) {
+  extern __shared__ float sm[];
+  float *Q = sm, *K = Q + TILE * (DP + 4), *V = K + TILE * (DP + 4), *P = V + TILE * (DP + 4);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * TILE;  // longest rows first
+  const int h = blockIdx.y, hk = h / (a.H / a.Hk);
+  const Span range = packed_range(a);
+  int start[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = q0 + ty * 4 + i;
+    start[i] = t < a.T ? span_of(a, t).start : t + 1;
+  }
+  load_tile<T, DP>(Q, static_cast<const T *>(a.q) + h * a.qh, a.qt, q0, a.D, range);
+  float acc[4][DP / 16] = {};
+  float mx[4], sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mx[i] = -INFINITY;
+    sum[i] = 0.f;
+  }
+  const int first = span_of(a, q0).start, last = min((int64_t)q0 + TILE, a.T);
+  for (int k0 = first; k0 < last; k0 += TILE) {
+    __syncthreads();
+    load_tile<T, DP>(K, static_cast<const T *>(a.k) + hk * a.kh, a.kt, k0, a.D, range);
+    load_tile<T, DP>(V, static_cast<const T *>(a.v) + hk * a.vh, a.vt, k0, a.D, range);
+    __syncthreads();
+    float s[4][4];
+    scores<DP>(Q, K, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = q0 + ty * 4 + i;
+      float m = mx[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx + 16 * j;
+        s[i][j] = key >= start[i] && key <= t ? s[i][j] * a.scale_log2 : -INFINITY;
+        m = fmaxf(m, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float base = m == -INFINITY ? 0.f : m;  // nothing visible yet
+      const float fix = exp2f(mx[i] - base);
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        part += p;
+        P[(ty * 4 + i) * PP + tx + 16 * j] = p;
+      }
+#pragma unroll
+      for (int o = 8; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      sum[i] = sum[i] * fix + part;
+      mx[i] = m;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= fix;
+    }
+    __syncwarp();  // a row of P is written and read by the same 16 lanes
+    accumulate<DP>(P, V, ty, tx, acc);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = q0 + ty * 4 + i;
+    inv[i] = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+    if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.T + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
+  }
+  T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
+  store_rows<T, DP>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
+}
+
+// DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
+// DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
+// that see them, of every head of the group.
+template <typename T, int DP, bool DKV>
+__global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a) {
+  extern __shared__ float sm[];
+  constexpr int TS = TILE * (DP + 4);
+  float *R1 = sm, *R2 = R1 + TS, *C1 = R2 + TS, *C2 = C1 + TS, *W = C2 + TS, *L = W + TILE * PP, *Dl = L + TILE;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int r0 = (int)(DKV ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TILE;
+  const int G = a.H / a.Hk;
+  const int rh = blockIdx.y;
+  const Span range = packed_range(a);
+  const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
+  const T *dout = static_cast<const T *>(a.dout);
+  const int64_t ot = (int64_t)a.H * a.D;
+  int bound[4];  // DKV: the end of the key's sequence; else the start of the query's
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = r0 + ty * 4 + i;
+    const Span s = t < a.T ? span_of(a, t) : Span{t + 1, t};
+    bound[i] = DKV ? s.end : s.start;
+  }
+  if (DKV) {
+    load_tile<T, DP>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
+    load_tile<T, DP>(R2, v + rh * a.vh, a.vt, r0, a.D, range);
+  } else {
+    load_tile<T, DP>(R1, q + rh * a.qh, a.qt, r0, a.D, range);
+    load_tile<T, DP>(R2, dout + (int64_t)rh * a.D, ot, r0, a.D, range);
+  }
+  float acc1[4][DP / 16] = {}, acc2[DKV ? 4 : 1][DP / 16] = {};
+  const int64_t end_rows = min((int64_t)r0 + TILE, a.T);
+  const int first = DKV ? r0 : span_of(a, r0).start;
+  const int last = DKV ? span_of(a, (int)end_rows - 1).end : (int)end_rows;
+  for (int g = 0; g < (DKV ? G : 1); ++g) {
+    const int h = DKV ? rh * G + g : rh;
+    for (int c0 = first; c0 < last; c0 += TILE) {
+      __syncthreads();
+      if (DKV) {
+        load_tile<T, DP>(C1, q + h * a.qh, a.qt, c0, a.D, range);
+        load_tile<T, DP>(C2, dout + (int64_t)h * a.D, ot, c0, a.D, range);
+      } else {
+        load_tile<T, DP>(C1, k + (rh / G) * a.kh, a.kt, c0, a.D, range);
+        load_tile<T, DP>(C2, v + (rh / G) * a.vh, a.vt, c0, a.D, range);
+      }
+      if (tid < TILE) {
+        const int64_t t = (DKV ? c0 : r0) + tid;
+        L[tid] = t < a.T ? a.lse[(int64_t)h * a.T + t] : INFINITY;
+        Dl[tid] = t < a.T ? a.delta[(int64_t)h * a.T + t] : 0.f;
+      }
+      __syncthreads();
+      float p[4][4], ds[4][4];
+      scores<DP>(R1, C1, ty, tx, p);
+      scores<DP>(R2, C2, ty, tx, ds);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + ty * 4 + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = c0 + tx + 16 * j;
+          const bool seen = DKV ? c >= r && c < bound[i] : c <= r && c >= bound[i];
+          const int n = DKV ? tx + 16 * j : ty * 4 + i;
+          p[i][j] = seen ? exp2f(fmaf(p[i][j], a.scale_log2, -L[n])) : 0.f;
+          ds[i][j] = seen ? p[i][j] * (ds[i][j] - Dl[n]) : 0.f;
+        }
+      }
+      if constexpr (DKV) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) W[(ty * 4 + i) * PP + tx + 16 * j] = p[i][j];
+        __syncwarp();
+        accumulate<DP>(W, C2, ty, tx, acc2);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) W[(ty * 4 + i) * PP + tx + 16 * j] = ds[i][j];
+      __syncwarp();
+      accumulate<DP>(W, C1, ty, tx, acc1);
+    }
+  }
+  const float sc[4] = {a.scale, a.scale, a.scale, a.scale};
+  if constexpr (DKV) {
+    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    const int64_t kt = (int64_t)a.Hk * a.D;
+    store_rows<T, DP>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
+    store_rows<T, DP>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+  } else {
+    store_rows<T, DP>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
+  }
+}
+
+// D_i = dO_i . O_i, one warp a (token, head).  O is its rounded value plus what the
+// rounding left over: D is subtracted from dO . V, of which it is the mean, so with
+// few keys the rounding of O alone would show in dS as an error of its own size.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const Args a) {
+  const int64_t rows = a.T * a.H;
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const T *o = static_cast<const T *>(a.out) + r * a.D, *d = static_cast<const T *>(a.dout) + r * a.D;
+    float s = 0.f;
+    const T *l = a.out_lo ? static_cast<const T *>(a.out_lo) + r * a.D : nullptr;
+    for (int c = lane; c < a.D; c += 32) {
+      const float v = to_f(o[c]) + (l ? to_f(l[c]) : 0.f);
+      s = fmaf(v, to_f(d[c]), s);
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    const int64_t t = r / a.H;
+    if (lane == 0) a.delta[(r - t * a.H) * a.T + t] = s;
+  }
+}
+
+template <typename F>
+static cudaError_t with_dim(int D, F &&f) {
+  if (D <= 32) return f(IC<32>{});
+  if (D <= 64) return f(IC<64>{});
+  if (D <= 96) return f(IC<96>{});
+  return f(IC<128>{});
+}
+
+// opt-in shared memory of a kernel, set once per device
+template <auto KERN>
+static cudaError_t allow_smem(size_t bytes) {
+  static std::mutex mu;
+  static bool done[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 64 && done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <typename T, int DP>
+static cudaError_t run_fwd(const Args &a, cudaStream_t stream) {
+  constexpr size_t smem = (size_t)(3 * TILE * (DP + 4) + TILE * PP) * 4;
+  cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP>>(smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)((a.T + TILE - 1) / TILE), (unsigned)a.H);
+  attn_fwd_generic_kernel<T, DP><<<grid, THREADS, smem, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP, bool DKV>
+static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
+  constexpr size_t smem = (size_t)(4 * TILE * (DP + 4) + TILE * PP + 2 * TILE) * 4;
+  cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, DKV>>(smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)((a.T + TILE - 1) / TILE), (unsigned)(DKV ? a.Hk : a.H));
+  attn_bwd_generic_kernel<T, DP, DKV><<<grid, THREADS, smem, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace attn
+
+cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
+  return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
+    using T = decltype(tag);
+    return attn::with_dim(a.D, [&](auto d) -> cudaError_t { return attn::run_fwd<T, decltype(d)::value>(a, stream); });
+  });
+}
+
+cudaError_t launch_attn_delta(const attn::Args &a, cudaStream_t stream) {
+  const unsigned grid = grid_for(a.T * a.H, 8, device_sm_count(), 8);
+  return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
+    attn::attn_delta_kernel<decltype(tag)><<<grid, 256, 0, stream>>>(a);
+    return cudaGetLastError();
+  });
+}
+
+cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream) {
+  return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
+    using T = decltype(tag);
+    return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
+      constexpr int DP = decltype(d)::value;
+      const cudaError_t e = attn::run_bwd<T, DP, false>(a, stream);
+      return e != cudaSuccess ? e : attn::run_bwd<T, DP, true>(a, stream);
+    });
+  });
+}
+
+}  // namespace mhc
+
+using namespace mhc;
+
+static int check_attn(const char *who, attn::Args &a, const int64_t *strides, float scale) {
+  if (a.T < 0 || a.T > 2147483647LL - 512) return fail(MHC_ERR_SHAPE, "%s: T = %lld", who, (long long)a.T);
+  if (a.H < 1 || a.Hk < 1 || a.H > 65535 || a.H % a.Hk)
+    return fail(MHC_ERR_SHAPE, "%s: %d query heads cannot share %d key heads", who, a.H, a.Hk);
+  if (a.D < 1 || a.D > 128) return fail(MHC_ERR_SHAPE, "%s: head sizes up to 128 are supported (got %d)", who, a.D);
+  if (a.dtype != MHC_F32 && a.dtype != MHC_BF16 && a.dtype != MHC_F16) return fail(MHC_ERR_DTYPE, "%s: bad dtype code %d", who, a.dtype);
+  if (!(scale > 0.f) || scale > 3e38f) return fail(MHC_ERR_SHAPE, "%s: scale must be positive and finite", who);
+  if (a.cu) {
+    if (a.batch < 1) return fail(MHC_ERR_SHAPE, "%s: cu_seqlens of %d sequences", who, a.batch);
+    if ((uintptr_t)a.cu & 3) return fail(MHC_ERR_ALIGN, "%s: cu_seqlens is misaligned", who);
+  } else if (a.T > 0 && (a.seqlen < 1 || a.T % a.seqlen)) {
+    return fail(MHC_ERR_SHAPE, "%s: %lld tokens are not sequences of %lld", who, (long long)a.T, (long long)a.seqlen);
+  }
+  if (!strides) return fail(MHC_ERR_NULL, "%s: strides is NULL", who);
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < 0) return fail(MHC_ERR_SHAPE, "%s: negative stride", who);
+  a.qt = strides[0]; a.qh = strides[1]; a.kt = strides[2]; a.kh = strides[3]; a.vt = strides[4]; a.vh = strides[5];
+  a.scale = scale;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.err_flag = host_error_flag();
+  return MHC_OK;
+}
+
+static bool misaligned(size_t es, std::initializer_list<const void *> ps) {
+  for (const void *p : ps)
+    if ((uintptr_t)p % es) return true;
+  return false;
+}
+
+extern "C" {
+
+int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t T, int H, int Hk, int D,
+                 const int64_t *strides, const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale, void *out,
+                 void *out_lo, float *lse, void *stream) {
+  clear_error();
+  attn::Args a{};
+  a.q = q; a.k = k; a.v = v; a.o = out; a.o_lo = out_lo; a.lse = lse;
+  a.T = T; a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
+  a.cu = cu_seqlens; a.batch = batch; a.seqlen = seqlen;
+  if (int st = check_attn("mhc_attn_fwd", a, strides, scale)) return st;
+  if (T == 0) return MHC_OK;
+  if (!q || !k || !v || !out || !lse) return fail(MHC_ERR_NULL, "mhc_attn_fwd: required pointer is NULL");
+  if (misaligned(dtype == MHC_F32 ? 4 : 2, {q, k, v, out, out_lo}) || ((uintptr_t)lse & 3))
+    return fail(MHC_ERR_ALIGN, "mhc_attn_fwd: a pointer is not aligned to its elements");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return cuda_status(launch_attn_fwd_generic(a, st), "mhc_attn_fwd");
+}
+
+size_t mhc_attn_bwd_workspace(int64_t T, int H) { return T < 1 || H < 1 ? 256 : (size_t)T * H * 4 + 256; }
+
+int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo, const void *dout,
+                 const float *lse, int dtype, int64_t T, int H, int Hk, int D, const int64_t *strides, const int32_t *cu_seqlens,
+                 int batch, int64_t seqlen, float scale, void *dq, void *dk, void *dv, void *workspace,
+                 size_t workspace_bytes, void *stream) {
+  clear_error();
+  attn::Args a{};
+  a.q = q; a.k = k; a.v = v; a.out = out; a.out_lo = out_lo; a.dout = dout; a.lse = const_cast<float *>(lse);
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.T = T; a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
+  a.cu = cu_seqlens; a.batch = batch; a.seqlen = seqlen;
+  if (int st = check_attn("mhc_attn_bwd", a, strides, scale)) return st;
+  if (T == 0) return MHC_OK;
+  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv)
+    return fail(MHC_ERR_NULL, "mhc_attn_bwd: required pointer is NULL");
+  if (misaligned(dtype == MHC_F32 ? 4 : 2, {q, k, v, out, out_lo, dout, dq, dk, dv}) || ((uintptr_t)lse & 3))
+    return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: a pointer is not aligned to its elements");
+  if (!workspace || workspace_bytes < mhc_attn_bwd_workspace(T, H))
+    return fail(MHC_ERR_WORKSPACE, "mhc_attn_bwd: workspace %zu < %zu bytes", workspace_bytes, mhc_attn_bwd_workspace(T, H));
+  if ((uintptr_t)workspace & 15) return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: workspace is not 16-byte aligned");
+  a.delta = static_cast<float *>(workspace);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_attn_delta(a, st);
+  if (e == cudaSuccess) e = launch_attn_bwd_generic(a, st);
+  return cuda_status(e, "mhc_attn_bwd");
+}
+
+}  // extern "C"

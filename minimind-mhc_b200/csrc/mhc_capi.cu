@@ -15,7 +15,9 @@ namespace mhc {
 
 static thread_local char g_err[512] = "";
 
-static int fail(int code, const char *fmt, ...) {
+void clear_error() { g_err[0] = 0; }
+
+int fail(int code, const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -23,7 +25,7 @@ static int fail(int code, const char *fmt, ...) {
   return code;
 }
 
-static int cuda_status(cudaError_t e, const char *where) {
+int cuda_status(cudaError_t e, const char *where) {
   if (e == cudaSuccess) return MHC_OK;
   return fail(MHC_ERR_CUDA, "%s: %s", where, cudaGetErrorString(e));
 }

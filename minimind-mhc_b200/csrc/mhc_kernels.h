@@ -9,6 +9,12 @@
 
 namespace mhc {
 
+// Error message of the calling thread (mhc_last_error), shared by the files that
+// define entry points: fail() stores the message and returns `code`.
+void clear_error();
+int fail(int code, const char *fmt, ...);
+int cuda_status(cudaError_t e, const char *where);
+
 struct CoefParams {
   const void *alpha_pre, *bias_pre, *alpha_post, *bias_post, *alpha_res, *bias_res;
   int param_dtype;

@@ -25,6 +25,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes)
@@ -54,6 +55,17 @@ _PROTOS = {
                           _P, _P, _SZ, _P]),
     "mhc_stream_expand_fwd": (_I, [_P, _P, _I, _I64, _I, _I, _P]),
     "mhc_stream_expand_bwd": (_I, [_P, _P, _I, _I64, _I, _I, _P]),
+    "mhc_attn_fwd": (_I, [_P, _P, _P, _I, _I64, _I, _I, _I, _P, _P, _I, _I64, _F, _P, _P, _P, _P]),
+    "mhc_attn_bwd_workspace": (_SZ, [_I64, _I]),
+    "mhc_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I, _I, _I, _P, _P, _I, _I64, _F, _P, _P, _P, _P, _SZ,
+                          _P]),
+    "mhc_route_fwd_workspace": (_SZ, [_I64, _I]),
+    "mhc_route_fwd": (_I, [_P, _I, _I64, _I, _I64, _I, _F, _P, _P, _P, _P, _P, _SZ, _P]),
+    "mhc_route_bwd": (_I, [_P, _I, _I64, _I, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "mhc_grad_norm_workspace": (_SZ, []),
+    "mhc_grad_norm": (_I, [_P, _I, _I, _P, _SZ, _P]),
+    "mhc_adamw_step": (_I, [_P, _I, _I, _D, _D, _D, _D, _D, _D, _P, _P, _P]),
+    "mhc_adamw_unpack": (_I, [_P, _I, _P, _P, _I64, _P]),
     "mhc_set_path_policy": (_I, [_I]),
     "mhc_last_path": (_I, []),
     "mhc_device_error": (_I, [_I]),

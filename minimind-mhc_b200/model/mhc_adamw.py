@@ -1,0 +1,264 @@
+"""AdamW over many tensors in one launch, with moments in fp32 or in 8 bits.
+
+``adamw_step`` / ``adamw_step_8bit`` are the step itself on lists of tensors, in
+place; :class:`AdamW` is a ``torch.optim.Optimizer`` around them.  The update is
+``torch.optim.AdamW``'s (decoupled weight decay, bias correction), which the
+reference's trainers use (``trainer/train_pretrain.py:146``), with the gradient
+clipping of the line before the step (``:45-52``) as an argument: the norm is
+taken on the device, scales the gradients inside the step and is never read by
+the host.  CUDA tensors only.
+
+8-bit moments: 256 consecutive values of a tensor share one fp32 scale, the
+largest magnitude among them.  The first moment is int8, ``(c/127)^2 * sign *
+scale``, the second uint8, ``(c/255)^4 * scale``; a parameter's optimizer state
+is 2.03 bytes a value instead of 8.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import _native as nat
+
+QUANT_BLOCK = 256  # values that share a scale
+
+_Tensor = torch.Tensor
+_CODE = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
+
+
+class Moment8(NamedTuple):
+    """One tensor's moment in 8 bits: ``codes`` int8 (first moment) or uint8
+    (second), ``scales`` fp32, one for every 256 values."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def zero_moment(p: torch.Tensor, signed: bool) -> Moment8:
+    """The 8-bit moment of ``p`` before the first step."""
+    n = p.numel()
+    return Moment8(torch.zeros(p.shape, dtype=torch.int8 if signed else torch.uint8, device=p.device),
+                   torch.zeros(-(-n // QUANT_BLOCK), dtype=torch.float32, device=p.device))
+
+
+def unpack_moment(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The fp32 values that an 8-bit moment stands for, in the codes' shape."""
+    nat.require_cuda(codes, scales)
+    n = codes.numel()
+    if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
+        raise TypeError(f"unpack_moment: int8 / uint8 codes and fp32 scales are wanted, got {codes.dtype} and "
+                        f"{scales.dtype}")
+    if scales.numel() != -(-n // QUANT_BLOCK):
+        raise ValueError(f"unpack_moment: {n} codes have {-(-n // QUANT_BLOCK)} scales, got {scales.numel()}")
+    if scales.device != codes.device:
+        raise ValueError("unpack_moment: codes and scales are on different devices")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    with torch.cuda.device(codes.device):
+        out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+        nat.call("mhc_adamw_unpack", codes.data_ptr(), int(codes.dtype == torch.int8), scales.data_ptr(),
+                 out.data_ptr(), n, nat.stream_of(codes))
+    return out
+
+
+def _pointers(ts):
+    return list(map(_Tensor.data_ptr, ts))
+
+
+def _check_list(what, ts, sizes, device, dtypes):
+    if len(ts) != len(sizes):
+        raise ValueError(f"adamw: {len(sizes)} params but {len(ts)} {what}")
+    found = {t.dtype for t in ts}
+    if not found <= dtypes:
+        raise TypeError(f"adamw: {what} must be {' / '.join(sorted(str(d) for d in dtypes))}, got "
+                        f"{', '.join(sorted(str(d) for d in found - dtypes))}")
+    if {t.device for t in ts} != {device}:
+        raise ValueError(f"adamw: every tensor must be on {device}; {what} are not")
+    if not all(map(_Tensor.is_contiguous, ts)):
+        raise ValueError(f"adamw: {what} must be contiguous")
+    if list(map(_Tensor.numel, ts)) != sizes:
+        raise ValueError(f"adamw: {what} and params differ in size")
+
+
+_FLOATS = frozenset(_CODE)
+_F32 = frozenset((torch.float32,))
+
+
+def _table(params, grads, ms, vs, steps, bits):
+    """The host array of ``mhc_adamw_tensor`` (9 words each) of checked tensors."""
+    count = len(params)
+    if len(grads) != count or len(ms) != count or len(vs) != count:
+        raise ValueError(f"adamw: {count} params, {len(grads)} grads, {len(ms)} and {len(vs)} moments")
+    device = params[0].device
+    nat.require_cuda(params[0])
+    sizes = list(map(_Tensor.numel, params))
+    _check_list("params", params, sizes, device, _FLOATS)
+    _check_list("grads", grads, sizes, device, _FLOATS)
+    table = np.zeros((count, 9), dtype=np.uint64)
+    table[:, 0] = _pointers(params)
+    table[:, 1] = _pointers(grads)
+    if bits == 32:
+        _check_list("exp_avgs", ms, sizes, device, _F32)
+        _check_list("exp_avg_sqs", vs, sizes, device, _F32)
+        table[:, 2] = _pointers(ms)
+        table[:, 3] = _pointers(vs)
+    else:
+        scales = [-(-n // QUANT_BLOCK) for n in sizes]
+        for col, what, pairs, dt in ((2, "exp_avgs", ms, torch.int8), (3, "exp_avg_sqs", vs, torch.uint8)):
+            codes, sc = [m[0] for m in pairs], [m[1] for m in pairs]
+            _check_list(what + " codes", codes, sizes, device, frozenset((dt,)))
+            _check_list(what + " scales", sc, scales, device, _F32)
+            table[:, col] = _pointers(codes)
+            table[:, col + 2] = _pointers(sc)
+    table[:, 6] = sizes
+    table[:, 7] = steps
+    types = table.view(np.int32)[:, 16:18]
+    types[:, 0] = [_CODE[p.dtype] for p in params]
+    types[:, 1] = [_CODE[g.dtype] for g in grads]
+    return table
+
+
+def _grad_norm(tables, device):
+    """The workspace that holds the squared norm of all the tables' gradients."""
+    ws = nat.workspace(nat.lib().mhc_grad_norm_workspace(), device)
+    for i, t in enumerate(tables):
+        nat.call("mhc_grad_norm", t.ctypes.data, len(t), int(i > 0), ws.data_ptr(), ws.numel(),
+                 torch.cuda.current_stream(device).cuda_stream)
+    return ws
+
+
+def _run(table, bits, device, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm):
+    nat.call("mhc_adamw_step", table.ctypes.data, len(table), bits, lr, betas[0], betas[1], eps, weight_decay,
+             max_grad_norm or 0.0, nat.ptr(norm_ws), nat.ptr(norm), torch.cuda.current_stream(device).cuda_stream)
+
+
+def _check_call(max_grad_norm):
+    if max_grad_norm is not None and not max_grad_norm > 0:
+        raise ValueError(f"adamw: max_grad_norm must be positive or None, got {max_grad_norm}")
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw: the step number is an argument of the launch, so a step cannot be captured in a "
+                           "CUDA graph")
+
+
+def _step(params, grads, ms, vs, bits, step, lr, betas, eps, weight_decay, max_grad_norm):
+    _check_call(max_grad_norm)
+    if not params:
+        return None
+    table = _table(params, grads, ms, vs, step, bits)
+    device = params[0].device
+    with torch.cuda.device(device):
+        norm_ws = norm = None
+        if max_grad_norm is not None:
+            norm_ws = _grad_norm([table], device)
+            norm = torch.zeros((), dtype=torch.float32, device=device)
+        _run(table, bits, device, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm)
+    return norm
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               max_grad_norm=None):
+    """One step of AdamW, in place, over lists of contiguous tensors: parameters
+    and gradients fp32 / bf16 / fp16, moments fp32.
+
+    ``step`` counts the updates, this one included, from 1: one number, or one
+    for every tensor.  ``max_grad_norm`` scales the gradients to a norm (over
+    all of them) of at most that; the gradients themselves are left alone.
+    Returns that norm as a device scalar, or ``None`` without clipping.
+    """
+    return _step(params, grads, exp_avgs, exp_avg_sqs, 32, step, lr, betas, eps, weight_decay, max_grad_norm)
+
+
+@torch.no_grad()
+def adamw_step_8bit(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8,
+                    weight_decay=1e-2, max_grad_norm=None):
+    """:func:`adamw_step` with the moments as lists of (codes, scales)
+    (:class:`Moment8`).  The step itself uses the moments before they are
+    rounded to 8 bits again."""
+    return _step(params, grads, exp_avgs, exp_avg_sqs, 8, step, lr, betas, eps, weight_decay, max_grad_norm)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` on the kernels above.
+
+    ``state_bits`` 32 or 8 chooses how the moments are held.  ``max_grad_norm``
+    scales the gradients of all parameter groups to that norm as part of the
+    step; the norm before scaling is kept in ``grad_norm`` (a device scalar).
+    A parameter without a gradient is left out of a step and keeps its own step
+    count, as in torch.  All parameters are on one device.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 max_grad_norm=None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
+        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("AdamW: lr, eps, weight_decay >= 0 and betas in [0, 1) are wanted")
+        _check_call(max_grad_norm)
+        self.state_bits = state_bits
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def _state_of(self, p):
+        s = self.state[p]
+        if not s:
+            s["step"] = 0
+            if self.state_bits == 32:
+                s["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                s["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                s["exp_avg"], s["exp_avg_scale"] = zero_moment(p, True)
+                s["exp_avg_sq"], s["exp_avg_sq_scale"] = zero_moment(p, False)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        _check_call(self.max_grad_norm)
+        work, keep, states = [], [], []
+        for group in self.param_groups:
+            live = [p for p in group["params"] if p.grad is not None]
+            if not live:
+                continue
+            mine = [self._state_of(p) for p in live]
+            grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in live]
+            if self.state_bits == 32:
+                ms, vs = [s["exp_avg"] for s in mine], [s["exp_avg_sq"] for s in mine]
+            else:
+                ms = [(s["exp_avg"], s["exp_avg_scale"]) for s in mine]
+                vs = [(s["exp_avg_sq"], s["exp_avg_sq_scale"]) for s in mine]
+            work.append((group, _table(live, grads, ms, vs, [s["step"] + 1 for s in mine], self.state_bits)))
+            states += mine
+            keep.append((live[0].device, grads))
+        if not work:
+            return loss
+        device = keep[0][0]
+        if any(d != device for d, _ in keep):
+            raise ValueError("AdamW: all parameters must be on one device")
+        with torch.cuda.device(device):
+            norm_ws = norm = None
+            if self.max_grad_norm is not None:
+                norm_ws = _grad_norm([t for _, t in work], device)
+                self.grad_norm = norm = torch.zeros((), dtype=torch.float32, device=device)
+            for group, table in work:
+                _run(table, self.state_bits, device, group["lr"], group["betas"], group["eps"],
+                     group["weight_decay"], self.max_grad_norm, norm_ws, norm)
+        for s in states:
+            s["step"] += 1
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments keep the types they were saved in (torch
+        casts an optimizer's state to its parameter's type)."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        here = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, here):
+            for name, t in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(t):
+                    self.state[p][name] = t.detach().to(p.device, copy=True).contiguous()
