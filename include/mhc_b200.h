@@ -224,6 +224,9 @@ int mhc_pre_bwd(const void *x, int x_dtype, int64_t T, int n, int C,
 /* Training step: causal attention over packed sequences                     */
 /* ------------------------------------------------------------------------ */
 
+/* Bytes of scratch `mhc_attn_fwd` needs. */
+size_t mhc_attn_fwd_workspace(int64_t T);
+
 /*
  * out[i,h] = sum_j P[i,j] v[j,h'],  P[i,:] = softmax over the visible j of scale q[i,h] . k[j,h']
  *
@@ -246,7 +249,7 @@ int mhc_pre_bwd(const void *x, int x_dtype, int64_t T, int n, int C,
  */
 int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t T, int H, int Hk, int D,
                  const int64_t *strides, const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale,
-                 void *out, void *out_lo, float *lse, void *stream);
+                 void *out, void *out_lo, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Bytes of scratch `mhc_attn_bwd` needs. */
 size_t mhc_attn_bwd_workspace(int64_t T, int H);
@@ -472,7 +475,8 @@ int mhc_last_path(void);
  * 21..26 = the producer / MMA / ingest / coefficient / Sinkhorn / z role of
  * the single-read forward kernel, 31..37 = the producer / MMA / row /
  * coefficient / pre-aggregate / Sinkhorn / merge role of the fused merge +
- * coefficient kernel, 11..14 = one of the producer / MMA /
+ * coefficient kernel, 41..43 = the TMA / MMA / softmax role of the attention
+ * forward kernel, 11..14 = one of the producer / MMA /
  * epilogue / prep roles of the backward tensor-core kernel, 99 = the
  * self-test below).  A kernel whose wait runs out gives up
  * instead of hanging and overwrites the outputs it owns with NaN.

@@ -20,7 +20,7 @@
 #include <initializer_list>
 #include <mutex>
 
-#include "mhc_attn.cuh"
+#include "mhc_attn_tc.cuh"
 #include "mhc_b200.h"
 #include "mhc_device.cuh"
 #include "mhc_dispatch.cuh"
@@ -411,9 +411,11 @@ static bool misaligned(size_t es, std::initializer_list<const void *> ps) {
 
 extern "C" {
 
+size_t mhc_attn_fwd_workspace(int64_t T) { return T < 1 ? 256 : attn_order_bytes(T) + 256; }
+
 int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t T, int H, int Hk, int D,
                  const int64_t *strides, const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale, void *out,
-                 void *out_lo, float *lse, void *stream) {
+                 void *out_lo, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
   clear_error();
   attn::Args a{};
   a.q = q; a.k = k; a.v = v; a.o = out; a.o_lo = out_lo; a.lse = lse;
@@ -424,7 +426,15 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
   if (!q || !k || !v || !out || !lse) return fail(MHC_ERR_NULL, "mhc_attn_fwd: required pointer is NULL");
   if (misaligned(dtype == MHC_F32 ? 4 : 2, {q, k, v, out, out_lo}) || ((uintptr_t)lse & 3))
     return fail(MHC_ERR_ALIGN, "mhc_attn_fwd: a pointer is not aligned to its elements");
+  if (!workspace || workspace_bytes < mhc_attn_fwd_workspace(T))
+    return fail(MHC_ERR_WORKSPACE, "mhc_attn_fwd: workspace %zu < %zu bytes", workspace_bytes, mhc_attn_fwd_workspace(T));
+  if ((uintptr_t)workspace & 15) return fail(MHC_ERR_ALIGN, "mhc_attn_fwd: workspace is not 16-byte aligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!generic_forced() && attn_tc_eligible(a, false)) {
+    const cudaError_t e = launch_attn_fwd_tc(a, static_cast<int *>(workspace), st);
+    if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_fwd");
+    cudaGetLastError();
+  }
   return cuda_status(launch_attn_fwd_generic(a, st), "mhc_attn_fwd");
 }
 

@@ -56,6 +56,7 @@ static int check_shape(int64_t T, int n, int C) {
 }
 
 static int g_policy = MHC_PATH_AUTO;
+bool generic_forced() { return g_policy == MHC_PATH_GENERIC; }
 // kernel family of the last pre-stage call in the process (the autograd
 // engine runs backward on its own thread, so this is not thread-local)
 static std::atomic<int> g_last_path{0};
@@ -115,7 +116,7 @@ int mhc_last_path(void) { return g_last_path.load(); }
 
 int mhc_device_error(int clear) {
   if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  const int words[5] = {read_sr_error(clear != 0), read_tc_error(clear != 0), read_tcb_error(clear != 0),
+  const int words[6] = {read_atf_error(clear != 0), read_sr_error(clear != 0), read_tc_error(clear != 0), read_tcb_error(clear != 0),
                         read_ch_error(clear != 0), read_selftest_error(clear != 0)};
   for (int w : words)
     if (w < 0) return -1;

@@ -124,6 +124,8 @@ int read_tcb_error(bool clear);
 // their device error words.
 int *host_error_flag();
 int read_selftest_error(bool clear);
+int read_atf_error(bool clear);  // attention forward
+bool generic_forced();           // MHC_PATH_GENERIC is set
 
 // ---- stand-alone pieces -----------------------------------------------------
 cudaError_t launch_sinkhorn_fwd(int n, const void *M, int m_dtype, void *Y, int y_dtype,

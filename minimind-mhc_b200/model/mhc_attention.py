@@ -41,9 +41,10 @@ class _PackedAttentionFn(torch.autograd.Function):
             strides = (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
                                            v.stride(1))
             batch = 0 if cu is None else cu.numel() - 1
+            ws = nat.workspace(nat.lib().mhc_attn_fwd_workspace(t), dev)
             nat.call("mhc_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.dtype_code(q.dtype), t, h, hk, d,
                      strides, nat.ptr(cu), batch, seqlen, scale, out.data_ptr(), nat.ptr(out_lo), lse.data_ptr(),
-                     nat.stream_of(q))
+                     ws.data_ptr(), ws.numel(), nat.stream_of(q))
         ctx.save_for_backward(q, k, v, cu, out, out_lo, lse)
         ctx.meta = (strides, batch, seqlen, scale)
         return out
