@@ -224,6 +224,9 @@ int mhc_pre_bwd(const void *x, int x_dtype, int64_t T, int n, int C,
 /* Training step: causal attention over packed sequences                     */
 /* ------------------------------------------------------------------------ */
 
+/* Values from one head's row of lse to the next: T up to whole tiles of 128. */
+int64_t mhc_attn_lse_pitch(int64_t T);
+
 /* Bytes of scratch `mhc_attn_fwd` needs. */
 size_t mhc_attn_fwd_workspace(int64_t T);
 
@@ -240,8 +243,9 @@ size_t mhc_attn_fwd_workspace(int64_t T);
  *
  * q, k, v: element (t, h, d) at t * strides[0] + h * strides[1] + d (q), strides
  * [2], [3] (k), [4], [5] (v); host array of 6, in elements.  out is (T, H, D)
- * contiguous in `dtype`.  For mhc_attn_bwd: lse (H, T) fp32, log2 of the row's sum
- * of exp2(scale log2(e) score), +inf for a row that sees nothing; out_lo (NULL:
+ * contiguous in `dtype`.  For mhc_attn_bwd: lse (H, mhc_attn_lse_pitch(T)) fp32, the first
+ * T of each row log2 of the token's sum of exp2(scale log2(e) score), +inf where it
+ * sees nothing; out_lo (NULL:
  * not wanted), laid out like out, what the rounding of out left over, in `dtype`.
  *
  * Replaces: scaled_dot_product_attention in Attention.forward
@@ -475,8 +479,8 @@ int mhc_last_path(void);
  * 21..26 = the producer / MMA / ingest / coefficient / Sinkhorn / z role of
  * the single-read forward kernel, 31..37 = the producer / MMA / row /
  * coefficient / pre-aggregate / Sinkhorn / merge role of the fused merge +
- * coefficient kernel, 41..43 = the TMA / MMA / softmax role of the attention
- * forward kernel, 11..14 = one of the producer / MMA /
+ * coefficient kernel, 41..43 and 51..53 = the TMA / MMA / softmax
+ * role of the attention forward and backward kernels, 11..14 = one of the producer / MMA /
  * epilogue / prep roles of the backward tensor-core kernel, 99 = the
  * self-test below).  A kernel whose wait runs out gives up
  * instead of hanging and overwrites the outputs it owns with NaN.

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
   for (int i = 0; i < 4; ++i) {
     const int t = q0 + ty * 4 + i;
     inv[i] = sum[i] == 0.f ? 0.f : 1.f / sum[i];
-    if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.T + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
+    if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.Tp + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
   }
   T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
   store_rows<T, DP>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
       }
       if (tid < TILE) {
         const int64_t t = (DKV ? c0 : r0) + tid;
-        L[tid] = t < a.T ? a.lse[(int64_t)h * a.T + t] : INFINITY;
-        Dl[tid] = t < a.T ? a.delta[(int64_t)h * a.T + t] : 0.f;
+        L[tid] = t < a.T ? a.lse[(int64_t)h * a.Tp + t] : INFINITY;
+        Dl[tid] = t < a.T ? a.delta[(int64_t)h * a.Tp + t] : 0.f;
       }
       __syncthreads();
       float p[4][4], ds[4][4];
@@ -283,25 +283,57 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
   }
 }
 
-// D_i = dO_i . O_i, one warp a (token, head).  O is its rounded value plus what the
-// rounding left over: D is subtracted from dO . V, of which it is the mean, so with
-// few keys the rounding of O alone would show in dS as an error of its own size.
-template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const Args a) {
-  const int64_t rows = a.T * a.H;
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    const T *o = static_cast<const T *>(a.out) + r * a.D, *d = static_cast<const T *>(a.dout) + r * a.D;
+// D_i = dO_i . O_i.  O is its rounded value plus what the rounding left over: D is
+// subtracted from dO . V, of which it is the mean, so with few keys the rounding of
+// O alone would show in dS as an error of its own size.  16 lanes a row, a block 128
+// tokens of one head; it reads O, its rest and dO once and is bound by that.
+// fp16: also the largest |dO| and |V| inside of the sequences.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t *amax) {
+  const int h = blockIdx.y, l = threadIdx.x & 15;
+  const Span range = packed_range(a);
+  const T *o = static_cast<const T *>(a.out), *lo = static_cast<const T *>(a.out_lo), *d = static_cast<const T *>(a.dout);
+  float most_o = 0.f, most_v = 0.f;
+#pragma unroll 2
+  for (int it = 0; it < 8; ++it) {
+    const int64_t t = (int64_t)blockIdx.x * 128 + it * 16 + (threadIdx.x >> 4);
+    if (t >= a.T) break;
+    const bool inside = t >= range.start && t < range.end;
+    const int64_t at = (t * a.H + h) * a.D;
     float s = 0.f;
-    const T *l = a.out_lo ? static_cast<const T *>(a.out_lo) + r * a.D : nullptr;
-    for (int c = lane; c < a.D; c += 32) {
-      const float v = to_f(o[c]) + (l ? to_f(l[c]) : 0.f);
-      s = fmaf(v, to_f(d[c]), s);
+    for (int c = l * VEC; c < a.D; c += 16 * VEC) {
+      T ov[VEC], lv[VEC], dv[VEC];
+      if constexpr (VEC == 8) {
+        *reinterpret_cast<uint4 *>(ov) = ldg_stream(o + at + c);
+        *reinterpret_cast<uint4 *>(dv) = *reinterpret_cast<const uint4 *>(d + at + c);
+        if (lo) *reinterpret_cast<uint4 *>(lv) = ldg_stream(lo + at + c);
+      } else {
+        ov[0] = o[at + c];
+        dv[0] = d[at + c];
+        if (lo) lv[0] = lo[at + c];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        s = fmaf(to_f(ov[e]) + (lo ? to_f(lv[e]) : 0.f), to_f(dv[e]), s);
+        if (amax && inside) most_o = fmaxf(most_o, fabsf(to_f(dv[e])));
+      }
     }
 #pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const int64_t t = r / a.H;
-    if (lane == 0) a.delta[(r - t * a.H) * a.T + t] = s;
+    for (int x = 8; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x, 16);
+    if (l == 0) a.delta[(int64_t)h * a.Tp + t] = s;
+    if (amax && inside && h < a.Hk)
+      for (int c = l; c < a.D; c += 16) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
+  }
+  if (amax) {
+#pragma unroll
+    for (int x = 16; x; x >>= 1) {
+      most_o = fmaxf(most_o, __shfl_xor_sync(0xffffffffu, most_o, x));
+      most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, x));
+    }
+    if ((threadIdx.x & 31) == 0) {  // of non-negative floats the bits are in order: a maximum in any order
+      atomicMax(amax, __float_as_uint(most_o));
+      atomicMax(amax + 1, __float_as_uint(most_v));
+    }
   }
 }
 
@@ -357,10 +389,18 @@ cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
   });
 }
 
-cudaError_t launch_attn_delta(const attn::Args &a, cudaStream_t stream) {
-  const unsigned grid = grid_for(a.T * a.H, 8, device_sm_count(), 8);
+cudaError_t launch_attn_delta(const attn::Args &a, uint32_t *amax, cudaStream_t stream) {
+  const dim3 grid((unsigned)((a.T + 127) / 128), (unsigned)a.H);
+  const bool vec = a.D % 8 == 0 && !(((uintptr_t)a.out | (uintptr_t)a.out_lo | (uintptr_t)a.dout) & 15);
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
-    attn::attn_delta_kernel<decltype(tag)><<<grid, 256, 0, stream>>>(a);
+    using T = decltype(tag);
+    if constexpr (sizeof(T) == 2) {
+      if (vec) {
+        attn::attn_delta_kernel<T, 8><<<grid, 256, 0, stream>>>(a, amax);
+        return cudaGetLastError();
+      }
+    }
+    attn::attn_delta_kernel<T, 1><<<grid, 256, 0, stream>>>(a, amax);
     return cudaGetLastError();
   });
 }
@@ -419,7 +459,7 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
   clear_error();
   attn::Args a{};
   a.q = q; a.k = k; a.v = v; a.o = out; a.o_lo = out_lo; a.lse = lse;
-  a.T = T; a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
+  a.T = T; a.Tp = mhc_attn_lse_pitch(T); a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
   a.cu = cu_seqlens; a.batch = batch; a.seqlen = seqlen;
   if (int st = check_attn("mhc_attn_fwd", a, strides, scale)) return st;
   if (T == 0) return MHC_OK;
@@ -430,7 +470,7 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
     return fail(MHC_ERR_WORKSPACE, "mhc_attn_fwd: workspace %zu < %zu bytes", workspace_bytes, mhc_attn_fwd_workspace(T));
   if ((uintptr_t)workspace & 15) return fail(MHC_ERR_ALIGN, "mhc_attn_fwd: workspace is not 16-byte aligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (!generic_forced() && attn_tc_eligible(a, false)) {
+  if (!generic_forced() && attn_tc_eligible(a)) {
     const cudaError_t e = launch_attn_fwd_tc(a, static_cast<int *>(workspace), st);
     if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_fwd");
     cudaGetLastError();
@@ -438,7 +478,12 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
   return cuda_status(launch_attn_fwd_generic(a, st), "mhc_attn_fwd");
 }
 
-size_t mhc_attn_bwd_workspace(int64_t T, int H) { return T < 1 || H < 1 ? 256 : (size_t)T * H * 4 + 256; }
+int64_t mhc_attn_lse_pitch(int64_t T) { return T < 1 ? 0 : (T + 127) / 128 * 128; }
+
+// delta, the two orders of the work, the two maxima of fp16
+size_t mhc_attn_bwd_workspace(int64_t T, int H) {
+  return T < 1 || H < 1 ? 256 : (size_t)mhc_attn_lse_pitch(T) * H * 4 + 2 * attn_order_bytes(T) + 256;
+}
 
 int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo, const void *dout,
                  const float *lse, int dtype, int64_t T, int H, int Hk, int D, const int64_t *strides, const int32_t *cu_seqlens,
@@ -448,7 +493,7 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
   attn::Args a{};
   a.q = q; a.k = k; a.v = v; a.out = out; a.out_lo = out_lo; a.dout = dout; a.lse = const_cast<float *>(lse);
   a.dq = dq; a.dk = dk; a.dv = dv;
-  a.T = T; a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
+  a.T = T; a.Tp = mhc_attn_lse_pitch(T); a.H = H; a.Hk = Hk; a.D = D; a.dtype = dtype;
   a.cu = cu_seqlens; a.batch = batch; a.seqlen = seqlen;
   if (int st = check_attn("mhc_attn_bwd", a, strides, scale)) return st;
   if (T == 0) return MHC_OK;
@@ -461,7 +506,23 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
   if ((uintptr_t)workspace & 15) return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: workspace is not 16-byte aligned");
   a.delta = static_cast<float *>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_attn_delta(a, st);
+  const bool tc = !generic_forced() && attn_tc_bwd_eligible(a);
+  int *order = reinterpret_cast<int *>(a.delta + a.Tp * H);
+  const size_t on = attn_order_bytes(T) / 4;
+  uint32_t *amax = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (tc && dtype == MHC_F16) {
+    amax = reinterpret_cast<uint32_t *>(order + 2 * on);
+    a.amax = amax;
+    e = cudaMemsetAsync(amax, 0, 8, st);
+  }
+  if (e == cudaSuccess) e = launch_attn_delta(a, amax, st);
+  if (e == cudaSuccess && tc) {
+    e = launch_attn_bwd_tc(a, order, order + on, st);
+    if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_bwd");
+    cudaGetLastError();
+    e = cudaSuccess;
+  }
   if (e == cudaSuccess) e = launch_attn_bwd_generic(a, st);
   return cuda_status(e, "mhc_attn_bwd");
 }

@@ -9,12 +9,13 @@ namespace attn {
 
 // q (T, H, D), k / v (T, Hk, D) with token and head strides in elements and
 // contiguous rows; out, dout, dq and dk / dv are contiguous; lse and delta are
-// (H, T) fp32; o_lo / out_lo hold what the rounding of out left over, or are null.  lse is in base 2: log2 of the sum of exp2(score * scale_log2).
+// (H, Tp) fp32; o_lo / out_lo hold what the rounding of out left over, or are null.  lse is in base 2: log2 of the sum of exp2(score * scale_log2).
 struct Args {
   const void *q, *k, *v, *out, *out_lo, *dout;
   void *o, *o_lo, *dq, *dk, *dv;
   float *lse, *delta;
-  int64_t T;
+  const uint32_t *amax;  // fp16 backward: the bits of max|dO| and max|V|
+  int64_t T, Tp;         // Tp: T up to whole tiles of 128, the pitch of lse and delta
   int H, Hk, D, dtype;
   int64_t qt, qh, kt, kh, vt, vh;
   const int32_t *cu;  // (batch + 1) offsets of the packed sequences, or null: sequences of seqlen tokens
@@ -64,6 +65,6 @@ __device__ __forceinline__ Span packed_range(const Args &a) {
 
 cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream);
 cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream);
-cudaError_t launch_attn_delta(const attn::Args &a, cudaStream_t stream);
+cudaError_t launch_attn_delta(const attn::Args &a, uint32_t *amax, cudaStream_t stream);
 
 }  // namespace mhc

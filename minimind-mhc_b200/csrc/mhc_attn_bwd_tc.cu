@@ -1,0 +1,593 @@
+// Backward of causal attention over packed sequences on the 5th-generation tensor
+// cores (bf16 / fp16, head sizes that are multiples of 8 up to 128).
+//
+// Two kernels of one form, each of which owns the rows of what it sums, so no two
+// blocks add to the same gradient and every sum has a fixed order:
+//
+//   DKV: a block owns 128 keys of one key head and walks the queries that see them,
+//        of every head of the group:       rows R1 = K, R2 = V, columns C1 = Q, C2 = dO
+//          S = R1 C1^T, P = exp2(S c - lse_col);       dV += P C2
+//          dP = R2 C2^T, dS = P (dP - D_col);          dK += dS C1
+//   DQ:  a block owns 128 queries of one head and walks their keys:
+//                                          rows R1 = Q, R2 = dO, columns C1 = K, C2 = V
+//          S, P, dP, dS as above with lse and D of the row;   dQ += dS C1
+//
+// (seven products of 128 x 128 x D a tile where five would do if dQ were added up
+// over blocks: two more on the tensor core instead of atomics in an order that
+// changes).  P and dS never leave TMEM: a thread reads its half row of S, writes P
+// over it as 16-bit values, which is the A operand of the next product; the column
+// operands serve S and dP as they are (K-major) and the gradients as they lie
+// (their rows are the summed index: MN-major).
+//
+// Per tile the tensor core is given S(j+1) behind dV(j), and dP(j+1) behind dK(j),
+// so it works while the 8 warps of the softmax are at the other half of the step.
+//
+// fp16 has no room for small dS or P: P is held times 2^10, and dS times a power of
+// two from the largest |dO| and |V| of the call that no dS can overflow
+// (|dS| <= 2 D max|dO| max|V|); both come off in fp32 at the end.  bf16 needs
+// neither.
+//
+// Grid, order of the work, masks and tokens outside of the sequences: as in the
+// forward kernel.  Warps 0-7: softmax (two to each quarter of the rows, 64 columns
+// each) and epilogue; 8: TMA; 9: MMA issue.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "mhc_attn_tc.cuh"
+
+namespace mhc {
+
+__device__ int g_atb_error = 0;
+
+namespace attn {
+
+namespace {
+
+constexpr int NTHREADS = 320;
+constexpr int W_TMA = 8, W_MMA = 9;
+constexpr int TMEM_COLS = 512;
+constexpr uint32_t S_COL = 0, DP_COL = 128, A1_COL = 256, A2_COL = 384;
+constexpr float P_SHIFT = 10.f;  // fp16: P times 2^10
+
+enum { ERR_TMA = 51, ERR_MMA = 52, ERR_SOFTMAX = 53 };
+
+struct Item {
+  int r0, head;   // first row, row head (DKV: key head)
+  int c0, cols;   // first column tile's first token, column tiles
+  int n;          // steps: cols, times the group's heads for DKV
+  int done;
+};
+
+template <int DP>
+struct Cfg {
+  static constexpr int NB = nblk(DP);
+  static constexpr uint32_t TILE = NB * BLK;
+  static constexpr int ST = NB == 1 ? 4 : 2;        // stages of C1 and of C2
+  static constexpr uint32_t VEC = 2 * TM * 4;       // a stage's lse and D of its columns
+};
+
+constexpr int B_ITEM_F = 0, B_ITEM_E = 2, B_RF = 4, B_RE = 5, B_LAND = 6, B_SF = 7, B_PF = 8, B_DPF = 9, B_DSF = 10,
+              B_ACC = 11, B_DRAIN = 12, B_1F = 13;
+// then ST each: 1F, 1E, 2F, 2E
+
+struct Sched {
+  const int *order;  // null: tile 0 first for keys, the last first for queries
+  int tiles, heads, items;
+};
+
+__device__ __forceinline__ void give_up(int code, volatile int *abort_flag, int *err_flag) {
+  *abort_flag = 1;
+  report_give_up(&g_atb_error, err_flag, code);
+}
+
+template <bool DKV>
+__device__ __forceinline__ bool item_of(const Args &a, const Sched &s, int64_t rank, Item &it) {
+  if (rank >= s.items) {
+    it.done = 1;
+    it.n = 0;
+    return false;
+  }
+  it.done = 0;
+  const int at = (int)(rank / s.heads);
+  it.head = (int)(rank % s.heads);
+  const int tile = s.order ? s.order[at] : (DKV ? at : s.tiles - 1 - at);
+  it.r0 = tile * TM;
+  const int r1 = (int)min((int64_t)it.r0 + TM, a.T) - 1;
+  int lo, hi;  // column tiles
+  if (DKV) {
+    const int end = span_of(a, r1).end;
+    lo = tile;
+    hi = end > it.r0 ? (end - 1) / TM + 1 : tile;
+  } else {
+    const int first = span_of(a, it.r0).start;
+    lo = first / TM;
+    hi = first <= r1 ? tile + 1 : lo;
+  }
+  it.c0 = lo * TM;
+  it.cols = hi - lo;
+  it.n = it.cols * (DKV ? a.H / a.Hk : 1);
+  return true;
+}
+
+// fp16: the power of two that dS is held times, from the bits of max|dO| and max|V|
+template <typename T>
+__device__ __forceinline__ float ds_factor(const Args &a) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const float b = 2.f * (float)a.D * __uint_as_float(a.amax[0]) * __uint_as_float(a.amax[1]);
+    if (!(b > 0.f) || b > 1e38f) return 1.f;
+    const int e = 15 - (ilogbf(b) + 1);  // b 2^e < 2^15
+    return ldexpf(1.f, max(-60, min(60, e)));
+  }
+  return 1.f;
+}
+
+template <typename T, int DP, bool DKV>
+__global__ void __launch_bounds__(NTHREADS, 1)
+attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Map r2map, const __grid_constant__ Map c1map,
+                   const __grid_constant__ Map c2map, const Args a, const Sched sched) {
+  using C = Cfg<DP>;
+  constexpr int NB = C::NB, ST = C::ST;
+  constexpr int B_1E = B_1F + ST, B_2F = B_1E + ST, B_2E = B_2F + ST, NBARS = B_2E + ST;
+  constexpr bool F16 = std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Item items[2];
+  __shared__ __align__(8) uint64_t bars[NBARS];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *gen = smem_raw + (base - raw);
+  const uint32_t rs = base, c1s = rs + 2 * C::TILE, c2s = c1s + ST * C::TILE, vecs = c2s + ST * C::TILE;
+  volatile int *abort_flag = &abort_word;
+  const uint32_t bar0 = smem_u32(bars);
+#define BAR(i) (bar0 + 8u * (uint32_t)(i))
+#define WAIT_WARP(bar, par) (__all_sync(0xffffffffu, wait_parity<false>((bar), (par), abort_flag)))
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.H / a.Hk;
+
+  if (tid == 0) {
+    abort_word = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(BAR(B_ITEM_F + i), 1);
+      mbar_init(BAR(B_ITEM_E + i), 257);  // the softmax threads and the MMA thread have read it
+    }
+    mbar_init(BAR(B_RF), 1);
+    mbar_init(BAR(B_RE), 1);
+    mbar_init(BAR(B_LAND), 1);
+    mbar_init(BAR(B_SF), 1);
+    mbar_init(BAR(B_PF), 256);
+    mbar_init(BAR(B_DPF), 1);
+    mbar_init(BAR(B_DSF), 256);
+    mbar_init(BAR(B_ACC), 1);
+    mbar_init(BAR(B_DRAIN), 1);
+    for (int i = 0; i < 4 * ST; ++i) mbar_init(BAR(B_1F + i), 1);
+    fence_mbar_init_cluster();
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  grid_dep_launch();
+  grid_dep_wait();
+
+  if (warp == W_TMA) {
+    // ---------------- TMA: whole warp, lane 0 issues ----------------
+    const Span range = packed_range(a);
+    bool ok = true;
+    int g = 0, lands = 0, rn = 0;
+    // a column tile: rows outside of the sequences are zeroed, since as B operands of the gradients they
+    // meet P = dS = 0, which a NaN would survive
+    auto column = [&](uint32_t dst, const Map &map, int head, int row, int full, bool vec, int h) {
+      const bool clean = row < range.start || min((int64_t)row + TM, a.T) > range.end;
+      const uint32_t bar = clean ? BAR(B_LAND) : BAR(full);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::TILE + (vec ? C::VEC : 0u));
+        load_rows(dst, map, NB, head, row, bar);
+        if (vec) {
+          const uint32_t v = vecs + (uint32_t)(g % ST) * C::VEC;
+          bulk_load(v, a.lse + (int64_t)h * a.Tp + row, TM * 4, bar);
+          bulk_load(v + TM * 4, a.delta + (int64_t)h * a.Tp + row, TM * 4, bar);
+        }
+      }
+      __syncwarp();
+      if (clean) {
+        if (!WAIT_WARP(BAR(B_LAND), (uint32_t)lands & 1u)) ok = false;
+        ++lands;
+        zero_outside(gen + (dst - base), NB, row, range, lane);
+        if (lane == 0) mbar_arrive(BAR(full));
+      }
+    };
+    for (int i = 0; ok; ++i) {
+      Item it;
+      const bool live = item_of<DKV>(a, sched, snake(i, blockIdx.x, gridDim.x), it);
+      if (!WAIT_WARP(BAR(B_ITEM_E + (i & 1)), ((uint32_t)(i >> 1) & 1u) ^ 1u)) { ok = false; break; }
+      if (lane == 0) {
+        items[i & 1] = it;
+        mbar_arrive(BAR(B_ITEM_F + (i & 1)));
+      }
+      __syncwarp();
+      if (!live) break;
+      if (it.n == 0) continue;
+      if (!WAIT_WARP(BAR(B_RE), ((uint32_t)rn & 1u) ^ 1u)) { ok = false; break; }
+      ++rn;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(BAR(B_RF), 2 * C::TILE);
+        load_rows(rs, r1map, NB, it.head, it.r0, BAR(B_RF));
+        load_rows(rs + C::TILE, r2map, NB, it.head, it.r0, BAR(B_RF));
+      }
+      for (int j = 0; j < it.n && ok; ++j, ++g) {
+        const int s = g % ST;
+        const uint32_t free_par = ((uint32_t)(g / ST) & 1u) ^ 1u;
+        const int row = it.c0 + (j % it.cols) * TM;
+        const int head = DKV ? it.head * G + j / it.cols : it.head / G;
+        if (!WAIT_WARP(BAR(B_1E + s), free_par)) { ok = false; break; }
+        column(c1s + s * C::TILE, c1map, head, row, B_1F + s, DKV, head);
+        if (!WAIT_WARP(BAR(B_2E + s), free_par)) { ok = false; break; }
+        column(c2s + s * C::TILE, c2map, head, row, B_2F + s, false, head);
+      }
+    }
+    if (!ok && lane == 0) give_up(ERR_TMA, abort_flag, a.err_flag);
+    // copies in flight land before the block may exit
+    for (int p = g > ST ? g - ST : 0; p < g; ++p) {
+      wait_parity<false>(BAR(B_1F + p % ST), (uint32_t)(p / ST) & 1u, nullptr);
+      wait_parity<false>(BAR(B_2F + p % ST), (uint32_t)(p / ST) & 1u, nullptr);
+    }
+    if (rn > 0) wait_parity<false>(BAR(B_RF), (uint32_t)(rn - 1) & 1u, nullptr);
+  } else if (warp == W_MMA) {
+    // ---------------- MMA issue: one thread ----------------
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_of<T>(128, 0), id_g = idesc_of<T>(DP, 1);
+      bool ok = true;
+      int i = 0, rn = 0, gk = 0, steps = 0;
+      struct Step {
+        int j, n, g;
+      } cur, nxt;
+      auto advance = [&](Step &s) -> bool {  // the next step, of this item or of the next one that has any
+        if (s.j + 1 < s.n) {
+          ++s.j;
+        } else {
+          while (true) {
+            if (!wait_parity<false>(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u, abort_flag)) { ok = false; return false; }
+            const bool done = items[i & 1].done;
+            s.j = 0;
+            s.n = items[i & 1].n;
+            mbar_arrive(BAR(B_ITEM_E + (i & 1)));
+            ++i;
+            if (done) return false;
+            if (s.n > 0) break;
+          }
+          if (!wait_parity<false>(BAR(B_RF), (uint32_t)rn & 1u, abort_flag)) { ok = false; return false; }
+          ++rn;
+        }
+        s.g = gk++;
+        return true;
+      };
+      // [128 x 128] = rows (K-major) times columns^T (K-major)
+      auto cross = [&](uint32_t d, uint32_t r, uint32_t c) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_bf16(d, umma_desc_sw128(r + (kk >> 2) * BLK + (kk & 3) * 32),
+                    umma_desc_sw128(c + (kk >> 2) * BLK + (kk & 3) * 32), id_s, kk > 0);
+      };
+      // accumulator += W C: W [128 x 128] 16-bit in TMEM, its second 64 columns 64 TMEM columns on; C MN-major
+      auto add = [&](uint32_t d, uint32_t w, uint32_t c, bool begin) {
+#pragma unroll
+        for (int kk = 0; kk < TM / 16; ++kk)
+          umma_f16_ts(d, w + (kk >> 2) * 64u + (kk & 3) * 8u, umma_desc(c + kk * 2048, BLK, 1024, 2), id_g, !begin || kk > 0);
+      };
+      auto scores = [&](const Step &s) {
+        if (!wait_parity<false>(BAR(B_1F + s.g % ST), (uint32_t)(s.g / ST) & 1u, abort_flag)) { ok = false; return; }
+        tc_fence_after();
+        cross(tmem + S_COL, rs, c1s + (s.g % ST) * C::TILE);
+        umma_commit(BAR(B_SF));
+      };
+      auto dprob = [&](const Step &s) {
+        if (!wait_parity<false>(BAR(B_2F + s.g % ST), (uint32_t)(s.g / ST) & 1u, abort_flag)) { ok = false; return; }
+        tc_fence_after();
+        cross(tmem + DP_COL, rs + C::TILE, c2s + (s.g % ST) * C::TILE);
+        umma_commit(BAR(B_DPF));
+        if (!DKV) umma_commit(BAR(B_2E + s.g % ST));
+        if (s.j == s.n - 1) umma_commit(BAR(B_RE));
+      };
+      cur.j = cur.n = 0;
+      bool have = advance(cur);
+      if (have) scores(cur);
+      if (have && ok) dprob(cur);
+      while (have && ok) {
+        nxt = cur;
+        const bool same_item = cur.j + 1 < cur.n;
+        bool more = same_item && advance(nxt);
+        const uint32_t par = (uint32_t)steps & 1u;
+        ++steps;
+        if (!wait_parity<false>(BAR(B_PF), par, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (DKV) {
+          add(tmem + A2_COL, tmem + S_COL, c2s + (cur.g % ST) * C::TILE, cur.j == 0);
+          umma_commit(BAR(B_2E + cur.g % ST));
+        }
+        if (more) scores(nxt);
+        if (!ok) break;
+        if (!wait_parity<false>(BAR(B_DSF), par, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        add(tmem + A1_COL, tmem + DP_COL, c1s + (cur.g % ST) * C::TILE, cur.j == 0);
+        umma_commit(BAR(B_1E + cur.g % ST));
+        if (!same_item) umma_commit(BAR(B_ACC));
+        if (!same_item) {
+          more = advance(nxt);  // the next item's rows may still be on their way
+          if (!ok) break;
+          if (more) scores(nxt);
+          if (!ok) break;
+        }
+        if (more) dprob(nxt);
+        cur = nxt;
+        have = more;
+      }
+      if (!ok) give_up(ERR_MMA, abort_flag, a.err_flag);
+      umma_commit(BAR(B_DRAIN));
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax: thread = half a row ----------------
+    const int half = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + S_COL + half * 64u, d_addr = tmem + lanes + DP_COL + half * 64u;
+    const int row = (warp & 3) * 32 + lane;
+    const float c = a.scale_log2;
+    const uint64_t c2 = f2_pack(c, c);
+    const float shift = F16 ? P_SHIFT : 0.f;
+    const float dsf = F16 ? ds_factor<T>(a) * exp2f(-P_SHIFT) : 1.f;  // what dS is held times, P's own factor off
+    const float out1 = a.scale / (F16 ? ds_factor<T>(a) : 1.f), out2 = F16 ? exp2f(-P_SHIFT) : 1.f;
+    bool ok = true;
+    int step = 0, nacc = 0, g = 0;
+    for (int i = 0; ok; ++i) {
+      if (!WAIT_WARP(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; break; }
+      const int r0 = items[i & 1].r0, head = items[i & 1].head, c00 = items[i & 1].c0, cols = items[i & 1].cols;
+      const int n = items[i & 1].n, done = items[i & 1].done;
+      mbar_arrive(BAR(B_ITEM_E + (i & 1)));
+      if (done) break;
+      const int tok = r0 + row;
+      Span sp{tok + 1, tok};
+      if (tok < a.T) sp = span_of(a, tok);
+      float row_lse = 0.f, row_d = 0.f;
+      if (!DKV) {
+        row_lse = shift - a.lse[(int64_t)head * a.Tp + tok];  // padded to whole tiles
+        row_d = -a.delta[(int64_t)head * a.Tp + tok];
+      }
+      int ct = 0;
+      for (int j = 0; j < n; ++j, ++g, ++step) {
+        const int col0 = c00 + ct * TM + half * 64;
+        ct = ct + 1 == cols ? 0 : ct + 1;
+        const float *vec = reinterpret_cast<const float *>(gen + (vecs - base) + (g % ST) * C::VEC) + half * 64;
+        if (!WAIT_WARP(BAR(B_SF), (uint32_t)step & 1u)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t r[2][32];
+        tmem_ld32x2u(s_addr, s_addr + 32, r);
+        if (!DKV) {
+          tc_fence_before();
+          mbar_arrive(BAR(B_PF));  // S may be overwritten
+        } else {
+          // the columns' lse and D came with C1: its barrier orders them (its phase is complete, S was formed from it)
+          if (!WAIT_WARP(BAR(B_1F + g % ST), (uint32_t)(g / ST) & 1u)) { ok = false; break; }
+        }
+        // columns of this half that the row sees: [lo, hi)
+        const int lo = (DKV ? tok : sp.start) - col0, hi = (DKV ? sp.end : tok + 1) - col0;
+        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 64);
+        float p[64];
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          float n0 = row_lse, n1 = row_lse, n2 = row_lse, n3 = row_lse;
+          if (DKV) {
+            const float4 l = *reinterpret_cast<const float4 *>(vec + e);
+            n0 = shift - l.x; n1 = shift - l.y; n2 = shift - l.z; n3 = shift - l.w;
+          }
+          float x0, x1, x2, x3;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1])), c2, f2_pack(n0, n1)), x0, x1);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e >> 5][(e & 31) + 2]), __uint_as_float(r[e >> 5][(e & 31) + 3])), c2, f2_pack(n2, n3)), x2, x3);
+          p[e] = exp2_approx(x0);
+          p[e + 1] = exp2_approx(x1);
+          p[e + 2] = exp2_approx(x2);
+          p[e + 3] = exp2_approx(x3);
+        }
+        if (cut) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e < lo || e >= hi) p[e] = 0.f;
+        }
+        if (DKV) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w[e] = pack2<T>(p[2 * e], p[2 * e + 1]);
+          tmem_st32(s_addr, w);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(BAR(B_PF));
+        }
+        if (!WAIT_WARP(BAR(B_DPF), (uint32_t)step & 1u)) { ok = false; break; }
+        tc_fence_after();
+        tmem_ld32x2u(d_addr, d_addr + 32, r);
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          float m0 = row_d, m1 = row_d, m2 = row_d, m3 = row_d;
+          if (DKV) {
+            const float4 d = *reinterpret_cast<const float4 *>(vec + TM + e);
+            m0 = -d.x; m1 = -d.y; m2 = -d.z; m3 = -d.w;
+          }
+          const uint64_t u = f2_mul(f2_pack(p[e], p[e + 1]),
+                                    f2_add(f2_pack(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1])), f2_pack(m0, m1)));
+          const uint64_t v = f2_mul(f2_pack(p[e + 2], p[e + 3]),
+                                    f2_add(f2_pack(__uint_as_float(r[e >> 5][(e & 31) + 2]), __uint_as_float(r[e >> 5][(e & 31) + 3])), f2_pack(m2, m3)));
+          float x0, x1, x2, x3;
+          f2_unpack(u, x0, x1);
+          f2_unpack(v, x2, x3);
+          if (F16) {
+            x0 *= dsf; x1 *= dsf; x2 *= dsf; x3 *= dsf;
+          }
+          if (cut) {  // P = 0 there, but dP or D may be a NaN of a token outside
+            if (e < lo || e >= hi) x0 = 0.f;
+            if (e + 1 < lo || e + 1 >= hi) x1 = 0.f;
+            if (e + 2 < lo || e + 2 >= hi) x2 = 0.f;
+            if (e + 3 < lo || e + 3 >= hi) x3 = 0.f;
+          }
+          w[e >> 1] = pack2<T>(x0, x1);
+          w[(e >> 1) + 1] = pack2<T>(x2, x3);
+        }
+        tmem_st32(d_addr, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(BAR(B_DSF));
+      }
+      if (!ok) break;
+      if (n > 0) {
+        if (!WAIT_WARP(BAR(B_ACC), (uint32_t)nacc & 1u)) { ok = false; break; }
+        ++nacc;
+        tc_fence_after();
+      }
+      // epilogue: this half's share of the row's columns, 16 at a time
+      const int64_t at = ((int64_t)tok * (DKV ? a.Hk : a.H) + head) * a.D;
+#pragma unroll
+      for (int which = 0; which < (DKV ? 2 : 1); ++which) {
+        T *dst = static_cast<T *>(DKV ? (which ? a.dv : a.dk) : a.dq) + at;
+        const uint32_t acc = tmem + lanes + (which ? A2_COL : A1_COL);
+        const float mul = which ? out2 : out1;
+#pragma unroll
+        for (int d = 0; d < DP; d += 32) {
+          const int dd = d + half * 16;
+          uint32_t o[16];
+          if (n > 0) {
+            tmem_ld16u(acc + dd, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0u;
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * mul, __uint_as_float(o[2 * e + 1]) * mul);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (tok < a.T && dd + h * 8 < a.D)
+              *reinterpret_cast<uint4 *>(dst + dd + h * 8) = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+    if (!ok && lane == 0) give_up(ERR_SOFTMAX, abort_flag, a.err_flag);
+  }
+
+  // ---------------- teardown ----------------
+  __syncthreads();
+  if (warp == W_MMA) {
+    wait_parity<false>(BAR(B_DRAIN), 0u, nullptr);
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+  if (*abort_flag) {
+    // a wait gave up: this block's share becomes NaN instead of partly written
+    const T bad = from_f<T>(__int_as_float(0x7fc00000));
+    for (int i = 0;; ++i) {
+      Item it;
+      if (!item_of<DKV>(a, sched, snake(i, blockIdx.x, gridDim.x), it)) break;
+      for (int e = tid; e < TM * a.D; e += NTHREADS) {
+        const int64_t tok = it.r0 + e / a.D;
+        if (tok >= a.T) continue;
+        const int64_t at = (tok * (DKV ? a.Hk : a.H) + it.head) * a.D + e % a.D;
+        if (DKV) {
+          static_cast<T *>(a.dk)[at] = bad;
+          static_cast<T *>(a.dv)[at] = bad;
+        } else {
+          static_cast<T *>(a.dq)[at] = bad;
+        }
+      }
+    }
+  }
+#undef WAIT_WARP
+#undef BAR
+}
+
+template <typename T, int DP, bool DKV>
+cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, const Map &c2, int *order, int sms,
+                cudaStream_t stream) {
+  using C = Cfg<DP>;
+  constexpr size_t smem = 2 * C::TILE + C::ST * (2 * C::TILE + C::VEC) + 1024;
+  static_assert(smem <= 232448 - 1024, "shared memory of a block");
+  auto kern = attn_bwd_tc_kernel<T, DP, DKV>;
+  static std::mutex mu;
+  static bool done[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 64 || !done[dev]) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return e;
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  Sched s;
+  s.tiles = (int)((a.T + TM - 1) / TM);
+  s.heads = DKV ? a.Hk : a.H;
+  if ((int64_t)s.tiles * s.heads > 0x7fffffff) return cudaErrorNotSupported;
+  s.items = s.tiles * s.heads;
+  s.order = nullptr;
+  if (s.items > sms) {  // with a block for every piece of work their order does not matter
+    e = launch_attn_order(a, DKV, order, stream);
+    if (e != cudaSuccess) return e;
+    s.order = order;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(s.items < sms ? s.items : sms), 1, 1);
+  cfg.blockDim = dim3(NTHREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  e = cudaLaunchKernelEx(&cfg, kern, r1, r2, c1, c2, a, s);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace attn
+
+cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream) {
+  attn::Map q, k, v, d;
+  const int64_t ot = (int64_t)a.H * a.D;
+  if (!attn::make_map(q, a.q, a.dtype, a.T, a.H, a.D, a.qt, a.qh) || !attn::make_map(k, a.k, a.dtype, a.T, a.Hk, a.D, a.kt, a.kh) ||
+      !attn::make_map(v, a.v, a.dtype, a.T, a.Hk, a.D, a.vt, a.vh) || !attn::make_map(d, a.dout, a.dtype, a.T, a.H, a.D, ot, a.D))
+    return cudaErrorNotSupported;
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  auto both = [&](auto tag, auto dim) -> cudaError_t {
+    using T = decltype(tag);
+    constexpr int DP = decltype(dim)::value;
+    const cudaError_t e = attn::run<T, DP, true>(a, k, v, q, d, order_k, sms, stream);
+    return e != cudaSuccess ? e : attn::run<T, DP, false>(a, q, d, k, v, order_q, sms, stream);
+  };
+  auto go = [&](auto tag) -> cudaError_t {
+    if (a.D <= 32) return both(tag, IC<32>{});
+    if (a.D <= 64) return both(tag, IC<64>{});
+    if (a.D <= 96) return both(tag, IC<96>{});
+    return both(tag, IC<128>{});
+  };
+  return a.dtype == MHC_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+}
+
+int read_atb_error(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_atb_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_atb_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace mhc

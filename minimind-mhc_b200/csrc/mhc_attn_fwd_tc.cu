@@ -438,7 +438,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         tc_fence_after();
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (tok < a.T) a.lse[(int64_t)head * a.T + tok] = sum == 0.f ? INFINITY : ref + log2f(sum);
+      if (tok < a.T) a.lse[(int64_t)head * a.Tp + tok] = sum == 0.f ? INFINITY : ref + log2f(sum);
       const int64_t at = ((int64_t)tok * a.H + head) * a.D;
       T *out = static_cast<T *>(a.o) + at, *lo = a.o_lo ? static_cast<T *>(a.o_lo) + at : nullptr;
 #pragma unroll
@@ -619,11 +619,16 @@ cudaError_t launch_attn_order(const attn::Args &a, int keys, int *order, cudaStr
   return cudaGetLastError();
 }
 
-bool attn_tc_eligible(const attn::Args &a, bool backward) {
+bool attn_tc_eligible(const attn::Args &a) {
   if (a.dtype != MHC_BF16 && a.dtype != MHC_F16) return false;
   if (((uintptr_t)a.o | (uintptr_t)a.o_lo) & 15) return false;
   return attn::map_eligible(a.q, a.D, a.H, a.T, a.qt, a.qh) && attn::map_eligible(a.k, a.D, a.Hk, a.T, a.kt, a.kh) &&
-         attn::map_eligible(a.v, a.D, a.Hk, a.T, a.vt, a.vh) && !backward;
+         attn::map_eligible(a.v, a.D, a.Hk, a.T, a.vt, a.vh);
+}
+
+bool attn_tc_bwd_eligible(const attn::Args &a) {
+  if (((uintptr_t)a.dout | (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.lse) & 15) return false;
+  return attn_tc_eligible(a);
 }
 
 cudaError_t launch_attn_fwd_tc(const attn::Args &a, int *order, cudaStream_t stream) {

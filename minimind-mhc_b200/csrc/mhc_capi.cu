@@ -116,7 +116,7 @@ int mhc_last_path(void) { return g_last_path.load(); }
 
 int mhc_device_error(int clear) {
   if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  const int words[6] = {read_atf_error(clear != 0), read_sr_error(clear != 0), read_tc_error(clear != 0), read_tcb_error(clear != 0),
+  const int words[7] = {read_atb_error(clear != 0), read_atf_error(clear != 0), read_sr_error(clear != 0), read_tc_error(clear != 0), read_tcb_error(clear != 0),
                         read_ch_error(clear != 0), read_selftest_error(clear != 0)};
   for (int w : words)
     if (w < 0) return -1;

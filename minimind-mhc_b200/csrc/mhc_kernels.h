@@ -125,6 +125,7 @@ int read_tcb_error(bool clear);
 int *host_error_flag();
 int read_selftest_error(bool clear);
 int read_atf_error(bool clear);  // attention forward
+int read_atb_error(bool clear);  // attention backward
 bool generic_forced();           // MHC_PATH_GENERIC is set
 
 // ---- stand-alone pieces -----------------------------------------------------

@@ -55,6 +55,7 @@ _PROTOS = {
                           _P, _P, _SZ, _P]),
     "mhc_stream_expand_fwd": (_I, [_P, _P, _I, _I64, _I, _I, _P]),
     "mhc_stream_expand_bwd": (_I, [_P, _P, _I, _I64, _I, _I, _P]),
+    "mhc_attn_lse_pitch": (_I64, [_I64]),
     "mhc_attn_fwd_workspace": (_SZ, [_I64]),
     "mhc_attn_fwd": (_I, [_P, _P, _P, _I, _I64, _I, _I, _I, _P, _P, _I, _I64, _F, _P, _P, _P, _P, _SZ, _P]),
     "mhc_attn_bwd_workspace": (_SZ, [_I64, _I]),
@@ -169,7 +170,9 @@ ERROR_ROLES = {1: "forward TMA producer", 2: "forward MMA issuer", 3: "forward r
                34: "merge + coefficient coefficient warp", 35: "merge + coefficient pre-aggregate warps",
                36: "merge + coefficient Sinkhorn warp", 37: "merge + coefficient merge warps",
                41: "attention forward TMA warp", 42: "attention forward MMA issuer",
-               43: "attention forward softmax warps", 99: "bounded-wait self-test"}
+               43: "attention forward softmax warps",
+               51: "attention backward TMA warp", 52: "attention backward MMA issuer",
+               53: "attention backward softmax warps", 99: "bounded-wait self-test"}
 
 _flag_tensor = None   # pinned int32 host tensor registered with the library
 _flag_word = None     # ctypes view of its first element

@@ -37,7 +37,7 @@ class _PackedAttentionFn(torch.autograd.Function):
             out = torch.empty(t, h, d, dtype=q.dtype, device=dev)
             # the backward's row sums use out before its rounding to 16 bits
             out_lo = torch.empty_like(out) if any(ctx.needs_input_grad) and q.dtype != torch.float32 else None
-            lse = torch.empty(h, t, dtype=torch.float32, device=dev)
+            lse = torch.empty(h, nat.lib().mhc_attn_lse_pitch(t), dtype=torch.float32, device=dev)
             strides = (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
                                            v.stride(1))
             batch = 0 if cu is None else cu.numel() - 1
