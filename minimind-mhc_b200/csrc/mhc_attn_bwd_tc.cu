@@ -19,8 +19,12 @@
 // operands serve S and dP as they are (K-major) and the gradients as they lie
 // (their rows are the summed index: MN-major).
 //
-// Per tile the tensor core is given S(j+1) behind dV(j), and dP(j+1) behind dK(j),
-// so it works while the 8 warps of the softmax are at the other half of the step.
+// A tile's columns are two halves of 64, each with its own S and dP in TMEM and its
+// own four warps.  The tensor core is given S(j+1) of a half behind its dV(j), and
+// dP(j+1) behind dK(j), so a half's scores are there when its warps come for them,
+// and the two halves fall into turns by themselves.  (Both halves as one 128-column
+// step made the warps wait for the products: 1.55 against MEASURED_HERE ms at 16384
+// tokens, D = 96.)
 //
 // fp16 has no room for small dS or P: P is held times 2^10, and dS times a power of
 // two from the largest |dO| and |V| of the call that no dS can overflow
@@ -45,8 +49,9 @@ namespace attn {
 
 namespace {
 
-constexpr int NTHREADS = 320;
-constexpr int W_TMA = 8, W_MMA = 9;
+constexpr int NSOFT = 16;             // softmax warps: four to each quarter of the rows
+constexpr int W_TMA = NSOFT, W_MMA = NSOFT + 1;
+constexpr int NTHREADS = (NSOFT + 2) * 32;
 constexpr int TMEM_COLS = 512;
 constexpr uint32_t S_COL = 0, DP_COL = 128, A1_COL = 256, A2_COL = 384;
 constexpr float P_SHIFT = 10.f;  // fp16: P times 2^10
@@ -69,7 +74,7 @@ struct Cfg {
 };
 
 constexpr int B_ITEM_F = 0, B_ITEM_E = 2, B_RF = 4, B_RE = 5, B_LAND = 6, B_SF = 7, B_PF = 8, B_DPF = 9, B_DSF = 10,
-              B_ACC = 11, B_DRAIN = 12, B_1F = 13;
+              B_ACC_F = 11, B_DRAIN = 12, B_1F = 13;
 // then ST each: 1F, 1E, 2F, 2E
 
 struct Sched {
@@ -144,23 +149,23 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
 #define WAIT_WARP(bar, par) (__all_sync(0xffffffffu, wait_parity<false>((bar), (par), abort_flag)))
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int G = a.H / a.Hk;
 
   if (tid == 0) {
     abort_word = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(B_ITEM_F + i), 1);
-      mbar_init(BAR(B_ITEM_E + i), 257);  // the softmax threads and the MMA thread have read it
+      mbar_init(BAR(B_ITEM_E + i), NSOFT + 1);  // the softmax warps and the MMA warp have read it
     }
     mbar_init(BAR(B_RF), 1);
     mbar_init(BAR(B_RE), 1);
     mbar_init(BAR(B_LAND), 1);
     mbar_init(BAR(B_SF), 1);
-    mbar_init(BAR(B_PF), 256);
+    mbar_init(BAR(B_PF), NSOFT);
     mbar_init(BAR(B_DPF), 1);
-    mbar_init(BAR(B_DSF), 256);
-    mbar_init(BAR(B_ACC), 1);
+    mbar_init(BAR(B_DSF), NSOFT);
+    mbar_init(BAR(B_ACC_F), 1);
     mbar_init(BAR(B_DRAIN), 1);
     for (int i = 0; i < 4 * ST; ++i) mbar_init(BAR(B_1F + i), 1);
     fence_mbar_init_cluster();
@@ -172,7 +177,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
   grid_dep_launch();
   grid_dep_wait();
 
@@ -180,7 +185,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     // ---------------- TMA: whole warp, lane 0 issues ----------------
     const Span range = packed_range(a);
     bool ok = true;
-    int g = 0, lands = 0, rn = 0;
+    int g = 0, lands = 0, rn = 0;  // g: column tiles so far
     // a column tile: rows outside of the sequences are zeroed, since as B operands of the gradients they
     // meet P = dS = 0, which a NaN would survive
     auto column = [&](uint32_t dst, const Map &map, int head, int row, int full, bool vec, int h) {
@@ -199,7 +204,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       if (clean) {
         if (!WAIT_WARP(BAR(B_LAND), (uint32_t)lands & 1u)) ok = false;
         ++lands;
-        zero_outside(gen + (dst - base), NB, row, range, lane);
+        zero_outside(gen + (dst - base), NB, BLK, TM, row, range, lane);
         if (lane == 0) mbar_arrive(BAR(full));
       }
     };
@@ -240,10 +245,14 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     }
     if (rn > 0) wait_parity<false>(BAR(B_RF), (uint32_t)(rn - 1) & 1u, nullptr);
   } else if (warp == W_MMA) {
-    // ---------------- MMA issue: one thread ----------------
-    if (lane == 0) {
+    // ---------------- MMA issue: the warp runs it, one lane issues ----------------
+    {
       constexpr uint32_t id_s = idesc_of<T>(128, 0), id_g = idesc_of<T>(DP, 1);
       bool ok = true;
+      auto wait_warp = [&](uint32_t bar, uint32_t par) { return __all_sync(0xffffffffu, wait_parity<false>(bar, par, abort_flag)); };
+      auto commit = [&](uint32_t bar) {
+        if (elect_one()) umma_commit(bar);
+      };
       int i = 0, rn = 0, gk = 0, steps = 0;
       struct Step {
         int j, n, g;
@@ -253,16 +262,16 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           ++s.j;
         } else {
           while (true) {
-            if (!wait_parity<false>(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u, abort_flag)) { ok = false; return false; }
-            const bool done = items[i & 1].done;
+            if (!wait_warp(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; return false; }
+            const bool done = uniform(items[i & 1].done);
             s.j = 0;
-            s.n = items[i & 1].n;
-            mbar_arrive(BAR(B_ITEM_E + (i & 1)));
+            s.n = uniform(items[i & 1].n);
+            if (elect_one()) mbar_arrive(BAR(B_ITEM_E + (i & 1)));
             ++i;
             if (done) return false;
             if (s.n > 0) break;
           }
-          if (!wait_parity<false>(BAR(B_RF), (uint32_t)rn & 1u, abort_flag)) { ok = false; return false; }
+          if (!wait_warp(BAR(B_RF), (uint32_t)rn & 1u)) { ok = false; return false; }
           ++rn;
         }
         s.g = gk++;
@@ -270,55 +279,60 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       };
       // [128 x 128] = rows (K-major) times columns^T (K-major)
       auto cross = [&](uint32_t d, uint32_t r, uint32_t c) {
+        const uint64_t rd = umma_desc_sw128(r), cd = umma_desc_sw128(c);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          umma_bf16(d, umma_desc_sw128(r + (kk >> 2) * BLK + (kk & 3) * 32),
-                    umma_desc_sw128(c + (kk >> 2) * BLK + (kk & 3) * 32), id_s, kk > 0);
+          for (int kk = 0; kk < DP / 16; ++kk) umma_bf16(d, rd + k_step(kk, BLK), cd + k_step(kk, BLK), id_s, kk > 0);
+        }
       };
-      // accumulator += W C: W [128 x 128] 16-bit in TMEM, its second 64 columns 64 TMEM columns on; C MN-major
+      // accumulator += W C: W [128 x 128] in TMEM, 32 of its columns in 16 of each 32; C MN-major
       auto add = [&](uint32_t d, uint32_t w, uint32_t c, bool begin) {
+        const uint64_t cd = umma_desc(c, BLK, 1024, 2);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < TM / 16; ++kk)
-          umma_f16_ts(d, w + (kk >> 2) * 64u + (kk & 3) * 8u, umma_desc(c + kk * 2048, BLK, 1024, 2), id_g, !begin || kk > 0);
+          for (int kk = 0; kk < TM / 16; ++kk)
+            umma_f16_ts(d, w + (kk >> 1) * 32u + (kk & 1) * 8u, cd + mn_step(kk), id_g, !begin || kk > 0);
+        }
       };
       auto scores = [&](const Step &s) {
-        if (!wait_parity<false>(BAR(B_1F + s.g % ST), (uint32_t)(s.g / ST) & 1u, abort_flag)) { ok = false; return; }
+        if (!wait_warp(BAR(B_1F + s.g % ST), (uint32_t)(s.g / ST) & 1u)) { ok = false; return; }
         tc_fence_after();
         cross(tmem + S_COL, rs, c1s + (s.g % ST) * C::TILE);
-        umma_commit(BAR(B_SF));
+        commit(BAR(B_SF));
       };
       auto dprob = [&](const Step &s) {
-        if (!wait_parity<false>(BAR(B_2F + s.g % ST), (uint32_t)(s.g / ST) & 1u, abort_flag)) { ok = false; return; }
+        if (!wait_warp(BAR(B_2F + s.g % ST), (uint32_t)(s.g / ST) & 1u)) { ok = false; return; }
         tc_fence_after();
         cross(tmem + DP_COL, rs + C::TILE, c2s + (s.g % ST) * C::TILE);
-        umma_commit(BAR(B_DPF));
-        if (!DKV) umma_commit(BAR(B_2E + s.g % ST));
-        if (s.j == s.n - 1) umma_commit(BAR(B_RE));
+        commit(BAR(B_DPF));
+        if (!DKV) commit(BAR(B_2E + s.g % ST));
+        if (s.j == s.n - 1) commit(BAR(B_RE));
       };
       cur.j = cur.n = 0;
       bool have = advance(cur);
-      if (have) scores(cur);
+      if (have && ok) scores(cur);
       if (have && ok) dprob(cur);
       while (have && ok) {
         nxt = cur;
         const bool same_item = cur.j + 1 < cur.n;
         bool more = same_item && advance(nxt);
+        if (!ok) break;
         const uint32_t par = (uint32_t)steps & 1u;
         ++steps;
-        if (!wait_parity<false>(BAR(B_PF), par, abort_flag)) { ok = false; break; }
+        if (!wait_warp(BAR(B_PF), par)) { ok = false; break; }
         tc_fence_after();
         if (DKV) {
           add(tmem + A2_COL, tmem + S_COL, c2s + (cur.g % ST) * C::TILE, cur.j == 0);
-          umma_commit(BAR(B_2E + cur.g % ST));
+          commit(BAR(B_2E + cur.g % ST));
         }
         if (more) scores(nxt);
         if (!ok) break;
-        if (!wait_parity<false>(BAR(B_DSF), par, abort_flag)) { ok = false; break; }
+        if (!wait_warp(BAR(B_DSF), par)) { ok = false; break; }
         tc_fence_after();
         add(tmem + A1_COL, tmem + DP_COL, c1s + (cur.g % ST) * C::TILE, cur.j == 0);
-        umma_commit(BAR(B_1E + cur.g % ST));
-        if (!same_item) umma_commit(BAR(B_ACC));
+        commit(BAR(B_1E + cur.g % ST));
         if (!same_item) {
+          commit(BAR(B_ACC_F));
           more = advance(nxt);  // the next item's rows may still be on their way
           if (!ok) break;
           if (more) scores(nxt);
@@ -328,15 +342,15 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         cur = nxt;
         have = more;
       }
-      if (!ok) give_up(ERR_MMA, abort_flag, a.err_flag);
-      umma_commit(BAR(B_DRAIN));
+      if (!ok && lane == 0) give_up(ERR_MMA, abort_flag, a.err_flag);
+      commit(BAR(B_DRAIN));
     }
     __syncwarp();
   } else {
-    // ---------------- softmax: thread = half a row ----------------
-    const int half = warp >> 2;
+    // ---------------- softmax: thread = a quarter of a row ----------------
+    const int part = warp >> 2;  // its columns: 32 from 32 part
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + S_COL + half * 64u, d_addr = tmem + lanes + DP_COL + half * 64u;
+    const uint32_t s_addr = tmem + lanes + S_COL + part * 32u, d_addr = tmem + lanes + DP_COL + part * 32u;
     const int row = (warp & 3) * 32 + lane;
     const float c = a.scale_log2;
     const uint64_t c2 = f2_pack(c, c);
@@ -344,12 +358,18 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     const float dsf = F16 ? ds_factor<T>(a) * exp2f(-P_SHIFT) : 1.f;  // what dS is held times, P's own factor off
     const float out1 = a.scale / (F16 ? ds_factor<T>(a) : 1.f), out2 = F16 ? exp2f(-P_SHIFT) : 1.f;
     bool ok = true;
-    int step = 0, nacc = 0, g = 0;
+    int step = 0, nacc = 0;
+    auto arrive = [&](int bar) {  // the warp's TMEM accesses are complete
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(bar));
+    };
     for (int i = 0; ok; ++i) {
       if (!WAIT_WARP(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; break; }
       const int r0 = items[i & 1].r0, head = items[i & 1].head, c00 = items[i & 1].c0, cols = items[i & 1].cols;
       const int n = items[i & 1].n, done = items[i & 1].done;
-      mbar_arrive(BAR(B_ITEM_E + (i & 1)));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(B_ITEM_E + (i & 1)));
       if (done) break;
       const int tok = r0 + row;
       Span sp{tok + 1, tok};
@@ -360,35 +380,34 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         row_d = -a.delta[(int64_t)head * a.Tp + tok];
       }
       int ct = 0;
-      for (int j = 0; j < n; ++j, ++g, ++step) {
-        const int col0 = c00 + ct * TM + half * 64;
+      for (int j = 0; j < n; ++j, ++step) {
+        const int col0 = c00 + ct * TM + part * 32;
         ct = ct + 1 == cols ? 0 : ct + 1;
-        const float *vec = reinterpret_cast<const float *>(gen + (vecs - base) + (g % ST) * C::VEC) + half * 64;
+        const float *vec = reinterpret_cast<const float *>(gen + (vecs - base) + (step % ST) * C::VEC) + part * 32;
         if (!WAIT_WARP(BAR(B_SF), (uint32_t)step & 1u)) { ok = false; break; }
         tc_fence_after();
-        uint32_t r[2][32];
-        tmem_ld32x2u(s_addr, s_addr + 32, r);
+        uint32_t r[32];
+        tmem_ld32u(s_addr, r);
         if (!DKV) {
-          tc_fence_before();
-          mbar_arrive(BAR(B_PF));  // S may be overwritten
+          arrive(B_PF);  // S may be overwritten
         } else {
           // the columns' lse and D came with C1: its barrier orders them (its phase is complete, S was formed from it)
-          if (!WAIT_WARP(BAR(B_1F + g % ST), (uint32_t)(g / ST) & 1u)) { ok = false; break; }
+          if (!WAIT_WARP(BAR(B_1F + step % ST), (uint32_t)(step / ST) & 1u)) { ok = false; break; }
         }
-        // columns of this half that the row sees: [lo, hi)
+        // columns of this part that the row sees: [lo, hi)
         const int lo = (DKV ? tok : sp.start) - col0, hi = (DKV ? sp.end : tok + 1) - col0;
-        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 64);
-        float p[64];
+        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 32);
+        float p[32];
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
+        for (int e = 0; e < 32; e += 4) {
           float n0 = row_lse, n1 = row_lse, n2 = row_lse, n3 = row_lse;
           if (DKV) {
             const float4 l = *reinterpret_cast<const float4 *>(vec + e);
             n0 = shift - l.x; n1 = shift - l.y; n2 = shift - l.z; n3 = shift - l.w;
           }
           float x0, x1, x2, x3;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1])), c2, f2_pack(n0, n1)), x0, x1);
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e >> 5][(e & 31) + 2]), __uint_as_float(r[e >> 5][(e & 31) + 3])), c2, f2_pack(n2, n3)), x2, x3);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, f2_pack(n0, n1)), x0, x1);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2, f2_pack(n2, n3)), x2, x3);
           p[e] = exp2_approx(x0);
           p[e + 1] = exp2_approx(x1);
           p[e + 2] = exp2_approx(x2);
@@ -396,33 +415,32 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         }
         if (cut) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < 32; ++e)
             if (e < lo || e >= hi) p[e] = 0.f;
         }
         if (DKV) {
-          uint32_t w[32];
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = pack2<T>(p[2 * e], p[2 * e + 1]);
-          tmem_st32(s_addr, w);
+          for (int e = 0; e < 16; ++e) w[e] = pack2<T>(p[2 * e], p[2 * e + 1]);
+          tmem_st16(s_addr, w);
           tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(BAR(B_PF));
+          arrive(B_PF);
         }
         if (!WAIT_WARP(BAR(B_DPF), (uint32_t)step & 1u)) { ok = false; break; }
         tc_fence_after();
-        tmem_ld32x2u(d_addr, d_addr + 32, r);
-        uint32_t w[32];
+        tmem_ld32u(d_addr, r);
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
+        for (int e = 0; e < 32; e += 4) {
           float m0 = row_d, m1 = row_d, m2 = row_d, m3 = row_d;
           if (DKV) {
             const float4 d = *reinterpret_cast<const float4 *>(vec + TM + e);
             m0 = -d.x; m1 = -d.y; m2 = -d.z; m3 = -d.w;
           }
           const uint64_t u = f2_mul(f2_pack(p[e], p[e + 1]),
-                                    f2_add(f2_pack(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1])), f2_pack(m0, m1)));
+                                    f2_add(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), f2_pack(m0, m1)));
           const uint64_t v = f2_mul(f2_pack(p[e + 2], p[e + 3]),
-                                    f2_add(f2_pack(__uint_as_float(r[e >> 5][(e & 31) + 2]), __uint_as_float(r[e >> 5][(e & 31) + 3])), f2_pack(m2, m3)));
+                                    f2_add(f2_pack(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), f2_pack(m2, m3)));
           float x0, x1, x2, x3;
           f2_unpack(u, x0, x1);
           f2_unpack(v, x2, x3);
@@ -438,42 +456,39 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           w[e >> 1] = pack2<T>(x0, x1);
           w[(e >> 1) + 1] = pack2<T>(x2, x3);
         }
-        tmem_st32(d_addr, w);
+        tmem_st16(d_addr, w);
         tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(BAR(B_DSF));
+        arrive(B_DSF);
       }
       if (!ok) break;
       if (n > 0) {
-        if (!WAIT_WARP(BAR(B_ACC), (uint32_t)nacc & 1u)) { ok = false; break; }
+        if (!WAIT_WARP(BAR(B_ACC_F), (uint32_t)nacc & 1u)) { ok = false; break; }
         ++nacc;
         tc_fence_after();
       }
-      // epilogue: this half's share of the row's columns, 16 at a time
+      // epilogue: every fourth 16 columns of the row's results
       const int64_t at = ((int64_t)tok * (DKV ? a.Hk : a.H) + head) * a.D;
+      constexpr int PIECES = DP / 16;
+#pragma unroll 1
+      for (int q = part; q < (DKV ? 2 : 1) * PIECES; q += 4) {
+        const bool second = DKV && q >= PIECES;
+        const int d = (second ? q - PIECES : q) * 16;
+        T *dst = static_cast<T *>(DKV ? (second ? a.dv : a.dk) : a.dq) + at;
+        const float mul = second ? out2 : out1;
+        uint32_t o[16];
+        if (n > 0) {
+          tmem_ld16u(tmem + lanes + (second ? A2_COL : A1_COL) + d, o);
+        } else {
 #pragma unroll
-      for (int which = 0; which < (DKV ? 2 : 1); ++which) {
-        T *dst = static_cast<T *>(DKV ? (which ? a.dv : a.dk) : a.dq) + at;
-        const uint32_t acc = tmem + lanes + (which ? A2_COL : A1_COL);
-        const float mul = which ? out2 : out1;
-#pragma unroll
-        for (int d = 0; d < DP; d += 32) {
-          const int dd = d + half * 16;
-          uint32_t o[16];
-          if (n > 0) {
-            tmem_ld16u(acc + dd, o);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0u;
-          }
-          uint32_t w[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * mul, __uint_as_float(o[2 * e + 1]) * mul);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (tok < a.T && dd + h * 8 < a.D)
-              *reinterpret_cast<uint4 *>(dst + dd + h * 8) = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
+          for (int e = 0; e < 16; ++e) o[e] = 0u;
         }
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * mul, __uint_as_float(o[2 * e + 1]) * mul);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (tok < a.T && d + h * 8 < a.D)
+            *reinterpret_cast<uint4 *>(dst + d + h * 8) = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
       }
       tc_fence_before();
     }

@@ -142,7 +142,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
   volatile int *abort_flag = &abort_word;
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
     abort_word = 0;
@@ -172,7 +172,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
   grid_dep_launch();
   grid_dep_wait();
 
@@ -219,7 +219,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         if (clean) {
           if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_LAND), (uint32_t)lands & 1u, abort_flag))) ok = false;
           ++lands;
-          zero_outside(gen + (vs - base) + s * C::TILE, NB, row, range, lane);
+          zero_outside(gen + (vs - base) + s * C::TILE, NB, BLK, TM, row, range, lane);
           if (lane == 0) mbar_arrive(BAR(B_VF + s));
         }
       }
@@ -232,10 +232,14 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
     }
     if (qn > 0) wait_parity<false>(BAR(B_QF), (uint32_t)(qn - 1) & 1u, nullptr);
   } else if (warp == W_MMA) {
-    // ---------------- MMA issue: one thread ----------------
-    if (lane == 0) {
+    // ---------------- MMA issue: the warp runs it, one lane issues ----------------
+    {
       constexpr uint32_t id_s = idesc_of<T>(128, 0), id_o = idesc_of<T>(DP, 1);
       bool ok = true;
+      auto wait_warp = [&](uint32_t bar, uint32_t par) { return __all_sync(0xffffffffu, wait_parity<false>(bar, par, abort_flag)); };
+      auto commit = [&](uint32_t bar) {
+        if (elect_one()) umma_commit(bar);
+      };
       int i = 0, qn = 0, gk = 0, pf[2] = {0, 0};
       struct Step {
         int j, n, first[2], last[2], g;
@@ -246,21 +250,22 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
           ++s.j;
         } else {
           while (true) {
-            if (!wait_parity<false>(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u, abort_flag)) { ok = false; return false; }
+            if (!wait_warp(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; return false; }
             const Item &it = items[i & 1];
-            const bool done = it.done;
+            const bool done = uniform(it.done);
             s.j = 0;
-            s.n = it.n;
+            s.n = uniform(it.n);
+#pragma unroll
             for (int t = 0; t < 2; ++t) {
-              s.first[t] = it.first[t];
-              s.last[t] = it.last[t];
+              s.first[t] = uniform(it.first[t]);
+              s.last[t] = uniform(it.last[t]);
             }
-            mbar_arrive(BAR(B_ITEM_E + (i & 1)));
+            if (elect_one()) mbar_arrive(BAR(B_ITEM_E + (i & 1)));
             ++i;
             if (done) return false;
             if (s.n > 0) break;
           }
-          if (!wait_parity<false>(BAR(B_QF), (uint32_t)qn & 1u, abort_flag)) { ok = false; return false; }
+          if (!wait_warp(BAR(B_QF), (uint32_t)qn & 1u)) { ok = false; return false; }
           ++qn;
         }
         s.g = gk++;
@@ -268,19 +273,20 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       };
       auto scores = [&](const Step &s, int t) {
         if (s.j < s.first[t] || s.j >= s.last[t]) return;
-        const uint32_t q = qs + t * C::TILE, k = ks + (s.g % ST) * C::TILE;
+        const uint64_t q = umma_desc_sw128(qs + t * C::TILE), k = umma_desc_sw128(ks + (s.g % ST) * C::TILE);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          umma_bf16(tmem + S_COL + t * 128u, umma_desc_sw128(q + (kk >> 2) * BLK + (kk & 3) * 32),
-                    umma_desc_sw128(k + (kk >> 2) * BLK + (kk & 3) * 32), id_s, kk > 0);
-        umma_commit(BAR(B_SF + t));
+          for (int kk = 0; kk < DP / 16; ++kk)
+            umma_bf16(tmem + S_COL + t * 128u, q + k_step(kk, BLK), k + k_step(kk, BLK), id_s, kk > 0);
+        }
+        commit(BAR(B_SF + t));
       };
       auto after_scores = [&](const Step &s) {
-        umma_commit(BAR(B_KE + s.g % ST));
-        if (s.j == s.n - 1) umma_commit(BAR(B_QE));
+        commit(BAR(B_KE + s.g % ST));
+        if (s.j == s.n - 1) commit(BAR(B_QE));
       };
       auto wait_k = [&](const Step &s) {
-        if (!wait_parity<false>(BAR(B_KF + s.g % ST), (uint32_t)(s.g / ST) & 1u, abort_flag)) ok = false;
+        if (!wait_warp(BAR(B_KF + s.g % ST), (uint32_t)(s.g / ST) & 1u)) ok = false;
         tc_fence_after();
       };
       cur.j = cur.n = 0;
@@ -295,15 +301,17 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       }
       auto product = [&](const Step &s, int t) {
         if (s.j < s.first[t] || s.j >= s.last[t]) return;
-        if (!wait_parity<false>(BAR(B_PF + t), (uint32_t)pf[t] & 1u, abort_flag)) { ok = false; return; }
+        if (!wait_warp(BAR(B_PF + t), (uint32_t)pf[t] & 1u)) { ok = false; return; }
         ++pf[t];
         tc_fence_after();
-        const uint32_t v = vs + (s.g % ST) * C::TILE;
+        const uint64_t v = umma_desc(vs + (s.g % ST) * C::TILE, BLK, 1024, 2);
+        const bool more = s.j > s.first[t];
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < TM / 16; ++kk)
-          umma_f16_ts(tmem + O_COL + t * 128u, tmem + S_COL + t * 128u + kk * 8u, umma_desc(v + kk * 2048, BLK, 1024, 2),
-                      id_o, s.j > s.first[t] || kk > 0);
-        umma_commit(BAR(B_OF + t));
+          for (int kk = 0; kk < TM / 16; ++kk)
+            umma_f16_ts(tmem + O_COL + t * 128u, tmem + S_COL + t * 128u + kk * 8u, v + mn_step(kk), id_o, more || kk > 0);
+        }
+        commit(BAR(B_OF + t));
       };
       // tile 0's product, its next scores, then the same for tile 1: each tile's softmax runs beside the other's
       // products.  S of the next step may follow P V of this one at once: the tensor core runs them in order.
@@ -311,7 +319,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         nxt = cur;
         const bool same_item = cur.j + 1 < cur.n;
         bool more = same_item && advance(nxt);
-        if (!wait_parity<false>(BAR(B_VF + cur.g % ST), (uint32_t)(cur.g / ST) & 1u, abort_flag)) { ok = false; break; }
+        if (!wait_warp(BAR(B_VF + cur.g % ST), (uint32_t)(cur.g / ST) & 1u)) { ok = false; break; }
         if (more) wait_k(nxt);
         if (!ok) break;
         product(cur, 0);
@@ -319,7 +327,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         if (more) scores(nxt, 0);
         product(cur, 1);
         if (!ok) break;
-        umma_commit(BAR(B_VE + cur.g % ST));
+        commit(BAR(B_VE + cur.g % ST));
         if (!same_item) {  // the next item's queries may still be on their way
           more = advance(nxt);
           if (!ok) break;
@@ -334,8 +342,8 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         cur = nxt;
         have = more;
       }
-      if (!ok) give_up(ERR_MMA, abort_flag, a.err_flag);
-      umma_commit(BAR(B_DRAIN));
+      if (!ok && lane == 0) give_up(ERR_MMA, abort_flag, a.err_flag);
+      commit(BAR(B_DRAIN));
     }
     __syncwarp();
   } else {
@@ -602,7 +610,7 @@ bool make_map(Map &map, const void *p, int dtype, int64_t T, int heads, int D, i
   const bool f = map.token_first != 0;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)(f ? T : heads), (cuuint64_t)(f ? heads : T)};
   const cuuint64_t strides[2] = {(cuuint64_t)(f ? ts : hs) * 2, (cuuint64_t)(f ? hs : ts) * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(f ? TM : 1), (cuuint32_t)(f ? 1 : TM)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(f ? 64 : 1), (cuuint32_t)(f ? 1 : 64)};
   const cuuint32_t estr[3] = {1, 1, 1};
   return enc(&map.m, dtype == MHC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
              const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -20,6 +20,7 @@ using namespace sm100;
 
 constexpr int TM = 128;               // rows of a tile, queries or keys
 constexpr uint32_t BLK = TM * 128;    // 128 rows x 64 values of 16 bits, 128-byte swizzle
+constexpr uint32_t HALF = BLK / 2;    // 64 rows of them
 
 // blocks of 64 columns that a head of D <= DP values takes
 __host__ __device__ constexpr int nblk(int DP) { return (DP + 63) / 64; }
@@ -32,17 +33,34 @@ __host__ __device__ constexpr uint32_t idesc_of(int N, int b_mn) {
          ((uint32_t)(TM >> 4) << 24);
 }
 
-// A tensor map of (T, heads, D) and whether its second axis is the token (heads farther apart than tokens).
+// What a descriptor's start address (16-byte units) moves by for the kk-th 16 values
+// of the summed index: along a row of a K-major tile, or 16 rows of an MN-major one.
+// `block`: from 64 columns to the next 64.
+__host__ __device__ constexpr uint64_t k_step(int kk, uint32_t block) { return (uint64_t)((kk >> 2) * (int)block + (kk & 3) * 32) >> 4; }
+__host__ __device__ constexpr uint64_t mn_step(int kk) { return (uint64_t)(kk * 2048) >> 4; }
+
+// A tensor map of (T, heads, D) in boxes of 64 rows x 64 columns, and whether its
+// second axis is the token (heads farther apart than tokens).
 struct Map {
   CUtensorMap m;
   int token_first;
 };
+__device__ __forceinline__ void load_box(uint32_t dst, const Map &map, int col, int head, int row, uint32_t bar) {
+  tma_load_3d(dst, &map.m, col, map.token_first ? row : head, map.token_first ? head : row, bar);
+}
+// 64 rows, blocks of 64 columns HALF bytes apart
+__device__ __forceinline__ void load_half(uint32_t dst, const Map &map, int nb, int head, int row, uint32_t bar) {
+  for (int b = 0; b < nb; ++b) load_box(dst + b * HALF, map, b * 64, head, row, bar);
+}
+// 128 rows, blocks of 64 columns BLK bytes apart
 __device__ __forceinline__ void load_rows(uint32_t dst, const Map &map, int nb, int head, int row, uint32_t bar) {
-  for (int b = 0; b < nb; ++b)
-    tma_load_3d(dst + b * BLK, &map.m, b * 64, map.token_first ? row : head, map.token_first ? head : row, bar);
+  for (int b = 0; b < nb; ++b) {
+    load_box(dst + b * BLK, map, b * 64, head, row, bar);
+    load_box(dst + b * BLK + HALF, map, b * 64, head, row + 64, bar);
+  }
 }
 
-// 128 rows x 64 columns boxes of a 16-bit (T, heads, D) tensor; false where TMA cannot read it
+// false where TMA cannot read the tensor
 bool make_map(Map &map, const void *p, int dtype, int64_t T, int heads, int D, int64_t ts, int64_t hs);
 // the same test without building the map
 bool map_eligible(const void *p, int D, int heads, int64_t T, int64_t ts, int64_t hs);
@@ -70,14 +88,14 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// Zeroes the rows of a landed tile that lie outside of [range.start, range.end):
-// a masked score of exactly 0 times a NaN there would still be NaN.  One warp; the
-// caller signals the tile afterwards.
-__device__ __forceinline__ void zero_outside(uint8_t *tile, int nb, int row0, Span range, int lane) {
-  for (int r = 0; r < TM; ++r) {
+// Zeroes the rows of landed blocks of `rows` rows x 64 columns, `pitch` bytes apart,
+// that lie outside of [range.start, range.end): a masked score of exactly 0 times a
+// NaN there would still be NaN.  One warp; the caller signals the tile afterwards.
+__device__ __forceinline__ void zero_outside(uint8_t *tile, int nb, uint32_t pitch, int rows, int row0, Span range, int lane) {
+  for (int r = 0; r < rows; ++r) {
     if (row0 + r >= range.start && row0 + r < range.end) continue;
     for (int b = lane; b < nb * 8; b += 32)
-      *reinterpret_cast<uint4 *>(tile + (b >> 3) * BLK + r * 128 + (b & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4 *>(tile + (b >> 3) * pitch + r * 128 + (b & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
   __syncwarp();
