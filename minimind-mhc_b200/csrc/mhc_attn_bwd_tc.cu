@@ -53,7 +53,8 @@ constexpr int NSOFT = 16;             // softmax warps: four to each quarter of 
 constexpr int W_TMA = NSOFT, W_MMA = NSOFT + 1;
 constexpr int NTHREADS = (NSOFT + 2) * 32;
 constexpr int TMEM_COLS = 512;
-constexpr uint32_t S_COL = 0, DP_COL = 128, A1_COL = 256, A2_COL = 384;
+// columns of TMEM: S; dP (two of them for DQ); the results; P
+constexpr uint32_t S_COL = 0, DP_COL = 128, A1_COL = 256;
 constexpr float P_SHIFT = 10.f;  // fp16: P times 2^10
 
 enum { ERR_TMA = 51, ERR_MMA = 52, ERR_SOFTMAX = 53 };
@@ -67,14 +68,17 @@ struct Item {
 
 template <int DP>
 struct Cfg {
-  static constexpr int NB = nblk(DP);
-  static constexpr uint32_t TILE = NB * BLK;
-  static constexpr int ST = NB == 1 ? 4 : 2;        // stages of C1 and of C2
+  using L = Tile<DP, true>;
+  static constexpr uint32_t TILE = L::BYTES;
+  static constexpr int ST = DP <= 64 ? 4 : (DP <= 96 ? 3 : 2);  // stages of C1 and of C2
   static constexpr uint32_t VEC = 2 * TM * 4;       // a stage's lse and D of its columns
+  static constexpr uint32_t A2_COL = A1_COL + DP;   // dV
+  static constexpr bool OWN_P = DP <= 96;           // P has 64 columns of its own; else it replaces S
+  static constexpr uint32_t P_COL = OWN_P ? 448 : S_COL;
 };
 
-constexpr int B_ITEM_F = 0, B_ITEM_E = 2, B_RF = 4, B_RE = 5, B_LAND = 6, B_SF = 7, B_PF = 8, B_DPF = 9, B_DSF = 10,
-              B_ACC_F = 11, B_DRAIN = 12, B_1F = 13;
+constexpr int B_ITEM_F = 0, B_ITEM_E = 2, B_RF = 4, B_RE = 5, B_LAND = 6, B_SF = 7, B_SE = 8, B_PF = 9, B_DPF = 10,
+              B_DSF = 12, B_ACC_F = 14, B_DRAIN = 15, B_1F = 16;  // dP and dS: one for even steps, one for odd
 // then ST each: 1F, 1E, 2F, 2E
 
 struct Sched {
@@ -128,12 +132,17 @@ __device__ __forceinline__ float ds_factor(const Args &a) {
   return 1.f;
 }
 
+// where the dP of the g-th column tile lies
+template <bool DKV>
+__device__ __forceinline__ uint32_t dp_col(int g) { return DKV || (g & 1) == 0 ? DP_COL : DP_COL + 256u; }
+
 template <typename T, int DP, bool DKV>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Map r2map, const __grid_constant__ Map c1map,
                    const __grid_constant__ Map c2map, const Args a, const Sched sched) {
   using C = Cfg<DP>;
-  constexpr int NB = C::NB, ST = C::ST;
+  using L = typename C::L;
+  constexpr int ST = C::ST;
   constexpr int B_1E = B_1F + ST, B_2F = B_1E + ST, B_2E = B_2F + ST, NBARS = B_2E + ST;
   constexpr bool F16 = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -148,7 +157,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   volatile int *abort_flag = &abort_word;
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
-#define WAIT_WARP(bar, par) (__all_sync(0xffffffffu, wait_parity<false>((bar), (par), abort_flag)))
+#define WAIT_WARP(bar, par) (wait_warp_parity((bar), (par), abort_flag))
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int G = a.H / a.Hk;
 
@@ -162,9 +171,12 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     mbar_init(BAR(B_RE), 1);
     mbar_init(BAR(B_LAND), 1);
     mbar_init(BAR(B_SF), 1);
+    mbar_init(BAR(B_SE), NSOFT);
     mbar_init(BAR(B_PF), NSOFT);
-    mbar_init(BAR(B_DPF), 1);
-    mbar_init(BAR(B_DSF), NSOFT);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(BAR(B_DPF + i), 1);
+      mbar_init(BAR(B_DSF + i), NSOFT);
+    }
     mbar_init(BAR(B_ACC_F), 1);
     mbar_init(BAR(B_DRAIN), 1);
     for (int i = 0; i < 4 * ST; ++i) mbar_init(BAR(B_1F + i), 1);
@@ -193,7 +205,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       const uint32_t bar = clean ? BAR(B_LAND) : BAR(full);
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, C::TILE + (vec ? C::VEC : 0u));
-        load_rows(dst, map, NB, head, row, bar);
+        load_rows<L>(dst, map, head, row, bar);
         if (vec) {
           const uint32_t v = vecs + (uint32_t)(g % ST) * C::VEC;
           bulk_load(v, a.lse + (int64_t)h * a.Tp + row, TM * 4, bar);
@@ -204,7 +216,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       if (clean) {
         if (!WAIT_WARP(BAR(B_LAND), (uint32_t)lands & 1u)) ok = false;
         ++lands;
-        zero_outside(gen + (dst - base), NB, BLK, TM, row, range, lane);
+        zero_outside<L>(gen + (dst - base), row, range, lane);
         if (lane == 0) mbar_arrive(BAR(full));
       }
     };
@@ -223,8 +235,8 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       ++rn;
       if (lane == 0) {
         mbar_arrive_expect_tx(BAR(B_RF), 2 * C::TILE);
-        load_rows(rs, r1map, NB, it.head, it.r0, BAR(B_RF));
-        load_rows(rs + C::TILE, r2map, NB, it.head, it.r0, BAR(B_RF));
+        load_rows<L>(rs, r1map, it.head, it.r0, BAR(B_RF));
+        load_rows<L>(rs + C::TILE, r2map, it.head, it.r0, BAR(B_RF));
       }
       for (int j = 0; j < it.n && ok; ++j, ++g) {
         const int s = g % ST;
@@ -247,100 +259,129 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   } else if (warp == W_MMA) {
     // ---------------- MMA issue: the warp runs it, one lane issues ----------------
     {
-      constexpr uint32_t id_s = idesc_of<T>(128, 0), id_g = idesc_of<T>(DP, 1);
+      constexpr uint32_t id_s = idesc_of<T>(128, 0), id_g = idesc_of<T>(L::N_FULL, 1), id_t = idesc_of<T>(32, 1);
       bool ok = true;
-      auto wait_warp = [&](uint32_t bar, uint32_t par) { return __all_sync(0xffffffffu, wait_parity<false>(bar, par, abort_flag)); };
+      auto wait_warp = [&](uint32_t bar, uint32_t par) { return wait_warp_parity(bar, par, abort_flag); };
       auto commit = [&](uint32_t bar) {
         if (elect_one()) umma_commit(bar);
       };
-      int i = 0, rn = 0, gk = 0, steps = 0;
+      int i = 0, rn = 0, gk = 0;
       struct Step {
         int j, n, g;
       } cur, nxt;
-      auto advance = [&](Step &s) -> bool {  // the next step, of this item or of the next one that has any
-        if (s.j + 1 < s.n) {
-          ++s.j;
-        } else {
+      bool rows_due = false;  // an item's steps are known, its rows not yet here
+      // The next step, of this item or of the next one that has any: 1, or 0 past the last, or (block = false) -1
+      // while it is not known or its rows are still on their way.
+      auto advance = [&](Step &s, bool block) -> int {
+        if (!rows_due) {
+          if (s.j + 1 < s.n) {
+            ++s.j;
+            s.g = gk++;
+            return 1;
+          }
           while (true) {
-            if (!wait_warp(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; return false; }
+            const uint32_t bar = BAR(B_ITEM_F + (i & 1)), par = (uint32_t)(i >> 1) & 1u;
+            if (!block && !__all_sync(0xffffffffu, mbar_test_wait(bar, par))) return -1;
+            if (!wait_warp(bar, par)) { ok = false; return 0; }
             const bool done = uniform(items[i & 1].done);
             s.j = 0;
             s.n = uniform(items[i & 1].n);
+            __syncwarp();
             if (elect_one()) mbar_arrive(BAR(B_ITEM_E + (i & 1)));
             ++i;
-            if (done) return false;
+            if (done) return 0;
             if (s.n > 0) break;
           }
-          if (!wait_warp(BAR(B_RF), (uint32_t)rn & 1u)) { ok = false; return false; }
-          ++rn;
+          rows_due = true;
         }
+        if (!block && !__all_sync(0xffffffffu, mbar_test_wait(BAR(B_RF), (uint32_t)rn & 1u))) return -1;
+        if (!wait_warp(BAR(B_RF), (uint32_t)rn & 1u)) { ok = false; return 0; }
+        rows_due = false;
+        ++rn;
         s.g = gk++;
-        return true;
+        return 1;
       };
-      // [128 x 128] = rows (K-major) times columns^T (K-major)
-      auto cross = [&](uint32_t d, uint32_t r, uint32_t c) {
-        const uint64_t rd = umma_desc_sw128(r), cd = umma_desc_sw128(c);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) umma_bf16(d, rd + k_step(kk, BLK), cd + k_step(kk, BLK), id_s, kk > 0);
-        }
+      auto arrived = [&](int bar, const Step &s) {
+        if (!wait_warp(BAR(bar + s.g % ST), (uint32_t)(s.g / ST) & 1u)) ok = false;
       };
-      // accumulator += W C: W [128 x 128] in TMEM, 32 of its columns in 16 of each 32; C MN-major
-      auto add = [&](uint32_t d, uint32_t w, uint32_t c, bool begin) {
-        const uint64_t cd = umma_desc(c, BLK, 1024, 2);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < TM / 16; ++kk)
-            umma_f16_ts(d, w + (kk >> 1) * 32u + (kk & 1) * 8u, cd + mn_step(kk), id_g, !begin || kk > 0);
-        }
+      auto is_here = [&](int bar, const Step &s) {
+        return __all_sync(0xffffffffu, mbar_test_wait(BAR(bar + s.g % ST), (uint32_t)(s.g / ST) & 1u)) != 0;
       };
       auto scores = [&](const Step &s) {
-        if (!wait_warp(BAR(B_1F + s.g % ST), (uint32_t)(s.g / ST) & 1u)) { ok = false; return; }
         tc_fence_after();
-        cross(tmem + S_COL, rs, c1s + (s.g % ST) * C::TILE);
+        mma_rows<L>(tmem + S_COL, rs, c1s + (s.g % ST) * C::TILE, id_s);
         commit(BAR(B_SF));
       };
       auto dprob = [&](const Step &s) {
-        if (!wait_warp(BAR(B_2F + s.g % ST), (uint32_t)(s.g / ST) & 1u)) { ok = false; return; }
         tc_fence_after();
-        cross(tmem + DP_COL, rs + C::TILE, c2s + (s.g % ST) * C::TILE);
-        commit(BAR(B_DPF));
+        mma_rows<L>(tmem + dp_col<DKV>(s.g), rs + C::TILE, c2s + (s.g % ST) * C::TILE, id_s);
+        commit(BAR(B_DPF + (s.g & 1)));
         if (!DKV) commit(BAR(B_2E + s.g % ST));
         if (s.j == s.n - 1) commit(BAR(B_RE));
       };
+      // The order of a step: S(j+1) goes out as soon as S(j) has been read (P with columns of its own, or DQ) or
+      // behind dV(j) (P in its place); dP(j+1) with it where dP has two places (DQ), else behind dK(j).  What has not
+      // arrived by then goes out at the end of the step.  The next step may be another item's.
       cur.j = cur.n = 0;
-      bool have = advance(cur);
-      if (have && ok) scores(cur);
-      if (have && ok) dprob(cur);
-      while (have && ok) {
+      int have = advance(cur, true);
+      if (have == 1 && ok) {
+        arrived(B_1F, cur);
+        if (ok) scores(cur);
+        if (ok) arrived(B_2F, cur);
+        if (ok) dprob(cur);
+      }
+      while (have == 1 && ok) {
+        const bool last = cur.j == cur.n - 1;
         nxt = cur;
-        const bool same_item = cur.j + 1 < cur.n;
-        bool more = same_item && advance(nxt);
+        have = advance(nxt, false);
         if (!ok) break;
-        const uint32_t par = (uint32_t)steps & 1u;
-        ++steps;
-        if (!wait_warp(BAR(B_PF), par)) { ok = false; break; }
-        tc_fence_after();
+        bool s_due = have != 0, d_due = s_due;
+        if (!DKV || C::OWN_P) {
+          if (!wait_warp(BAR(B_SE), (uint32_t)cur.g & 1u)) { ok = false; break; }
+          // DQ has nothing else to issue until dS: with three stages the next tile is as good as here
+          const bool sure = !DKV && ST >= 3 && !last;
+          if (sure) {
+            arrived(B_1F, nxt);
+            arrived(B_2F, nxt);
+            if (!ok) break;
+          }
+          if (have == 1 && (sure || is_here(B_1F, nxt))) {
+            scores(nxt);
+            s_due = false;
+            if (!DKV && (sure || is_here(B_2F, nxt))) {
+              dprob(nxt);
+              d_due = false;
+            }
+          }
+        }
         if (DKV) {
-          add(tmem + A2_COL, tmem + S_COL, c2s + (cur.g % ST) * C::TILE, cur.j == 0);
+          if (!wait_warp(BAR(B_PF), (uint32_t)cur.g & 1u)) { ok = false; break; }
+          tc_fence_after();
+          mma_sum<L>(tmem + C::A2_COL, tmem + C::P_COL, C::OWN_P ? 16u : 32u, c2s + (cur.g % ST) * C::TILE, id_g, id_t, cur.j == 0);
           commit(BAR(B_2E + cur.g % ST));
+          if (s_due && have == 1 && is_here(B_1F, nxt)) {
+            scores(nxt);
+            s_due = false;
+          }
         }
-        if (more) scores(nxt);
-        if (!ok) break;
-        if (!wait_warp(BAR(B_DSF), par)) { ok = false; break; }
+        if (!wait_warp(BAR(B_DSF + (cur.g & 1)), (uint32_t)(cur.g >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();
-        add(tmem + A1_COL, tmem + DP_COL, c1s + (cur.g % ST) * C::TILE, cur.j == 0);
+        mma_sum<L>(tmem + A1_COL, tmem + dp_col<DKV>(cur.g), 32u, c1s + (cur.g % ST) * C::TILE, id_g, id_t, cur.j == 0);
         commit(BAR(B_1E + cur.g % ST));
-        if (!same_item) {
-          commit(BAR(B_ACC_F));
-          more = advance(nxt);  // the next item's rows may still be on their way
+        if (last) commit(BAR(B_ACC_F));
+        if (have == -1) have = advance(nxt, true);
+        if (have != 1 || !ok) break;
+        if (s_due) {
+          arrived(B_1F, nxt);
           if (!ok) break;
-          if (more) scores(nxt);
-          if (!ok) break;
+          scores(nxt);
         }
-        if (more) dprob(nxt);
+        if (d_due) {
+          arrived(B_2F, nxt);
+          if (!ok) break;
+          dprob(nxt);
+        }
         cur = nxt;
-        have = more;
       }
       if (!ok && lane == 0) give_up(ERR_MMA, abort_flag, a.err_flag);
       commit(BAR(B_DRAIN));
@@ -350,7 +391,8 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     // ---------------- softmax: thread = a quarter of a row ----------------
     const int part = warp >> 2;  // its columns: 32 from 32 part
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + S_COL + part * 32u, d_addr = tmem + lanes + DP_COL + part * 32u;
+    const uint32_t s_addr = tmem + lanes + S_COL + part * 32u;
+    const uint32_t p_addr = tmem + lanes + C::P_COL + part * (C::OWN_P ? 16u : 32u);
     const int row = (warp & 3) * 32 + lane;
     const float c = a.scale_log2;
     const uint64_t c2 = f2_pack(c, c);
@@ -388,9 +430,8 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         tc_fence_after();
         uint32_t r[32];
         tmem_ld32u(s_addr, r);
-        if (!DKV) {
-          arrive(B_PF);  // S may be overwritten
-        } else {
+        if (!DKV || C::OWN_P) arrive(B_SE);  // S may be overwritten
+        if (DKV) {
           // the columns' lse and D came with C1: its barrier orders them (its phase is complete, S was formed from it)
           if (!WAIT_WARP(BAR(B_1F + step % ST), (uint32_t)(step / ST) & 1u)) { ok = false; break; }
         }
@@ -422,12 +463,17 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = pack2<T>(p[2 * e], p[2 * e + 1]);
-          tmem_st16(s_addr, w);
+          if (C::OWN_P && step > 0) {  // the last P has been used: its dV released the stage of its C2
+            if (!WAIT_WARP(BAR(B_2E + (step - 1) % ST), (uint32_t)((step - 1) / ST) & 1u)) { ok = false; break; }
+            tc_fence_after();
+          }
+          tmem_st16(p_addr, w);
           tmem_wait_st();
           arrive(B_PF);
         }
-        if (!WAIT_WARP(BAR(B_DPF), (uint32_t)step & 1u)) { ok = false; break; }
+        if (!WAIT_WARP(BAR(B_DPF + (step & 1)), (uint32_t)(step >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();
+        const uint32_t d_addr = tmem + lanes + dp_col<DKV>(step) + part * 32u;
         tmem_ld32u(d_addr, r);
         uint32_t w[16];
 #pragma unroll
@@ -458,7 +504,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         }
         tmem_st16(d_addr, w);
         tmem_wait_st();
-        arrive(B_DSF);
+        arrive(B_DSF + (step & 1));
       }
       if (!ok) break;
       if (n > 0) {
@@ -477,7 +523,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         const float mul = second ? out2 : out1;
         uint32_t o[16];
         if (n > 0) {
-          tmem_ld16u(tmem + lanes + (second ? A2_COL : A1_COL) + d, o);
+          tmem_ld16u(tmem + lanes + (second ? C::A2_COL : A1_COL) + d, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0u;

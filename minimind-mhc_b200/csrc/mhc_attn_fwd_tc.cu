@@ -60,9 +60,9 @@ struct Item {
 
 template <int DP>
 struct Cfg {
-  static constexpr int NB = nblk(DP);
-  static constexpr uint32_t TILE = NB * BLK;
-  static constexpr int ST = NB == 1 ? 4 : 2;  // stages of K and of V
+  using L = Tile<DP, false>;
+  static constexpr uint32_t TILE = L::BYTES;
+  static constexpr int ST = DP <= 64 ? 4 : 2;  // stages of K and of V
 };
 
 constexpr int B_ITEM_F = 0, B_ITEM_E = 2, B_QF = 4, B_QE = 5, B_LAND = 6, B_SF = 7, B_PF = 9, B_OF = 11, B_DRAIN = 13,
@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map kmap, const __grid_constant__ Map vmap,
                    const Args a, const Sched sched) {
   using C = Cfg<DP>;
-  constexpr int NB = C::NB, ST = C::ST;
+  using L = typename C::L;
+  constexpr int ST = C::ST;
   constexpr int B_KE = B_KF + ST, B_VF = B_KE + ST, B_VE = B_VF + ST, NBARS = B_VE + ST;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Item items[2];
@@ -184,7 +185,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
     for (int i = 0; ok; ++i) {
       Item it;
       const bool live = item_of(a, sched, snake(i, blockIdx.x, gridDim.x), it);
-      if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_ITEM_E + (i & 1)), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag))) { ok = false; break; }
+      if (!wait_warp_parity(BAR(B_ITEM_E + (i & 1)), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
       if (lane == 0) {
         items[i & 1] = it;
         mbar_arrive(BAR(B_ITEM_F + (i & 1)));
@@ -192,34 +193,34 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       __syncwarp();
       if (!live) break;
       if (it.n == 0) continue;
-      if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_QE), ((uint32_t)qn & 1u) ^ 1u, abort_flag))) { ok = false; break; }
+      if (!wait_warp_parity(BAR(B_QE), ((uint32_t)qn & 1u) ^ 1u, abort_flag)) { ok = false; break; }
       ++qn;
       if (lane == 0) {
         mbar_arrive_expect_tx(BAR(B_QF), 2 * C::TILE);
-        load_rows(qs, qmap, NB, it.head[0], it.q0[0], BAR(B_QF));
+        load_rows<L>(qs, qmap, it.head[0], it.q0[0], BAR(B_QF));
         // without a second tile the first is loaded twice: the products of its copy are not used
-        load_rows(qs + C::TILE, qmap, NB, it.head[1], it.q0[1] < 0 ? it.q0[0] : it.q0[1], BAR(B_QF));
+        load_rows<L>(qs + C::TILE, qmap, it.head[1], it.q0[1] < 0 ? it.q0[0] : it.q0[1], BAR(B_QF));
       }
       for (int j = 0; j < it.n && ok; ++j, ++g) {
         const int s = g % ST;
         const uint32_t free_par = ((uint32_t)(g / ST) & 1u) ^ 1u;
         const int row = it.k0 + j * TM;
-        if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_KE + s), free_par, abort_flag))) { ok = false; break; }
+        if (!wait_warp_parity(BAR(B_KE + s), free_par, abort_flag)) { ok = false; break; }
         if (lane == 0) {
           mbar_arrive_expect_tx(BAR(B_KF + s), C::TILE);
-          load_rows(ks + s * C::TILE, kmap, NB, it.kv_head, row, BAR(B_KF + s));
+          load_rows<L>(ks + s * C::TILE, kmap, it.kv_head, row, BAR(B_KF + s));
         }
-        if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_VE + s), free_par, abort_flag))) { ok = false; break; }
+        if (!wait_warp_parity(BAR(B_VE + s), free_par, abort_flag)) { ok = false; break; }
         const bool clean = row < range.start || min((int64_t)row + TM, a.T) > range.end;
         if (lane == 0) {
           mbar_arrive_expect_tx(BAR(clean ? B_LAND : B_VF + s), C::TILE);
-          load_rows(vs + s * C::TILE, vmap, NB, it.kv_head, row, BAR(clean ? B_LAND : B_VF + s));
+          load_rows<L>(vs + s * C::TILE, vmap, it.kv_head, row, BAR(clean ? B_LAND : B_VF + s));
         }
         __syncwarp();
         if (clean) {
-          if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_LAND), (uint32_t)lands & 1u, abort_flag))) ok = false;
+          if (!wait_warp_parity(BAR(B_LAND), (uint32_t)lands & 1u, abort_flag)) ok = false;
           ++lands;
-          zero_outside(gen + (vs - base) + s * C::TILE, NB, BLK, TM, row, range, lane);
+          zero_outside<L>(gen + (vs - base) + s * C::TILE, row, range, lane);
           if (lane == 0) mbar_arrive(BAR(B_VF + s));
         }
       }
@@ -234,9 +235,9 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
   } else if (warp == W_MMA) {
     // ---------------- MMA issue: the warp runs it, one lane issues ----------------
     {
-      constexpr uint32_t id_s = idesc_of<T>(128, 0), id_o = idesc_of<T>(DP, 1);
+      constexpr uint32_t id_s = idesc_of<T>(128, 0), id_o = idesc_of<T>(L::N_FULL, 1), id_t = idesc_of<T>(32, 1);
       bool ok = true;
-      auto wait_warp = [&](uint32_t bar, uint32_t par) { return __all_sync(0xffffffffu, wait_parity<false>(bar, par, abort_flag)); };
+      auto wait_warp = [&](uint32_t bar, uint32_t par) { return wait_warp_parity(bar, par, abort_flag); };
       auto commit = [&](uint32_t bar) {
         if (elect_one()) umma_commit(bar);
       };
@@ -273,12 +274,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       };
       auto scores = [&](const Step &s, int t) {
         if (s.j < s.first[t] || s.j >= s.last[t]) return;
-        const uint64_t q = umma_desc_sw128(qs + t * C::TILE), k = umma_desc_sw128(ks + (s.g % ST) * C::TILE);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            umma_bf16(tmem + S_COL + t * 128u, q + k_step(kk, BLK), k + k_step(kk, BLK), id_s, kk > 0);
-        }
+        mma_rows<L>(tmem + S_COL + t * 128u, qs + t * C::TILE, ks + (s.g % ST) * C::TILE, id_s);
         commit(BAR(B_SF + t));
       };
       auto after_scores = [&](const Step &s) {
@@ -304,13 +300,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         if (!wait_warp(BAR(B_PF + t), (uint32_t)pf[t] & 1u)) { ok = false; return; }
         ++pf[t];
         tc_fence_after();
-        const uint64_t v = umma_desc(vs + (s.g % ST) * C::TILE, BLK, 1024, 2);
-        const bool more = s.j > s.first[t];
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < TM / 16; ++kk)
-            umma_f16_ts(tmem + O_COL + t * 128u, tmem + S_COL + t * 128u + kk * 8u, v + mn_step(kk), id_o, more || kk > 0);
-        }
+        mma_sum<L>(tmem + O_COL + t * 128u, tmem + S_COL + t * 128u, 16u, vs + (s.g % ST) * C::TILE, id_o, id_t, s.j == s.first[t]);
         commit(BAR(B_OF + t));
       };
       // tile 0's product, its next scores, then the same for tile 1: each tile's softmax runs beside the other's
@@ -357,7 +347,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
     bool ok = true;
     int sf = 0, of = 0;
     for (int i = 0; ok; ++i) {
-      if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u, abort_flag))) { ok = false; break; }
+      if (!wait_warp_parity(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u, abort_flag)) { ok = false; break; }
       const int q0 = items[i & 1].q0[t], head = items[i & 1].head[t], first = items[i & 1].first[t], last = items[i & 1].last[t];
       const int k00 = items[i & 1].k0, done = items[i & 1].done;
       mbar_arrive(BAR(B_ITEM_E + (i & 1)));
@@ -368,7 +358,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       float ref = -INFINITY, sum = 0.f;
       for (int j = first; j < last; ++j) {
         const int k0 = k00 + j * TM;
-        if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_SF + t), (uint32_t)sf & 1u, abort_flag))) { ok = false; break; }
+        if (!wait_warp_parity(BAR(B_SF + t), (uint32_t)sf & 1u, abort_flag)) { ok = false; break; }
         ++sf;
         tc_fence_after();
         uint32_t r[4][32];
@@ -400,7 +390,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
           ref = next;
           sum *= fix;
           if (j > first) {  // O holds the earlier tiles' sum, once their product is done
-            if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag))) { ok = false; break; }
+            if (!wait_warp_parity(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag)) { ok = false; break; }
             tc_fence_after();
             // in pieces that leave the scores in their registers
 #pragma unroll
@@ -442,7 +432,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       if (!ok) break;
       const bool seen = last > first;
       if (seen) {
-        if (!__all_sync(0xffffffffu, wait_parity<false>(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag))) { ok = false; break; }
+        if (!wait_warp_parity(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -610,11 +600,16 @@ bool make_map(Map &map, const void *p, int dtype, int64_t T, int heads, int D, i
   const bool f = map.token_first != 0;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)(f ? T : heads), (cuuint64_t)(f ? heads : T)};
   const cuuint64_t strides[2] = {(cuuint64_t)(f ? ts : hs) * 2, (cuuint64_t)(f ? hs : ts) * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(f ? 64 : 1), (cuuint32_t)(f ? 1 : 64)};
   const cuuint32_t estr[3] = {1, 1, 1};
-  return enc(&map.m, dtype == MHC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-             const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  for (int tail = 0; tail < 2; ++tail) {
+    const cuuint32_t box[3] = {tail ? 32u : 64u, (cuuint32_t)(f ? TM : 1), (cuuint32_t)(f ? 1 : TM)};
+    if (enc(tail ? &map.t : &map.m, dtype == MHC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            tail ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  return true;
 }
 
 }  // namespace attn
