@@ -255,8 +255,8 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
                  const int64_t *strides, const int32_t *cu_seqlens, int batch, int64_t seqlen, float scale,
                  void *out, void *out_lo, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Bytes of scratch `mhc_attn_bwd` needs. */
-size_t mhc_attn_bwd_workspace(int64_t T, int H);
+/* Bytes of scratch `mhc_attn_bwd` needs on the current device. */
+size_t mhc_attn_bwd_workspace(int64_t T, int H, int Hk, int D);
 
 /*
  * Gradients of mhc_attn_fwd from out, out_lo (or NULL), lse and dout (T, H, D) contiguous:
@@ -272,7 +272,7 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
 /* Training step: top-k router with its balance loss                         */
 /* ------------------------------------------------------------------------ */
 
-/* Bytes of scratch `mhc_route_fwd` needs (on the device the call will run on). */
+/* Bytes of scratch `mhc_route_fwd` needs on the current device (0: none, workspace may be NULL). */
 size_t mhc_route_fwd_workspace(int64_t T, int E);
 
 /*

@@ -19,9 +19,9 @@
 // v rounded to zero would divide by eps.  The step itself uses the fp32 m' and
 // v'; only what is stored is rounded.  A block with a non-finite moment gets the
 // non-finite scale and so reads back as NaN, as fp32 moments would.
-// The arithmetic uses single IEEE operations (no contraction, no approximate
-// division or root): a value next to the edge between two codes then falls on
-// the same side wherever the formula is evaluated in fp32.
+// What decides a code uses single IEEE operations (no contraction, no approximate
+// division or root): a value next to the edge between two codes then falls on the
+// same side wherever the formula is evaluated in fp32.
 //
 // A warp owns one block of 256 values at a time, a lane 4 + 4 of them (16-byte
 // accesses in fp32, 8-byte in 16-bit types, 4-byte for codes), so the block's
@@ -83,24 +83,48 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   return v;
 }
 
-// 4 consecutive values of a runtime-typed tensor, at value index i
-__device__ __forceinline__ void load4(const void *p, int dt, int64_t i, float (&o)[4]) {
+// The values a lane holds of its warp's block: value index base + lane_value(e),
+// e < 8; two runs of four.
+__device__ __forceinline__ int lane_value(int lane, int e) { return (e >> 2) * 128 + lane * 4 + (e & 3); }
+
+// A lane's 8 values of a runtime-typed tensor as they lie in memory.  Loading and
+// converting are apart, so that a lane asks for everything before it waits for the
+// first of it (bf16 parameters converted as they came: 1.40 ms for the 321 M values
+// of the MoE decoder, against MOE_MS).
+struct Raw {
+  uint4 a, b;  // 16-bit types: the lower halves
+};
+__device__ __forceinline__ Raw load_raw(const void *p, int dt, int64_t base, int lane) {
+  Raw r;
   if (dt == MHC_F32) {
-    const float4 r = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i));
-    o[0] = r.x; o[1] = r.y; o[2] = r.z; o[3] = r.w;
+    const float *q = static_cast<const float *>(p) + base + lane * 4;
+    r.a = __ldcs(reinterpret_cast<const uint4 *>(q));
+    r.b = __ldcs(reinterpret_cast<const uint4 *>(q + 128));
   } else {
-    const uint2 r = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i));
-    if (dt == MHC_BF16) {
-      o[0] = __uint_as_float(r.x << 16); o[1] = __uint_as_float(r.x & 0xffff0000u);
-      o[2] = __uint_as_float(r.y << 16); o[3] = __uint_as_float(r.y & 0xffff0000u);
-    } else {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&r.x));
-      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
-      o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
-    }
+    const uint16_t *q = static_cast<const uint16_t *>(p) + base + lane * 4;
+    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(q)), y = __ldcs(reinterpret_cast<const uint2 *>(q + 128));
+    r.a.x = x.x; r.a.y = x.y;
+    r.b.x = y.x; r.b.y = y.y;
+  }
+  return r;
+}
+__device__ __forceinline__ void convert4(const uint4 &r, int dt, float *o) {
+  if (dt == MHC_F32) {
+    o[0] = __uint_as_float(r.x); o[1] = __uint_as_float(r.y); o[2] = __uint_as_float(r.z); o[3] = __uint_as_float(r.w);
+  } else if (dt == MHC_BF16) {
+    o[0] = __uint_as_float(r.x << 16); o[1] = __uint_as_float(r.x & 0xffff0000u);
+    o[2] = __uint_as_float(r.y << 16); o[3] = __uint_as_float(r.y & 0xffff0000u);
+  } else {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&r.x));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
+    o[0] = x.x; o[1] = x.y; o[2] = y.x; o[3] = y.y;
   }
 }
-__device__ __forceinline__ void store4(void *p, int dt, int64_t i, const float (&v)[4]) {
+__device__ __forceinline__ void convert8(const Raw &r, int dt, float (&o)[8]) {
+  convert4(r.a, dt, o);
+  convert4(r.b, dt, o + 4);
+}
+__device__ __forceinline__ void store4(void *p, int dt, int64_t i, const float *v) {
   if (dt == MHC_F32) {
     __stcs(reinterpret_cast<float4 *>(static_cast<float *>(p) + i), make_float4(v[0], v[1], v[2], v[3]));
   } else {
@@ -117,33 +141,18 @@ __device__ __forceinline__ void store4(void *p, int dt, int64_t i, const float (
     __stcs(reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + i), r);
   }
 }
-
-// The values a lane holds of its warp's block: value index base + idx(e),
-// e < 8; two runs of four.
-__device__ __forceinline__ int lane_value(int lane, int e) { return (e >> 2) * 128 + lane * 4 + (e & 3); }
-
-__device__ __forceinline__ void load8(const void *p, int dt, int64_t base, int64_t n, bool whole, int lane,
-                                      float (&o)[8]) {
-  if (whole) {
-    float a[4], b[4];
-    load4(p, dt, base + lane * 4, a);
-    load4(p, dt, base + 128 + lane * 4, b);
+// value by value, for blocks that end early or lie at odd addresses
+__device__ __forceinline__ void load_each(const void *p, int dt, int64_t base, int64_t n, int lane, float (&o)[8]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { o[e] = a[e]; o[4 + e] = b[e]; }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t i = base + lane_value(lane, e);
-      o[e] = i < n ? load_dyn(p, dt, i) : 0.f;
-    }
+  for (int e = 0; e < 8; ++e) {
+    const int64_t i = base + lane_value(lane, e);
+    o[e] = i < n ? load_dyn(p, dt, i) : 0.f;
   }
 }
-__device__ __forceinline__ void store8(void *p, int dt, int64_t base, int64_t n, bool whole, int lane,
-                                       const float (&v)[8]) {
+__device__ __forceinline__ void store8(void *p, int dt, int64_t base, int64_t n, bool whole, int lane, const float (&v)[8]) {
   if (whole) {
-    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-    store4(p, dt, base + lane * 4, a);
-    store4(p, dt, base + 128 + lane * 4, b);
+    store4(p, dt, base + lane * 4, v);
+    store4(p, dt, base + 128 + lane * 4, v + 4);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -153,26 +162,24 @@ __device__ __forceinline__ void store8(void *p, int dt, int64_t base, int64_t n,
   }
 }
 
-// 8-bit codes of a lane as integers (signed for m, unsigned for v)
-template <bool SIGNED>
-__device__ __forceinline__ void load_codes(const void *p, int64_t base, int64_t n, bool whole, int lane, float (&o)[8]) {
+// 8-bit codes of a lane, four to a word, and as numbers (signed for m, unsigned for v)
+__device__ __forceinline__ uint2 load_codes(const void *p, int64_t base, int64_t n, bool whole, int lane) {
   const uint8_t *q = static_cast<const uint8_t *>(p);
-  if (whole) {
-    const uint32_t w[2] = {__ldcs(reinterpret_cast<const uint32_t *>(q + base + lane * 4)),
-                           __ldcs(reinterpret_cast<const uint32_t *>(q + base + 128 + lane * 4))};
+  if (whole)
+    return make_uint2(__ldcs(reinterpret_cast<const uint32_t *>(q + base + lane * 4)),
+                      __ldcs(reinterpret_cast<const uint32_t *>(q + base + 128 + lane * 4)));
+  uint32_t w[2] = {0u, 0u};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t b = (w[e >> 2] >> (8 * (e & 3))) & 0xffu;
-      o[e] = SIGNED ? (float)(int)(int8_t)b : (float)b;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t i = base + lane_value(lane, e);
-      const uint8_t b = i < n ? q[i] : 0;
-      o[e] = SIGNED ? (float)(int)(int8_t)b : (float)b;
-    }
+  for (int e = 0; e < 8; ++e) {
+    const int64_t i = base + lane_value(lane, e);
+    if (i < n) w[e >> 2] |= (uint32_t)q[i] << (8 * (e & 3));
   }
+  return make_uint2(w[0], w[1]);
+}
+template <bool SIGNED>
+__device__ __forceinline__ float code_value(const uint2 &w, int e) {
+  const uint32_t b = ((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu;
+  return SIGNED ? (float)(int)(int8_t)b : (float)b;
 }
 __device__ __forceinline__ void store_codes(void *p, int64_t base, int64_t n, bool whole, int lane, const int (&c)[8]) {
   uint8_t *q = static_cast<uint8_t *>(p);
@@ -207,6 +214,45 @@ __device__ __forceinline__ int pack_m(float m, float safe) {
 __device__ __forceinline__ int pack_v(float v, float safe) {
   const int c = __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, safe))), 255.f));
   return v > 0.f && c < 1 ? 1 : c;
+}
+
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The same codes, mostly without the IEEE division and roots (three long sequences
+// a value; with them the 8-bit step took 2.02 ms for 321 M values, against EIGHT_MS
+// ms): 127 sqrt(|m| / safe) from a reciprocal and an approximate root is within 127
+// * 2^-21 of the exact value, 255 (v / safe)^(1/4) within 255 * 2^-21.  Only a
+// value nearer than EDGE to the middle between two codes can round to the other
+// one; it is done again exactly.  `inv` = 1 / safe; scales too small for it to be a
+// normal number are passed with inv = 0 and are all done exactly.
+constexpr float EDGE = 4e-4f;
+template <bool SIGNED>
+__device__ __forceinline__ void pack_codes(const float (&x)[8], float safe, float inv, int (&c)[8]) {
+  bool near = inv == 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = fabsf(x[e]) * inv;
+    const float y = SIGNED ? sqrt_approx(q) * 127.f : sqrt_approx(sqrt_approx(q)) * 255.f;
+    const float r = rintf(y);
+    near |= !(fabsf(y - r) < 0.5f - EDGE);  // NaN too
+    c[e] = __float2int_rn(SIGNED && x[e] < 0.f ? -r : r);
+    if (!SIGNED && x[e] > 0.f && c[e] < 1) c[e] = 1;
+  }
+  if (near) {
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      float v = x[0];
+#pragma unroll
+      for (int u = 1; u < 8; ++u) v = e == u ? x[u] : v;
+      const int k = SIGNED ? pack_m(v, safe) : pack_v(v, safe);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) c[u] = e == u ? k : c[u];
+    }
+  }
 }
 
 // table entry of a chunk: the last one whose first chunk is not above it
@@ -248,26 +294,40 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     const int ei = entry_of(tab, chunk);
     const Entry &t = tab.t[ei];
     const int64_t first = (int64_t)(chunk - t.first_chunk) * CHUNK;
-#pragma unroll
+#pragma unroll 1
     for (int it = 0; it < CHUNK / (QB * WARPS); ++it) {
       const int64_t base = first + (int64_t)(it * WARPS + warp) * QB;
       if (base >= t.n) break;
       const bool whole = t.vec && base + QB <= t.n;
       float p[8], g[8], m[8], v[8];
-      load8(t.p, t.pdt, base, t.n, whole, lane, p);
-      load8(t.g, t.gdt, base, t.n, whole, lane, g);
       if constexpr (Q8) {
         const float sm = t.ms[base / QB], sv = t.vs[base / QB];
-        load_codes<true>(t.m, base, t.n, whole, lane, m);
-        load_codes<false>(t.v, base, t.n, whole, lane, v);
+        const uint2 cm = load_codes(t.m, base, t.n, whole, lane), cv = load_codes(t.v, base, t.n, whole, lane);
+        if (whole) {
+          const Raw rp = load_raw(t.p, t.pdt, base, lane), rg = load_raw(t.g, t.gdt, base, lane);
+          convert8(rp, t.pdt, p);
+          convert8(rg, t.gdt, g);
+        } else {
+          load_each(t.p, t.pdt, base, t.n, lane, p);
+          load_each(t.g, t.gdt, base, t.n, lane, g);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          m[e] = unpack_m(m[e], sm);
-          v[e] = unpack_v(v[e], sv);
+          m[e] = unpack_m(code_value<true>(cm, e), sm);
+          v[e] = unpack_v(code_value<false>(cv, e), sv);
         }
+      } else if (whole) {
+        const Raw rm = load_raw(t.m, MHC_F32, base, lane), rv = load_raw(t.v, MHC_F32, base, lane);
+        const Raw rp = load_raw(t.p, t.pdt, base, lane), rg = load_raw(t.g, t.gdt, base, lane);
+        convert8(rp, t.pdt, p);
+        convert8(rg, t.gdt, g);
+        convert8(rm, MHC_F32, m);
+        convert8(rv, MHC_F32, v);
       } else {
-        load8(t.m, MHC_F32, base, t.n, whole, lane, m);
-        load8(t.v, MHC_F32, base, t.n, whole, lane, v);
+        load_each(t.p, t.pdt, base, t.n, lane, p);
+        load_each(t.g, t.gdt, base, t.n, lane, g);
+        load_each(t.m, MHC_F32, base, t.n, lane, m);
+        load_each(t.v, MHC_F32, base, t.n, lane, v);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -293,14 +353,11 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
         }
         // an empty block divides by one; every code is then zero
         const float dm = am > 0.f ? am : 1.f, dv = av > 0.f ? av : 1.f;
-        int cm[8], cv[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          cm[e] = pack_m(m[e], dm);
-          cv[e] = pack_v(v[e], dv);
-        }
-        store_codes(t.m, base, t.n, whole, lane, cm);
-        store_codes(t.v, base, t.n, whole, lane, cv);
+        int c[8];
+        pack_codes<true>(m, dm, dm > 1e-30f ? __fdiv_rn(1.f, dm) : 0.f, c);
+        store_codes(t.m, base, t.n, whole, lane, c);
+        pack_codes<false>(v, dv, dv > 1e-30f ? __fdiv_rn(1.f, dv) : 0.f, c);
+        store_codes(t.v, base, t.n, whole, lane, c);
       } else {
         store8(t.m, MHC_F32, base, t.n, whole, lane, m);
         store8(t.v, MHC_F32, base, t.n, whole, lane, v);
@@ -327,7 +384,10 @@ __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constan
       const int64_t base = first + (int64_t)(it * WARPS + warp) * QB;
       if (base >= t.n) break;
       float g[8];
-      load8(t.g, t.gdt, base, t.n, t.vec && base + QB <= t.n, lane, g);
+      if (t.vec && base + QB <= t.n)
+        convert8(load_raw(t.g, t.gdt, base, lane), t.gdt, g);
+      else
+        load_each(t.g, t.gdt, base, t.n, lane, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) a = fmaf(g[e], g[e], a);
     }
@@ -354,10 +414,10 @@ __global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *codes, c
     const int64_t base = b * QB;
     const bool whole = vec && base + QB <= n;
     const float s = scales[b];
+    const uint2 w = load_codes(codes, base, n, whole, lane);
     float c[8];
-    load_codes<SIGNED>(codes, base, n, whole, lane, c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = SIGNED ? unpack_m(c[e], s) : unpack_v(c[e], s);
+    for (int e = 0; e < 8; ++e) c[e] = SIGNED ? unpack_m(code_value<true>(w, e), s) : unpack_v(code_value<false>(w, e), s);
     store8(out, MHC_F32, base, n, whole, lane, c);
   }
 }

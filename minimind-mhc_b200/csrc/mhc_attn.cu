@@ -294,35 +294,49 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t 
   const Span range = packed_range(a);
   const T *o = static_cast<const T *>(a.out), *lo = static_cast<const T *>(a.out_lo), *d = static_cast<const T *>(a.dout);
   float most_o = 0.f, most_v = 0.f;
-#pragma unroll 2
-  for (int it = 0; it < 8; ++it) {
-    const int64_t t = (int64_t)blockIdx.x * 128 + it * 16 + (threadIdx.x >> 4);
-    if (t >= a.T) break;
-    const bool inside = t >= range.start && t < range.end;
-    const int64_t at = (t * a.H + h) * a.D;
-    float s = 0.f;
+  constexpr int ROWS = 4;  // in flight at a time
+#pragma unroll 1
+  for (int it = 0; it < 8; it += ROWS) {
+    float s[ROWS] = {};
+    const int64_t t0 = (int64_t)blockIdx.x * 128 + it * 16 + (threadIdx.x >> 4);
     for (int c = l * VEC; c < a.D; c += 16 * VEC) {
-      T ov[VEC], lv[VEC], dv[VEC];
-      if constexpr (VEC == 8) {
-        *reinterpret_cast<uint4 *>(ov) = ldg_stream(o + at + c);
-        *reinterpret_cast<uint4 *>(dv) = *reinterpret_cast<const uint4 *>(d + at + c);
-        if (lo) *reinterpret_cast<uint4 *>(lv) = ldg_stream(lo + at + c);
-      } else {
-        ov[0] = o[at + c];
-        dv[0] = d[at + c];
-        if (lo) lv[0] = lo[at + c];
+      T ov[ROWS][VEC], lv[ROWS][VEC], dv[ROWS][VEC];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const int64_t t = t0 + r * 16;
+        if (t >= a.T) continue;
+        const int64_t at = (t * a.H + h) * a.D + c;
+        if constexpr (VEC == 8) {
+          *reinterpret_cast<uint4 *>(ov[r]) = ldg_stream(o + at);
+          *reinterpret_cast<uint4 *>(dv[r]) = *reinterpret_cast<const uint4 *>(d + at);
+          if (lo) *reinterpret_cast<uint4 *>(lv[r]) = ldg_stream(lo + at);
+        } else {
+          ov[r][0] = o[at];
+          dv[r][0] = d[at];
+          if (lo) lv[r][0] = lo[at];
+        }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        s = fmaf(to_f(ov[e]) + (lo ? to_f(lv[e]) : 0.f), to_f(dv[e]), s);
-        if (amax && inside) most_o = fmaxf(most_o, fabsf(to_f(dv[e])));
+      for (int r = 0; r < ROWS; ++r) {
+        const int64_t t = t0 + r * 16;
+        if (t >= a.T) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s[r] = fmaf(to_f(ov[r][e]) + (lo ? to_f(lv[r][e]) : 0.f), to_f(dv[r][e]), s[r]);
+          if (amax && t >= range.start && t < range.end) most_o = fmaxf(most_o, fabsf(to_f(dv[r][e])));
+        }
       }
     }
 #pragma unroll
-    for (int x = 8; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x, 16);
-    if (l == 0) a.delta[(int64_t)h * a.Tp + t] = s;
-    if (amax && inside && h < a.Hk)
-      for (int c = l; c < a.D; c += 16) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
+    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+      for (int x = 8; x; x >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], x, 16);
+      const int64_t t = t0 + r * 16;
+      if (t >= a.T) continue;
+      if (l == 0) a.delta[(int64_t)h * a.Tp + t] = s[r];
+      if (amax && t >= range.start && t < range.end && h < a.Hk)
+        for (int c = l; c < a.D; c += 16) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
+    }
   }
   if (amax) {
 #pragma unroll
@@ -480,9 +494,12 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
 
 int64_t mhc_attn_lse_pitch(int64_t T) { return T < 1 ? 0 : (T + 127) / 128 * 128; }
 
-// delta, the two orders of the work, the two maxima of fp16
-size_t mhc_attn_bwd_workspace(int64_t T, int H) {
-  return T < 1 || H < 1 ? 256 : (size_t)mhc_attn_lse_pitch(T) * H * 4 + 2 * attn_order_bytes(T) + 256;
+// delta, the two orders of the work, the two maxima of fp16, the parts of dK and dV
+size_t mhc_attn_bwd_workspace(int64_t T, int H, int Hk, int D) {
+  if (T < 1 || H < 1 || Hk < 1 || H % Hk || D < 1 || D > 128) return 256;
+  const int splits = attn_bwd_splits(T, H, Hk);
+  const size_t parts = splits > 1 ? (size_t)splits * 2 * T * Hk * D * 4 : 0;
+  return (size_t)mhc_attn_lse_pitch(T) * H * 4 + 2 * attn_order_bytes(T) + 256 + parts;
 }
 
 int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo, const void *dout,
@@ -501,8 +518,8 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
     return fail(MHC_ERR_NULL, "mhc_attn_bwd: required pointer is NULL");
   if (misaligned(dtype == MHC_F32 ? 4 : 2, {q, k, v, out, out_lo, dout, dq, dk, dv}) || ((uintptr_t)lse & 3))
     return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: a pointer is not aligned to its elements");
-  if (!workspace || workspace_bytes < mhc_attn_bwd_workspace(T, H))
-    return fail(MHC_ERR_WORKSPACE, "mhc_attn_bwd: workspace %zu < %zu bytes", workspace_bytes, mhc_attn_bwd_workspace(T, H));
+  if (!workspace || workspace_bytes < mhc_attn_bwd_workspace(T, H, Hk, D))
+    return fail(MHC_ERR_WORKSPACE, "mhc_attn_bwd: workspace %zu < %zu bytes", workspace_bytes, mhc_attn_bwd_workspace(T, H, Hk, D));
   if ((uintptr_t)workspace & 15) return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: workspace is not 16-byte aligned");
   a.delta = static_cast<float *>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -518,6 +535,9 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
   }
   if (e == cudaSuccess) e = launch_attn_delta(a, amax, st);
   if (e == cudaSuccess && tc) {
+    a.splits = attn_bwd_splits(T, H, Hk);
+    const uintptr_t at = (reinterpret_cast<uintptr_t>(order + 2 * on) + 8 + 15) & ~(uintptr_t)15;
+    a.parts = a.splits > 1 ? reinterpret_cast<float *>(at) : nullptr;
     e = launch_attn_bwd_tc(a, order, order + on, st);
     if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_bwd");
     cudaGetLastError();

@@ -22,6 +22,8 @@ struct Args {
   int batch;
   int64_t seqlen;
   float scale, scale_log2;
+  int splits;    // blocks that share a tile of keys in the backward, each with some of the group's heads
+  float *parts;  // their dK and dV: (splits, 2, T, Hk, D) fp32, where there are more than one
   int *err_flag;
 };
 

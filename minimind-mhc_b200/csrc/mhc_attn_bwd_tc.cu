@@ -61,6 +61,8 @@ enum { ERR_TMA = 51, ERR_MMA = 52, ERR_SOFTMAX = 53 };
 
 struct Item {
   int r0, head;   // first row, row head (DKV: key head)
+  int c_head;     // first column head
+  int part;       // DKV: which of the blocks that share the keys
   int c0, cols;   // first column tile's first token, column tiles
   int n;          // steps: cols, times the group's heads for DKV
   int done;
@@ -100,7 +102,10 @@ __device__ __forceinline__ bool item_of(const Args &a, const Sched &s, int64_t r
   }
   it.done = 0;
   const int at = (int)(rank / s.heads);
-  it.head = (int)(rank % s.heads);
+  const int p = (int)(rank % s.heads), G = a.H / a.Hk, per = DKV ? G / a.splits : 1;
+  it.head = DKV ? p / a.splits : p;
+  it.part = DKV ? p % a.splits : 0;
+  it.c_head = DKV ? it.head * G + it.part * per : p / G;
   const int tile = s.order ? s.order[at] : (DKV ? at : s.tiles - 1 - at);
   it.r0 = tile * TM;
   const int r1 = (int)min((int64_t)it.r0 + TM, a.T) - 1;
@@ -116,7 +121,7 @@ __device__ __forceinline__ bool item_of(const Args &a, const Sched &s, int64_t r
   }
   it.c0 = lo * TM;
   it.cols = hi - lo;
-  it.n = it.cols * (DKV ? a.H / a.Hk : 1);
+  it.n = it.cols * per;
   return true;
 }
 
@@ -159,7 +164,6 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
 #define WAIT_WARP(bar, par) (wait_warp_parity((bar), (par), abort_flag))
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
-  const int G = a.H / a.Hk;
 
   if (tid == 0) {
     abort_word = 0;
@@ -242,7 +246,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         const int s = g % ST;
         const uint32_t free_par = ((uint32_t)(g / ST) & 1u) ^ 1u;
         const int row = it.c0 + (j % it.cols) * TM;
-        const int head = DKV ? it.head * G + j / it.cols : it.head / G;
+        const int head = it.c_head + j / it.cols;
         if (!WAIT_WARP(BAR(B_1E + s), free_par)) { ok = false; break; }
         column(c1s + s * C::TILE, c1map, head, row, B_1F + s, DKV, head);
         if (!WAIT_WARP(BAR(B_2E + s), free_par)) { ok = false; break; }
@@ -409,7 +413,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     for (int i = 0; ok; ++i) {
       if (!WAIT_WARP(BAR(B_ITEM_F + (i & 1)), (uint32_t)(i >> 1) & 1u)) { ok = false; break; }
       const int r0 = items[i & 1].r0, head = items[i & 1].head, c00 = items[i & 1].c0, cols = items[i & 1].cols;
-      const int n = items[i & 1].n, done = items[i & 1].done;
+      const int n = items[i & 1].n, done = items[i & 1].done, split = items[i & 1].part;
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(B_ITEM_E + (i & 1)));
       if (done) break;
@@ -528,6 +532,15 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0u;
         }
+        if (DKV && a.splits > 1) {
+          float *pd = a.parts + ((int64_t)(split * 2 + second) * a.T * a.Hk * a.D) + at + d;
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            if (tok < a.T && d + h * 4 < a.D)
+              *reinterpret_cast<float4 *>(pd + h * 4) = make_float4(__uint_as_float(o[4 * h]) * mul, __uint_as_float(o[4 * h + 1]) * mul,
+                                                                    __uint_as_float(o[4 * h + 2]) * mul, __uint_as_float(o[4 * h + 3]) * mul);
+          continue;
+        }
         uint32_t w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * mul, __uint_as_float(o[2 * e + 1]) * mul);
@@ -558,7 +571,9 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         const int64_t tok = it.r0 + e / a.D;
         if (tok >= a.T) continue;
         const int64_t at = (tok * (DKV ? a.Hk : a.H) + it.head) * a.D + e % a.D;
-        if (DKV) {
+        if (DKV && a.splits > 1) {
+          for (int w = 0; w < 2; ++w) a.parts[(int64_t)(it.part * 2 + w) * a.T * a.Hk * a.D + at] = __int_as_float(0x7fc00000);
+        } else if (DKV) {
           static_cast<T *>(a.dk)[at] = bad;
           static_cast<T *>(a.dv)[at] = bad;
         } else {
@@ -571,8 +586,24 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
 #undef BAR
 }
 
+// dK and dV from the parts of the blocks that share their keys, in order
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const Args a) {
+  const int64_t n = a.T * a.Hk * a.D, quads = n / 4;  // D is a multiple of 8
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < 2 * quads; q += (int64_t)gridDim.x * 256) {
+    const int second = q >= quads;
+    const int64_t at = (q - second * quads) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < a.splits; ++p) {
+      const float4 v = __ldcs(reinterpret_cast<const float4 *>(a.parts + (int64_t)(p * 2 + second) * n + at));
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    *reinterpret_cast<uint2 *>(static_cast<T *>(second ? a.dv : a.dk) + at) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+  }
+}
+
 template <typename T, int DP, bool DKV>
-cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, const Map &c2, int *order, int sms,
+cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, const Map &c2, const int *order, int sms,
                 cudaStream_t stream) {
   using C = Cfg<DP>;
   constexpr size_t smem = 2 * C::TILE + C::ST * (2 * C::TILE + C::VEC) + 1024;
@@ -593,15 +624,10 @@ cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, cons
   }
   Sched s;
   s.tiles = (int)((a.T + TM - 1) / TM);
-  s.heads = DKV ? a.Hk : a.H;
+  s.heads = DKV ? a.Hk * a.splits : a.H;
   if ((int64_t)s.tiles * s.heads > 0x7fffffff) return cudaErrorNotSupported;
   s.items = s.tiles * s.heads;
-  s.order = nullptr;
-  if (s.items > sms) {  // with a block for every piece of work their order does not matter
-    e = launch_attn_order(a, DKV, order, stream);
-    if (e != cudaSuccess) return e;
-    s.order = order;
-  }
+  s.order = s.items > sms ? order : nullptr;  // with a block for every piece of work their order does not matter
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -619,6 +645,17 @@ cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, cons
 }  // namespace
 }  // namespace attn
 
+// Into how many the heads of a group are shared out where keys alone make too few
+// pieces of work: two for every SM or all heads apart.  (13 sequences, 8191 tokens, 8
+// heads over 2, D = 64: dK and dV in 166 us with 128 pieces, SPLIT_US with 512.)
+int attn_bwd_splits(int64_t T, int H, int Hk) {
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148, G = H / Hk;
+  const int64_t tiles = (T + attn::TM - 1) / attn::TM;
+  int s = 1;
+  while (s < G && (tiles * Hk * s < 2 * (int64_t)sms || G % s)) ++s;
+  return s;
+}
+
 cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream) {
   attn::Map q, k, v, d;
   const int64_t ot = (int64_t)a.H * a.D;
@@ -629,8 +666,16 @@ cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, 
   auto both = [&](auto tag, auto dim) -> cudaError_t {
     using T = decltype(tag);
     constexpr int DP = decltype(dim)::value;
-    const cudaError_t e = attn::run<T, DP, true>(a, k, v, q, d, order_k, sms, stream);
-    return e != cudaSuccess ? e : attn::run<T, DP, false>(a, q, d, k, v, order_q, sms, stream);
+    cudaError_t e = cudaSuccess;
+    // DQ has at least as many pieces of work as DKV
+    if ((a.T + attn::TM - 1) / attn::TM * a.H > sms) e = launch_attn_orders(a, order_q, order_k, stream);
+    if (e == cudaSuccess) e = attn::run<T, DP, true>(a, k, v, q, d, order_k, sms, stream);
+    if (e == cudaSuccess) e = attn::run<T, DP, false>(a, q, d, k, v, order_q, sms, stream);
+    if (e == cudaSuccess && a.splits > 1) {
+      attn::attn_join_kernel<T><<<grid_for(2 * a.T * a.Hk * a.D / 4, 256, sms, 8), 256, 0, stream>>>(a);
+      e = cudaGetLastError();
+    }
+    return e;
   };
   auto go = [&](auto tag) -> cudaError_t {
     if (a.D <= 32) return both(tag, IC<32>{});

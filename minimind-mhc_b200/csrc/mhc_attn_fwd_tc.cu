@@ -523,10 +523,13 @@ cudaError_t run(const Args &a, const Map &q, const Map &k, const Map &v, const S
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// Counting sort of the tiles by work, largest first, in one block.  Equal bins come
+// Counting sort of the tiles by work, largest first, one block each for queries (by
+// the keys they see) and keys (by the queries that see them).  Equal bins come
 // out in any order: the order decides who computes a tile, not what comes out.
 constexpr int BINS = 1024;
-__global__ void __launch_bounds__(BINS) attn_order_kernel(const Args a, int step, int tiles, int keys, int *order) {
+__global__ void __launch_bounds__(BINS) attn_order_kernel(const Args a, int step, int tiles, int *order_q, int *order_k) {
+  const int keys = blockIdx.x;  // 0: tiles of queries, 1: of keys
+  int *order = keys ? order_k : order_q;
   __shared__ int hist[BINS], warps[32], most;
   const int tid = threadIdx.x;
   hist[tid] = 0;
@@ -616,9 +619,9 @@ bool make_map(Map &map, const void *p, int dtype, int64_t T, int heads, int D, i
 
 size_t attn_order_bytes(int64_t T) { return (size_t)((T + attn::TM - 1) / attn::TM) * 4; }
 
-cudaError_t launch_attn_order(const attn::Args &a, int keys, int *order, cudaStream_t stream) {
+cudaError_t launch_attn_orders(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream) {
   const int tiles = (int)((a.T + attn::TM - 1) / attn::TM);
-  attn::attn_order_kernel<<<1, attn::BINS, 0, stream>>>(a, 1, tiles, keys, order);
+  attn::attn_order_kernel<<<2, attn::BINS, 0, stream>>>(a, 1, tiles, order_q, order_k);
   return cudaGetLastError();
 }
 
@@ -650,7 +653,7 @@ cudaError_t launch_attn_fwd_tc(const attn::Args &a, int *order, cudaStream_t str
   s.order = nullptr;
   // with a block for every piece of work their order does not matter
   if (s.items > sms && order) {
-    attn::attn_order_kernel<<<1, attn::BINS, 0, stream>>>(a, s.by_head ? 1 : 2, rows, 0, order);
+    attn::attn_order_kernel<<<1, attn::BINS, 0, stream>>>(a, s.by_head ? 1 : 2, rows, order, nullptr);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     s.order = order;

@@ -151,14 +151,13 @@ __device__ __forceinline__ int64_t snake(int i, int block, int blocks) {
 
 }  // namespace attn
 
-// tiles of 128 tokens in the order of their work, largest first: order[rank] = tile.
-// keys != 0: the work of a tile of keys (the queries that see it)
-cudaError_t launch_attn_order(const attn::Args &a, int keys, int *order, cudaStream_t stream);
-
+int attn_bwd_splits(int64_t T, int H, int Hk);
 bool attn_tc_eligible(const attn::Args &a);      // what both directions ask of q, k, v, out
 bool attn_tc_bwd_eligible(const attn::Args &a);
 size_t attn_order_bytes(int64_t T);
 cudaError_t launch_attn_fwd_tc(const attn::Args &a, int *order, cudaStream_t stream);
+// the two orders of the backward (queries, then keys) in one launch
+cudaError_t launch_attn_orders(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream);
 cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream);
 
 }  // namespace mhc

@@ -36,57 +36,80 @@ namespace router {
 constexpr int THREADS = 256;
 constexpr int MAX_E = 512;
 
-// order-preserving keys: larger value, then lower expert index, is the larger key;
-// 0 is below every key of a real logit
-__device__ __forceinline__ uint32_t order32(float v) {
-  if (v != v) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(v + 0.f);  // -0 and 0 are equal
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
+// Order-preserving keys: larger value, then lower expert index, is the larger key; 0
+// is below every key of a real logit.  The logit can be read back from its key.
 template <typename T>
-struct KeyOf {  // 16-bit logits: the upper 16 bits of the fp32 order (bf16) or the order of the half's own bits
+struct KeyOf {  // 16-bit logits: the order of their own bits above the reversed index
   using type = uint32_t;
-  static __device__ __forceinline__ uint32_t make(T x, float v, int e) {
-    uint32_t o;
-    if (v != v) {
-      o = 0xffffu;
-    } else if constexpr (sizeof(T) == 2) {
-      uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&x);
-      if (b == 0x8000u) b = 0;
-      o = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
-    }
+  static __device__ __forceinline__ uint32_t make(T x, int e) {
+    uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&x), o;
+    if (b == 0x8000u) b = 0;  // -0 and 0 are equal
+    o = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+    if (to_f(x) != to_f(x)) o = 0xffffu;
     return (o << 16) | (0xffffu - (uint32_t)e);
   }
   static __device__ __forceinline__ int expert(uint32_t k) { return (int)(0xffffu - (k & 0xffffu)); }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    const uint32_t o = k >> 16;
+    const uint16_t b = (uint16_t)((o & 0x8000u) ? (o & 0x7fffu) : ~o);
+    return to_f(*reinterpret_cast<const T *>(&b));
+  }
 };
 template <>
 struct KeyOf<float> {
   using type = unsigned long long;
-  static __device__ __forceinline__ unsigned long long make(float x, float v, int e) {
-    return ((unsigned long long)order32(v) << 32) | (0xffffffffu - (uint32_t)e);
+  static __device__ __forceinline__ unsigned long long make(float x, int e) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    const uint32_t o = x != x ? 0xffffffffu : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
+    return ((unsigned long long)o << 32) | (0xffffffffu - (uint32_t)e);
   }
   static __device__ __forceinline__ int expert(unsigned long long k) { return (int)(0xffffffffu - (uint32_t)k); }
+  static __device__ __forceinline__ float value(unsigned long long k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+  }
 };
 
+// largest first: bitonic network
+template <int V, typename K>
+__device__ __forceinline__ void sort_down(K (&k)[V]) {
+#pragma unroll
+  for (int size = 2; size <= V; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int j = i ^ d;
+        if (j > i) {
+          const bool down = (i & size) == 0;
+          const K hi = k[i] > k[j] ? k[i] : k[j], lo = k[i] > k[j] ? k[j] : k[i];
+          k[i] = down ? hi : lo;
+          k[j] = down ? lo : hi;
+        }
+      }
+}
+
+// Over the G lanes of a group.  Whole warps run these (a group past the last token
+// repeats it): with a mask for each group the groups of a warp would take turns.
 template <int G, typename K>
-__device__ __forceinline__ K group_max(K v, unsigned mask) {
+__device__ __forceinline__ K group_max(K v) {
 #pragma unroll
   for (int o = G / 2; o; o >>= 1) {
-    const K w = __shfl_xor_sync(mask, v, o);
+    const K w = __shfl_xor_sync(0xffffffffu, v, o);
     v = w > v ? w : v;
   }
   return v;
 }
 template <int G>
-__device__ __forceinline__ float group_maxf(float v, unsigned mask) {
+__device__ __forceinline__ float group_maxf(float v) {
 #pragma unroll
-  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
+  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 template <int G>
-__device__ __forceinline__ float group_sum(float v, unsigned mask) {
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -109,26 +132,28 @@ __device__ __forceinline__ void load_logits(const T *row, int e0, int E, bool ve
 }
 
 // softmax of the group's row; lanes past E hold p = 0.  An all -inf row gives 0.
+// p = exp(z - base) * scale for any logit z of the row.
 template <typename T, int G, int V>
-__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, unsigned mask, float (&p)[V]) {
+__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, float (&p)[V], float &base,
+                                            float &scale) {
   float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     p[i] = e0 + i < E ? to_f(x[i]) : -INFINITY;
     mx = fmaxf(mx, p[i]);
   }
-  mx = group_maxf<G>(mx, mask);
-  const float base = mx == -INFINITY ? 0.f : mx;
+  mx = group_maxf<G>(mx);
+  base = mx == -INFINITY ? 0.f : mx;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     p[i] = expf(p[i] - base);  // +inf logits: inf - inf = NaN, as the quotient would be
     sum += p[i];
   }
-  sum = group_sum<G>(sum, mask);
-  const float r = sum == 0.f ? 0.f : 1.f / sum;
+  sum = group_sum<G>(sum);
+  scale = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int i = 0; i < V; ++i) p[i] *= r;
+  for (int i = 0; i < V; ++i) p[i] *= scale;
 }
 
 struct Args {
@@ -164,7 +189,6 @@ __global__ void __launch_bounds__(THREADS) route_fwd_kernel(Args a, float *w, in
   __shared__ int64_t sh_cnt[G * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gl = lane % G, e0 = gl * V;
-  const unsigned mask = G == 32 ? 0xffffffffu : (((1u << (G & 31)) - 1u) << (lane / G * G));
   float col[V];
   int cnt[V];
 #pragma unroll
@@ -173,57 +197,60 @@ __global__ void __launch_bounds__(THREADS) route_fwd_kernel(Args a, float *w, in
     cnt[i] = 0;
   }
   const T *z = static_cast<const T *>(a.z);
-  for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; t < a.T; t += (int64_t)gridDim.x * ROWS) {
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  T next[V];
+  auto fetch = [&](int64_t t) { load_logits<T, V>(z + (t < a.T ? t : a.T - 1) * a.row_stride, e0, a.E, a.vec, next); };
+  fetch((int64_t)blockIdx.x * ROWS + threadIdx.x / G);
+  for (int64_t tb = (int64_t)blockIdx.x * ROWS; tb < a.T; tb += stride) {
+    const int64_t t = tb + threadIdx.x / G;
+    const bool live = t < a.T;
     T x[V];
-    load_logits<T, V>(z + t * a.row_stride, e0, a.E, a.vec, x);
-    float p[V];
-    softmax_row<T, G, V>(x, e0, a.E, mask, p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = next[i];
+    if (tb + stride < a.T) fetch(t + stride);
+    float p[V], base, scale;
+    softmax_row<T, G, V>(x, e0, a.E, p, base, scale);
     K key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      key[i] = e0 + i < a.E ? Key::make(x[i], to_f(x[i]), e0 + i) : (K)0;
-      col[i] += p[i];
+      key[i] = e0 + i < a.E ? Key::make(x[i], e0 + i) : (K)0;
+      col[i] += live ? p[i] : 0.f;
     }
-    // the j-th choice is kept by lane j % G of the group, in slot j / G (k <= E <= G V: V slots are enough)
-    float top[V];
-    int exp_[V];
+    // a lane's keys in order, so that only its first can be the next choice.  The j-th choice is kept by lane j % G of
+    // the group, in slot j / G (k <= E <= G V: V slots are enough).
+    sort_down<V, K>(key);
+    K top[V];
     unsigned chosen = 0;
-    float total = 0.f;
 #pragma unroll
     for (int s = 0; s < V; ++s) {
-      top[s] = 0.f;
-      exp_[s] = 0;
+      top[s] = 0;
       for (int r = 0; r < G && s * G + r < a.k; ++r) {
-        K best = key[0];
+        const K best = group_max<G, K>(key[0]);
+        if (key[0] == best) {
+          chosen |= 1u << (Key::expert(best) - e0);
 #pragma unroll
-        for (int i = 1; i < V; ++i) best = key[i] > best ? key[i] : best;
-        best = group_max<G, K>(best, mask);
-        float pe = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (key[i] == best) {
-            key[i] = 0;
-            chosen |= 1u << i;
-            pe = p[i];
-          }
-        const int e = Key::expert(best);
-        if constexpr (G > 1) pe = __shfl_sync(mask, pe, e / V, G);
-        total += pe;
-        if (gl == r) {
-          top[s] = pe;
-          exp_[s] = e;
+          for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+          key[V - 1] = 0;
         }
+        if (gl == r) top[s] = best;
       }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) cnt[i] += (chosen >> i) & 1u;
-    total += 1e-20f;
+    for (int i = 0; i < V; ++i) cnt[i] += live ? (chosen >> i) & 1u : 0u;
+    float pe[V], total = 0.f;
+#pragma unroll
+    for (int s = 0; s < V; ++s) {
+      pe[s] = 0.f;
+      if (s * G + gl < a.k) pe[s] = expf(Key::value(top[s]) - base) * scale;
+      total += pe[s];
+    }
+    total = group_sum<G>(total) + 1e-20f;
 #pragma unroll
     for (int s = 0; s < V; ++s) {
       const int j = s * G + gl;
-      if (j < a.k) {
-        w[t * a.k + j] = top[s] / total;  // k = 1: exactly 1
-        idx[t * a.k + j] = exp_[s];
+      if (live && j < a.k) {
+        w[t * a.k + j] = pe[s] / total;  // k = 1: exactly 1
+        idx[t * a.k + j] = Key::expert(top[s]);
       }
     }
   }
@@ -303,39 +330,54 @@ __global__ void __launch_bounds__(THREADS) route_bwd_kernel(Args a, const float 
   constexpr int ROWS = THREADS / G;
   const int lane = threadIdx.x & 31;
   const int gl = lane % G, e0 = gl * V;
-  const unsigned mask = G == 32 ? 0xffffffffu : (((1u << (G & 31)) - 1u) << (lane / G * G));
   float load[V];
   const double f = dloss ? (double)*dloss * (double)a.scale / ((double)a.T * (double)a.T) : 0.0;
 #pragma unroll
   for (int i = 0; i < V; ++i) load[i] = dloss && e0 + i < a.E ? (float)(f * (double)counts[e0 + i]) : 0.f;
   const T *z = static_cast<const T *>(a.z);
-  for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; t < a.T; t += (int64_t)gridDim.x * ROWS) {
+  for (int64_t tb = (int64_t)blockIdx.x * ROWS; tb < a.T; tb += (int64_t)gridDim.x * ROWS) {
+    const bool live = tb + threadIdx.x / G < a.T;
+    const int64_t t = live ? tb + threadIdx.x / G : a.T - 1;
     T x[V];
     load_logits<T, V>(z + t * a.row_stride, e0, a.E, a.vec, x);
-    float p[V], dp[V];
-    softmax_row<T, G, V>(x, e0, a.E, mask, p);
+    float p[V], dp[V], base, scale;
+    softmax_row<T, G, V>(x, e0, a.E, p, base, scale);
 #pragma unroll
     for (int i = 0; i < V; ++i) dp[i] = load[i];
     if (dw) {
-      float dot = 0.f, own = 0.f;
-      for (int j = 0; j < a.k; ++j) dot = fmaf(dw[t * a.k + j], w[t * a.k + j], dot);
-      for (int j = 0; j < a.k; ++j) {
-        const int e = (int)idx[t * a.k + j];
+      // lane j % G has the j-th choice: its gradient, its weight and the probability of its expert
+      int es[V];
+      float ds[V], dot = 0.f, total = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) own += e == e0 + i ? p[i] : 0.f;
+      for (int s = 0; s < V; ++s) {
+        const int j = s * G + gl;
+        es[s] = -1;
+        ds[s] = 0.f;
+        if (j < a.k) {
+          es[s] = (int)idx[t * a.k + j];
+          ds[s] = dw[t * a.k + j];
+          dot = fmaf(ds[s], w[t * a.k + j], dot);
+          total += expf(to_f(z[t * a.row_stride + es[s]]) - base) * scale;
+        }
       }
-      const float inv = 1.f / (group_sum<G>(own, mask) + 1e-20f);
-      for (int j = 0; j < a.k; ++j) {
-        const int e = (int)idx[t * a.k + j];
-        const float d = (dw[t * a.k + j] - dot) * inv;
+      dot = group_sum<G>(dot);
+      const float inv = 1.f / (group_sum<G>(total) + 1e-20f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) dp[i] += e == e0 + i ? d : 0.f;
+      for (int s = 0; s < V; ++s) {
+        ds[s] = (ds[s] - dot) * inv;
+        for (int r = 0; r < G && s * G + r < a.k; ++r) {
+          const int e = G == 1 ? es[s] : __shfl_sync(0xffffffffu, es[s], r, G);
+          const float d = G == 1 ? ds[s] : __shfl_sync(0xffffffffu, ds[s], r, G);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dp[i] += e == e0 + i ? d : 0.f;
+        }
       }
     }
     float pd = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) pd = fmaf(p[i], dp[i], pd);
-    pd = group_sum<G>(pd, mask);
+    pd = group_sum<G>(pd);
+    if (!live) continue;  // the last round
     T *out = dz + t * a.E + e0;
     constexpr int PER = 16 / (int)sizeof(T);
     T o[V];
@@ -398,8 +440,9 @@ static int check_router(const char *who, int64_t T, int E, int k, int dtype, int
 extern "C" {
 
 size_t mhc_route_fwd_workspace(int64_t T, int E) {
-  if (T < 1 || E < 1 || E > router::MAX_E) return 256;
-  return (size_t)router::blocks_for(T, E, device_sm_count()) * (size_t)E * 8 + 256;
+  if (T < 1 || E < 1 || E > router::MAX_E) return 0;
+  const int blocks = router::blocks_for(T, E, device_sm_count());
+  return blocks > 1 ? (size_t)blocks * (size_t)E * 8 : 0;  // one block keeps its sums to itself
 }
 
 int mhc_route_fwd(const void *logits, int dtype, int64_t T, int E, int64_t row_stride, int k, float coef, float *weights,

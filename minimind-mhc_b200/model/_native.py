@@ -58,7 +58,7 @@ _PROTOS = {
     "mhc_attn_lse_pitch": (_I64, [_I64]),
     "mhc_attn_fwd_workspace": (_SZ, [_I64]),
     "mhc_attn_fwd": (_I, [_P, _P, _P, _I, _I64, _I, _I, _I, _P, _P, _I, _I64, _F, _P, _P, _P, _P, _SZ, _P]),
-    "mhc_attn_bwd_workspace": (_SZ, [_I64, _I]),
+    "mhc_attn_bwd_workspace": (_SZ, [_I64, _I, _I, _I]),
     "mhc_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I, _I, _I, _P, _P, _I, _I64, _F, _P, _P, _P, _P, _SZ,
                           _P]),
     "mhc_route_fwd_workspace": (_SZ, [_I64, _I]),
@@ -127,6 +127,33 @@ def ptr(t):
 
 def stream_of(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+# The raw handle without building a Stream object (2.2 us a call on the host
+# side of a small operator), where torch has the accessor.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int):
+    """The current stream's handle on device ``index``."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def call_on(index: int, name: str, *args):
+    """``call`` with device ``index`` current and its current stream as the last argument."""
+    if torch.cuda.current_device() == index:
+        call(name, *args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, raw_stream(index))
+
+
+def refuse_double_backward(what: str):
+    """For a backward that autograd must not differentiate again: grad mode is on there only under create_graph."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: second derivatives are not implemented")
 
 
 def require_cuda(*ts):

@@ -16,9 +16,10 @@ is 2.03 bytes a value instead of 8.
 
 from __future__ import annotations
 
+from array import array
+from itertools import chain, repeat
 from typing import NamedTuple
 
-import numpy as np
 import torch
 
 from . import _native as nat
@@ -55,26 +56,21 @@ def unpack_moment(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     if scales.device != codes.device:
         raise ValueError("unpack_moment: codes and scales are on different devices")
     codes, scales = codes.contiguous(), scales.contiguous()
-    with torch.cuda.device(codes.device):
-        out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
-        nat.call("mhc_adamw_unpack", codes.data_ptr(), int(codes.dtype == torch.int8), scales.data_ptr(),
-                 out.data_ptr(), n, nat.stream_of(codes))
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    nat.call_on(codes.get_device(), "mhc_adamw_unpack", codes.data_ptr(), int(codes.dtype == torch.int8),
+                scales.data_ptr(), out.data_ptr(), n)
     return out
 
 
-def _pointers(ts):
-    return list(map(_Tensor.data_ptr, ts))
-
-
-def _check_list(what, ts, sizes, device, dtypes):
+def _check_list(what, ts, sizes, index, dtypes):
     if len(ts) != len(sizes):
         raise ValueError(f"adamw: {len(sizes)} params but {len(ts)} {what}")
     found = {t.dtype for t in ts}
     if not found <= dtypes:
         raise TypeError(f"adamw: {what} must be {' / '.join(sorted(str(d) for d in dtypes))}, got "
                         f"{', '.join(sorted(str(d) for d in found - dtypes))}")
-    if {t.device for t in ts} != {device}:
-        raise ValueError(f"adamw: every tensor must be on {device}; {what} are not")
+    if set(map(_Tensor.get_device, ts)) != {index}:
+        raise ValueError(f"adamw: every tensor must be on cuda:{index}; {what} are not")
     if not all(map(_Tensor.is_contiguous, ts)):
         raise ValueError(f"adamw: {what} must be contiguous")
     if list(map(_Tensor.numel, ts)) != sizes:
@@ -83,54 +79,67 @@ def _check_list(what, ts, sizes, device, dtypes):
 
 _FLOATS = frozenset(_CODE)
 _F32 = frozenset((torch.float32,))
+_POINTER = _Tensor.data_ptr
+_WORDS = 9  # of 8 bytes, one mhc_adamw_tensor
 
 
 def _table(params, grads, ms, vs, steps, bits):
-    """The host array of ``mhc_adamw_tensor`` (9 words each) of checked tensors."""
+    """The host array of ``mhc_adamw_tensor`` of checked tensors."""
     count = len(params)
     if len(grads) != count or len(ms) != count or len(vs) != count:
         raise ValueError(f"adamw: {count} params, {len(grads)} grads, {len(ms)} and {len(vs)} moments")
-    device = params[0].device
     nat.require_cuda(params[0])
+    index = params[0].get_device()
     sizes = list(map(_Tensor.numel, params))
-    _check_list("params", params, sizes, device, _FLOATS)
-    _check_list("grads", grads, sizes, device, _FLOATS)
-    table = np.zeros((count, 9), dtype=np.uint64)
-    table[:, 0] = _pointers(params)
-    table[:, 1] = _pointers(grads)
+    _check_list("params", params, sizes, index, _FLOATS)
+    _check_list("grads", grads, sizes, index, _FLOATS)
     if bits == 32:
-        _check_list("exp_avgs", ms, sizes, device, _F32)
-        _check_list("exp_avg_sqs", vs, sizes, device, _F32)
-        table[:, 2] = _pointers(ms)
-        table[:, 3] = _pointers(vs)
+        _check_list("exp_avgs", ms, sizes, index, _F32)
+        _check_list("exp_avg_sqs", vs, sizes, index, _F32)
+        moments = (map(_POINTER, ms), map(_POINTER, vs), repeat(0), repeat(0))
     else:
-        scales = [-(-n // QUANT_BLOCK) for n in sizes]
-        for col, what, pairs, dt in ((2, "exp_avgs", ms, torch.int8), (3, "exp_avg_sqs", vs, torch.uint8)):
-            codes, sc = [m[0] for m in pairs], [m[1] for m in pairs]
-            _check_list(what + " codes", codes, sizes, device, frozenset((dt,)))
-            _check_list(what + " scales", sc, scales, device, _F32)
-            table[:, col] = _pointers(codes)
-            table[:, col + 2] = _pointers(sc)
-    table[:, 6] = sizes
-    table[:, 7] = steps
-    types = table.view(np.int32)[:, 16:18]
-    types[:, 0] = [_CODE[p.dtype] for p in params]
-    types[:, 1] = [_CODE[g.dtype] for g in grads]
-    return table
+        blocks = [-(-n // QUANT_BLOCK) for n in sizes]
+        moments = []
+        for what, pairs, dt in (("exp_avgs", ms, torch.int8), ("exp_avg_sqs", vs, torch.uint8)):
+            codes, scales = [m[0] for m in pairs], [m[1] for m in pairs]
+            _check_list(what + " codes", codes, sizes, index, frozenset((dt,)))
+            _check_list(what + " scales", scales, blocks, index, _F32)
+            moments += [map(_POINTER, codes), map(_POINTER, scales)]
+        moments = (moments[0], moments[2], moments[1], moments[3])
+    types = [_CODE[p.dtype] | _CODE[g.dtype] << 32 for p, g in zip(params, grads)]
+    steps = steps if isinstance(steps, (list, tuple)) else repeat(int(steps))
+    rows = zip(map(_POINTER, params), map(_POINTER, grads), *moments, sizes, steps, types)
+    return array("Q", chain.from_iterable(rows))
 
 
-def _grad_norm(tables, device):
+def _grad_norm(tables, index):
     """The workspace that holds the squared norm of all the tables' gradients."""
-    ws = nat.workspace(nat.lib().mhc_grad_norm_workspace(), device)
+    ws = nat.workspace(nat.lib().mhc_grad_norm_workspace(), torch.device("cuda", index))
     for i, t in enumerate(tables):
-        nat.call("mhc_grad_norm", t.ctypes.data, len(t), int(i > 0), ws.data_ptr(), ws.numel(),
-                 torch.cuda.current_stream(device).cuda_stream)
+        nat.call("mhc_grad_norm", t.buffer_info()[0], len(t) // _WORDS, int(i > 0), ws.data_ptr(), ws.numel(),
+                 nat.raw_stream(index))
     return ws
 
 
-def _run(table, bits, device, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm):
-    nat.call("mhc_adamw_step", table.ctypes.data, len(table), bits, lr, betas[0], betas[1], eps, weight_decay,
-             max_grad_norm or 0.0, nat.ptr(norm_ws), nat.ptr(norm), torch.cuda.current_stream(device).cuda_stream)
+def _run(table, bits, index, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm):
+    nat.call("mhc_adamw_step", table.buffer_info()[0], len(table) // _WORDS, bits, lr, betas[0], betas[1], eps,
+             weight_decay, max_grad_norm or 0.0, nat.ptr(norm_ws), nat.ptr(norm), nat.raw_stream(index))
+
+
+def _run_all(tables, bits, index, max_grad_norm):
+    """Steps the (table, hyperparameters) pairs under one norm; returns it."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _run_all(tables, bits, index, max_grad_norm)
+    norm_ws = norm = None
+    if max_grad_norm is not None:
+        norm_ws = _grad_norm([t for t, _ in tables], index)
+        # written by the step, unless there is nothing to step
+        make = torch.empty if any(any(t[6::_WORDS]) for t, _ in tables) else torch.zeros
+        norm = make((), dtype=torch.float32, device=norm_ws.device)
+    for table, hyper in tables:
+        _run(table, bits, index, *hyper, max_grad_norm, norm_ws, norm)
+    return norm
 
 
 def _check_call(max_grad_norm):
@@ -146,14 +155,7 @@ def _step(params, grads, ms, vs, bits, step, lr, betas, eps, weight_decay, max_g
     if not params:
         return None
     table = _table(params, grads, ms, vs, step, bits)
-    device = params[0].device
-    with torch.cuda.device(device):
-        norm_ws = norm = None
-        if max_grad_norm is not None:
-            norm_ws = _grad_norm([table], device)
-            norm = torch.zeros((), dtype=torch.float32, device=device)
-        _run(table, bits, device, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm)
-    return norm
+    return _run_all([(table, (lr, betas, eps, weight_decay))], bits, params[0].get_device(), max_grad_norm)
 
 
 @torch.no_grad()
@@ -232,22 +234,16 @@ class AdamW(torch.optim.Optimizer):
             else:
                 ms = [(s["exp_avg"], s["exp_avg_scale"]) for s in mine]
                 vs = [(s["exp_avg_sq"], s["exp_avg_sq_scale"]) for s in mine]
-            work.append((group, _table(live, grads, ms, vs, [s["step"] + 1 for s in mine], self.state_bits)))
+            work.append((_table(live, grads, ms, vs, [s["step"] + 1 for s in mine], self.state_bits),
+                         (group["lr"], group["betas"], group["eps"], group["weight_decay"])))
             states += mine
-            keep.append((live[0].device, grads))
+            keep.append((live[0].get_device(), grads))
         if not work:
             return loss
-        device = keep[0][0]
-        if any(d != device for d, _ in keep):
+        index = keep[0][0]
+        if any(d != index for d, _ in keep):
             raise ValueError("AdamW: all parameters must be on one device")
-        with torch.cuda.device(device):
-            norm_ws = norm = None
-            if self.max_grad_norm is not None:
-                norm_ws = _grad_norm([t for _, t in work], device)
-                self.grad_norm = norm = torch.zeros((), dtype=torch.float32, device=device)
-            for group, table in work:
-                _run(table, self.state_bits, device, group["lr"], group["betas"], group["eps"],
-                     group["weight_decay"], self.max_grad_norm, norm_ws, norm)
+        self.grad_norm = _run_all(work, self.state_bits, index, self.max_grad_norm)
         for s in states:
             s["step"] += 1
         return loss

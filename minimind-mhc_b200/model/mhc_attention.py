@@ -21,8 +21,16 @@ from . import _native as nat
 
 
 def _rows(x):
-    """x (T, heads, D) with contiguous rows: the kernels take any token and head strides."""
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+    """x (T, heads, D) as the kernels read it: any token and head strides, but contiguous rows, and for 16-bit types
+    what TMA can address (rows that begin at multiples of 16 bytes, heads that do not overlap), where a copy costs less
+    than the kernels that do without."""
+    st, sh, sd = x.stride()
+    t, h, d = x.shape
+    if sd != 1 and d != 1:
+        return x.contiguous()
+    if x.element_size() == 2 and d % 8 == 0 and (st % 8 or sh % 8 or x.data_ptr() % 16 or (h > 1 and sh < d)):
+        return x.contiguous()
+    return x
 
 
 class _PackedAttentionFn(torch.autograd.Function):
@@ -32,40 +40,39 @@ class _PackedAttentionFn(torch.autograd.Function):
         t, h, d = q.shape
         hk = k.shape[1]
         q, k, v = _rows(q), _rows(k), _rows(v)
-        dev = q.device
-        with torch.cuda.device(dev):
-            out = torch.empty(t, h, d, dtype=q.dtype, device=dev)
-            # the backward's row sums use out before its rounding to 16 bits
-            out_lo = torch.empty_like(out) if any(ctx.needs_input_grad) and q.dtype != torch.float32 else None
-            lse = torch.empty(h, nat.lib().mhc_attn_lse_pitch(t), dtype=torch.float32, device=dev)
-            strides = (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-                                           v.stride(1))
-            batch = 0 if cu is None else cu.numel() - 1
-            ws = nat.workspace(nat.lib().mhc_attn_fwd_workspace(t), dev)
-            nat.call("mhc_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.dtype_code(q.dtype), t, h, hk, d,
-                     strides, nat.ptr(cu), batch, seqlen, scale, out.data_ptr(), nat.ptr(out_lo), lse.data_ptr(),
-                     ws.data_ptr(), ws.numel(), nat.stream_of(q))
-        ctx.save_for_backward(q, k, v, cu, out, out_lo, lse)
-        ctx.meta = (strides, batch, seqlen, scale)
+        index = q.get_device()
+        out = q.new_empty((t, h, d))
+        # the backward's row sums use out before its rounding to 16 bits
+        out_lo = q.new_empty((t, h, d)) if any(ctx.needs_input_grad) and q.dtype != torch.float32 else None
+        lib = nat.lib()
+        lse = q.new_empty((h, lib.mhc_attn_lse_pitch(t)), dtype=torch.float32)
+        strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+        batch = 0 if cu is None else cu.numel() - 1
+        need = lib.mhc_attn_fwd_workspace(t)
+        ws = q.new_empty((need,), dtype=torch.uint8)
+        nat.call_on(index, "mhc_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.dtype_code(q.dtype), t, h,
+                    hk, d, strides, nat.ptr(cu), batch, seqlen, scale, out.data_ptr(), nat.ptr(out_lo),
+                    lse.data_ptr(), ws.data_ptr(), need)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(q, k, v, cu, out, out_lo, lse)
+            ctx.meta = (strides, batch, seqlen, scale)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        nat.refuse_double_backward("packed_attention")
         q, k, v, cu, out, out_lo, lse = ctx.saved_tensors
         strides, batch, seqlen, scale = ctx.meta
         t, h, d = q.shape
         hk = k.shape[1]
-        dev = q.device
         dout = dout.contiguous()
-        with torch.cuda.device(dev):
-            dq = torch.empty(t, h, d, dtype=q.dtype, device=dev)
-            dk = torch.empty(t, hk, d, dtype=q.dtype, device=dev)
-            dv = torch.empty(t, hk, d, dtype=q.dtype, device=dev)
-            ws = nat.workspace(nat.lib().mhc_attn_bwd_workspace(t, h), dev)
-            nat.call("mhc_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                     nat.ptr(out_lo), dout.data_ptr(), lse.data_ptr(), nat.dtype_code(q.dtype), t, h, hk, d, strides, nat.ptr(cu), batch, seqlen, scale,
-                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(q))
+        dq, dk, dv = q.new_empty((t, h, d)), q.new_empty((t, hk, d)), q.new_empty((t, hk, d))
+        need = nat.lib().mhc_attn_bwd_workspace(t, h, hk, d)
+        ws = q.new_empty((need,), dtype=torch.uint8)
+        nat.call_on(q.get_device(), "mhc_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                    nat.ptr(out_lo), dout.data_ptr(), lse.data_ptr(), nat.dtype_code(q.dtype), t, h, hk, d, strides,
+                    nat.ptr(cu), batch, seqlen, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                    need)
         return dq, dk, dv, None, None, None
 
 

@@ -31,18 +31,17 @@ class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, coef):
         t, e = logits.shape
-        dev = logits.device
         z = logits if t == 0 or (logits.stride(1) == 1 and logits.stride(0) >= e) else logits.contiguous()
         rs = z.stride(0) if t > 1 else e
-        with torch.cuda.device(dev):
-            weights = torch.empty(t, k, dtype=torch.float32, device=dev)
-            experts = torch.empty(t, k, dtype=torch.int64, device=dev)
-            counts = torch.empty(e, dtype=torch.int64, device=dev)
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            ws = nat.workspace(nat.lib().mhc_route_fwd_workspace(t, e), dev)
-            nat.call("mhc_route_fwd", z.data_ptr(), nat.dtype_code(z.dtype), t, e, rs, k, coef, weights.data_ptr(),
-                     experts.data_ptr(), counts.data_ptr(), loss.data_ptr(), ws.data_ptr(), ws.numel(),
-                     nat.stream_of(z))
+        index = z.get_device()
+        weights = z.new_empty((t, k), dtype=torch.float32)
+        experts = z.new_empty((t, k), dtype=torch.int64)
+        counts = z.new_empty((e,), dtype=torch.int64)
+        loss = z.new_empty((), dtype=torch.float32)
+        need = nat.lib().mhc_route_fwd_workspace(t, e)
+        ws = z.new_empty((need,), dtype=torch.uint8) if need else None
+        nat.call_on(index, "mhc_route_fwd", z.data_ptr(), nat.dtype_code(z.dtype), t, e, rs, k, coef,
+                    weights.data_ptr(), experts.data_ptr(), counts.data_ptr(), loss.data_ptr(), nat.ptr(ws), need)
         ctx.save_for_backward(z, weights, experts, counts)
         ctx.meta = (k, coef, rs)
         ctx.mark_non_differentiable(experts, counts)
@@ -50,22 +49,21 @@ class _RouteFn(torch.autograd.Function):
         return weights, experts, counts, loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dw, _experts, _counts, dloss):
+        nat.refuse_double_backward("route_topk")
+        if dw is None and dloss is None:
+            return None, None, None
         z, weights, experts, counts = ctx.saved_tensors
         k, coef, rs = ctx.meta
         t, e = z.shape
-        if dw is None and dloss is None:
-            return None, None, None
         if dw is not None:
             dw = dw.to(torch.float32).contiguous()
         if dloss is not None:
-            dloss = dloss.to(torch.float32).contiguous()
-        with torch.cuda.device(z.device):
-            dz = torch.empty(t, e, dtype=z.dtype, device=z.device)
-            nat.call("mhc_route_bwd", z.data_ptr(), nat.dtype_code(z.dtype), t, e, rs, k, coef, weights.data_ptr(),
-                     experts.data_ptr(), counts.data_ptr(), nat.ptr(dw), nat.ptr(dloss), dz.data_ptr(),
-                     nat.stream_of(z))
+            dloss = dloss.to(torch.float32)
+        dz = z.new_empty((t, e))
+        nat.call_on(z.get_device(), "mhc_route_bwd", z.data_ptr(), nat.dtype_code(z.dtype), t, e, rs, k, coef,
+                    weights.data_ptr(), experts.data_ptr(), counts.data_ptr(), nat.ptr(dw), nat.ptr(dloss),
+                    dz.data_ptr())
         return dz, None, None
 
 
