@@ -176,10 +176,13 @@ __device__ __forceinline__ uint2 load_codes(const void *p, int64_t base, int64_t
   }
   return make_uint2(w[0], w[1]);
 }
+// through the low bits of 2^23 (byte 0x4B, then the code): the integer conversions and
+// rounding instructions run at the special function unit's rate, which the roots need
 template <bool SIGNED>
 __device__ __forceinline__ float code_value(const uint2 &w, int e) {
-  const uint32_t b = ((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu;
-  return SIGNED ? (float)(int)(int8_t)b : (float)b;
+  const uint32_t word = SIGNED ? (e < 4 ? w.x : w.y) ^ 0x80808080u : (e < 4 ? w.x : w.y);
+  const float f = __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650u | (e & 3)));
+  return f - (SIGNED ? 8388736.f : 8388608.f);
 }
 __device__ __forceinline__ void store_codes(void *p, int64_t base, int64_t n, bool whole, int lane, const int (&c)[8]) {
   uint8_t *q = static_cast<uint8_t *>(p);
@@ -237,10 +240,12 @@ __device__ __forceinline__ void pack_codes(const float (&x)[8], float safe, floa
   for (int e = 0; e < 8; ++e) {
     const float q = fabsf(x[e]) * inv;
     const float y = SIGNED ? sqrt_approx(q) * 127.f : sqrt_approx(sqrt_approx(q)) * 255.f;
-    const float r = rintf(y);
-    near |= !(fabsf(y - r) < 0.5f - EDGE);  // NaN too
-    c[e] = __float2int_rn(SIGNED && x[e] < 0.f ? -r : r);
-    if (!SIGNED && x[e] > 0.f && c[e] < 1) c[e] = 1;
+    const float t = y + 12582912.f;  // 1.5 * 2^23: rounds to the nearest integer, held in the low bits
+    near |= !(fabsf(y - (t - 12582912.f)) < 0.5f - EDGE);  // NaN too
+    int k = (int)(__float_as_uint(t) & 0xffu);
+    if (SIGNED && x[e] < 0.f) k = -k;
+    if (!SIGNED && x[e] > 0.f && k < 1) k = 1;
+    c[e] = k;
   }
   if (near) {
 #pragma unroll 1
@@ -286,7 +291,7 @@ __device__ __forceinline__ float clip_factor(const Scalars &s) {
 }
 
 template <int N, bool Q8>
-__global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ Table<N> tab, const Scalars s) {
+__global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant__ Table<N> tab, const Scalars s) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float clip = 1.f;
   if (s.partials) clip = clip_factor(s);

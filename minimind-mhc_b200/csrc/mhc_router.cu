@@ -42,11 +42,19 @@ template <typename T>
 struct KeyOf {  // 16-bit logits: the order of their own bits above the reversed index
   using type = uint32_t;
   static __device__ __forceinline__ uint32_t make(T x, int e) {
-    uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&x), o;
-    if (b == 0x8000u) b = 0;  // -0 and 0 are equal
-    o = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
-    if (to_f(x) != to_f(x)) o = 0xffffu;
-    return (o << 16) | (0xffffu - (uint32_t)e);
+    const uint32_t low = 0xffffu - (uint32_t)e;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // bf16 is the upper half of an fp32
+      const float v = to_f(x) + 0.f;                        // -0 and 0 are equal
+      const uint32_t b = __float_as_uint(v);
+      const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+      return ((v == v ? o : 0xffffffffu) & 0xffff0000u) | low;
+    } else {
+      uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&x);
+      if (b == 0x8000u) b = 0;
+      uint32_t o = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+      if (to_f(x) != to_f(x)) o = 0xffffu;
+      return (o << 16) | low;
+    }
   }
   static __device__ __forceinline__ int expert(uint32_t k) { return (int)(0xffffu - (k & 0xffffu)); }
   static __device__ __forceinline__ float value(uint32_t k) {
@@ -131,11 +139,19 @@ __device__ __forceinline__ void load_logits(const T *row, int e0, int E, bool ve
   }
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float LOG2E = 1.44269504088896340736f;
+
 // softmax of the group's row; lanes past E hold p = 0.  An all -inf row gives 0.
-// p = exp(z - base) * scale for any logit z of the row.
+// p = exp2(z log2(e) - base) * scale for any logit z of the row: one FMA and the
+// special function's 2^x (2 ulp) in place of expf's 9 instructions.  The rounding of
+// base is common to the row and leaves p with its sum.
 template <typename T, int G, int V>
-__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, float (&p)[V], float &base,
-                                            float &scale) {
+__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, float (&p)[V], float &base, float &scale) {
   float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -143,11 +159,11 @@ __device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, floa
     mx = fmaxf(mx, p[i]);
   }
   mx = group_maxf<G>(mx);
-  base = mx == -INFINITY ? 0.f : mx;
+  base = mx == -INFINITY ? 0.f : mx * LOG2E;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    p[i] = expf(p[i] - base);  // +inf logits: inf - inf = NaN, as the quotient would be
+    p[i] = exp2_approx(fmaf(p[i], LOG2E, -base));  // +inf logits: inf - inf = NaN, as the quotient would be
     sum += p[i];
   }
   sum = group_sum<G>(sum);
@@ -177,8 +193,8 @@ __device__ __forceinline__ void write_loss(const float *sums, const int64_t *cnt
   }
 }
 
-template <typename T, int G, int V>
-__global__ void __launch_bounds__(THREADS) route_fwd_kernel(Args a, float *w, int64_t *idx, int64_t *counts, float *loss,
+template <typename T, int G, int V, int SL>
+__global__ void __launch_bounds__(THREADS, 4) route_fwd_kernel(Args a, float *w, int64_t *idx, int64_t *counts, float *loss,
                                                             float *part_sum, int *part_cnt) {
   using Key = KeyOf<T>;
   using K = typename Key::type;
@@ -214,15 +230,14 @@ __global__ void __launch_bounds__(THREADS) route_fwd_kernel(Args a, float *w, in
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       key[i] = e0 + i < a.E ? Key::make(x[i], e0 + i) : (K)0;
-      col[i] += live ? p[i] : 0.f;
     }
     // a lane's keys in order, so that only its first can be the next choice.  The j-th choice is kept by lane j % G of
-    // the group, in slot j / G (k <= E <= G V: V slots are enough).
+    // the group, in slot j / G of SL.
     sort_down<V, K>(key);
-    K top[V];
+    K top[SL];
     unsigned chosen = 0;
 #pragma unroll
-    for (int s = 0; s < V; ++s) {
+    for (int s = 0; s < SL; ++s) {
       top[s] = 0;
       for (int r = 0; r < G && s * G + r < a.k; ++r) {
         const K best = group_max<G, K>(key[0]);
@@ -235,18 +250,23 @@ __global__ void __launch_bounds__(THREADS) route_fwd_kernel(Args a, float *w, in
         if (gl == r) top[s] = best;
       }
     }
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) cnt[i] += live ? (chosen >> i) & 1u : 0u;
-    float pe[V], total = 0.f;
+      for (int i = 0; i < V; ++i) {
+        col[i] += p[i];
+        cnt[i] += (chosen >> i) & 1u;
+      }
+    }
+    float pe[SL], total = 0.f;
 #pragma unroll
-    for (int s = 0; s < V; ++s) {
+    for (int s = 0; s < SL; ++s) {
       pe[s] = 0.f;
-      if (s * G + gl < a.k) pe[s] = expf(Key::value(top[s]) - base) * scale;
+      if (s * G + gl < a.k) pe[s] = exp2_approx(fmaf(Key::value(top[s]), LOG2E, -base)) * scale;
       total += pe[s];
     }
     total = group_sum<G>(total) + 1e-20f;
 #pragma unroll
-    for (int s = 0; s < V; ++s) {
+    for (int s = 0; s < SL; ++s) {
       const int j = s * G + gl;
       if (live && j < a.k) {
         w[t * a.k + j] = pe[s] / total;  // k = 1: exactly 1
@@ -301,11 +321,24 @@ __global__ void __launch_bounds__(1024) route_join_kernel(Args a, const float *p
   const int lanes = 1024 / pad, e = threadIdx.x % pad, l = threadIdx.x / pad;
   float s = 0.f;
   int64_t c = 0;
-  if (e < a.E)
-    for (int b = l; b < blocks; b += lanes) {
-      s += part_sum[(int64_t)b * a.E + e];
-      c += part_cnt[(int64_t)b * a.E + e];
+  if (e < a.E) {
+    constexpr int AT_ONCE = 8;  // in flight; summed in order
+    for (int b0 = l; b0 < blocks; b0 += lanes * AT_ONCE) {
+      float vs[AT_ONCE];
+      int vc[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int b = b0 + u * lanes;
+        vs[u] = b < blocks ? part_sum[(int64_t)b * a.E + e] : 0.f;
+        vc[u] = b < blocks ? part_cnt[(int64_t)b * a.E + e] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        s += vs[u];
+        c += vc[u];
+      }
     }
+  }
   st_sum[threadIdx.x] = s;
   st_cnt[threadIdx.x] = c;
   __syncthreads();
@@ -323,8 +356,8 @@ __global__ void __launch_bounds__(1024) route_join_kernel(Args a, const float *p
   write_loss(sh_sum, sh_cnt, a, counts, loss);
 }
 
-template <typename T, int G, int V>
-__global__ void __launch_bounds__(THREADS) route_bwd_kernel(Args a, const float *w, const int64_t *idx,
+template <typename T, int G, int V, int SL>
+__global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const float *w, const int64_t *idx,
                                                             const int64_t *counts, const float *dw, const float *dloss,
                                                             T *dz) {
   constexpr int ROWS = THREADS / G;
@@ -346,10 +379,10 @@ __global__ void __launch_bounds__(THREADS) route_bwd_kernel(Args a, const float 
     for (int i = 0; i < V; ++i) dp[i] = load[i];
     if (dw) {
       // lane j % G has the j-th choice: its gradient, its weight and the probability of its expert
-      int es[V];
-      float ds[V], dot = 0.f, total = 0.f;
+      int es[SL];
+      float ds[SL], dot = 0.f, total = 0.f;
 #pragma unroll
-      for (int s = 0; s < V; ++s) {
+      for (int s = 0; s < SL; ++s) {
         const int j = s * G + gl;
         es[s] = -1;
         ds[s] = 0.f;
@@ -357,13 +390,13 @@ __global__ void __launch_bounds__(THREADS) route_bwd_kernel(Args a, const float 
           es[s] = (int)idx[t * a.k + j];
           ds[s] = dw[t * a.k + j];
           dot = fmaf(ds[s], w[t * a.k + j], dot);
-          total += expf(to_f(z[t * a.row_stride + es[s]]) - base) * scale;
+          total += exp2_approx(fmaf(to_f(z[t * a.row_stride + es[s]]), LOG2E, -base)) * scale;
         }
       }
       dot = group_sum<G>(dot);
       const float inv = 1.f / (group_sum<G>(total) + 1e-20f);
 #pragma unroll
-      for (int s = 0; s < V; ++s) {
+      for (int s = 0; s < SL; ++s) {
         ds[s] = (ds[s] - dot) * inv;
         for (int r = 0; r < G && s * G + r < a.k; ++r) {
           const int e = G == 1 ? es[s] : __shfl_sync(0xffffffffu, es[s], r, G);
@@ -400,16 +433,24 @@ __global__ void __launch_bounds__(THREADS) route_bwd_kernel(Args a, const float 
   }
 }
 
-// f(IC<G>, IC<V>) of the smallest group that covers E experts
+// f(IC<G>, IC<V>, IC<SL>) of the smallest group that covers E experts, and of the
+// slots a lane needs for k choices: one where the group has a lane for each, else
+// two, else the most there can be (k <= E <= G V)
 template <typename F>
-static cudaError_t with_group(int E, F &&f) {
-  if (E <= 8) return f(IC<1>{}, IC<8>{});
-  if (E <= 16) return f(IC<2>{}, IC<8>{});
-  if (E <= 32) return f(IC<4>{}, IC<8>{});
-  if (E <= 64) return f(IC<8>{}, IC<8>{});
-  if (E <= 128) return f(IC<16>{}, IC<8>{});
-  if (E <= 256) return f(IC<32>{}, IC<8>{});
-  return f(IC<32>{}, IC<16>{});
+static cudaError_t with_group(int E, int k, F &&f) {
+  auto slots = [&](auto g, auto v) -> cudaError_t {
+    constexpr int G = decltype(g)::value, V = decltype(v)::value;
+    if (k <= G) return f(g, v, IC<1>{});
+    if (k <= 2 * G) return f(g, v, IC<2>{});
+    return f(g, v, IC<V>{});
+  };
+  if (E <= 8) return slots(IC<1>{}, IC<8>{});
+  if (E <= 16) return slots(IC<2>{}, IC<8>{});
+  if (E <= 32) return slots(IC<4>{}, IC<8>{});
+  if (E <= 64) return slots(IC<8>{}, IC<8>{});
+  if (E <= 128) return slots(IC<16>{}, IC<8>{});
+  if (E <= 256) return slots(IC<32>{}, IC<8>{});
+  return slots(IC<32>{}, IC<16>{});
 }
 static int group_of(int E) {
   int g = 1;
@@ -470,8 +511,8 @@ int mhc_route_fwd(const void *logits, int dtype, int64_t T, int E, int64_t row_s
   int *pc = reinterpret_cast<int *>(ps + (size_t)blocks * E);
   cudaError_t e = with_dtype(dtype, [&](auto tag) -> cudaError_t {
     using T_ = decltype(tag);
-    return router::with_group(E, [&](auto g, auto v) -> cudaError_t {
-      router::route_fwd_kernel<T_, decltype(g)::value, decltype(v)::value>
+    return router::with_group(E, k, [&](auto g, auto v, auto sl) -> cudaError_t {
+      router::route_fwd_kernel<T_, decltype(g)::value, decltype(v)::value, decltype(sl)::value>
           <<<blocks, router::THREADS, 0, st>>>(a, weights, experts, counts, loss, ps, pc);
       return cudaGetLastError();
     });
@@ -503,8 +544,8 @@ int mhc_route_bwd(const void *logits, int dtype, int64_t T, int E, int64_t row_s
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = with_dtype(dtype, [&](auto tag) -> cudaError_t {
     using T_ = decltype(tag);
-    return router::with_group(E, [&](auto g, auto v) -> cudaError_t {
-      router::route_bwd_kernel<T_, decltype(g)::value, decltype(v)::value>
+    return router::with_group(E, k, [&](auto g, auto v, auto sl) -> cudaError_t {
+      router::route_bwd_kernel<T_, decltype(g)::value, decltype(v)::value, decltype(sl)::value>
           <<<grid, router::THREADS, 0, st>>>(a, weights, experts, counts, dweights, dloss, static_cast<T_ *>(dlogits));
       return cudaGetLastError();
     });
