@@ -184,15 +184,14 @@ __device__ __forceinline__ float code_value(const uint2 &w, int e) {
   const float f = __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650u | (e & 3)));
   return f - (SIGNED ? 8388736.f : 8388608.f);
 }
-__device__ __forceinline__ void store_codes(void *p, int64_t base, int64_t n, bool whole, int lane, const int (&c)[8]) {
+// codes in the low bytes of eight words
+__device__ __forceinline__ void store_codes(void *p, int64_t base, int64_t n, bool whole, int lane, const uint32_t (&c)[8]) {
   uint8_t *q = static_cast<uint8_t *>(p);
   if (whole) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w |= ((uint32_t)c[h * 4 + e] & 0xffu) << (8 * e);
-      __stcs(reinterpret_cast<uint32_t *>(q + base + h * 128 + lane * 4), w);
+      const uint32_t lo = __byte_perm(c[h * 4], c[h * 4 + 1], 0x0040), hi = __byte_perm(c[h * 4 + 2], c[h * 4 + 3], 0x0040);
+      __stcs(reinterpret_cast<uint32_t *>(q + base + h * 128 + lane * 4), __byte_perm(lo, hi, 0x5410));
     }
   } else {
 #pragma unroll
@@ -221,31 +220,37 @@ __device__ __forceinline__ int pack_v(float v, float safe) {
 
 __device__ __forceinline__ float sqrt_approx(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
 // The same codes, mostly without the IEEE division and roots (three long sequences
-// a value; with them the 8-bit step took 2.02 ms for 321 M values, against EIGHT_MS
-// ms): 127 sqrt(|m| / safe) from a reciprocal and an approximate root is within 127
-// * 2^-21 of the exact value, 255 (v / safe)^(1/4) within 255 * 2^-21.  Only a
-// value nearer than EDGE to the middle between two codes can round to the other
-// one; it is done again exactly.  `inv` = 1 / safe; scales too small for it to be a
-// normal number are passed with inv = 0 and are all done exactly.
-constexpr float EDGE = 4e-4f;
+// a value: with them the 8-bit step took 2.02 ms for 321 M values, against EIGHT_MS).
+// y = 127 sqrt(|m| / safe), or 255 (v / safe)^(1/4), from a reciprocal and
+// approximate roots is off by at most 4 and 5 units of 2^-23 of itself (roundings of
+// the reciprocal, two or three products, a root of 2^-23 each), 6.1e-5 and 1.6e-4 at
+// the largest code.  Only where y is nearer than EDGE to the middle between two codes
+// can the exact value round to the other; there the lane's codes are done again
+// exactly.  `inv` = 1 / safe; scales too small for it to be a normal number are
+// passed with inv = 0 and are all done exactly.  A code is the low byte of y + 1.5 *
+// 2^23, where the addition rounds to the nearest integer (in two's complement).
 template <bool SIGNED>
-__device__ __forceinline__ void pack_codes(const float (&x)[8], float safe, float inv, int (&c)[8]) {
+__device__ __forceinline__ void pack_codes(const float (&x)[8], float safe, float inv, uint32_t (&c)[8]) {
+  constexpr float EDGE = SIGNED ? 1e-4f : 2.5e-4f;
+  constexpr float kMagic = 12582912.f;
   bool near = inv == 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float q = fabsf(x[e]) * inv;
-    const float y = SIGNED ? sqrt_approx(q) * 127.f : sqrt_approx(sqrt_approx(q)) * 255.f;
-    const float t = y + 12582912.f;  // 1.5 * 2^23: rounds to the nearest integer, held in the low bits
-    near |= !(fabsf(y - (t - 12582912.f)) < 0.5f - EDGE);  // NaN too
-    int k = (int)(__float_as_uint(t) & 0xffu);
-    if (SIGNED && x[e] < 0.f) k = -k;
-    if (!SIGNED && x[e] > 0.f && k < 1) k = 1;
-    c[e] = k;
+    float y;
+    if (SIGNED)
+      y = copysignf(sqrt_approx(q) * 127.f, x[e]);
+    else
+      y = fmaxf(sqrt_approx(sqrt_approx(q)) * 255.f, x[e] > 0.f ? 1.f : 0.f);  // above zero stays above zero
+    const float t = y + kMagic;
+    near |= !(fabsf(y - (t - kMagic)) < 0.5f - EDGE);  // NaN too
+    if (!SIGNED) near |= q != q;                       // which fmaxf drops
+    c[e] = __float_as_uint(t);
   }
   if (near) {
 #pragma unroll 1
@@ -253,7 +258,7 @@ __device__ __forceinline__ void pack_codes(const float (&x)[8], float safe, floa
       float v = x[0];
 #pragma unroll
       for (int u = 1; u < 8; ++u) v = e == u ? x[u] : v;
-      const int k = SIGNED ? pack_m(v, safe) : pack_v(v, safe);
+      const uint32_t k = (uint32_t)(SIGNED ? pack_m(v, safe) : pack_v(v, safe));
 #pragma unroll
       for (int u = 0; u < 8; ++u) c[u] = e == u ? k : c[u];
     }
@@ -358,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
         }
         // an empty block divides by one; every code is then zero
         const float dm = am > 0.f ? am : 1.f, dv = av > 0.f ? av : 1.f;
-        int c[8];
+        uint32_t c[8];
         pack_codes<true>(m, dm, dm > 1e-30f ? __fdiv_rn(1.f, dm) : 0.f, c);
         store_codes(t.m, base, t.n, whole, lane, c);
         pack_codes<false>(v, dv, dv > 1e-30f ? __fdiv_rn(1.f, dv) : 0.f, c);

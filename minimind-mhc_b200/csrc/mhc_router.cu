@@ -90,7 +90,7 @@ __device__ __forceinline__ void sort_down(K (&k)[V]) {
         const int j = i ^ d;
         if (j > i) {
           const bool down = (i & size) == 0;
-          const K hi = k[i] > k[j] ? k[i] : k[j], lo = k[i] > k[j] ? k[j] : k[i];
+          const K hi = max(k[i], k[j]), lo = min(k[i], k[j]);
           k[i] = down ? hi : lo;
           k[j] = down ? lo : hi;
         }
@@ -104,7 +104,7 @@ __device__ __forceinline__ K group_max(K v) {
 #pragma unroll
   for (int o = G / 2; o; o >>= 1) {
     const K w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
+    v = max(v, w);
   }
   return v;
 }
@@ -367,6 +367,11 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
   const double f = dloss ? (double)*dloss * (double)a.scale / ((double)a.T * (double)a.T) : 0.0;
 #pragma unroll
   for (int i = 0; i < V; ++i) load[i] = dloss && e0 + i < a.E ? (float)(f * (double)counts[e0 + i]) : 0.f;
+  __shared__ __align__(16) float scatter[THREADS * V];
+  float *stripe = scatter + threadIdx.x / G * (G * V);
+#pragma unroll
+  for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(stripe + e0 + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncwarp();
   const T *z = static_cast<const T *>(a.z);
   for (int64_t tb = (int64_t)blockIdx.x * ROWS; tb < a.T; tb += (int64_t)gridDim.x * ROWS) {
     const bool live = tb + threadIdx.x / G < a.T;
@@ -378,7 +383,8 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
 #pragma unroll
     for (int i = 0; i < V; ++i) dp[i] = load[i];
     if (dw) {
-      // lane j % G has the j-th choice: its gradient, its weight and the probability of its expert
+      // Lane j % G has the j-th choice: its gradient, its weight and the probability of its expert.  What comes of it
+      // goes to the lane that owns the expert through the row's stripe of shared memory, all zeros in between.
       int es[SL];
       float ds[SL], dot = 0.f, total = 0.f;
 #pragma unroll
@@ -396,15 +402,18 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
       dot = group_sum<G>(dot);
       const float inv = 1.f / (group_sum<G>(total) + 1e-20f);
 #pragma unroll
-      for (int s = 0; s < SL; ++s) {
-        ds[s] = (ds[s] - dot) * inv;
-        for (int r = 0; r < G && s * G + r < a.k; ++r) {
-          const int e = G == 1 ? es[s] : __shfl_sync(0xffffffffu, es[s], r, G);
-          const float d = G == 1 ? ds[s] : __shfl_sync(0xffffffffu, ds[s], r, G);
+      for (int s = 0; s < SL; ++s)
+        if (es[s] >= 0) stripe[es[s]] = (ds[s] - dot) * inv;
+      __syncwarp();
 #pragma unroll
-          for (int i = 0; i < V; ++i) dp[i] += e == e0 + i ? d : 0.f;
-        }
+      for (int i = 0; i < V; i += 4) {
+        const float4 d = *reinterpret_cast<const float4 *>(stripe + e0 + i);
+        dp[i] += d.x; dp[i + 1] += d.y; dp[i + 2] += d.z; dp[i + 3] += d.w;
       }
+      __syncwarp();
+#pragma unroll
+      for (int s = 0; s < SL; ++s)
+        if (es[s] >= 0) stripe[es[s]] = 0.f;
     }
     float pd = 0.f;
 #pragma unroll
