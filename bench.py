@@ -920,7 +920,7 @@ def _train_step_entry(args, rank, world, dev):
 
 def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=4, inter=2048, vocab=6400,
                    experts=8, topk=2, moe_inter=None, theta=1e6, eps=1e-6, iters=20, use_mhc=1, chain=False,
-                   aux_coef=5e-4, dtype=torch.bfloat16):
+                   aux_coef=5e-4, dtype=torch.bfloat16, native_ops=False):
     """The reference's model with this build's mHC modules: a module tree whose
     state_dict keys, shapes and forward math are those of the reference's
     ``MiniMindForCausalLM`` with ``use_mhc`` 1 or 2 (``model/model_minimind.py``:
@@ -932,13 +932,18 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
     GQA), the reference's CUDA path minus the optional flash-attn library.  The
     MoE layer computes the same routing (softmax, top-k, renormalised) and
     auxiliary loss as the reference but groups each expert's rows with one sort
-    instead of a mask per expert.  Random init N(0, 0.02) for the matrices."""
+    instead of a mask per expert.  ``native_ops`` takes attention and the router
+    from this build (``model/mhc_attention.py``, ``model/mhc_router.py``)
+    instead.  Random init N(0, 0.02) for the matrices."""
     import torch.nn as nn
     import torch.nn.functional as F
 
     from model.mhc_common import MHCHead, StreamExpand
     from model.mhc_fused import MHCConnection_Fused
     from model.mhc_fused_no_hres import MHCConnection_FusedNoHres
+    if native_ops:
+        from model.mhc_attention import packed_attention
+        from model.mhc_router import route_topk
 
     hd = hidden // heads
     moe_inter = moe_inter or inter
@@ -965,6 +970,8 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
                 return (t * cos + rot * sin).to(t.dtype)
 
             q, k = rope(q), rope(k)
+            if native_ops:
+                return self.o_proj(packed_attention(q, k, v).reshape(b, l, heads * hd))
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
                                                is_causal=True, enable_gqa=True)
             return self.o_proj(o.transpose(1, 2).reshape(b, l, heads * hd))
@@ -990,13 +997,18 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
         def forward(self, x):
             shape = x.shape
             xf = x.reshape(-1, hidden)
-            scores = torch.softmax(self.gate(xf), dim=-1)
-            w, idx = scores.topk(topk, dim=-1)
-            w = w / (w.sum(dim=-1, keepdim=True) + 1e-20)
-            flat = idx.flatten()
+            if native_ops:
+                w, idx, counts, aux = route_topk(self.gate(xf), topk, aux_coef)
+                flat = idx.flatten()
+            else:
+                scores = torch.softmax(self.gate(xf), dim=-1)
+                w, idx = scores.topk(topk, dim=-1)
+                w = w / (w.sum(dim=-1, keepdim=True) + 1e-20)
+                flat = idx.flatten()
+                counts = torch.bincount(flat, minlength=experts)
             order = flat.argsort()
             tok = order // topk
-            counts = torch.bincount(flat, minlength=experts).tolist()
+            counts = counts.tolist()
             xs = xf.index_select(0, tok)
             # each expert's rows are zero-padded to a multiple of 1024, so the
             # GEMM shapes come from a small set (new shapes every step would
@@ -1009,7 +1021,9 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
                 outs.append(e(F.pad(c, (0, 0, 0, pad)))[:c.shape[0]] if pad else e(c))
             ys = torch.cat(outs) if outs else xs[:0]
             ys = ys * w.flatten()[order].unsqueeze(1).to(ys.dtype)
-            if self.training and aux_coef > 0:
+            if native_ops:
+                self.aux_loss = aux
+            elif self.training and aux_coef > 0:
                 load = F.one_hot(idx, experts).float().mean(0)
                 self.aux_loss = (load * scores.float().mean(0)).sum() * experts * aux_coef
             else:
@@ -1207,14 +1221,19 @@ def run_model(args, rank, world, local_rank):
     torch.cuda.set_device(dev)
     train = args.workload == "c5"
     torch.manual_seed(1234 + rank)
-    model = _build_decoder(moe=train, dev=dev, chain=args.chain)
+    model = _build_decoder(moe=train, dev=dev, chain=args.chain, native_ops=args.native_ops)
     batch = 8 if train else 32
     seq = 2048
     gen = torch.Generator(device=dev).manual_seed(77 + rank)
     ids = torch.randint(0, 6400, (batch, seq), device=dev, generator=gen)
     labels = torch.randint(0, 6400, (batch, seq), device=dev, generator=gen)
     params = [p for p in model.parameters()]
-    opt = torch.optim.AdamW(params, lr=1e-4, fused=True) if train else None
+    opt = None
+    if train and args.native_ops:
+        from model.mhc_adamw import AdamW
+        opt = AdamW(params, lr=1e-4)
+    elif train:
+        opt = torch.optim.AdamW(params, lr=1e-4, fused=True)
     dist = None
     if world > 1:
         import torch.distributed as dist
@@ -1279,6 +1298,7 @@ def run_model(args, rank, world, local_rank):
             "global_batch": world * batch, "seq_len": seq, "parallelism": f"dp{world}",
             "mhc_api": "block-level mhc_chain (merge + next coefficient pass + input norm per call)"
                        if args.chain else "drop-in modules, input norms in the closures",
+            "attention_router_optimizer": "this build's kernels" if args.native_ops else "torch",
         },
         "clocks": clocks,
     }
@@ -1308,6 +1328,8 @@ def main():
     ap.add_argument("--no-train", action="store_true", help="skip the config-5 training-step sub-measurement")
     ap.add_argument("--chain", action="store_true",
                     help="c4 / c5: run the decoder's sublayers through the block-level mhc_chain API")
+    ap.add_argument("--native-ops", action="store_true",
+                    help="c4 / c5: attention, router and optimizer step through this build's kernels instead of torch's")
     ap.add_argument("--flat-allreduce", action="store_true",
                     help="c5: one flat all-reduce per dtype after backward instead of the overlapped buckets")
     args = ap.parse_args()

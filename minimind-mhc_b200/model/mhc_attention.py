@@ -33,29 +33,31 @@ def _rows(x):
     return x
 
 
+def _forward(q, k, v, cu, seqlen, scale, for_grad):
+    """out, and what the backward needs beside it."""
+    t, h, d = q.shape
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = q.new_empty((t, h, d))
+    # the backward's row sums use out before its rounding to 16 bits
+    out_lo = q.new_empty((t, h, d)) if for_grad and q.dtype != torch.float32 else None
+    lib = nat.lib()
+    lse = q.new_empty((h, lib.mhc_attn_lse_pitch(t)), dtype=torch.float32)
+    strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    batch = 0 if cu is None else cu.numel() - 1
+    need = lib.mhc_attn_fwd_workspace(t)
+    ws = q.new_empty((need,), dtype=torch.uint8)
+    nat.call_on(q.get_device(), "mhc_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.dtype_code(q.dtype), t,
+                h, k.shape[1], d, strides, nat.ptr(cu), batch, seqlen, scale, out.data_ptr(), nat.ptr(out_lo),
+                lse.data_ptr(), ws.data_ptr(), need)
+    return out, (q, k, v, cu, out, out_lo, lse), (strides, batch, seqlen, scale)
+
+
 class _PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu, seqlen, scale):
-        t, h, d = q.shape
-        hk = k.shape[1]
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        index = q.get_device()
-        out = q.new_empty((t, h, d))
-        # the backward's row sums use out before its rounding to 16 bits
-        out_lo = q.new_empty((t, h, d)) if any(ctx.needs_input_grad) and q.dtype != torch.float32 else None
-        lib = nat.lib()
-        lse = q.new_empty((h, lib.mhc_attn_lse_pitch(t)), dtype=torch.float32)
-        strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
-        batch = 0 if cu is None else cu.numel() - 1
-        need = lib.mhc_attn_fwd_workspace(t)
-        ws = q.new_empty((need,), dtype=torch.uint8)
-        nat.call_on(index, "mhc_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.dtype_code(q.dtype), t, h,
-                    hk, d, strides, nat.ptr(cu), batch, seqlen, scale, out.data_ptr(), nat.ptr(out_lo),
-                    lse.data_ptr(), ws.data_ptr(), need)
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(q, k, v, cu, out, out_lo, lse)
-            ctx.meta = (strides, batch, seqlen, scale)
+        out, saved, ctx.meta = _forward(q, k, v, cu, seqlen, scale, True)
+        ctx.save_for_backward(*saved)
         return out
 
     @staticmethod
@@ -74,6 +76,12 @@ class _PackedAttentionFn(torch.autograd.Function):
                     nat.ptr(cu), batch, seqlen, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
                     need)
         return dq, dk, dv, None, None, None
+
+
+def _attend(q, k, v, cu, seqlen, scale):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttentionFn.apply(q, k, v, cu, seqlen, scale)
+    return _forward(q, k, v, cu, seqlen, scale, False)[0]
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
@@ -116,9 +124,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
     if cu_seqlens is None:
         b, l = q.shape[:2]
-        out = _PackedAttentionFn.apply(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), None, l, scale)
-        return out.view(b, l, h, d)
+        return _attend(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), None, l, scale).view(b, l, h, d)
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         raise ValueError("packed_attention: cu_seqlens must be int32 with one offset more than there are sequences, "
                          f"got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
-    return _PackedAttentionFn.apply(q, k, v, cu_seqlens.contiguous(), 0, scale)
+    return _attend(q, k, v, cu_seqlens.contiguous(), 0, scale)

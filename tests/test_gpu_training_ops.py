@@ -1,0 +1,87 @@
+"""The training-step operators together: the benchmark decoder with them against the same decoder on torch's, and the
+packed example; the tensor-core attention against the CUDA-core one."""
+
+import os
+import sys
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_decoder_with_native_ops_matches_torch_ops(dtype):
+    """One step of the MoE + mHC decoder, same weights, same tokens.  fp32: the two differ by fp32 roundings through 2
+    layers (1e-4 of the largest gradient).  bf16: the router of torch's side rounds its probabilities to bf16, so a
+    token whose choice is a near tie may go to another expert; the losses agree to 2^-8 and the gradients of the
+    embedding, which average over the tokens, to 10 %."""
+    import bench
+    dev = torch.device("cuda")
+    args = dict(moe=True, dev=dev, hidden=256, layers=2, heads=4, kv_heads=2, inter=256, vocab=300, dtype=dtype)
+    torch.manual_seed(3)
+    a = bench._build_decoder(**args)
+    b = bench._build_decoder(native_ops=True, **args)
+    b.load_state_dict(a.state_dict())
+    ids = torch.randint(0, 300, (3, 200), device=dev)
+    grads, losses = [], []
+    for m in (a, b):
+        logits = m(ids)
+        loss = F.cross_entropy(logits[:, :-1].reshape(-1, 300).float(), ids[:, 1:].reshape(-1)) + m.aux_loss()
+        loss.backward()
+        losses.append(loss.item())
+        grads.append(m.lm_head.weight.grad.double())
+    off = (grads[0] - grads[1]).norm() / grads[0].norm()
+    if dtype == torch.float32:
+        assert abs(losses[0] - losses[1]) <= 1e-4 * losses[0]
+        assert off <= 1e-4
+    else:
+        assert abs(losses[0] - losses[1]) <= 2.0 ** -8 * losses[0]
+        assert off <= 0.1
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_packed_example_learns(bits):
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import train_packed_moe
+    losses = train_packed_moe.train(30, bits)
+    # a uniform guess over 512 tokens costs log 512 = 6.24
+    assert losses[0] > 5.5 and losses[-1] < 0.5 * losses[0]
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_tensor_core_attention_against_cuda_core_attention(dtype):
+    """Both from the same inputs; the difference is the tensor-core side's rounding of P and dS (2 u each)."""
+    from model import _native as nat
+    from model.mhc_attention import packed_attention
+    u = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v, do = (torch.randn(1500, h, 96, device="cuda", generator=g).to(dtype) for h in (8, 4, 4, 8))
+    cu = torch.tensor([0, 700, 701, 1400], dtype=torch.int32, device="cuda")
+    sides = []
+    for policy in (nat.PATH_AUTO, nat.PATH_GENERIC):
+        prev = nat.lib().mhc_set_path_policy(policy)
+        try:
+            x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = packed_attention(*x, cu)
+            sides.append((out.detach(), *torch.autograd.grad(out, x, do)))
+        finally:
+            nat.lib().mhc_set_path_policy(prev)
+    for a, b in zip(*sides):
+        assert not torch.equal(a, b)  # two kernels ran
+        assert (a.double() - b.double()).norm() <= 4 * u * b.double().norm()
+
+
+def test_second_derivatives_are_refused():
+    from model.mhc_attention import packed_attention
+    from model.mhc_router import route_topk
+    q = torch.randn(4, 2, 64, device="cuda", requires_grad=True)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(packed_attention(q, q, q, cu).sum(), q, create_graph=True)
+    z = torch.randn(4, 8, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(route_topk(z, 2, 1.0).weights.square().sum(), z, create_graph=True)
