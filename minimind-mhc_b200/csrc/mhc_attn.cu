@@ -6,9 +6,11 @@
 //   dQ_i = scale sum_j dS_ij K_j
 //   dK_j = scale sum_{h in group, i} dS_ij Q_i,   dV_j = sum_{h in group, i} P_ij dO_i
 //
-// fp32 throughout.  A block of 16 x 16 threads owns 64 rows and walks tiles of 64
-// columns; a thread holds a 4 x 4 piece of the scores and 4 rows x D / 16 columns
-// of the result in registers, the operands are staged as fp32 in shared memory.
+// fp32 throughout.  A block of 16 x 16 threads owns 64 rows (32 where that leaves SMs
+// with less than four blocks: it is the loads' latency that other blocks then cover)
+// and walks tiles of 64 columns; a thread holds a 4 x 4 piece of the scores and 4 rows
+// x D / 16 columns of the result in registers (half the rows with 32), the operands
+// are staged as fp32 in shared memory and multiplied two at a time (fma.rn.f32x2).
 // Forward: one pass with the running maximum and sum.  Backward: the scores again
 // from the saved L, in two kernels of the same form (a block owns 64 queries and
 // sums dQ, or 64 keys and sums dK and dV over the heads that share them), so
@@ -29,86 +31,94 @@
 namespace mhc {
 namespace attn {
 
-constexpr int TILE = 64;
+constexpr int TILE = 64;  // columns
 constexpr int THREADS = 256;
 constexpr int PP = TILE + 4;  // pitch of a score tile
 
-// 64 rows of one head as fp32 into shared memory, zero outside of the packed
-// range and past column D
-template <typename T, int DP>
+// ROWS rows of one head as fp32 into shared memory, zero outside of the packed range
+// and past column D
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t ts, int row0, int D, Span range) {
-  for (int e = threadIdx.x; e < TILE * DP; e += THREADS) {
+#pragma unroll 8
+  for (int e = threadIdx.x; e < ROWS * DP; e += THREADS) {
     const int r = e / DP, c = e - r * DP;
     const int t = row0 + r;
     dst[r * (DP + 4) + c] = t >= range.start && t < range.end && c < D ? to_f(src[(int64_t)t * ts + c]) : 0.f;
   }
 }
 
-// s[i][j] = sum_d A[ty*4+i][d] B[tx+16j][d]
-template <int DP>
-__device__ __forceinline__ void scores(const float *A, const float *B, int ty, int tx, float (&s)[4][4]) {
+// s[i][j] = sum_d A[ty*R+i][d] B[tx+16j][d], even and odd d apart until the end
+template <int DP, int R>
+__device__ __forceinline__ void scores(const float *A, const float *B, int ty, int tx, float (&s)[R][4]) {
+  uint64_t acc[R][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
-    float4 x[4], y[4];
+    ulonglong2 x[R], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(A + (ty * 4 + i) * (DP + 4) + d);
+    for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const ulonglong2 *>(A + (ty * R + i) * (DP + 4) + d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4 *>(B + (tx + 16 * j) * (DP + 4) + d);
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const ulonglong2 *>(B + (tx + 16 * j) * (DP + 4) + d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-        s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-        s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-        s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+        acc[i][j] = sm100::f2_fma(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = sm100::f2_fma(x[i].y, y[j].y, acc[i][j]);
       }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      sm100::f2_unpack(acc[i][j], lo, hi);
+      s[i][j] = lo + hi;
+    }
 }
 
-// acc[i][2c..2c+1] += sum_kk W[ty*4+i][kk] B[kk][2 tx + 32 c ..]
-template <int DP>
-__device__ __forceinline__ void accumulate(const float *W, const float *B, int ty, int tx, float (&acc)[4][DP / 16]) {
+// acc[i][c] += sum_kk W[ty*R+i][kk] B[kk][2 tx + 32 c, + 1], columns in pairs
+template <int DP, int R>
+__device__ __forceinline__ void accumulate(const float *W, const float *B, int ty, int tx, uint64_t (&acc)[R][DP / 32]) {
 #pragma unroll 2
   for (int kk = 0; kk < TILE; kk += 4) {
-    float4 w[4];
+    float4 w[R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4 *>(W + (ty * 4 + i) * PP + kk);
+    for (int i = 0; i < R; ++i) w[i] = *reinterpret_cast<const float4 *>(W + (ty * R + i) * PP + kk);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float2 b[DP / 32];
+      uint64_t b[DP / 32];
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) b[c] = *reinterpret_cast<const float2 *>(B + (kk + u) * (DP + 4) + 2 * tx + 32 * c);
+      for (int c = 0; c < DP / 32; ++c) b[c] = *reinterpret_cast<const uint64_t *>(B + (kk + u) * (DP + 4) + 2 * tx + 32 * c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < R; ++i) {
         const float wi = u == 0 ? w[i].x : (u == 1 ? w[i].y : (u == 2 ? w[i].z : w[i].w));
+        const uint64_t w2 = sm100::f2_pack(wi, wi);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          acc[i][2 * c] = fmaf(wi, b[c].x, acc[i][2 * c]);
-          acc[i][2 * c + 1] = fmaf(wi, b[c].y, acc[i][2 * c + 1]);
-        }
+        for (int c = 0; c < DP / 32; ++c) acc[i][c] = sm100::f2_fma(w2, b[c], acc[i][c]);
       }
     }
   }
 }
 
 // lo != null: what the rounding to T left over, itself in T
-template <typename T, int DP>
+template <typename T, int DP, int R>
 __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, int64_t T_, int D, int ty, int tx,
-                                           const float (&acc)[4][DP / 16], const float (&mul)[4]) {
+                                           const uint64_t (&acc)[R][DP / 32], const float (&mul)[R]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = row0 + ty * 4 + i;
+  for (int i = 0; i < R; ++i) {
+    const int t = row0 + ty * R + i;
     if (t >= T_) continue;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int col = 2 * tx + 32 * (c / 2) + (c & 1);
       if (col < D) {
-        const float v = acc[i][c] * mul[i];
+        float v, w;
+        sm100::f2_unpack(acc[i][c / 2], v, w);
+        v = (c & 1 ? w : v) * mul[i];
         const T r = from_f<T>(v);
         dst[(int64_t)t * ts + col] = r;
         if (lo) lo[(int64_t)t * ts + col] = from_f<T>(v - to_f(r));
@@ -117,39 +127,40 @@ __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, 
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a) {
+  constexpr int R = ROWS / 16;
   extern __shared__ float sm[];
-  float *Q = sm, *K = Q + TILE * (DP + 4), *V = K + TILE * (DP + 4), *P = V + TILE * (DP + 4);
+  float *Q = sm, *K = Q + ROWS * (DP + 4), *V = K + TILE * (DP + 4), *P = V + TILE * (DP + 4);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * TILE;  // longest rows first
+  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * ROWS;  // longest rows first
   const int h = blockIdx.y, hk = h / (a.H / a.Hk);
   const Span range = packed_range(a);
-  int start[4];
+  int start[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = q0 + ty * 4 + i;
+  for (int i = 0; i < R; ++i) {
+    const int t = q0 + ty * R + i;
     start[i] = t < a.T ? span_of(a, t).start : t + 1;
   }
-  load_tile<T, DP>(Q, static_cast<const T *>(a.q) + h * a.qh, a.qt, q0, a.D, range);
-  float acc[4][DP / 16] = {};
-  float mx[4], sum[4];
+  load_tile<T, DP, ROWS>(Q, static_cast<const T *>(a.q) + h * a.qh, a.qt, q0, a.D, range);
+  uint64_t acc[R][DP / 32] = {};
+  float mx[R], sum[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     mx[i] = -INFINITY;
     sum[i] = 0.f;
   }
-  const int first = span_of(a, q0).start, last = min((int64_t)q0 + TILE, a.T);
+  const int first = span_of(a, q0).start, last = min((int64_t)q0 + ROWS, a.T);
   for (int k0 = first; k0 < last; k0 += TILE) {
     __syncthreads();
-    load_tile<T, DP>(K, static_cast<const T *>(a.k) + hk * a.kh, a.kt, k0, a.D, range);
-    load_tile<T, DP>(V, static_cast<const T *>(a.v) + hk * a.vh, a.vt, k0, a.D, range);
+    load_tile<T, DP, TILE>(K, static_cast<const T *>(a.k) + hk * a.kh, a.kt, k0, a.D, range);
+    load_tile<T, DP, TILE>(V, static_cast<const T *>(a.v) + hk * a.vh, a.vt, k0, a.D, range);
     __syncthreads();
-    float s[4][4];
-    scores<DP>(Q, K, ty, tx, s);
+    float s[R][4];
+    scores<DP, R>(Q, K, ty, tx, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = q0 + ty * 4 + i;
+    for (int i = 0; i < R; ++i) {
+      const int t = q0 + ty * R + i;
       float m = mx[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -166,61 +177,62 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
       for (int j = 0; j < 4; ++j) {
         const float p = exp2f(s[i][j] - base);
         part += p;
-        P[(ty * 4 + i) * PP + tx + 16 * j] = p;
+        P[(ty * R + i) * PP + tx + 16 * j] = p;
       }
 #pragma unroll
       for (int o = 8; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
       sum[i] = sum[i] * fix + part;
       mx[i] = m;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= fix;
+      for (int c = 0; c < DP / 32; ++c) acc[i][c] = sm100::f2_mul(acc[i][c], sm100::f2_pack(fix, fix));
     }
     __syncwarp();  // a row of P is written and read by the same 16 lanes
-    accumulate<DP>(P, V, ty, tx, acc);
+    accumulate<DP, R>(P, V, ty, tx, acc);
   }
-  float inv[4];
+  float inv[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = q0 + ty * 4 + i;
+  for (int i = 0; i < R; ++i) {
+    const int t = q0 + ty * R + i;
     inv[i] = sum[i] == 0.f ? 0.f : 1.f / sum[i];
     if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.Tp + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
   }
   T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
-  store_rows<T, DP>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
+  store_rows<T, DP, R>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
 }
 
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
 // that see them, of every head of the group.
-template <typename T, int DP, bool DKV>
+template <typename T, int DP, int ROWS, bool DKV>
 __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a) {
+  constexpr int R = ROWS / 16;
   extern __shared__ float sm[];
-  constexpr int TS = TILE * (DP + 4);
-  float *R1 = sm, *R2 = R1 + TS, *C1 = R2 + TS, *C2 = C1 + TS, *W = C2 + TS, *L = W + TILE * PP, *Dl = L + TILE;
+  constexpr int TS = TILE * (DP + 4), RS = ROWS * (DP + 4);
+  float *R1 = sm, *R2 = R1 + RS, *C1 = R2 + RS, *C2 = C1 + TS, *W = C2 + TS, *L = W + ROWS * PP, *Dl = L + TILE;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int r0 = (int)(DKV ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TILE;
+  const int r0 = (int)(DKV ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * ROWS;
   const int G = a.H / a.Hk;
   const int rh = blockIdx.y;
   const Span range = packed_range(a);
   const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
   const T *dout = static_cast<const T *>(a.dout);
   const int64_t ot = (int64_t)a.H * a.D;
-  int bound[4];  // DKV: the end of the key's sequence; else the start of the query's
+  int bound[R];  // DKV: the end of the key's sequence; else the start of the query's
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = r0 + ty * 4 + i;
+  for (int i = 0; i < R; ++i) {
+    const int t = r0 + ty * R + i;
     const Span s = t < a.T ? span_of(a, t) : Span{t + 1, t};
     bound[i] = DKV ? s.end : s.start;
   }
   if (DKV) {
-    load_tile<T, DP>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
-    load_tile<T, DP>(R2, v + rh * a.vh, a.vt, r0, a.D, range);
+    load_tile<T, DP, ROWS>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
+    load_tile<T, DP, ROWS>(R2, v + rh * a.vh, a.vt, r0, a.D, range);
   } else {
-    load_tile<T, DP>(R1, q + rh * a.qh, a.qt, r0, a.D, range);
-    load_tile<T, DP>(R2, dout + (int64_t)rh * a.D, ot, r0, a.D, range);
+    load_tile<T, DP, ROWS>(R1, q + rh * a.qh, a.qt, r0, a.D, range);
+    load_tile<T, DP, ROWS>(R2, dout + (int64_t)rh * a.D, ot, r0, a.D, range);
   }
-  float acc1[4][DP / 16] = {}, acc2[DKV ? 4 : 1][DP / 16] = {};
-  const int64_t end_rows = min((int64_t)r0 + TILE, a.T);
+  uint64_t acc1[R][DP / 32] = {}, acc2[DKV ? R : 1][DP / 32] = {};
+  const int64_t end_rows = min((int64_t)r0 + ROWS, a.T);
   const int first = DKV ? r0 : span_of(a, r0).start;
   const int last = DKV ? span_of(a, (int)end_rows - 1).end : (int)end_rows;
   for (int g = 0; g < (DKV ? G : 1); ++g) {
@@ -228,11 +240,11 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
     for (int c0 = first; c0 < last; c0 += TILE) {
       __syncthreads();
       if (DKV) {
-        load_tile<T, DP>(C1, q + h * a.qh, a.qt, c0, a.D, range);
-        load_tile<T, DP>(C2, dout + (int64_t)h * a.D, ot, c0, a.D, range);
+        load_tile<T, DP, TILE>(C1, q + h * a.qh, a.qt, c0, a.D, range);
+        load_tile<T, DP, TILE>(C2, dout + (int64_t)h * a.D, ot, c0, a.D, range);
       } else {
-        load_tile<T, DP>(C1, k + (rh / G) * a.kh, a.kt, c0, a.D, range);
-        load_tile<T, DP>(C2, v + (rh / G) * a.vh, a.vt, c0, a.D, range);
+        load_tile<T, DP, TILE>(C1, k + (rh / G) * a.kh, a.kt, c0, a.D, range);
+        load_tile<T, DP, TILE>(C2, v + (rh / G) * a.vh, a.vt, c0, a.D, range);
       }
       if (tid < TILE) {
         const int64_t t = (DKV ? c0 : r0) + tid;
@@ -240,46 +252,50 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
         Dl[tid] = t < a.T ? a.delta[(int64_t)h * a.Tp + t] : 0.f;
       }
       __syncthreads();
-      float p[4][4], ds[4][4];
-      scores<DP>(R1, C1, ty, tx, p);
-      scores<DP>(R2, C2, ty, tx, ds);
+      float p[R][4], ds[R][4];
+      scores<DP, R>(R1, C1, ty, tx, p);
+      scores<DP, R>(R2, C2, ty, tx, ds);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + ty * 4 + i;
+      for (int i = 0; i < R; ++i) {
+        const int r = r0 + ty * R + i;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = c0 + tx + 16 * j;
           const bool seen = DKV ? c >= r && c < bound[i] : c <= r && c >= bound[i];
-          const int n = DKV ? tx + 16 * j : ty * 4 + i;
+          const int n = DKV ? tx + 16 * j : ty * R + i;
           p[i][j] = seen ? exp2f(fmaf(p[i][j], a.scale_log2, -L[n])) : 0.f;
           ds[i][j] = seen ? p[i][j] * (ds[i][j] - Dl[n]) : 0.f;
         }
       }
       if constexpr (DKV) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) W[(ty * 4 + i) * PP + tx + 16 * j] = p[i][j];
+          for (int j = 0; j < 4; ++j) W[(ty * R + i) * PP + tx + 16 * j] = p[i][j];
         __syncwarp();
-        accumulate<DP>(W, C2, ty, tx, acc2);
+        accumulate<DP, R>(W, C2, ty, tx, acc2);
         __syncwarp();
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) W[(ty * 4 + i) * PP + tx + 16 * j] = ds[i][j];
+        for (int j = 0; j < 4; ++j) W[(ty * R + i) * PP + tx + 16 * j] = ds[i][j];
       __syncwarp();
-      accumulate<DP>(W, C1, ty, tx, acc1);
+      accumulate<DP, R>(W, C1, ty, tx, acc1);
     }
   }
-  const float sc[4] = {a.scale, a.scale, a.scale, a.scale};
+  float sc[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) sc[i] = a.scale;
   if constexpr (DKV) {
-    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    float one[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) one[i] = 1.f;
     const int64_t kt = (int64_t)a.Hk * a.D;
-    store_rows<T, DP>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
-    store_rows<T, DP>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+    store_rows<T, DP, R>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
+    store_rows<T, DP, R>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
   } else {
-    store_rows<T, DP>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
+    store_rows<T, DP, R>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
   }
 }
 
@@ -374,23 +390,29 @@ static cudaError_t allow_smem(size_t bytes) {
   return e;
 }
 
-template <typename T, int DP>
+// whether blocks of 32 rows: with 64 an SM would have less than four
+static bool short_rows(int64_t T, int heads) {
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  return (T + TILE - 1) / TILE * heads < 4 * (int64_t)sms;
+}
+
+template <typename T, int DP, int ROWS>
 static cudaError_t run_fwd(const Args &a, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)(3 * TILE * (DP + 4) + TILE * PP) * 4;
-  cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP>>(smem);
+  constexpr size_t smem = (size_t)((ROWS + 2 * TILE) * (DP + 4) + ROWS * PP) * 4;
+  cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP, ROWS>>(smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.T + TILE - 1) / TILE), (unsigned)a.H);
-  attn_fwd_generic_kernel<T, DP><<<grid, THREADS, smem, stream>>>(a);
+  const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)a.H);
+  attn_fwd_generic_kernel<T, DP, ROWS><<<grid, THREADS, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, int DP, bool DKV>
+template <typename T, int DP, int ROWS, bool DKV>
 static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)(4 * TILE * (DP + 4) + TILE * PP + 2 * TILE) * 4;
-  cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, DKV>>(smem);
+  constexpr size_t smem = (size_t)(2 * (ROWS + TILE) * (DP + 4) + ROWS * PP + 2 * TILE) * 4;
+  cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, ROWS, DKV>>(smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.T + TILE - 1) / TILE), (unsigned)(DKV ? a.Hk : a.H));
-  attn_bwd_generic_kernel<T, DP, DKV><<<grid, THREADS, smem, stream>>>(a);
+  const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)(DKV ? a.Hk : a.H));
+  attn_bwd_generic_kernel<T, DP, ROWS, DKV><<<grid, THREADS, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -399,7 +421,10 @@ static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
 cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    return attn::with_dim(a.D, [&](auto d) -> cudaError_t { return attn::run_fwd<T, decltype(d)::value>(a, stream); });
+    return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
+      constexpr int DP = decltype(d)::value;
+      return attn::short_rows(a.T, a.H) ? attn::run_fwd<T, DP, 32>(a, stream) : attn::run_fwd<T, DP, 64>(a, stream);
+    });
   });
 }
 
@@ -424,8 +449,11 @@ cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream) {
     using T = decltype(tag);
     return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
       constexpr int DP = decltype(d)::value;
-      const cudaError_t e = attn::run_bwd<T, DP, false>(a, stream);
-      return e != cudaSuccess ? e : attn::run_bwd<T, DP, true>(a, stream);
+      const cudaError_t e = attn::short_rows(a.T, a.H) ? attn::run_bwd<T, DP, 32, false>(a, stream)
+                                                       : attn::run_bwd<T, DP, 64, false>(a, stream);
+      if (e != cudaSuccess) return e;
+      return attn::short_rows(a.T, a.Hk) ? attn::run_bwd<T, DP, 32, true>(a, stream)
+                                         : attn::run_bwd<T, DP, 64, true>(a, stream);
     });
   });
 }

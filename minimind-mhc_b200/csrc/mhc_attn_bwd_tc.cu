@@ -14,17 +14,20 @@
 //
 // (seven products of 128 x 128 x D a tile where five would do if dQ were added up
 // over blocks: two more on the tensor core instead of atomics in an order that
-// changes).  P and dS never leave TMEM: a thread reads its half row of S, writes P
-// over it as 16-bit values, which is the A operand of the next product; the column
-// operands serve S and dP as they are (K-major) and the gradients as they lie
-// (their rows are the summed index: MN-major).
+// changes).  P and dS never leave TMEM: a thread reads a quarter of a row of S, writes
+// P as 16-bit values, which is the A operand of the next product, and dS over dP the
+// same way; the column operands serve S and dP as they are (K-major) and the
+// gradients as they lie (their rows are the summed index: MN-major).
 //
-// A tile's columns are two halves of 64, each with its own S and dP in TMEM and its
-// own four warps.  The tensor core is given S(j+1) of a half behind its dV(j), and
-// dP(j+1) behind dK(j), so a half's scores are there when its warps come for them,
-// and the two halves fall into turns by themselves.  (Both halves as one 128-column
-// step made the warps wait for the products: 1.55 against MEASURED_HERE ms at 16384
-// tokens, D = 96.)
+// What bounds it is the chain of a step, not the tensor core (43 % busy) nor the 2^x
+// (30 %): scores, their reading, 2^x, dS, each handed on through an mbarrier at 150 to
+// 250 cycles.  So the tensor core is given S(j+1) as soon as S(j) has been read, where
+// P has columns of its own, and dP(j+1) behind dK(j); and 16 warps, not 8, share the
+// softmax, as a warp mostly waits on itself.  At 16384 tokens, D = 96, 8 over 4 heads:
+// 8 warps 1.55 ms, 16 warps 1.38 ms, scores ahead and a third stage of tiles 1.30 to
+// 1.37 ms (750 to 800 TFLOP/s, 0.46 to 0.49 of the measured peak); two halves of 64
+// columns with barriers of their own, which overlap better on paper, 2.19 ms, since
+// they double the hand-offs.
 //
 // fp16 has no room for small dS or P: P is held times 2^10, and dS times a power of
 // two from the largest |dO| and |V| of the call that no dS can overflow
@@ -32,8 +35,8 @@
 // neither.
 //
 // Grid, order of the work, masks and tokens outside of the sequences: as in the
-// forward kernel.  Warps 0-7: softmax (two to each quarter of the rows, 64 columns
-// each) and epilogue; 8: TMA; 9: MMA issue.
+// forward kernel.  Warps 0-15: softmax (four to each quarter of the rows, 32 columns
+// each) and epilogue; 16: TMA; 17: MMA issue.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -647,7 +650,7 @@ cudaError_t run(const Args &a, const Map &r1, const Map &r2, const Map &c1, cons
 
 // Into how many the heads of a group are shared out where keys alone make too few
 // pieces of work: two for every SM or all heads apart.  (13 sequences, 8191 tokens, 8
-// heads over 2, D = 64: dK and dV in 166 us with 128 pieces, SPLIT_US with 512.)
+// heads over 2, D = 64: dK and dV in 166 us with 128 pieces, 66 us with 512 and 7 us to join them.)
 int attn_bwd_splits(int64_t T, int H, int Hk) {
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148, G = H / Hk;
   const int64_t tiles = (T + attn::TM - 1) / attn::TM;
