@@ -47,6 +47,28 @@ __device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t ts, 
   }
 }
 
+// The same for fp32 rows at multiples of 16 bytes, as asynchronous copies: the next
+// tile is on its way while this one is worked on.
+template <int DP, int ROWS>
+__device__ __forceinline__ void copy_tile(float *dst, const float *src, int64_t ts, int row0, int D, Span range) {
+#pragma unroll 8
+  for (int e = threadIdx.x; e < ROWS * DP / 4; e += THREADS) {
+    const int r = e / (DP / 4), c = (e - r * (DP / 4)) * 4;
+    const int t = row0 + r;
+    const bool in = t >= range.start && t < range.end && c < D;
+    const float *from = in ? src + (int64_t)t * ts + c : src;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst + r * (DP + 4) + c)), "l"(from),
+                 "r"(in ? 16 : 0)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void copy_word(float *dst, const float *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
 // s[i][j] = sum_d A[ty*R+i][d] B[tx+16j][d], even and odd d apart until the end
 template <int DP, int R>
 __device__ __forceinline__ void scores(const float *A, const float *B, int ty, int tx, float (&s)[R][4]) {
@@ -127,11 +149,12 @@ __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, 
   }
 }
 
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, bool ASYNC>
 __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a) {
   constexpr int R = ROWS / 16;
   extern __shared__ float sm[];
-  float *Q = sm, *K = Q + ROWS * (DP + 4), *V = K + TILE * (DP + 4), *P = V + TILE * (DP + 4);
+  constexpr int TS = TILE * (DP + 4);
+  float *Q = sm, *P = Q + ROWS * (DP + 4), *KV = P + ROWS * PP;  // ASYNC: two pairs of tiles
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * ROWS;  // longest rows first
   const int h = blockIdx.y, hk = h / (a.H / a.Hk);
@@ -151,11 +174,33 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
     sum[i] = 0.f;
   }
   const int first = span_of(a, q0).start, last = min((int64_t)q0 + ROWS, a.T);
+  auto fetch = [&](int k0, int buf) {
+    const T *kp = static_cast<const T *>(a.k) + hk * a.kh, *vp = static_cast<const T *>(a.v) + hk * a.vh;
+    if constexpr (ASYNC) {
+      copy_tile<DP, TILE>(KV + 2 * buf * TS, kp, a.kt, k0, a.D, range);
+      copy_tile<DP, TILE>(KV + (2 * buf + 1) * TS, vp, a.vt, k0, a.D, range);
+    } else {
+      load_tile<T, DP, TILE>(KV, kp, a.kt, k0, a.D, range);
+      load_tile<T, DP, TILE>(KV + TS, vp, a.vt, k0, a.D, range);
+    }
+  };
+  if (ASYNC) {
+    if (first < last) fetch(first, 0);
+    copies_done();
+  }
+  int buf = 0;
   for (int k0 = first; k0 < last; k0 += TILE) {
+    __syncthreads();  // the tile before last is done with
+    if (ASYNC) {
+      if (k0 + TILE < last) fetch(k0 + TILE, buf ^ 1);
+      copies_done();
+      copies_wait<1>();
+    } else {
+      fetch(k0, 0);
+    }
     __syncthreads();
-    load_tile<T, DP, TILE>(K, static_cast<const T *>(a.k) + hk * a.kh, a.kt, k0, a.D, range);
-    load_tile<T, DP, TILE>(V, static_cast<const T *>(a.v) + hk * a.vh, a.vt, k0, a.D, range);
-    __syncthreads();
+    const float *K = KV + 2 * buf * TS, *V = K + TS;
+    if (ASYNC) buf ^= 1;
     float s[R][4];
     scores<DP, R>(Q, K, ty, tx, s);
 #pragma unroll
@@ -203,12 +248,13 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
 // that see them, of every head of the group.
-template <typename T, int DP, int ROWS, bool DKV>
+template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
 __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a) {
   constexpr int R = ROWS / 16;
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4), RS = ROWS * (DP + 4);
-  float *R1 = sm, *R2 = R1 + RS, *C1 = R2 + RS, *C2 = C1 + TS, *W = C2 + TS, *L = W + ROWS * PP, *Dl = L + TILE;
+  constexpr int STAGE = 2 * TS + 2 * TILE;  // two tiles, lse and D; ASYNC: two stages
+  float *R1 = sm, *R2 = R1 + RS, *W = R2 + RS, *CS = W + ROWS * PP;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int r0 = (int)(DKV ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * ROWS;
   const int G = a.H / a.Hk;
@@ -235,23 +281,51 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
   const int64_t end_rows = min((int64_t)r0 + ROWS, a.T);
   const int first = DKV ? r0 : span_of(a, r0).start;
   const int last = DKV ? span_of(a, (int)end_rows - 1).end : (int)end_rows;
-  for (int g = 0; g < (DKV ? G : 1); ++g) {
-    const int h = DKV ? rh * G + g : rh;
-    for (int c0 = first; c0 < last; c0 += TILE) {
-      __syncthreads();
-      if (DKV) {
-        load_tile<T, DP, TILE>(C1, q + h * a.qh, a.qt, c0, a.D, range);
-        load_tile<T, DP, TILE>(C2, dout + (int64_t)h * a.D, ot, c0, a.D, range);
+  const int tiles = last > first ? (last - first + TILE - 1) / TILE : 0, n = tiles * (DKV ? G : 1);
+  auto fetch = [&](int it, int buf) {
+    const int h = DKV ? rh * G + it / tiles : rh, c0 = first + it % tiles * TILE;
+    float *c1 = CS + buf * STAGE, *c2 = c1 + TS, *l = c2 + TS, *d = l + TILE;
+    const T *s1 = DKV ? q + h * a.qh : k + (rh / G) * a.kh, *s2 = DKV ? dout + (int64_t)h * a.D : v + (rh / G) * a.vh;
+    const int64_t t1 = DKV ? a.qt : a.kt, t2 = DKV ? ot : a.vt;
+    if constexpr (ASYNC) {
+      copy_tile<DP, TILE>(c1, s1, t1, c0, a.D, range);
+      copy_tile<DP, TILE>(c2, s2, t2, c0, a.D, range);
+    } else {
+      load_tile<T, DP, TILE>(c1, s1, t1, c0, a.D, range);
+      load_tile<T, DP, TILE>(c2, s2, t2, c0, a.D, range);
+    }
+    if (tid < TILE) {  // lse and D of the tile's columns, or of the block's rows
+      const int64_t t = (DKV ? c0 : r0) + tid;
+      const bool in = t < a.T;
+      const int64_t at = (int64_t)h * a.Tp + (in ? t : 0);
+      if (ASYNC) {
+        copy_word(l + tid, a.lse + at, in);
+        copy_word(d + tid, a.delta + at, in);
       } else {
-        load_tile<T, DP, TILE>(C1, k + (rh / G) * a.kh, a.kt, c0, a.D, range);
-        load_tile<T, DP, TILE>(C2, v + (rh / G) * a.vh, a.vt, c0, a.D, range);
+        l[tid] = in ? a.lse[at] : 0.f;
+        d[tid] = in ? a.delta[at] : 0.f;
       }
-      if (tid < TILE) {
-        const int64_t t = (DKV ? c0 : r0) + tid;
-        L[tid] = t < a.T ? a.lse[(int64_t)h * a.Tp + t] : INFINITY;
-        Dl[tid] = t < a.T ? a.delta[(int64_t)h * a.Tp + t] : 0.f;
+    }
+  };
+  if (ASYNC) {
+    if (n > 0) fetch(0, 0);
+    copies_done();
+  }
+  {
+    int buf = 0;
+    for (int it = 0; it < n; ++it) {
+      const int c0 = first + it % tiles * TILE;
+      __syncthreads();  // the tile before last is done with
+      if (ASYNC) {
+        if (it + 1 < n) fetch(it + 1, buf ^ 1);
+        copies_done();
+        copies_wait<1>();
+      } else {
+        fetch(it, 0);
       }
       __syncthreads();
+      const float *C1 = CS + buf * STAGE, *C2 = C1 + TS, *L = C2 + TS, *Dl = L + TILE;
+      if (ASYNC) buf ^= 1;
       float p[R][4], ds[R][4];
       scores<DP, R>(R1, C1, ty, tx, p);
       scores<DP, R>(R2, C2, ty, tx, ds);
@@ -396,24 +470,55 @@ static bool short_rows(int64_t T, int heads) {
   return (T + TILE - 1) / TILE * heads < 4 * (int64_t)sms;
 }
 
-template <typename T, int DP, int ROWS>
+// whether every row of the tensors the kernels walk begins at a multiple of 16 bytes
+static bool fp32_rows(const Args &a, bool backward) {
+  const uintptr_t ps = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (backward ? (uintptr_t)a.dout : 0);
+  return a.dtype == MHC_F32 && !(ps & 15) && !((a.qt | a.qh | a.kt | a.kh | a.vt | a.vh | a.D) & 3);
+}
+
+template <typename T, int DP, int ROWS, bool ASYNC>
 static cudaError_t run_fwd(const Args &a, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)((ROWS + 2 * TILE) * (DP + 4) + ROWS * PP) * 4;
-  cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP, ROWS>>(smem);
+  constexpr size_t smem = (size_t)((ROWS + (ASYNC ? 4 : 2) * TILE) * (DP + 4) + ROWS * PP) * 4;
+  static_assert(smem <= 232448, "shared memory of a block");
+  cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP, ROWS, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)a.H);
-  attn_fwd_generic_kernel<T, DP, ROWS><<<grid, THREADS, smem, stream>>>(a);
+  attn_fwd_generic_kernel<T, DP, ROWS, ASYNC><<<grid, THREADS, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, int DP, int ROWS, bool DKV>
+template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
 static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)(2 * (ROWS + TILE) * (DP + 4) + ROWS * PP + 2 * TILE) * 4;
-  cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, ROWS, DKV>>(smem);
+  constexpr size_t smem = (size_t)(2 * ROWS * (DP + 4) + ROWS * PP + (ASYNC ? 2 : 1) * 2 * TILE * (DP + 5)) * 4;
+  static_assert(smem <= 232448, "shared memory of a block");
+  cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)(DKV ? a.Hk : a.H));
-  attn_bwd_generic_kernel<T, DP, ROWS, DKV><<<grid, THREADS, smem, stream>>>(a);
+  attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, THREADS, smem, stream>>>(a);
   return cudaGetLastError();
+}
+
+// blocks of 32 or 64 rows, copied or loaded tiles.  Two stages of D = 128 with 64 rows
+// do not fit: those stay with 32.
+template <typename T, int DP>
+static cudaError_t pick_fwd(const Args &a, cudaStream_t stream) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (fp32_rows(a, false))
+      return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, true>(a, stream) : run_fwd<T, DP, 64, true>(a, stream);
+  }
+  return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, false>(a, stream) : run_fwd<T, DP, 64, false>(a, stream);
+}
+template <typename T, int DP, bool DKV>
+static cudaError_t pick_bwd(const Args &a, cudaStream_t stream) {
+  const bool few = short_rows(a.T, DKV ? a.Hk : a.H);
+  if constexpr (std::is_same<T, float>::value) {
+    if (fp32_rows(a, true)) {
+      if constexpr (DP <= 96)
+        if (!few) return run_bwd<T, DP, 64, DKV, true>(a, stream);
+      return run_bwd<T, DP, 32, DKV, true>(a, stream);
+    }
+  }
+  return few ? run_bwd<T, DP, 32, DKV, false>(a, stream) : run_bwd<T, DP, 64, DKV, false>(a, stream);
 }
 
 }  // namespace attn
@@ -421,10 +526,7 @@ static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
 cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
-      constexpr int DP = decltype(d)::value;
-      return attn::short_rows(a.T, a.H) ? attn::run_fwd<T, DP, 32>(a, stream) : attn::run_fwd<T, DP, 64>(a, stream);
-    });
+    return attn::with_dim(a.D, [&](auto d) -> cudaError_t { return attn::pick_fwd<T, decltype(d)::value>(a, stream); });
   });
 }
 
@@ -449,11 +551,8 @@ cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream) {
     using T = decltype(tag);
     return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
       constexpr int DP = decltype(d)::value;
-      const cudaError_t e = attn::short_rows(a.T, a.H) ? attn::run_bwd<T, DP, 32, false>(a, stream)
-                                                       : attn::run_bwd<T, DP, 64, false>(a, stream);
-      if (e != cudaSuccess) return e;
-      return attn::short_rows(a.T, a.Hk) ? attn::run_bwd<T, DP, 32, true>(a, stream)
-                                         : attn::run_bwd<T, DP, 64, true>(a, stream);
+      const cudaError_t e = attn::pick_bwd<T, DP, false>(a, stream);
+      return e != cudaSuccess ? e : attn::pick_bwd<T, DP, true>(a, stream);
     });
   });
 }
