@@ -17,7 +17,7 @@ is 2.03 bytes a value instead of 8.
 from __future__ import annotations
 
 from array import array
-from itertools import chain, repeat
+from operator import attrgetter, or_
 from typing import NamedTuple
 
 import torch
@@ -62,25 +62,37 @@ def unpack_moment(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return out
 
 
+_FLOATS = frozenset(_CODE)
+_F32 = frozenset((torch.float32,))
+_POINTER, _NUMEL, _DEVICE, _CONTIGUOUS = _Tensor.data_ptr, _Tensor.numel, _Tensor.get_device, _Tensor.is_contiguous
+_DTYPE = attrgetter("dtype")
+_WORDS = 9  # of 8 bytes, one mhc_adamw_tensor
+
+
+# The host side of a step grows with the number of tensors, not with their size: every check is one pass in C over a
+# list, and a column of the table is one slice assignment.
+
 def _check_list(what, ts, sizes, index, dtypes):
+    """The tensors' types, after making sure the kernels may read and write all of them."""
     if len(ts) != len(sizes):
         raise ValueError(f"adamw: {len(sizes)} params but {len(ts)} {what}")
-    found = {t.dtype for t in ts}
+    found = set(map(_DTYPE, ts))
     if not found <= dtypes:
         raise TypeError(f"adamw: {what} must be {' / '.join(sorted(str(d) for d in dtypes))}, got "
                         f"{', '.join(sorted(str(d) for d in found - dtypes))}")
-    if set(map(_Tensor.get_device, ts)) != {index}:
+    if set(map(_DEVICE, ts)) != {index}:
         raise ValueError(f"adamw: every tensor must be on cuda:{index}; {what} are not")
-    if not all(map(_Tensor.is_contiguous, ts)):
+    if False in map(_CONTIGUOUS, ts):
         raise ValueError(f"adamw: {what} must be contiguous")
-    if list(map(_Tensor.numel, ts)) != sizes:
+    if list(map(_NUMEL, ts)) != sizes:
         raise ValueError(f"adamw: {what} and params differ in size")
+    return found
 
 
-_FLOATS = frozenset(_CODE)
-_F32 = frozenset((torch.float32,))
-_POINTER = _Tensor.data_ptr
-_WORDS = 9  # of 8 bytes, one mhc_adamw_tensor
+def _codes_of(ts, found, shift):
+    if len(found) == 1:
+        return [_CODE[next(iter(found))] << shift] * len(ts)
+    return [_CODE[d] << shift for d in map(_DTYPE, ts)]
 
 
 def _table(params, grads, ms, vs, steps, bits):
@@ -90,26 +102,33 @@ def _table(params, grads, ms, vs, steps, bits):
         raise ValueError(f"adamw: {count} params, {len(grads)} grads, {len(ms)} and {len(vs)} moments")
     nat.require_cuda(params[0])
     index = params[0].get_device()
-    sizes = list(map(_Tensor.numel, params))
-    _check_list("params", params, sizes, index, _FLOATS)
-    _check_list("grads", grads, sizes, index, _FLOATS)
+    sizes = list(map(_NUMEL, params))
+    ptypes = _check_list("params", params, sizes, index, _FLOATS)
+    gtypes = _check_list("grads", grads, sizes, index, _FLOATS)
+    table = array("Q", bytes(8 * _WORDS * count))
+
+    def column(i, values):
+        table[i::_WORDS] = array("Q", values)
+
+    column(0, map(_POINTER, params))
+    column(1, map(_POINTER, grads))
     if bits == 32:
         _check_list("exp_avgs", ms, sizes, index, _F32)
         _check_list("exp_avg_sqs", vs, sizes, index, _F32)
-        moments = (map(_POINTER, ms), map(_POINTER, vs), repeat(0), repeat(0))
+        column(2, map(_POINTER, ms))
+        column(3, map(_POINTER, vs))
     else:
         blocks = [-(-n // QUANT_BLOCK) for n in sizes]
-        moments = []
-        for what, pairs, dt in (("exp_avgs", ms, torch.int8), ("exp_avg_sqs", vs, torch.uint8)):
-            codes, scales = [m[0] for m in pairs], [m[1] for m in pairs]
+        for i, what, pairs, dt in ((2, "exp_avgs", ms, torch.int8), (3, "exp_avg_sqs", vs, torch.uint8)):
+            codes, scales = zip(*pairs)
             _check_list(what + " codes", codes, sizes, index, frozenset((dt,)))
             _check_list(what + " scales", scales, blocks, index, _F32)
-            moments += [map(_POINTER, codes), map(_POINTER, scales)]
-        moments = (moments[0], moments[2], moments[1], moments[3])
-    types = [_CODE[p.dtype] | _CODE[g.dtype] << 32 for p, g in zip(params, grads)]
-    steps = steps if isinstance(steps, (list, tuple)) else repeat(int(steps))
-    rows = zip(map(_POINTER, params), map(_POINTER, grads), *moments, sizes, steps, types)
-    return array("Q", chain.from_iterable(rows))
+            column(i, map(_POINTER, codes))
+            column(i + 2, map(_POINTER, scales))
+    column(6, sizes)
+    column(7, steps if isinstance(steps, (list, tuple)) else [int(steps)] * count)
+    column(8, map(or_, _codes_of(params, ptypes, 0), _codes_of(grads, gtypes, 32)))
+    return table
 
 
 def _grad_norm(tables, index):
