@@ -1,7 +1,9 @@
 """Build the sm_100a shared library ``model/libmhc_b200.so`` with nvcc.
 
 The library is the C-ABI boundary declared in ``include/mhc_b200.h``; it links
-only the CUDA runtime (no PyTorch headers), so any FFI can bind it.  Objects go
+only the CUDA runtime (no PyTorch headers), so any FFI can bind it.  Beside it
+``model/_mhc_torch.so`` is compiled from ``csrc/host``: the PyTorch host side of
+the training-step operators, which calls the library through its C header.  Objects go
 to ``_build/`` at the repository root; every translation unit compiles in
 parallel.  Usage::
 
@@ -23,6 +25,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "model", "libmhc_b200.so")
+HOST_LIB = os.path.join(PKG, "model", "_mhc_torch.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
@@ -41,7 +44,8 @@ def sources():
 
 
 def _deps():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "mhc_b200.h")]
+    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))] + [
+        os.path.join(INCLUDE, "mhc_b200.h")]
 
 
 def _stale(target, deps):
@@ -87,9 +91,36 @@ def build(force: bool = False, ptxas_verbose: bool = False, quiet: bool = False)
     return LIB
 
 
+def build_host(force: bool = False, quiet: bool = False) -> str:
+    """The PyTorch host module (a C++ compile against torch's headers, about a minute)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src = os.path.join(CSRC, "host", "mhc_torch.cpp")
+    if not force and not _stale(HOST_LIB, [src, os.path.join(INCLUDE, "mhc_b200.h")]):
+        return HOST_LIB
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    incs = include_paths() + [os.path.join(cuda, "include"), INCLUDE, sysconfig.get_paths()["include"]]
+    libs = library_paths()
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_mhc_torch",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-isystem{i}" for i in incs], src, "-o", HOST_LIB, *[f"-L{p}" for p in libs],
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on mhc_torch.cpp")
+    if not quiet:
+        print(f"built {HOST_LIB}")
+    return HOST_LIB
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--ptxas-verbose", action="store_true")
     a = ap.parse_args()
     build(force=a.force, ptxas_verbose=a.ptxas_verbose)
+    build_host(force=a.force)

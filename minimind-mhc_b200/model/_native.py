@@ -10,6 +10,7 @@ error, raised before anything is launched.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -129,31 +130,46 @@ def stream_of(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-# The raw handle without building a Stream object (2.2 us a call on the host
-# side of a small operator), where torch has the accessor.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# ---------------------------------------------------------------------------
+# The training-step operators' host side (csrc/host/mhc_torch.cpp): checks,
+# allocations and autograd nodes in C++.  It calls whichever libmhc_b200.so this
+# process has loaded, through the addresses handed over here.
+# ---------------------------------------------------------------------------
+
+HOST_PATH = os.path.join(_HERE, "_mhc_torch.so")
+# in the order of the module's table
+_HOST_ENTRIES = ("mhc_last_error", "mhc_attn_lse_pitch", "mhc_attn_fwd_workspace", "mhc_attn_fwd",
+                 "mhc_attn_bwd_workspace", "mhc_attn_bwd", "mhc_route_fwd_workspace", "mhc_route_fwd",
+                 "mhc_route_bwd", "mhc_grad_norm_workspace", "mhc_grad_norm", "mhc_adamw_step")
+_host = None
 
 
-def raw_stream(index: int):
-    """The current stream's handle on device ``index``."""
-    if _raw_stream is not None:
-        return _raw_stream(index)
-    return torch.cuda.current_stream(index).cuda_stream
+def host():
+    """The operators' host module, loaded and bound to the library once."""
+    if _host is not None:
+        return _host
+    return _load_host()
 
 
-def call_on(index: int, name: str, *args):
-    """``call`` with device ``index`` current and its current stream as the last argument."""
-    if torch.cuda.current_device() == index:
-        call(name, *args, raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, raw_stream(index))
-
-
-def refuse_double_backward(what: str):
-    """For a backward that autograd must not differentiate again: grad mode is on there only under create_graph."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: second derivatives are not implemented")
+def _load_host():
+    global _host
+    with _lock:
+        if _host is None:
+            if not os.path.exists(HOST_PATH):
+                raise RuntimeError(f"mHC host module not found at {HOST_PATH}; build it with "
+                                   f"`python minimind-mhc_b200/build.py`")
+            spec = importlib.util.spec_from_file_location("_mhc_torch", HOST_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            handle = lib()
+            module.bind([ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
+            if torch.cuda.is_available():
+                _register_error_flag()
+                module.set_flag(_flag_tensor.data_ptr())
+                _host = module
+            else:
+                return module  # without a device the checks still answer; asked again once there is one
+        return _host
 
 
 def require_cuda(*ts):

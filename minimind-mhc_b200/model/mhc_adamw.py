@@ -16,8 +16,6 @@ is 2.03 bytes a value instead of 8.
 
 from __future__ import annotations
 
-from array import array
-from operator import attrgetter, or_
 from typing import NamedTuple
 
 import torch
@@ -25,9 +23,6 @@ import torch
 from . import _native as nat
 
 QUANT_BLOCK = 256  # values that share a scale
-
-_Tensor = torch.Tensor
-_CODE = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
 
 
 class Moment8(NamedTuple):
@@ -56,125 +51,26 @@ def unpack_moment(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     if scales.device != codes.device:
         raise ValueError("unpack_moment: codes and scales are on different devices")
     codes, scales = codes.contiguous(), scales.contiguous()
-    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
-    nat.call_on(codes.get_device(), "mhc_adamw_unpack", codes.data_ptr(), int(codes.dtype == torch.int8),
-                scales.data_ptr(), out.data_ptr(), n)
+    with torch.cuda.device(codes.device):
+        out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+        nat.call("mhc_adamw_unpack", codes.data_ptr(), int(codes.dtype == torch.int8), scales.data_ptr(),
+                 out.data_ptr(), n, nat.stream_of(codes))
     return out
 
 
-_FLOATS = frozenset(_CODE)
-_F32 = frozenset((torch.float32,))
-_POINTER, _NUMEL, _DEVICE, _CONTIGUOUS = _Tensor.data_ptr, _Tensor.numel, _Tensor.get_device, _Tensor.is_contiguous
-_DTYPE = attrgetter("dtype")
-_WORDS = 9  # of 8 bytes, one mhc_adamw_tensor
-
-
-# The host side of a step grows with the number of tensors, not with their size: every check is one pass in C over a
-# list, and a column of the table is one slice assignment.
-
-def _check_list(what, ts, sizes, index, dtypes):
-    """The tensors' types, after making sure the kernels may read and write all of them."""
-    if len(ts) != len(sizes):
-        raise ValueError(f"adamw: {len(sizes)} params but {len(ts)} {what}")
-    found = set(map(_DTYPE, ts))
-    if not found <= dtypes:
-        raise TypeError(f"adamw: {what} must be {' / '.join(sorted(str(d) for d in dtypes))}, got "
-                        f"{', '.join(sorted(str(d) for d in found - dtypes))}")
-    if set(map(_DEVICE, ts)) != {index}:
-        raise ValueError(f"adamw: every tensor must be on cuda:{index}; {what} are not")
-    if False in map(_CONTIGUOUS, ts):
-        raise ValueError(f"adamw: {what} must be contiguous")
-    if list(map(_NUMEL, ts)) != sizes:
-        raise ValueError(f"adamw: {what} and params differ in size")
-    return found
-
-
-def _codes_of(ts, found, shift):
-    if len(found) == 1:
-        return [_CODE[next(iter(found))] << shift] * len(ts)
-    return [_CODE[d] << shift for d in map(_DTYPE, ts)]
-
-
-def _table(params, grads, ms, vs, steps, bits):
-    """The host array of ``mhc_adamw_tensor`` of checked tensors."""
-    count = len(params)
-    if len(grads) != count or len(ms) != count or len(vs) != count:
-        raise ValueError(f"adamw: {count} params, {len(grads)} grads, {len(ms)} and {len(vs)} moments")
-    nat.require_cuda(params[0])
-    index = params[0].get_device()
-    sizes = list(map(_NUMEL, params))
-    ptypes = _check_list("params", params, sizes, index, _FLOATS)
-    gtypes = _check_list("grads", grads, sizes, index, _FLOATS)
-    table = array("Q", bytes(8 * _WORDS * count))
-
-    def column(i, values):
-        table[i::_WORDS] = array("Q", values)
-
-    column(0, map(_POINTER, params))
-    column(1, map(_POINTER, grads))
-    if bits == 32:
-        _check_list("exp_avgs", ms, sizes, index, _F32)
-        _check_list("exp_avg_sqs", vs, sizes, index, _F32)
-        column(2, map(_POINTER, ms))
-        column(3, map(_POINTER, vs))
-    else:
-        blocks = [-(-n // QUANT_BLOCK) for n in sizes]
-        for i, what, pairs, dt in ((2, "exp_avgs", ms, torch.int8), (3, "exp_avg_sqs", vs, torch.uint8)):
-            codes, scales = zip(*pairs)
-            _check_list(what + " codes", codes, sizes, index, frozenset((dt,)))
-            _check_list(what + " scales", scales, blocks, index, _F32)
-            column(i, map(_POINTER, codes))
-            column(i + 2, map(_POINTER, scales))
-    column(6, sizes)
-    column(7, steps if isinstance(steps, (list, tuple)) else [int(steps)] * count)
-    column(8, map(or_, _codes_of(params, ptypes, 0), _codes_of(grads, gtypes, 32)))
-    return table
-
-
-def _grad_norm(tables, index):
-    """The workspace that holds the squared norm of all the tables' gradients."""
-    ws = nat.workspace(nat.lib().mhc_grad_norm_workspace(), torch.device("cuda", index))
-    for i, t in enumerate(tables):
-        nat.call("mhc_grad_norm", t.buffer_info()[0], len(t) // _WORDS, int(i > 0), ws.data_ptr(), ws.numel(),
-                 nat.raw_stream(index))
-    return ws
-
-
-def _run(table, bits, index, lr, betas, eps, weight_decay, max_grad_norm, norm_ws, norm):
-    nat.call("mhc_adamw_step", table.buffer_info()[0], len(table) // _WORDS, bits, lr, betas[0], betas[1], eps,
-             weight_decay, max_grad_norm or 0.0, nat.ptr(norm_ws), nat.ptr(norm), nat.raw_stream(index))
-
-
-def _run_all(tables, bits, index, max_grad_norm):
-    """Steps the (table, hyperparameters) pairs under one norm; returns it."""
-    if torch.cuda.current_device() != index:
-        with torch.cuda.device(index):
-            return _run_all(tables, bits, index, max_grad_norm)
-    norm_ws = norm = None
-    if max_grad_norm is not None:
-        norm_ws = _grad_norm([t for t, _ in tables], index)
-        # written by the step, unless there is nothing to step
-        make = torch.empty if any(any(t[6::_WORDS]) for t, _ in tables) else torch.zeros
-        norm = make((), dtype=torch.float32, device=norm_ws.device)
-    for table, hyper in tables:
-        _run(table, bits, index, *hyper, max_grad_norm, norm_ws, norm)
-    return norm
-
-
-def _check_call(max_grad_norm):
-    if max_grad_norm is not None and not max_grad_norm > 0:
-        raise ValueError(f"adamw: max_grad_norm must be positive or None, got {max_grad_norm}")
-    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw: the step number is an argument of the launch, so a step cannot be captured in a "
-                           "CUDA graph")
+def _group(params, grads, ms, vs, steps, bits, lr, betas, eps, weight_decay):
+    """One group of tensors as the host module takes it."""
+    mscales = vscales = []
+    if bits == 8:
+        ms, mscales = zip(*ms) if ms else ([], [])
+        vs, vscales = zip(*vs) if vs else ([], [])
+    return params, grads, ms, vs, mscales, vscales, steps, lr, betas[0], betas[1], eps, weight_decay
 
 
 def _step(params, grads, ms, vs, bits, step, lr, betas, eps, weight_decay, max_grad_norm):
-    _check_call(max_grad_norm)
-    if not params:
-        return None
-    table = _table(params, grads, ms, vs, step, bits)
-    return _run_all([(table, (lr, betas, eps, weight_decay))], bits, params[0].get_device(), max_grad_norm)
+    steps = list(step) if isinstance(step, (list, tuple)) else [int(step)]
+    return nat.host().adamw([_group(params, grads, ms, vs, steps, bits, lr, betas, eps, weight_decay)], bits,
+                            max_grad_norm)
 
 
 @torch.no_grad()
@@ -216,7 +112,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
             raise ValueError("AdamW: lr, eps, weight_decay >= 0 and betas in [0, 1) are wanted")
-        _check_call(max_grad_norm)
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"AdamW: max_grad_norm must be positive or None, got {max_grad_norm}")
         self.state_bits = state_bits
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None
@@ -240,8 +137,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        _check_call(self.max_grad_norm)
-        work, keep, states = [], [], []
+        work, states = [], []
         for group in self.param_groups:
             live = [p for p in group["params"] if p.grad is not None]
             if not live:
@@ -253,16 +149,12 @@ class AdamW(torch.optim.Optimizer):
             else:
                 ms = [(s["exp_avg"], s["exp_avg_scale"]) for s in mine]
                 vs = [(s["exp_avg_sq"], s["exp_avg_sq_scale"]) for s in mine]
-            work.append((_table(live, grads, ms, vs, [s["step"] + 1 for s in mine], self.state_bits),
-                         (group["lr"], group["betas"], group["eps"], group["weight_decay"])))
+            work.append(_group(live, grads, ms, vs, [s["step"] + 1 for s in mine], self.state_bits, group["lr"],
+                               group["betas"], group["eps"], group["weight_decay"]))
             states += mine
-            keep.append((live[0].get_device(), grads))
         if not work:
             return loss
-        index = keep[0][0]
-        if any(d != index for d, _ in keep):
-            raise ValueError("AdamW: all parameters must be on one device")
-        self.grad_norm = _run_all(work, self.state_bits, index, self.max_grad_norm)
+        self.grad_norm = nat.host().adamw(work, self.state_bits, self.max_grad_norm)
         for s in states:
             s["step"] += 1
         return loss

@@ -11,7 +11,7 @@ import torch
 @pytest.fixture(scope="module")
 def lib():
     from model import _native
-    if not os.path.exists(_native.LIB_PATH):
+    if not os.path.exists(_native.LIB_PATH) or not os.path.exists(_native.HOST_PATH):
         import __graft_entry__
         __graft_entry__.build()
     return _native.load_library()
@@ -105,7 +105,7 @@ def test_adamw_refusals(lib):
     assert lib.mhc_adamw_unpack(None, 1, None, None, 0, None) == 0
 
 
-def test_python_refuses_cpu_tensors():
+def test_python_refuses_cpu_tensors(lib):
     from model.mhc_adamw import AdamW, adamw_step, unpack_moment
     from model.mhc_attention import packed_attention
     from model.mhc_router import route_topk
