@@ -7,6 +7,7 @@
 // step over 14 tensors 57 (20).  The library itself stays free of
 // PyTorch: this file is compiled against its C header only and receives the entry
 // points' addresses (bind), so it works on whichever library the process has loaded.
+#include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -141,9 +142,14 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   }
 };
 
-Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const std::optional<Tensor> &cu_seqlens,
-                        std::optional<double> scale_) {
+Tensor packed_attention(Tensor q, Tensor k, Tensor v, const std::optional<Tensor> &cu_seqlens, std::optional<double> scale_) {
   const char *who = "packed_attention";
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {  // as scaled_dot_product_attention under autocast
+    const at::ScalarType to = at::autocast::get_autocast_dtype(at::kCUDA);
+    q = at::autocast::cached_cast(to, q, at::kCUDA);
+    k = at::autocast::cached_cast(to, k, at::kCUDA);
+    v = at::autocast::cached_cast(to, v, at::kCUDA);
+  }
   const bool packed = cu_seqlens.has_value();
   for (const Tensor *t : {&q, &k, &v}) require_cuda(*t);
   if (packed) require_cuda(*cu_seqlens);
@@ -352,6 +358,10 @@ std::optional<Tensor> adamw(const std::vector<Group> &groups, int bits, std::opt
   for (size_t i = 0; i < tables.size(); ++i) {
     if (tables[i].empty()) continue;
     const Group &g = groups[i];
+    // written in place, as autograd sees it: a graph that saved one of them must not run on the new values
+    for (const Tensors *ts : {&std::get<0>(g), &std::get<2>(g), &std::get<3>(g), &std::get<4>(g), &std::get<5>(g)})
+      for (const Tensor &t : *ts)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     check(E.adamw_step(tables[i].data(), (int)tables[i].size(), bits, std::get<7>(g), std::get<8>(g), std::get<9>(g), std::get<10>(g),
                        std::get<11>(g), max_norm.value_or(0.0), ptr(ws), static_cast<float *>(ptr(norm)), stream),
           "mhc_adamw_step");

@@ -26,8 +26,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     device, the sequences' offsets; or q (B, L, H, D) with k, v (B, L, Hk, D)
     and no ``cu_seqlens``.  H is a multiple of Hk, D at most 128; fp32, bf16 or
     fp16, all three alike; rows may lie at any strides (slices of one
-    projection's output are read in place).  ``scale`` defaults to
-    ``D ** -0.5``.
+    projection's output are read in place).  Under autocast all three are cast
+    to its type, as ``scaled_dot_product_attention`` does.  ``scale`` defaults
+    to ``D ** -0.5``.
 
     Sequences may be empty.  Tokens before ``cu_seqlens[0]`` or from
     ``cu_seqlens[-1]`` on belong to none: their output and gradients are 0, and

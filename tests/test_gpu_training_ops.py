@@ -85,3 +85,26 @@ def test_second_derivatives_are_refused():
     z = torch.randn(4, 8, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError, match="second derivatives"):
         torch.autograd.grad(route_topk(z, 2, 1.0).weights.square().sum(), z, create_graph=True)
+
+
+def test_attention_under_autocast_takes_the_autocast_type():
+    from model.mhc_attention import packed_attention
+    q = torch.randn(1, 50, 4, 64, device="cuda", requires_grad=True)
+    v = torch.randn(1, 50, 4, 64, device="cuda").bfloat16()
+    with torch.autocast("cuda", torch.bfloat16):
+        out = packed_attention(q, q, v)  # fp32 queries beside bf16 values
+    assert out.dtype == torch.bfloat16
+    assert torch.equal(out, packed_attention(q.detach().bfloat16(), q.detach().bfloat16(), v))
+    g, = torch.autograd.grad(out.float().sum(), q)
+    assert g.dtype == torch.float32 and torch.isfinite(g).all()
+
+
+def test_a_step_counts_as_an_in_place_change():
+    """Autograd refuses a backward through a parameter that the step has changed since."""
+    from model.mhc_adamw import adamw_step
+    p = torch.randn(8, device="cuda", requires_grad=True)
+    y = (p * p).sum()
+    m, v = torch.zeros(8, device="cuda"), torch.zeros(8, device="cuda")
+    adamw_step([p], [torch.ones(8, device="cuda")], [m], [v], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
