@@ -375,60 +375,57 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
 
 // D_i = dO_i . O_i.  O is its rounded value plus what the rounding left over: D is
 // subtracted from dO . V, of which it is the mean, so with few keys the rounding of
-// O alone would show in dS as an error of its own size.  16 lanes a row, a block 128
-// tokens of one head; it reads O, its rest and dO once and is bound by that.
-// fp16: also the largest |dO| and |V| inside of the sequences.
+// O alone would show in dS as an error of its own size.  Four lanes a row, the rows
+// of all heads as they lie; it reads O, its rest and dO once, and a lane asks for all
+// of its part before it adds (16 lanes a row, 4 rows in turn: 22 us at 16384 tokens, 8
+// heads of 96; so: 11.6).  fp16: also the largest |dO| and |V| inside of the
+// sequences.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t *amax) {
-  const int h = blockIdx.y, l = threadIdx.x & 15;
-  const Span range = packed_range(a);
+  const int l = threadIdx.x & 3;
   const T *o = static_cast<const T *>(a.out), *lo = static_cast<const T *>(a.out_lo), *d = static_cast<const T *>(a.dout);
-  float most_o = 0.f, most_v = 0.f;
-  constexpr int ROWS = 4;  // in flight at a time
-#pragma unroll 1
-  for (int it = 0; it < 8; it += ROWS) {
-    float s[ROWS] = {};
-    const int64_t t0 = (int64_t)blockIdx.x * 128 + it * 16 + (threadIdx.x >> 4);
-    for (int c = l * VEC; c < a.D; c += 16 * VEC) {
-      T ov[ROWS][VEC], lv[ROWS][VEC], dv[ROWS][VEC];
+  const int64_t row = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2), rows = a.T * a.H;
+  constexpr int MOST = VEC == 8 ? 4 : 1;  // pieces of a row of 128 that a lane has at once
+  float s = 0.f, most_o = 0.f, most_v = 0.f;
+  if (row < rows) {
+    for (int c0 = l * VEC; c0 < a.D; c0 += MOST * 4 * VEC) {
+      T ov[MOST][VEC], lv[MOST][VEC], dv[MOST][VEC];
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const int64_t t = t0 + r * 16;
-        if (t >= a.T) continue;
-        const int64_t at = (t * a.H + h) * a.D + c;
+      for (int u = 0; u < MOST; ++u) {
+        const int c = c0 + u * 4 * VEC;
+        if (c >= a.D) continue;
+        const int64_t at = row * a.D + c;
         if constexpr (VEC == 8) {
-          *reinterpret_cast<uint4 *>(ov[r]) = ldg_stream(o + at);
-          *reinterpret_cast<uint4 *>(dv[r]) = *reinterpret_cast<const uint4 *>(d + at);
-          if (lo) *reinterpret_cast<uint4 *>(lv[r]) = ldg_stream(lo + at);
+          *reinterpret_cast<uint4 *>(ov[u]) = ldg_stream(o + at);
+          *reinterpret_cast<uint4 *>(dv[u]) = *reinterpret_cast<const uint4 *>(d + at);
+          if (lo) *reinterpret_cast<uint4 *>(lv[u]) = ldg_stream(lo + at);
         } else {
-          ov[r][0] = o[at];
-          dv[r][0] = d[at];
-          if (lo) lv[r][0] = lo[at];
+          ov[u][0] = o[at];
+          dv[u][0] = d[at];
+          if (lo) lv[u][0] = lo[at];
         }
       }
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const int64_t t = t0 + r * 16;
-        if (t >= a.T) continue;
+      for (int u = 0; u < MOST; ++u) {
+        if (c0 + u * 4 * VEC >= a.D) continue;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          s[r] = fmaf(to_f(ov[r][e]) + (lo ? to_f(lv[r][e]) : 0.f), to_f(dv[r][e]), s[r]);
-          if (amax && t >= range.start && t < range.end) most_o = fmaxf(most_o, fabsf(to_f(dv[r][e])));
+          s = fmaf(to_f(ov[u][e]) + (lo ? to_f(lv[u][e]) : 0.f), to_f(dv[u][e]), s);
+          if (amax) most_o = fmaxf(most_o, fabsf(to_f(dv[u][e])));
         }
       }
     }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-#pragma unroll
-      for (int x = 8; x; x >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], x, 16);
-      const int64_t t = t0 + r * 16;
-      if (t >= a.T) continue;
-      if (l == 0) a.delta[(int64_t)h * a.Tp + t] = s[r];
-      if (amax && t >= range.start && t < range.end && h < a.Hk)
-        for (int c = l; c < a.D; c += 16) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
-    }
   }
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  const int64_t t = row / a.H, h = row - t * a.H;
+  if (row < rows && l == 0) a.delta[h * a.Tp + t] = s;
   if (amax) {
+    const Span range = packed_range(a);
+    if (row >= rows || t < range.start || t >= range.end)
+      most_o = 0.f;
+    else if (h < a.Hk)
+      for (int c = l; c < a.D; c += 4) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
 #pragma unroll
     for (int x = 16; x; x >>= 1) {
       most_o = fmaxf(most_o, __shfl_xor_sync(0xffffffffu, most_o, x));
@@ -531,7 +528,9 @@ cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
 }
 
 cudaError_t launch_attn_delta(const attn::Args &a, uint32_t *amax, cudaStream_t stream) {
-  const dim3 grid((unsigned)((a.T + 127) / 128), (unsigned)a.H);
+  const int64_t blocks = (a.T * a.H + 63) / 64;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)blocks);
   const bool vec = a.D % 8 == 0 && !(((uintptr_t)a.out | (uintptr_t)a.out_lo | (uintptr_t)a.dout) & 15);
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
