@@ -418,10 +418,15 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t 
   }
   s += __shfl_xor_sync(0xffffffffu, s, 1);
   s += __shfl_xor_sync(0xffffffffu, s, 2);
+  // the rest of the last tile, which the kernels load with it
+  const int64_t pad = a.Tp - a.T;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pad * a.H; i += (int64_t)gridDim.x * 256)
+    a.delta[i / pad * a.Tp + a.T + i % pad] = 0.f;
   const int64_t t = row / a.H, h = row - t * a.H;
-  if (row < rows && l == 0) a.delta[h * a.Tp + t] = s;
+  const Span range = packed_range(a);
+  // outside of the sequences dO may hold anything; there D must not make a NaN of P = 0 times dP - D
+  if (row < rows && l == 0) a.delta[h * a.Tp + t] = t >= range.start && t < range.end ? s : 0.f;
   if (amax) {
-    const Span range = packed_range(a);
     if (row >= rows || t < range.start || t >= range.end)
       most_o = 0.f;
     else if (h < a.Hk)

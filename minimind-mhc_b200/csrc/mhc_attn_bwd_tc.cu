@@ -240,10 +240,21 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       if (it.n == 0) continue;
       if (!WAIT_WARP(BAR(B_RE), ((uint32_t)rn & 1u) ^ 1u)) { ok = false; break; }
       ++rn;
+      // rows of tokens outside of the sequences are zeroed as well: P = 0 is not enough where dP could be a NaN
+      const bool clean = it.r0 < range.start || min((int64_t)it.r0 + TM, a.T) > range.end;
       if (lane == 0) {
-        mbar_arrive_expect_tx(BAR(B_RF), 2 * C::TILE);
-        load_rows<L>(rs, r1map, it.head, it.r0, BAR(B_RF));
-        load_rows<L>(rs + C::TILE, r2map, it.head, it.r0, BAR(B_RF));
+        const uint32_t bar = BAR(clean ? B_LAND : B_RF);
+        mbar_arrive_expect_tx(bar, 2 * C::TILE);
+        load_rows<L>(rs, r1map, it.head, it.r0, bar);
+        load_rows<L>(rs + C::TILE, r2map, it.head, it.r0, bar);
+      }
+      __syncwarp();
+      if (clean) {
+        if (!WAIT_WARP(BAR(B_LAND), (uint32_t)lands & 1u)) { ok = false; break; }
+        ++lands;
+        zero_outside<L>(gen, it.r0, range, lane);
+        zero_outside<L>(gen + C::TILE, it.r0, range, lane);
+        if (lane == 0) mbar_arrive(BAR(B_RF));
       }
       for (int j = 0; j < it.n && ok; ++j, ++g) {
         const int s = g % ST;
@@ -462,9 +473,10 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           p[e + 3] = exp2_approx(x3);
         }
         if (cut) {
+          const uint32_t seen = bits_between(lo, hi);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (e < lo || e >= hi) p[e] = 0.f;
+            if (!(seen & (1u << e))) p[e] = 0.f;
         }
         if (DKV) {
           uint32_t w[16];
@@ -499,12 +511,6 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           f2_unpack(v, x2, x3);
           if (F16) {
             x0 *= dsf; x1 *= dsf; x2 *= dsf; x3 *= dsf;
-          }
-          if (cut) {  // P = 0 there, but dP or D may be a NaN of a token outside
-            if (e < lo || e >= hi) x0 = 0.f;
-            if (e + 1 < lo || e + 1 >= hi) x1 = 0.f;
-            if (e + 2 < lo || e + 2 >= hi) x2 = 0.f;
-            if (e + 3 < lo || e + 3 >= hi) x3 = 0.f;
           }
           w[e >> 1] = pack2<T>(x0, x1);
           w[(e >> 1) + 1] = pack2<T>(x2, x3);

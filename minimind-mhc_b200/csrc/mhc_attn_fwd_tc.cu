@@ -370,12 +370,13 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
 #pragma unroll
           for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(r[q][e]));  // not read before the wait
         if (__any_sync(0xffffffffu, k0 < start || k0 + TM - 1 > tok)) {
-          const int lo = start - k0, hi = tok - k0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t seen = bits_between(start - k0 - q * 32, tok + 1 - k0 - q * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (q * 32 + e < lo || q * 32 + e > hi) r[q][e] = 0xff800000u;
+              if (!(seen & (1u << e))) r[q][e] = 0xff800000u;
+          }
         }
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

@@ -143,6 +143,14 @@ __device__ __forceinline__ void zero_outside(uint8_t *tile, int row0, Span range
   __syncwarp();
 }
 
+// Bits [lo, hi) of 32: which of a row's columns it sees.  Tested one constant bit at a
+// time they turn into predicates several at once, where comparing each column's index
+// with both ends took three instructions a column.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  const uint32_t below = hi <= 0 ? 0u : (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u);
+  return lo <= 0 ? below : (lo >= 32 ? 0u : below & (0xffffffffu << lo));
+}
+
 // rank of the i-th piece of work of a block among pieces sorted by size: forwards and
 // backwards in turn, so that every block's pieces sum to nearly the same
 __device__ __forceinline__ int64_t snake(int i, int block, int blocks) {
