@@ -94,15 +94,16 @@ __device__ __forceinline__ int lane_value(int lane, int e) { return (e >> 2) * 1
 struct Raw {
   uint4 a, b;  // 16-bit types: the lower halves
 };
+template <bool KEEP = false>  // for another pass over the same values
 __device__ __forceinline__ Raw load_raw(const void *p, int dt, int64_t base, int lane) {
   Raw r;
   if (dt == MHC_F32) {
-    const float *q = static_cast<const float *>(p) + base + lane * 4;
-    r.a = __ldcs(reinterpret_cast<const uint4 *>(q));
-    r.b = __ldcs(reinterpret_cast<const uint4 *>(q + 128));
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + base + lane * 4);
+    r.a = KEEP ? __ldg(q) : __ldcs(q);
+    r.b = KEEP ? __ldg(q + 32) : __ldcs(q + 32);
   } else {
-    const uint16_t *q = static_cast<const uint16_t *>(p) + base + lane * 4;
-    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(q)), y = __ldcs(reinterpret_cast<const uint2 *>(q + 128));
+    const uint2 *q = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + base + lane * 4);
+    const uint2 x = KEEP ? __ldg(q) : __ldcs(q), y = KEEP ? __ldg(q + 32) : __ldcs(q + 32);
     r.a.x = x.x; r.a.y = x.y;
     r.b.x = y.x; r.b.y = y.y;
   }
@@ -300,7 +301,9 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float clip = 1.f;
   if (s.partials) clip = clip_factor(s);
-  for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
+  for (int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    // behind the norm's pass the last gradients are the ones still in L2
+    const int chunk = s.partials ? tab.chunks - 1 - c : c;
     const int ei = entry_of(tab, chunk);
     const Entry &t = tab.t[ei];
     const int64_t first = (int64_t)(chunk - t.first_chunk) * CHUNK;
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constan
       if (base >= t.n) break;
       float g[8];
       if (t.vec && base + QB <= t.n)
-        convert8(load_raw(t.g, t.gdt, base, lane), t.gdt, g);
+        convert8(load_raw<true>(t.g, t.gdt, base, lane), t.gdt, g);
       else
         load_each(t.g, t.gdt, base, t.n, lane, g);
 #pragma unroll
