@@ -6,11 +6,14 @@
 //   dQ_i = scale sum_j dS_ij K_j
 //   dK_j = scale sum_{h in group, i} dS_ij Q_i,   dV_j = sum_{h in group, i} P_ij dO_i
 //
-// fp32 throughout.  A block of 16 x 16 threads owns 64 rows (32 where that leaves SMs
-// with less than four blocks: it is the loads' latency that other blocks then cover)
-// and walks tiles of 64 columns; a thread holds a 4 x 4 piece of the scores and 4 rows
-// x D / 16 columns of the result in registers (half the rows with 32), the operands
-// are staged as fp32 in shared memory and multiplied two at a time (fma.rn.f32x2).
+// fp32 throughout.  A block owns 64 rows (32 where that leaves SMs with less than four
+// blocks: it is the loads' latency that other blocks then cover) and walks tiles of 64
+// columns; a thread, 16 for every 4 rows, holds a 4 x 4 piece of the scores and 4 rows
+// x D / 16 columns of the result in registers, the operands are staged as fp32 in
+// shared memory and multiplied two at a time (fma.rn.f32x2).  A value that a lane
+// reads from shared memory costs a wavefront of the SM, a pair of products half a
+// cycle: 4 rows of a thread rather than 2 (and 256 threads) in blocks of 32 rows took
+// 2 x 512 tokens, 8 heads of 64, from 212 to 171 us, forward and backward.
 // Forward: one pass with the running maximum and sum.  Backward: the scores again
 // from the saved L, in two kernels of the same form (a block owns 64 queries and
 // sums dQ, or 64 keys and sums dK and dV over the heads that share them), so
@@ -32,12 +35,13 @@ namespace mhc {
 namespace attn {
 
 constexpr int TILE = 64;  // columns
-constexpr int THREADS = 256;
+constexpr int R = 4;      // rows of a thread
+constexpr int threads_of(int rows) { return rows / R * 16; }
 constexpr int PP = TILE + 4;  // pitch of a score tile
 
 // ROWS rows of one head as fp32 into shared memory, zero outside of the packed range
 // and past column D
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t ts, int row0, int D, Span range) {
 #pragma unroll 8
   for (int e = threadIdx.x; e < ROWS * DP; e += THREADS) {
@@ -49,7 +53,7 @@ __device__ __forceinline__ void load_tile(float *dst, const T *src, int64_t ts, 
 
 // The same for fp32 rows at multiples of 16 bytes, as asynchronous copies: the next
 // tile is on its way while this one is worked on.
-template <int DP, int ROWS>
+template <int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void copy_tile(float *dst, const float *src, int64_t ts, int row0, int D, Span range) {
 #pragma unroll 8
   for (int e = threadIdx.x; e < ROWS * DP / 4; e += THREADS) {
@@ -70,7 +74,7 @@ template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // s[i][j] = sum_d A[ty*R+i][d] B[tx+16j][d], even and odd d apart until the end
-template <int DP, int R>
+template <int DP>
 __device__ __forceinline__ void scores(const float *A, const float *B, int ty, int tx, float (&s)[R][4]) {
   uint64_t acc[R][4];
 #pragma unroll
@@ -103,7 +107,7 @@ __device__ __forceinline__ void scores(const float *A, const float *B, int ty, i
 }
 
 // acc[i][c] += sum_kk W[ty*R+i][kk] B[kk][2 tx + 32 c, + 1], columns in pairs
-template <int DP, int R>
+template <int DP>
 __device__ __forceinline__ void accumulate(const float *W, const float *B, int ty, int tx, uint64_t (&acc)[R][DP / 32]) {
 #pragma unroll 2
   for (int kk = 0; kk < TILE; kk += 4) {
@@ -127,7 +131,7 @@ __device__ __forceinline__ void accumulate(const float *W, const float *B, int t
 }
 
 // lo != null: what the rounding to T left over, itself in T
-template <typename T, int DP, int R>
+template <typename T, int DP>
 __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, int64_t T_, int D, int ty, int tx,
                                            const uint64_t (&acc)[R][DP / 32], const float (&mul)[R]) {
 #pragma unroll
@@ -150,8 +154,8 @@ __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, 
 }
 
 template <typename T, int DP, int ROWS, bool ASYNC>
-__global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a) {
-  constexpr int R = ROWS / 16;
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(const Args a) {
+  constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4);
   float *Q = sm, *P = Q + ROWS * (DP + 4), *KV = P + ROWS * PP;  // ASYNC: two pairs of tiles
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
     const int t = q0 + ty * R + i;
     start[i] = t < a.T ? span_of(a, t).start : t + 1;
   }
-  load_tile<T, DP, ROWS>(Q, static_cast<const T *>(a.q) + h * a.qh, a.qt, q0, a.D, range);
+  load_tile<T, DP, ROWS, THREADS>(Q, static_cast<const T *>(a.q) + h * a.qh, a.qt, q0, a.D, range);
   uint64_t acc[R][DP / 32] = {};
   float mx[R], sum[R];
 #pragma unroll
@@ -177,11 +181,11 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
   auto fetch = [&](int k0, int buf) {
     const T *kp = static_cast<const T *>(a.k) + hk * a.kh, *vp = static_cast<const T *>(a.v) + hk * a.vh;
     if constexpr (ASYNC) {
-      copy_tile<DP, TILE>(KV + 2 * buf * TS, kp, a.kt, k0, a.D, range);
-      copy_tile<DP, TILE>(KV + (2 * buf + 1) * TS, vp, a.vt, k0, a.D, range);
+      copy_tile<DP, TILE, THREADS>(KV + 2 * buf * TS, kp, a.kt, k0, a.D, range);
+      copy_tile<DP, TILE, THREADS>(KV + (2 * buf + 1) * TS, vp, a.vt, k0, a.D, range);
     } else {
-      load_tile<T, DP, TILE>(KV, kp, a.kt, k0, a.D, range);
-      load_tile<T, DP, TILE>(KV + TS, vp, a.vt, k0, a.D, range);
+      load_tile<T, DP, TILE, THREADS>(KV, kp, a.kt, k0, a.D, range);
+      load_tile<T, DP, TILE, THREADS>(KV + TS, vp, a.vt, k0, a.D, range);
     }
   };
   if (ASYNC) {
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
     const float *K = KV + 2 * buf * TS, *V = K + TS;
     if (ASYNC) buf ^= 1;
     float s[R][4];
-    scores<DP, R>(Q, K, ty, tx, s);
+    scores<DP>(Q, K, ty, tx, s);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int t = q0 + ty * R + i;
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
       for (int c = 0; c < DP / 32; ++c) acc[i][c] = sm100::f2_mul(acc[i][c], sm100::f2_pack(fix, fix));
     }
     __syncwarp();  // a row of P is written and read by the same 16 lanes
-    accumulate<DP, R>(P, V, ty, tx, acc);
+    accumulate<DP>(P, V, ty, tx, acc);
   }
   float inv[R];
 #pragma unroll
@@ -242,15 +246,15 @@ __global__ void __launch_bounds__(THREADS) attn_fwd_generic_kernel(const Args a)
     if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.Tp + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
   }
   T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
-  store_rows<T, DP, R>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
+  store_rows<T, DP>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
 }
 
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
 // that see them, of every head of the group.
 template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
-__global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a) {
-  constexpr int R = ROWS / 16;
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const Args a) {
+  constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4), RS = ROWS * (DP + 4);
   constexpr int STAGE = 2 * TS + 2 * TILE;  // two tiles, lse and D; ASYNC: two stages
@@ -271,11 +275,11 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
     bound[i] = DKV ? s.end : s.start;
   }
   if (DKV) {
-    load_tile<T, DP, ROWS>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
-    load_tile<T, DP, ROWS>(R2, v + rh * a.vh, a.vt, r0, a.D, range);
+    load_tile<T, DP, ROWS, THREADS>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
+    load_tile<T, DP, ROWS, THREADS>(R2, v + rh * a.vh, a.vt, r0, a.D, range);
   } else {
-    load_tile<T, DP, ROWS>(R1, q + rh * a.qh, a.qt, r0, a.D, range);
-    load_tile<T, DP, ROWS>(R2, dout + (int64_t)rh * a.D, ot, r0, a.D, range);
+    load_tile<T, DP, ROWS, THREADS>(R1, q + rh * a.qh, a.qt, r0, a.D, range);
+    load_tile<T, DP, ROWS, THREADS>(R2, dout + (int64_t)rh * a.D, ot, r0, a.D, range);
   }
   uint64_t acc1[R][DP / 32] = {}, acc2[DKV ? R : 1][DP / 32] = {};
   const int64_t end_rows = min((int64_t)r0 + ROWS, a.T);
@@ -288,11 +292,11 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
     const T *s1 = DKV ? q + h * a.qh : k + (rh / G) * a.kh, *s2 = DKV ? dout + (int64_t)h * a.D : v + (rh / G) * a.vh;
     const int64_t t1 = DKV ? a.qt : a.kt, t2 = DKV ? ot : a.vt;
     if constexpr (ASYNC) {
-      copy_tile<DP, TILE>(c1, s1, t1, c0, a.D, range);
-      copy_tile<DP, TILE>(c2, s2, t2, c0, a.D, range);
+      copy_tile<DP, TILE, THREADS>(c1, s1, t1, c0, a.D, range);
+      copy_tile<DP, TILE, THREADS>(c2, s2, t2, c0, a.D, range);
     } else {
-      load_tile<T, DP, TILE>(c1, s1, t1, c0, a.D, range);
-      load_tile<T, DP, TILE>(c2, s2, t2, c0, a.D, range);
+      load_tile<T, DP, TILE, THREADS>(c1, s1, t1, c0, a.D, range);
+      load_tile<T, DP, TILE, THREADS>(c2, s2, t2, c0, a.D, range);
     }
     if (tid < TILE) {  // lse and D of the tile's columns, or of the block's rows
       const int64_t t = (DKV ? c0 : r0) + tid;
@@ -327,8 +331,8 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
       const float *C1 = CS + buf * STAGE, *C2 = C1 + TS, *L = C2 + TS, *Dl = L + TILE;
       if (ASYNC) buf ^= 1;
       float p[R][4], ds[R][4];
-      scores<DP, R>(R1, C1, ty, tx, p);
-      scores<DP, R>(R2, C2, ty, tx, ds);
+      scores<DP>(R1, C1, ty, tx, p);
+      scores<DP>(R2, C2, ty, tx, ds);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const int r = r0 + ty * R + i;
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
 #pragma unroll
           for (int j = 0; j < 4; ++j) W[(ty * R + i) * PP + tx + 16 * j] = p[i][j];
         __syncwarp();
-        accumulate<DP, R>(W, C2, ty, tx, acc2);
+        accumulate<DP>(W, C2, ty, tx, acc2);
         __syncwarp();
       }
 #pragma unroll
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
 #pragma unroll
         for (int j = 0; j < 4; ++j) W[(ty * R + i) * PP + tx + 16 * j] = ds[i][j];
       __syncwarp();
-      accumulate<DP, R>(W, C1, ty, tx, acc1);
+      accumulate<DP>(W, C1, ty, tx, acc1);
     }
   }
   float sc[R];
@@ -366,10 +370,10 @@ __global__ void __launch_bounds__(THREADS) attn_bwd_generic_kernel(const Args a)
 #pragma unroll
     for (int i = 0; i < R; ++i) one[i] = 1.f;
     const int64_t kt = (int64_t)a.Hk * a.D;
-    store_rows<T, DP, R>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
-    store_rows<T, DP, R>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+    store_rows<T, DP>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
+    store_rows<T, DP>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
   } else {
-    store_rows<T, DP, R>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
+    store_rows<T, DP>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
   }
 }
 
@@ -485,7 +489,7 @@ static cudaError_t run_fwd(const Args &a, cudaStream_t stream) {
   cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP, ROWS, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)a.H);
-  attn_fwd_generic_kernel<T, DP, ROWS, ASYNC><<<grid, THREADS, smem, stream>>>(a);
+  attn_fwd_generic_kernel<T, DP, ROWS, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -496,7 +500,7 @@ static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
   cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)(DKV ? a.Hk : a.H));
-  attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, THREADS, smem, stream>>>(a);
+  attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a);
   return cudaGetLastError();
 }
 
