@@ -153,15 +153,39 @@ __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, 
   }
 }
 
+// Which rows of which head a block has.  The blocks go out in the order of their work,
+// longest first; where all of them are resident at once, a second one on each SM, the
+// second ones go out the other way around, so that a long one shares its SM with a
+// short one.
+struct Work {
+  const int *order;  // tiles of TM rows by their work; null: with an SM for every block it does not matter
+  int heads;
+  int total;  // blocks with work
+  int fold;   // 0, or the SMs: blocks behind that many take the ranks backwards
+};
+struct Rows {
+  int row0, head;  // row0 < 0: none
+};
+template <int ROWS, bool LATE>  // LATE: later rows of a tile have more work
+__device__ __forceinline__ Rows rows_of(const Work &w, int64_t T) {
+  constexpr int SUB = TM / ROWS;
+  const int block = (int)blockIdx.x, rank = w.fold && block >= w.fold ? 3 * w.fold - 1 - block : block;
+  if (rank >= w.total) return {-1, 0};
+  const int at = rank / w.heads, sub = at % SUB, tile = at / SUB;
+  const int64_t row0 = (int64_t)(w.order ? w.order[tile] : tile) * TM + (LATE ? SUB - 1 - sub : sub) * ROWS;
+  return {row0 < T ? (int)row0 : -1, rank % w.heads};
+}
+
 template <typename T, int DP, int ROWS, bool ASYNC>
-__global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(const Args a) {
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(const Args a, const Work work) {
   constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4);
   float *Q = sm, *P = Q + ROWS * (DP + 4), *KV = P + ROWS * PP;  // ASYNC: two pairs of tiles
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * ROWS;  // longest rows first
-  const int h = blockIdx.y, hk = h / (a.H / a.Hk);
+  const Rows own = rows_of<ROWS, true>(work, a.T);
+  if (own.row0 < 0) return;
+  const int q0 = own.row0, h = own.head, hk = h / (a.H / a.Hk);
   const Span range = packed_range(a);
   int start[R];
 #pragma unroll
@@ -253,16 +277,17 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(cons
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
 // that see them, of every head of the group.
 template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
-__global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const Args a) {
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const Args a, const Work work) {
   constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4), RS = ROWS * (DP + 4);
   constexpr int STAGE = 2 * TS + 2 * TILE;  // two tiles, lse and D; ASYNC: two stages
   float *R1 = sm, *R2 = R1 + RS, *W = R2 + RS, *CS = W + ROWS * PP;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int r0 = (int)(DKV ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * ROWS;
+  const Rows own = rows_of<ROWS, !DKV>(work, a.T);
+  if (own.row0 < 0) return;
+  const int r0 = own.row0, rh = own.head;
   const int G = a.H / a.Hk;
-  const int rh = blockIdx.y;
   const Span range = packed_range(a);
   const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
   const T *dout = static_cast<const T *>(a.dout);
@@ -482,57 +507,76 @@ static bool fp32_rows(const Args &a, bool backward) {
   return a.dtype == MHC_F32 && !(ps & 15) && !((a.qt | a.qh | a.kt | a.kh | a.vt | a.vh | a.D) & 3);
 }
 
+// The grid; order: where the tiles' order stands, or will once it is needed.
+template <int ROWS>
+static cudaError_t plan(const Args &a, int heads, size_t smem, const int *order, Work &w, unsigned &grid) {
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  const int64_t tiles = (a.T + TM - 1) / TM, total = tiles * (TM / ROWS) * heads;
+  if (total > 0x7fffffff) return cudaErrorInvalidValue;
+  const bool two = 2 * (smem + 1024) <= 228 * 1024;  // blocks of an SM
+  w = {total > sms ? order : nullptr, heads, (int)total, two && total > sms && total <= 2 * sms ? sms : 0};
+  grid = (unsigned)(w.fold ? 2 * sms : total);
+  return cudaSuccess;
+}
+
 template <typename T, int DP, int ROWS, bool ASYNC>
-static cudaError_t run_fwd(const Args &a, cudaStream_t stream) {
+static cudaError_t run_fwd(const Args &a, int *order, cudaStream_t stream) {
   constexpr size_t smem = (size_t)((ROWS + (ASYNC ? 4 : 2) * TILE) * (DP + 4) + ROWS * PP) * 4;
   static_assert(smem <= 232448, "shared memory of a block");
   cudaError_t e = allow_smem<attn_fwd_generic_kernel<T, DP, ROWS, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)a.H);
-  attn_fwd_generic_kernel<T, DP, ROWS, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a);
+  Work w;
+  unsigned grid;
+  e = plan<ROWS>(a, a.H, smem, order, w, grid);
+  if (e == cudaSuccess && w.order) e = launch_attn_orders(a, order, nullptr, stream);
+  if (e != cudaSuccess) return e;
+  attn_fwd_generic_kernel<T, DP, ROWS, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a, w);
   return cudaGetLastError();
 }
 
 template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
-static cudaError_t run_bwd(const Args &a, cudaStream_t stream) {
+static cudaError_t run_bwd(const Args &a, const int *order, cudaStream_t stream) {
   constexpr size_t smem = (size_t)(2 * ROWS * (DP + 4) + ROWS * PP + (ASYNC ? 2 : 1) * 2 * TILE * (DP + 5)) * 4;
   static_assert(smem <= 232448, "shared memory of a block");
   cudaError_t e = allow_smem<attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC>>(smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)(DKV ? a.Hk : a.H));
-  attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a);
+  Work w;
+  unsigned grid;
+  e = plan<ROWS>(a, DKV ? a.Hk : a.H, smem, order, w, grid);
+  if (e != cudaSuccess) return e;
+  attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a, w);
   return cudaGetLastError();
 }
 
 // blocks of 32 or 64 rows, copied or loaded tiles.  Two stages of D = 128 with 64 rows
 // do not fit: those stay with 32.
 template <typename T, int DP>
-static cudaError_t pick_fwd(const Args &a, cudaStream_t stream) {
+static cudaError_t pick_fwd(const Args &a, int *order, cudaStream_t stream) {
   if constexpr (std::is_same<T, float>::value) {
     if (fp32_rows(a, false))
-      return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, true>(a, stream) : run_fwd<T, DP, 64, true>(a, stream);
+      return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, true>(a, order, stream) : run_fwd<T, DP, 64, true>(a, order, stream);
   }
-  return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, false>(a, stream) : run_fwd<T, DP, 64, false>(a, stream);
+  return short_rows(a.T, a.H) ? run_fwd<T, DP, 32, false>(a, order, stream) : run_fwd<T, DP, 64, false>(a, order, stream);
 }
 template <typename T, int DP, bool DKV>
-static cudaError_t pick_bwd(const Args &a, cudaStream_t stream) {
+static cudaError_t pick_bwd(const Args &a, const int *order, cudaStream_t stream) {
   const bool few = short_rows(a.T, DKV ? a.Hk : a.H);
   if constexpr (std::is_same<T, float>::value) {
     if (fp32_rows(a, true)) {
       if constexpr (DP <= 96)
-        if (!few) return run_bwd<T, DP, 64, DKV, true>(a, stream);
-      return run_bwd<T, DP, 32, DKV, true>(a, stream);
+        if (!few) return run_bwd<T, DP, 64, DKV, true>(a, order, stream);
+      return run_bwd<T, DP, 32, DKV, true>(a, order, stream);
     }
   }
-  return few ? run_bwd<T, DP, 32, DKV, false>(a, stream) : run_bwd<T, DP, 64, DKV, false>(a, stream);
+  return few ? run_bwd<T, DP, 32, DKV, false>(a, order, stream) : run_bwd<T, DP, 64, DKV, false>(a, order, stream);
 }
 
 }  // namespace attn
 
-cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream) {
+cudaError_t launch_attn_fwd_generic(const attn::Args &a, int *order, cudaStream_t stream) {
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    return attn::with_dim(a.D, [&](auto d) -> cudaError_t { return attn::pick_fwd<T, decltype(d)::value>(a, stream); });
+    return attn::with_dim(a.D, [&](auto d) -> cudaError_t { return attn::pick_fwd<T, decltype(d)::value>(a, order, stream); });
   });
 }
 
@@ -554,13 +598,16 @@ cudaError_t launch_attn_delta(const attn::Args &a, uint32_t *amax, cudaStream_t 
   });
 }
 
-cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream) {
+cudaError_t launch_attn_bwd_generic(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream) {
   return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
     return attn::with_dim(a.D, [&](auto d) -> cudaError_t {
       constexpr int DP = decltype(d)::value;
-      const cudaError_t e = attn::pick_bwd<T, DP, false>(a, stream);
-      return e != cudaSuccess ? e : attn::pick_bwd<T, DP, true>(a, stream);
+      const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+      cudaError_t e = cudaSuccess;  // one direction's blocks of 32 rows could be more than the SMs
+      if ((a.T + attn::TM - 1) / attn::TM * 4 * a.H > sms) e = launch_attn_orders(a, order_q, order_k, stream);
+      if (e == cudaSuccess) e = attn::pick_bwd<T, DP, false>(a, order_q, stream);
+      return e != cudaSuccess ? e : attn::pick_bwd<T, DP, true>(a, order_k, stream);
     });
   });
 }
@@ -624,7 +671,7 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
     if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_fwd");
     cudaGetLastError();
   }
-  return cuda_status(launch_attn_fwd_generic(a, st), "mhc_attn_fwd");
+  return cuda_status(launch_attn_fwd_generic(a, static_cast<int *>(workspace), st), "mhc_attn_fwd");
 }
 
 int64_t mhc_attn_lse_pitch(int64_t T) { return T < 1 ? 0 : (T + 127) / 128 * 128; }
@@ -678,7 +725,7 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
     cudaGetLastError();
     e = cudaSuccess;
   }
-  if (e == cudaSuccess) e = launch_attn_bwd_generic(a, st);
+  if (e == cudaSuccess) e = launch_attn_bwd_generic(a, order, order + on, st);
   return cuda_status(e, "mhc_attn_bwd");
 }
 

@@ -65,8 +65,8 @@ __device__ __forceinline__ Span packed_range(const Args &a) {
 
 }  // namespace attn
 
-cudaError_t launch_attn_fwd_generic(const attn::Args &a, cudaStream_t stream);
-cudaError_t launch_attn_bwd_generic(const attn::Args &a, cudaStream_t stream);
+cudaError_t launch_attn_fwd_generic(const attn::Args &a, int *order, cudaStream_t stream);
+cudaError_t launch_attn_bwd_generic(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream);
 cudaError_t launch_attn_delta(const attn::Args &a, uint32_t *amax, cudaStream_t stream);
 
 }  // namespace mhc

@@ -622,7 +622,7 @@ size_t attn_order_bytes(int64_t T) { return (size_t)((T + attn::TM - 1) / attn::
 
 cudaError_t launch_attn_orders(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream) {
   const int tiles = (int)((a.T + attn::TM - 1) / attn::TM);
-  attn::attn_order_kernel<<<2, attn::BINS, 0, stream>>>(a, 1, tiles, order_q, order_k);
+  attn::attn_order_kernel<<<order_k ? 2 : 1, attn::BINS, 0, stream>>>(a, 1, tiles, order_q, order_k);
   return cudaGetLastError();
 }
 

@@ -164,7 +164,7 @@ bool attn_tc_eligible(const attn::Args &a);      // what both directions ask of 
 bool attn_tc_bwd_eligible(const attn::Args &a);
 size_t attn_order_bytes(int64_t T);
 cudaError_t launch_attn_fwd_tc(const attn::Args &a, int *order, cudaStream_t stream);
-// the two orders of the backward (queries, then keys) in one launch
+// the order of the tiles of queries and, where order_k is not null, of keys, in one launch
 cudaError_t launch_attn_orders(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream);
 cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, cudaStream_t stream);
 
