@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(cons
 
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
-// that see them, of every head of the group.
+// that see them, of every head of the group or, with splits, of its share of them.
 template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
 __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const Args a, const Work work) {
   constexpr int THREADS = threads_of(ROWS);
@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const Rows own = rows_of<ROWS, !DKV>(work, a.T);
   if (own.row0 < 0) return;
-  const int r0 = own.row0, rh = own.head;
-  const int G = a.H / a.Hk;
+  const int G = a.H / a.Hk, splits = DKV ? a.splits : 1, per = G / splits;
+  const int r0 = own.row0, rh = own.head / splits, part = own.head % splits;
   const Span range = packed_range(a);
   const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
   const T *dout = static_cast<const T *>(a.dout);
@@ -310,9 +310,9 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
   const int64_t end_rows = min((int64_t)r0 + ROWS, a.T);
   const int first = DKV ? r0 : span_of(a, r0).start;
   const int last = DKV ? span_of(a, (int)end_rows - 1).end : (int)end_rows;
-  const int tiles = last > first ? (last - first + TILE - 1) / TILE : 0, n = tiles * (DKV ? G : 1);
+  const int tiles = last > first ? (last - first + TILE - 1) / TILE : 0, n = tiles * (DKV ? per : 1);
   auto fetch = [&](int it, int buf) {
-    const int h = DKV ? rh * G + it / tiles : rh, c0 = first + it % tiles * TILE;
+    const int h = DKV ? rh * G + part * per + it / tiles : rh, c0 = first + it % tiles * TILE;
     float *c1 = CS + buf * STAGE, *c2 = c1 + TS, *l = c2 + TS, *d = l + TILE;
     const T *s1 = DKV ? q + h * a.qh : k + (rh / G) * a.kh, *s2 = DKV ? dout + (int64_t)h * a.D : v + (rh / G) * a.vh;
     const int64_t t1 = DKV ? a.qt : a.kt, t2 = DKV ? ot : a.vt;
@@ -395,10 +395,30 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
 #pragma unroll
     for (int i = 0; i < R; ++i) one[i] = 1.f;
     const int64_t kt = (int64_t)a.Hk * a.D;
-    store_rows<T, DP>(static_cast<T *>(a.dk) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
-    store_rows<T, DP>(static_cast<T *>(a.dv) + (int64_t)rh * a.D, static_cast<T *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+    auto store = [&](auto *dk, auto *dv) {
+      using U = std::remove_pointer_t<decltype(dk)>;
+      store_rows<U, DP>(dk + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
+      store_rows<U, DP>(dv + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+    };
+    if (splits > 1)
+      store(a.parts + 2 * part * a.T * kt, a.parts + (2 * part + 1) * a.T * kt);
+    else
+      store(static_cast<T *>(a.dk), static_cast<T *>(a.dv));
   } else {
     store_rows<T, DP>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
+  }
+}
+
+// dK and dV from the parts of the blocks that share their keys, in order
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_any_kernel(const Args a) {
+  const int64_t n = a.T * a.Hk * a.D;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < 2 * n; e += (int64_t)gridDim.x * 256) {
+    const int second = e >= n;
+    const int64_t at = e - second * n;
+    float s = 0.f;
+    for (int p = 0; p < a.splits; ++p) s += __ldcs(a.parts + (int64_t)(p * 2 + second) * n + at);
+    static_cast<T *>(second ? a.dv : a.dk)[at] = from_f<T>(s);
   }
 }
 
@@ -542,7 +562,7 @@ static cudaError_t run_bwd(const Args &a, const int *order, cudaStream_t stream)
   if (e != cudaSuccess) return e;
   Work w;
   unsigned grid;
-  e = plan<ROWS>(a, DKV ? a.Hk : a.H, smem, order, w, grid);
+  e = plan<ROWS>(a, DKV ? a.Hk * a.splits : a.H, smem, order, w, grid);
   if (e != cudaSuccess) return e;
   attn_bwd_generic_kernel<T, DP, ROWS, DKV, ASYNC><<<grid, threads_of(ROWS), smem, stream>>>(a, w);
   return cudaGetLastError();
@@ -560,7 +580,7 @@ static cudaError_t pick_fwd(const Args &a, int *order, cudaStream_t stream) {
 }
 template <typename T, int DP, bool DKV>
 static cudaError_t pick_bwd(const Args &a, const int *order, cudaStream_t stream) {
-  const bool few = short_rows(a.T, DKV ? a.Hk : a.H);
+  const bool few = short_rows(a.T, DKV ? a.Hk * a.splits : a.H);
   if constexpr (std::is_same<T, float>::value) {
     if (fp32_rows(a, true)) {
       if constexpr (DP <= 96)
@@ -607,7 +627,12 @@ cudaError_t launch_attn_bwd_generic(const attn::Args &a, int *order_q, int *orde
       cudaError_t e = cudaSuccess;  // one direction's blocks of 32 rows could be more than the SMs
       if ((a.T + attn::TM - 1) / attn::TM * 4 * a.H > sms) e = launch_attn_orders(a, order_q, order_k, stream);
       if (e == cudaSuccess) e = attn::pick_bwd<T, DP, false>(a, order_q, stream);
-      return e != cudaSuccess ? e : attn::pick_bwd<T, DP, true>(a, order_k, stream);
+      if (e == cudaSuccess) e = attn::pick_bwd<T, DP, true>(a, order_k, stream);
+      if (e == cudaSuccess && a.splits > 1) {
+        attn::attn_join_any_kernel<T><<<grid_for(2 * a.T * a.Hk * a.D, 256, sms, 8), 256, 0, stream>>>(a);
+        e = cudaGetLastError();
+      }
+      return e;
     });
   });
 }
@@ -716,10 +741,10 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
     e = cudaMemsetAsync(amax, 0, 8, st);
   }
   if (e == cudaSuccess) e = launch_attn_delta(a, amax, st);
+  a.splits = attn_bwd_splits(T, H, Hk);
+  const uintptr_t at = (reinterpret_cast<uintptr_t>(order + 2 * on) + 8 + 15) & ~(uintptr_t)15;
+  a.parts = a.splits > 1 ? reinterpret_cast<float *>(at) : nullptr;
   if (e == cudaSuccess && tc) {
-    a.splits = attn_bwd_splits(T, H, Hk);
-    const uintptr_t at = (reinterpret_cast<uintptr_t>(order + 2 * on) + 8 + 15) & ~(uintptr_t)15;
-    a.parts = a.splits > 1 ? reinterpret_cast<float *>(at) : nullptr;
     e = launch_attn_bwd_tc(a, order, order + on, st);
     if (e != cudaErrorNotSupported) return cuda_status(e, "mhc_attn_bwd");
     cudaGetLastError();
