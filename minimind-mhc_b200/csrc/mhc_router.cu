@@ -22,6 +22,7 @@
 //
 // A row of -inf only has p = 0 and w = 0 (and the experts of lowest index);
 // a NaN counts as the largest logit and makes the row's weights and the loss NaN.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -309,13 +310,18 @@ __global__ void __launch_bounds__(THREADS, 4) route_fwd_kernel(Args a, float *w,
   }
 }
 
-// Joins the blocks' partial sums in a fixed order: `lanes` threads share an expert.
-__global__ void __launch_bounds__(1024) route_join_kernel(Args a, const float *part_sum, const int *part_cnt, int blocks,
+// Joins the blocks' partial sums in a fixed order: `lanes` threads of each block of a
+// cluster share an expert, the first block adds the others' sums to its own and forms
+// the loss.  It is the reading that counts, one SM has too few loads under way: 592
+// blocks, 64 / 512 experts: one block 8.4 / 45 us, a cluster of eight 4.5 / 10.
+constexpr int JOIN = 8;
+__global__ void __cluster_dims__(JOIN, 1, 1) __launch_bounds__(1024) route_join_kernel(Args a, const float *part_sum, const int *part_cnt, int blocks,
                                                           int64_t *counts, float *loss) {
   __shared__ float sh_sum[MAX_E];
   __shared__ int64_t sh_cnt[MAX_E];
   __shared__ float st_sum[1024];
   __shared__ int64_t st_cnt[1024];
+  const int rank = (int)blockIdx.x;  // one cluster
   int pad = 1;
   while (pad < a.E) pad <<= 1;
   const int lanes = 1024 / pad, e = threadIdx.x % pad, l = threadIdx.x / pad;
@@ -323,12 +329,12 @@ __global__ void __launch_bounds__(1024) route_join_kernel(Args a, const float *p
   int64_t c = 0;
   if (e < a.E) {
     constexpr int AT_ONCE = 8;  // in flight; summed in order
-    for (int b0 = l; b0 < blocks; b0 += lanes * AT_ONCE) {
+    for (int b0 = rank + JOIN * l; b0 < blocks; b0 += JOIN * lanes * AT_ONCE) {
       float vs[AT_ONCE];
       int vc[AT_ONCE];
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        const int b = b0 + u * lanes;
+        const int b = b0 + u * JOIN * lanes;
         vs[u] = b < blocks ? part_sum[(int64_t)b * a.E + e] : 0.f;
         vc[u] = b < blocks ? part_cnt[(int64_t)b * a.E + e] : 0;
       }
@@ -352,8 +358,20 @@ __global__ void __launch_bounds__(1024) route_join_kernel(Args a, const float *p
     sh_sum[threadIdx.x] = ts;
     sh_cnt[threadIdx.x] = tc;
   }
-  __syncthreads();
-  write_loss(sh_sum, sh_cnt, a, counts, loss);
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  if (rank == 0 && threadIdx.x < a.E) {  // the own thread's values: the others read nothing of this block
+    float ts = sh_sum[threadIdx.x];
+    int64_t tc = sh_cnt[threadIdx.x];
+    for (int r = 1; r < JOIN; ++r) {
+      ts += cluster.map_shared_rank(sh_sum, r)[threadIdx.x];
+      tc += cluster.map_shared_rank(sh_cnt, r)[threadIdx.x];
+    }
+    sh_sum[threadIdx.x] = ts;
+    sh_cnt[threadIdx.x] = tc;
+  }
+  cluster.sync();  // the others' memory has been read
+  if (rank == 0) write_loss(sh_sum, sh_cnt, a, counts, loss);
 }
 
 template <typename T, int G, int V, int SL>
@@ -527,7 +545,7 @@ int mhc_route_fwd(const void *logits, int dtype, int64_t T, int E, int64_t row_s
     });
   });
   if (e == cudaSuccess && blocks > 1) {
-    router::route_join_kernel<<<1, 1024, 0, st>>>(a, ps, pc, blocks, counts, loss);
+    router::route_join_kernel<<<router::JOIN, 1024, 0, st>>>(a, ps, pc, blocks, counts, loss);
     e = cudaGetLastError();
   }
   return cuda_status(e, "mhc_route_fwd");
