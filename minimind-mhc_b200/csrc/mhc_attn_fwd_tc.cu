@@ -23,7 +23,7 @@
 // compare indices.
 //
 // The grid is one block per SM and walks the tiles in the order of their work
-// (launch_attn_order), forwards and backwards in turn.  Warps 0-3 and 4-7: the two
+// (attn_order_kernel), forwards and backwards in turn.  Warps 0-3 and 4-7: the two
 // tiles' softmax and epilogue; 8: TMA; 9: MMA issue.
 #include <cuda.h>
 #include <cudaTypedefs.h>
