@@ -119,6 +119,19 @@ def test_packed_lengths(dtype, lengths):
     check(cu, 4, 2, 64, dtype, seed=sum(lengths))
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("d", (64, 36))
+@pytest.mark.parametrize("lengths,h,hk", (
+    ([512, 512], 8, 8), ([1024], 8, 4), ([300] * 7, 4, 4), ([1, 700, 0, 333, 64], 6, 2), ([1900, 1300, 77, 1], 16, 4)))
+def test_more_blocks_than_sms(dtype, d, lengths, h, hk):
+    """Ordered blocks, one or two for an SM and many, of both heights; shared-out heads.  Random signs: sums of 64
+    products and at most 1900 keys are within sqrt(1964) < 64 roundings."""
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    check(cu, h, hk, d, dtype, seed=cu[-1] + d)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cu,total", (([5, 90], 140), ([0, 130], 131), ([130, 260], 400), ([3, 3, 4], 9), ([0, 0], 5),
                                       ([200, 200], 300)))
