@@ -423,15 +423,16 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
       for (int s = 0; s < SL; ++s)
         if (es[s] >= 0) stripe[es[s]] = (ds[s] - dot) * inv;
       __syncwarp();
+      // An expert's lane also clears its word: the barrier then stands between every access of one lane and the next
+      // access of another, the next token's write included (the shuffles in between order no memory).
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
-        const float4 d = *reinterpret_cast<const float4 *>(stripe + e0 + i);
+        float4 *mine = reinterpret_cast<float4 *>(stripe + e0 + i);
+        const float4 d = *mine;
+        *mine = make_float4(0.f, 0.f, 0.f, 0.f);
         dp[i] += d.x; dp[i + 1] += d.y; dp[i + 2] += d.z; dp[i + 3] += d.w;
       }
       __syncwarp();
-#pragma unroll
-      for (int s = 0; s < SL; ++s)
-        if (es[s] >= 0) stripe[es[s]] = 0.f;
     }
     float pd = 0.f;
 #pragma unroll

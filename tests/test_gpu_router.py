@@ -165,6 +165,15 @@ def test_one_gradient_only():
         close(dz, ref[4], 128 * EPS)
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("e,k", ((16, 9), (64, 40), (256, 160), (512, 300)))
+def test_gradient_of_many_tokens_a_group(dtype, e, k):
+    """Three and a half turns of every group of lanes, most experts chosen in one turn and the next, each time by
+    another lane: what one turn leaves in shared memory must not meet the next."""
+    lanes = min(32, e // 8)
+    check(int(3.5 * 8 * torch.cuda.get_device_properties(0).multi_processor_count * (256 // lanes)), e, k, dtype, seed=e)
+
+
 def test_no_tokens():
     z = torch.empty(0, 8, device="cuda", requires_grad=True)
     w, idx, counts, loss = route_topk(z, 2, 1.0)
