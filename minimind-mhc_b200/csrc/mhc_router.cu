@@ -147,12 +147,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 constexpr float LOG2E = 1.44269504088896340736f;
 
+// exp(z - top) for a logit of a row whose largest is `top`: the special function's
+// 2^x (2 ulp) in place of expf's 9 instructions.  The difference is taken before it is
+// scaled: it is never above zero, so the largest logit gives exactly 1 and a row's sum
+// is at least 1 however large the logits are (scaled first, the rounding of top log2(e)
+// would be an exponent of hundreds from 1e10 on).  +inf - inf is NaN, as the quotient
+// would be.
+__device__ __forceinline__ float exp_below(float z, float top) { return exp2_approx((z - top) * LOG2E); }
+
 // softmax of the group's row; lanes past E hold p = 0.  An all -inf row gives 0.
-// p = exp2(z log2(e) - base) * scale for any logit z of the row: one FMA and the
-// special function's 2^x (2 ulp) in place of expf's 9 instructions.  The rounding of
-// base is common to the row and leaves p with its sum.
+// p = exp_below(z, top) * scale for any logit z of the row.
 template <typename T, int G, int V>
-__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, float (&p)[V], float &base, float &scale) {
+__device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, float (&p)[V], float &top, float &scale) {
   float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -160,11 +166,11 @@ __device__ __forceinline__ void softmax_row(const T (&x)[V], int e0, int E, floa
     mx = fmaxf(mx, p[i]);
   }
   mx = group_maxf<G>(mx);
-  base = mx == -INFINITY ? 0.f : mx * LOG2E;
+  top = mx == -INFINITY ? 0.f : mx;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    p[i] = exp2_approx(fmaf(p[i], LOG2E, -base));  // +inf logits: inf - inf = NaN, as the quotient would be
+    p[i] = exp_below(p[i], top);
     sum += p[i];
   }
   sum = group_sum<G>(sum);
@@ -225,8 +231,8 @@ __global__ void __launch_bounds__(THREADS, 4) route_fwd_kernel(Args a, float *w,
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = next[i];
     if (tb + stride < a.T) fetch(t + stride);
-    float p[V], base, scale;
-    softmax_row<T, G, V>(x, e0, a.E, p, base, scale);
+    float p[V], largest, scale;
+    softmax_row<T, G, V>(x, e0, a.E, p, largest, scale);
     K key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 4) route_fwd_kernel(Args a, float *w,
 #pragma unroll
     for (int s = 0; s < SL; ++s) {
       pe[s] = 0.f;
-      if (s * G + gl < a.k) pe[s] = exp2_approx(fmaf(Key::value(top[s]), LOG2E, -base)) * scale;
+      if (s * G + gl < a.k) pe[s] = exp_below(Key::value(top[s]), largest) * scale;
       total += pe[s];
     }
     total = group_sum<G>(total) + 1e-20f;
@@ -396,8 +402,8 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
     const int64_t t = live ? tb + threadIdx.x / G : a.T - 1;
     T x[V];
     load_logits<T, V>(z + t * a.row_stride, e0, a.E, a.vec, x);
-    float p[V], dp[V], base, scale;
-    softmax_row<T, G, V>(x, e0, a.E, p, base, scale);
+    float p[V], dp[V], largest, scale;
+    softmax_row<T, G, V>(x, e0, a.E, p, largest, scale);
 #pragma unroll
     for (int i = 0; i < V; ++i) dp[i] = load[i];
     if (dw) {
@@ -414,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 4) route_bwd_kernel(Args a, const flo
           es[s] = (int)idx[t * a.k + j];
           ds[s] = dw[t * a.k + j];
           dot = fmaf(ds[s], w[t * a.k + j], dot);
-          total += exp2_approx(fmaf(to_f(z[t * a.row_stride + es[s]]), LOG2E, -base)) * scale;
+          total += exp_below(to_f(z[t * a.row_stride + es[s]]), largest) * scale;
         }
       }
       dot = group_sum<G>(dot);

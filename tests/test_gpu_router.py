@@ -108,6 +108,27 @@ def test_a_row_without_experts(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_very_large_logits(dtype):
+    """Finite rows of any size have a softmax: all alike (a token that no expert may take, masked with the type's
+    lowest value or -1e10) 1 / E, one far above the rest 1, and between large logits only their difference counts."""
+    lim = torch.finfo(dtype)
+    sizes = [lim.min, lim.max, lim.min / 2] + ([] if dtype == torch.float16 else [-1e10, 1e10, -1e11, -1e30, 1e38, 5e9])
+    rows = [[s] * 8 for s in sizes]
+    rows += [[lim.max] + [0.0] * 7, [0.0] * 5 + [lim.max, lim.min, 1.0], [lim.min] * 7 + [lim.max]]
+    if dtype != torch.float16:
+        rows += [[3.3e38] + [1.0] * 7, [1e10] + [0.0] * 7, [-1e10] * 7 + [-2e10]]
+    if dtype == torch.float32:
+        rows += [[1e6 + i for i in range(8)], [-1e7 - i for i in range(8)], [3e9 - 256 * (i % 2) for i in range(8)]]
+    z = torch.randn(64, 8, device="cuda").to(dtype)  # ordinary rows beside them
+    z[:len(rows)] = torch.tensor(rows, dtype=torch.float64, device="cuda").to(dtype)
+    check(64, 8, 3, dtype, z)
+    wide = torch.zeros(40, 300, device="cuda", dtype=dtype)
+    wide[:20], wide[20:] = lim.min, lim.max
+    wide[::2, 7] = 1.0
+    check(40, 300, 5, dtype, wide)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_nan_and_inf_stay_in_their_row(dtype):
     z = torch.randn(300, 8, device="cuda").to(dtype)
     clean = route_topk(z, 2)
