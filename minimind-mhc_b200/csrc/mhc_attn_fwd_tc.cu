@@ -15,7 +15,11 @@
 // m is a row's reference, not its exact running maximum: it is moved, and O and the
 // row's sum rescaled, only when the maximum has grown past it by more than 2^8.
 // That is rare after the first tiles, exact in the end (the reference cancels), and
-// keeps O in TMEM from start to end.  The row sum is of the fp32 P.
+// keeps O in TMEM from start to end.  The row sum is of the fp32 P.  m is kept as a
+// score, before its scaling: P = exp2(fma(S, c, -round(m c))) leaves the rounding of m c
+// in every P of the row, where it cancels, but it is an exponent that grows with m.
+// Rows with |m c| above 2^10 (a part in 2^14 there) are subtracted first and scaled
+// then, one more addition a score.
 //
 // Which keys a row sees is decided per row (its sequence's start, itself), so one
 // tile may hold many short sequences: the number of tiles depends on T only, and
@@ -45,6 +49,7 @@ constexpr int W_TMA = 8, W_MMA = 9;
 constexpr int TMEM_COLS = 512;
 constexpr uint32_t S_COL = 0, O_COL = 256;  // two score tiles, two results, 128 columns each
 constexpr float LAZY = 8.f;                 // a row's reference may lag its maximum by 2^8
+constexpr float FAR = 1024.f;               // scaled references beyond it are subtracted before the scaling
 
 enum { ERR_TMA = 41, ERR_MMA = 42, ERR_SOFTMAX = 43 };
 
@@ -383,11 +388,11 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         for (int e = 0; e < 32; ++e)
 #pragma unroll
           for (int q = 0; q < 4; ++q) m[q] = fmaxf(m[q], __uint_as_float(r[q][e]));
-        const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
-        const bool grow = top > ref + LAZY;
+        const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        const bool grow = (top - ref) * c > LAZY;  // both -inf or both inf: NaN, no
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? top : ref;
-          const float fix = grow ? exp2_approx(ref - next) : 1.f;  // 0 for the first visible keys
+          const float fix = grow ? exp2_approx((ref - next) * c) : 1.f;  // 0 for the first visible keys
           ref = next;
           sum *= fix;
           if (j > first) {  // O holds the earlier tiles' sum, once their product is done
@@ -405,7 +410,16 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
             tmem_wait_st();
           }
         }
-        const float neg = ref == -INFINITY ? 0.f : -ref;
+        float neg = ref == -INFINITY ? 0.f : -ref * c;
+        const bool far = fabsf(neg) > FAR;
+        if (__any_sync(0xffffffffu, far)) {
+          const float off = far ? ref : 0.f;
+          neg = far ? 0.f : neg;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) - off);
+        }
         const uint64_t n2 = f2_pack(neg, neg);
         uint64_t acc[2] = {0ull, 0ull};
         uint32_t p[2][32];
@@ -437,7 +451,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         tc_fence_after();
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (tok < a.T) a.lse[(int64_t)head * a.Tp + tok] = sum == 0.f ? INFINITY : ref + log2f(sum);
+      if (tok < a.T) a.lse[(int64_t)head * a.Tp + tok] = sum == 0.f ? INFINITY : ref * c + log2f(sum);
       const int64_t at = ((int64_t)tok * a.H + head) * a.D;
       T *out = static_cast<T *>(a.o) + at, *lo = a.o_lo ? static_cast<T *>(a.o_lo) + at : nullptr;
 #pragma unroll

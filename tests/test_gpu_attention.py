@@ -185,6 +185,25 @@ def test_large_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 36))
+def test_very_large_scores(dtype, d):
+    """Scores from 1e8 to 1e11: equal ones share their weight, and one that is far above the rest has all of it.  The
+    products of a score are whole multiples of 2^18 whose sums are exact in fp32, so both hold exactly."""
+    t, h = 300, 2
+    g = torch.Generator(device="cuda").manual_seed(9)
+    v = torch.randn(t, h, d, device="cuda", generator=g).to(dtype)
+    for size in (3 * 2 ** 10, 5 * 2 ** 11, 3 * 2 ** 13, 7 * 2 ** 13):
+        q = torch.full((t, h, d), float(size), device="cuda", dtype=dtype)
+        q[::3] = -q[::3]
+        cu = torch.tensor([0, 100, t], dtype=torch.int32, device="cuda")
+        same = torch.full_like(q, float(size))
+        assert err(packed_attention(q, same, v, cu), reference(q, same, v, [0, 100, t])[0]) <= OUT[dtype] * U[dtype]
+        one = same / 2
+        one[[20, 90, 130, 259]] = same[0]
+        assert err(packed_attention(q, one, v, cu), reference(q, one, v, [0, 100, t])[0]) <= OUT[dtype] * U[dtype]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", (64, 96, 80))
 def test_slices_of_one_projection(dtype, d):
     check([0, 150, 331], 4, 2, d, dtype, fused=True)
