@@ -10,7 +10,9 @@
 #include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <cuda_runtime_api.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -67,6 +69,16 @@ int dtype_code(const Tensor &t, const char *who) {
 }
 void require_cuda(const Tensor &t) {
   TORCH_CHECK(t.is_cuda(), "mHC B200 kernels run on CUDA tensors only (this build has no CPU path); got a tensor on ", t.device());
+}
+// What would pass through a call without a trace of it: a tangent (a dual tensor does not require grad, so the call
+// would not meet the autograd node, which refuses it), and the launches themselves under a tracer, which sees the
+// allocation of the outputs only.
+void require_plain(const char *who, std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    TORCH_CHECK(!t->_fw_grad(0).defined(), who, ": forward-mode derivatives are not implemented");
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+              who, " cannot be traced: its kernels are launched outside of torch's operators");
 }
 void *stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 Tensor scratch(const Tensor &like, size_t bytes) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
@@ -144,6 +156,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
 
 Tensor packed_attention(Tensor q, Tensor k, Tensor v, const std::optional<Tensor> &cu_seqlens, std::optional<double> scale_) {
   const char *who = "packed_attention";
+  require_plain(who, {&q, &k, &v});
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {  // as scaled_dot_product_attention under autocast
     const at::ScalarType to = at::autocast::get_autocast_dtype(at::kCUDA);
     q = at::autocast::cached_cast(to, q, at::kCUDA);
@@ -247,6 +260,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> route_topk(const Tensor &logits, int64_t k, double coef) {
   const char *who = "route_topk";
+  require_plain(who, {&logits});
   require_cuda(logits);
   TORCH_CHECK_VALUE(logits.dim() >= 1, who, ": logits must have at least one dimension");
   dtype_code(logits, who);
@@ -288,6 +302,7 @@ bool is_param_type(const Tensor &t) {
 }
 
 std::optional<Tensor> adamw(const std::vector<Group> &groups, int bits, std::optional<double> max_norm) {
+  require_plain("adamw", {});
   TORCH_CHECK_VALUE(!max_norm.has_value() || *max_norm > 0, "adamw: max_grad_norm must be positive or None, got ", max_norm.value_or(0));
   std::vector<std::vector<mhc_adamw_tensor>> tables;
   Tensor like;

@@ -28,7 +28,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     fp16, all three alike; rows may lie at any strides (slices of one
     projection's output are read in place).  Under autocast all three are cast
     to its type, as ``scaled_dot_product_attention`` does.  ``scale`` defaults
-    to ``D ** -0.5``.
+    to ``D ** -0.5``.  Second and forward-mode derivatives are refused, as are
+    tracers (``torch.jit.trace``, ``make_fx``).
 
     Sequences may be empty.  Tokens before ``cu_seqlens[0]`` or from
     ``cu_seqlens[-1]`` on belong to none: their output and gradients are 0, and

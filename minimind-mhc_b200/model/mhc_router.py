@@ -34,6 +34,7 @@ def route_topk(logits: torch.Tensor, k: int, aux_coef: float = 0.0) -> Routing:
     logits: fp32 / bf16 / fp16, E <= 512; the softmax and everything after it
     are fp32.  Among equal logits the lower expert index wins; NaN is above
     everything; a row of ``-inf`` has weights 0.  The gradient flows through
-    ``weights`` and ``aux_loss``; the counts are constants of the loss.
+    ``weights`` and ``aux_loss``; the counts are constants of the loss.  Second
+    and forward-mode derivatives and tracers are refused.
     """
     return Routing(*nat.host().route_topk(logits, int(k), float(aux_coef)))

@@ -87,6 +87,50 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(route_topk(z, 2, 1.0).weights.square().sum(), z, create_graph=True)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require grad: without a check its tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+    from model.mhc_attention import packed_attention
+    from model.mhc_router import route_topk
+    x = [torch.randn(1, 6, 2, 64, device="cuda") for _ in range(3)]
+    z = torch.randn(4, 8, device="cuda")
+    with fwad.dual_level():
+        for place in range(3):
+            for other_grad in (False, True):
+                y = [t.clone().requires_grad_(other_grad) for t in x]
+                y[place] = fwad.make_dual(x[place], torch.ones_like(x[place]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    packed_attention(*y)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            route_topk(fwad.make_dual(z, torch.ones_like(z)), 2, 1.0)
+    packed_attention(*x)
+    route_topk(z, 2, 1.0)
+
+
+def test_tracing_is_refused():
+    """A trace would keep the empty outputs and not the launch."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from model.mhc_attention import packed_attention
+    from model.mhc_router import route_topk
+    from model.mhc_adamw import adamw_step
+
+    def step(t):
+        adamw_step([t], [t], [t.clone()], [t.square()], step=1, lr=1e-3)
+        return t
+
+    q, z = torch.randn(1, 6, 2, 64, device="cuda"), torch.randn(4, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(step)(z)
+    for grad in (False, True):
+        q.requires_grad_(grad)
+        z.requires_grad_(grad)
+        for f, x in ((lambda t: packed_attention(t, t, t), q), (lambda t: route_topk(t, 2, 1.0).weights, z)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(f, x, check_trace=False)
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(f)(x)
+
+
 def test_attention_under_autocast_takes_the_autocast_type():
     from model.mhc_attention import packed_attention
     q = torch.randn(1, 50, 4, 64, device="cuda", requires_grad=True)
