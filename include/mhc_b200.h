@@ -361,6 +361,14 @@ int mhc_adamw_step(const mhc_adamw_tensor *tensors, int count, int state_bits, d
                    double beta2, double eps, double weight_decay, double max_norm,
                    const void *norm_workspace, float *norm_out, void *stream);
 
+/*
+ * Whether mhc_adamw_step would take these arguments: its status code without a
+ * launch.  For a step of several groups: check every group first, so that no group
+ * has moved when another is refused.
+ */
+int mhc_adamw_check(const mhc_adamw_tensor *tensors, int count, int state_bits, double lr, double beta1,
+                    double beta2, double eps, double weight_decay);
+
 /* The n values that 8-bit codes stand for, as fp32: is_signed selects exp_avg's
  * form (int8) or exp_avg_sq's (uint8). */
 int mhc_adamw_unpack(const void *codes, int is_signed, const float *scales, float *out, int64_t n, void *stream);

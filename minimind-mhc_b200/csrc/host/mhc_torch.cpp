@@ -40,6 +40,7 @@ struct Entry {
   decltype(&mhc_route_bwd) route_bwd;
   decltype(&mhc_grad_norm_workspace) grad_norm_workspace;
   decltype(&mhc_grad_norm) grad_norm;
+  decltype(&mhc_adamw_check) adamw_check;
   decltype(&mhc_adamw_step) adamw_step;
 } E{};
 volatile int *give_up_flag = nullptr;  // the pinned word a kernel whose bounded wait ran out writes to
@@ -357,6 +358,11 @@ std::optional<Tensor> adamw(const std::vector<Group> &groups, int bits, std::opt
   C10_CUDA_CHECK(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
   TORCH_CHECK(capture == cudaStreamCaptureStatusNone,
               "adamw: the step number is an argument of the launch, so a step cannot be captured in a CUDA graph");
+  // all of them before the first launch: a refused step has changed nothing
+  for (size_t i = 0; i < tables.size(); ++i)
+    check(E.adamw_check(tables[i].data(), (int)tables[i].size(), bits, std::get<7>(groups[i]), std::get<8>(groups[i]),
+                        std::get<9>(groups[i]), std::get<10>(groups[i]), std::get<11>(groups[i])),
+          "mhc_adamw_check");
   Tensor ws, norm;
   if (max_norm.has_value()) {
     const size_t need = E.grad_norm_workspace();

@@ -547,6 +547,17 @@ static int64_t check_tensors(const char *who, const mhc_adamw_tensor *ts, int co
   return live;
 }
 
+// mhc_adamw_step's arguments: tensors with values, or a status code < 0
+static int64_t check_step(const char *who, const mhc_adamw_tensor *ts, int count, int state_bits, double lr, double beta1,
+                          double beta2, double eps, double weight_decay) {
+  if (state_bits != 8 && state_bits != 32)
+    return fail(MHC_ERR_UNSUPPORTED, "%s: state_bits must be 8 or 32 (got %d)", who, state_bits);
+  if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) ||
+      !(beta2 >= 0.0 && beta2 < 1.0))
+    return fail(MHC_ERR_SHAPE, "%s: lr, eps, weight_decay >= 0 and betas in [0, 1) are wanted", who);
+  return check_tensors(who, ts, count, state_bits, false);
+}
+
 extern "C" {
 
 size_t mhc_grad_norm_workspace(void) {
@@ -573,16 +584,18 @@ int mhc_grad_norm(const mhc_adamw_tensor *tensors, int count, int accumulate, vo
                      "mhc_grad_norm");
 }
 
+int mhc_adamw_check(const mhc_adamw_tensor *tensors, int count, int state_bits, double lr, double beta1, double beta2,
+                    double eps, double weight_decay) {
+  clear_error();
+  const int64_t live = check_step("mhc_adamw_check", tensors, count, state_bits, lr, beta1, beta2, eps, weight_decay);
+  return live < 0 ? (int)live : MHC_OK;
+}
+
 int mhc_adamw_step(const mhc_adamw_tensor *tensors, int count, int state_bits, double lr, double beta1, double beta2,
                    double eps, double weight_decay, double max_norm, const void *norm_workspace, float *norm_out,
                    void *stream) {
   clear_error();
-  if (state_bits != 8 && state_bits != 32)
-    return fail(MHC_ERR_UNSUPPORTED, "mhc_adamw_step: state_bits must be 8 or 32 (got %d)", state_bits);
-  if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) ||
-      !(beta2 >= 0.0 && beta2 < 1.0))
-    return fail(MHC_ERR_SHAPE, "mhc_adamw_step: lr, eps, weight_decay >= 0 and betas in [0, 1) are wanted");
-  const int64_t live = check_tensors("mhc_adamw_step", tensors, count, state_bits, false);
+  const int64_t live = check_step("mhc_adamw_step", tensors, count, state_bits, lr, beta1, beta2, eps, weight_decay);
   if (live < 0) return (int)live;
   if (max_norm > 0.0 && (!norm_workspace || ((uintptr_t)norm_workspace & 7)))
     return fail(MHC_ERR_WORKSPACE, "mhc_adamw_step: clipping needs the workspace that mhc_grad_norm filled");

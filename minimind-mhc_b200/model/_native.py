@@ -67,6 +67,7 @@ _PROTOS = {
     "mhc_route_bwd": (_I, [_P, _I, _I64, _I, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _P]),
     "mhc_grad_norm_workspace": (_SZ, []),
     "mhc_grad_norm": (_I, [_P, _I, _I, _P, _SZ, _P]),
+    "mhc_adamw_check": (_I, [_P, _I, _I, _D, _D, _D, _D, _D]),
     "mhc_adamw_step": (_I, [_P, _I, _I, _D, _D, _D, _D, _D, _D, _P, _P, _P]),
     "mhc_adamw_unpack": (_I, [_P, _I, _P, _P, _I64, _P]),
     "mhc_set_path_policy": (_I, [_I]),
@@ -140,7 +141,7 @@ HOST_PATH = os.path.join(_HERE, "_mhc_torch.so")
 # in the order of the module's table
 _HOST_ENTRIES = ("mhc_last_error", "mhc_attn_lse_pitch", "mhc_attn_fwd_workspace", "mhc_attn_fwd",
                  "mhc_attn_bwd_workspace", "mhc_attn_bwd", "mhc_route_fwd_workspace", "mhc_route_fwd",
-                 "mhc_route_bwd", "mhc_grad_norm_workspace", "mhc_grad_norm", "mhc_adamw_step")
+                 "mhc_route_bwd", "mhc_grad_norm_workspace", "mhc_grad_norm", "mhc_adamw_check", "mhc_adamw_step")
 _host = None
 
 

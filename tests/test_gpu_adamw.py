@@ -266,6 +266,36 @@ def test_optimizer_state_survives_saving(bits, dtype):
         assert v.dtype == w.dtype and torch.equal(v, w) if torch.is_tensor(v) else v == w
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("bad", (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0)))
+def test_a_refused_step_changes_nothing(bits, bad):
+    """The second group's options are out of range: no parameter, moment or count of the first has moved either, and
+    the step that follows is the one that a fresh optimizer makes."""
+    def build():
+        torch.manual_seed(5)
+        ps = [torch.nn.Parameter(torch.randn(n, device="cuda")) for n in (700, 33)]
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        return ps, AdamW([dict(params=[p]) for p in ps], state_bits=bits, max_grad_norm=1.0, **HYPER)
+
+    (ps, opt), (qs, ref) = build(), build()
+    opt.step()
+    ref.step()
+    flat = lambda o, params: [x.clone() if torch.is_tensor(x) else x for p in params  # noqa: E731
+                              for x in (p.detach(), *o.state[p].values())]
+    before, versions = flat(opt, ps), [p._version for p in ps]
+    good = {k: opt.param_groups[1][k] for k in bad}
+    opt.param_groups[1].update(bad)
+    with pytest.raises(RuntimeError):
+        opt.step()
+    same = lambda a, b: all(torch.equal(x, y) if torch.is_tensor(x) else x == y for x, y in zip(a, b))  # noqa: E731
+    assert same(before, flat(opt, ps)) and versions == [p._version for p in ps]
+    opt.param_groups[1].update(good)
+    opt.step()
+    ref.step()
+    assert same(flat(opt, ps), flat(ref, qs))
+
+
 def test_on_another_stream():
     a, b = make([100000], torch.float32, seed=2), make([100000], torch.float32, seed=2)
     adamw_step(*a, step=1, max_grad_norm=0.1, **HYPER)

@@ -105,6 +105,19 @@ def test_adamw_refusals(lib):
     assert lib.mhc_adamw_unpack(None, 1, None, None, 0, None) == 0
 
 
+def test_adamw_check_answers_as_the_step(lib):
+    """The same refusals, without a launch; what the step would take is fine."""
+    def ask(t, bits=32, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.1, count=1):
+        return lib.mhc_adamw_check(t, count, bits, lr, b1, b2, eps, wd)
+
+    assert ask(tensors()) == 0 and ask(tensors(), bits=8) == 0 and ask(None, count=0) == 0
+    for args in (dict(bits=16), dict(count=-1), dict(lr=-1.0), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(wd=-1.0),
+                 dict(lr=float("nan"))):
+        assert ask(tensors(), **args) == adamw(lib, tensors(), **args) < 0
+    for t in (dict(step=0), dict(n=-5), dict(pdt=5), dict(gdt=5), dict(p=0), dict(m=4098)):
+        assert ask(tensors(**t)) == adamw(lib, tensors(**t)) < 0
+
+
 def test_python_refuses_cpu_tensors(lib):
     from model.mhc_adamw import AdamW, adamw_step, unpack_moment
     from model.mhc_attention import packed_attention
