@@ -159,13 +159,55 @@ class AdamW(torch.optim.Optimizer):
             s["step"] += 1
         return loss
 
+    def _converted(self, saved, p):
+        """One parameter's saved state in this optimizer's own form, on its device."""
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else \
+                ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
+        if not saved:
+            return {}
+        held = 8 if "exp_avg_scale" in saved else 32
+        if held != self.state_bits:
+            raise ValueError(f"AdamW: the saved moments are held in {held} bits, this optimizer's in {self.state_bits}")
+        if "step" not in saved or any(n not in saved for n in names):
+            raise ValueError(f"AdamW: a parameter's saved state must have step, {', '.join(names)}; got {', '.join(saved)}")
+        own = {"step": int(saved["step"])}  # torch's is a tensor, on the device in its fused form
+        for name in names:
+            t = saved[name].detach()
+            scale = name.endswith("_scale")
+            want = (-(-p.numel() // QUANT_BLOCK),) if scale else p.shape
+            dtype = torch.float32 if scale or held == 32 else torch.int8 if name == "exp_avg" else torch.uint8
+            if t.shape != want:
+                raise ValueError(f"AdamW: {name} of a parameter {tuple(p.shape)} is saved as {tuple(t.shape)}")
+            if t.dtype != dtype and not (held == 32 and t.is_floating_point()):
+                raise ValueError(f"AdamW: {name} is saved as {t.dtype}, {dtype} is wanted")
+            own[name] = t.to(device=p.device, dtype=dtype, copy=True).contiguous()
+        return own
+
+    # torch.optim.AdamW's options that change what a step computes, with the value this class computes
+    _ONLY = dict(amsgrad=False, maximize=False, differentiable=False, decoupled_weight_decay=True)
+
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments keep the types they were saved in (torch
-        casts an optimizer's state to its parameter's type)."""
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        """Takes checkpoints of this class and of ``torch.optim.AdamW`` (for
+        ``state_bits=32``; moments of any floating type become fp32).  What it
+        cannot go on from is a ``ValueError`` and changes nothing: moments held in
+        another number of bits, ``amsgrad``, ``maximize``, another optimizer's
+        weight decay."""
+        groups = state_dict["param_groups"]
+        for g in groups:
+            if any(name not in g for name in self.defaults):
+                raise ValueError(f"AdamW: a checkpoint's groups must have {', '.join(self.defaults)}; got {', '.join(g)}")
+            for name, value in self._ONLY.items():
+                if g.get(name, value) != value:
+                    raise ValueError(f"AdamW: a checkpoint with {name}={g[name]} cannot be continued")
+        saved = [i for g in groups for i in g["params"]]
         here = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, here):
-            for name, t in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(t):
-                    self.state[p][name] = t.detach().to(p.device, copy=True).contiguous()
+        states = [self._converted(state_dict["state"].get(i, {}), p) for i, p in zip(saved, here)]
+        super().load_state_dict(state_dict)  # torch casts an optimizer's state to its parameter's type
+        for p, own in zip(here, states):
+            self.state.pop(p, None)
+            if own:
+                self.state[p] = own
+        for g in self.param_groups:
+            for name in (*self._ONLY, "foreach", "capturable", "fused"):
+                g.pop(name, None)
+            g["lr"] = float(g["lr"])  # a device tensor in torch's capturable form

@@ -266,6 +266,38 @@ def test_optimizer_state_survives_saving(bits, dtype):
         assert v.dtype == w.dtype and torch.equal(v, w) if torch.is_tensor(v) else v == w
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("kind", ({}, dict(fused=True), dict(capturable=True)))
+def test_goes_on_from_a_checkpoint_of_torch(dtype, kind):
+    """Five steps of torch's optimizer, then five of each from its checkpoint.  fp32: as above.  bf16: torch rounds its
+    moments and every operation to bf16: 16 roundings of 2^-9 of an update (at most 1.5 lr
+    here) and three roundings of the parameter a step, its decay apart."""
+    torch.manual_seed(2)
+    theirs = [torch.nn.Parameter(torch.randn(s, device="cuda").to(dtype)) for s in ((40, 33), (7,))]
+    b = torch.optim.AdamW(theirs, lr=1e-3, weight_decay=0.1, **kind)
+    for _ in range(5):
+        for p in theirs:
+            p.grad = torch.randn_like(p)
+        b.step()
+    mine = [torch.nn.Parameter(p.detach().clone()) for p in theirs]
+    a = AdamW(mine, lr=5.0)
+    a.load_state_dict(copy.deepcopy(b.state_dict()))
+    assert all(s["step"] == 5 and type(s["step"]) is int and s["exp_avg"].dtype == torch.float32
+               for s in a.state.values())
+    for _ in range(5):
+        for p, q in zip(mine, theirs):
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad.clone()
+        a.step()
+        b.step()
+    for p, q in zip(mine, theirs):
+        if dtype == torch.float32:
+            assert torch.allclose(p, q, rtol=1e-5, atol=1e-6)
+        else:
+            off = (p.double() - q.double()).abs()
+            assert (off <= 5 * (8 * 2.0 ** -8 * 1.5e-3 + 3 * 2.0 ** -8 * q.double().abs())).all()
+
+
 @pytest.mark.parametrize("bits", (32, 8))
 @pytest.mark.parametrize("bad", (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0)))
 def test_a_refused_step_changes_nothing(bits, bad):

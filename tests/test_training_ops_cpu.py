@@ -118,6 +118,63 @@ def test_adamw_check_answers_as_the_step(lib):
         assert ask(tensors(**t)) == adamw(lib, tensors(**t)) < 0
 
 
+def trained_by_torch(cls=torch.optim.AdamW, dtype=torch.float32, **kind):
+    ps = [torch.nn.Parameter(torch.randn(s).to(dtype)) for s in ((5, 3), (300,))]
+    opt = cls(ps, lr=1e-3, **kind)
+    for _ in range(3):
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        opt.step()
+    return ps, opt.state_dict()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_a_checkpoint_of_torch_is_converted(dtype):
+    """Counts become ints, moments fp32; a parameter that was never stepped has no state; options of how torch runs
+    its step do not stay behind."""
+    from model.mhc_adamw import AdamW
+    ps, saved = trained_by_torch(dtype=dtype, betas=(0.8, 0.9), foreach=True)
+    del saved["state"][1]
+    saved["param_groups"][0]["lr"] = torch.tensor(2e-3)
+    opt = AdamW([torch.nn.Parameter(p.detach().clone()) for p in ps])
+    opt.load_state_dict(saved)
+    group, = opt.param_groups
+    assert set(group) == {"params", "lr", "betas", "eps", "weight_decay"} and group["betas"] == (0.8, 0.9)
+    assert type(group["lr"]) is float and abs(group["lr"] - 2e-3) < 1e-9
+    s = opt.state[group["params"][0]]
+    assert type(s["step"]) is int and s["step"] == 3 and group["params"][1] not in opt.state
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert s[name].dtype == torch.float32 and torch.equal(s[name], saved["state"][0][name].float())
+        assert s[name].data_ptr() != saved["state"][0][name].data_ptr()
+
+
+def test_checkpoints_that_cannot_be_continued_are_refused(lib):
+    """At the load, and nothing of the optimizer has changed by then."""
+    from model.mhc_adamw import AdamW, zero_moment
+    ps, saved = trained_by_torch()
+    own8 = AdamW(ps, state_bits=8)
+    for p in ps:
+        own8._state_of(p)
+    cases = [(8, saved), (32, own8.state_dict()),
+             (32, trained_by_torch(amsgrad=True)[1]), (32, trained_by_torch(maximize=True)[1]),
+             (32, trained_by_torch(torch.optim.Adam)[1]), (32, trained_by_torch(torch.optim.Adagrad)[1]),
+             (32, trained_by_torch(torch.optim.SGD)[1])]
+    _, short = trained_by_torch()
+    short["state"][1]["exp_avg"] = torch.zeros(299)
+    cases.append((32, short))
+    codes = own8.state_dict()
+    codes["state"][0] = codes["state"][0] | {"exp_avg": zero_moment(ps[0], False).codes}
+    cases.append((8, codes))
+    for bits, bad in cases:
+        opt = AdamW(ps, lr=0.5, state_bits=bits)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        assert not opt.state and opt.param_groups[0]["lr"] == 0.5
+    opt = AdamW(ps, state_bits=8)
+    opt.load_state_dict(own8.state_dict())
+    assert opt.state[ps[0]]["exp_avg"].dtype == torch.int8 and opt.state[ps[0]]["step"] == 0
+
+
 def test_python_refuses_cpu_tensors(lib):
     from model.mhc_adamw import AdamW, adamw_step, unpack_moment
     from model.mhc_attention import packed_attention
