@@ -119,6 +119,10 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        """For copies and pickles: torch's has the groups and the state only."""
+        return super().__getstate__() | {k: getattr(self, k) for k in ("state_bits", "max_grad_norm", "grad_norm")}
+
     def _state_of(self, p):
         s = self.state[p]
         if not s:

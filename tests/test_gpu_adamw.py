@@ -6,6 +6,7 @@ equals the plain fp32 form's code for code: both do the same single IEEE operati
 
 import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -264,6 +265,23 @@ def test_optimizer_state_survives_saving(bits, dtype):
     for k, v in opt.state[p].items():
         w = opt2.state[p2][k]
         assert v.dtype == w.dtype and torch.equal(v, w) if torch.is_tensor(v) else v == w
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_a_copied_optimizer_steps_as_the_first(bits):
+    p = torch.nn.Parameter(torch.randn(600, device="cuda"))
+    opt = AdamW([p], state_bits=bits, max_grad_norm=0.1)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    for clone in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = clone.param_groups[0]["params"][0]
+        assert (clone.state_bits, clone.max_grad_norm) == (bits, 0.1) and torch.equal(clone.grad_norm, opt.grad_norm)
+        old = q.detach().clone()
+        q.grad = p.grad.clone()
+        clone.step()
+        assert not torch.equal(q, old) and clone.state[q]["step"] == 2
+    opt.step()
+    assert torch.equal(p, q)
 
 
 @pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
