@@ -1021,13 +1021,13 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
                 outs.append(e(F.pad(c, (0, 0, 0, pad)))[:c.shape[0]] if pad else e(c))
             ys = torch.cat(outs) if outs else xs[:0]
             ys = ys * w.flatten()[order].unsqueeze(1).to(ys.dtype)
-            if native_ops:
+            if not self.training or aux_coef <= 0:
+                self.aux_loss = w.new_zeros(())
+            elif native_ops:
                 self.aux_loss = aux
-            elif self.training and aux_coef > 0:
+            else:
                 load = F.one_hot(idx, experts).float().mean(0)
                 self.aux_loss = (load * scores.float().mean(0)).sum() * experts * aux_coef
-            else:
-                self.aux_loss = scores.new_zeros(())
             return torch.zeros_like(xf).index_add_(0, tok, ys.to(xf.dtype)).view(shape)
 
     conn = MHCConnection_Fused if use_mhc == 1 else MHCConnection_FusedNoHres

@@ -43,6 +43,21 @@ def test_decoder_with_native_ops_matches_torch_ops(dtype):
         assert off <= 0.1
 
 
+def test_decoder_has_no_balance_loss_outside_of_training():
+    """Evaluation: both sides' auxiliary loss is zero, as in the reference's MoE layer."""
+    import bench
+    args = dict(moe=True, dev=torch.device("cuda"), hidden=256, layers=2, heads=4, kv_heads=2, inter=256, vocab=300)
+    ids = torch.randint(0, 300, (2, 50), device="cuda")
+    for native in (False, True):
+        torch.manual_seed(3)
+        m = bench._build_decoder(native_ops=native, **args)
+        m(ids)
+        assert m.aux_loss().item() > 0
+        m.eval()
+        m(ids)
+        assert m.aux_loss().item() == 0
+
+
 @pytest.mark.parametrize("bits", (32, 8))
 def test_packed_example_learns(bits):
     sys.path.insert(0, os.path.join(ROOT, "examples"))
