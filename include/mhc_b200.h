@@ -261,7 +261,8 @@ size_t mhc_attn_bwd_workspace(int64_t T, int H, int Hk, int D);
 /*
  * Gradients of mhc_attn_fwd from out, out_lo (or NULL), lse and dout (T, H, D) contiguous:
  * dq (T, H, D), dk and dv (T, Hk, D) contiguous, each summed in fp32 in a fixed
- * order (no atomics), the heads of a group included.
+ * order (no atomics), the heads of a group included.  dq, or dk and dv together,
+ * may be NULL: not wanted, and not computed.
  */
 int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo,
                  const void *dout, const float *lse, int dtype, int64_t T, int H, int Hk, int D, const int64_t *strides,

@@ -142,13 +142,19 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const int64_t t = q.size(0), h = q.size(1), d = q.size(2), hk = k.size(1), seqlen = ctx->saved_data["seqlen"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     const Tensor dout = g[0].contiguous();
-    const Tensor dq = at::empty({t, h, d}, q.options()), dk = at::empty({t, hk, d}, q.options()), dv = at::empty({t, hk, d}, q.options());
+    // those that this backward is asked for; dk and dv come from one kernel
+    Tensor dq, dk, dv;
+    if (ctx->needs_input_grad(0)) dq = at::empty({t, h, d}, q.options());
+    if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+      dk = at::empty({t, hk, d}, q.options());
+      dv = at::empty({t, hk, d}, q.options());
+    }
     const size_t need = E.attn_bwd_workspace(t, (int)h, (int)hk, (int)d);
     const Tensor ws = scratch(q, need);
     const int64_t strides[6] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
     check(E.attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(out_lo), dout.data_ptr(), lse.data_ptr<float>(),
                      dtype_code(q, "packed_attention"), t, (int)h, (int)hk, (int)d, strides, static_cast<const int32_t *>(ptr(cu)),
-                     cu.defined() ? (int)cu.numel() - 1 : 0, seqlen, (float)scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                     cu.defined() ? (int)cu.numel() - 1 : 0, seqlen, (float)scale, ptr(dq), ptr(dk), ptr(dv),
                      ws.data_ptr(), need, stream_of(q)),
           "mhc_attn_bwd");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor()};

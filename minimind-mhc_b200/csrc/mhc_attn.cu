@@ -632,9 +632,9 @@ cudaError_t launch_attn_bwd_generic(const attn::Args &a, int *order_q, int *orde
       const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
       cudaError_t e = cudaSuccess;  // one direction's blocks of 32 rows could be more than the SMs
       if ((a.T + attn::TM - 1) / attn::TM * 4 * a.H > sms) e = launch_attn_orders(a, order_q, order_k, stream);
-      if (e == cudaSuccess) e = attn::pick_bwd<T, DP, false>(a, order_q, stream);
-      if (e == cudaSuccess) e = attn::pick_bwd<T, DP, true>(a, order_k, stream);
-      if (e == cudaSuccess && a.splits > 1) {
+      if (e == cudaSuccess && a.dq) e = attn::pick_bwd<T, DP, false>(a, order_q, stream);
+      if (e == cudaSuccess && a.dk) e = attn::pick_bwd<T, DP, true>(a, order_k, stream);
+      if (e == cudaSuccess && a.dk && a.splits > 1) {
         attn::attn_join_any_kernel<T><<<grid_for(2 * a.T * a.Hk * a.D, 256, sms, 8), 256, 0, stream>>>(a);
         e = cudaGetLastError();
       }
@@ -727,7 +727,8 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
   a.cu = cu_seqlens; a.batch = batch; a.seqlen = seqlen;
   if (int st = check_attn("mhc_attn_bwd", a, strides, scale)) return st;
   if (T == 0) return MHC_OK;
-  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv)
+  // dq, or dk and dv together, may be left out
+  if (!q || !k || !v || !out || !dout || !lse || !dk != !dv || (!dq && !dk))
     return fail(MHC_ERR_NULL, "mhc_attn_bwd: required pointer is NULL");
   if (misaligned(dtype == MHC_F32 ? 4 : 2, {q, k, v, out, out_lo, dout, dq, dk, dv}) || ((uintptr_t)lse & 3))
     return fail(MHC_ERR_ALIGN, "mhc_attn_bwd: a pointer is not aligned to its elements");

@@ -680,9 +680,9 @@ cudaError_t launch_attn_bwd_tc(const attn::Args &a, int *order_q, int *order_k, 
     cudaError_t e = cudaSuccess;
     // DQ has at least as many pieces of work as DKV
     if ((a.T + attn::TM - 1) / attn::TM * a.H > sms) e = launch_attn_orders(a, order_q, order_k, stream);
-    if (e == cudaSuccess) e = attn::run<T, DP, true>(a, k, v, q, d, order_k, sms, stream);
-    if (e == cudaSuccess) e = attn::run<T, DP, false>(a, q, d, k, v, order_q, sms, stream);
-    if (e == cudaSuccess && a.splits > 1) {
+    if (e == cudaSuccess && a.dk) e = attn::run<T, DP, true>(a, k, v, q, d, order_k, sms, stream);
+    if (e == cudaSuccess && a.dq) e = attn::run<T, DP, false>(a, q, d, k, v, order_q, sms, stream);
+    if (e == cudaSuccess && a.dk && a.splits > 1) {
       attn::attn_join_kernel<T><<<grid_for(2 * a.T * a.Hk * a.D / 4, 256, sms, 8), 256, 0, stream>>>(a);
       e = cudaGetLastError();
     }

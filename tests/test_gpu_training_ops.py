@@ -146,6 +146,35 @@ def test_tracing_is_refused():
                 make_fx(f)(x)
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_attention_computes_the_gradients_that_are_asked_for(dtype):
+    """Frozen keys and values, or a frozen query: the others' gradients are the same bits as with all three, and those
+    not asked for take no memory."""
+    from model.mhc_attention import packed_attention
+    t, h, hk, d = 6000, 8, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(7)
+    base = [torch.randn(t, n, d, device="cuda", generator=g).to(dtype) for n in (h, hk, hk)]
+    do = torch.randn(t, h, d, device="cuda", generator=g).to(dtype)
+    cu = torch.tensor([0, 1000, 1001, 5000], dtype=torch.int32, device="cuda")
+
+    def run(which, leaves):
+        x = [b.clone().requires_grad_(i in leaves) for i, b in enumerate(base)]
+        out = packed_attention(*x, cu)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(out, [x[i] for i in which], do)
+        return grads, torch.cuda.max_memory_allocated() - before
+
+    full, most = run((0, 1, 2), (0, 1, 2))
+    size = base[0].numel() * base[0].element_size()
+    for which, saved in (((0,), 2), ((1, 2), 1), ((1,), 1), ((2,), 1), ((0, 2), 0)):
+        for leaves in (which, (0, 1, 2)):
+            grads, peak = run(which, leaves)
+            assert all(torch.equal(a, full[i]) for a, i in zip(grads, which))
+            assert peak <= most - saved * size
+
+
 def test_attention_under_autocast_takes_the_autocast_type():
     from model.mhc_attention import packed_attention
     q = torch.randn(1, 50, 4, 64, device="cuda", requires_grad=True)

@@ -50,6 +50,14 @@ def test_attention_refusals(lib):
     assert st == -1
 
 
+def test_attention_gradients_that_may_be_left_out(lib):
+    """dq, or dk and dv together; what is left is checked as ever (here it stops at the workspace)."""
+    for dq, dk, dv, want in ((P, None, None, -5), (None, P, P, -5), (None, None, None, -1), (P, None, P, -1),
+                             (P, P, None, -1), (None, P, None, -1), (None, ODD, P, -4)):
+        assert lib.mhc_attn_bwd(P, P, P, P, None, P, P, 1, 100, 8, 4, 64, SIX, None, 0, 100, 0.125, dq, dk, dv, P, 16,
+                                None) == want
+
+
 def test_attention_workspaces(lib):
     assert lib.mhc_attn_lse_pitch(0) == 0 and lib.mhc_attn_lse_pitch(1) == 128 and lib.mhc_attn_lse_pitch(129) == 256
     assert lib.mhc_attn_fwd_workspace(100000) >= 782 * 4
