@@ -141,7 +141,9 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const c10::cuda::CUDAGuard guard(q.device());
     const int64_t t = q.size(0), h = q.size(1), d = q.size(2), hk = k.size(1), seqlen = ctx->saved_data["seqlen"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
-    const Tensor dout = g[0].contiguous();
+    // contiguous, and for 16-bit types at a multiple of 16 bytes, as rows() has it
+    Tensor dout = g[0].contiguous();
+    if (dout.element_size() == 2 && d % 8 == 0 && reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16) dout = dout.clone();
     // those that this backward is asked for; dk and dv come from one kernel
     Tensor dq, dk, dv;
     if (ctx->needs_input_grad(0)) dq = at::empty({t, h, d}, q.options());

@@ -175,6 +175,21 @@ def test_attention_computes_the_gradients_that_are_asked_for(dtype):
             assert peak <= most - saved * size
 
 
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_attention_gradient_at_an_odd_address(dtype):
+    """dO that begins at no multiple of 16 bytes goes through the same kernels as one that does."""
+    from model.mhc_attention import packed_attention
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = (torch.randn(1, 500, n, 64, device="cuda", generator=g).to(dtype).requires_grad_(True) for n in (4, 2, 2))
+    flat = torch.randn(500 * 4 * 64 + 3, device="cuda", generator=g).to(dtype)
+    odd = flat[3:].view(1, 500, 4, 64)
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    out = packed_attention(q, k, v)
+    a = torch.autograd.grad(out, (q, k, v), odd, retain_graph=True)
+    b = torch.autograd.grad(out, (q, k, v), odd.clone())
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_attention_under_autocast_takes_the_autocast_type():
     from model.mhc_attention import packed_attention
     q = torch.randn(1, 50, 4, 64, device="cuda", requires_grad=True)
