@@ -28,6 +28,7 @@
 #include <initializer_list>
 #include <mutex>
 
+#include "mhc_attn_redo.cuh"
 #include "mhc_attn_tc.cuh"
 #include "mhc_b200.h"
 #include "mhc_device.cuh"
@@ -133,10 +134,11 @@ __device__ __forceinline__ void accumulate(const float *W, const float *B, int t
   }
 }
 
-// lo != null: what the rounding to T left over, itself in T
+// lo != null: what the rounding to T left over, itself in T.  Whether there was a NaN.
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, int64_t T_, int D, int ty, int tx,
+__device__ __forceinline__ bool store_rows(T *dst, T *lo, int64_t ts, int row0, int64_t T_, int D, int ty, int tx,
                                            const uint64_t (&acc)[R][DP / 32], const float (&mul)[R]) {
+  bool bad = false;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int t = row0 + ty * R + i;
@@ -148,12 +150,14 @@ __device__ __forceinline__ void store_rows(T *dst, T *lo, int64_t ts, int row0, 
         float v, w;
         sm100::f2_unpack(acc[i][c / 2], v, w);
         v = (c & 1 ? w : v) * mul[i];
+        bad |= isnan(v);
         const T r = from_f<T>(v);
         dst[(int64_t)t * ts + col] = r;
         if (lo) lo[(int64_t)t * ts + col] = from_f<T>(v - to_f(r));
       }
     }
   }
+  return bad;
 }
 
 // Which rows of which head a block has.  The blocks go out in the order of their work,
@@ -183,7 +187,7 @@ __device__ __forceinline__ Rows rows_of(const Work &w, int64_t T) {
 }
 
 template <typename T, int DP, int ROWS, bool ASYNC>
-__global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(const Args a, const Work work) {
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(const __grid_constant__ Args a, const Work work) {
   constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4);
@@ -276,7 +280,10 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(cons
     if (tx == 0 && t < a.T) a.lse[(int64_t)h * a.Tp + t] = sum[i] == 0.f ? INFINITY : mx[i] + log2f(sum[i]);
   }
   T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
-  store_rows<T, DP>(static_cast<T *>(a.o) + (int64_t)h * a.D, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv);
+  T *out = static_cast<T *>(a.o) + (int64_t)h * a.D;
+  if (__syncthreads_or(store_rows<T, DP>(out, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv)))
+    for (int r = tid >> 5; r < ROWS && q0 + r < a.T; r += THREADS / 32)
+      if (row_has_nan(out + (int64_t)(q0 + r) * a.H * a.D, a.D, tid & 31)) redo_out<T>(a, h, q0 + r, tid & 31);
 }
 
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.

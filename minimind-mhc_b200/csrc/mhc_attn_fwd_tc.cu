@@ -34,6 +34,7 @@
 
 #include <mutex>
 
+#include "mhc_attn_redo.cuh"
 #include "mhc_attn_tc.cuh"
 
 namespace mhc {
@@ -131,7 +132,7 @@ __device__ __forceinline__ bool item_of(const Args &a, const Sched &s, int64_t r
 template <typename T, int DP>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map kmap, const __grid_constant__ Map vmap,
-                   const Args a, const Sched sched) {
+                   const __grid_constant__ Args a, const Sched sched) {
   using C = Cfg<DP>;
   using L = typename C::L;
   constexpr int ST = C::ST;
@@ -140,7 +141,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
   __shared__ Item items[2];
   __shared__ __align__(8) uint64_t bars[NBARS];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int abort_word, redo_word;  // redo: a NaN has been written
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *gen = smem_raw + (base - raw);
@@ -151,7 +152,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
-    abort_word = 0;
+    abort_word = redo_word = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(B_ITEM_F + i), 1);
       mbar_init(BAR(B_ITEM_E + i), 257);  // the softmax threads and the MMA thread have read it
@@ -452,6 +453,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       if (tok < a.T) a.lse[(int64_t)head * a.Tp + tok] = sum == 0.f ? INFINITY : ref * c + log2f(sum);
+      bool bad = false;
       const int64_t at = ((int64_t)tok * a.H + head) * a.D;
       T *out = static_cast<T *>(a.o) + at, *lo = a.o_lo ? static_cast<T *>(a.o_lo) + at : nullptr;
 #pragma unroll
@@ -467,6 +469,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float x = __uint_as_float(o[2 * e]) * inv, y = __uint_as_float(o[2 * e + 1]) * inv;
+          bad |= isnan(x) || isnan(y);
           w[e] = pack2<T>(x, y);
           const float2 back = unpack2<T>(w[e]);
           l[e] = pack2<T>(x - back.x, y - back.y);
@@ -478,6 +481,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
             if (lo) *reinterpret_cast<uint4 *>(lo + d + h * 8) = make_uint4(l[h * 4], l[h * 4 + 1], l[h * 4 + 2], l[h * 4 + 3]);
           }
       }
+      if (bad && tok < a.T) redo_word = 1;
       tc_fence_before();
     }
     if (!ok && lane == 0) give_up(ERR_SOFTMAX, abort_flag, a.err_flag);
@@ -500,6 +504,17 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
         for (int e = tid; it.q0[t] >= 0 && e < TM * a.D; e += NTHREADS) {
           const int64_t tok = it.q0[t] + e / a.D;
           if (tok < a.T) static_cast<T *>(a.o)[(tok * a.H + it.head[t]) * a.D + e % a.D] = bad;
+        }
+    }
+  } else if (redo_word) {
+    for (int i = 0;; ++i) {
+      Item it;
+      if (!item_of(a, sched, snake(i, blockIdx.x, gridDim.x), it)) break;
+      for (int t = 0; t < 2; ++t)
+        for (int r = warp; it.q0[t] >= 0 && r < TM && it.q0[t] + r < a.T; r += NTHREADS / 32) {
+          const int tok = it.q0[t] + r;
+          if (row_has_nan(static_cast<const T *>(a.o) + ((int64_t)tok * a.H + it.head[t]) * a.D, a.D, lane))
+            redo_out<T>(a, it.head[t], tok, lane);
         }
     }
   }

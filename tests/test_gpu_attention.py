@@ -169,6 +169,65 @@ def test_values_of_the_future_and_of_other_sequences(dtype):
     assert torch.equal(one[100:250], two[100:250])
 
 
+def poisoned(place, fill, at, head, col, cu, h, hk, t, d):
+    """Which entries of out, dq, dk and dv the definition lets a non-finite entry of an input reach."""
+    lo, hi = next((a, b) for a, b in zip(cu[:-1], cu[1:]) if a <= at < b)
+    m = [torch.zeros(t, n, d, dtype=torch.bool, device="cuda") for n in (h, h, hk, hk)]
+    g = h // hk
+    if place == "q":      # a row of P
+        m[0][at, head] = m[1][at, head] = True
+        m[2][lo:at + 1, head // g] = m[3][lo:at + 1, head // g] = True
+    elif place == "k":    # every row of P that sees it, for the heads of the group
+        m[0][at:hi, head * g:head * g + g] = m[1][at:hi, head * g:head * g + g] = True
+        m[2][lo:hi, head] = m[3][lo:hi, head] = True
+    elif place == "v":    # a column of those rows of out; D of those rows, and with it dS; not dv
+        m[0][at:hi, head * g:head * g + g, col] = True
+        m[1][at:hi, head * g:head * g + g] = True
+        m[2][lo:hi, head] = True
+    else:                 # dO: a row of dS, a column of dv
+        m[1][at, head] = True
+        m[2][lo:at + 1, head // g] = True
+        m[3][lo:at + 1, head // g, col] = True
+    return m
+
+
+NAN_LENGTHS = (([100, 200, 37, 300], 150, 637), ([513, 3, 1, 700], 2, 1300), ([1000], 400, 1000),
+               ([60, 1, 1, 200], 60, 262))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 36, 128))
+@pytest.mark.parametrize("place,fill", (("q", "nan"), ("k", "nan"), ("v", "nan"), ("v", "inf"), ("v", "-inf")))
+@pytest.mark.parametrize("lengths,at,total", NAN_LENGTHS)
+def test_non_finite_values_reach_what_sees_them_only(dtype, d, place, fill, lengths, at, total):
+    """A NaN or an infinity in one entry of one head: what the formula takes it to is not finite, and everything else,
+    in the same tiles, of later and of earlier tokens of the same sequence, is as without it."""
+    h, hk, col = 4, 2, 5
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    q, k, v, _ = make(total, h, hk, d, dtype, 31)
+    want = reference(q, k, v, cu)[0]
+    {"q": q, "k": k, "v": v}[place][at, 1, col] = float(fill)
+    bad = poisoned(place, fill, at, 1, col, cu, h, hk, total, d)[0]
+    for grad in (False, True):  # with a gradient to come the forward also saves what out's rounding left over
+        got = packed_attention(q.requires_grad_(grad), k, v, torch.tensor(cu, dtype=torch.int32, device="cuda")).detach()
+        assert not torch.isfinite(got[bad]).any()
+        assert err(got[~bad], want[~bad]) <= OUT[dtype] * U[dtype]
+
+
+def test_everything_not_finite():
+    """Inputs of NaN only come back as NaN, and calls after it are as ever."""
+    for dtype in DTYPES:
+        q, k, v, do = make(2000, 4, 2, 64, dtype, 37)
+        cu = torch.tensor([0, 900, 901, 2000], dtype=torch.int32, device="cuda")
+        x = [torch.full_like(y, float("nan")).requires_grad_(True) for y in (q, k, v)]
+        out = packed_attention(*x, cu)
+        assert torch.isnan(out).all()
+        assert all(torch.isnan(y).all() for y in torch.autograd.grad(out, x, do))
+        check([0, 900, 901, 2000], 4, 2, 64, dtype, seed=37)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_large_scores(dtype):
     """Scores of several hundreds: the running maximum moves by more than exp2's range from tile to tile."""
