@@ -238,7 +238,8 @@ size_t mhc_attn_fwd_workspace(int64_t T);
  * sequences: cu_seqlens != NULL: sequence b is the tokens [cu_seqlens[b],
  * cu_seqlens[b+1]), b < batch (device int32, non-decreasing; sequences may be
  * empty, and tokens before the first and after the last belong to none: their
- * out is 0 and what their q, k, v hold, NaN included, touches no other token);
+ * out is 0 and what their q, k, v hold, NaN included, touches no other token; nor
+ * does a NaN or an infinity of a sequence touch a token that does not see it);
  * NULL: sequences of seqlen tokens each, T a multiple of it.
  *
  * q, k, v: element (t, h, d) at t * strides[0] + h * strides[1] + d (q), strides

@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(cons
 // DKV = true: a block owns 64 keys of one key head, sums dK and dV over the queries
 // that see them, of every head of the group or, with splits, of its share of them.
 template <typename T, int DP, int ROWS, bool DKV, bool ASYNC>
-__global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const Args a, const Work work) {
+__global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(const __grid_constant__ Args a, const Work work) {
   constexpr int THREADS = threads_of(ROWS);
   extern __shared__ float sm[];
   constexpr int TS = TILE * (DP + 4), RS = ROWS * (DP + 4);
@@ -410,15 +410,19 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
     const int64_t kt = (int64_t)a.Hk * a.D;
     auto store = [&](auto *dk, auto *dv) {
       using U = std::remove_pointer_t<decltype(dk)>;
-      store_rows<U, DP>(dk + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
-      store_rows<U, DP>(dv + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+      bool bad = store_rows<U, DP>(dk + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
+      bad |= store_rows<U, DP>(dv + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
+      if (__syncthreads_or(bad)) redo_dkv_rows<T>(a, rh, r0, ROWS, rh * G + part * per, per, dk, dv, tid >> 5, THREADS / 32, tid & 31);
     };
     if (splits > 1)
       store(a.parts + 2 * part * a.T * kt, a.parts + (2 * part + 1) * a.T * kt);
     else
       store(static_cast<T *>(a.dk), static_cast<T *>(a.dv));
   } else {
-    store_rows<T, DP>(static_cast<T *>(a.dq) + (int64_t)rh * a.D, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc);
+    T *dq = static_cast<T *>(a.dq) + (int64_t)rh * a.D;
+    if (__syncthreads_or(store_rows<T, DP>(dq, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc)))
+      for (int r = tid >> 5; r < ROWS && r0 + r < a.T; r += THREADS / 32)
+        if (row_has_nan(dq + (r0 + r) * ot, a.D, tid & 31)) redo_dq<T>(a, rh, r0 + r, tid & 31);
   }
 }
 

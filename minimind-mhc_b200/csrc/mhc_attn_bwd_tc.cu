@@ -42,6 +42,7 @@
 
 #include <mutex>
 
+#include "mhc_attn_redo.cuh"
 #include "mhc_attn_tc.cuh"
 
 namespace mhc {
@@ -147,7 +148,7 @@ __device__ __forceinline__ uint32_t dp_col(int g) { return DKV || (g & 1) == 0 ?
 template <typename T, int DP, bool DKV>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Map r2map, const __grid_constant__ Map c1map,
-                   const __grid_constant__ Map c2map, const Args a, const Sched sched) {
+                   const __grid_constant__ Map c2map, const __grid_constant__ Args a, const Sched sched) {
   using C = Cfg<DP>;
   using L = typename C::L;
   constexpr int ST = C::ST;
@@ -157,7 +158,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   __shared__ Item items[2];
   __shared__ __align__(8) uint64_t bars[NBARS];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int abort_word, redo_word;  // redo: a NaN has been written
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *gen = smem_raw + (base - raw);
@@ -169,7 +170,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
-    abort_word = 0;
+    abort_word = redo_word = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(B_ITEM_F + i), 1);
       mbar_init(BAR(B_ITEM_E + i), NSOFT + 1);  // the softmax warps and the MMA warp have read it
@@ -528,6 +529,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       // epilogue: every fourth 16 columns of the row's results
       const int64_t at = ((int64_t)tok * (DKV ? a.Hk : a.H) + head) * a.D;
       constexpr int PIECES = DP / 16;
+      bool bad = false;
 #pragma unroll 1
       for (int q = part; q < (DKV ? 2 : 1) * PIECES; q += 4) {
         const bool second = DKV && q >= PIECES;
@@ -541,6 +543,8 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0u;
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) bad |= isnan(__uint_as_float(o[e]));
         if (DKV && a.splits > 1) {
           float *pd = a.parts + ((int64_t)(split * 2 + second) * a.T * a.Hk * a.D) + at + d;
 #pragma unroll
@@ -558,6 +562,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           if (tok < a.T && d + h * 8 < a.D)
             *reinterpret_cast<uint4 *>(dst + d + h * 8) = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
       }
+      if (bad && tok < a.T) redo_word = 1;
       tc_fence_before();
     }
     if (!ok && lane == 0) give_up(ERR_SOFTMAX, abort_flag, a.err_flag);
@@ -588,6 +593,25 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         } else {
           static_cast<T *>(a.dq)[at] = bad;
         }
+      }
+    }
+  } else if (redo_word) {
+    constexpr int WARPS = NTHREADS / 32;
+    for (int i = 0;; ++i) {
+      Item it;
+      if (!item_of<DKV>(a, sched, snake(i, blockIdx.x, gridDim.x), it)) break;
+      if constexpr (DKV) {
+        const int64_t n = a.T * a.Hk * a.D;
+        const int per = a.H / a.Hk / a.splits;
+        if (a.splits > 1)
+          redo_dkv_rows<T>(a, it.head, it.r0, TM, it.c_head, per, a.parts + 2 * it.part * n, a.parts + (2 * it.part + 1) * n, warp, WARPS,
+                           lane);
+        else
+          redo_dkv_rows<T>(a, it.head, it.r0, TM, it.c_head, per, static_cast<T *>(a.dk), static_cast<T *>(a.dv), warp, WARPS, lane);
+      } else {
+        for (int r = warp; r < TM && it.r0 + r < a.T; r += WARPS)
+          if (row_has_nan(static_cast<const T *>(a.dq) + ((int64_t)(it.r0 + r) * a.H + it.head) * a.D, a.D, lane))
+            redo_dq<T>(a, it.head, it.r0 + r, lane);
       }
     }
   }

@@ -82,5 +82,68 @@ __device__ __noinline__ void redo_out(const Args &a, int h, int i, int lane) {
   if (a.o_lo) lane_store(static_cast<T *>(a.o_lo) + at, a.D, lane, lo);
 }
 
+// dq of token i, head h
+template <typename T>
+__device__ __noinline__ void redo_dq(const Args &a, int h, int i, int lane) {
+  const int hk = h / (a.H / a.Hk);
+  const int64_t at = ((int64_t)i * a.H + h) * a.D, stat = (int64_t)h * a.Tp + i;
+  float q[LANE_D], g[LANE_D], dq[LANE_D] = {};
+  lane_row<T>(a.q, (int64_t)i * a.qt + h * a.qh, a.D, lane, q);
+  lane_row<T>(a.dout, at, a.D, lane, g);
+  const float lse = a.lse[stat], mean = a.delta[stat];
+  const int start = span_of(a, i).start;
+  for (int j = start; j <= i; ++j) {
+    float k[LANE_D], v[LANE_D];
+    lane_row<T>(a.k, (int64_t)j * a.kt + hk * a.kh, a.D, lane, k);
+    lane_row<T>(a.v, (int64_t)j * a.vt + hk * a.vh, a.D, lane, v);
+    const float ds = exp2f(fmaf(lane_dot(q, k), a.scale_log2, -lse)) * (lane_dot(g, v) - mean);
+#pragma unroll
+    for (int u = 0; u < LANE_D; ++u) dq[u] = fmaf(ds, k[u], dq[u]);
+    if (((j - start) & 31) == 31 && lane_all_nan(dq, a.D, lane)) break;
+  }
+#pragma unroll
+  for (int u = 0; u < LANE_D; ++u) dq[u] *= a.scale;
+  lane_store(static_cast<T *>(a.dq) + at, a.D, lane, dq);
+}
+
+// dk and dv of token j, key head hk, over `heads` query heads from h0 on
+template <typename T, typename U>
+__device__ __noinline__ void redo_dkv(const Args &a, int hk, int j, int h0, int heads, U *dk_row, U *dv_row, int lane) {
+  float k[LANE_D], v[LANE_D], dk[LANE_D] = {}, dv[LANE_D] = {};
+  lane_row<T>(a.k, (int64_t)j * a.kt + hk * a.kh, a.D, lane, k);
+  lane_row<T>(a.v, (int64_t)j * a.vt + hk * a.vh, a.D, lane, v);
+  const int end = span_of(a, j).end;
+  bool dead = false;
+  for (int h = h0; h < h0 + heads && !dead; ++h)
+    for (int i = j; i < end && !dead; ++i) {
+      float q[LANE_D], g[LANE_D];
+      lane_row<T>(a.q, (int64_t)i * a.qt + h * a.qh, a.D, lane, q);
+      lane_row<T>(a.dout, ((int64_t)i * a.H + h) * a.D, a.D, lane, g);
+      const int64_t stat = (int64_t)h * a.Tp + i;
+      const float p = exp2f(fmaf(lane_dot(k, q), a.scale_log2, -a.lse[stat])), ds = p * (lane_dot(v, g) - a.delta[stat]);
+#pragma unroll
+      for (int u = 0; u < LANE_D; ++u) {
+        dk[u] = fmaf(ds, q[u], dk[u]);
+        dv[u] = fmaf(p, g[u], dv[u]);
+      }
+      dead = ((i - j) & 31) == 31 && lane_all_nan(dk, a.D, lane) && lane_all_nan(dv, a.D, lane);
+    }
+#pragma unroll
+  for (int u = 0; u < LANE_D; ++u) dk[u] *= a.scale;
+  lane_store(dk_row, a.D, lane, dk);
+  lane_store(dv_row, a.D, lane, dv);
+}
+
+// The same where one of the two rows has a NaN: rows of dk and dv, or of a block's part of them
+template <typename T, typename U>
+__device__ __forceinline__ void redo_dkv_rows(const Args &a, int hk, int row0, int rows, int h0, int heads, U *dk, U *dv, int warp,
+                                              int warps, int lane) {
+  for (int r = warp; r < rows && row0 + r < a.T; r += warps) {
+    const int64_t at = ((int64_t)(row0 + r) * a.Hk + hk) * a.D;
+    const bool bad = row_has_nan(dk + at, a.D, lane) || row_has_nan(dv + at, a.D, lane);
+    if (bad) redo_dkv<T, U>(a, hk, row0 + r, h0, heads, dk + at, dv + at, lane);
+  }
+}
+
 }  // namespace attn
 }  // namespace mhc

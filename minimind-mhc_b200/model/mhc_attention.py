@@ -34,8 +34,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Sequences may be empty.  Tokens before ``cu_seqlens[0]`` or from
     ``cu_seqlens[-1]`` on belong to none: their output and gradients are 0, and
     nothing they hold reaches another token.  The offsets are read on the
-    device: they are not checked beyond their type.  A NaN or infinity inside of
-    a sequence can reach its neighbours within 128 tokens (a masked weight of 0
-    times it is NaN), as it reaches its own sequence by the definition.
+    device: they are not checked beyond their type.  A NaN or infinity reaches
+    what sees it by the formula, and neither another sequence nor an earlier
+    token.
     """
     return nat.host().packed_attention(q, k, v, cu_seqlens, scale)

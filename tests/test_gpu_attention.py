@@ -216,6 +216,33 @@ def test_non_finite_values_reach_what_sees_them_only(dtype, d, place, fill, leng
         assert err(got[~bad], want[~bad]) <= OUT[dtype] * U[dtype]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 36, 128))
+@pytest.mark.parametrize("place,fill", (("q", "nan"), ("k", "nan"), ("v", "nan"), ("v", "inf"), ("v", "-inf"),
+                                        ("do", "nan"), ("do", "inf")))
+@pytest.mark.parametrize("lengths,at,total", NAN_LENGTHS)
+@pytest.mark.parametrize("h,hk", ((4, 2), (16, 2)))
+def test_non_finite_values_reach_the_gradients_that_meet_them_only(dtype, d, place, fill, lengths, at, total, h, hk):
+    """The same of dq, dk and dv, with the heads of a group in one block and shared out over several."""
+    col = 5
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    q, k, v, do = make(total, h, hk, d, dtype, 31)
+    want = reference(q, k, v, cu, do)[1:]
+    x = [y.clone() for y in (q, k, v, do)]
+    x["qkv".index(place) if place != "do" else 3][at, 1, col] = float(fill)
+    reach = poisoned(place, fill, at, 1, col, cu, h, hk, total, d)[1:]
+    a, b, c = (y.requires_grad_(True) for y in x[:3])
+    out = packed_attention(a, b, c, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    for got, ref, bad in zip(torch.autograd.grad(out, (a, b, c), x[3]), want, reach):
+        assert not torch.isfinite(got[bad]).any()
+        assert torch.isfinite(got[~bad]).all()
+        off = (got[~bad].double() - ref[~bad]).norm().item()
+        floor = 2.0 ** -20 * do.double().norm().item() * d ** 0.5
+        assert off <= GRAD[dtype] * U[dtype] * ref[~bad].norm().item() + floor
+
+
 def test_everything_not_finite():
     """Inputs of NaN only come back as NaN, and calls after it are as ever."""
     for dtype in DTYPES:
