@@ -282,8 +282,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_fwd_generic_kernel(cons
   T *lo = a.o_lo ? static_cast<T *>(a.o_lo) + (int64_t)h * a.D : nullptr;
   T *out = static_cast<T *>(a.o) + (int64_t)h * a.D;
   if (__syncthreads_or(store_rows<T, DP>(out, lo, (int64_t)a.H * a.D, q0, a.T, a.D, ty, tx, acc, inv)))
-    for (int r = tid >> 5; r < ROWS && q0 + r < a.T; r += THREADS / 32)
-      if (row_has_nan(out + (int64_t)(q0 + r) * a.H * a.D, a.D, tid & 31)) redo_out<T>(a, h, q0 + r, tid & 31);
+    redo_out_rows<T>(a, h, q0, ROWS, tid >> 5, THREADS / 32, tid & 31);
 }
 
 // DKV = false: a block owns 64 queries of one head, sums dQ over their keys.
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
       using U = std::remove_pointer_t<decltype(dk)>;
       bool bad = store_rows<U, DP>(dk + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc1, sc);
       bad |= store_rows<U, DP>(dv + (int64_t)rh * a.D, static_cast<U *>(nullptr), kt, r0, a.T, a.D, ty, tx, acc2, one);
-      if (__syncthreads_or(bad)) redo_dkv_rows<T>(a, rh, r0, ROWS, rh * G + part * per, per, dk, dv, tid >> 5, THREADS / 32, tid & 31);
+      if (__syncthreads_or(bad)) redo_dkv_rows<T, U>(a, rh, r0, ROWS, rh * G + part * per, per, dk, dv, tid >> 5, THREADS / 32, tid & 31);
     };
     if (splits > 1)
       store(a.parts + 2 * part * a.T * kt, a.parts + (2 * part + 1) * a.T * kt);
@@ -421,8 +420,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
   } else {
     T *dq = static_cast<T *>(a.dq) + (int64_t)rh * a.D;
     if (__syncthreads_or(store_rows<T, DP>(dq, static_cast<T *>(nullptr), ot, r0, a.T, a.D, ty, tx, acc1, sc)))
-      for (int r = tid >> 5; r < ROWS && r0 + r < a.T; r += THREADS / 32)
-        if (row_has_nan(dq + (r0 + r) * ot, a.D, tid & 31)) redo_dq<T>(a, rh, r0 + r, tid & 31);
+      redo_dq_rows<T>(a, rh, r0, ROWS, tid >> 5, THREADS / 32, tid & 31);
   }
 }
 

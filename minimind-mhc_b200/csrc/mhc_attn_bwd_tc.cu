@@ -604,14 +604,12 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
         const int64_t n = a.T * a.Hk * a.D;
         const int per = a.H / a.Hk / a.splits;
         if (a.splits > 1)
-          redo_dkv_rows<T>(a, it.head, it.r0, TM, it.c_head, per, a.parts + 2 * it.part * n, a.parts + (2 * it.part + 1) * n, warp, WARPS,
-                           lane);
+          redo_dkv_rows<T, float>(a, it.head, it.r0, TM, it.c_head, per, a.parts + 2 * it.part * n, a.parts + (2 * it.part + 1) * n, warp,
+                                  WARPS, lane);
         else
-          redo_dkv_rows<T>(a, it.head, it.r0, TM, it.c_head, per, static_cast<T *>(a.dk), static_cast<T *>(a.dv), warp, WARPS, lane);
+          redo_dkv_rows<T, T>(a, it.head, it.r0, TM, it.c_head, per, static_cast<T *>(a.dk), static_cast<T *>(a.dv), warp, WARPS, lane);
       } else {
-        for (int r = warp; r < TM && it.r0 + r < a.T; r += WARPS)
-          if (row_has_nan(static_cast<const T *>(a.dq) + ((int64_t)(it.r0 + r) * a.H + it.head) * a.D, a.D, lane))
-            redo_dq<T>(a, it.head, it.r0 + r, lane);
+        redo_dq_rows<T>(a, it.head, it.r0, TM, warp, WARPS, lane);
       }
     }
   }

@@ -511,11 +511,7 @@ attn_fwd_tc_kernel(const __grid_constant__ Map qmap, const __grid_constant__ Map
       Item it;
       if (!item_of(a, sched, snake(i, blockIdx.x, gridDim.x), it)) break;
       for (int t = 0; t < 2; ++t)
-        for (int r = warp; it.q0[t] >= 0 && r < TM && it.q0[t] + r < a.T; r += NTHREADS / 32) {
-          const int tok = it.q0[t] + r;
-          if (row_has_nan(static_cast<const T *>(a.o) + ((int64_t)tok * a.H + it.head[t]) * a.D, a.D, lane))
-            redo_out<T>(a, it.head[t], tok, lane);
-        }
+        if (it.q0[t] >= 0) redo_out_rows<T>(a, it.head[t], it.q0[t], TM, warp, NTHREADS / 32, lane);
     }
   }
 #undef BAR
