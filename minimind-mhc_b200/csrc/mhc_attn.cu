@@ -442,8 +442,10 @@ __global__ void __launch_bounds__(256) attn_join_any_kernel(const Args a) {
 // O alone would show in dS as an error of its own size.  Four lanes a row, the rows
 // of all heads as they lie; it reads O, its rest and dO once, and a lane asks for all
 // of its part before it adds (16 lanes a row, 4 rows in turn: 22 us at 16384 tokens, 8
-// heads of 96; so: 11.6).  fp16: also the largest |dO| and |V| inside of the
-// sequences.
+// heads of 96; so: 11.6).  fp16: also the largest finite |dO| and |V| of every
+// sequence, kept at its first token.
+__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t *amax) {
   const int l = threadIdx.x & 3;
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t 
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           s = fmaf(to_f(ov[u][e]) + (lo ? to_f(lv[u][e]) : 0.f), to_f(dv[u][e]), s);
-          if (amax) most_o = fmaxf(most_o, fabsf(to_f(dv[u][e])));
+          if (amax) most_o = fmaxf(most_o, finite_abs(to_f(dv[u][e])));
         }
       }
     }
@@ -494,15 +496,23 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const Args a, uint32_t 
     if (row >= rows || t < range.start || t >= range.end)
       most_o = 0.f;
     else if (h < a.Hk)
-      for (int c = l; c < a.D; c += 4) most_v = fmaxf(most_v, fabsf(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
-#pragma unroll
-    for (int x = 16; x; x >>= 1) {
-      most_o = fmaxf(most_o, __shfl_xor_sync(0xffffffffu, most_o, x));
-      most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, x));
-    }
-    if ((threadIdx.x & 31) == 0) {  // of non-negative floats the bits are in order: a maximum in any order
-      atomicMax(amax, __float_as_uint(most_o));
-      atomicMax(amax + 1, __float_as_uint(most_v));
+      for (int c = l; c < a.D; c += 4) most_v = fmaxf(most_v, finite_abs(to_f(static_cast<const T *>(a.v)[t * a.vt + h * a.vh + c])));
+    // a row's sequence by its first token; rows outside of all go with the warp's first
+    const bool in = row < rows && t >= range.start && t < range.end;
+    int start = in ? span_of(a, (int)t).start : -1;
+    const unsigned have = __ballot_sync(0xffffffffu, in);
+    if (have) {
+      const int one = __shfl_sync(0xffffffffu, start, __ffs((int)have) - 1);
+      start = in ? start : one;
+      const bool whole = __all_sync(0xffffffffu, start == one);
+      for (int x = whole ? 16 : 2; x; x >>= 1) {
+        most_o = fmaxf(most_o, __shfl_xor_sync(0xffffffffu, most_o, x));
+        most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, x));
+      }
+      if ((threadIdx.x & (whole ? 31 : 3)) == 0) {  // of non-negative floats the bits are in order: a maximum in any order
+        atomicMax(amax + 2 * (int64_t)start, __float_as_uint(most_o));
+        atomicMax(amax + 2 * (int64_t)start + 1, __float_as_uint(most_v));
+      }
     }
   }
 }
@@ -716,12 +726,12 @@ int mhc_attn_fwd(const void *q, const void *k, const void *v, int dtype, int64_t
 
 int64_t mhc_attn_lse_pitch(int64_t T) { return T < 1 ? 0 : (T + 127) / 128 * 128; }
 
-// delta, the two orders of the work, the two maxima of fp16, the parts of dK and dV
+// delta, the two orders of the work, the maxima of fp16, the parts of dK and dV
 size_t mhc_attn_bwd_workspace(int64_t T, int H, int Hk, int D) {
   if (T < 1 || H < 1 || Hk < 1 || H % Hk || D < 1 || D > 128) return 256;
   const int splits = attn_bwd_splits(T, H, Hk);
   const size_t parts = splits > 1 ? (size_t)splits * 2 * T * Hk * D * 4 : 0;
-  return (size_t)mhc_attn_lse_pitch(T) * H * 4 + 2 * attn_order_bytes(T) + 256 + parts;
+  return (size_t)mhc_attn_lse_pitch(T) * (4 * (size_t)H + 8) + 2 * attn_order_bytes(T) + 256 + parts;
 }
 
 int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, const void *out_lo, const void *dout,
@@ -754,11 +764,11 @@ int mhc_attn_bwd(const void *q, const void *k, const void *v, const void *out, c
   if (tc && dtype == MHC_F16) {
     amax = reinterpret_cast<uint32_t *>(order + 2 * on);
     a.amax = amax;
-    e = cudaMemsetAsync(amax, 0, 8, st);
+    e = cudaMemsetAsync(amax, 0, (size_t)a.Tp * 8, st);
   }
   if (e == cudaSuccess) e = launch_attn_delta(a, amax, st);
   a.splits = attn_bwd_splits(T, H, Hk);
-  const uintptr_t at = (reinterpret_cast<uintptr_t>(order + 2 * on) + 8 + 15) & ~(uintptr_t)15;
+  const uintptr_t at = (reinterpret_cast<uintptr_t>(order + 2 * on) + (uintptr_t)a.Tp * 8 + 15) & ~(uintptr_t)15;
   a.parts = a.splits > 1 ? reinterpret_cast<float *>(at) : nullptr;
   if (e == cudaSuccess && tc) {
     e = launch_attn_bwd_tc(a, order, order + on, st);

@@ -14,7 +14,7 @@ struct Args {
   const void *q, *k, *v, *out, *out_lo, *dout;
   void *o, *o_lo, *dq, *dk, *dv;
   float *lse, *delta;
-  const uint32_t *amax;  // fp16 backward: the bits of max|dO| and max|V|
+  const uint32_t *amax;  // fp16 backward: at a sequence's start s, 2 s and 2 s + 1: the bits of its largest finite |dO| and |V|
   int64_t T, Tp;         // Tp: T up to whole tiles of 128, the pitch of lse and delta
   int H, Hk, D, dtype;
   int64_t qt, qh, kt, kh, vt, vh;

@@ -30,7 +30,7 @@
 // they double the hand-offs.
 //
 // fp16 has no room for small dS or P: P is held times 2^10, and dS times a power of
-// two from the largest |dO| and |V| of the call that no dS can overflow
+// two from the largest finite |dO| and |V| of its sequence that no dS can overflow
 // (|dS| <= 2 D max|dO| max|V|); both come off in fp32 at the end.  bf16 needs
 // neither.
 //
@@ -129,16 +129,13 @@ __device__ __forceinline__ bool item_of(const Args &a, const Sched &s, int64_t r
   return true;
 }
 
-// fp16: the power of two that dS is held times, from the bits of max|dO| and max|V|
-template <typename T>
-__device__ __forceinline__ float ds_factor(const Args &a) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const float b = 2.f * (float)a.D * __uint_as_float(a.amax[0]) * __uint_as_float(a.amax[1]);
-    if (!(b > 0.f) || b > 1e38f) return 1.f;
-    const int e = 15 - (ilogbf(b) + 1);  // b 2^e < 2^15
-    return ldexpf(1.f, max(-60, min(60, e)));
-  }
-  return 1.f;
+// fp16: the power of two that a token's row of dS is held times, from max|dO| and max|V| of its sequence
+__device__ __forceinline__ float ds_factor(const Args &a, int tok, int start) {
+  if (start > tok) return 1.f;  // outside of every sequence
+  const float b = 2.f * (float)a.D * __uint_as_float(a.amax[2 * (int64_t)start]) * __uint_as_float(a.amax[2 * (int64_t)start + 1]);
+  if (!(b > 0.f)) return 1.f;
+  const int e = 15 - (ilogbf(b) + 1);  // b 2^e < 2^15
+  return ldexpf(1.f, max(-60, min(60, e)));
 }
 
 // where the dP of the g-th column tile lies
@@ -416,8 +413,7 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
     const float c = a.scale_log2;
     const uint64_t c2 = f2_pack(c, c);
     const float shift = F16 ? P_SHIFT : 0.f;
-    const float dsf = F16 ? ds_factor<T>(a) * exp2f(-P_SHIFT) : 1.f;  // what dS is held times, P's own factor off
-    const float out1 = a.scale / (F16 ? ds_factor<T>(a) : 1.f), out2 = F16 ? exp2f(-P_SHIFT) : 1.f;
+    const float out2 = F16 ? exp2f(-P_SHIFT) : 1.f;
     bool ok = true;
     int step = 0, nacc = 0;
     auto arrive = [&](int bar) {  // the warp's TMEM accesses are complete
@@ -435,6 +431,9 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
       const int tok = r0 + row;
       Span sp{tok + 1, tok};
       if (tok < a.T) sp = span_of(a, tok);
+      const float held = F16 ? ds_factor(a, tok, sp.start) : 1.f;
+      const float dsf = F16 ? held * out2 : 1.f;  // what dS is held times, P's own factor off
+      const float out1 = a.scale / held;
       float row_lse = 0.f, row_d = 0.f;
       if (!DKV) {
         row_lse = shift - a.lse[(int64_t)head * a.Tp + tok];  // padded to whole tiles

@@ -243,6 +243,24 @@ def test_non_finite_values_reach_the_gradients_that_meet_them_only(dtype, d, pla
         assert off <= GRAD[dtype] * U[dtype] * ref[~bad].norm().item() + floor
 
 
+@pytest.mark.parametrize("fill", (float("inf"), -float("inf"), float("nan"), 60000.0))
+@pytest.mark.parametrize("place", ("v", "do"))
+def test_small_fp16_gradients_beside_a_large_entry(place, fill):
+    """dO of size 2^-16 (an unscaled mean over tokens) beside an entry of another sequence that is not finite, or large: dS
+    is still held in the range of fp16.  Keys of size 2^8 beside queries of 2^-8 make a dq that fp16 can hold."""
+    cu = [0, 256, 700]
+    q, k, v, do = make(700, 4, 2, 64, torch.float16, 41)
+    q, k, do = q * 2.0 ** -8, k * 2.0 ** 8, do * 2.0 ** -16
+    want = reference(q, k, v, cu, do)[1:]
+    {"v": v, "do": do}[place][100, 1, 3] = fill
+    x = [y.requires_grad_(True) for y in (q, k, v)]
+    out = packed_attention(*x, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    for got, ref in zip(torch.autograd.grad(out, x, do), want):
+        # the results themselves are fp16: half a step of its smallest numbers, 2^-25, each, beside the relative bound
+        off = (got[256:].double() - ref[256:]).norm().item()
+        assert off <= GRAD[torch.float16] * U[torch.float16] * ref[256:].norm().item() + 2.0 ** -25 * ref[256:].numel() ** 0.5
+
+
 def test_everything_not_finite():
     """Inputs of NaN only come back as NaN, and calls after it are as ever."""
     for dtype in DTYPES:
