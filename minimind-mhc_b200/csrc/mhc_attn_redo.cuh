@@ -96,7 +96,7 @@ __device__ __noinline__ void redo_out(const Args &a, int h, int i, int lane) {
 
 // Rows [row0, row0 + rows) of head h of out; each warp of the block calls it
 template <typename T>
-__device__ __forceinline__ void redo_out_rows(const Args &a, int h, int row0, int rows, int warp, int warps, int lane) {
+__device__ __noinline__ void redo_out_rows(const Args &a, int h, int row0, int rows, int warp, int warps, int lane) {
   const int hk = h / (a.H / a.Hk), last = (int)min((int64_t)row0 + rows, a.T);
   int start = -1, at[LANE_D];
   for (int i = row0 + warp; i < last; i += warps) {
@@ -143,7 +143,7 @@ __device__ __noinline__ void redo_dq(const Args &a, int h, int i, int lane) {
 
 // Rows of head h of dq.  A D that is not finite leaves no dS of its row finite.
 template <typename T>
-__device__ __forceinline__ void redo_dq_rows(const Args &a, int h, int row0, int rows, int warp, int warps, int lane) {
+__device__ __noinline__ void redo_dq_rows(const Args &a, int h, int row0, int rows, int warp, int warps, int lane) {
   for (int i = row0 + warp; i < row0 + rows && i < a.T; i += warps) {
     const int64_t stat = (int64_t)h * a.Tp + i;
     if (isnan(a.lse[stat]) || !isfinite(a.delta[stat])) continue;
@@ -186,7 +186,7 @@ __device__ __noinline__ void redo_dkv(const Args &a, int hk, int j, int h0, int 
 // Rows of key head hk of dk and dv, or of a block's part of them.  Every column of dk has to do with all of dS; a
 // column of dv only with that column of dO.
 template <typename T, typename U>
-__device__ __forceinline__ void redo_dkv_rows(const Args &a, int hk, int row0, int rows, int h0, int heads, U *dk, U *dv, int warp,
+__device__ __noinline__ void redo_dkv_rows(const Args &a, int hk, int row0, int rows, int h0, int heads, U *dk, U *dv, int warp,
                                               int warps, int lane) {
   // the rows backwards, so that what a row adds to the queries of the last one is looked at once
   const int last = (int)min((int64_t)row0 + rows, a.T) - 1;
