@@ -305,11 +305,13 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
   const T *dout = static_cast<const T *>(a.dout);
   const int64_t ot = (int64_t)a.H * a.D;
   int bound[R];  // DKV: the end of the key's sequence; else the start of the query's
+  int alone[R];  // the column whose dS is 0: a sequence's first token, as a query, sees itself only; none: -1
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int t = r0 + ty * R + i;
     const Span s = t < a.T ? span_of(a, t) : Span{t + 1, t};
     bound[i] = DKV ? s.end : s.start;
+    alone[i] = s.start == t ? t : -1;
   }
   if (DKV) {
     load_tile<T, DP, ROWS, THREADS>(R1, k + rh * a.kh, a.kt, r0, a.D, range);
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(threads_of(ROWS)) attn_bwd_generic_kernel(cons
           const bool seen = DKV ? c >= r && c < bound[i] : c <= r && c >= bound[i];
           const int n = DKV ? tx + 16 * j : ty * R + i;
           p[i][j] = seen ? exp2f(fmaf(p[i][j], a.scale_log2, -L[n])) : 0.f;
-          ds[i][j] = seen ? p[i][j] * (ds[i][j] - Dl[n]) : 0.f;
+          ds[i][j] = seen ? (c == alone[i] ? 0.f : p[i][j]) * (ds[i][j] - Dl[n]) : 0.f;
         }
       }
       if constexpr (DKV) {

@@ -12,6 +12,9 @@
 //                                          rows R1 = Q, R2 = dO, columns C1 = K, C2 = V
 //          S, P, dP, dS as above with lse and D of the row;   dQ += dS C1
 //
+// A sequence's first token sees itself only: its P is 1 whatever the score, and its dS
+// is made the 0 that dP - D is but for the order of two sums.
+//
 // (seven products of 128 x 128 x D a tile where five would do if dQ were added up
 // over blocks: two more on the tensor core instead of atomics in an order that
 // changes).  P and dS never leave TMEM: a thread reads a quarter of a row of S, writes
@@ -454,7 +457,8 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           if (!WAIT_WARP(BAR(B_1F + step % ST), (uint32_t)(step / ST) & 1u)) { ok = false; break; }
         }
         // columns of this part that the row sees: [lo, hi)
-        const int lo = (DKV ? tok : sp.start) - col0, hi = (DKV ? sp.end : tok + 1) - col0;
+        // (dS of a sequence's first token, which sees itself only, is 0: DQ takes it as a row that sees nothing)
+        const int lo = (DKV ? tok : sp.start) - col0, hi = (DKV ? sp.end : sp.start == tok ? tok : tok + 1) - col0;
         const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 32);
         float p[32];
 #pragma unroll
@@ -489,6 +493,13 @@ attn_bwd_tc_kernel(const __grid_constant__ Map r1map, const __grid_constant__ Ma
           tmem_st16(p_addr, w);
           tmem_wait_st();
           arrive(B_PF);
+          // behind P, which dV needs: the first token's dS with itself
+          const uint32_t self = sp.start == tok && lo >= 0 && lo < 32 ? 1u << lo : 0u;
+          if (cut && __any_sync(0xffffffffu, self != 0u)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (self & (1u << e)) p[e] = 0.f;
+          }
         }
         if (!WAIT_WARP(BAR(B_DPF + (step & 1)), (uint32_t)(step >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();

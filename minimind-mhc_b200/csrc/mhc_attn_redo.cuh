@@ -127,12 +127,14 @@ __device__ __noinline__ void redo_dq(const Args &a, int h, int i, int lane) {
   lane_row<T>(a.q, (int64_t)i * a.qt + h * a.qh, a.D, lane, q);
   lane_row<T>(a.dout, at, a.D, lane, g);
   const float lse = a.lse[stat], mean = a.delta[stat];
+  const int start = span_of(a, i).start;
 #pragma unroll 4
-  for (int j = span_of(a, i).start; j <= i; ++j) {
+  for (int j = start; j <= i; ++j) {
     float k[LANE_D], v[LANE_D];
     lane_row<T>(a.k, (int64_t)j * a.kt + hk * a.kh, a.D, lane, k);
     lane_row<T>(a.v, (int64_t)j * a.vt + hk * a.vh, a.D, lane, v);
-    const float ds = exp2f(fmaf(lane_dot(q, k), a.scale_log2, -lse)) * (lane_dot(g, v) - mean);
+    const float p = exp2f(fmaf(lane_dot(q, k), a.scale_log2, -lse));
+    const float ds = (start == i ? 0.f : p) * (lane_dot(g, v) - mean);  // alone: 0 but for rounding
 #pragma unroll
     for (int u = 0; u < LANE_D; ++u) dq[u] = fmaf(ds, k[u], dq[u]);
   }
@@ -162,7 +164,7 @@ __device__ __noinline__ void redo_dkv(const Args &a, int hk, int j, int h0, int 
   float k[LANE_D], v[LANE_D], dk[LANE_D] = {}, dv[LANE_D] = {};
   lane_row<T>(a.k, (int64_t)j * a.kt + hk * a.kh, a.D, lane, k);
   lane_row<T>(a.v, (int64_t)j * a.vt + hk * a.vh, a.D, lane, v);
-  const int end = span_of(a, j).end;
+  const int start = span_of(a, j).start, end = span_of(a, j).end;
   for (int h = h0; h < h0 + heads; ++h)
 #pragma unroll 4
     for (int i = j; i < end; ++i) {
@@ -170,7 +172,8 @@ __device__ __noinline__ void redo_dkv(const Args &a, int hk, int j, int h0, int 
       lane_row<T>(a.q, (int64_t)i * a.qt + h * a.qh, a.D, lane, q);
       lane_row<T>(a.dout, ((int64_t)i * a.H + h) * a.D, a.D, lane, g);
       const int64_t stat = (int64_t)h * a.Tp + i;
-      const float p = exp2f(fmaf(lane_dot(k, q), a.scale_log2, -a.lse[stat])), ds = p * (lane_dot(v, g) - a.delta[stat]);
+      const float p = exp2f(fmaf(lane_dot(k, q), a.scale_log2, -a.lse[stat]));
+      const float ds = (start == i ? 0.f : p) * (lane_dot(v, g) - a.delta[stat]);
 #pragma unroll
       for (int u = 0; u < LANE_D; ++u) {
         dk[u] = fmaf(ds, q[u], dk[u]);

@@ -133,6 +133,30 @@ def test_more_blocks_than_sms(dtype, d, lengths, h, hk):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 36, 96, 128))
+@pytest.mark.parametrize("h,hk", ((4, 2), (1, 1), (16, 1)))
+def test_a_token_alone_has_no_gradient_but_its_value(dtype, d, h, hk):
+    """Its weight is 1 whatever q and k are: dq and dk are exactly 0, and dv is dO summed over the group's heads (its
+    weight in the backward comes from the saved log of the sum: 2^-22 of a score of up to 2^5 beside the rounding)."""
+    for cu in (list(range(301)), [0, 0, 1], [3, 4, 5, 5]):
+        t = cu[-1]
+        q, k, v, do = make(t, h, hk, d, dtype, 43)
+        x = [y.requires_grad_(True) for y in (q, k, v)]
+        out = packed_attention(*x, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+        dq, dk, dv = torch.autograd.grad(out, x, do)
+        assert torch.equal(out[cu[0]:], v.repeat_interleave(h // hk, 1)[cu[0]:])
+        assert torch.count_nonzero(dq) == 0 and torch.count_nonzero(dk) == 0
+        want = do.double().view(t, hk, h // hk, d).sum(2)
+        want[:cu[0]] = 0
+        assert (dv.double() - want).norm() <= (2 * U[dtype] + 2.0 ** -17) * want.norm()
+    # and the first token of a longer sequence has no dq
+    q, k, v, do = make(200, h, hk, d, dtype, 44)
+    x = [y.requires_grad_(True) for y in (q, k, v)]
+    out = packed_attention(*x, torch.tensor([0, 150, 200], dtype=torch.int32, device="cuda"))
+    assert torch.count_nonzero(torch.autograd.grad(out, x, do)[0][[0, 150]]) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cu,total", (([5, 90], 140), ([0, 130], 131), ([130, 260], 400), ([3, 3, 4], 9), ([0, 0], 5),
                                       ([200, 200], 300)))
 def test_tokens_outside_of_every_sequence(dtype, cu, total):
