@@ -20,8 +20,9 @@
 // Forward: one pass with the running maximum and sum.  Backward: the scores again
 // from the saved L, in two kernels of the same form (a block owns 64 queries and
 // sums dQ, or 64 keys and sums dK and dV over the heads that share them), so
-// every gradient is a sum in a fixed order.  The shared-memory operands bound it (70 to
-// 79 % of the wavefronts an SM can have, 27 to 34 % of the FFMA pipe, 4 x 2048 tokens); fp32 inputs have no tensor-core form of this accuracy.
+// every gradient is a sum in a fixed order.  The shared-memory operands bound it (71 to
+// 78 % of the wavefronts an SM can have, 28 to 34 % of the FFMA pipe, 4 x 2048 tokens).
+// Not tried: each fp32 operand as three bf16 parts, six products on the tensor cores.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -491,6 +491,8 @@ static int group_of(int E) {
   while (g * 8 < E && g < 32) g <<= 1;
   return g;
 }
+// Four blocks an SM, as many as are resident: more partial sums to join buy nothing (262,144 x 64, top 6, bf16, forward:
+// 2: 69 us, 4: 58, 8: 58; 65,536 x 256: 85, 71, 75).
 static int blocks_for(int64_t T, int E, int sms) {
   const int rows = THREADS / group_of(E);
   const int64_t b = (T + rows - 1) / rows;
@@ -573,6 +575,7 @@ int mhc_route_bwd(const void *logits, int dtype, int64_t T, int E, int64_t row_s
   router::Args a{logits, T, row_stride, E, k, ((uintptr_t)logits % 16 == 0 && (row_stride * es) % 16 == 0) ? 1 : 0,
                  coef * (float)E};
   const int rows = router::THREADS / router::group_of(E);
+  // nothing to join here: 4 to 8 blocks an SM are alike (50 to 54 us at 262,144 x 64 with autograd's part), 16 take 58
   const int64_t want = (T + rows - 1) / rows, cap = (int64_t)(device_sm_count() > 0 ? device_sm_count() : 148) * 8;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
