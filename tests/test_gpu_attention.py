@@ -133,6 +133,33 @@ def test_more_blocks_than_sms(dtype, d, lengths, h, hk):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (30, 32, 84, 90, 96, 100, 127, 128))
+def test_head_sizes_in_blocks_of_both_heights(dtype, d):
+    """Every padded head size of the CUDA-core kernels, tiles that are copied and loaded, with enough tiles for blocks of
+    64 rows.  Sums of at most 128 products and 1900 keys: sqrt(2028) < 64 roundings."""
+    check([0, 1900, 3200, 3277, 3278], 16, 8, d, dtype, seed=d)
+
+
+@pytest.mark.parametrize("dtype,d", ((torch.float32, 64), (torch.float32, 96), (torch.float32, 98), (torch.bfloat16, 36),
+                                     (torch.bfloat16, 100), (torch.bfloat16, 128), (torch.float16, 96)))
+@pytest.mark.parametrize("place", ("q", "k", "v", "do"))
+def test_non_finite_values_with_many_blocks(dtype, d, place):
+    """A NaN among 3278 tokens of 16 heads, blocks of 64 rows on the CUDA cores: it reaches what sees it only."""
+    cu, at, h, hk = [0, 1900, 3200, 3277, 3278], 1990, 16, 8
+    x = dict(zip(("q", "k", "v", "do"), make(cu[-1], h, hk, d, dtype, 47)))
+    want = reference(x["q"], x["k"], x["v"], cu, x["do"])
+    x[place][at, 1, 5] = float("nan")
+    reach = poisoned(place, "nan", at, 1, 5, cu, h, hk, cu[-1], d)
+    y = [x[n].requires_grad_(True) for n in ("q", "k", "v")]
+    out = packed_attention(*y, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    grads = torch.autograd.grad(out, y, x["do"])
+    for i, (got, ref, bad) in enumerate(zip((out, *grads), want, reach)):
+        assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+        off = (got[~bad].double() - ref[~bad]).norm().item()
+        assert off <= (OUT if i == 0 else GRAD)[dtype] * U[dtype] * ref[~bad].norm().item()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", (64, 36, 96, 128))
 @pytest.mark.parametrize("h,hk", ((4, 2), (1, 1), (16, 1)))
 def test_a_token_alone_has_no_gradient_but_its_value(dtype, d, h, hk):
