@@ -376,6 +376,143 @@ int mhc_adamw_check(const mhc_adamw_tensor *tensors, int count, int state_bits, 
 int mhc_adamw_unpack(const void *codes, int is_signed, const float *scales, float *out, int64_t n, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Answering: rotary positions                                               */
+/* ------------------------------------------------------------------------ */
+
+/* A rotation by position.  The first `part` elements of a head (even) are part / 2
+ * pairs, elements (i, i + part / 2) or, interleaved, (2 i, 2 i + 1); the others stay.
+ * turns (device, part / 2): pair i turns by turns[i] / 2^64 of a full turn for
+ * every position, so a position's angle is the product modulo 2^64: exact at any
+ * distance.  cos and sin are multiplied by gain. */
+typedef struct {
+  const uint64_t *turns;
+  int32_t part, interleaved;
+  float gain;
+} mhc_rotary;
+
+/*
+ * Rotates the heads of q (T, H, D) and k (T, Hk, D) by their tokens' positions:
+ * (a, b) -> (a c - b s, b c + a s) in fp32, rounded once to `dtype`.  Either may be
+ * left out (H or Hk 0, its pointers NULL).  Element (t, h, d) of q at
+ * t * strides[0] + h * strides[1] + d, of k at strides [2], [3] (host array of 4, in
+ * elements); q_out and k_out are contiguous and do not overlap the inputs.  Token
+ * t's position is positions[t % period] (device int32 or int64 by position_bytes 4 or
+ * 8), or t % period where positions is NULL.  inverse != 0: by the negative angle,
+ * which takes the gradients of the outputs to those of the inputs.
+ *
+ * Replaces: apply_rotary_pos_emb and its tables (model/model_minimind.py:132-159).
+ */
+int mhc_rotate(const mhc_rotary *rotary, const void *q, void *q_out, int H, const void *k, void *k_out, int Hk,
+               int dtype, int64_t T, int D, const int64_t *strides, const void *positions, int position_bytes,
+               int64_t period, int inverse, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Answering: a paged cache of keys and values and the attention over it     */
+/* ------------------------------------------------------------------------ */
+
+/* Keys and values of `layers` layers in pages of page_size tokens: element (layer,
+ * page, slot, head, d) of keys at the sum of its indexes times strides[0..3], plus d;
+ * of values with strides[4..7] (in elements). */
+typedef struct {
+  void *keys, *values;
+  int64_t pages, strides[8];
+  int32_t dtype, layers, page_size, kv_heads, dim;
+} mhc_kv_cache;
+
+/* What one step adds to the cache.  Sequence b has lengths[b] tokens in it; its new
+ * tokens are the rows [cu_tokens[b], cu_tokens[b + 1]) of the step's T rows and take
+ * the places lengths[b], lengths[b] + 1, ...; place p of a sequence is slot p %
+ * page_size of page page_table[b * table_pitch + p / page_size].  All three arrays are
+ * on the device and only read there: places past table_width * page_size, negative
+ * ones and pages outside [0, pages) do not exist, nothing is read or written there.
+ * cu_tokens is non-decreasing; rows of no sequence (behind cu_tokens[batch]) get 0
+ * where a call has an output for them. */
+typedef struct {
+  const int32_t *page_table, *lengths, *cu_tokens;
+  int64_t table_pitch, T;
+  int32_t table_width, batch;
+} mhc_cache_step;
+
+/*
+ * Writes the new tokens' keys k and values v, (T, kv_heads, dim) each, to their
+ * places in layer 0 of the cache.  With a rotation (rotary != NULL) k is rotated on
+ * the way, and q (T, H, dim), if given, is rotated into q_out (contiguous); a token's
+ * position is positions[t], or its place where positions is NULL.  Without one q is
+ * not used.  strides: q's, k's and v's token and head strides (host array of 6).  No
+ * place may be given to two tokens.
+ *
+ * Replaces: the concatenation of past and new keys and values and the rotation
+ * before it (model/model_minimind.py:200-219).
+ */
+int mhc_append_kv(const mhc_kv_cache *cache, const mhc_cache_step *step, const void *k, const void *v, const void *q,
+                  void *q_out, int H, const int64_t *strides, const mhc_rotary *rotary, const void *positions,
+                  int position_bytes, void *stream);
+
+/*
+ * Moves the kept ones of a step's tokens up: for every layer and sequence the keys
+ * and values of new token path[cu_tokens[b] + i] go to the place of new token i, i <
+ * kept[b].  path holds indexes within the sequence, ascending; one below i or past the
+ * sequence's new tokens is skipped.
+ */
+int mhc_keep_drafts(const mhc_kv_cache *cache, const mhc_cache_step *step, const int32_t *path, const int32_t *kept,
+                    void *stream);
+
+/* Bytes of scratch `mhc_cached_attn` needs on the current device. */
+size_t mhc_cached_attn_workspace(const mhc_kv_cache *cache, const mhc_cache_step *step, int H);
+
+/*
+ * Attention of the new tokens over layer 0 of the cache, their own keys and values
+ * included (they have been appended): out = softmax(scale q K^T) V over what a token
+ * sees, all of its sequence's lengths[b] earlier tokens and of the new ones
+ *   mask == NULL: itself and those before it;
+ *   else:         new token c of its sequence if bit c of mask[t] is set (c < 64).
+ * q (T, H, dim) with token and head strides q_strides, out (T, H, dim) contiguous, both
+ * in the cache's type; H a multiple of kv_heads, dim up to 128.  Scores, softmax and
+ * sums are fp32.  A token that sees nothing gets 0.  What it does not see, NaN
+ * included, does not touch it.  The same bits every time.
+ *
+ * Replaces: scaled_dot_product_attention over past and new keys
+ * (model/model_minimind.py:220-250).
+ */
+int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const void *q, int H,
+                    const int64_t *q_strides, const int64_t *mask, float scale, void *out, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Answering: verification of drafted tokens                                 */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Which drafted tokens are kept.  Sequence b's rows [cu_tokens[b], cu_tokens[b + 1])
+ * are a tree in which a parent comes before its children: row 0 its last token,
+ * the others drafted ones with tokens[t] and parents[t] (index within the sequence).
+ * Row t of target (T, V) holds the target's probabilities behind node t, of draft
+ * those that the children of t were drawn from (NULL: the children were not drawn).
+ * Rows of probabilities are target_stride and draft_stride elements apart, of type
+ * `dtype`, and taken to sum to 1.  random (T) fp32 in [0, 1).
+ *
+ * The walk starts at row 0 with rest = its target row and mass = 1, and tests the
+ * children x of the last kept node in their order:
+ *   kept    if random[x] * mass * draft(x) < rest(x)   (draft(x) = 1 without a draft);
+ *           then rest = x's target row, mass = 1;
+ *   refused otherwise: rest = max(rest - mass * draft, 0), mass = sum of rest; without a
+ *           draft mass -= rest(x), rest(x) = 0.
+ * In the end next[b] is drawn from rest: the first token whose cumulative sum passes
+ * random[row 0] * sum.  If nothing is left of rest, it is drawn from the node's target
+ * row; if that holds nothing positive and finite either, next[b] is -1.  NaN and negative entries
+ * count as 0.  Computed in fp64.
+ *
+ * path[cu_tokens[b] + i] (T, int32) is the i-th kept row within the sequence (row 0
+ * first), -1 behind the last; kept[b] (int32) how many there are; rows of no sequence
+ * get path -1, an empty sequence kept 0 and next -1.  tokens and next are int64.  Rows
+ * behind a sequence's first 1024, tokens outside [0, V) and parents that do not come
+ * before their child are never kept.
+ */
+int mhc_verify_drafts(const int64_t *tokens, const int32_t *parents, const int32_t *cu_tokens, int batch, int64_t T,
+                      const void *target, int64_t target_stride, const void *draft, int64_t draft_stride, int dtype,
+                      int64_t V, const float *random, int32_t *path, int32_t *kept, int64_t *next, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Stand-alone Sinkhorn-Knopp                                                */
 /* ------------------------------------------------------------------------ */
 

@@ -42,6 +42,12 @@ struct Entry {
   decltype(&mhc_grad_norm) grad_norm;
   decltype(&mhc_adamw_check) adamw_check;
   decltype(&mhc_adamw_step) adamw_step;
+  decltype(&mhc_rotate) rotate;
+  decltype(&mhc_append_kv) append_kv;
+  decltype(&mhc_keep_drafts) keep_drafts;
+  decltype(&mhc_cached_attn_workspace) cached_attn_workspace;
+  decltype(&mhc_cached_attn) cached_attn;
+  decltype(&mhc_verify_drafts) verify_drafts;
 } E{};
 volatile int *give_up_flag = nullptr;  // the pinned word a kernel whose bounded wait ran out writes to
 
@@ -399,6 +405,317 @@ std::optional<Tensor> adamw(const std::vector<Group> &groups, int bits, std::opt
   return norm;
 }
 
+// ---- rotary positions -------------------------------------------------------------
+
+using Maybe = std::optional<Tensor>;
+
+// a dimension's stride; of one element none is needed, and whatever stands there must not cost the wide copies
+int64_t step_of(const Tensor &x, int64_t dim) { return x.size(dim) > 1 ? x.stride(dim) : 0; }
+// (T, heads, D) rows with contiguous heads
+Tensor flat_rows(const Tensor &x) {
+  const Tensor y = x.dim() == 4 ? x.flatten(0, 1) : x;
+  return y.stride(2) == 1 || y.size(2) == 1 ? y : y.contiguous();
+}
+void require_index(const Tensor &t, const char *who, const char *what, at::ScalarType type, const Tensor &like) {
+  require_cuda(t);
+  TORCH_CHECK_TYPE(t.scalar_type() == type, who, ": ", what, " must be ", type, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == like.device(), who, ": ", what, " is on ", t.device(), ", the rest on ", like.device());
+}
+// what has no backward must not swallow a gradient that somebody waits for
+void require_no_grad(const char *who, std::initializer_list<const Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor *t : ts)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), who, " has no gradient: call it under torch.no_grad()");
+}
+
+struct Turned {
+  Tensor q, k;
+};
+Turned turn(const Tensor &q, const Tensor &k, const Tensor &positions, int64_t period, const Tensor &turns, bool interleaved, double gain,
+            bool inverse) {
+  ready();
+  const Tensor &like = q.defined() ? q : k;
+  const c10::cuda::CUDAGuard guard(like.device());
+  Tensor q3, k3;
+  Turned out;
+  int64_t strides[4] = {0, 0, 0, 0}, t = 0;
+  if (q.defined()) {
+    q3 = flat_rows(q);
+    out.q = at::empty(q.sizes(), q.options());
+    strides[0] = step_of(q3, 0), strides[1] = step_of(q3, 1), t = q3.size(0);
+  }
+  if (k.defined()) {
+    k3 = flat_rows(k);
+    out.k = at::empty(k.sizes(), k.options());
+    strides[2] = step_of(k3, 0), strides[3] = step_of(k3, 1), t = k3.size(0);
+  }
+  const mhc_rotary r{static_cast<const uint64_t *>(turns.data_ptr()), (int32_t)(2 * turns.numel()), interleaved, (float)gain};
+  check(E.rotate(&r, ptr(q3), ptr(out.q), q.defined() ? (int)q3.size(1) : 0, ptr(k3), ptr(out.k), k.defined() ? (int)k3.size(1) : 0,
+                 dtype_code(like, "rotate"), t, (int)like.size(-1), strides, ptr(positions),
+                 positions.defined() ? (int)positions.element_size() : 0, period, inverse, stream_of(like)),
+        "mhc_rotate");
+  return out;
+}
+
+struct RotateFn : torch::autograd::Function<RotateFn> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Maybe &positions, int64_t period,
+                               const Tensor &turns, bool interleaved, double gain) {
+    const Tensor pos = positions.value_or(Tensor());
+    ctx->save_for_backward({pos, turns});
+    ctx->saved_data["period"] = period;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["gain"] = gain;
+    ctx->set_materialize_grads(false);
+    const Turned out = turn(q, k, pos, period, turns, interleaved, gain, false);
+    return {out.q, out.k};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rotate: second derivatives are not implemented");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor dq = ctx->needs_input_grad(0) ? g[0] : Tensor(), dk = ctx->needs_input_grad(1) ? g[1] : Tensor();
+    Turned out;
+    if (dq.defined() || dk.defined())
+      out = turn(dq, dk, s[0], ctx->saved_data["period"].toInt(), s[1], ctx->saved_data["interleaved"].toBool(),
+                 ctx->saved_data["gain"].toDouble(), true);
+    return {out.q, out.k, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> rotate(const Tensor &q, const Tensor &k, const Maybe &positions, const Tensor &turns, bool interleaved,
+                                  double gain) {
+  const char *who = "rotate";
+  require_plain(who, {&q, &k});
+  require_cuda(q);
+  require_cuda(k);
+  TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), who, ": q and k must have one type, got ", q.scalar_type(), " and ", k.scalar_type());
+  dtype_code(q, who);
+  const int64_t n = q.dim();
+  TORCH_CHECK_VALUE((n == 3 || n == 4) && k.dim() == n, who, ": (T, heads, D) or (B, L, heads, D) tensors are wanted, got ", q.sizes(), ", ",
+                    k.sizes());
+  bool same = q.size(-1) == k.size(-1) && q.size(0) == k.size(0) && (n == 3 || q.size(1) == k.size(1));
+  TORCH_CHECK_VALUE(same && q.size(-2) >= 1 && k.size(-2) >= 1, who, ": shapes do not match: ", q.sizes(), ", ", k.sizes());
+  TORCH_CHECK_VALUE(q.device() == k.device() && turns.device() == q.device(), who, ": q, k and the frequencies must be on one device");
+  const int64_t d = q.size(-1), part = 2 * turns.numel();
+  TORCH_CHECK_VALUE(part <= d && d <= 256, who, ": heads of ", part, " (what is rotated) to 256 elements are wanted, got ", d);
+  Tensor pos;
+  int64_t period = n == 4 ? q.size(1) : 0;
+  if (positions.has_value()) {
+    require_cuda(*positions);
+    TORCH_CHECK_TYPE(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong, who, ": positions must be int32 or int64, got ",
+                     positions->scalar_type());
+    TORCH_CHECK_VALUE(positions->device() == q.device(), who, ": positions must be on the device of q and k");
+    const bool each = positions->sizes() == q.sizes().slice(0, n - 2), row = n == 4 && positions->dim() == 1 && positions->size(0) == q.size(1);
+    TORCH_CHECK_VALUE(each || row, who, ": positions for every token are wanted, got ", positions->sizes(), " for ", q.sizes());
+    pos = positions->contiguous();
+    if (each) period = 0;
+  }
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
+    const variable_list r = RotateFn::apply(q, k, pos.defined() ? Maybe(pos) : std::nullopt, period, turns, interleaved, gain);
+    return {r[0], r[1]};
+  }
+  const Turned r = turn(q, k, pos, period, turns, interleaved, gain, false);
+  return {r.q, r.k};
+}
+
+// ---- paged cache --------------------------------------------------------------------
+
+struct Step {
+  mhc_kv_cache cache;
+  mhc_cache_step step;
+  Tensor table, lengths, cu;  // what the pointers point to
+};
+// checks keys and values ((layers,) pages, slots, heads, D) and a step of t rows
+Step step_of_cache(const char *who, const Tensor &keys, const Tensor &values, const Tensor &table, const Tensor &lengths, const Tensor &cu,
+                   int64_t t, bool layers) {
+  require_plain(who, {&keys, &values});
+  require_cuda(keys);
+  require_cuda(values);
+  TORCH_CHECK_TYPE(keys.scalar_type() == values.scalar_type(), who, ": keys and values must have one type, got ", keys.scalar_type(), " and ",
+                   values.scalar_type());
+  Step s{};
+  s.cache.dtype = dtype_code(keys, who);
+  const int64_t n = keys.dim(), f = n - 4;
+  TORCH_CHECK_VALUE((n == 4 || (layers && n == 5)) && keys.sizes() == values.sizes(), who, ": keys and values must be ",
+                    layers ? "(layers, pages, page size, heads, D) or " : "", "(pages, page size, heads, D), got ", keys.sizes(), ", ", values.sizes());
+  TORCH_CHECK_VALUE(keys.device() == values.device(), who, ": keys and values must be on one device");
+  const int64_t d = keys.size(f + 3);
+  TORCH_CHECK_VALUE(keys.size(f + 1) >= 1 && keys.size(f + 2) >= 1 && d >= 1 && d <= 256, who, ": bad cache shape ", keys.sizes());
+  TORCH_CHECK_VALUE((keys.stride(f + 3) == 1 && values.stride(f + 3) == 1) || d == 1, who, ": the cache's heads must be contiguous");
+  require_index(table, who, "page_table", at::kInt, keys);
+  require_index(lengths, who, "lengths", at::kInt, keys);
+  require_index(cu, who, "cu_tokens", at::kInt, keys);
+  TORCH_CHECK_VALUE(table.dim() == 2 && lengths.dim() == 1 && cu.dim() == 1 && table.size(0) == lengths.size(0) && cu.size(0) == lengths.size(0) + 1,
+                    who, ": page_table (B, pages), lengths (B,) and cu_tokens (B + 1,) are wanted, got ", table.sizes(), ", ", lengths.sizes(), ", ",
+                    cu.sizes());
+  TORCH_CHECK_VALUE(table.size(1) * keys.size(f + 1) < ((int64_t)1 << 31) - 4096, who, ": a sequence of ", table.size(1), " pages is too long");
+  s.table = table.size(1) > 1 && table.stride(1) != 1 ? table.contiguous() : table;
+  s.lengths = lengths.contiguous();
+  s.cu = cu.contiguous();
+  s.cache.keys = keys.data_ptr();
+  s.cache.values = values.data_ptr();
+  s.cache.layers = n == 5 ? (int32_t)keys.size(0) : 1;
+  s.cache.pages = keys.size(f);
+  s.cache.page_size = (int32_t)keys.size(f + 1);
+  s.cache.kv_heads = (int32_t)keys.size(f + 2);
+  s.cache.dim = (int32_t)d;
+  for (int64_t i = 1 - f; i < 4; ++i) {  // layer (of five dimensions), page, slot, head
+    s.cache.strides[i] = step_of(keys, i - 1 + f);
+    s.cache.strides[4 + i] = step_of(values, i - 1 + f);
+  }
+  s.step.page_table = static_cast<const int32_t *>(s.table.data_ptr());
+  s.step.lengths = static_cast<const int32_t *>(s.lengths.data_ptr());
+  s.step.cu_tokens = static_cast<const int32_t *>(s.cu.data_ptr());
+  s.step.table_pitch = step_of(s.table, 0);
+  s.step.table_width = (int32_t)s.table.size(1);
+  s.step.batch = (int32_t)lengths.size(0);
+  s.step.T = t;
+  return s;
+}
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Maybe append_kv(const Tensor &keys, const Tensor &values, const Tensor &table, const Tensor &lengths, const Tensor &cu, const Tensor &k,
+                const Tensor &v, const Maybe &q_, const Maybe &positions, const Maybe &turns, bool interleaved, double gain) {
+  const char *who = "append_kv";
+  const Tensor q = q_.value_or(Tensor());
+  require_plain(who, {&k, &v});
+  if (q.defined()) require_plain(who, {&q});
+  require_no_grad(who, {&keys, &values, &k, &v, &q});
+  require_cuda(k);
+  require_cuda(v);
+  TORCH_CHECK_VALUE(k.dim() == 3 && k.sizes() == v.sizes(), who, ": k and v (T, heads, D) are wanted, got ", k.sizes(), ", ", v.sizes());
+  Step s = step_of_cache(who, keys, values, table, lengths, cu, k.size(0), false);
+  TORCH_CHECK_VALUE(k.size(1) == s.cache.kv_heads && k.size(2) == s.cache.dim, who, ": k and v ", k.sizes(), " do not fit the cache ", keys.sizes());
+  TORCH_CHECK_TYPE(k.scalar_type() == keys.scalar_type() && v.scalar_type() == keys.scalar_type(), who, ": k, v and the cache must have one type, got ",
+                   k.scalar_type(), ", ", v.scalar_type(), ", ", keys.scalar_type());
+  TORCH_CHECK_VALUE(k.device() == keys.device() && v.device() == keys.device(), who, ": k, v and the cache must be on one device");
+  TORCH_CHECK_VALUE(turns.has_value() || (!q.defined() && !positions.has_value()), who, ": q and positions are of use with a rotary only");
+  Tensor pos;
+  if (turns.has_value()) {
+    TORCH_CHECK_VALUE(turns->device() == keys.device(), who, ": the frequencies must be on the cache's device");
+    TORCH_CHECK_VALUE(2 * turns->numel() <= s.cache.dim, who, ": heads of ", s.cache.dim, " cannot have ", 2 * turns->numel(), " elements rotated");
+  }
+  if (q.defined()) {
+    require_cuda(q);
+    TORCH_CHECK_TYPE(q.scalar_type() == keys.scalar_type(), who, ": q and the cache must have one type, got ", q.scalar_type(), ", ", keys.scalar_type());
+    TORCH_CHECK_VALUE(q.device() == keys.device() && q.dim() == 3 && q.size(0) == k.size(0) && q.size(1) >= 1 && q.size(2) == k.size(2), who,
+                      ": q (T, heads, D) on the cache's device is wanted, got ", q.sizes(), " for k ", k.sizes());
+  }
+  if (positions.has_value()) {
+    require_cuda(*positions);
+    TORCH_CHECK_TYPE(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong, who, ": positions must be int32 or int64, got ",
+                     positions->scalar_type());
+    TORCH_CHECK_VALUE(positions->device() == keys.device() && positions->dim() == 1 && positions->size(0) == k.size(0), who,
+                      ": a position for every token is wanted, got ", positions->sizes());
+    pos = positions->contiguous();
+  }
+  ready();
+  const c10::cuda::CUDAGuard guard(keys.device());
+  const Tensor k3 = flat_rows(k), v3 = flat_rows(v), q3 = q.defined() ? flat_rows(q) : Tensor();
+  Tensor out = q.defined() ? at::empty(q.sizes(), q.options()) : Tensor();
+  int64_t strides[6] = {0, 0, step_of(k3, 0), step_of(k3, 1), step_of(v3, 0), step_of(v3, 1)};
+  if (q3.defined()) strides[0] = step_of(q3, 0), strides[1] = step_of(q3, 1);
+  mhc_rotary r{};
+  if (turns.has_value())
+    r = mhc_rotary{static_cast<const uint64_t *>(turns->data_ptr()), (int32_t)(2 * turns->numel()), interleaved, (float)gain};
+  written(keys);
+  written(values);
+  check(E.append_kv(&s.cache, &s.step, k3.data_ptr(), v3.data_ptr(), ptr(q3), ptr(out), q3.defined() ? (int)q3.size(1) : 0, strides,
+                    turns.has_value() ? &r : nullptr, ptr(pos), pos.defined() ? (int)pos.element_size() : 0, stream_of(keys)),
+        "mhc_append_kv");
+  return out.defined() ? Maybe(out) : std::nullopt;
+}
+
+Tensor cached_attention(const Tensor &q, const Tensor &keys, const Tensor &values, const Tensor &table, const Tensor &lengths, const Tensor &cu,
+                        const Maybe &mask, std::optional<double> scale_) {
+  const char *who = "cached_attention";
+  require_plain(who, {&q});
+  require_no_grad(who, {&q, &keys, &values});
+  require_cuda(q);
+  TORCH_CHECK_VALUE(q.dim() == 3, who, ": q (T, heads, D) is wanted, got ", q.sizes());
+  Step s = step_of_cache(who, keys, values, table, lengths, cu, q.size(0), false);
+  TORCH_CHECK_TYPE(q.scalar_type() == keys.scalar_type(), who, ": q and the cache must have one type, got ", q.scalar_type(), ", ", keys.scalar_type());
+  TORCH_CHECK_VALUE(q.device() == keys.device(), who, ": q and the cache must be on one device");
+  const int64_t t = q.size(0), h = q.size(1), d = q.size(2);
+  TORCH_CHECK_VALUE(d == s.cache.dim && h >= 1 && h % s.cache.kv_heads == 0, who, ": ", h, " query heads of ", d, " cannot share ", s.cache.kv_heads,
+                    " key heads of ", s.cache.dim);
+  TORCH_CHECK_VALUE(d <= 128, who, ": head sizes up to 128 are supported, got ", d);
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)d);
+  TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale), who, ": scale must be positive and finite, got ", scale);
+  Tensor bits;
+  if (mask.has_value()) {
+    require_index(*mask, who, "mask", at::kLong, keys);
+    TORCH_CHECK_VALUE(mask->dim() == 1 && mask->size(0) == t, who, ": a mask for every token is wanted, got ", mask->sizes());
+    bits = mask->contiguous();
+  }
+  ready();
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor q3 = rows(q), out = at::empty({t, h, d}, q.options());
+  const size_t need = E.cached_attn_workspace(&s.cache, &s.step, (int)h);
+  const Tensor ws = need ? scratch(q, need) : Tensor();
+  const int64_t strides[2] = {step_of(q3, 0), step_of(q3, 1)};
+  check(E.cached_attn(&s.cache, &s.step, ptr(q3), (int)h, strides, static_cast<const int64_t *>(ptr(bits)), (float)scale, out.data_ptr(), ptr(ws),
+                      need, stream_of(q)),
+        "mhc_cached_attn");
+  return out;
+}
+
+void keep_drafts(const Tensor &keys, const Tensor &values, const Tensor &table, const Tensor &lengths, const Tensor &cu, const Tensor &path,
+                 const Tensor &kept) {
+  const char *who = "keep_drafts";
+  require_no_grad(who, {&keys, &values});
+  TORCH_CHECK_VALUE(path.dim() == 1, who, ": path (T,) is wanted, got ", path.sizes());
+  Step s = step_of_cache(who, keys, values, table, lengths, cu, path.size(0), true);
+  require_index(path, who, "path", at::kInt, keys);
+  require_index(kept, who, "kept", at::kInt, keys);
+  TORCH_CHECK_VALUE(kept.sizes() == lengths.sizes(), who, ": a number of kept tokens for every sequence is wanted, got ", kept.sizes());
+  ready();
+  const c10::cuda::CUDAGuard guard(keys.device());
+  const Tensor p = path.contiguous(), n = kept.contiguous();
+  written(keys);
+  written(values);
+  check(E.keep_drafts(&s.cache, &s.step, static_cast<const int32_t *>(ptr(p)), static_cast<const int32_t *>(ptr(n)), stream_of(keys)),
+        "mhc_keep_drafts");
+}
+
+// ---- verification of drafted tokens -------------------------------------------------
+
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor &tokens, const Tensor &parents, const Tensor &cu, const Tensor &target,
+                                                 const Maybe &draft, const Tensor &random) {
+  const char *who = "verify_drafts";
+  require_plain(who, {&target, &random});
+  require_cuda(target);
+  dtype_code(target, who);
+  TORCH_CHECK_VALUE(target.dim() == 2 && target.size(1) >= 1, who, ": target (T, V) is wanted, got ", target.sizes());
+  const int64_t t = target.size(0), v = target.size(1);
+  if (draft.has_value()) {
+    require_plain(who, {&*draft});
+    require_index(*draft, who, "draft", target.scalar_type(), target);
+    TORCH_CHECK_VALUE(draft->sizes() == target.sizes(), who, ": draft ", draft->sizes(), " and target ", target.sizes(), " must have one shape");
+  }
+  require_index(tokens, who, "tokens", at::kLong, target);
+  require_index(parents, who, "parents", at::kInt, target);
+  require_index(cu, who, "cu_tokens", at::kInt, target);
+  require_index(random, who, "random", at::kFloat, target);
+  for (const Tensor *x : {&tokens, &parents, &random})
+    TORCH_CHECK_VALUE(x->dim() == 1 && x->size(0) == t, who, ": tokens, parents and random of ", t, " rows are wanted, got ", x->sizes());
+  TORCH_CHECK_VALUE(cu.dim() == 1 && cu.size(0) >= 1, who, ": cu_tokens (B + 1,) is wanted, got ", cu.sizes());
+  ready();
+  const c10::cuda::CUDAGuard guard(target.device());
+  auto whole = [](const Tensor &x) { return (x.stride(1) == 1 || x.size(1) == 1) && (x.size(0) <= 1 || x.stride(0) >= x.size(1)) ? x : x.contiguous(); };
+  const Tensor p = whole(target), q = draft.has_value() ? whole(*draft) : Tensor();
+  const Tensor tk = tokens.contiguous(), pr = parents.contiguous(), c = cu.contiguous(), u = random.contiguous();
+  const int64_t batch = cu.size(0) - 1;
+  const Tensor path = at::empty({t}, pr.options()), kept = at::empty({batch}, pr.options()), next = at::empty({batch}, tk.options());
+  check(E.verify_drafts(static_cast<const int64_t *>(ptr(tk)), static_cast<const int32_t *>(ptr(pr)), static_cast<const int32_t *>(ptr(c)), (int)batch,
+                        t, ptr(p), t > 1 ? p.stride(0) : v, ptr(q), q.defined() && t > 1 ? q.stride(0) : v, dtype_code(target, who), v,
+                        static_cast<const float *>(ptr(u)), static_cast<int32_t *>(ptr(path)), static_cast<int32_t *>(ptr(kept)),
+                        static_cast<int64_t *>(ptr(next)), stream_of(target)),
+        "mhc_verify_drafts");
+  return {path, kept, next};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -407,4 +724,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("packed_attention", &packed_attention);
   m.def("route_topk", &route_topk);
   m.def("adamw", &adamw);
+  m.def("rotate", &rotate);
+  m.def("append_kv", &append_kv);
+  m.def("cached_attention", &cached_attention);
+  m.def("keep_drafts", &keep_drafts);
+  m.def("verify_drafts", &verify_drafts);
 }

@@ -1,0 +1,65 @@
+// Shared by the kernels over a paged cache: where a sequence's tokens lie, and how the
+// work of attention over caches of any lengths is cut into equal pieces on the device.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "mhc_b200.h"
+
+namespace mhc {
+namespace cache {
+
+// What the kernels need of a cache and a step (the C structs, checked and flattened).
+struct View {
+  void *keys, *values;
+  int64_t kp, ks, kh, vp, vs, vh;  // page, slot and head strides in elements
+  const int32_t *table, *lengths, *cu;
+  int64_t pitch;
+  int pages, size, shift;  // shift: log2(size), or -1 where size is no power of two
+  int capacity;            // table_width * page_size
+  int batch, T, Hk, D;
+};
+
+// New tokens [start, start + n) of sequence b, `len` tokens before them.  Within the
+// step's rows whatever the offsets hold.
+struct Seq {
+  int start, n, len;
+};
+__device__ __forceinline__ Seq seq_of(const View &v, int b) {
+  Seq s;
+  const int lo = min(max(v.cu[b], 0), v.T), hi = min(max(v.cu[b + 1], 0), v.T);
+  s.start = lo;
+  s.n = max(hi - lo, 0);
+  s.len = v.lengths[b];
+  return s;
+}
+
+// the sequence of row t, or -1: cu[b] <= t < cu[b + 1]
+__device__ __forceinline__ int seq_at(const View &v, int t) {
+  if (t < v.cu[0] || t >= v.cu[v.batch]) return -1;
+  int lo = 0, hi = v.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v.cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int page_index(const View &v, int place) { return v.shift >= 0 ? place >> v.shift : place / v.size; }
+
+// page and slot of a sequence's place; false where there is none
+__device__ __forceinline__ bool locate(const View &v, int b, int64_t place, int &page, int &slot) {
+  if (place < 0 || place >= v.capacity) return false;
+  const int i = page_index(v, (int)place);
+  page = v.table[b * v.pitch + i];
+  slot = (int)place - i * v.size;
+  return page >= 0 && page < v.pages;
+}
+
+}  // namespace cache
+
+// Checks the structs and fills the view; MHC_OK or a status with its message set.
+int cache_view(const char *who, const mhc_kv_cache *c, const mhc_cache_step *s, cache::View &v);
+
+}  // namespace mhc

@@ -1,0 +1,868 @@
+// Attention of new tokens over a paged cache (single tokens, trees of drafted tokens,
+// pieces of prompts).
+//
+//   s_j = scale q . k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)     over the keys that a row sees
+//
+// Few rows share a long row of keys: the bound is reading keys and values once.  All
+// query heads of a key head and all new tokens of a sequence are rows of one item (see
+// the header for the cut), so a key is read once for up to 16 or 32 rows.
+//
+// A warp works alone: of every tile of 64 keys it takes 16, brings their K and V rows into
+// a ring of its own with cp.async, three to eight chunks ahead, forms the scores, keeps its
+// own running reference and sums, and adds up O in registers.  No barrier stands between
+// the warps until an item ends; then their four sums are joined through shared memory.
+// Page numbers are fetched one chunk ahead of the rows that they lead to.
+//
+// 16-bit types: mma.sync m16n8k16, S = Q K^T with Q in registers, O += P V with P from the
+// scores' registers.  The matrix unit is not what bounds these few rows (16 rows of 128 need
+// 104 TFLOP/s at the copy rate); the rows are few for the 128 of tcgen05.mma.
+// fp32 and what 16-byte copies cannot fetch (odd head sizes, strides, alignment): CUDA cores,
+// the same structure on fp32 copies of the rows, two lanes to a key.
+//
+// The reference m of a row is moved (and O and the sum rescaled) only when a score passes it
+// by 2^8 (fp16: 2^4, and P is held times 2^10, so that what is 2^-34 of the largest still
+// counts).  P is rounded to 16 bits for the second product; its sum is of the unrounded ones.
+//
+// What a row does not see: its scores are set aside before the maximum and its P is 0.  In
+// the second product 0 would meet a NaN or an infinity of V there, so a chunk in which rows
+// differ in what they see is searched for them, and with one the products are formed one by
+// one.  Keys that do not exist (behind the last, on a page that is none) are not read: zeros.
+// m starts at -inf, "nothing seen yet"; what is seen holds it at the lowest finite number
+// at least, so that a row that sees only scores of -inf gives NaN, as the formula does, and
+// a row that sees nothing 0.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cfloat>
+
+#include "mhc_b200.h"
+#include "mhc_cached_attn.cuh"
+#include "mhc_device.cuh"
+#include "mhc_dispatch.cuh"
+#include "mhc_kernels.h"
+#include "mhc_sm100.cuh"
+
+namespace mhc {
+namespace cattn {
+
+constexpr int WARPS = 4;
+constexpr int THREADS = 32 * WARPS;
+constexpr int CHUNK = 16;           // keys that a warp takes at a time
+constexpr int KT = CHUNK * WARPS;   // keys of a tile
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
+  const int bytes = there ? 16 : 0;  // the rest is filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// What a sum with reference m is multiplied by to have reference top.
+__device__ __forceinline__ float factor(float m, float top, float c2) { return m == -INFINITY ? 0.f : ex2((m - top) * c2); }
+
+// ---- which row of the item is which query -----------------------------------------
+
+struct Row {
+  int j;           // token of the sequence; -1 past the item's rows
+  int64_t q, out;  // offsets of its elements
+  uint64_t bits;
+};
+__device__ __forceinline__ Row row_of(const Args &a, const Segment &g, int r) {
+  Row x{-1, 0, 0, 0};
+  if (r < g.rows) {
+    const int at = g.row0 + r;
+    x.j = at / a.G;
+    const int h = g.hk * a.G + (at - x.j * a.G);
+    const int64_t t = g.s.start + x.j;
+    x.q = t * a.qt + h * a.qh;
+    x.out = (t * a.H + h) * a.c.D;
+    if (a.mask) x.bits = (uint64_t)a.mask[t];
+  }
+  return x;
+}
+
+// ---- fetching chunks -----------------------------------------------------------------
+
+// One lane's key of a chunk: its page number is asked for one chunk ahead.
+struct Places {
+  int page;  // of the chunk that is fetched next; -1: none
+  __device__ __forceinline__ void ask(const Args &a, const Segment &g, int key) {
+    page = key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
+  }
+};
+
+// ---- joining the warps of a block and the blocks of an item ----------------------------
+
+// Every warp has left its (M, DP) sums at `o` (rows of `pitch` floats, `apart` floats between
+// warps) and reference and sum at ml (WARPS, M).
+template <typename T, int M, int DP>
+__device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int slot, const float *o, int pitch, int apart,
+                                           float2 (*ml)[M], float (*fac)[M], bool vec) {
+  for (int r = threadIdx.x; r < g.rows; r += THREADS) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w][r].x);
+    float sum = 0.f, f[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      f[w] = factor(ml[w][r].x, top, a.c2);
+      sum = fmaf(f[w], ml[w][r].y, sum);
+    }
+    float scale = 1.f;
+    if (slot < 0) scale = top == -INFINITY ? 0.f : 1.f / sum;
+    else a.part_ml[(int64_t)slot * M + r] = make_float2(top, sum);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) fac[w][r] = f[w] * scale;
+  }
+  __syncthreads();
+  constexpr int V = 4;
+  for (int i = threadIdx.x; i < g.rows * (DP / V); i += THREADS) {
+    const int r = i / (DP / V), col = (i - r * (DP / V)) * V;
+    if (col >= a.c.D) continue;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = fac[w][r];
+      const float4 y = *reinterpret_cast<const float4 *>(o + (int64_t)w * apart + r * pitch + col);
+      x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+    }
+    if (slot >= 0) {
+      *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * M + r) * DP + col) = x;
+      continue;
+    }
+    T *out = static_cast<T *>(a.out) + row_of(a, g, r).out + col;
+    const float y[4] = {x.x, x.y, x.z, x.w};
+    if (vec) {
+      struct alignas(4 * sizeof(T)) { T e[4]; } p;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p.e[k] = from_f<T>(y[k]);
+      *reinterpret_cast<decltype(p) *>(out) = p;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col + k < a.c.D) out[k] = from_f<T>(y[k]);
+    }
+  }
+}
+
+// Joins the blocks that had part of a cut item.  A warp takes every JW-th block's part of one row, JW warps a row.
+constexpr int JOIN_ROWS = 2, JW = 4;
+template <typename T, int M, int DP>
+__global__ void __launch_bounds__(32 * JW * JOIN_ROWS) join_kernel(const Args a) {
+  wait_for_primary();
+  const int c = blockIdx.x;
+  const int4 d0 = a.desc[2 * c];
+  const int count = d0.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = blockIdx.y * JOIN_ROWS;
+  if (count == 0 || r0 >= d0.w) return;
+  const int which = warp / JW, part = warp % JW, r = r0 + which;
+  const bool live = r < d0.w;
+  __shared__ float st_m[JOIN_ROWS][JW], st_l[JOIN_ROWS][JW];
+  __shared__ float st_o[JOIN_ROWS][JW][DP];
+  constexpr int PER = DP / 32;
+  float o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) o[k] = 0.f;
+  // part i of the item: its first block's last slot, then the first slots of the blocks behind it
+  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i); };
+  if (live) {
+    constexpr int AT_ONCE = 4;
+    for (int i0 = part; i0 < count; i0 += JW * AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float x[AT_ONCE][PER];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * JW;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (i < count) {
+          ml[u] = a.part_ml[slot(i) * M + r];
+#pragma unroll
+          for (int k = 0; k < PER; ++k) x[u][k] = a.part_o[(slot(i) * M + r) * DP + lane + 32 * k];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        if (ml[u].x == -INFINITY) continue;  // nothing was seen there (or there is no such part)
+        const float top = fmaxf(m, ml[u].x), f = factor(m, top, a.c2), g = factor(ml[u].x, top, a.c2);
+        m = top;
+        l = fmaf(l, f, ml[u].y * g);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o[k] = fmaf(o[k], f, x[u][k] * g);
+      }
+    }
+  }
+  if (lane == 0) {
+    st_m[which][part] = m;
+    st_l[which][part] = l;
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) st_o[which][part][lane + 32 * k] = o[k];
+  __syncthreads();
+  if (!live || part != 0) return;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < JW; ++p) top = fmaxf(top, st_m[which][p]);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) o[k] = 0.f;
+#pragma unroll
+  for (int p = 0; p < JW; ++p) {
+    const float f = factor(st_m[which][p], top, a.c2);
+    sum = fmaf(f, st_l[which][p], sum);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = fmaf(f, st_o[which][p][lane + 32 * k], o[k]);
+  }
+  const float scale = top == -INFINITY ? 0.f : 1.f / sum;
+  const int at = d0.z + r, j = at / a.G, hk = a.desc[2 * c + 1].x;
+  T *out = static_cast<T *>(a.out) + ((int64_t)(d0.y + j) * a.H + hk * a.G + (at - j * a.G)) * a.c.D;
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+    if (lane + 32 * k < a.c.D) out[lane + 32 * k] = from_f<T>(top == -INFINITY ? 0.f : o[k] * scale);
+}
+
+// ---- 16-bit types ------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+// infinities and NaN among the two values of a word
+template <typename T>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  constexpr uint32_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return (w & E) == E || ((w >> 16) & E) == E;
+}
+
+template <int DP>
+struct MmaShape {
+  static constexpr int PITCH = DP * 2 + 16;  // bytes of a row: eight of them begin in different banks
+  static constexpr int STAGE = 2 * CHUNK * PITCH;
+  static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 4 : DP >= 64 ? 6 : 8;
+  static constexpr int RING = STAGES * STAGE;  // of a warp
+  static constexpr int SMEM = WARPS * RING;
+  static constexpr int OP = DP + 8;  // floats of a row of O while the warps are joined
+};
+
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(THREADS, 2) mma_kernel(const Args a) {
+  using S = MmaShape<DP>;
+  constexpr int M = 16 * MT, KS = DP / 16, NT = DP / 8;
+  constexpr int VPR = DP / 8, IT = CHUNK * VPR / 32;  // 16-byte vectors of a row; copies of a lane for 16 rows
+  constexpr float AHEAD = std::is_same<T, __half>::value ? 4.f : 8.f, LIFT = std::is_same<T, __half>::value ? 10.f : 0.f;
+  static_assert(M * S::OP * 4 <= S::RING, "O of a warp fits its ring");
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
+  __shared__ uint32_t have[WARPS][S::STAGES];  // which keys of a chunk exist
+  __shared__ float2 ml[WARPS][M];
+  __shared__ float fac[WARPS][M];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = sm100::smem_u32(smem) + warp * S::RING;
+  const int D = a.c.D, vpr = D / 8;
+  const float ahead = AHEAD / a.c2;
+  for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  clear_rest<T>(a);
+  __syncthreads();
+
+  walk<M, KT>(a, [&](const Segment &g, int slot) {
+    Row row[MT][2];
+    uint32_t q[MT][KS][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) row[t][h] = row_of(a, g, 16 * t + 8 * h + lane / 4);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Row &x = row[t][i & 1];
+          const int col = 16 * k + 8 * (i >> 1) + 2 * (lane & 3);
+          q[t][k][i] = x.j >= 0 && col < D ? *reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.q) + x.q + col) : 0u;
+        }
+    }
+    const T *kbase = static_cast<const T *>(a.c.keys) + g.hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + g.hk * a.c.vh;
+    const int chunks = g.k1 - g.k0;
+    const int key0 = g.k0 * KT + warp * CHUNK;  // of chunk i: key0 + i * KT
+    Places places;
+    places.ask(a, g, key0 + (lane & 15));
+    auto fetch = [&](int i) {
+      if (i < chunks) {
+        const int key = key0 + i * KT + (lane & 15), st = i % S::STAGES;
+        const bool there = places.page >= 0 && places.page < a.c.pages;
+        const uint32_t got = __ballot_sync(0xffffffffu, there) & 0xffffu;
+        if (lane < CHUNK) {
+          const int slot_at = key - cache::page_index(a.c, key) * a.c.size;
+          off_k[warp][lane] = there ? places.page * a.c.kp + slot_at * a.c.ks : -1;
+          off_v[warp][lane] = there ? places.page * a.c.vp + slot_at * a.c.vs : -1;
+        }
+        if (lane == 0) have[warp][st] = got;
+        places.ask(a, g, key + KT);
+        __syncwarp();
+        const uint32_t dst = ring + st * S::STAGE;
+#pragma unroll
+        for (int u = 0; u < IT; ++u) {
+          const int at = u * 32 + lane, r = at / VPR, x = at - r * VPR;
+          if (x < vpr) {
+            const int64_t ok = off_k[warp][r], ov = off_v[warp][r];
+            cp16(dst + r * S::PITCH + x * 16, kbase + (ok >= 0 ? ok + x * 8 : 0), ok >= 0);
+            cp16(dst + (CHUNK + r) * S::PITCH + x * 16, vbase + (ov >= 0 ? ov + x * 8 : 0), ov >= 0);
+          }
+        }
+        __syncwarp();  // the offsets have been read
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+
+    float o[MT][NT][4], m[MT][2], l[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][n][i] = 0.f;
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+    }
+    for (int i = 0; i < chunks; ++i) {
+      cp_wait<S::STAGES - 2>();
+      __syncwarp();
+      const int st = i % S::STAGES, key = key0 + i * KT;
+      const uint32_t kt = ring + st * S::STAGE, vt = kt + CHUNK * S::PITCH;
+      const uint32_t got = have[warp][st];
+      if (got) {
+        float s[MT][2][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][n][e] = 0.f;
+        const uint32_t ka = kt + ((lane & 7) + ((lane >> 4) & 1) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t b[4];
+          ldsm4(b, ka + k * 32);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma16816<T>(s[t][0], q[t][k], b[0], b[1]);
+            mma16816<T>(s[t][1], q[t][k], b[2], b[3]);
+          }
+        }
+        // rows differ in what they see only from the first new token on, or where keys are missing
+        const bool uneven = got != 0xffffu || key + CHUNK > g.s.len;
+        uint32_t seen[MT][2];  // bit n * 2 + e: keys 8 n + 2 (lane % 4) + e
+        bool move = false;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = -FLT_MAX;
+            if (uneven) {
+              uint32_t v = 0;
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int at = 8 * n + 2 * (lane & 3) + e;
+                  const bool ok = ((got >> at) & 1) && row[t][h].j >= 0 &&
+                                  sees(a.mask != nullptr, row[t][h].bits, row[t][h].j, key + at - g.s.len);
+                  v |= (uint32_t)ok << (2 * n + e);
+                  if (ok) top = fmaxf(top, s[t][n][2 * h + e]);
+                }
+              seen[t][h] = v;
+              if (!v) top = -INFINITY;
+            } else {
+              seen[t][h] = 0xfu;
+#pragma unroll
+              for (int n = 0; n < 2; ++n) top = fmaxf(top, fmaxf(s[t][n][2 * h], s[t][n][2 * h + 1]));
+            }
+            move = move || top > m[t][h] + ahead;
+          }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float top = seen[t][h] ? -FLT_MAX : -INFINITY;
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if ((seen[t][h] >> (2 * n + e)) & 1) top = fmaxf(top, s[t][n][2 * h + e]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              top = fmaxf(top, m[t][h]);
+              const float f = m[t][h] == top ? 1.f : factor(m[t][h], top, a.c2);
+              m[t][h] = top;
+              l[t][h] *= f;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                o[t][n][2 * h] *= f;
+                o[t][n][2 * h + 1] *= f;
+              }
+            }
+        }
+        uint32_t p[MT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x = ex2(fmaf(s[t][n][2 * h] - m[t][h], a.c2, LIFT)), y = ex2(fmaf(s[t][n][2 * h + 1] - m[t][h], a.c2, LIFT));
+              if (uneven) {
+                if (!((seen[t][h] >> (2 * n)) & 1)) x = 0.f;
+                if (!((seen[t][h] >> (2 * n + 1)) & 1)) y = 0.f;
+              }
+              l[t][h] += x + y;
+              p[t][2 * n + h] = pack2<T>(x, y);
+            }
+        const uint32_t va = vt + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + ((lane >> 4) & 1) * 16;
+        bool odd = false;
+        if (uneven) {
+          for (int at = lane; at < CHUNK * (DP / 2); at += 32) {
+            const int r = at / (DP / 2), x = at - r * (DP / 2);
+            uint32_t w;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vt + r * S::PITCH + x * 4));
+            odd = odd || odd_pair<T>(w);
+          }
+          odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+          for (int n = 0; n < NT / 2; ++n) {
+            uint32_t b[4];
+            ldsm4t(b, va + n * 32);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              mma16816<T>(o[t][2 * n], p[t], b[0], b[1]);
+              mma16816<T>(o[t][2 * n + 1], p[t], b[2], b[3]);
+            }
+          }
+        } else {
+          // key by key: P of the row's four lanes that hold it, V of this lane's columns
+#pragma unroll 1
+          for (int at = 0; at < CHUNK; ++at) {
+            const int from = (lane & ~3) | ((at & 7) >> 1);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w = __shfl_sync(0xffffffffu, at < 8 ? p[t][h] : p[t][2 + h], from);
+                const uint32_t sees_it = __shfl_sync(0xffffffffu, seen[t][h], from) >> ((at < 8 ? 0 : 2) + (at & 1)) & 1;
+                const uint16_t half_word = (uint16_t)((at & 1) ? w >> 16 : w);
+                const float x = to_f(*reinterpret_cast<const T *>(&half_word));
+                if (sees_it) {
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    uint32_t v;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(vt + at * S::PITCH + (n * 8 + 2 * (lane & 3)) * 2));
+                    const uint16_t v0 = (uint16_t)v, v1 = (uint16_t)(v >> 16);
+                    o[t][n][2 * h] = fmaf(x, to_f(*reinterpret_cast<const T *>(&v0)), o[t][n][2 * h]);
+                    o[t][n][2 * h + 1] = fmaf(x, to_f(*reinterpret_cast<const T *>(&v1)), o[t][n][2 * h + 1]);
+                  }
+                }
+              }
+          }
+        }
+      }
+      __syncwarp();  // the chunk has been read
+      fetch(i + S::STAGES - 1);
+    }
+    cp_wait<0>();
+    __syncwarp();
+    float *mine = reinterpret_cast<float *>(smem + warp * S::RING);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
+        l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
+        const int r = 16 * t + 8 * h + lane / 4;
+        if ((lane & 3) == 0) ml[warp][r] = make_float2(m[t][h], l[t][h]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<float2 *>(mine + r * S::OP + n * 8 + 2 * (lane & 3)) = make_float2(o[t][n][2 * h], o[t][n][2 * h + 1]);
+      }
+    __syncthreads();
+    join_warps<T, M, DP>(a, g, slot, reinterpret_cast<const float *>(smem), S::OP, S::RING / 4, ml, fac, true);
+    __syncthreads();
+    if (D < DP)  // columns past D are zeros again
+      for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  });
+  launch_dependents();
+}
+
+// ---- CUDA cores ---------------------------------------------------------------------------
+
+template <int DP>
+struct CoreShape {
+  static constexpr int KP = DP + 8, VP = DP + 4;  // floats of a row of K (two lanes to a key: no conflicts) and of V
+  static constexpr int STAGE = CHUNK * (KP + VP);
+  static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 4 : DP >= 64 ? 5 : 6;
+  static constexpr int RING = STAGES * STAGE;  // floats of a warp
+  static constexpr int OP = DP + 4;
+};
+template <int DP, int R>
+constexpr int core_smem() {
+  return 4 * (WARPS * CoreShape<DP>::RING + R * DP + WARPS * CHUNK * R);
+}
+
+// ASYNC: fp32 rows that begin at multiples of 16 bytes, copied ahead; else element by element
+template <typename T, int DP, int R, bool ASYNC>
+__global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
+  using S = CoreShape<DP>;
+  constexpr int SPLIT = DP <= 32 ? 4 : DP <= 64 ? 2 : 1;  // lanes that share four columns of O, each with every SPLIT-th key
+  static_assert(R * S::OP <= S::RING, "O of a warp fits its ring");
+  extern __shared__ __align__(128) float fsm[];
+  float *ring = fsm + (threadIdx.x >> 5) * S::RING;
+  float *qs = fsm + WARPS * S::RING;                      // (R, DP)
+  float *ps = qs + R * DP + (threadIdx.x >> 5) * CHUNK * R;  // (CHUNK, R); below 0: not seen
+  __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
+  __shared__ uint32_t have[WARPS][S::STAGES];
+  __shared__ Row rows[R];
+  __shared__ float2 ml[WARPS][R];
+  __shared__ float fac[WARPS][R];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.D;
+  const float ahead = 8.f / a.c2;
+  for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
+  clear_rest<T>(a);
+  __syncthreads();
+
+  walk<R, KT>(a, [&](const Segment &g, int slot) {
+    for (int r = tid; r < R; r += THREADS) rows[r] = row_of(a, g, r);
+    __syncthreads();
+    for (int i = tid; i < R * DP; i += THREADS) {
+      const int r = i / DP, x = i - r * DP;
+      qs[i] = rows[r].j >= 0 && x < D ? to_f(static_cast<const T *>(a.q)[rows[r].q + x]) : 0.f;
+    }
+    const T *kbase = static_cast<const T *>(a.c.keys) + g.hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + g.hk * a.c.vh;
+    const int chunks = g.k1 - g.k0, key0 = g.k0 * KT + warp * CHUNK;
+    Places places;
+    places.ask(a, g, key0 + (lane & 15));
+    auto fetch = [&](int i) {
+      if (i < chunks) {
+        const int key = key0 + i * KT + (lane & 15), st = i % S::STAGES;
+        const bool there = places.page >= 0 && places.page < a.c.pages;
+        const uint32_t got = __ballot_sync(0xffffffffu, there) & 0xffffu;
+        if (lane < CHUNK) {
+          const int slot_at = key - cache::page_index(a.c, key) * a.c.size;
+          off_k[warp][lane] = there ? places.page * a.c.kp + slot_at * a.c.ks : -1;
+          off_v[warp][lane] = there ? places.page * a.c.vp + slot_at * a.c.vs : -1;
+        }
+        if (lane == 0) have[warp][st] = got;
+        places.ask(a, g, key + KT);
+        __syncwarp();
+        float *kt = ring + st * S::STAGE, *vt = kt + CHUNK * S::KP;
+        if constexpr (ASYNC) {
+          for (int at = lane; at < CHUNK * (DP / 4); at += 32) {
+            const int r = at / (DP / 4), x = (at - r * (DP / 4)) * 4;
+            if (x < D) {
+              const int64_t ok = off_k[warp][r], ov = off_v[warp][r];
+              cp16(sm100::smem_u32(kt + r * S::KP + x), kbase + (ok >= 0 ? ok + x : 0), ok >= 0);
+              cp16(sm100::smem_u32(vt + r * S::VP + x), vbase + (ov >= 0 ? ov + x : 0), ov >= 0);
+            }
+          }
+        } else {
+          for (int r = 0; r < CHUNK; ++r) {
+            const int64_t ok = off_k[warp][r], ov = off_v[warp][r];
+            for (int x = lane; x < D; x += 32) {
+              kt[r * S::KP + x] = ok >= 0 ? to_f(kbase[ok + x]) : 0.f;
+              vt[r * S::VP + x] = ov >= 0 ? to_f(vbase[ov + x]) : 0.f;
+            }
+          }
+        }
+        __syncwarp();  // the offsets have been read
+      }
+      cp_commit();
+    };
+    for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+    __syncthreads();  // qs
+    float o[R][4], m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      o[r][0] = o[r][1] = o[r][2] = o[r][3] = 0.f;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
+    const int mykey = lane >> 1, part = lane & 1;
+    const int col = SPLIT == 1 ? lane * 4 : (lane % (32 / SPLIT)) * 4, share = SPLIT == 1 ? 0 : lane / (32 / SPLIT);
+    for (int i = 0; i < chunks; ++i) {
+      cp_wait<S::STAGES - 2>();
+      __syncwarp();
+      const int st = i % S::STAGES, key = key0 + i * KT;
+      const float *kt = ring + st * S::STAGE, *vt = kt + CHUNK * S::KP;
+      const uint32_t got = have[warp][st];
+      if (got) {
+        float s[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = 0.f;
+#pragma unroll 4
+        for (int x = 0; x < DP / 8; ++x) {
+          const float4 k = *reinterpret_cast<const float4 *>(kt + mykey * S::KP + (2 * x + part) * 4);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float4 q = *reinterpret_cast<const float4 *>(qs + r * DP + (2 * x + part) * 4);
+            s[r] = fmaf(q.x, k.x, s[r]);
+            s[r] = fmaf(q.y, k.y, s[r]);
+            s[r] = fmaf(q.z, k.z, s[r]);
+            s[r] = fmaf(q.w, k.w, s[r]);
+          }
+        }
+        const bool uneven = got != 0xffffu || key + CHUNK > g.s.len;
+        uint32_t seen = 0;
+        bool move = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+          bool ok = true;
+          if (uneven)
+            ok = ((got >> mykey) & 1) && rows[r].j >= 0 && sees(a.mask != nullptr, rows[r].bits, rows[r].j, key + mykey - g.s.len);
+          seen |= (uint32_t)ok << r;
+          move = move || (ok && fmaxf(s[r], -FLT_MAX) > m[r] + ahead);
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float top = (seen >> r) & 1 ? fmaxf(s[r], -FLT_MAX) : -INFINITY;
+#pragma unroll
+            for (int w = 2; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            top = fmaxf(top, m[r]);
+            const float f = m[r] == top ? 1.f : factor(m[r], top, a.c2);
+            m[r] = top;
+            l[r] *= f;
+            o[r][0] *= f, o[r][1] *= f, o[r][2] *= f, o[r][3] *= f;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool ok = (seen >> r) & 1;
+          const float p = ok ? ex2((s[r] - m[r]) * a.c2) : -1.f;
+          if (part == 0) {
+            if (ok) l[r] += p;
+            ps[mykey * R + r] = p;
+          }
+        }
+        __syncwarp();
+        if (col < DP) {
+#pragma unroll 4
+          for (int at = share; at < CHUNK; at += SPLIT) {
+            const float4 v = *reinterpret_cast<const float4 *>(vt + at * S::VP + col);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const float p = ps[at * R + r];
+              if (uneven && p < 0.f) continue;
+              o[r][0] = fmaf(p, v.x, o[r][0]);
+              o[r][1] = fmaf(p, v.y, o[r][1]);
+              o[r][2] = fmaf(p, v.z, o[r][2]);
+              o[r][3] = fmaf(p, v.w, o[r][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // the chunk and P have been read
+      fetch(i + S::STAGES - 1);
+    }
+    cp_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int w = 2; w < 32; w <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+      if (lane == 0) ml[warp][r] = make_float2(m[r], l[r]);
+#pragma unroll
+      for (int w = 32 / SPLIT; w < 32; w <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[r][k] += __shfl_xor_sync(0xffffffffu, o[r][k], w);
+      if (share == 0 && col < DP) *reinterpret_cast<float4 *>(ring + r * S::OP + col) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+    }
+    __syncthreads();
+    join_warps<T, R, DP>(a, g, slot, fsm, S::OP, S::RING, ml, fac, a.c.D % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0);
+    __syncthreads();
+    if (D < DP)  // columns past D are zeros again
+      for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
+    __syncthreads();
+  });
+  launch_dependents();
+}
+
+// ---- choice and launch ---------------------------------------------------------------------
+
+// Which kernel, for how many rows, on how many blocks.  The lengths of the sequences' new tokens are on the device; on
+// average there are T / batch of them.
+struct Choice {
+  bool mma;
+  int m, dp, pieces;
+  size_t desc, ml, o, total;  // bytes of the workspace
+};
+static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, bool aligned) {
+  Choice x{};
+  const int G = H / c->kv_heads, sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  const int64_t rows = (s->T + s->batch - 1) / s->batch * G;
+  x.mma = aligned;
+  x.dp = (c->dim + 31) / 32 * 32;
+  x.m = x.mma ? (rows <= 16 ? 16 : 32) : (rows <= 4 ? 4 : 16);
+  x.pieces = sms * (x.mma ? 2 : 1);
+  auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+  x.desc = up((size_t)x.pieces * 2 * sizeof(int4));
+  x.ml = up((size_t)x.pieces * 2 * x.m * sizeof(float2));
+  x.o = up((size_t)x.pieces * 2 * x.m * x.dp * sizeof(float));
+  x.total = x.desc + x.ml + x.o;
+  return x;
+}
+
+template <typename K>
+static cudaError_t start(K kernel, const Args &a, int blocks, int smem, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<blocks, THREADS, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+// the join begins while the last blocks of the first kernel still run, and waits for them on the device
+template <typename T, int M, int DP>
+static cudaError_t join(const Args &a, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.pieces, (M + JOIN_ROWS - 1) / JOIN_ROWS);
+  cfg.blockDim = dim3(32 * JW * JOIN_ROWS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<T, M, DP>, a);
+}
+
+template <typename F>
+static cudaError_t with_dp(int dp, F &&f) {
+  switch (dp) {
+    case 32: return f(IC<32>{});
+    case 64: return f(IC<64>{});
+    case 96: return f(IC<96>{});
+    default: return f(IC<128>{});
+  }
+}
+
+static cudaError_t launch(const Args &a, const Choice &x, bool async, cudaStream_t st) {
+  return with_dp(x.dp, [&](auto dp) -> cudaError_t {
+    constexpr int DP = decltype(dp)::value;
+    if (x.mma) {
+      auto go = [&](auto tag, auto mt) -> cudaError_t {
+        using T = decltype(tag);
+        constexpr int MT = decltype(mt)::value;
+        cudaError_t e = start(mma_kernel<T, DP, MT>, a, x.pieces, MmaShape<DP>::SMEM, st);
+        return e != cudaSuccess ? e : join<T, 16 * MT, DP>(a, st);
+      };
+      if (a.dtype == MHC_BF16) return x.m == 16 ? go(__nv_bfloat16{}, IC<1>{}) : go(__nv_bfloat16{}, IC<2>{});
+      return x.m == 16 ? go(__half{}, IC<1>{}) : go(__half{}, IC<2>{});
+    }
+    return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
+      using T = decltype(tag);
+      auto go = [&](auto r) -> cudaError_t {
+        constexpr int R = decltype(r)::value;
+        cudaError_t e;
+        if constexpr (std::is_same<T, float>::value)
+          e = async ? start(core_kernel<T, DP, R, true>, a, x.pieces, core_smem<DP, R>(), st)
+                    : start(core_kernel<T, DP, R, false>, a, x.pieces, core_smem<DP, R>(), st);
+        else
+          e = start(core_kernel<T, DP, R, false>, a, x.pieces, core_smem<DP, R>(), st);
+        return e != cudaSuccess ? e : join<T, R, DP>(a, st);
+      };
+      return x.m == 4 ? go(IC<4>{}) : go(IC<16>{});
+    });
+  });
+}
+
+// rows of the cache (and, for the tensor cores, of q) that 16-byte copies can fetch
+static bool rows_aligned(const mhc_kv_cache *c) {
+  const int es = c->dtype == MHC_F32 ? 4 : 2;
+  bool ok = (c->dim * es) % 16 == 0 && (uintptr_t)c->keys % 16 == 0 && (uintptr_t)c->values % 16 == 0;
+  for (int i : {1, 2, 3, 5, 6, 7}) ok = ok && (c->strides[i] * es) % 16 == 0;
+  return ok;
+}
+
+}  // namespace cattn
+}  // namespace mhc
+
+using namespace mhc;
+
+extern "C" {
+
+size_t mhc_cached_attn_workspace(const mhc_kv_cache *cache, const mhc_cache_step *step, int H) {
+  if (!cache || !step || step->batch < 1 || cache->kv_heads < 1 || H < 1 || H % cache->kv_heads || cache->dim < 1 || cache->dim > 128) return 0;
+  // for either kernel: which one runs depends on the pointers
+  const size_t a = cattn::choose(cache, step, H, true).total, b = cattn::choose(cache, step, H, false).total;
+  return a > b ? a : b;
+}
+
+int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const void *q, int H, const int64_t *q_strides,
+                    const int64_t *mask, float scale, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *who = "mhc_cached_attn";
+  clear_error();
+  cattn::Args a{};
+  if (int st = cache_view(who, cache, step, a.c)) return st;
+  if (cache->dim > 128) return fail(MHC_ERR_SHAPE, "%s: head sizes up to 128 are supported (got %d)", who, cache->dim);
+  if (H < 1 || H % cache->kv_heads) return fail(MHC_ERR_SHAPE, "%s: %d query heads cannot share %d key heads", who, H, cache->kv_heads);
+  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(MHC_ERR_SHAPE, "%s: scale must be positive and finite (got %g)", who, scale);
+  if (step->T == 0) return MHC_OK;
+  if (!q || !out || !q_strides) return fail(MHC_ERR_NULL, "%s: required pointer is NULL", who);
+  const size_t es = cache->dtype == MHC_F32 ? 4 : 2;
+  if ((uintptr_t)q % es || (uintptr_t)out % es || (uintptr_t)mask % 8) return fail(MHC_ERR_ALIGN, "%s: a pointer is not aligned to its elements", who);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (step->batch == 0 || cache->pages == 0)  // nothing is seen
+    return cuda_status(cudaMemsetAsync(out, 0, (size_t)step->T * H * cache->dim * es, st), who);
+  const size_t need = mhc_cached_attn_workspace(cache, step, H);
+  if (!workspace || workspace_bytes < need) return fail(MHC_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
+  if ((uintptr_t)workspace % 256) return fail(MHC_ERR_ALIGN, "%s: workspace must be 256-byte aligned", who);
+  const bool async = cattn::rows_aligned(cache);
+  const bool mma = async && cache->dtype != MHC_F32 && (uintptr_t)q % 16 == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
+                   (uintptr_t)out % 8 == 0 && !generic_forced();
+  const cattn::Choice x = cattn::choose(cache, step, H, mma);
+  a.q = q, a.out = out, a.qt = q_strides[0], a.qh = q_strides[1];
+  a.mask = mask, a.H = H, a.G = H / cache->kv_heads;
+  a.c2 = (float)((double)scale * 1.4426950408889634);
+  a.pieces = x.pieces, a.dtype = cache->dtype;
+  char *ws = static_cast<char *>(workspace);
+  a.desc = reinterpret_cast<int4 *>(ws);
+  a.part_ml = reinterpret_cast<float2 *>(ws + x.desc);
+  a.part_o = reinterpret_cast<float *>(ws + x.desc + x.ml);
+  return cuda_status(cattn::launch(a, x, async, st), who);
+}
+
+}  // extern "C"

@@ -1,0 +1,151 @@
+// Attention over a paged cache: arguments, and the cut of the work into equal pieces.
+//
+// The unit of work is a tile of KT keys for up to M rows (new tokens x heads of a group) of
+// one sequence and key head, the item.  The lengths are known on the device only, so
+// every block sums the units of all sequences itself (a few loads and one warp's scan) and
+// takes its share of the row of all units, [W c / N, W (c + 1) / N): equal work whatever the
+// lengths.  An item that lies in one block is finished there; of one that is cut the blocks
+// leave their sums, maxima and rows, which a second kernel joins, in the blocks' order.
+#pragma once
+
+#include "mhc_cache.cuh"
+
+namespace mhc {
+namespace cattn {
+
+struct Args {
+  cache::View c;
+  const void *q;
+  void *out;
+  int64_t qt, qh;
+  const int64_t *mask;
+  int H, G;
+  float c2;       // scale log2(e)
+  int pieces;     // N
+  int dtype;
+  // what cut items leave: slot 2 c of block c's first item, 2 c + 1 of its last
+  int4 *desc;     // (N, 2)
+  float2 *part_ml;  // (2 N, M): reference (a score) and sum
+  float *part_o;    // (2 N, M, DP)
+  int *err_flag;
+};
+
+struct Segment {
+  cache::Seq s;
+  int b, hk, row0, rows;  // rows [row0, row0 + rows) of the sequence's n G
+  int keys;               // places [0, keys) hold keys
+  int k0, k1, kt;         // key tiles of this block, of the item
+};
+
+__device__ __forceinline__ int keys_of(const cache::View &v, const cache::Seq &s) {
+  const int64_t l = (int64_t)s.len + s.n;
+  return (int)max((int64_t)0, min(l, (int64_t)v.capacity));
+}
+
+template <int M, int KT>
+struct Cut {
+  const Args &a;
+  int64_t first, sum, total;  // units before this lane's sequences, of them, of all
+  int per;                    // sequences of a lane
+  __device__ __forceinline__ Cut(const Args &args) : a(args) {
+    const int lane = threadIdx.x & 31;
+    per = (a.c.batch + 31) / 32;
+    sum = 0;
+    for (int i = 0; i < per; ++i) sum += units(lane * per + i);
+    int64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    first = inc - sum;
+    total = __shfl_sync(0xffffffffu, inc, 31);
+  }
+  __device__ __forceinline__ static int tiles(int keys) { return max(1, (keys + KT - 1) / KT); }
+  __device__ __forceinline__ int row_tiles(int n) const { return (int)(((int64_t)n * a.G + M - 1) / M); }
+  __device__ __forceinline__ int64_t units(int b) const {
+    if (b >= a.c.batch) return 0;
+    const cache::Seq s = cache::seq_of(a.c, b);
+    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * a.c.Hk * tiles(keys_of(a.c, s));
+  }
+  // the sequence of unit w < total, and the unit within it; whole warps
+  __device__ __forceinline__ void find(int64_t w, int &b, int64_t &at) const {
+    const int lane = threadIdx.x & 31;
+    const unsigned has = __ballot_sync(0xffffffffu, w >= first && w < first + sum);
+    const int owner = __ffs(has) - 1;
+    int mine = lane * per;
+    int64_t left = w - first;
+    if (lane == owner)
+      for (int64_t u; left >= (u = units(mine)); ++mine) left -= u;
+    b = __shfl_sync(0xffffffffu, mine, owner);
+    at = __shfl_sync(0xffffffffu, left, owner);
+  }
+};
+
+// Runs `work(segment, slot)` over block `piece`'s units of `pieces`: slot < 0 where the item is whole.
+// Writes the block's entry of the join's table.
+template <int M, int KT, typename F>
+__device__ __forceinline__ void walk(const Args &a, F &&work) {
+  const Cut<M, KT> cut(a);
+  const int64_t W = cut.total, N = min((int64_t)a.pieces, W), piece = blockIdx.x;
+  int4 d0 = make_int4(0, 0, 0, 0), d1 = d0;
+  if (piece < N) {
+    const int64_t w1 = W * (piece + 1) / N;
+    int64_t w = W * piece / N, at;
+    int b;
+    cut.find(w, b, at);
+    while (w < w1) {
+      Segment g;
+      g.b = b;
+      g.s = cache::seq_of(a.c, b);
+      g.keys = keys_of(a.c, g.s);
+      g.kt = Cut<M, KT>::tiles(g.keys);
+      const int mt = cut.row_tiles(g.s.n);
+      const int64_t all = g.s.n == 0 ? 0 : (int64_t)mt * a.c.Hk * g.kt;
+      if (at >= all) {  // the next sequence that has any
+        ++b;
+        at = 0;
+        continue;
+      }
+      const int item = (int)(at / g.kt);
+      g.k0 = (int)(at - (int64_t)item * g.kt);
+      g.k1 = (int)min((int64_t)g.kt, g.k0 + (w1 - w));
+      g.hk = item / mt;
+      g.row0 = (item - g.hk * mt) * M;
+      g.rows = (int)min((int64_t)M, (int64_t)g.s.n * a.G - g.row0);
+      const bool whole = g.k0 == 0 && g.k1 == g.kt;
+      if (g.k0 == 0 && !whole) {  // the last of this block, and it goes on: who else has some of it
+        const int64_t last = w + g.kt - 1, e = ((last + 1) * N - 1) / W;
+        d0 = make_int4((int)(e - piece + 1), g.s.start, g.row0, g.rows);
+        d1 = make_int4(g.hk, 0, 0, 0);
+      }
+      work(g, whole ? -1 : g.k0 == 0 ? (int)(2 * piece + 1) : (int)(2 * piece));
+      w += g.k1 - g.k0;
+      at += g.k1 - g.k0;
+    }
+  }
+  if (threadIdx.x == 0) {
+    a.desc[2 * piece] = d0;
+    a.desc[2 * piece + 1] = d1;
+  }
+}
+
+// rows of no sequence get 0
+template <typename T>
+__device__ __forceinline__ void clear_rest(const Args &a) {
+  const int lo = min(max(a.c.cu[0], 0), a.c.T), hi = min(max(a.c.cu[a.c.batch], 0), a.c.T);
+  T *out = static_cast<T *>(a.out);
+  const int64_t row = (int64_t)a.H * a.c.D, head = lo * row, tail = (int64_t)a.c.T * row;
+  const int64_t step = (int64_t)gridDim.x * blockDim.x, at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (int64_t i = at; i < head; i += step) out[i] = T(0.f);
+  for (int64_t i = hi * row + at; i < tail; i += step) out[i] = T(0.f);
+}
+
+// Whether token j of a sequence sees new token c (place len + c): c < 0 is the context.
+__device__ __forceinline__ bool sees(bool masked, uint64_t bits, int j, int c) {
+  return c < 0 || (masked ? c < 64 && ((bits >> c) & 1) : c <= j);
+}
+
+}  // namespace cattn
+
+}  // namespace mhc

@@ -70,6 +70,12 @@ _PROTOS = {
     "mhc_adamw_check": (_I, [_P, _I, _I, _D, _D, _D, _D, _D]),
     "mhc_adamw_step": (_I, [_P, _I, _I, _D, _D, _D, _D, _D, _D, _P, _P, _P]),
     "mhc_adamw_unpack": (_I, [_P, _I, _P, _P, _I64, _P]),
+    "mhc_rotate": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I64, _I, _P, _P, _I, _I64, _I, _P]),
+    "mhc_append_kv": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _P]),
+    "mhc_keep_drafts": (_I, [_P, _P, _P, _P, _P]),
+    "mhc_cached_attn_workspace": (_SZ, [_P, _P, _I]),
+    "mhc_cached_attn": (_I, [_P, _P, _P, _I, _P, _P, _F, _P, _P, _SZ, _P]),
+    "mhc_verify_drafts": (_I, [_P, _P, _P, _I, _I64, _P, _I64, _P, _I64, _I, _I64, _P, _P, _P, _P, _P]),
     "mhc_set_path_policy": (_I, [_I]),
     "mhc_last_path": (_I, []),
     "mhc_device_error": (_I, [_I]),
@@ -141,7 +147,8 @@ HOST_PATH = os.path.join(_HERE, "_mhc_torch.so")
 # in the order of the module's table
 _HOST_ENTRIES = ("mhc_last_error", "mhc_attn_lse_pitch", "mhc_attn_fwd_workspace", "mhc_attn_fwd",
                  "mhc_attn_bwd_workspace", "mhc_attn_bwd", "mhc_route_fwd_workspace", "mhc_route_fwd",
-                 "mhc_route_bwd", "mhc_grad_norm_workspace", "mhc_grad_norm", "mhc_adamw_check", "mhc_adamw_step")
+                 "mhc_route_bwd", "mhc_grad_norm_workspace", "mhc_grad_norm", "mhc_adamw_check", "mhc_adamw_step", "mhc_rotate",
+                 "mhc_append_kv", "mhc_keep_drafts", "mhc_cached_attn_workspace", "mhc_cached_attn", "mhc_verify_drafts")
 _host = None
 
 
