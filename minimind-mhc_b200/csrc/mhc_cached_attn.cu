@@ -72,74 +72,67 @@ __device__ __forceinline__ float factor(float m, float top, float c2) { return m
 // ---- which row of the item is which query -----------------------------------------
 
 struct Row {
-  int j;           // token of the sequence; -1 past the item's rows
-  int64_t q, out;  // offsets of its elements
   uint64_t bits;
+  int j, h;  // token of the sequence (-1 past the item's rows), head of the group
 };
 __device__ __forceinline__ Row row_of(const Args &a, const Segment &g, int r) {
-  Row x{-1, 0, 0, 0};
+  Row x{0, -1, 0};
   if (r < g.rows) {
     const int at = g.row0 + r;
     x.j = at / a.G;
-    const int h = g.hk * a.G + (at - x.j * a.G);
-    const int64_t t = g.s.start + x.j;
-    x.q = t * a.qt + h * a.qh;
-    x.out = (t * a.H + h) * a.c.D;
-    if (a.mask) x.bits = (uint64_t)a.mask[t];
+    x.h = at - x.j * a.G;
+    if (a.mask) x.bits = (uint64_t)a.mask[g.s.start + x.j];
   }
   return x;
+}
+// offsets of a row's elements, hk its key head
+__device__ __forceinline__ int64_t q_at(const Args &a, const Segment &g, const Row &x, int hk) {
+  return (int64_t)(g.s.start + x.j) * a.qt + (int64_t)(hk * a.G + x.h) * a.qh;
+}
+__device__ __forceinline__ int64_t out_at(const Args &a, const Segment &g, const Row &x, int hk) {
+  return ((int64_t)(g.s.start + x.j) * a.H + hk * a.G + x.h) * a.c.D;
 }
 
 // ---- fetching chunks -----------------------------------------------------------------
 
-// One lane's key of a chunk: its page number is asked for one chunk ahead.
-struct Places {
-  int page;  // of the chunk that is fetched next; -1: none
-  __device__ __forceinline__ void ask(const Args &a, const Segment &g, int key) {
-    page = key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
-  }
-};
+// The page of a key, asked for one chunk ahead.
+__device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key) {
+  return key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
+}
 
 // ---- joining the warps of a block and the blocks of an item ----------------------------
 
-// Every warp has left its (M, DP) sums at `o` (rows of `pitch` floats, `apart` floats between
-// warps) and reference and sum at ml (WARPS, M).
+// Warp w has left its sums for key head w % hw at o + w * apart (M rows of `pitch` floats), reference and sum at ml[w].
 template <typename T, int M, int DP>
-__device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int slot, const float *o, int pitch, int apart,
-                                           float2 (*ml)[M], float (*fac)[M], bool vec) {
-  for (int r = threadIdx.x; r < g.rows; r += THREADS) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w][r].x);
-    float sum = 0.f, f[WARPS];
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      f[w] = factor(ml[w][r].x, top, a.c2);
-      sum = fmaf(f[w], ml[w][r].y, sum);
-    }
+__device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int slot, const Row *rows, const float *o, int pitch,
+                                           int apart, float2 (*ml)[M], float (*fac)[M], bool vec) {
+  const int hw = a.hw, all = hw * g.rows;
+  for (int i = threadIdx.x; i < all; i += THREADS) {
+    const int head = i / g.rows, r = i - head * g.rows;
+    float top = -INFINITY, sum = 0.f;
+    for (int w = head; w < WARPS; w += hw) top = fmaxf(top, ml[w][r].x);
+    for (int w = head; w < WARPS; w += hw) sum = fmaf(factor(ml[w][r].x, top, a.c2), ml[w][r].y, sum);
     float scale = 1.f;
     if (slot < 0) scale = top == -INFINITY ? 0.f : 1.f / sum;
-    else a.part_ml[(int64_t)slot * M + r] = make_float2(top, sum);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) fac[w][r] = f[w] * scale;
+    else a.part_ml[((int64_t)slot * hw + head) * M + r] = make_float2(top, sum);
+    for (int w = head; w < WARPS; w += hw) fac[w][r] = factor(ml[w][r].x, top, a.c2) * scale;
   }
   __syncthreads();
-  constexpr int V = 4;
-  for (int i = threadIdx.x; i < g.rows * (DP / V); i += THREADS) {
-    const int r = i / (DP / V), col = (i - r * (DP / V)) * V;
+  constexpr int V = 4, PER = DP / V;
+  for (int i = threadIdx.x; i < all * PER; i += THREADS) {
+    const int at = i / PER, col = (i - at * PER) * V, head = at / g.rows, r = at - head * g.rows;
     if (col >= a.c.D) continue;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = head; w < WARPS; w += hw) {
       const float f = fac[w][r];
       const float4 y = *reinterpret_cast<const float4 *>(o + (int64_t)w * apart + r * pitch + col);
       x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
     }
     if (slot >= 0) {
-      *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * M + r) * DP + col) = x;
+      *reinterpret_cast<float4 *>(a.part_o + (((int64_t)slot * hw + head) * M + r) * DP + col) = x;
       continue;
     }
-    T *out = static_cast<T *>(a.out) + row_of(a, g, r).out + col;
+    T *out = static_cast<T *>(a.out) + out_at(a, g, rows[r], g.hk + head) + col;
     const float y[4] = {x.x, x.y, x.z, x.w};
     if (vec) {
       struct alignas(4 * sizeof(T)) { T e[4]; } p;
@@ -154,39 +147,77 @@ __device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int 
   }
 }
 
-// Joins the blocks that had part of a cut item.  A warp takes every JW-th block's part of one row, JW warps a row.
-constexpr int JOIN_ROWS = 2, JW = 4;
+// Joins the blocks that had part of a cut item.  Every block lists the cut items (one entry for each block of the first
+// kernel) and takes rows of them in turn; the eight warps share a row's parts, AT_ONCE of them under way in each.
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_PIECES = 1024;
 template <typename T, int M, int DP>
-__global__ void __launch_bounds__(32 * JW * JOIN_ROWS) join_kernel(const Args a) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   wait_for_primary();
-  const int c = blockIdx.x;
-  const int4 d0 = a.desc[2 * c];
-  const int count = d0.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = blockIdx.y * JOIN_ROWS;
-  if (count == 0 || r0 >= d0.w) return;
-  const int which = warp / JW, part = warp % JW, r = r0 + which;
-  const bool live = r < d0.w;
-  __shared__ float st_m[JOIN_ROWS][JW], st_l[JOIN_ROWS][JW];
-  __shared__ float st_o[JOIN_ROWS][JW][DP];
-  constexpr int PER = DP / 32;
-  float o[PER], m = -INFINITY, l = 0.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int first_row[JOIN_PIECES + 1];  // rows of the cut items that begin in blocks before c
+  __shared__ int warp_rows[JOIN_WARPS];
+  __shared__ float st_m[JOIN_WARPS], st_l[JOIN_WARPS];
+  __shared__ float st_o[JOIN_WARPS][DP];
+  constexpr int LIST = JOIN_PIECES / JOIN_THREADS;
+  int mine[LIST], sum = 0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) o[k] = 0.f;
-  // part i of the item: its first block's last slot, then the first slots of the blocks behind it
-  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i); };
-  if (live) {
+  for (int i = 0; i < LIST; ++i) {
+    const int c = threadIdx.x * LIST + i;
+    mine[i] = 0;
+    if (c < a.pieces) {
+      const int4 d = a.desc[2 * c];
+      if (d.x > 0) mine[i] = d.w * a.hw;
+    }
+    sum += mine[i];
+  }
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) warp_rows[warp] = inc;
+  __syncthreads();
+  int at = inc - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < JOIN_WARPS; ++w) {
+    if (w < warp) at += warp_rows[w];
+    total += warp_rows[w];
+  }
+#pragma unroll
+  for (int i = 0; i < LIST; ++i) {
+    first_row[threadIdx.x * LIST + i] = at;
+    at += mine[i];
+  }
+  if (threadIdx.x == 0) first_row[JOIN_PIECES] = total;
+  __syncthreads();
+  constexpr int PER = DP / 32;
+  for (int task = blockIdx.x; task < total; task += gridDim.x) {
+    int c = 0;
+#pragma unroll
+    for (int step = JOIN_PIECES / 2; step; step >>= 1)
+      if (first_row[c + step] <= task) c += step;  // the last block whose rows begin at or before it
+    const int4 d0 = a.desc[2 * c];
+    const int count = d0.x, local = task - first_row[c], head = local / d0.w, r = local - head * d0.w;
+    const int64_t row = (int64_t)head * M + r, rows = (int64_t)a.hw * M;
+    float o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = 0.f;
+    // part i of the item: its first block's last slot, then the first slots of the blocks behind it
+    auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i); };
     constexpr int AT_ONCE = 4;
-    for (int i0 = part; i0 < count; i0 += JW * AT_ONCE) {
+    for (int i0 = warp; i0 < count; i0 += JOIN_WARPS * AT_ONCE) {
       float2 ml[AT_ONCE];
       float x[AT_ONCE][PER];
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = i0 + u * JW;
+        const int i = i0 + u * JOIN_WARPS;
         ml[u] = make_float2(-INFINITY, 0.f);
         if (i < count) {
-          ml[u] = a.part_ml[slot(i) * M + r];
+          const int64_t at_row = slot(i) * rows + row;
+          ml[u] = a.part_ml[at_row];
 #pragma unroll
-          for (int k = 0; k < PER; ++k) x[u][k] = a.part_o[(slot(i) * M + r) * DP + lane + 32 * k];
+          for (int k = 0; k < PER; ++k) x[u][k] = a.part_o[at_row * DP + lane + 32 * k];
         }
       }
 #pragma unroll
@@ -199,33 +230,29 @@ __global__ void __launch_bounds__(32 * JW * JOIN_ROWS) join_kernel(const Args a)
         for (int k = 0; k < PER; ++k) o[k] = fmaf(o[k], f, x[u][k] * g);
       }
     }
+    if (lane == 0) {
+      st_m[warp] = m;
+      st_l[warp] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) st_o[warp][lane + 32 * k] = o[k];
+    __syncthreads();
+    if (threadIdx.x < DP && threadIdx.x < a.c.D) {
+      float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, st_m[w]);
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        const float f = factor(st_m[w], top, a.c2);
+        sum = fmaf(f, st_l[w], sum);
+        y = fmaf(f, st_o[w][threadIdx.x], y);
+      }
+      const int row_at = d0.z + r, j = row_at / a.G, hk = a.desc[2 * c + 1].x + head;
+      T *out = static_cast<T *>(a.out) + ((int64_t)(d0.y + j) * a.H + hk * a.G + (row_at - j * a.G)) * a.c.D;
+      out[threadIdx.x] = from_f<T>(top == -INFINITY ? 0.f : y * (1.f / sum));
+    }
+    __syncthreads();
   }
-  if (lane == 0) {
-    st_m[which][part] = m;
-    st_l[which][part] = l;
-  }
-#pragma unroll
-  for (int k = 0; k < PER; ++k) st_o[which][part][lane + 32 * k] = o[k];
-  __syncthreads();
-  if (!live || part != 0) return;
-  float top = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int p = 0; p < JW; ++p) top = fmaxf(top, st_m[which][p]);
-#pragma unroll
-  for (int k = 0; k < PER; ++k) o[k] = 0.f;
-#pragma unroll
-  for (int p = 0; p < JW; ++p) {
-    const float f = factor(st_m[which][p], top, a.c2);
-    sum = fmaf(f, st_l[which][p], sum);
-#pragma unroll
-    for (int k = 0; k < PER; ++k) o[k] = fmaf(f, st_o[which][p][lane + 32 * k], o[k]);
-  }
-  const float scale = top == -INFINITY ? 0.f : 1.f / sum;
-  const int at = d0.z + r, j = at / a.G, hk = a.desc[2 * c + 1].x;
-  T *out = static_cast<T *>(a.out) + ((int64_t)(d0.y + j) * a.H + hk * a.G + (at - j * a.G)) * a.c.D;
-#pragma unroll
-  for (int k = 0; k < PER; ++k)
-    if (lane + 32 * k < a.c.D) out[lane + 32 * k] = from_f<T>(top == -INFINITY ? 0.f : o[k] * scale);
 }
 
 // ---- 16-bit types ------------------------------------------------------------------------
@@ -266,235 +293,250 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
   return (w & E) == E || ((w >> 16) & E) == E;
 }
 
-template <int DP>
+template <int DP, int R>
 struct MmaShape {
+  static constexpr int M = 8 * R;
   static constexpr int PITCH = DP * 2 + 16;  // bytes of a row: eight of them begin in different banks
   static constexpr int STAGE = 2 * CHUNK * PITCH;
-  static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 4 : DP >= 64 ? 6 : 8;
+  // blocks of an SM by registers (32 R and more for O), then chunks of a warp's ring by shared memory
+  static constexpr int BLOCKS = R == 4 ? 2 : DP >= 128 ? 3 : 4;
+  static constexpr int STAGES = BLOCKS == 2 ? (DP >= 128 ? 3 : DP >= 96 ? 4 : DP >= 64 ? 6 : 8) : DP >= 96 ? 2 : DP >= 64 ? 3 : 5;
   static constexpr int RING = STAGES * STAGE;  // of a warp
   static constexpr int SMEM = WARPS * RING;
-  static constexpr int OP = DP + 8;  // floats of a row of O while the warps are joined
+  static constexpr int OP = DP + 4;  // floats of a row of O while the warps are joined
 };
 
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(THREADS, 2) mma_kernel(const Args a) {
-  using S = MmaShape<DP>;
-  constexpr int M = 16 * MT, KS = DP / 16, NT = DP / 8;
-  constexpr int VPR = DP / 8, IT = CHUNK * VPR / 32;  // 16-byte vectors of a row; copies of a lane for 16 rows
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // of an 8 x 8 matrix of 16-bit values over the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(const Args a) {
+  using S = MmaShape<DP, R>;
+  constexpr int M = S::M, KS = DP / 16, VPR = DP / 8;
+  constexpr int RPI = 32 / VPR, IT = CHUNK / RPI;  // rows that a warp's lanes copy at a time (VPR 12: 24 lanes)
   constexpr float AHEAD = std::is_same<T, __half>::value ? 4.f : 8.f, LIFT = std::is_same<T, __half>::value ? 10.f : 0.f;
   static_assert(M * S::OP * 4 <= S::RING, "O of a warp fits its ring");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
   __shared__ uint32_t have[WARPS][S::STAGES];  // which keys of a chunk exist
+  __shared__ Row rows[M];
   __shared__ float2 ml[WARPS][M];
   __shared__ float fac[WARPS][M];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
   const uint32_t ring = sm100::smem_u32(smem) + warp * S::RING;
-  const int D = a.c.D, vpr = D / 8;
+  const int D = a.c.D;
+  const int head = warp % a.hw, part = warp / a.hw;  // key head of the item; which of the tile's chunks
+  const bool one_page = a.c.size % CHUNK == 0;       // a chunk never crosses a page's end
+  const int fetch_row = lane / VPR, fetch_col = lane - fetch_row * VPR;
+  const bool fetches = fetch_row < RPI && fetch_col * 8 < D;
   const float ahead = AHEAD / a.c2;
-  for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  if (D < DP)
+    for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   clear_rest<T>(a);
   __syncthreads();
 
-  walk<M, KT>(a, [&](const Segment &g, int slot) {
-    Row row[MT][2];
-    uint32_t q[MT][KS][4];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) row[t][h] = row_of(a, g, 16 * t + 8 * h + lane / 4);
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const Row &x = row[t][i & 1];
-          const int col = 16 * k + 8 * (i >> 1) + 2 * (lane & 3);
-          q[t][k][i] = x.j >= 0 && col < D ? *reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.q) + x.q + col) : 0u;
-        }
-    }
-    const T *kbase = static_cast<const T *>(a.c.keys) + g.hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + g.hk * a.c.vh;
+  walk<M>(a, [&](const Segment &g, int slot) {
+    const int hk = g.hk + head;
+    const T *kbase = static_cast<const T *>(a.c.keys) + hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + hk * a.c.vh;
     const int chunks = g.k1 - g.k0;
-    const int key0 = g.k0 * KT + warp * CHUNK;  // of chunk i: key0 + i * KT
-    Places places;
-    places.ask(a, g, key0 + (lane & 15));
+    const int key0 = g.k0 * a.tile + part * CHUNK;  // of chunk i: key0 + i * tile
+    int page = page_of(a, g, one_page ? key0 : key0 + (lane & 15));
     auto fetch = [&](int i) {
       if (i < chunks) {
-        const int key = key0 + i * KT + (lane & 15), st = i % S::STAGES;
-        const bool there = places.page >= 0 && places.page < a.c.pages;
-        const uint32_t got = __ballot_sync(0xffffffffu, there) & 0xffffu;
-        if (lane < CHUNK) {
-          const int slot_at = key - cache::page_index(a.c, key) * a.c.size;
-          off_k[warp][lane] = there ? places.page * a.c.kp + slot_at * a.c.ks : -1;
-          off_v[warp][lane] = there ? places.page * a.c.vp + slot_at * a.c.vs : -1;
-        }
-        if (lane == 0) have[warp][st] = got;
-        places.ask(a, g, key + KT);
-        __syncwarp();
-        const uint32_t dst = ring + st * S::STAGE;
-#pragma unroll
-        for (int u = 0; u < IT; ++u) {
-          const int at = u * 32 + lane, r = at / VPR, x = at - r * VPR;
-          if (x < vpr) {
-            const int64_t ok = off_k[warp][r], ov = off_v[warp][r];
-            cp16(dst + r * S::PITCH + x * 16, kbase + (ok >= 0 ? ok + x * 8 : 0), ok >= 0);
-            cp16(dst + (CHUNK + r) * S::PITCH + x * 16, vbase + (ov >= 0 ? ov + x * 8 : 0), ov >= 0);
+        const int key = key0 + i * a.tile, st = i % S::STAGES;
+        const uint32_t kd = ring + st * S::STAGE + fetch_row * S::PITCH + fetch_col * 16, vd = kd + CHUNK * S::PITCH;
+        if (one_page) {
+          const int there = page >= 0 && page < a.c.pages ? min(max(g.keys - key, 0), CHUNK) : 0;
+          if (lane == 0) have[warp][st] = (1u << there) - 1;
+          const int first = key - cache::page_index(a.c, key) * a.c.size + fetch_row;
+          const T *ks = kbase + fetch_col * 8, *vs = vbase + fetch_col * 8;
+          if (there > 0) {
+            ks += page * a.c.kp + first * a.c.ks;
+            vs += page * a.c.vp + first * a.c.vs;
           }
+          page = page_of(a, g, key + a.tile);
+          if (fetches) {
+#pragma unroll
+            for (int u = 0; u < IT; ++u) {
+              const bool ok = u * RPI + fetch_row < there;
+              cp16(kd + u * RPI * S::PITCH, ok ? ks + (int64_t)(u * RPI) * a.c.ks : kbase, ok);
+              cp16(vd + u * RPI * S::PITCH, ok ? vs + (int64_t)(u * RPI) * a.c.vs : vbase, ok);
+            }
+          }
+        } else {
+          const int mine = key + (lane & 15);
+          const bool there = page >= 0 && page < a.c.pages;
+          const uint32_t got = __ballot_sync(0xffffffffu, there) & 0xffffu;
+          if (lane < CHUNK) {
+            const int slot_at = mine - cache::page_index(a.c, mine) * a.c.size;
+            off_k[warp][lane] = there ? page * a.c.kp + slot_at * a.c.ks : -1;
+            off_v[warp][lane] = there ? page * a.c.vp + slot_at * a.c.vs : -1;
+          }
+          if (lane == 0) have[warp][st] = got;
+          page = page_of(a, g, mine + a.tile);
+          __syncwarp();
+          if (fetches) {
+#pragma unroll
+            for (int u = 0; u < IT; ++u) {
+              const int64_t ok = off_k[warp][u * RPI + fetch_row], ov = off_v[warp][u * RPI + fetch_row];
+              cp16(kd + u * RPI * S::PITCH, kbase + (ok >= 0 ? ok + fetch_col * 8 : 0), ok >= 0);
+              cp16(vd + u * RPI * S::PITCH, vbase + (ov >= 0 ? ov + fetch_col * 8 : 0), ov >= 0);
+            }
+          }
+          __syncwarp();  // the offsets have been read
         }
-        __syncwarp();  // the offsets have been read
       }
       cp_commit();
     };
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
 
-    float o[MT][NT][4], m[MT][2], l[MT][2];
+    if (tid < M) rows[tid] = row_of(a, g, tid);
+    __syncthreads();
+    uint32_t q[R][KS][2];  // Q^T as the second operand: elements 16 k + 2 quad (+ 8) of row oct
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < R; ++t) {
+      const Row x = rows[8 * t + oct];
+      const T *src = static_cast<const T *>(a.q) + (x.j >= 0 ? q_at(a, g, x, hk) : 0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][n][i] = 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const int col = 16 * k + 8 * i + 2 * quad;
+          q[t][k][i] = x.j >= 0 && col < D ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
+        }
+    }
+    float o[R][KS][4];  // O^T: elements 16 k + oct (+ 8) of rows 2 quad, 2 quad + 1
+    float m[R][2], l[R][2];
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][k][i] = 0.f;
       m[t][0] = m[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
     for (int i = 0; i < chunks; ++i) {
       cp_wait<S::STAGES - 2>();
       __syncwarp();
-      const int st = i % S::STAGES, key = key0 + i * KT;
+      const int st = i % S::STAGES, key = key0 + i * a.tile;
       const uint32_t kt = ring + st * S::STAGE, vt = kt + CHUNK * S::PITCH;
       const uint32_t got = have[warp][st];
       if (got) {
-        float s[MT][2][4];
+        float s[R][4];  // S^T: keys oct and oct + 8 of rows 2 quad, 2 quad + 1
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][n][e] = 0.f;
-        const uint32_t ka = kt + ((lane & 7) + ((lane >> 4) & 1) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+        for (int t = 0; t < R; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+        const uint32_t ka = kt + (lane & 15) * S::PITCH + (lane >> 4) * 16;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          uint32_t b[4];
-          ldsm4(b, ka + k * 32);
+          uint32_t w[4];
+          ldsm4(w, ka + k * 32);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma16816<T>(s[t][0], q[t][k], b[0], b[1]);
-            mma16816<T>(s[t][1], q[t][k], b[2], b[3]);
-          }
+          for (int t = 0; t < R; ++t) mma16816<T>(s[t], w, q[t][k][0], q[t][k][1]);
         }
         // rows differ in what they see only from the first new token on, or where keys are missing
         const bool uneven = got != 0xffffu || key + CHUNK > g.s.len;
-        uint32_t seen[MT][2];  // bit n * 2 + e: keys 8 n + 2 (lane % 4) + e
+        uint32_t seen[R];  // bit 2 h + e: key oct + 8 h by row 2 quad + e
         bool move = false;
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < R; ++t) {
+          seen[t] = 0xfu;
+          if (uneven) {
+            seen[t] = 0;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top = -FLT_MAX;
-            if (uneven) {
-              uint32_t v = 0;
+            for (int e = 0; e < 2; ++e) {
+              const Row x = rows[8 * t + 2 * quad + e];
 #pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int at = 8 * n + 2 * (lane & 3) + e;
-                  const bool ok = ((got >> at) & 1) && row[t][h].j >= 0 &&
-                                  sees(a.mask != nullptr, row[t][h].bits, row[t][h].j, key + at - g.s.len);
-                  v |= (uint32_t)ok << (2 * n + e);
-                  if (ok) top = fmaxf(top, s[t][n][2 * h + e]);
-                }
-              seen[t][h] = v;
-              if (!v) top = -INFINITY;
-            } else {
-              seen[t][h] = 0xfu;
-#pragma unroll
-              for (int n = 0; n < 2; ++n) top = fmaxf(top, fmaxf(s[t][n][2 * h], s[t][n][2 * h + 1]));
+              for (int h = 0; h < 2; ++h) {
+                const int at = oct + 8 * h;
+                const bool ok = ((got >> at) & 1) && x.j >= 0 && sees(a.mask != nullptr, x.bits, x.j, key + at - g.s.len);
+                seen[t] |= (uint32_t)ok << (2 * h + e);
+              }
             }
-            move = move || top > m[t][h] + ahead;
           }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool k0 = (seen[t] >> e) & 1, k1 = (seen[t] >> (2 + e)) & 1;
+            const float top = fmaxf(k0 ? fmaxf(s[t][e], -FLT_MAX) : -INFINITY, k1 ? fmaxf(s[t][2 + e], -FLT_MAX) : -INFINITY);
+            move = move || top > m[t][e] + ahead;
+          }
+        }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
+          for (int t = 0; t < R; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float top = seen[t][h] ? -FLT_MAX : -INFINITY;
+            for (int e = 0; e < 2; ++e) {
+              const bool k0 = (seen[t] >> e) & 1, k1 = (seen[t] >> (2 + e)) & 1;
+              float top = fmaxf(k0 ? fmaxf(s[t][e], -FLT_MAX) : -INFINITY, k1 ? fmaxf(s[t][2 + e], -FLT_MAX) : -INFINITY);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              top = fmaxf(top, m[t][e]);
+              const float f = m[t][e] == top ? 1.f : factor(m[t][e], top, a.c2);
+              m[t][e] = top;
+              l[t][e] *= f;
 #pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if ((seen[t][h] >> (2 * n + e)) & 1) top = fmaxf(top, s[t][n][2 * h + e]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              top = fmaxf(top, m[t][h]);
-              const float f = m[t][h] == top ? 1.f : factor(m[t][h], top, a.c2);
-              m[t][h] = top;
-              l[t][h] *= f;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                o[t][n][2 * h] *= f;
-                o[t][n][2 * h + 1] *= f;
+              for (int k = 0; k < KS; ++k) {
+                o[t][k][e] *= f;
+                o[t][k][2 + e] *= f;
               }
             }
         }
-        uint32_t p[MT][4];
+        uint32_t p[R][2];  // P^T as the second operand: keys 2 quad, 2 quad + 1 (+ 8) of row oct
+        float x[R][4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < R; ++t) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float x = ex2(fmaf(s[t][n][2 * h] - m[t][h], a.c2, LIFT)), y = ex2(fmaf(s[t][n][2 * h + 1] - m[t][h], a.c2, LIFT));
-              if (uneven) {
-                if (!((seen[t][h] >> (2 * n)) & 1)) x = 0.f;
-                if (!((seen[t][h] >> (2 * n + 1)) & 1)) y = 0.f;
-              }
-              l[t][h] += x + y;
-              p[t][2 * n + h] = pack2<T>(x, y);
-            }
-        const uint32_t va = vt + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + ((lane >> 4) & 1) * 16;
+          for (int i = 0; i < 4; ++i) {
+            x[t][i] = ex2(fmaf(s[t][i] - m[t][i & 1], a.c2, LIFT));
+            if (uneven && !((seen[t] >> i) & 1)) x[t][i] = 0.f;
+            l[t][i & 1] += x[t][i];
+          }
+          p[t][0] = transposed(pack2<T>(x[t][0], x[t][1]));
+          p[t][1] = transposed(pack2<T>(x[t][2], x[t][3]));
+        }
         bool odd = false;
         if (uneven) {
           for (int at = lane; at < CHUNK * (DP / 2); at += 32) {
-            const int r = at / (DP / 2), x = at - r * (DP / 2);
+            const int r = at / (DP / 2), c = at - r * (DP / 2);
             uint32_t w;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vt + r * S::PITCH + x * 4));
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vt + r * S::PITCH + c * 4));
             odd = odd || odd_pair<T>(w);
           }
           odd = __any_sync(0xffffffffu, odd);
         }
         if (!odd) {
+          const uint32_t va = vt + ((lane & 7) + ((lane >> 4) & 1) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
-          for (int n = 0; n < NT / 2; ++n) {
-            uint32_t b[4];
-            ldsm4t(b, va + n * 32);
+          for (int k = 0; k < KS; ++k) {
+            uint32_t w[4];
+            ldsm4t(w, va + k * 32);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              mma16816<T>(o[t][2 * n], p[t], b[0], b[1]);
-              mma16816<T>(o[t][2 * n + 1], p[t], b[2], b[3]);
-            }
+            for (int t = 0; t < R; ++t) mma16816<T>(o[t][k], w, p[t][0], p[t][1]);
           }
         } else {
-          // key by key: P of the row's four lanes that hold it, V of this lane's columns
+          // key by key: its P from the lanes that hold it (rounded, as in the product), V of this lane's elements
 #pragma unroll 1
           for (int at = 0; at < CHUNK; ++at) {
-            const int from = (lane & ~3) | ((at & 7) >> 1);
+            const int from = ((at & 7) << 2) | quad;
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int t = 0; t < R; ++t)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t w = __shfl_sync(0xffffffffu, at < 8 ? p[t][h] : p[t][2 + h], from);
-                const uint32_t sees_it = __shfl_sync(0xffffffffu, seen[t][h], from) >> ((at < 8 ? 0 : 2) + (at & 1)) & 1;
-                const uint16_t half_word = (uint16_t)((at & 1) ? w >> 16 : w);
-                const float x = to_f(*reinterpret_cast<const T *>(&half_word));
-                if (sees_it) {
+              for (int e = 0; e < 2; ++e) {
+                const float w = to_f(from_f<T>(__shfl_sync(0xffffffffu, at < 8 ? x[t][e] : x[t][2 + e], from)));
+                if ((__shfl_sync(0xffffffffu, seen[t], from) >> ((at < 8 ? 0 : 2) + e)) & 1) {
 #pragma unroll
-                  for (int n = 0; n < NT; ++n) {
-                    uint32_t v;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(vt + at * S::PITCH + (n * 8 + 2 * (lane & 3)) * 2));
-                    const uint16_t v0 = (uint16_t)v, v1 = (uint16_t)(v >> 16);
-                    o[t][n][2 * h] = fmaf(x, to_f(*reinterpret_cast<const T *>(&v0)), o[t][n][2 * h]);
-                    o[t][n][2 * h + 1] = fmaf(x, to_f(*reinterpret_cast<const T *>(&v1)), o[t][n][2 * h + 1]);
-                  }
+                  for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                      uint16_t v;
+                      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(vt + at * S::PITCH + (16 * k + 8 * h + oct) * 2));
+                      o[t][k][2 * h + e] = fmaf(w, to_f(*reinterpret_cast<const T *>(&v)), o[t][k][2 * h + e]);
+                    }
                 }
               }
           }
@@ -507,23 +549,27 @@ __global__ void __launch_bounds__(THREADS, 2) mma_kernel(const Args a) {
     __syncwarp();
     float *mine = reinterpret_cast<float *>(smem + warp * S::RING);
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < R; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
-        l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
-        const int r = 16 * t + 8 * h + lane / 4;
-        if ((lane & 3) == 0) ml[warp][r] = make_float2(m[t][h], l[t][h]);
+      for (int e = 0; e < 2; ++e) {
+        l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
+        l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
+        l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
+        const int r = 8 * t + 2 * quad + e;
+        if (oct == 0) ml[warp][r] = make_float2(m[t][e], l[t][e]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          *reinterpret_cast<float2 *>(mine + r * S::OP + n * 8 + 2 * (lane & 3)) = make_float2(o[t][n][2 * h], o[t][n][2 * h + 1]);
+        for (int k = 0; k < KS; ++k) {
+          mine[r * S::OP + 16 * k + oct] = o[t][k][e];
+          mine[r * S::OP + 16 * k + 8 + oct] = o[t][k][2 + e];
+        }
       }
     __syncthreads();
-    join_warps<T, M, DP>(a, g, slot, reinterpret_cast<const float *>(smem), S::OP, S::RING / 4, ml, fac, true);
+    join_warps<T, M, DP>(a, g, slot, rows, reinterpret_cast<const float *>(smem), S::OP, S::RING / 4, ml, fac, true);
     __syncthreads();
-    if (D < DP)  // columns past D are zeros again
+    if (D < DP) {  // columns past D are zeros again
       for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+      __syncthreads();
+    }
   });
   launch_dependents();
 }
@@ -564,29 +610,28 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
   clear_rest<T>(a);
   __syncthreads();
 
-  walk<R, KT>(a, [&](const Segment &g, int slot) {
+  walk<R>(a, [&](const Segment &g, int slot) {
     for (int r = tid; r < R; r += THREADS) rows[r] = row_of(a, g, r);
     __syncthreads();
     for (int i = tid; i < R * DP; i += THREADS) {
       const int r = i / DP, x = i - r * DP;
-      qs[i] = rows[r].j >= 0 && x < D ? to_f(static_cast<const T *>(a.q)[rows[r].q + x]) : 0.f;
+      qs[i] = rows[r].j >= 0 && x < D ? to_f(static_cast<const T *>(a.q)[q_at(a, g, rows[r], g.hk) + x]) : 0.f;
     }
     const T *kbase = static_cast<const T *>(a.c.keys) + g.hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + g.hk * a.c.vh;
-    const int chunks = g.k1 - g.k0, key0 = g.k0 * KT + warp * CHUNK;
-    Places places;
-    places.ask(a, g, key0 + (lane & 15));
+    const int chunks = g.k1 - g.k0, key0 = g.k0 * KT + warp * CHUNK;  // hw is 1 here, a tile KT keys
+    int page = page_of(a, g, key0 + (lane & 15));
     auto fetch = [&](int i) {
       if (i < chunks) {
         const int key = key0 + i * KT + (lane & 15), st = i % S::STAGES;
-        const bool there = places.page >= 0 && places.page < a.c.pages;
+        const bool there = page >= 0 && page < a.c.pages;
         const uint32_t got = __ballot_sync(0xffffffffu, there) & 0xffffu;
         if (lane < CHUNK) {
           const int slot_at = key - cache::page_index(a.c, key) * a.c.size;
-          off_k[warp][lane] = there ? places.page * a.c.kp + slot_at * a.c.ks : -1;
-          off_v[warp][lane] = there ? places.page * a.c.vp + slot_at * a.c.vs : -1;
+          off_k[warp][lane] = there ? page * a.c.kp + slot_at * a.c.ks : -1;
+          off_v[warp][lane] = there ? page * a.c.vp + slot_at * a.c.vs : -1;
         }
         if (lane == 0) have[warp][st] = got;
-        places.ask(a, g, key + KT);
+        page = page_of(a, g, key + KT);
         __syncwarp();
         float *kt = ring + st * S::STAGE, *vt = kt + CHUNK * S::KP;
         if constexpr (ASYNC) {
@@ -712,7 +757,7 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
       if (share == 0 && col < DP) *reinterpret_cast<float4 *>(ring + r * S::OP + col) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
     }
     __syncthreads();
-    join_warps<T, R, DP>(a, g, slot, fsm, S::OP, S::RING, ml, fac, a.c.D % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0);
+    join_warps<T, R, DP>(a, g, slot, rows, fsm, S::OP, S::RING, ml, fac, a.c.D % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0);
     __syncthreads();
     if (D < DP)  // columns past D are zeros again
       for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
@@ -727,7 +772,7 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
 // average there are T / batch of them.
 struct Choice {
   bool mma;
-  int m, dp, pieces;
+  int m, dp, hw, pieces;
   size_t desc, ml, o, total;  // bytes of the workspace
 };
 static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, bool aligned) {
@@ -736,12 +781,22 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, bool
   const int64_t rows = (s->T + s->batch - 1) / s->batch * G;
   x.mma = aligned;
   x.dp = (c->dim + 31) / 32 * 32;
-  x.m = x.mma ? (rows <= 16 ? 16 : 32) : (rows <= 4 ? 4 : 16);
-  x.pieces = sms * (x.mma ? 2 : 1);
+  x.hw = 1;
+  if (x.mma) {
+    x.m = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    // the warps of a block take neighbouring key heads of the same keys, which lie side by side in memory
+    x.hw = c->kv_heads % 4 == 0 ? 4 : c->kv_heads % 2 == 0 ? 2 : 1;
+    x.pieces = sms * (x.m == 32 ? 2 : x.dp >= 128 ? 3 : 4);
+  } else {
+    x.m = rows <= 4 ? 4 : 16;
+    x.pieces = sms;
+  }
+  if (x.pieces > JOIN_PIECES) x.pieces = JOIN_PIECES;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+  const size_t rows_kept = (size_t)x.pieces * 2 * x.hw * x.m;
   x.desc = up((size_t)x.pieces * 2 * sizeof(int4));
-  x.ml = up((size_t)x.pieces * 2 * x.m * sizeof(float2));
-  x.o = up((size_t)x.pieces * 2 * x.m * x.dp * sizeof(float));
+  x.ml = up(rows_kept * sizeof(float2));
+  x.o = up(rows_kept * x.dp * sizeof(float));
   x.total = x.desc + x.ml + x.o;
   return x;
 }
@@ -758,8 +813,10 @@ static cudaError_t start(K kernel, const Args &a, int blocks, int smem, cudaStre
 template <typename T, int M, int DP>
 static cudaError_t join(const Args &a, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.pieces, (M + JOIN_ROWS - 1) / JOIN_ROWS);
-  cfg.blockDim = dim3(32 * JW * JOIN_ROWS);
+  const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  const int64_t rows = (int64_t)a.c.T * a.H;
+  cfg.gridDim = dim3((unsigned)(rows < 4 * sms ? rows : 4 * sms));
+  cfg.blockDim = dim3(JOIN_THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -783,14 +840,16 @@ static cudaError_t launch(const Args &a, const Choice &x, bool async, cudaStream
   return with_dp(x.dp, [&](auto dp) -> cudaError_t {
     constexpr int DP = decltype(dp)::value;
     if (x.mma) {
-      auto go = [&](auto tag, auto mt) -> cudaError_t {
+      auto go = [&](auto tag, auto r) -> cudaError_t {
         using T = decltype(tag);
-        constexpr int MT = decltype(mt)::value;
-        cudaError_t e = start(mma_kernel<T, DP, MT>, a, x.pieces, MmaShape<DP>::SMEM, st);
-        return e != cudaSuccess ? e : join<T, 16 * MT, DP>(a, st);
+        constexpr int R = decltype(r)::value;
+        cudaError_t e = start(mma_kernel<T, DP, R>, a, x.pieces, MmaShape<DP, R>::SMEM, st);
+        return e != cudaSuccess ? e : join<T, 8 * R, DP>(a, st);
       };
-      if (a.dtype == MHC_BF16) return x.m == 16 ? go(__nv_bfloat16{}, IC<1>{}) : go(__nv_bfloat16{}, IC<2>{});
-      return x.m == 16 ? go(__half{}, IC<1>{}) : go(__half{}, IC<2>{});
+      auto by_rows = [&](auto tag) -> cudaError_t {
+        return x.m == 8 ? go(tag, IC<1>{}) : x.m == 16 ? go(tag, IC<2>{}) : go(tag, IC<4>{});
+      };
+      return a.dtype == MHC_BF16 ? by_rows(__nv_bfloat16{}) : by_rows(__half{});
     }
     return with_dtype(a.dtype, [&](auto tag) -> cudaError_t {
       using T = decltype(tag);
@@ -857,7 +916,7 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   a.q = q, a.out = out, a.qt = q_strides[0], a.qh = q_strides[1];
   a.mask = mask, a.H = H, a.G = H / cache->kv_heads;
   a.c2 = (float)((double)scale * 1.4426950408889634);
-  a.pieces = x.pieces, a.dtype = cache->dtype;
+  a.pieces = x.pieces, a.hw = x.hw, a.tile = cattn::KT / x.hw, a.dtype = cache->dtype;
   char *ws = static_cast<char *>(workspace);
   a.desc = reinterpret_cast<int4 *>(ws);
   a.part_ml = reinterpret_cast<float2 *>(ws + x.desc);

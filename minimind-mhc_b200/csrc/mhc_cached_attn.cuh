@@ -1,11 +1,12 @@
 // Attention over a paged cache: arguments, and the cut of the work into equal pieces.
 //
-// The unit of work is a tile of KT keys for up to M rows (new tokens x heads of a group) of
-// one sequence and key head, the item.  The lengths are known on the device only, so
+// The unit of work is a tile of `tile` keys for up to M rows (new tokens x heads of a
+// group) of one sequence and `hw` neighbouring key heads, the item; an item counts COST
+// units more, for its beginning and end.  The lengths are known on the device only, so
 // every block sums the units of all sequences itself (a few loads and one warp's scan) and
 // takes its share of the row of all units, [W c / N, W (c + 1) / N): equal work whatever the
 // lengths.  An item that lies in one block is finished there; of one that is cut the blocks
-// leave their sums, maxima and rows, which a second kernel joins, in the blocks' order.
+// leave their sums, references and rows, which a second kernel joins, in the blocks' order.
 #pragma once
 
 #include "mhc_cache.cuh"
@@ -22,27 +23,30 @@ struct Args {
   int H, G;
   float c2;       // scale log2(e)
   int pieces;     // N
+  int hw, tile;   // key heads and keys of a unit
   int dtype;
   // what cut items leave: slot 2 c of block c's first item, 2 c + 1 of its last
-  int4 *desc;     // (N, 2)
-  float2 *part_ml;  // (2 N, M): reference (a score) and sum
-  float *part_o;    // (2 N, M, DP)
-  int *err_flag;
+  int4 *desc;       // (N, 2)
+  float2 *part_ml;  // (2 N, hw M): reference (a score) and sum
+  float *part_o;    // (2 N, hw M, DP)
 };
 
 struct Segment {
   cache::Seq s;
-  int b, hk, row0, rows;  // rows [row0, row0 + rows) of the sequence's n G
+  int b, hk, row0, rows;  // key heads [hk, hk + hw), rows [row0, row0 + rows) of the sequence's n G
   int keys;               // places [0, keys) hold keys
   int k0, k1, kt;         // key tiles of this block, of the item
 };
+
+// An item's beginning (pages, then rows, one after the other; queries) and end take a block about as long as two tiles.
+constexpr int COST = 2;
 
 __device__ __forceinline__ int keys_of(const cache::View &v, const cache::Seq &s) {
   const int64_t l = (int64_t)s.len + s.n;
   return (int)max((int64_t)0, min(l, (int64_t)v.capacity));
 }
 
-template <int M, int KT>
+template <int M>
 struct Cut {
   const Args &a;
   int64_t first, sum, total;  // units before this lane's sequences, of them, of all
@@ -61,12 +65,12 @@ struct Cut {
     first = inc - sum;
     total = __shfl_sync(0xffffffffu, inc, 31);
   }
-  __device__ __forceinline__ static int tiles(int keys) { return max(1, (keys + KT - 1) / KT); }
+  __device__ __forceinline__ int tiles(int keys) const { return max(1, (keys + a.tile - 1) / a.tile); }
   __device__ __forceinline__ int row_tiles(int n) const { return (int)(((int64_t)n * a.G + M - 1) / M); }
   __device__ __forceinline__ int64_t units(int b) const {
     if (b >= a.c.batch) return 0;
     const cache::Seq s = cache::seq_of(a.c, b);
-    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * a.c.Hk * tiles(keys_of(a.c, s));
+    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * (a.c.Hk / a.hw) * (tiles(keys_of(a.c, s)) + COST);
   }
   // the sequence of unit w < total, and the unit within it; whole warps
   __device__ __forceinline__ void find(int64_t w, int &b, int64_t &at) const {
@@ -82,11 +86,11 @@ struct Cut {
   }
 };
 
-// Runs `work(segment, slot)` over block `piece`'s units of `pieces`: slot < 0 where the item is whole.
+// Runs `work(segment, slot)` over block blockIdx.x's units: slot < 0 where the item is whole.
 // Writes the block's entry of the join's table.
-template <int M, int KT, typename F>
+template <int M, typename F>
 __device__ __forceinline__ void walk(const Args &a, F &&work) {
-  const Cut<M, KT> cut(a);
+  const Cut<M> cut(a);
   const int64_t W = cut.total, N = min((int64_t)a.pieces, W), piece = blockIdx.x;
   int4 d0 = make_int4(0, 0, 0, 0), d1 = d0;
   if (piece < N) {
@@ -99,29 +103,33 @@ __device__ __forceinline__ void walk(const Args &a, F &&work) {
       g.b = b;
       g.s = cache::seq_of(a.c, b);
       g.keys = keys_of(a.c, g.s);
-      g.kt = Cut<M, KT>::tiles(g.keys);
-      const int mt = cut.row_tiles(g.s.n);
-      const int64_t all = g.s.n == 0 ? 0 : (int64_t)mt * a.c.Hk * g.kt;
+      g.kt = cut.tiles(g.keys);
+      const int mt = cut.row_tiles(g.s.n), span = g.kt + COST;
+      const int64_t all = g.s.n == 0 ? 0 : (int64_t)mt * (a.c.Hk / a.hw) * span;
       if (at >= all) {  // the next sequence that has any
         ++b;
         at = 0;
         continue;
       }
-      const int item = (int)(at / g.kt);
-      g.k0 = (int)(at - (int64_t)item * g.kt);
-      g.k1 = (int)min((int64_t)g.kt, g.k0 + (w1 - w));
-      g.hk = item / mt;
-      g.row0 = (item - g.hk * mt) * M;
+      const int item = (int)(at / span), from = (int)(at - (int64_t)item * span);
+      const int to = (int)min((int64_t)span, from + (w1 - w));  // units of the item; its tiles follow the first COST
+      g.k0 = max(0, from - COST);
+      g.k1 = max(0, to - COST);
+      const int group = item / mt;
+      g.hk = group * a.hw;
+      g.row0 = (item - group * mt) * M;
       g.rows = (int)min((int64_t)M, (int64_t)g.s.n * a.G - g.row0);
-      const bool whole = g.k0 == 0 && g.k1 == g.kt;
-      if (g.k0 == 0 && !whole) {  // the last of this block, and it goes on: who else has some of it
-        const int64_t last = w + g.kt - 1, e = ((last + 1) * N - 1) / W;
-        d0 = make_int4((int)(e - piece + 1), g.s.start, g.row0, g.rows);
-        d1 = make_int4(g.hk, 0, 0, 0);
+      if (g.k1 > g.k0) {
+        const bool whole = g.k0 == 0 && g.k1 == g.kt;
+        if (g.k0 == 0 && !whole) {  // the last of this block, and it goes on: who else has some of it
+          const int64_t last = w - from + span - 1, e = ((last + 1) * N - 1) / W;
+          d0 = make_int4((int)(e - piece + 1), g.s.start, g.row0, g.rows);
+          d1 = make_int4(g.hk, 0, 0, 0);
+        }
+        work(g, whole ? -1 : g.k0 == 0 ? (int)(2 * piece + 1) : (int)(2 * piece));
       }
-      work(g, whole ? -1 : g.k0 == 0 ? (int)(2 * piece + 1) : (int)(2 * piece));
-      w += g.k1 - g.k0;
-      at += g.k1 - g.k0;
+      w += to - from;
+      at += to - from;
     }
   }
   if (threadIdx.x == 0) {
