@@ -48,12 +48,8 @@ constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int CHUNK = 16;           // keys that a warp takes at a time
 constexpr int KT = CHUNK * WARPS;   // keys of a tile
+constexpr int TC_FROM = 16;         // rows of an item above which the tcgen05 kernel takes over
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
   const int bytes = there ? 16 : 0;  // the rest is filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -63,43 +59,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// What a sum with reference m is multiplied by to have reference top.
-__device__ __forceinline__ float factor(float m, float top, float c2) { return m == -INFINITY ? 0.f : ex2((m - top) * c2); }
-
-// ---- which row of the item is which query -----------------------------------------
-
-struct Row {
-  uint64_t bits;
-  int j, h;  // token of the sequence (-1 past the item's rows), head of the group
-};
-__device__ __forceinline__ Row row_of(const Args &a, const Segment &g, int r) {
-  Row x{0, -1, 0};
-  if (r < g.rows) {
-    const int at = g.row0 + r;
-    x.j = at / a.G;
-    x.h = at - x.j * a.G;
-    if (a.mask) x.bits = (uint64_t)a.mask[g.s.start + x.j];
-  }
-  return x;
-}
-// offsets of a row's elements, hk its key head
-__device__ __forceinline__ int64_t q_at(const Args &a, const Segment &g, const Row &x, int hk) {
-  return (int64_t)(g.s.start + x.j) * a.qt + (int64_t)(hk * a.G + x.h) * a.qh;
-}
-__device__ __forceinline__ int64_t out_at(const Args &a, const Segment &g, const Row &x, int hk) {
-  return ((int64_t)(g.s.start + x.j) * a.H + hk * a.G + x.h) * a.c.D;
-}
-
-// ---- fetching chunks -----------------------------------------------------------------
-
-// The page of a key, asked for one chunk ahead.
-__device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key) {
-  return key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
-}
-
 // ---- joining the warps of a block and the blocks of an item ----------------------------
 
 // Warp w has left its sums for key head w % hw at o + w * apart (M rows of `pitch` floats), reference and sum at ml[w].
@@ -152,7 +111,7 @@ __device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int 
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_PIECES = 1024;
 template <typename T, int M, int DP>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
-  wait_for_primary();
+  grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int first_row[JOIN_PIECES + 1];  // rows of the cut items that begin in blocks before c
   __shared__ int warp_rows[JOIN_WARPS];
@@ -571,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
       __syncthreads();
     }
   });
-  launch_dependents();
+  grid_dep_launch();
 }
 
 // ---- CUDA cores ---------------------------------------------------------------------------
@@ -763,26 +722,32 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
       for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
     __syncthreads();
   });
-  launch_dependents();
+  grid_dep_launch();
 }
 
 // ---- choice and launch ---------------------------------------------------------------------
 
 // Which kernel, for how many rows, on how many blocks.  The lengths of the sequences' new tokens are on the device; on
 // average there are T / batch of them.
+enum Kind { CORE, MMA, TC };
 struct Choice {
-  bool mma;
-  int m, dp, hw, pieces;
+  Kind kind;
+  int m, dp, hw, pieces, cost;
   size_t desc, ml, o, total;  // bytes of the workspace
 };
-static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, bool aligned) {
+static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind most) {
   Choice x{};
   const int G = H / c->kv_heads, sms = device_sm_count() > 0 ? device_sm_count() : 148;
   const int64_t rows = (s->T + s->batch - 1) / s->batch * G;
-  x.mma = aligned;
+  x.kind = most == TC && rows <= TC_FROM ? MMA : most;
   x.dp = (c->dim + 31) / 32 * 32;
   x.hw = 1;
-  if (x.mma) {
+  x.cost = 2;
+  if (x.kind == TC) {
+    x.m = CATTN_TC_ROWS;
+    x.pieces = sms;
+    x.cost = 3;
+  } else if (x.kind == MMA) {
     x.m = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     // the warps of a block take neighbouring key heads of the same keys, which lie side by side in memory
     x.hw = c->kv_heads % 4 == 0 ? 4 : c->kv_heads % 2 == 0 ? 2 : 1;
@@ -836,10 +801,15 @@ static cudaError_t with_dp(int dp, F &&f) {
   }
 }
 
-static cudaError_t launch(const Args &a, const Choice &x, bool async, cudaStream_t st) {
+static cudaError_t launch(const Args &a, const Choice &x, const mhc_kv_cache *cache, bool async, cudaStream_t st) {
   return with_dp(x.dp, [&](auto dp) -> cudaError_t {
     constexpr int DP = decltype(dp)::value;
-    if (x.mma) {
+    if (x.kind == TC) {
+      const cudaError_t e = launch_cached_attn_tc(a, cache, st);
+      if (e != cudaSuccess) return e;
+      return a.dtype == MHC_BF16 ? join<__nv_bfloat16, CATTN_TC_ROWS, DP>(a, st) : join<__half, CATTN_TC_ROWS, DP>(a, st);
+    }
+    if (x.kind == MMA) {
       auto go = [&](auto tag, auto r) -> cudaError_t {
         using T = decltype(tag);
         constexpr int R = decltype(r)::value;
@@ -885,9 +855,12 @@ extern "C" {
 
 size_t mhc_cached_attn_workspace(const mhc_kv_cache *cache, const mhc_cache_step *step, int H) {
   if (!cache || !step || step->batch < 1 || cache->kv_heads < 1 || H < 1 || H % cache->kv_heads || cache->dim < 1 || cache->dim > 128) return 0;
-  // for either kernel: which one runs depends on the pointers
-  const size_t a = cattn::choose(cache, step, H, true).total, b = cattn::choose(cache, step, H, false).total;
-  return a > b ? a : b;
+  size_t most = 0;  // for any of the kernels: which one runs depends on the pointers too
+  for (cattn::Kind k : {cattn::CORE, cattn::MMA, cattn::TC}) {
+    const size_t need = cattn::choose(cache, step, H, k).total;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const void *q, int H, const int64_t *q_strides,
@@ -911,17 +884,19 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   if ((uintptr_t)workspace % 256) return fail(MHC_ERR_ALIGN, "%s: workspace must be 256-byte aligned", who);
   const bool async = cattn::rows_aligned(cache);
   const bool mma = async && cache->dtype != MHC_F32 && (uintptr_t)q % 16 == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
-                   (uintptr_t)out % 8 == 0 && !generic_forced();
-  const cattn::Choice x = cattn::choose(cache, step, H, mma);
+                   (uintptr_t)out % 16 == 0 && !generic_forced();
+  const cattn::Choice x = cattn::choose(cache, step, H, !mma ? cattn::CORE : cached_attn_tc_eligible(cache) ? cattn::TC : cattn::MMA);
   a.q = q, a.out = out, a.qt = q_strides[0], a.qh = q_strides[1];
   a.mask = mask, a.H = H, a.G = H / cache->kv_heads;
   a.c2 = (float)((double)scale * 1.4426950408889634);
-  a.pieces = x.pieces, a.hw = x.hw, a.tile = cattn::KT / x.hw, a.dtype = cache->dtype;
+  a.pieces = x.pieces, a.hw = x.hw, a.cost = x.cost, a.dtype = cache->dtype;
+  a.tile = x.kind == cattn::TC ? CATTN_TC_KEYS : cattn::KT / x.hw;
+  a.err_flag = host_error_flag();
   char *ws = static_cast<char *>(workspace);
   a.desc = reinterpret_cast<int4 *>(ws);
   a.part_ml = reinterpret_cast<float2 *>(ws + x.desc);
   a.part_o = reinterpret_cast<float *>(ws + x.desc + x.ml);
-  return cuda_status(cattn::launch(a, x, async, st), who);
+  return cuda_status(cattn::launch(a, x, cache, async, st), who);
 }
 
 }  // extern "C"

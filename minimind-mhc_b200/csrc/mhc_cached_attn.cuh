@@ -1,7 +1,7 @@
 // Attention over a paged cache: arguments, and the cut of the work into equal pieces.
 //
 // The unit of work is a tile of `tile` keys for up to M rows (new tokens x heads of a
-// group) of one sequence and `hw` neighbouring key heads, the item; an item counts COST
+// group) of one sequence and `hw` neighbouring key heads, the item; an item counts some
 // units more, for its beginning and end.  The lengths are known on the device only, so
 // every block sums the units of all sequences itself (a few loads and one warp's scan) and
 // takes its share of the row of all units, [W c / N, W (c + 1) / N): equal work whatever the
@@ -10,6 +10,7 @@
 #pragma once
 
 #include "mhc_cache.cuh"
+#include "mhc_device.cuh"
 
 namespace mhc {
 namespace cattn {
@@ -24,11 +25,13 @@ struct Args {
   float c2;       // scale log2(e)
   int pieces;     // N
   int hw, tile;   // key heads and keys of a unit
+  int cost;       // what an item's beginning (pages, rows and queries, one after the other) and end count, in units
   int dtype;
   // what cut items leave: slot 2 c of block c's first item, 2 c + 1 of its last
   int4 *desc;       // (N, 2)
   float2 *part_ml;  // (2 N, hw M): reference (a score) and sum
   float *part_o;    // (2 N, hw M, DP)
+  int *err_flag;    // registered host word of kernels that give up
 };
 
 struct Segment {
@@ -37,9 +40,6 @@ struct Segment {
   int keys;               // places [0, keys) hold keys
   int k0, k1, kt;         // key tiles of this block, of the item
 };
-
-// An item's beginning (pages, then rows, one after the other; queries) and end take a block about as long as two tiles.
-constexpr int COST = 2;
 
 __device__ __forceinline__ int keys_of(const cache::View &v, const cache::Seq &s) {
   const int64_t l = (int64_t)s.len + s.n;
@@ -70,7 +70,7 @@ struct Cut {
   __device__ __forceinline__ int64_t units(int b) const {
     if (b >= a.c.batch) return 0;
     const cache::Seq s = cache::seq_of(a.c, b);
-    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * (a.c.Hk / a.hw) * (tiles(keys_of(a.c, s)) + COST);
+    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * (a.c.Hk / a.hw) * (tiles(keys_of(a.c, s)) + a.cost);
   }
   // the sequence of unit w < total, and the unit within it; whole warps
   __device__ __forceinline__ void find(int64_t w, int &b, int64_t &at) const {
@@ -104,7 +104,7 @@ __device__ __forceinline__ void walk(const Args &a, F &&work) {
       g.s = cache::seq_of(a.c, b);
       g.keys = keys_of(a.c, g.s);
       g.kt = cut.tiles(g.keys);
-      const int mt = cut.row_tiles(g.s.n), span = g.kt + COST;
+      const int mt = cut.row_tiles(g.s.n), span = g.kt + a.cost;
       const int64_t all = g.s.n == 0 ? 0 : (int64_t)mt * (a.c.Hk / a.hw) * span;
       if (at >= all) {  // the next sequence that has any
         ++b;
@@ -112,9 +112,9 @@ __device__ __forceinline__ void walk(const Args &a, F &&work) {
         continue;
       }
       const int item = (int)(at / span), from = (int)(at - (int64_t)item * span);
-      const int to = (int)min((int64_t)span, from + (w1 - w));  // units of the item; its tiles follow the first COST
-      g.k0 = max(0, from - COST);
-      g.k1 = max(0, to - COST);
+      const int to = (int)min((int64_t)span, from + (w1 - w));  // units of the item; its tiles follow the first a.cost
+      g.k0 = max(0, from - a.cost);
+      g.k1 = max(0, to - a.cost);
       const int group = item / mt;
       g.hk = group * a.hw;
       g.row0 = (item - group * mt) * M;
@@ -154,6 +154,48 @@ __device__ __forceinline__ bool sees(bool masked, uint64_t bits, int j, int c) {
   return c < 0 || (masked ? c < 64 && ((bits >> c) & 1) : c <= j);
 }
 
+// what a sum with reference m is multiplied by to have reference top
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float factor(float m, float top, float c2) { return m == -INFINITY ? 0.f : ex2((m - top) * c2); }
+
+// ---- which row of the item is which query -----------------------------------------
+
+struct Row {
+  uint64_t bits;
+  int j, h;  // token of the sequence (-1 past the item's rows), head of the group
+};
+__device__ __forceinline__ Row row_of(const Args &a, const Segment &g, int r) {
+  Row x{0, -1, 0};
+  if (r < g.rows) {
+    const int at = g.row0 + r;
+    x.j = at / a.G;
+    x.h = at - x.j * a.G;
+    if (a.mask) x.bits = (uint64_t)a.mask[g.s.start + x.j];
+  }
+  return x;
+}
+// offsets of a row's elements, hk its key head
+__device__ __forceinline__ int64_t q_at(const Args &a, const Segment &g, const Row &x, int hk) {
+  return (int64_t)(g.s.start + x.j) * a.qt + (int64_t)(hk * a.G + x.h) * a.qh;
+}
+__device__ __forceinline__ int64_t out_at(const Args &a, const Segment &g, const Row &x, int hk) {
+  return ((int64_t)(g.s.start + x.j) * a.H + hk * a.G + x.h) * a.c.D;
+}
+
+// The page of a key; -1: none
+__device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key) {
+  return key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
+}
+
 }  // namespace cattn
+
+constexpr int CATTN_TC_ROWS = 128, CATTN_TC_KEYS = 128;
+bool cached_attn_tc_eligible(const mhc_kv_cache *c);
+cudaError_t launch_cached_attn_tc(const cattn::Args &a, const mhc_kv_cache *c, cudaStream_t stream);
+int read_cat_error(bool clear);
 
 }  // namespace mhc

@@ -126,6 +126,7 @@ int *host_error_flag();
 int read_selftest_error(bool clear);
 int read_atf_error(bool clear);  // attention forward
 int read_atb_error(bool clear);  // attention backward
+int read_cat_error(bool clear);  // attention over a paged cache
 bool generic_forced();           // MHC_PATH_GENERIC is set
 
 // ---- stand-alone pieces -----------------------------------------------------
