@@ -26,14 +26,14 @@ struct View {
 struct Seq {
   int start, n, len;
 };
-__device__ __forceinline__ Seq seq_of(const View &v, int b) {
+__device__ __forceinline__ Seq seq_between(const View &v, int from, int to, int len) {
   Seq s;
-  const int lo = min(max(v.cu[b], 0), v.T), hi = min(max(v.cu[b + 1], 0), v.T);
-  s.start = lo;
-  s.n = max(hi - lo, 0);
-  s.len = v.lengths[b];
+  s.start = min(max(from, 0), v.T);
+  s.n = max(min(max(to, 0), v.T) - s.start, 0);
+  s.len = len;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const View &v, int b) { return seq_between(v, v.cu[b], v.cu[b + 1], v.lengths[b]); }
 
 // the sequence of row t, or -1: cu[b] <= t < cu[b + 1]
 __device__ __forceinline__ int seq_at(const View &v, int t) {

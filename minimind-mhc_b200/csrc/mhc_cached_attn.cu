@@ -48,6 +48,8 @@ constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int CHUNK = 16;           // keys that a warp takes at a time
 constexpr int KT = CHUNK * WARPS;   // keys of a tile
+// Where the page table has room for so few keys, an item is one block's: nothing is cut and nothing joined.
+constexpr int WHOLE = 512;
 constexpr int TC_FROM = 16;         // rows of an item above which the tcgen05 kernel takes over
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
@@ -107,27 +109,68 @@ __device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int 
 }
 
 // Joins the blocks that had part of a cut item.  Every block lists the cut items (one entry for each block of the first
-// kernel) and takes rows of them in turn; the eight warps share a row's parts, AT_ONCE of them under way in each.
+// kernel); a warp takes one row at a time and goes through its parts, AT_ONCE of them under way.  Where a row has more
+// than a few the block's eight warps share them and join what they have through shared memory.
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_PIECES = 1024;
+constexpr int JOIN_ALONE = 16;  // parts that a warp goes through by itself
+
+template <int DP>
+struct Joined {
+  float o[DP / 32], m = -INFINITY, l = 0.f;
+  // parts begin, begin + step, ... of `count`: part i of the item of block c, row `row` of the `rows` of a slot
+  __device__ __forceinline__ void add(const Args &a, int c, int count, int64_t row, int64_t rows, int begin, int step) {
+    constexpr int PER = DP / 32, AT_ONCE = 4;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = 0.f;
+    for (int i0 = begin; i0 < count; i0 += step * AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float x[AT_ONCE][PER];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * step;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (i < count) {
+          // the item's first block's last slot, then the first slots of the blocks behind it
+          const int64_t at = (i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i)) * rows + row;
+          ml[u] = a.part_ml[at];
+#pragma unroll
+          for (int k = 0; k < PER; ++k) x[u][k] = a.part_o[at * DP + lane + 32 * k];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        if (ml[u].x == -INFINITY) continue;  // nothing was seen there (or there is no such part)
+        const float top = fmaxf(m, ml[u].x), f = factor(m, top, a.c2), g = factor(ml[u].x, top, a.c2);
+        m = top;
+        l = fmaf(l, f, ml[u].y * g);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o[k] = fmaf(o[k], f, x[u][k] * g);
+      }
+    }
+  }
+};
+
 template <typename T, int M, int DP>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int first_row[JOIN_PIECES + 1];  // rows of the cut items that begin in blocks before c
+  __shared__ int parts[JOIN_PIECES];
   __shared__ int warp_rows[JOIN_WARPS];
   __shared__ float st_m[JOIN_WARPS], st_l[JOIN_WARPS];
   __shared__ float st_o[JOIN_WARPS][DP];
   constexpr int LIST = JOIN_PIECES / JOIN_THREADS;
-  int mine[LIST], sum = 0;
+  int mine[LIST], sum = 0, most = 0;
 #pragma unroll
   for (int i = 0; i < LIST; ++i) {
     const int c = threadIdx.x * LIST + i;
-    mine[i] = 0;
-    if (c < a.pieces) {
-      const int4 d = a.desc[2 * c];
-      if (d.x > 0) mine[i] = d.w * a.hw;
-    }
+    int4 d = make_int4(0, 0, 0, 0);
+    if (c < a.pieces) d = a.desc[c];
+    mine[i] = d.x > 0 ? (d.w & 255) * a.hw : 0;
+    parts[c] = d.x;
     sum += mine[i];
+    most = max(most, d.x);
   }
   int inc = sum;
 #pragma unroll
@@ -136,7 +179,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
     if (lane >= o) inc += up;
   }
   if (lane == 31) warp_rows[warp] = inc;
-  __syncthreads();
+  const bool shared_out = __syncthreads_or(most > JOIN_ALONE);
   int at = inc - sum, total = 0;
 #pragma unroll
   for (int w = 0; w < JOIN_WARPS; ++w) {
@@ -151,66 +194,67 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   if (threadIdx.x == 0) first_row[JOIN_PIECES] = total;
   __syncthreads();
   constexpr int PER = DP / 32;
-  for (int task = blockIdx.x; task < total; task += gridDim.x) {
+  auto block_of = [&](int task) {  // the last block whose rows begin at or before it
     int c = 0;
 #pragma unroll
     for (int step = JOIN_PIECES / 2; step; step >>= 1)
-      if (first_row[c + step] <= task) c += step;  // the last block whose rows begin at or before it
-    const int4 d0 = a.desc[2 * c];
-    const int count = d0.x, local = task - first_row[c], head = local / d0.w, r = local - head * d0.w;
-    const int64_t row = (int64_t)head * M + r, rows = (int64_t)a.hw * M;
-    float o[PER], m = -INFINITY, l = 0.f;
+      if (first_row[c + step] <= task) c += step;
+    return c;
+  };
+  // row and place in `out` of row `local` of the item that begins in block c
+  auto row_at = [&](int c, int local, int64_t &row) -> T * {
+    const int4 d = a.desc[c];
+    const int n = d.w & 255, head = local / n, r = local - head * n;
+    row = (int64_t)head * M + r;
+    const int at = d.z + r, j = at / a.G;
+    return static_cast<T *>(a.out) + ((int64_t)(d.y + j) * a.H + ((d.w >> 8) + head) * a.G + (at - j * a.G)) * a.c.D;
+  };
+  const int64_t rows = (int64_t)a.hw * M;
+  // neighbouring rows to different blocks: the few rows of long items keep many blocks busy
+  for (int base = blockIdx.x; base < total; base += gridDim.x * JOIN_WARPS) {
+    const int task = base + warp * gridDim.x;
+    if (task < total) {
+      const int c = block_of(task);
+      if (parts[c] <= JOIN_ALONE) {
+        int64_t row;
+        T *out = row_at(c, task - first_row[c], row);
+        Joined<DP> s;
+        s.add(a, c, parts[c], row, rows, 0, 1);
+        const float scale = 1.f / s.l;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) o[k] = 0.f;
-    // part i of the item: its first block's last slot, then the first slots of the blocks behind it
-    auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i); };
-    constexpr int AT_ONCE = 4;
-    for (int i0 = warp; i0 < count; i0 += JOIN_WARPS * AT_ONCE) {
-      float2 ml[AT_ONCE];
-      float x[AT_ONCE][PER];
+        for (int k = 0; k < PER; ++k)
+          if (lane + 32 * k < a.c.D) out[lane + 32 * k] = from_f<T>(s.m == -INFINITY ? 0.f : s.o[k] * scale);
+      }
+    }
+    if (!shared_out) continue;
+    for (int i = 0; i < JOIN_WARPS && base + i * gridDim.x < total; ++i) {
+      const int task = base + i * gridDim.x, c = block_of(task);
+      if (parts[c] <= JOIN_ALONE) continue;
+      int64_t row;
+      T *out = row_at(c, task - first_row[c], row);
+      Joined<DP> s;
+      s.add(a, c, parts[c], row, rows, warp, JOIN_WARPS);
+      if (lane == 0) {
+        st_m[warp] = s.m;
+        st_l[warp] = s.l;
+      }
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = i0 + u * JOIN_WARPS;
-        ml[u] = make_float2(-INFINITY, 0.f);
-        if (i < count) {
-          const int64_t at_row = slot(i) * rows + row;
-          ml[u] = a.part_ml[at_row];
+      for (int k = 0; k < PER; ++k) st_o[warp][lane + 32 * k] = s.o[k];
+      __syncthreads();
+      if (threadIdx.x < DP && threadIdx.x < a.c.D) {
+        float top = -INFINITY, l = 0.f, y = 0.f;
 #pragma unroll
-          for (int k = 0; k < PER; ++k) x[u][k] = a.part_o[at_row * DP + lane + 32 * k];
+        for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, st_m[w]);
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) {
+          const float f = factor(st_m[w], top, a.c2);
+          l = fmaf(f, st_l[w], l);
+          y = fmaf(f, st_o[w][threadIdx.x], y);
         }
+        out[threadIdx.x] = from_f<T>(top == -INFINITY ? 0.f : y * (1.f / l));
       }
-#pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        if (ml[u].x == -INFINITY) continue;  // nothing was seen there (or there is no such part)
-        const float top = fmaxf(m, ml[u].x), f = factor(m, top, a.c2), g = factor(ml[u].x, top, a.c2);
-        m = top;
-        l = fmaf(l, f, ml[u].y * g);
-#pragma unroll
-        for (int k = 0; k < PER; ++k) o[k] = fmaf(o[k], f, x[u][k] * g);
-      }
+      __syncthreads();
     }
-    if (lane == 0) {
-      st_m[warp] = m;
-      st_l[warp] = l;
-    }
-#pragma unroll
-    for (int k = 0; k < PER; ++k) st_o[warp][lane + 32 * k] = o[k];
-    __syncthreads();
-    if (threadIdx.x < DP && threadIdx.x < a.c.D) {
-      float top = -INFINITY, sum = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, st_m[w]);
-#pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float f = factor(st_m[w], top, a.c2);
-        sum = fmaf(f, st_l[w], sum);
-        y = fmaf(f, st_o[w][threadIdx.x], y);
-      }
-      const int row_at = d0.z + r, j = row_at / a.G, hk = a.desc[2 * c + 1].x + head;
-      T *out = static_cast<T *>(a.out) + ((int64_t)(d0.y + j) * a.H + hk * a.G + (row_at - j * a.G)) * a.c.D;
-      out[threadIdx.x] = from_f<T>(top == -INFINITY ? 0.f : y * (1.f / sum));
-    }
-    __syncthreads();
   }
 }
 
@@ -281,6 +325,7 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
   __shared__ uint32_t have[WARPS][S::STAGES];  // which keys of a chunk exist
+  __shared__ Near near;
   __shared__ Row rows[M];
   __shared__ float2 ml[WARPS][M];
   __shared__ float fac[WARPS][M];
@@ -294,10 +339,11 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
   const float ahead = AHEAD / a.c2;
   if (D < DP)
     for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  near.fill(a);
   clear_rest<T>(a);
   __syncthreads();
 
-  walk<M>(a, [&](const Segment &g, int slot) {
+  walk<M>(a, near, [&](const Segment &g, int slot) {
     const int hk = g.hk + head;
     const T *kbase = static_cast<const T *>(a.c.keys) + hk * a.c.kh, *vbase = static_cast<const T *>(a.c.values) + hk * a.c.vh;
     const int chunks = g.k1 - g.k0;
@@ -381,7 +427,8 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
     }
     for (int i = 0; i < chunks; ++i) {
       cp_wait<S::STAGES - 2>();
-      __syncwarp();
+      __syncwarp();  // for all lanes, and the chunk before has been read
+      fetch(i + S::STAGES - 1);
       const int st = i % S::STAGES, key = key0 + i * a.tile;
       const uint32_t kt = ring + st * S::STAGE, vt = kt + CHUNK * S::PITCH;
       const uint32_t got = have[warp][st];
@@ -501,8 +548,6 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
           }
         }
       }
-      __syncwarp();  // the chunk has been read
-      fetch(i + S::STAGES - 1);
     }
     cp_wait<0>();
     __syncwarp();
@@ -560,16 +605,18 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
   float *ps = qs + R * DP + (threadIdx.x >> 5) * CHUNK * R;  // (CHUNK, R); below 0: not seen
   __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
   __shared__ uint32_t have[WARPS][S::STAGES];
+  __shared__ Near near;
   __shared__ Row rows[R];
   __shared__ float2 ml[WARPS][R];
   __shared__ float fac[WARPS][R];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.D;
   const float ahead = 8.f / a.c2;
   for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
+  near.fill(a);
   clear_rest<T>(a);
   __syncthreads();
 
-  walk<R>(a, [&](const Segment &g, int slot) {
+  walk<R>(a, near, [&](const Segment &g, int slot) {
     for (int r = tid; r < R; r += THREADS) rows[r] = row_of(a, g, r);
     __syncthreads();
     for (int i = tid; i < R * DP; i += THREADS) {
@@ -628,7 +675,8 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
     const int col = SPLIT == 1 ? lane * 4 : (lane % (32 / SPLIT)) * 4, share = SPLIT == 1 ? 0 : lane / (32 / SPLIT);
     for (int i = 0; i < chunks; ++i) {
       cp_wait<S::STAGES - 2>();
-      __syncwarp();
+      __syncwarp();  // for all lanes, and the chunk before has been read
+      fetch(i + S::STAGES - 1);
       const int st = i % S::STAGES, key = key0 + i * KT;
       const float *kt = ring + st * S::STAGE, *vt = kt + CHUNK * S::KP;
       const uint32_t got = have[warp][st];
@@ -699,8 +747,7 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
           }
         }
       }
-      __syncwarp();  // the chunk and P have been read
-      fetch(i + S::STAGES - 1);
+      __syncwarp();  // P has been read
     }
     cp_wait<0>();
     __syncwarp();
@@ -733,6 +780,7 @@ enum Kind { CORE, MMA, TC };
 struct Choice {
   Kind kind;
   int m, dp, hw, pieces, cost;
+  bool whole;
   size_t desc, ml, o, total;  // bytes of the workspace
 };
 static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind most) {
@@ -743,14 +791,15 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
   x.dp = (c->dim + 31) / 32 * 32;
   x.hw = 1;
   x.cost = 2;
+  x.whole = (int64_t)s->table_width * c->page_size <= WHOLE;
   if (x.kind == TC) {
     x.m = CATTN_TC_ROWS;
-    x.pieces = sms;
-    x.cost = 3;
+    x.pieces = sms * CATTN_TC_BLOCKS;
+    x.cost = 7;
   } else if (x.kind == MMA) {
     x.m = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     // the warps of a block take neighbouring key heads of the same keys, which lie side by side in memory
-    x.hw = c->kv_heads % 4 == 0 ? 4 : c->kv_heads % 2 == 0 ? 2 : 1;
+    if (!x.whole) x.hw = c->kv_heads % 4 == 0 ? 4 : c->kv_heads % 2 == 0 ? 2 : 1;
     x.pieces = sms * (x.m == 32 ? 2 : x.dp >= 128 ? 3 : 4);
   } else {
     x.m = rows <= 4 ? 4 : 16;
@@ -759,7 +808,7 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
   if (x.pieces > JOIN_PIECES) x.pieces = JOIN_PIECES;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
   const size_t rows_kept = (size_t)x.pieces * 2 * x.hw * x.m;
-  x.desc = up((size_t)x.pieces * 2 * sizeof(int4));
+  x.desc = up((size_t)x.pieces * sizeof(int4));
   x.ml = up(rows_kept * sizeof(float2));
   x.o = up(rows_kept * x.dp * sizeof(float));
   x.total = x.desc + x.ml + x.o;
@@ -777,6 +826,7 @@ static cudaError_t start(K kernel, const Args &a, int blocks, int smem, cudaStre
 // the join begins while the last blocks of the first kernel still run, and waits for them on the device
 template <typename T, int M, int DP>
 static cudaError_t join(const Args &a, cudaStream_t st) {
+  if (a.whole) return cudaSuccess;
   cudaLaunchConfig_t cfg{};
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
   const int64_t rows = (int64_t)a.c.T * a.H;
@@ -889,9 +939,12 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   a.q = q, a.out = out, a.qt = q_strides[0], a.qh = q_strides[1];
   a.mask = mask, a.H = H, a.G = H / cache->kv_heads;
   a.c2 = (float)((double)scale * 1.4426950408889634);
-  a.pieces = x.pieces, a.hw = x.hw, a.cost = x.cost, a.dtype = cache->dtype;
+  a.pieces = x.pieces, a.hw = x.hw, a.groups = a.c.Hk / x.hw, a.cost = x.cost, a.whole = x.whole, a.dtype = cache->dtype;
   a.tile = x.kind == cattn::TC ? CATTN_TC_KEYS : cattn::KT / x.hw;
   a.err_flag = host_error_flag();
+  // an upper bound of the units of all sequences
+  const double units = ((double)step->T * a.G / x.m + step->batch) * a.groups * ((double)a.c.capacity / a.tile + 1 + x.cost);
+  if (units > 2e9) return fail(MHC_ERR_SHAPE, "%s: %lld tokens over up to %d keys are more than one call takes", who, (long long)step->T, a.c.capacity);
   char *ws = static_cast<char *>(workspace);
   a.desc = reinterpret_cast<int4 *>(ws);
   a.part_ml = reinterpret_cast<float2 *>(ws + x.desc);

@@ -4,8 +4,8 @@
 // group) of one sequence and `hw` neighbouring key heads, the item; an item counts some
 // units more, for its beginning and end.  The lengths are known on the device only, so
 // every block sums the units of all sequences itself (a few loads and one warp's scan) and
-// takes its share of the row of all units, [W c / N, W (c + 1) / N): equal work whatever the
-// lengths.  An item that lies in one block is finished there; of one that is cut the blocks
+// takes its share of the row of all units, W / N of them and the first W % N blocks one more:
+// equal work whatever the lengths.  An item that lies in one block is finished there; of one that is cut the blocks
 // leave their sums, references and rows, which a second kernel joins, in the blocks' order.
 #pragma once
 
@@ -25,10 +25,12 @@ struct Args {
   float c2;       // scale log2(e)
   int pieces;     // N
   int hw, tile;   // key heads and keys of a unit
+  int groups;     // Hk / hw
+  int whole;      // items are not cut: a block takes those that begin in its share
   int cost;       // what an item's beginning (pages, rows and queries, one after the other) and end count, in units
   int dtype;
   // what cut items leave: slot 2 c of block c's first item, 2 c + 1 of its last
-  int4 *desc;       // (N, 2)
+  int4 *desc;       // (N): of the item that begins in block c and ends in another: parts, first new token, first row, rows + 256 key head
   float2 *part_ml;  // (2 N, hw M): reference (a score) and sum
   float *part_o;    // (2 N, hw M, DP)
   int *err_flag;    // registered host word of kernels that give up
@@ -46,20 +48,39 @@ __device__ __forceinline__ int keys_of(const cache::View &v, const cache::Seq &s
   return (int)max((int64_t)0, min(l, (int64_t)v.capacity));
 }
 
+// The step's offsets and lengths in shared memory, where they are few: every warp looks them up for every item.
+constexpr int NEAR = 128;
+struct Near {
+  int cu[NEAR + 1], len[NEAR];
+  // by all threads of the block; a barrier has to follow
+  __device__ __forceinline__ void fill(const Args &a) {
+    if (a.c.batch > NEAR) return;
+    for (int i = threadIdx.x; i <= a.c.batch; i += blockDim.x) {
+      cu[i] = a.c.cu[i];
+      if (i < a.c.batch) len[i] = a.c.lengths[i];
+    }
+  }
+  __device__ __forceinline__ cache::Seq at(const Args &a, int b) const {
+    if (a.c.batch > NEAR) return cache::seq_of(a.c, b);
+    return cache::seq_between(a.c, cu[b], cu[b + 1], len[b]);
+  }
+};
+
 template <int M>
 struct Cut {
   const Args &a;
-  int64_t first, sum, total;  // units before this lane's sequences, of them, of all
+  const Near &near;
+  int first, sum, total;      // units before this lane's sequences, of them, of all
   int per;                    // sequences of a lane
-  __device__ __forceinline__ Cut(const Args &args) : a(args) {
+  __device__ __forceinline__ Cut(const Args &args, const Near &steps) : a(args), near(steps) {
     const int lane = threadIdx.x & 31;
     per = (a.c.batch + 31) / 32;
     sum = 0;
     for (int i = 0; i < per; ++i) sum += units(lane * per + i);
-    int64_t inc = sum;
+    int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += up;
     }
     first = inc - sum;
@@ -67,54 +88,56 @@ struct Cut {
   }
   __device__ __forceinline__ int tiles(int keys) const { return max(1, (keys + a.tile - 1) / a.tile); }
   __device__ __forceinline__ int row_tiles(int n) const { return (int)(((int64_t)n * a.G + M - 1) / M); }
-  __device__ __forceinline__ int64_t units(int b) const {
+  __device__ __forceinline__ int units(int b) const {
     if (b >= a.c.batch) return 0;
-    const cache::Seq s = cache::seq_of(a.c, b);
-    return s.n == 0 ? 0 : (int64_t)row_tiles(s.n) * (a.c.Hk / a.hw) * (tiles(keys_of(a.c, s)) + a.cost);
+    const cache::Seq s = near.at(a, b);
+    return s.n == 0 ? 0 : row_tiles(s.n) * a.groups * (tiles(keys_of(a.c, s)) + a.cost);
   }
   // the sequence of unit w < total, and the unit within it; whole warps
-  __device__ __forceinline__ void find(int64_t w, int &b, int64_t &at) const {
+  __device__ __forceinline__ void find(int w, int &b, int &at) const {
     const int lane = threadIdx.x & 31;
     const unsigned has = __ballot_sync(0xffffffffu, w >= first && w < first + sum);
     const int owner = __ffs(has) - 1;
     int mine = lane * per;
-    int64_t left = w - first;
+    int left = w - first;
     if (lane == owner)
-      for (int64_t u; left >= (u = units(mine)); ++mine) left -= u;
+      for (int u; left >= (u = units(mine)); ++mine) left -= u;
     b = __shfl_sync(0xffffffffu, mine, owner);
     at = __shfl_sync(0xffffffffu, left, owner);
   }
 };
 
-// Runs `work(segment, slot)` over block blockIdx.x's units: slot < 0 where the item is whole.
+// Runs `work(segment, slot)` over block blockIdx.x's units: slot < 0 where the item is not cut.
 // Writes the block's entry of the join's table.
 template <int M, typename F>
-__device__ __forceinline__ void walk(const Args &a, F &&work) {
-  const Cut<M> cut(a);
-  const int64_t W = cut.total, N = min((int64_t)a.pieces, W), piece = blockIdx.x;
-  int4 d0 = make_int4(0, 0, 0, 0), d1 = d0;
+__device__ __forceinline__ void walk(const Args &a, const Near &near, F &&work) {
+  const Cut<M> cut(a, near);
+  // (the host has seen to it that 32 bits hold the units of any lengths)
+  const int W = cut.total, N = min(a.pieces, W), piece = blockIdx.x;
+  int4 entry = make_int4(0, 0, 0, 0);
   if (piece < N) {
-    const int64_t w1 = W * (piece + 1) / N;
-    int64_t w = W * piece / N, at;
-    int b;
+    const int each = W / N, more = W - each * N;
+    const int w1 = each * (piece + 1) + min(piece + 1, more);
+    int w = each * piece + min(piece, more), at, b;
     cut.find(w, b, at);
     while (w < w1) {
       Segment g;
       g.b = b;
-      g.s = cache::seq_of(a.c, b);
+      g.s = near.at(a, b);
       g.keys = keys_of(a.c, g.s);
       g.kt = cut.tiles(g.keys);
       const int mt = cut.row_tiles(g.s.n), span = g.kt + a.cost;
-      const int64_t all = g.s.n == 0 ? 0 : (int64_t)mt * (a.c.Hk / a.hw) * span;
+      const int all = g.s.n == 0 ? 0 : mt * a.groups * span;
       if (at >= all) {  // the next sequence that has any
         ++b;
         at = 0;
         continue;
       }
-      const int item = (int)(at / span), from = (int)(at - (int64_t)item * span);
-      const int to = (int)min((int64_t)span, from + (w1 - w));  // units of the item; its tiles follow the first a.cost
+      const int item = at / span, from = at - item * span;
+      // units of the item; its tiles follow the first a.cost
+      const int to = a.whole ? span : min(span, from + (w1 - w));
       g.k0 = max(0, from - a.cost);
-      g.k1 = max(0, to - a.cost);
+      g.k1 = a.whole && from > 0 ? g.k0 : max(0, to - a.cost);
       const int group = item / mt;
       g.hk = group * a.hw;
       g.row0 = (item - group * mt) * M;
@@ -122,20 +145,17 @@ __device__ __forceinline__ void walk(const Args &a, F &&work) {
       if (g.k1 > g.k0) {
         const bool whole = g.k0 == 0 && g.k1 == g.kt;
         if (g.k0 == 0 && !whole) {  // the last of this block, and it goes on: who else has some of it
-          const int64_t last = w - from + span - 1, e = ((last + 1) * N - 1) / W;
-          d0 = make_int4((int)(e - piece + 1), g.s.start, g.row0, g.rows);
-          d1 = make_int4(g.hk, 0, 0, 0);
+          const int last = w - from + span - 1, longer = more * (each + 1);
+          const int e = last < longer ? last / (each + 1) : more + (last - longer) / each;
+          entry = make_int4(e - piece + 1, g.s.start, g.row0, g.rows + 256 * g.hk);
         }
-        work(g, whole ? -1 : g.k0 == 0 ? (int)(2 * piece + 1) : (int)(2 * piece));
+        work(g, whole ? -1 : g.k0 == 0 ? 2 * piece + 1 : 2 * piece);
       }
       w += to - from;
       at += to - from;
     }
   }
-  if (threadIdx.x == 0) {
-    a.desc[2 * piece] = d0;
-    a.desc[2 * piece + 1] = d1;
-  }
+  if (threadIdx.x == 0 && !a.whole) a.desc[piece] = entry;
 }
 
 // rows of no sequence get 0
@@ -193,7 +213,7 @@ __device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key)
 
 }  // namespace cattn
 
-constexpr int CATTN_TC_ROWS = 128, CATTN_TC_KEYS = 128;
+constexpr int CATTN_TC_ROWS = 128, CATTN_TC_KEYS = 64, CATTN_TC_BLOCKS = 2;  // rows of an item, keys of a tile, blocks of an SM
 bool cached_attn_tc_eligible(const mhc_kv_cache *c);
 cudaError_t launch_cached_attn_tc(const cattn::Args &a, const mhc_kv_cache *c, cudaStream_t stream);
 int read_cat_error(bool clear);

@@ -1,26 +1,28 @@
 // Attention over a paged cache on the 5th-generation tensor cores, for items of more rows
 // than the warp-wide products of mhc_cached_attn.cu take at once (bf16 / fp16; pages that
-// divide a tile of 128 keys or are made of such tiles).
+// divide a tile of 64 keys or are made of such tiles).
 //
-//   S = Q K^T    tcgen05.mma, M = N = 128, K = D, both operands in shared memory
+//   S = Q K^T    tcgen05.mma, M = 128, N = 64, K = D, both operands in shared memory
 //   P = exp2((S - m) c)                         c = scale log2(e), one thread per row
 //   O += P V     A = P from TMEM (it replaces S there), B = V as it lies in memory
 //
-// The rows are those of one item, up to 128 new tokens x heads of a group.  A step (S,
-// softmax, O) is a chain of waits; two of them run side by side: the key tiles of an item
-// go in turn to two sets of four softmax warps with scores, sums and O of their own, over
-// the same queries, and the tensor core serves one while the other's softmax runs.  In the
-// end the two O lie in TMEM in the same lanes, so each set joins half of the columns of
-// both without moving them; only references and sums cross through shared memory.
+// The rows are those of one item, up to 128 new tokens x heads of a group.  A step (scores,
+// softmax, product) is a chain of waits, an item begins with three loads one after another
+// (lengths, pages and rows; queries), and ends with O's way out: two blocks run on an SM, each
+// with half of TMEM and of shared memory, so that one works while the other waits.  (One
+// block with tiles of 128 keys and two sets of softmax warps, the key tiles in turn, took
+// 1.5 us a tile and 14 us for an item's two ends.)  Scores are formed one tile ahead, into the
+// other of two buffers.
 //
-// K and V come by TMA, one box for each page and 64 columns of a tile, the lanes of a
-// warp one page each, two or more tiles ahead, across the ends of items too.  V rows that do
+// K and V come by TMA, one box for each page and 64 columns of a tile of 64 keys, the lanes
+// of a warp one page each, across the ends of items too.  V rows that do
 // not exist are zeroed in shared memory (a P of 0 times a NaN would be NaN), and so are
 // infinities and NaN of new tokens' V, which some rows of the item do not see: the rows
-// that see one add it in the end.
+// that see one add it in the end.  The softmax threads do that, a row each, before they hand
+// over P.
 //
-// Warps 0-3 and 4-7: the two softmax sets; 8: TMA; 9: MMA issue.  Every wait is bounded; a
-// block whose wait runs out writes NaN over its share.
+// Warps 0-3: softmax, a row each; 4: TMA; 5: MMA issue.  Every wait is bounded; a block whose
+// wait runs out writes NaN over its share.
 #include <cfloat>
 #include <mutex>
 
@@ -38,32 +40,50 @@ namespace {
 using namespace sm100;
 using attn::BLK;
 using attn::TM;
-using attn::Tile;
 using attn::idesc_of;
-using attn::mma_rows;
-using attn::mma_sum;
 using attn::pack2;
 using attn::wait_warp_parity;
 
-constexpr int NTHREADS = 320;
-constexpr int W_TMA = 8, W_MMA = 9;
-constexpr int TMEM_COLS = 512;
-constexpr uint32_t S_COL = 0, O_COL = 256;  // two score tiles, two results, 128 columns each
+constexpr int TN = CATTN_TC_KEYS;
+constexpr uint32_t KBLK = TN * 128;  // 64 keys x 64 values of 16 bits, 128-byte swizzle
+constexpr int NTHREADS = 192;
+constexpr int W_TMA = 4, W_MMA = 5;
+constexpr int TMEM_COLS = 256;
+constexpr uint32_t S_COL = 0, O_COL = 128;  // two score tiles of 64 columns; the result
 enum { ERR_TMA = 61, ERR_MMA = 62, ERR_SOFTMAX = 63 };
-constexpr int ODD = 8;  // items whose odd values are remembered: more than the TMA warp can be ahead
 
 template <int DP>
 struct Cfg {
-  using L = Tile<DP, false>;
-  static constexpr uint32_t TILE = L::BYTES;
-  static constexpr int ST = DP <= 64 ? 6 : 3;  // stages of K and of V
-  static constexpr size_t SMEM = TILE + 2 * ST * TILE + 1024;
+  static constexpr int FULL = (DP + 63) / 64;  // blocks of 64 columns, filled up with zeros
+  static constexpr uint32_t Q = FULL * BLK, TILE = FULL * KBLK;
+  static constexpr int ST = DP <= 64 ? 5 : 2;  // stages of K and of V
+  static constexpr size_t SMEM = Q + 2 * ST * TILE + 1024;
 };
 
-constexpr int B_QF = 0, B_LAND = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_DRAIN = 8, B_KF = 9;
+constexpr int B_QF = 0, B_DRAIN = 1, B_SF = 2, B_PF = 4, B_OF = 6, B_KF = 8;
 // then ST each: KF, KE, VF, VE
 
-// Tensor maps of keys and values: (D, slots and heads by their strides, pages) in boxes of one page's rows (128 at most) x 64
+// S [128 x 64] = Q K^T over DP columns
+template <int DP>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t idesc) {
+  const uint64_t ad = umma_desc_sw128(q), bd = umma_desc_sw128(k);
+  if (elect_one()) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      umma_bf16(d, ad + ((uint64_t)((kk >> 2) * (int)BLK + (kk & 3) * 32) >> 4), bd + ((uint64_t)((kk >> 2) * (int)KBLK + (kk & 3) * 32) >> 4),
+                idesc, kk > 0);
+  }
+}
+// O [128 x DP] (+)= P V: P in TMEM, 32 keys in 16 columns; V's rows are the summed index
+__device__ __forceinline__ void mma_product(uint32_t d, uint32_t p, uint32_t v, uint32_t idesc, bool begin) {
+  const uint64_t bd = umma_desc(v, KBLK, 1024, 2);
+  if (elect_one()) {
+#pragma unroll
+    for (int kk = 0; kk < TN / 16; ++kk) umma_f16_ts(d, p + kk * 8u, bd + kk * (2048 >> 4), idesc, !begin || kk > 0);
+  }
+}
+
+// Tensor maps of keys and values: (D, slots and heads by their strides, pages) in boxes of one page's rows (64 at most) x 64
 // columns; head_first: the second axis is the head.
 struct Maps {
   CUtensorMap k, v;
@@ -80,13 +100,19 @@ __device__ __forceinline__ void give_up(int code, volatile int *abort_flag, int 
   *abort_flag = 1;
   report_give_up(&g_cat_error, err_flag, code);
 }
-// the softmax threads only
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 template <typename T>
 __device__ __forceinline__ bool finite16(uint16_t w) {
   constexpr uint16_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7f80 : 0x7c00;
   return (w & E) != E;
+}
+
+// two values with zeros in the place of infinities and NaN
+template <typename T>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  constexpr uint32_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  if ((w & E) == E) w &= 0xffff0000u;
+  if ((w & (E << 16)) == (E << 16)) w &= 0xffffu;
+  return w;
 }
 
 // the 32 columns from `base` on that a row sees: keys that exist, of the context or among its new tokens
@@ -103,9 +129,9 @@ __device__ __forceinline__ uint32_t seen_columns(const Args &a, const Segment &g
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(NTHREADS, CATTN_TC_BLOCKS)
+cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
   using C = Cfg<DP>;
-  using L = typename C::L;
   constexpr int ST = C::ST, M = CATTN_TC_ROWS;
   constexpr int B_KE = B_KF + ST, B_VF = B_KE + ST, B_VE = B_VF + ST, NBARS = B_VE + ST;
   constexpr float LAZY = std::is_same<T, __half>::value ? 4.f : 8.f, LIFT = std::is_same<T, __half>::value ? 10.f : 0.f;
@@ -113,28 +139,25 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
   __shared__ __align__(8) uint64_t bars[NBARS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  __shared__ volatile int odd_item[ODD];  // item i + 1 where item i has odd values among its new tokens' V
+  __shared__ volatile int odd_item;  // the block's last item that had infinities or NaN among its new tokens' V
+  __shared__ Near near;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *gen = smem_raw + (base - raw);
-  // references and sums of both sets, where the queries lie: their last product is done by then
-  float2(*sums)[TM] = reinterpret_cast<float2(*)[TM]>(gen);
-  const uint32_t qs = base, ks = qs + C::TILE, vs = ks + ST * C::TILE;
+  const uint32_t qs = base, ks = qs + C::Q, vs = ks + ST * C::TILE;
   volatile int *abort_flag = &abort_word;
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   if (tid == 0) {
-    abort_word = 0;
-    for (int i = 0; i < ODD; ++i) odd_item[i] = 0;
+    abort_word = odd_item = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(B_SF + i), 1);
       mbar_init(BAR(B_PF + i), 128);
       mbar_init(BAR(B_OF + i), 1);
     }
-    mbar_init(BAR(B_QF), 256);
-    mbar_init(BAR(B_LAND), 1);
+    mbar_init(BAR(B_QF), 128);
     mbar_init(BAR(B_DRAIN), 1);
     for (int i = 0; i < ST; ++i) {
       mbar_init(BAR(B_KF + i), 1);
@@ -148,6 +171,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
     tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
+  near.fill(a);
   clear_rest<T>(a);
   tc_fence_before();
   __syncthreads();
@@ -157,66 +181,31 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
   if (warp == W_TMA) {
     // ---------------- TMA: a lane for each page of a tile ----------------
     bool ok = true;
-    int t = 0, nk = 0, nv = 0, lands = 0, items = 0;  // key tiles, K and V tiles asked for, V tiles looked through, items so far
-    const int rows = min(a.c.size, TM), boxes = TM / rows;  // of a box, in a tile
-    walk<M>(a, [&](const Segment &g, int) {
-      const int item = items++;
+    int t = 0, nk = 0, nv = 0;  // key tiles, K and V tiles asked for so far
+    const int rows = min(a.c.size, TN), boxes = TN / rows;  // of a box, in a tile
+    walk<M>(a, near, [&](const Segment &g, int) {
       if (!ok) return;
       for (int j = g.k0; j < g.k1; ++j, ++t) {
-        const int s = t % ST, key = j * TM + lane * rows;
+        const int s = t % ST, key = j * TN + lane * rows;
         const uint32_t free_par = ((uint32_t)(t / ST) & 1u) ^ 1u;
         int page = lane < boxes ? page_of(a, g, key) : -1;
         if (page >= a.c.pages) page = -1;
         const int slot = page >= 0 ? key - cache::page_index(a.c, key) * a.c.size : 0;
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-        const uint32_t bytes = (uint32_t)(__popc(there) * rows * 128) * L::FULL;
+        const uint32_t bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, page >= 0)) * rows * 128) * C::FULL;
         auto load = [&](uint32_t dst, const CUtensorMap &map, int head_first, uint32_t bar) {
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
           if (page >= 0)
 #pragma unroll
-            for (int b = 0; b < L::FULL; ++b)
-              tma_load_4d(dst + b * BLK + lane * rows * 128, &map, b * 64, head_first ? g.hk : slot, head_first ? slot : g.hk, page, bar);
+            for (int b = 0; b < C::FULL; ++b)
+              tma_load_4d(dst + b * KBLK + lane * rows * 128, &map, b * 64, head_first ? g.hk : slot, head_first ? slot : g.hk, page, bar);
         };
         if (!wait_warp_parity(BAR(B_KE + s), free_par, abort_flag)) { ok = false; break; }
         load(ks + s * C::TILE, maps.k, maps.k_head_first, BAR(B_KF + s));
         nk = t + 1;
         if (!wait_warp_parity(BAR(B_VE + s), free_par, abort_flag)) { ok = false; break; }
-        const int end = (j + 1) * TM;
-        const bool gaps = g.keys < end || there != (boxes == 32 ? 0xffffffffu : (1u << boxes) - 1), fresh = (g.s.n > 1 || a.mask) && g.s.len < end;
-        load(vs + s * C::TILE, maps.v, maps.v_head_first, BAR(gaps || fresh ? B_LAND : B_VF + s));
+        load(vs + s * C::TILE, maps.v, maps.v_head_first, BAR(B_VF + s));
         nv = t + 1;
-        if (gaps || fresh) {
-          if (!wait_warp_parity(BAR(B_LAND), (uint32_t)lands & 1u, abort_flag)) ok = false;
-          ++lands;
-          uint8_t *tile = gen + (vs - base) + s * C::TILE;
-          bool odd = false;
-          for (int i = lane; i < TM * L::FULL * 8; i += 32) {  // 16 bytes at a time; neighbouring lanes in one row
-            const int r = i / (L::FULL * 8), c = i - r * (L::FULL * 8), at = j * TM + r;
-            uint4 *p = reinterpret_cast<uint4 *>(tile + (c >> 3) * BLK + r * 128 + (c & 7) * 16);
-            if (at >= g.keys || !((there >> (r / rows)) & 1)) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
-            } else if (fresh && at >= g.s.len) {
-              uint4 x = *p;
-              uint16_t *e = reinterpret_cast<uint16_t *>(&x);
-              bool bad = false;
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (!finite16<T>(e[k])) {
-                  e[k] = 0;
-                  bad = true;
-                }
-              if (bad) *p = x;
-              odd = odd || bad;
-            }
-          }
-          fence_proxy_async_smem();
-          if (__any_sync(0xffffffffu, odd) && lane == 0) odd_item[item % ODD] = item + 1;
-          __threadfence_block();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(BAR(B_VF + s));
-          if (!ok) break;
-        }
       }
     });
     if (!ok && lane == 0) give_up(ERR_TMA, abort_flag, a.err_flag);
@@ -225,7 +214,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
     for (int p = nv > ST ? nv - ST : 0; p < nv; ++p) wait_parity<false>(BAR(B_VF + p % ST), (uint32_t)(p / ST) & 1u, nullptr);
   } else if (warp == W_MMA) {
     // ---------------- MMA issue: the warp runs it, one lane issues ----------------
-    constexpr uint32_t id_s = idesc_of<T>(128, 0), id_o = idesc_of<T>(L::N_FULL, 1);
+    constexpr uint32_t id_s = idesc_of<T>(TN, 0), id_o = idesc_of<T>(DP, 1);
     bool ok = true;
     int t0 = 0, qn = 0, pf[2] = {0, 0};
     auto wait_warp = [&](uint32_t bar, uint32_t par) {
@@ -235,14 +224,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
     auto commit = [&](uint32_t bar) {
       if (elect_one()) umma_commit(bar);
     };
-    walk<M>(a, [&](const Segment &g, int) {
+    walk<M>(a, near, [&](const Segment &g, int) {
       if (!ok) return;
       const int n = g.k1 - g.k0;
       auto scores = [&](int j) {
         const int t = t0 + j;
         if (!wait_warp(BAR(B_KF + t % ST), (uint32_t)(t / ST) & 1u)) return;
         tc_fence_after();
-        mma_rows<L>(tmem + S_COL + (j & 1) * 128u, qs, ks + (t % ST) * C::TILE, id_s);
+        mma_scores<DP>(tmem + S_COL + (j & 1) * 64u, qs, ks + (t % ST) * C::TILE, id_s);
         commit(BAR(B_SF + (j & 1)));
         commit(BAR(B_KE + t % ST));
       };
@@ -250,18 +239,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
       ++qn;
       tc_fence_after();
       scores(0);
-      if (ok && n > 1) scores(1);
       for (int j = 0; j < n && ok; ++j) {
         const int t = t0 + j, s = j & 1;
-        if (!wait_warp(BAR(B_VF + t % ST), (uint32_t)(t / ST) & 1u)) return;
+        // beside the softmax of this tile; the buffer's last P has been read by then, the tensor core goes in order
+        if (j + 1 < n) scores(j + 1);
+        if (!ok || !wait_warp(BAR(B_VF + t % ST), (uint32_t)(t / ST) & 1u)) return;
         if (!wait_warp(BAR(B_PF + s), (uint32_t)pf[s] & 1u)) return;
         ++pf[s];
         tc_fence_after();
-        mma_sum<L>(tmem + O_COL + s * 128u, tmem + S_COL + s * 128u, 16u, vs + (t % ST) * C::TILE, id_o, 0u, j < 2);
+        mma_product(tmem + O_COL, tmem + S_COL + s * 64u, vs + (t % ST) * C::TILE, id_o, j == 0);
         commit(BAR(B_OF + s));
         commit(BAR(B_VE + t % ST));
-        // S of the step after next may follow P V of this one at once: the tensor core runs them in order
-        if (j + 2 < n) scores(j + 2);
       }
       t0 += n;
     });
@@ -269,60 +257,55 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
     commit(BAR(B_DRAIN));
     __syncwarp();
   } else {
-    // ---------------- softmax: thread = row, set t every other key tile ----------------
-    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + S_COL + t * 128u, o_addr = tmem + lanes + O_COL;
+    // ---------------- softmax: thread = row ----------------
+    const int r = tid;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + S_COL, o_addr = tmem + lanes + O_COL;
     const uint64_t c2 = f2_pack(a.c2, a.c2), lift2 = f2_pack(LIFT, LIFT);
+    const int psize = min(a.c.size, TN), boxes = TN / psize;
     bool ok = true;
-    int sf = 0, of = 0, items = 0;
-    walk<M>(a, [&](const Segment &g, int slot) {
-      // after a wait of any role has run out the items are walked through all the same: every thread meets the barriers
-      const int item = items++;
+    int sf[2] = {0, 0}, of[2] = {0, 0}, tile0 = 0, items = 0;  // score tiles taken from and products asked of each buffer; key tiles of earlier items
+    walk<M>(a, near, [&](const Segment &g, int slot) {
+      if (!ok) return;
+      ++items;
       const Row x = row_of(a, g, r);
-      if (ok) {  // this set's half of the row's queries; the last products on the tile are done
-        constexpr int VEC = L::FULL * 8, HALF = VEC / 2;  // 16-byte vectors
+      {  // the row's queries; the last products on the tile are done
+        constexpr int VEC = C::FULL * 8;  // 16-byte vectors
         const T *src = static_cast<const T *>(a.q) + (x.j >= 0 ? q_at(a, g, x, g.hk) : 0);
-        uint4 v[HALF];
+        uint4 v[VEC];
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-          const int c = t * HALF + i;
-          v[i] = x.j >= 0 && c * 8 < a.c.D ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int c = 0; c < VEC; ++c)
+          v[c] = x.j >= 0 && c * 8 < a.c.D ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-          const int c = t * HALF + i;
-          *reinterpret_cast<uint4 *>(gen + (c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = v[i];
-        }
+        for (int c = 0; c < VEC; ++c) *reinterpret_cast<uint4 *>(gen + (c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = v[c];
         fence_proxy_async_smem();
         mbar_arrive(BAR(B_QF));
       }
-      const bool any_rows = (warp & 3) * 32 < g.rows;
-      const int psize = min(a.c.size, TM), boxes = TM / psize;
+      const bool any_rows = warp * 32 < g.rows;
+      const int n = g.k1 - g.k0;
       float ref = -INFINITY, sum = 0.f;
-      int steps = 0;
-      for (int j = g.k0 + t; ok && j < g.k1; j += 2, ++steps) {
-        const int k0 = j * TM;
+      for (int i = 0; i < n; ++i) {
+        const int k0 = (g.k0 + i) * TN, s = i & 1;
         // which of the tile's pages there are
-        int page = lane < boxes ? page_of(a, g, k0 + lane * psize) : 0;
+        const int page = lane < boxes ? page_of(a, g, k0 + lane * psize) : 0;
         const unsigned missing = __ballot_sync(0xffffffffu, lane < boxes && k0 + lane * psize < g.keys && (page < 0 || page >= a.c.pages));
-        if (!wait_warp_parity(BAR(B_SF + t), (uint32_t)sf & 1u, abort_flag)) { ok = false; break; }
-        ++sf;
+        if (!wait_warp_parity(BAR(B_SF + s), (uint32_t)sf[s] & 1u, abort_flag)) { ok = false; break; }
+        ++sf[s];
         tc_fence_after();
         if (any_rows) {
-          uint32_t w[4][32];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) tmem_ld32_nowait(s_addr + q * 32, w[q]);
+          uint32_t w[2][32];
+          tmem_ld32_nowait(s_addr + s * 64u, w[0]);
+          tmem_ld32_nowait(s_addr + s * 64u + 32u, w[1]);
           tmem_wait_ld();
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(w[q][e]));  // not read before the wait
           bool some = true;
-          if (missing || k0 + TM > g.s.len || k0 + TM > g.keys) {
+          if (missing || k0 + TN > g.s.len || k0 + TN > g.keys) {
             some = false;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
               uint32_t seen = x.j >= 0 ? seen_columns(a, g, x, k0 + q * 32) : 0u;
               if (missing) {
 #pragma unroll 1
@@ -339,7 +322,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 32; ++e)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) m[q] = fmaxf(m[q], __uint_as_float(w[q][e]));
+            for (int q = 0; q < 2; ++q) m[2 * q + (e & 1)] = fmaxf(m[2 * q + (e & 1)], __uint_as_float(w[q][e]));
           const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), some ? -FLT_MAX : -INFINITY);
           const bool grow = (top - ref) * a.c2 > LAZY;  // both -inf: NaN, no
           if (__any_sync(0xffffffffu, grow)) {
@@ -347,16 +330,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
             const float fix = grow ? factor(ref, next, a.c2) : 1.f;  // 0 for the first visible keys
             ref = next;
             sum *= fix;
-            if (steps > 0) {  // O holds the earlier tiles' sum, once their product is done
-              if (!wait_warp_parity(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag)) { ok = false; break; }
+            if (i > 0) {  // O holds the earlier tiles' sum, once their product is done
+              if (!wait_warp_parity(BAR(B_OF + (s ^ 1)), (uint32_t)(of[s ^ 1] - 1) & 1u, abort_flag)) { ok = false; break; }
               tc_fence_after();
 #pragma unroll
               for (int d = 0; d < DP; d += 16) {  // in pieces that leave the scores in their registers
                 uint32_t o[16];
-                tmem_ld16u(o_addr + t * 128u + d, o);
+                tmem_ld16u(o_addr + d, o);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix);
-                tmem_st16(o_addr + t * 128u + d, o);
+                tmem_st16(o_addr + d, o);
               }
               tmem_wait_st();
             }
@@ -364,91 +347,102 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
           const float off = ref == -INFINITY ? 0.f : -ref;
           const uint64_t off2 = f2_pack(off, off);
           uint64_t acc[2] = {0ull, 0ull};
-          uint32_t p[2][32];
+          uint32_t p[32];
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               float y, z;
               f2_unpack(f2_fma(f2_add(f2_pack(__uint_as_float(w[q][e]), __uint_as_float(w[q][e + 1])), off2), c2, lift2), y, z);
               y = ex2(y);
               z = ex2(z);
-              acc[(e >> 1) & 1] = f2_add(acc[(e >> 1) & 1], f2_pack(y, z));
-              p[q >> 1][(q & 1) * 16 + (e >> 1)] = pack2<T>(y, z);
+              acc[q] = f2_add(acc[q], f2_pack(y, z));
+              p[q * 16 + (e >> 1)] = pack2<T>(y, z);
             }
-          tmem_st32(s_addr, p[0]);
-          tmem_st32(s_addr + 32, p[1]);
+          tmem_st32(s_addr + s * 64u, p);
           tmem_wait_st();
           float y, z;
           f2_unpack(f2_add(acc[0], acc[1]), y, z);
           sum += y + z;
         }
-        tc_fence_before();
-        mbar_arrive(BAR(B_PF + t));
-        ++of;
-      }
-      if (ok && steps > 0 && !wait_warp_parity(BAR(B_OF + t), (uint32_t)(of - 1) & 1u, abort_flag)) ok = false;
-      tc_fence_after();
-      if (steps > 0) sums[t][r] = make_float2(ref, sum);
-      tc_fence_before();
-      softmax_sync();
-      tc_fence_after();
-      if (any_rows && !*abort_flag) {
-        const bool both = g.k1 - g.k0 > 1;
-        const float2 s0 = sums[0][r], s1 = both ? sums[1][r] : make_float2(-INFINITY, 0.f);
-        const float top = fmaxf(s0.x, s1.x);
-        const float f0 = factor(s0.x, top, a.c2), f1 = factor(s1.x, top, a.c2);
-        const float all = fmaf(f0, s0.y, f1 * s1.y);
-        float scale = 1.f;
-        if (slot < 0) scale = top == -INFINITY ? 0.f : 1.f / all;
-        else if (t == 0 && x.j >= 0) a.part_ml[(int64_t)slot * M + r] = make_float2(top, all);
-        const float w0 = f0 * scale, w1 = f1 * scale;
-        const bool odd = odd_item[item % ODD] == item + 1;
+        const bool fresh = (g.s.n > 1 || a.mask) && k0 + TN > g.s.len;  // new tokens' V: not every row sees it
+        if (missing || fresh || k0 + TN > g.keys) {  // thread r looks after half of V's row r / 2
+          const int tile = tile0 + i, st = tile % ST, vr = r >> 1, at = k0 + vr;
+          if (!wait_warp_parity(BAR(B_VF + st), (uint32_t)(tile / ST) & 1u, abort_flag)) { ok = false; break; }
+          const bool gone = at >= g.keys || ((missing >> (vr / psize)) & 1);
+          if (gone || (fresh && at >= g.s.len)) {
+            uint8_t *row = gen + (vs - base) + st * C::TILE + vr * 128;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          const int d = t * (DP / 2) + i * 16;
-          uint32_t o0[16], o1[16];
-          tmem_ld16u(o_addr + d, o0);
-          float y[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o0[e]) * w0;
-          if (both) {
-            tmem_ld16u(o_addr + 128u + d, o1);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = fmaf(__uint_as_float(o1[e]), w1, y[e]);
-          }
-          if (odd && x.j >= 0) {  // infinities and NaN that the row sees, of the new tokens in this block's tiles
-#pragma unroll 1
-            for (int key = max(g.s.len, g.k0 * TM); key < min(g.keys, g.k1 * TM); ++key) {
-              const int c = key - g.s.len;
-              if (a.mask ? c >= 64 || !((x.bits >> c) & 1) : c > x.j) continue;
-              const int page = page_of(a, g, key);
-              if (page < 0 || page >= a.c.pages) continue;
-              const T *v = static_cast<const T *>(a.c.values) + page * a.c.vp +
-                           (key - cache::page_index(a.c, key) * a.c.size) * a.c.vs + g.hk * a.c.vh;
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (d + e < a.c.D && !finite16<T>(*reinterpret_cast<const uint16_t *>(v + d + e))) y[e] += to_f(v[d + e]);
+            for (int c = 0; c < C::FULL * 4; ++c) {
+              uint4 *v = reinterpret_cast<uint4 *>(row + (c >> 2) * KBLK + ((((c & 3) * 2 + (r & 1)) + (lane & ~1)) & 7) * 16);
+              const uint4 y = *v;
+              const uint4 z = gone ? make_uint4(0u, 0u, 0u, 0u)
+                                   : make_uint4(finite_pair<T>(y.x), finite_pair<T>(y.y), finite_pair<T>(y.z), finite_pair<T>(y.w));
+              if (z.x != y.x || z.y != y.y || z.z != y.z || z.w != y.w) {
+                *v = z;
+                if (!gone) odd_item = items;
+              }
             }
           }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        mbar_arrive(BAR(B_PF + s));
+        ++of[s];
+      }
+      if (!ok) return;
+      tile0 += n;
+      const int last = (n - 1) & 1;
+      if (!wait_warp_parity(BAR(B_OF + last), (uint32_t)(of[last] - 1) & 1u, abort_flag)) { ok = false; return; }
+      tc_fence_after();
+      if (any_rows) {
+        float scale = 1.f;
+        if (slot < 0) scale = ref == -INFINITY ? 0.f : 1.f / sum;
+        else if (x.j >= 0) a.part_ml[(int64_t)slot * M + r] = make_float2(ref, sum);
+#pragma unroll
+        for (int d = 0; d < DP; d += 32) {
+          uint32_t o[32];
+          tmem_ld32u(o_addr + d, o);
           if (x.j < 0) continue;
           if (slot >= 0) {
-            float *dst = a.part_o + ((int64_t)slot * M + r) * DP + d;
+            float4 *dst = reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * M + r) * DP + d);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
           } else {
             T *dst = static_cast<T *>(a.out) + out_at(a, g, x, g.hk) + d;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (d + h * 8 < a.c.D)  // D is a multiple of 8
-                *reinterpret_cast<uint4 *>(dst + h * 8) = make_uint4(pack2<T>(y[h * 8], y[h * 8 + 1]), pack2<T>(y[h * 8 + 2], y[h * 8 + 3]),
-                                                                    pack2<T>(y[h * 8 + 4], y[h * 8 + 5]), pack2<T>(y[h * 8 + 6], y[h * 8 + 7]));
+            for (int h = 0; h < 4; ++h)
+              if (d + h * 8 < a.c.D) {  // D is a multiple of 8
+                uint32_t p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  p[e] = pack2<T>(__uint_as_float(o[h * 8 + 2 * e]) * scale, __uint_as_float(o[h * 8 + 2 * e + 1]) * scale);
+                *reinterpret_cast<uint4 *>(dst + h * 8) = make_uint4(p[0], p[1], p[2], p[3]);
+              }
           }
         }
       }
       tc_fence_before();
-      softmax_sync();
-      tc_fence_after();
+      // (the next item's is set only after all have come to its queries)
+      if (odd_item == items && x.j >= 0) {  // a row adds what it sees of the infinities and NaN that were taken out of V
+        for (int key = max(g.s.len, g.k0 * TN); key < min(g.keys, g.k1 * TN); ++key) {
+          const int page = page_of(a, g, key);
+          if (!sees(a.mask != nullptr, x.bits, x.j, key - g.s.len) || page < 0 || page >= a.c.pages) continue;
+          const T *v = static_cast<const T *>(a.c.values) + page * a.c.vp + (key - cache::page_index(a.c, key) * a.c.size) * a.c.vs +
+                       g.hk * a.c.vh;
+          for (int d = 0; d < a.c.D; ++d) {
+            const T y = v[d];
+            if (finite16<T>(*reinterpret_cast<const uint16_t *>(&y))) continue;
+            if (slot >= 0) {
+              a.part_o[((int64_t)slot * M + r) * DP + d] += to_f(y);
+            } else {
+              T *out = static_cast<T *>(a.out) + out_at(a, g, x, g.hk) + d;
+              *out = from_f<T>(to_f(*out) + to_f(y));
+            }
+          }
+        }
+      }
     });
     if (!ok && lane == 0) give_up(ERR_SOFTMAX, abort_flag, a.err_flag);
   }
@@ -463,7 +457,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) cached_attn_tc_kernel(const __gri
   if (*abort_flag) {
     // a wait gave up: this block's share becomes NaN instead of partly written
     const T bad = from_f<T>(__int_as_float(0x7fc00000));
-    walk<M>(a, [&](const Segment &g, int slot) {
+    walk<M>(a, near, [&](const Segment &g, int slot) {
       for (int i = tid; i < g.rows * a.c.D; i += NTHREADS) {
         const int r = i / a.c.D;
         if (slot < 0) static_cast<T *>(a.out)[out_at(a, g, row_of(a, g, r), g.hk) + i % a.c.D] = bad;
@@ -509,7 +503,7 @@ bool axes_ok(const mhc_kv_cache *c, const Axes &x) {
 bool make_map(CUtensorMap *map, const mhc_kv_cache *c, void *p, const Axes &x) {
   auto enc = encode_fn();
   if (!enc) return false;
-  const cuuint32_t rows = c->page_size < TM ? c->page_size : TM;
+  const cuuint32_t rows = c->page_size < TN ? c->page_size : TN;
   const cuuint64_t dims[4] = {(cuuint64_t)c->dim, (cuuint64_t)(x.head_first ? c->kv_heads : c->page_size),
                               (cuuint64_t)(x.head_first ? c->page_size : c->kv_heads), (cuuint64_t)c->pages};
   const cuuint64_t strides[3] = {(cuuint64_t)(x.head_first ? x.head : x.slot) * 2, (cuuint64_t)(x.head_first ? x.slot : x.head) * 2,
@@ -533,10 +527,10 @@ cudaError_t run(const Args &a, const Maps &maps, cudaStream_t stream) {
 }  // namespace
 }  // namespace cattn
 
-// What TMA asks of the cache: rows of 16-byte multiples that do not overlap, in pages of which a tile of 128 keys has a
+// What TMA asks of the cache: rows of 16-byte multiples that do not overlap, in pages of which a tile of 64 keys has a
 // whole number, or the other way round.
 bool cached_attn_tc_eligible(const mhc_kv_cache *c) {
-  if (c->dtype == MHC_F32 || c->dim % 8 || c->page_size % 8 || (attn::TM % c->page_size && c->page_size % attn::TM)) return false;
+  if (c->dtype == MHC_F32 || c->dim % 8 || c->page_size % 8 || (CATTN_TC_KEYS % c->page_size && c->page_size % CATTN_TC_KEYS)) return false;
   if ((uintptr_t)c->keys % 16 || (uintptr_t)c->values % 16) return false;
   return cattn::axes_ok(c, cattn::axes_of(c, c->strides)) && cattn::axes_ok(c, cattn::axes_of(c, c->strides + 4));
 }
