@@ -12,11 +12,16 @@
 // rest, within an eighth of a turn, becomes a float and goes into two short Taylor series
 // (sincospif, which reduces its argument again, took a third of the kernel's instructions).
 //
-// Memory bound: every element is read and written once.  A block takes a few tokens: the
-// angles of a token are computed once for all its heads and kept in shared memory; then
-// a thread keeps its place in a head (two vectors that hold VEC pairs, or one that is only
-// copied) and walks over the rows (token, head) of q, k and, into a cache, v, which moves
-// with the others without a rotation.
+// Every element is read and written once; what bounds it besides is instructions.  A block takes
+// a few tokens: the angles of a token are computed once for all its heads and kept in
+// shared memory, in the order in which threads read them; then a thread keeps its place
+// in a head (two vectors that hold VEC pairs, or one that is only copied) and walks over
+// rows, two heads of one token at a time, so that they share the angles' way out of shared
+// memory.  v moves into a cache with the others, without a rotation.
+//
+// Neighbouring threads take neighbouring places and heads: with a token's angles in the
+// registers of a thread that walks over its heads the instructions are a third, but a
+// warp's accesses lie 1.5 KB apart, and 16384 tokens of 12 heads of 96 took 27 us for 19.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,6 +44,8 @@ struct Args {
   int64_t T, period;
   int H, Hk, Hv, D, part, half, tokens;  // Hv: 0, or Hk with a cache; tokens of a block
   int pair_items, items, rows_at_once;   // of a head: vectors of pairs, and all; rows that a block takes at a time
+  int twos;                              // rows of a token: head h < twos together with head h + twos
+  uint64_t by_twos;                      // 2^32 over it, rounded up: divides the rows of a block
   const uint64_t *turns;
   const void *pos;
   int pos_bytes;
@@ -76,9 +83,58 @@ struct alignas(sizeof(T) * VEC) Pack {
   T x[VEC];
 };
 
+// A word of two 16-bit values and back.
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t word(float x, float y) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+
+// The pairs of two vectors turned; pair i's cos and sin at cs[i * apart].
+template <typename T, int VEC, bool ILV>
+__device__ __forceinline__ void turn(Pack<T, VEC> &x, Pack<T, VEC> &y, const Cs *cs, int apart) {
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+    uint32_t *a = reinterpret_cast<uint32_t *>(&x), *b = reinterpret_cast<uint32_t *>(&y);
+    if constexpr (ILV) {  // a word is a pair
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        uint32_t &w = i < VEC / 2 ? a[i % (VEC / 2)] : b[i % (VEC / 2)];
+        const Cs k = cs[i * apart];
+        const float2 p = two<T>(w);
+        w = word<T>(p.x * k.c - p.y * k.s, p.y * k.c + p.x * k.s);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const Cs k = cs[2 * i * apart], l = cs[(2 * i + 1) * apart];
+        const float2 p = two<T>(a[i]), q = two<T>(b[i]);
+        a[i] = word<T>(p.x * k.c - q.x * k.s, p.y * l.c - q.y * l.s);
+        b[i] = word<T>(q.x * k.c + p.x * k.s, q.y * l.c + p.y * l.s);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      T &first = !ILV ? x.x[i] : 2 * i < VEC ? x.x[(2 * i) % VEC] : y.x[(2 * i) % VEC];
+      T &second = !ILV ? y.x[i] : 2 * i + 1 < VEC ? x.x[(2 * i + 1) % VEC] : y.x[(2 * i + 1) % VEC];
+      const float p = to_f(first), q = to_f(second);
+      const Cs k = cs[i * apart];
+      first = from_f<T>(p * k.c - q * k.s);
+      second = from_f<T>(q * k.c + p * k.s);
+    }
+  }
+}
+
 template <typename T, int VEC, bool ILV, bool CACHE>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
-  extern __shared__ Cs table[];  // (tokens, half)
+  extern __shared__ Cs table[];  // of token t: pair i of place p at t half + i (half / VEC) + p
   __shared__ int64_t at_k[MAX_TOKENS], at_v[MAX_TOKENS], at_pos[MAX_TOKENS];
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
@@ -104,8 +160,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
   }
   __syncthreads();
   for (int i = tid; i < tokens * a.half; i += THREADS) {
-    const int t = i / a.half;
-    table[i] = angle(a.turns[i - t * a.half], at_pos[t], a.gain, a.sign);
+    const int t = i / a.half, p = i - t * a.half, place = p / VEC;
+    table[t * a.half + (p - place * VEC) * a.pair_items + place] = angle(a.turns[p], at_pos[t], a.gain, a.sign);
   }
   __syncthreads();
   const int item = tid % a.items, lane_row = tid / a.items;
@@ -116,64 +172,53 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
   const int hop = ILV ? VEC : a.half;
   const int heads = a.H + a.Hk + a.Hv;
   using P = Pack<T, VEC>;
-  for (int r = lane_row; r < tokens * heads; r += a.rows_at_once) {
-    const int tl = r / heads;
-    int h = r - tl * heads;
+  for (int r = lane_row; r < tokens * a.twos; r += a.rows_at_once) {
+    const int tl = (int)(((uint64_t)r * a.by_twos) >> 32), h0 = r - tl * a.twos;
     const int64_t t = t0 + tl;
-    const T *src;
-    T *dst;
-    bool turn = pair, zero = false;
-    if (h < a.H) {
-      src = static_cast<const T *>(a.q) + t * a.qt + h * a.qh;
-      dst = static_cast<T *>(a.qo) + (t * a.H + h) * (int64_t)a.D;
-      zero = CACHE && at_v[tl] == -2;
-    } else if (h < a.H + a.Hk) {
-      h -= a.H;
-      src = static_cast<const T *>(a.k) + t * a.kt + h * a.kh;
-      if (CACHE) {
-        if (at_k[tl] < 0) continue;
-        dst = static_cast<T *>(a.c.keys) + at_k[tl] + h * a.c.kh;
-      } else {
-        dst = static_cast<T *>(a.ko) + (t * a.Hk + h) * (int64_t)a.D;
+    P x[2], y[2];
+    T *dst[2];
+    bool live[2], turns[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      int h = h0 + u * a.twos;
+      live[u] = h < heads;
+      turns[u] = pair && h < a.H + a.Hk;
+      const T *src = nullptr;
+      dst[u] = nullptr;
+      if (h < a.H) {
+        src = static_cast<const T *>(a.q) + t * a.qt + h * a.qh + col;
+        dst[u] = static_cast<T *>(a.qo) + (t * a.H + h) * (int64_t)a.D + col;
+      } else if ((h -= a.H) < a.Hk) {
+        src = static_cast<const T *>(a.k) + t * a.kt + h * a.kh + col;
+        if (CACHE) {
+          live[u] = live[u] && at_k[tl] >= 0;
+          dst[u] = static_cast<T *>(a.c.keys) + at_k[tl] + h * a.c.kh + col;
+        } else {
+          dst[u] = static_cast<T *>(a.ko) + (t * a.Hk + h) * (int64_t)a.D + col;
+        }
+      } else if (CACHE) {
+        h -= a.Hk;
+        live[u] = live[u] && at_k[tl] >= 0;
+        src = static_cast<const T *>(a.v) + t * a.vt + h * a.vh + col;
+        dst[u] = static_cast<T *>(a.c.values) + at_v[tl] + h * a.c.vh + col;
       }
-    } else {
-      h -= a.H + a.Hk;
-      if (at_k[tl] < 0) continue;
-      src = static_cast<const T *>(a.v) + t * a.vt + h * a.vh;
-      dst = static_cast<T *>(a.c.values) + at_v[tl] + h * a.c.vh;
-      turn = false;
-    }
-    P x = *reinterpret_cast<const P *>(src + col), y;
-    if (pair) y = *reinterpret_cast<const P *>(src + col + hop);
-    if (turn) {
-      const Cs *cs = table + tl * a.half + item * VEC;
-      if (ILV) {
-        T *e = x.x, *f = y.x;  // 2 VEC neighbouring elements
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          T &first = 2 * i < VEC ? e[(2 * i) % VEC] : f[(2 * i) % VEC];
-          T &second = 2 * i + 1 < VEC ? e[(2 * i + 1) % VEC] : f[(2 * i + 1) % VEC];
-          const float p = to_f(first), q = to_f(second);
-          const Cs w = cs[i];
-          first = from_f<T>(p * w.c - q * w.s);
-          second = from_f<T>(q * w.c + p * w.s);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float p = to_f(x.x[i]), q = to_f(y.x[i]);
-          const Cs w = cs[i];
-          x.x[i] = from_f<T>(p * w.c - q * w.s);
-          y.x[i] = from_f<T>(q * w.c + p * w.s);
-        }
+      if (live[u]) {
+        x[u] = *reinterpret_cast<const P *>(src);
+        if (pair) y[u] = *reinterpret_cast<const P *>(src + hop);
       }
     }
-    if (zero) {
+    const Cs *cs = table + tl * a.half + item;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x.x[i] = y.x[i] = from_f<T>(0.f);
+    for (int u = 0; u < 2; ++u) {
+      if (!live[u]) continue;
+      if (turns[u]) turn<T, VEC, ILV>(x[u], y[u], cs, a.pair_items);
+      if (CACHE && h0 + u * a.twos < a.H && at_v[tl] == -2) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[u].x[i] = y[u].x[i] = from_f<T>(0.f);
+      }
+      *reinterpret_cast<P *>(dst[u]) = x[u];
+      if (pair) *reinterpret_cast<P *>(dst[u] + hop) = y[u];
     }
-    *reinterpret_cast<P *>(dst + col) = x;
-    if (pair) *reinterpret_cast<P *>(dst + col + hop) = y;
   }
 }
 
@@ -201,9 +246,11 @@ static cudaError_t launch(Args a, int dtype, bool ilv, bool with_cache, cudaStre
   a.rows_at_once = THREADS / a.items;
   if (a.rows_at_once < 1) return cudaErrorInvalidValue;
   const int heads = a.H + a.Hk + a.Hv;
-  // a thread takes about four rows, fewer where that would leave SMs without a block
+  a.twos = (heads + 1) / 2;
+  a.by_twos = (((uint64_t)1 << 32) + a.twos - 1) / a.twos;
+  // a thread takes about two pairs of heads, fewer where that would leave SMs without a block
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
-  int64_t tokens = (4 * a.rows_at_once) / heads;
+  int64_t tokens = (2 * a.rows_at_once) / a.twos;
   tokens = tokens > MAX_TOKENS ? MAX_TOKENS : tokens;
   const int64_t spread = (a.T + sms - 1) / sms;
   tokens = tokens > spread ? spread : tokens;
@@ -292,7 +339,7 @@ int mhc_rotate(const mhc_rotary *r, const void *q, void *q_out, int H, const voi
   clear_error();
   if (!r || !strides) return fail(MHC_ERR_NULL, "%s: rotary or strides is NULL", who);
   if (dtype != MHC_F32 && dtype != MHC_BF16 && dtype != MHC_F16) return fail(MHC_ERR_DTYPE, "%s: bad dtype code %d", who, dtype);
-  if (T < 0 || T > 0x7fffffff || H < 0 || Hk < 0 || H + Hk < 1 || H > 65536 || Hk > 65536 || D < 2 || D > rotary::MAX_D || period < 0 || period > 0x7fffffff)
+  if (T < 0 || T > 0x7fffffff || H < 0 || Hk < 0 || H + Hk < 1 || H > 16384 || Hk > 16384 || D < 2 || D > rotary::MAX_D || period < 0 || period > 0x7fffffff)
     return fail(MHC_ERR_SHAPE, "%s: T = %lld, %d and %d heads of %d (up to %d), period %lld", who, (long long)T, H, Hk, D, rotary::MAX_D,
                 (long long)period);
   if (int st = rotary::check_rotary(who, r, D)) return st;
@@ -320,7 +367,7 @@ int mhc_append_kv(const mhc_kv_cache *cache, const mhc_cache_step *step, const v
   if (int st = cache_view(who, cache, step, a.c)) return st;
   if (!strides) return fail(MHC_ERR_NULL, "%s: strides is NULL", who);
   const int D = cache->dim;
-  if (H < 0 || H > 65536 || cache->kv_heads > 65536) return fail(MHC_ERR_SHAPE, "%s: %d query heads, %d key heads", who, H, cache->kv_heads);
+  if (H < 0 || H > 16384 || cache->kv_heads > 16384) return fail(MHC_ERR_SHAPE, "%s: %d query heads, %d key heads", who, H, cache->kv_heads);
   if (r) {
     if (int st = rotary::check_rotary(who, r, D)) return st;
   } else {
