@@ -932,20 +932,26 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
     GQA), the reference's CUDA path minus the optional flash-attn library.  The
     MoE layer computes the same routing (softmax, top-k, renormalised) and
     auxiliary loss as the reference but groups each expert's rows with one sort
-    instead of a mask per expert.  ``native_ops`` takes attention and the router
-    from this build (``model/mhc_attention.py``, ``model/mhc_router.py``)
-    instead.  Random init N(0, 0.02) for the matrices."""
+    instead of a mask per expert.  ``native_ops`` takes attention, the rotation
+    by position and the router from this build (``model/mhc_attention.py``,
+    ``model/mhc_rotary.py``, ``model/mhc_router.py``) instead, and the forward
+    then also takes new tokens of sequences in a paged cache
+    (``model/mhc_cache.py``), the reference's decoding with past keys and values
+    (``:200-250, 405-461``).  Random init N(0, 0.02) for the matrices."""
     import torch.nn as nn
     import torch.nn.functional as F
 
     from model.mhc_common import MHCHead, StreamExpand
     from model.mhc_fused import MHCConnection_Fused
     from model.mhc_fused_no_hres import MHCConnection_FusedNoHres
+    hd = hidden // heads
     if native_ops:
         from model.mhc_attention import packed_attention
+        from model.mhc_cache import append_kv, cached_attention
+        from model.mhc_rotary import Rotary, rotate
         from model.mhc_router import route_topk
+        rotary = Rotary(hd, theta, device=dev)
 
-    hd = hidden // heads
     moe_inter = moe_inter or inter
 
     class Attention(nn.Module):
@@ -958,11 +964,18 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
             self.q_norm = nn.RMSNorm(hd, eps=eps)
             self.k_norm = nn.RMSNorm(hd, eps=eps)
 
-        def forward(self, x, cos, sin):
+        def forward(self, x, cos, sin, cached=None):
             b, l, _ = x.shape
             q = self.q_norm(self.q_proj(x).view(b, l, heads, hd))
             k = self.k_norm(self.k_proj(x).view(b, l, kv_heads, hd))
             v = self.v_proj(x).view(b, l, kv_heads, hd)
+            if cached is not None:  # new tokens (b = 1) of the step's sequences, one after another
+                keys, values, step, positions, mask = cached
+                q = append_kv(keys, values, step, k[0], v[0], q=q[0], rotary=rotary, positions=positions)
+                return self.o_proj(cached_attention(q, keys, values, step, mask=mask).reshape(b, l, heads * hd))
+            if native_ops:
+                q, k = rotate(rotary, q, k)
+                return self.o_proj(packed_attention(q, k, v).reshape(b, l, heads * hd))
 
             def rope(t):
                 h = t.shape[-1] // 2
@@ -970,8 +983,6 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
                 return (t * cos + rot * sin).to(t.dtype)
 
             q, k = rope(q), rope(k)
-            if native_ops:
-                return self.o_proj(packed_attention(q, k, v).reshape(b, l, heads * hd))
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
                                                is_causal=True, enable_gqa=True)
             return self.o_proj(o.transpose(1, 2).reshape(b, l, heads * hd))
@@ -1047,8 +1058,8 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
                 self.attn_mhc.sinkhorn_iters = iters
                 self.mlp_mhc.sinkhorn_iters = iters
 
-        def forward(self, h, cos, sin):
-            h = self.attn_mhc(h, lambda z: self.self_attn(self.attn_in_norm(z), cos, sin))
+        def forward(self, h, cos, sin, cached=None):
+            h = self.attn_mhc(h, lambda z: self.self_attn(self.attn_in_norm(z), cos, sin, cached))
             return self.mlp_mhc(h, lambda z: self.mlp(self.ffn_in_norm(z)))
 
     class MiniMindModel(nn.Module):
@@ -1060,7 +1071,13 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
             self.norm = nn.Sequential(MHCHead(n, hidden, eps=eps), nn.RMSNorm(hidden, eps=eps))
             self.use_chain = chain
 
-        def forward(self, ids):
+        def forward(self, ids, cached=None):
+            if cached is not None:
+                cache, *rest = cached
+                h = self.embed_up_norm(self.embed_tokens(ids))
+                for i, blk in enumerate(self.layers):
+                    h = blk(h, None, None, (cache.keys[i], cache.values[i], *rest))
+                return self.norm(h)
             l = ids.shape[1]
             pos = torch.arange(l, device=ids.device, dtype=torch.float32)
             inv = 1.0 / (theta ** (torch.arange(0, hd, 2, device=ids.device, dtype=torch.float32) / hd))
@@ -1090,8 +1107,14 @@ def _build_decoder(moe: bool, dev, n=4, hidden=768, layers=8, heads=8, kv_heads=
             self.lm_head = nn.Linear(hidden, vocab, bias=False)
             self.model.embed_tokens.weight = self.lm_head.weight
 
-        def forward(self, ids):
-            return self.lm_head(self.model(ids))
+        def forward(self, ids, cache=None, step=None, positions=None, mask=None):
+            """ids (B, L): logits (B, L, vocab).  With a ``PagedCache`` and a ``CacheStep``: ids (T,), the step's new
+            tokens, logits (T, vocab); ``positions`` and ``mask`` as for ``append_kv`` and ``cached_attention``."""
+            if cache is None:
+                return self.lm_head(self.model(ids))
+            if not native_ops:
+                raise RuntimeError("the paged cache needs native_ops")
+            return self.lm_head(self.model(ids[None], (cache, step, positions, mask)))[0]
 
         def aux_loss(self):
             losses = [blk.mlp.aux_loss for blk in self.model.layers
@@ -1305,16 +1328,97 @@ def run_model(args, rank, world, local_rank):
     print(json.dumps(line), flush=True)
 
 
+def run_decode(args, rank, world, local_rank):
+    """Answering with drafted tokens: the 8-layer decoder over a paged cache, 64 sequences with prompts of 256 to 1024
+    tokens, every step a tree of 16 rows a sequence (its last token and 15 drafted ones): forward, softmax, verification,
+    the kept rows moved up.  The drafts are uniform over the vocabulary, as is nearly the random-init target, so most of a
+    path is kept.  Counted are the tokens that the steps add to the answers."""
+    from model.mhc_cache import CacheStep, PagedCache, keep_drafts, tree_mask
+    from model.mhc_verify import verify_drafts
+
+    dev = torch.device("cuda", local_rank)
+    torch.cuda.set_device(dev)
+    torch.manual_seed(1234 + rank)
+    gen = torch.Generator(device=dev).manual_seed(77 + rank)
+    model = _build_decoder(moe=False, dev=dev, native_ops=True).eval()
+    vocab, batch, rows, page = 6400, 64, 16, 64
+    steps = args.warmup + args.steps
+    prompts = torch.linspace(256, 1024, batch).long()
+    each = int((1024 + rows * (steps + 1)) // page + 1)
+    cache = PagedCache(8, batch * each, page, 4, 96, device=dev)
+    table = torch.randperm(batch * each, generator=gen, device=dev).to(torch.int32).view(batch, each)
+    lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), prompts.cumsum(0)]).to(torch.int32).to(dev)
+    start = torch.arange(0, batch * rows, rows, device=dev)
+    tree_cu = torch.arange(0, batch * rows + 1, rows, dtype=torch.int32, device=dev)
+    # a tree of 16 rows: up to three children of a node, four levels and more of the first ones
+    parents = torch.tensor([-1, 0, 0, 0, 1, 1, 2, 4, 4, 6, 7, 7, 10, 10, 12, 14], dtype=torch.int32, device=dev).repeat(batch)
+    mask, depth = tree_mask(parents, tree_cu)
+    draft = torch.full((1, vocab), 1.0 / vocab, device=dev).expand(batch * rows, vocab).contiguous()
+    added = []
+
+    with torch.no_grad():
+        ids = torch.randint(0, vocab, (int(prompts.sum()),), device=dev, generator=gen)
+        logits = model(ids, cache, CacheStep(table, lengths, cu))
+        last = logits[cu[1:].long() - 1].float().argmax(-1)
+        lengths += cu.diff()
+
+        def step():
+            nonlocal last, lengths
+            tokens = torch.randint(0, vocab, (batch * rows,), device=dev, generator=gen)
+            tokens[start] = last
+            now = CacheStep(table, lengths, tree_cu)
+            logits = model(tokens, cache, now, positions=lengths.repeat_interleave(rows) + depth, mask=mask)
+            target = torch.softmax(logits.float(), -1)
+            path, kept, last = verify_drafts(tokens, parents, tree_cu, target, draft, torch.rand(batch * rows, device=dev, generator=gen))
+            keep_drafts(cache.keys, cache.values, now, path, kept)
+            lengths = lengths + kept
+            added.append(kept)
+
+        for _ in range(args.warmup):
+            step()
+        added.clear()
+        torch.cuda.synchronize(dev)
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        sampler = ClockSampler(dev)
+        sampler.start()
+        e0.record()
+        for _ in range(args.steps):
+            step()
+        e1.record()
+        torch.cuda.synchronize(dev)
+        clocks = sampler.stop()
+    ms = _max_over_ranks(e0.elapsed_time(e1), world, dev)
+    count = float(torch.stack(added).sum().item())
+    if world > 1:
+        import torch.distributed as dist
+        t = torch.tensor([count], device=dev)
+        dist.all_reduce(t)
+        count = float(t.item())
+    if rank != 0:
+        return
+    print(json.dumps({
+        "metric": "answer tokens/s", "value": count / (ms / 1e3), "unit": "tokens/s", "n_gpus": world, "steps": args.steps,
+        "warmup": args.warmup, "ms_per_step": ms / args.steps, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+        "dtype": "bf16", "data": "synthetic (token ids and drafts uniform over the vocabulary, random-init weights)",
+        "config": {"workload": "decode: dense decoder + mHC over a paged cache, trees of 16 drafted rows",
+                   "model": "hidden 768, 8 layers, 8 q / 4 kv heads, RoPE 1e6, SwiGLU 2048, vocab 6400, n=4",
+                   "sequences": batch, "prompts": "256 to 1024 tokens", "rows_per_step": batch * rows,
+                   "kept_per_step_and_sequence": count / (args.steps * batch * world), "parallelism": f"dp{world}"},
+        "clocks": clocks}), flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--impl", choices=["ours", "reference"], default="ours")
-    ap.add_argument("--workload", choices=["layer", "c4", "c5", "post_pre", "fp32_stream"], default="layer",
+    ap.add_argument("--workload", choices=["layer", "c4", "c5", "post_pre", "fp32_stream", "decode"], default="layer",
                     help="layer: configs[1] mHC layer (the headline); c4 / c5: model-level configs[3] / [4]; "
                          "post_pre: the step between two sublayers, two kernels against the fused kernel; "
-                         "fp32_stream: the layer with an fp32 residual stream (forward and backward)")
+                         "fp32_stream: the layer with an fp32 residual stream (forward and backward); "
+                         "decode: answering with drafted tokens over a paged cache")
     ap.add_argument("--variant", choices=["full", "nohres"], default="full")
     ap.add_argument("--C", type=int, default=0, help="stream width for --variant nohres (768 or 1024)")
     ap.add_argument("--tokens", type=int, default=16 * 2048)
@@ -1329,7 +1433,7 @@ def main():
     ap.add_argument("--chain", action="store_true",
                     help="c4 / c5: run the decoder's sublayers through the block-level mhc_chain API")
     ap.add_argument("--native-ops", action="store_true",
-                    help="c4 / c5: attention, router and optimizer step through this build's kernels instead of torch's")
+                    help="c4 / c5: attention, rotary positions, router and optimizer step through this build's kernels instead of torch's")
     ap.add_argument("--flat-allreduce", action="store_true",
                     help="c5: one flat all-reduce per dtype after backward instead of the overlapped buckets")
     args = ap.parse_args()
@@ -1358,6 +1462,8 @@ def main():
             run_post_pre(args, rank, world, local_rank)
         elif args.workload == "fp32_stream":
             run_fp32_stream(args, rank, world, local_rank)
+        elif args.workload == "decode":
+            run_decode(args, rank, world, local_rank)
         else:
             run_model(args, rank, world, local_rank)
     finally:

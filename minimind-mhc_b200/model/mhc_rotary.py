@@ -13,14 +13,22 @@ are in ``csrc/host/mhc_torch.cpp``.
 from __future__ import annotations
 
 import math
-from fractions import Fraction
 
 import torch
 
 from . import _native as nat
 
-# 1 / (2 pi): a frequency's turns need the bits behind a double's last
-_INV_TWO_PI = Fraction("0.159154943091895335768883763372514362034459645740456448747667344058896797634226535")
+# 2^320 / (2 pi): a frequency's turns need the bits behind a double's last
+_TURNS_BITS = 320
+_TURNS = (159154943091895335768883763372514362034459645740456448747667344058896797634226535090113802766253085956072842726757958
+          << _TURNS_BITS) // 10 ** 117
+
+
+def _turns_of(f: float) -> int:
+    """round(f / (2 pi) * 2^64) modulo 2^64."""
+    n, d = f.as_integer_ratio()  # d is a power of two
+    shift = _TURNS_BITS - 64
+    return (((n * _TURNS // d) + (1 << (shift - 1))) >> shift) & ((1 << 64) - 1)
 
 
 class Rotary:
@@ -71,7 +79,7 @@ class Rotary:
         if not math.isfinite(self.gain):
             raise ValueError(f"Rotary: gain must be finite, got {gain}")
         self.inv_freq = torch.tensor(inv, dtype=torch.float64)
-        turns = [round(Fraction(f) * _INV_TWO_PI * (1 << 64)) & ((1 << 64) - 1) for f in inv]
+        turns = [_turns_of(f) for f in inv]
         self._host = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
         self._on = {}
         if device is not None or torch.cuda.is_available():
