@@ -1331,8 +1331,8 @@ def run_model(args, rank, world, local_rank):
 def run_decode(args, rank, world, local_rank):
     """Answering with drafted tokens: the 8-layer decoder over a paged cache, 64 sequences with prompts of 256 to 1024
     tokens, every step a tree of 16 rows a sequence (its last token and 15 drafted ones): forward, softmax, verification,
-    the kept rows moved up.  The drafts are uniform over the vocabulary, as is nearly the random-init target, so most of a
-    path is kept.  Counted are the tokens that the steps add to the answers."""
+    the kept rows moved up.  The drafts are uniform over the vocabulary, as is nearly the random-init target at a high
+    temperature, so most of a path is kept.  Counted are the tokens that the steps add to the answers."""
     from model.mhc_cache import CacheStep, PagedCache, keep_drafts, tree_mask
     from model.mhc_verify import verify_drafts
 
@@ -1369,8 +1369,9 @@ def run_decode(args, rank, world, local_rank):
             tokens[start] = last
             now = CacheStep(table, lengths, tree_cu)
             logits = model(tokens, cache, now, positions=lengths.repeat_interleave(rows) + depth, mask=mask)
-            target = torch.softmax(logits.float(), -1)
-            path, kept, last = verify_drafts(tokens, parents, tree_cu, target, draft, torch.rand(batch * rows, device=dev, generator=gen))
+            target = torch.softmax(logits.float() / 20, -1)  # the embedding is tied: without it a token follows itself
+            path, kept, last = verify_drafts(tokens, parents, tree_cu, target, draft,
+                                             torch.rand(batch * rows, device=dev, generator=gen))
             keep_drafts(cache.keys, cache.values, now, path, kept)
             lengths = lengths + kept
             added.append(kept)

@@ -217,22 +217,46 @@ __global__ void __launch_bounds__(THREADS, 2) verify_kernel(const Args a) {
         if (warp == w_at) {
           const T *prow = target + (int64_t)(start + cur) * a.ts;
           const T *qrow = drawn && r.gone != 0.0 ? draft + (int64_t)(start + cur) * a.ds : nullptr;
-          double sum = w_before;
-          int64_t positive = lo;
-          for (int64_t i0 = lo; i0 < hi && next < 0; i0 += 32) {
-            const int64_t i = i0 + lane;
-            const double v = i < hi ? rest_of<T>(sh, entry(prow, i), qrow ? entry(qrow, i) : 0.f, (int)i, drawn, r) : 0.0;
-            double inc = v;
+          auto at_token = [&](int64_t i) {
+            return rest_of<T>(sh, entry(prow, i), qrow ? entry(qrow, i) : 0.f, (int)i, drawn, r);
+          };
+          // a lane's sum of neighbouring tokens, then the tokens of the lane whose sums pass the goal, one each
+          const int64_t each = (hi - lo + 31) / 32, mine_lo = min(lo + lane * each, hi), mine_hi = min(mine_lo + each, hi);
+          double sum = 0.0;
+          for (int64_t i0 = mine_lo; i0 < mine_hi; i0 += AT_ONCE) {
+            float p[AT_ONCE], q[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+              p[i] = i0 + i < mine_hi ? entry(prow, i0 + i) : 0.f;
+              q[i] = qrow && i0 + i < mine_hi ? entry(qrow, i0 + i) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) sum += rest_of<T>(sh, p[i], q[i], (int)(i0 + i), drawn, r);
+          }
+          auto up_to = [&](double v) {  // the sum of the lanes up to this one
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-              const double up = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += up;
+              const double up = __shfl_up_sync(0xffffffffu, v, o);
+              if (lane >= o) v += up;
             }
-            const unsigned some = __ballot_sync(0xffffffffu, v > 0.0);
-            const unsigned past = __ballot_sync(0xffffffffu, v > 0.0 && sum + inc > goal);
-            if (some) positive = i0 + 31 - __clz(some);
-            if (!tail && past) next = i0 + __ffs(past) - 1;
-            sum += __shfl_sync(0xffffffffu, inc, 31);
+            return v;
+          };
+          const double inc = up_to(sum);
+          const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0);
+          const unsigned past = __ballot_sync(0xffffffffu, !tail && sum > 0.0 && w_before + inc > goal);
+          tail = tail || !past;
+          const int owner = past ? __ffs(past) - 1 : 31 - __clz(some);
+          double so_far = w_before + __shfl_sync(0xffffffffu, inc - sum, owner);
+          const int64_t from = min(lo + owner * each, hi), to = min(from + each, hi);
+          int64_t positive = from;
+          for (int64_t i0 = from; i0 < to && next < 0; i0 += 32) {
+            const int64_t i = i0 + lane;
+            const double v = i < to ? at_token(i) : 0.0, upto = up_to(v);
+            const unsigned any = __ballot_sync(0xffffffffu, v > 0.0);
+            const unsigned beyond = __ballot_sync(0xffffffffu, !tail && v > 0.0 && so_far + upto > goal);
+            if (any) positive = i0 + 31 - __clz(any);
+            if (beyond) next = i0 + __ffs(beyond) - 1;
+            so_far += __shfl_sync(0xffffffffu, upto, 31);
           }
           if (next < 0) next = positive;
           if (lane == 0) a.next[b] = next;
