@@ -35,13 +35,18 @@ __device__ __forceinline__ Seq seq_between(const View &v, int from, int to, int 
 }
 __device__ __forceinline__ Seq seq_of(const View &v, int b) { return seq_between(v, v.cu[b], v.cu[b + 1], v.lengths[b]); }
 
-// the sequence of row t, or -1: cu[b] <= t < cu[b + 1]
-__device__ __forceinline__ int seq_at(const View &v, int t) {
-  if (t < v.cu[0] || t >= v.cu[v.batch]) return -1;
-  int lo = 0, hi = v.batch;
-  while (hi - lo > 1) {
+// How many sequences end at or before row t, by a whole warp: the first that can hold it.  All offsets at once where they
+// are few (a bisection is a chain of loads), else bisected.
+__device__ __forceinline__ int seq_from(const View &v, int t) {
+  if (v.batch <= 512) {
+    int n = 0;
+    for (int i = threadIdx.x & 31; i < v.batch; i += 32) n += v.cu[i + 1] <= t;
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  int lo = 0, hi = v.batch;  // cu[lo] <= t < cu[hi + 1], if there is such
+  while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (v.cu[mid] <= t) lo = mid; else hi = mid;
+    if (v.cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
   }
   return lo;
 }

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
   const bool one_page = a.c.size % CHUNK == 0;       // a chunk never crosses a page's end
   const int fetch_row = lane / VPR, fetch_col = lane - fetch_row * VPR;
   const bool fetches = fetch_row < RPI && fetch_col * 8 < D;
-  const float ahead = AHEAD / a.c2;
+  const float ahead = fminf(AHEAD / a.c2, FLT_MAX);
   if (D < DP)
     for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   near.fill(a);
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
   __shared__ float2 ml[WARPS][R];
   __shared__ float fac[WARPS][R];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.D;
-  const float ahead = 8.f / a.c2;
+  const float ahead = fminf(8.f / a.c2, FLT_MAX);
   for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
   near.fill(a);
   clear_rest<T>(a);
@@ -795,7 +795,7 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
   if (x.kind == TC) {
     x.m = CATTN_TC_ROWS;
     x.pieces = sms * CATTN_TC_BLOCKS;
-    x.cost = 7;
+    x.cost = 8;
   } else if (x.kind == MMA) {
     x.m = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     // the warps of a block take neighbouring key heads of the same keys, which lie side by side in memory
@@ -921,7 +921,8 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   if (int st = cache_view(who, cache, step, a.c)) return st;
   if (cache->dim > 128) return fail(MHC_ERR_SHAPE, "%s: head sizes up to 128 are supported (got %d)", who, cache->dim);
   if (H < 1 || H % cache->kv_heads) return fail(MHC_ERR_SHAPE, "%s: %d query heads cannot share %d key heads", who, H, cache->kv_heads);
-  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(MHC_ERR_SHAPE, "%s: scale must be positive and finite (got %g)", who, scale);
+  a.c2 = (float)((double)scale * 1.4426950408889634);
+  if (!(scale > 0.f) || !(a.c2 < INFINITY)) return fail(MHC_ERR_SHAPE, "%s: scale must be positive and finite (got %g)", who, scale);
   if (step->T == 0) return MHC_OK;
   if (!q || !out || !q_strides) return fail(MHC_ERR_NULL, "%s: required pointer is NULL", who);
   const size_t es = cache->dtype == MHC_F32 ? 4 : 2;
@@ -938,7 +939,6 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   const cattn::Choice x = cattn::choose(cache, step, H, !mma ? cattn::CORE : cached_attn_tc_eligible(cache) ? cattn::TC : cattn::MMA);
   a.q = q, a.out = out, a.qt = q_strides[0], a.qh = q_strides[1];
   a.mask = mask, a.H = H, a.G = H / cache->kv_heads;
-  a.c2 = (float)((double)scale * 1.4426950408889634);
   a.pieces = x.pieces, a.hw = x.hw, a.groups = a.c.Hk / x.hw, a.cost = x.cost, a.whole = x.whole, a.dtype = cache->dtype;
   a.tile = x.kind == cattn::TC ? CATTN_TC_KEYS : cattn::KT / x.hw;
   a.err_flag = host_error_flag();

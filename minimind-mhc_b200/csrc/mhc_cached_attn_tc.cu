@@ -269,15 +269,24 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
       if (!ok) return;
       ++items;
       const Row x = row_of(a, g, r);
-      {  // the row's queries; the last products on the tile are done
-        constexpr int VEC = C::FULL * 8;  // 16-byte vectors
-        const T *src = static_cast<const T *>(a.q) + (x.j >= 0 ? q_at(a, g, x, g.hk) : 0);
-        uint4 v[VEC];
+      {  // the warp's rows of queries, neighbouring lanes along a row; the last products on the tile are done
+        constexpr int VEC = C::FULL * 8, AT = 32 / VEC;  // 16-byte vectors of a row, rows at a time
+        const int64_t mine = x.j >= 0 ? q_at(a, g, x, g.hk) : -1;
+        const int c = lane % VEC;
+#pragma unroll 1
+        for (int i0 = 0; i0 < VEC; i0 += 8) {
+          uint4 v[8];
 #pragma unroll
-        for (int c = 0; c < VEC; ++c)
-          v[c] = x.j >= 0 && c * 8 < a.c.D ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 8; ++i) {
+            const int64_t at = __shfl_sync(0xffffffffu, mine, (i0 + i) * AT + lane / VEC);
+            v[i] = at >= 0 && c * 8 < a.c.D ? *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + at + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) *reinterpret_cast<uint4 *>(gen + (c >> 3) * BLK + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = v[c];
+          for (int i = 0; i < 8; ++i) {
+            const int row = warp * 32 + (i0 + i) * AT + lane / VEC;
+            *reinterpret_cast<uint4 *>(gen + (c >> 3) * BLK + row * 128 + (((c & 7) ^ (row & 7)) * 16)) = v[i];
+          }
+        }
         fence_proxy_async_smem();
         mbar_arrive(BAR(B_QF));
       }
@@ -333,7 +342,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
             if (i > 0) {  // O holds the earlier tiles' sum, once their product is done
               if (!wait_warp_parity(BAR(B_OF + (s ^ 1)), (uint32_t)(of[s ^ 1] - 1) & 1u, abort_flag)) { ok = false; break; }
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int d = 0; d < DP; d += 16) {  // in pieces that leave the scores in their registers
                 uint32_t o[16];
                 tmem_ld16u(o_addr + d, o);
@@ -399,28 +408,28 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
         float scale = 1.f;
         if (slot < 0) scale = ref == -INFINITY ? 0.f : 1.f / sum;
         else if (x.j >= 0) a.part_ml[(int64_t)slot * M + r] = make_float2(ref, sum);
-#pragma unroll
-        for (int d = 0; d < DP; d += 32) {
+        // 32 columns at a time through the place of the warp's queries, so that neighbouring lanes write along a row
+        const int64_t mine = x.j < 0 ? -1 : slot >= 0 ? ((int64_t)slot * M + r) * DP : out_at(a, g, x, g.hk);
+        float4 *hold = reinterpret_cast<float4 *>(gen + warp * 4096);
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 32) {  // (what runs once for an item is kept short: its instructions come from far)
           uint32_t o[32];
           tmem_ld32u(o_addr + d, o);
-          if (x.j < 0) continue;
-          if (slot >= 0) {
-            float4 *dst = reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * M + r) * DP + d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-          } else {
-            T *dst = static_cast<T *>(a.out) + out_at(a, g, x, g.hk) + d;
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-              if (d + h * 8 < a.c.D) {  // D is a multiple of 8
-                uint32_t p[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  p[e] = pack2<T>(__uint_as_float(o[h * 8 + 2 * e]) * scale, __uint_as_float(o[h * 8 + 2 * e + 1]) * scale);
-                *reinterpret_cast<uint4 *>(dst + h * 8) = make_uint4(p[0], p[1], p[2], p[3]);
-              }
+          for (int e = 0; e < 8; ++e)
+            hold[lane * 8 + (e ^ (lane & 7))] = make_float4(__uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
+                                                            __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
+          __syncwarp();
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {
+            const int row = 4 * i + (lane >> 3), e = lane & 7;
+            const int64_t at = __shfl_sync(0xffffffffu, mine, row);
+            const float4 y = hold[row * 8 + (e ^ (row & 7))];
+            if (at < 0 || d + 4 * e >= a.c.D) continue;
+            if (slot >= 0) *reinterpret_cast<float4 *>(a.part_o + at + d + 4 * e) = y;
+            else *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at + d + 4 * e) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
           }
+          __syncwarp();
         }
       }
       tc_fence_before();

@@ -139,24 +139,28 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int tokens = (int)min((int64_t)a.tokens, a.T - t0);
-  if (tid < tokens) {
+  if (tid < 32) {  // at most as many tokens
     const int64_t t = t0 + tid;
-    int64_t pos = a.period > 0 ? (int64_t)((uint32_t)t % (uint32_t)a.period) : t;
-    if (a.pos) pos = a.pos_bytes == 8 ? static_cast<const int64_t *>(a.pos)[pos] : static_cast<const int32_t *>(a.pos)[pos];
-    if (CACHE) {
-      const int b = cache::seq_at(a.c, (int)t);
-      int page = 0, slot = 0;
-      bool there = false;
-      if (b >= 0) {
-        const int64_t place = (int64_t)a.c.lengths[b] + (t - a.c.cu[b]);
-        there = cache::locate(a.c, b, place, page, slot);
-        if (!a.pos) pos = place;
+    int b = CACHE ? cache::seq_from(a.c, (int)t0) : 0;
+    if (tid < tokens) {
+      int64_t pos = a.period > 0 ? (int64_t)((uint32_t)t % (uint32_t)a.period) : t;
+      if (a.pos) pos = a.pos_bytes == 8 ? static_cast<const int64_t *>(a.pos)[pos] : static_cast<const int32_t *>(a.pos)[pos];
+      if (CACHE) {
+        while (b < a.c.batch && a.c.cu[b + 1] <= t) ++b;
+        int page = 0, slot = 0;
+        const bool known = b < a.c.batch && a.c.cu[b] <= t;
+        bool there = false;
+        if (known) {
+          const int64_t place = (int64_t)a.c.lengths[b] + (t - a.c.cu[b]);
+          there = cache::locate(a.c, b, place, page, slot);
+          if (!a.pos) pos = place;
+        }
+        at_k[tid] = there ? page * a.c.kp + slot * a.c.ks : -1;
+        // -2: of no sequence, its rotated query is 0
+        at_v[tid] = there ? page * a.c.vp + slot * a.c.vs : (known ? -1 : -2);
       }
-      at_k[tid] = there ? page * a.c.kp + slot * a.c.ks : -1;
-      // -2: of no sequence, its rotated query is 0
-      at_v[tid] = there ? page * a.c.vp + slot * a.c.vs : (b >= 0 ? -1 : -2);
+      at_pos[tid] = pos;
     }
-    at_pos[tid] = pos;
   }
   __syncthreads();
   for (int i = tid; i < tokens * a.half; i += THREADS) {
