@@ -110,7 +110,7 @@ __device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int 
 
 // Joins the blocks that had part of a cut item.  Every block lists the cut items (one entry for each block of the first
 // kernel); a warp takes one row at a time and goes through its parts, AT_ONCE of them under way.  Where a row has more
-// than a few the block's eight warps share them and join what they have through shared memory.
+// than a few the block's warps share them and join what they have through shared memory.
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_PIECES = 1024;
 constexpr int JOIN_ALONE = 16;  // parts that a warp goes through by itself
 
@@ -118,8 +118,9 @@ template <int DP>
 struct Joined {
   float o[DP / 32], m = -INFINITY, l = 0.f;
   // parts begin, begin + step, ... of `count`: part i of the item of block c, row `row` of the `rows` of a slot
+  template <int AT_ONCE>
   __device__ __forceinline__ void add(const Args &a, int c, int count, int64_t row, int64_t rows, int begin, int step) {
-    constexpr int PER = DP / 32, AT_ONCE = 4;
+    constexpr int PER = DP / 32;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int k = 0; k < PER; ++k) o[k] = 0.f;
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
         int64_t row;
         T *out = row_at(c, task - first_row[c], row);
         Joined<DP> s;
-        s.add(a, c, parts[c], row, rows, 0, 1);
+        s.template add<4>(a, c, parts[c], row, rows, 0, 1);
         const float scale = 1.f / s.l;
 #pragma unroll
         for (int k = 0; k < PER; ++k)
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
       int64_t row;
       T *out = row_at(c, task - first_row[c], row);
       Joined<DP> s;
-      s.add(a, c, parts[c], row, rows, warp, JOIN_WARPS);
+      s.template add<8>(a, c, parts[c], row, rows, warp, JOIN_WARPS);
       if (lane == 0) {
         st_m[warp] = s.m;
         st_l[warp] = s.l;
@@ -584,7 +585,8 @@ template <int DP>
 struct CoreShape {
   static constexpr int KP = DP + 8, VP = DP + 4;  // floats of a row of K (two lanes to a key: no conflicts) and of V
   static constexpr int STAGE = CHUNK * (KP + VP);
-  static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 4 : DP >= 64 ? 5 : 6;
+  static constexpr int BLOCKS = DP >= 128 ? 1 : DP >= 64 ? 2 : 3;  // of an SM
+  static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 2 : DP >= 64 ? 2 : 3;
   static constexpr int RING = STAGES * STAGE;  // floats of a warp
   static constexpr int OP = DP + 4;
 };
@@ -602,7 +604,8 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
   extern __shared__ __align__(128) float fsm[];
   float *ring = fsm + (threadIdx.x >> 5) * S::RING;
   float *qs = fsm + WARPS * S::RING;                      // (R, DP)
-  float *ps = qs + R * DP + (threadIdx.x >> 5) * CHUNK * R;  // (CHUNK, R); below 0: not seen
+  // P of a chunk: (R / 4, CHUNK) times four rows; below 0: not seen
+  float4 *ps = reinterpret_cast<float4 *>(qs + R * DP + (threadIdx.x >> 5) * CHUNK * R);
   __shared__ int64_t off_k[WARPS][CHUNK], off_v[WARPS][CHUNK];
   __shared__ uint32_t have[WARPS][S::STAGES];
   __shared__ Near near;
@@ -724,25 +727,46 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const bool ok = (seen >> r) & 1;
-          const float p = ok ? ex2((s[r] - m[r]) * a.c2) : -1.f;
-          if (part == 0) {
-            if (ok) l[r] += p;
-            ps[mykey * R + r] = p;
-          }
+          s[r] = ok ? ex2((s[r] - m[r]) * a.c2) : -1.f;
+          if (part == 0 && ok) l[r] += s[r];
         }
+#pragma unroll
+        for (int r = 0; r < R / 4; ++r)  // a key's two lanes write half of its rows each
+          if (part == (2 * r) / (R / 4 + R / 4 % 2)) ps[r * CHUNK + mykey] = make_float4(s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]);
         __syncwarp();
         if (col < DP) {
+          if (!uneven) {
 #pragma unroll 4
-          for (int at = share; at < CHUNK; at += SPLIT) {
-            const float4 v = *reinterpret_cast<const float4 *>(vt + at * S::VP + col);
+            for (int at = share; at < CHUNK; at += SPLIT) {
+              const float4 v = *reinterpret_cast<const float4 *>(vt + at * S::VP + col);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-              const float p = ps[at * R + r];
-              if (uneven && p < 0.f) continue;
-              o[r][0] = fmaf(p, v.x, o[r][0]);
-              o[r][1] = fmaf(p, v.y, o[r][1]);
-              o[r][2] = fmaf(p, v.z, o[r][2]);
-              o[r][3] = fmaf(p, v.w, o[r][3]);
+              for (int r4 = 0; r4 < R / 4; ++r4) {
+                const float4 p4 = ps[r4 * CHUNK + at];
+                const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  float(&y)[4] = o[4 * r4 + k];
+                  y[0] = fmaf(p[k], v.x, y[0]);
+                  y[1] = fmaf(p[k], v.y, y[1]);
+                  y[2] = fmaf(p[k], v.z, y[2]);
+                  y[3] = fmaf(p[k], v.w, y[3]);
+                }
+              }
+            }
+          } else {
+#pragma unroll 1
+            for (int at = share; at < CHUNK; at += SPLIT) {
+              const float4 v = *reinterpret_cast<const float4 *>(vt + at * S::VP + col);
+              const float *p = reinterpret_cast<const float *>(ps + at);
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                const float x = p[(r / 4) * CHUNK * 4 + r % 4];
+                if (x < 0.f) continue;
+                o[r][0] = fmaf(x, v.x, o[r][0]);
+                o[r][1] = fmaf(x, v.y, o[r][1]);
+                o[r][2] = fmaf(x, v.z, o[r][2]);
+                o[r][3] = fmaf(x, v.w, o[r][3]);
+              }
             }
           }
         }
@@ -803,7 +827,7 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
     x.pieces = sms * (x.m == 32 ? 2 : x.dp >= 128 ? 3 : 4);
   } else {
     x.m = rows <= 4 ? 4 : 16;
-    x.pieces = sms;
+    x.pieces = sms * (x.dp >= 128 ? 1 : x.dp >= 64 ? 2 : 3);
   }
   if (x.pieces > JOIN_PIECES) x.pieces = JOIN_PIECES;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
