@@ -50,7 +50,11 @@ constexpr int CHUNK = 16;           // keys that a warp takes at a time
 constexpr int KT = CHUNK * WARPS;   // keys of a tile
 // Where the page table has room for so few keys, an item is one block's: nothing is cut and nothing joined.
 constexpr int WHOLE = 512;
-constexpr int TC_FROM = 16;         // rows of an item above which the tcgen05 kernel takes over
+// Rows of an item above which the tcgen05 kernel takes over, by the rows of a TMA box: small boxes are many copies for a
+// tile.  16 sequences, up to 8192 keys, 8 / 4 heads of 96, trees of 16 (32 rows) and of 64 (128 rows), us, tcgen05 / warps:
+// pages of 16 (boxes of 16) 38 / 60 and 38 / 145; of 100 (boxes of 4) 57 / 60 and 58 / 145; of 34 (2) 87 / 61 and 86 / 146;
+// of 17 (1) 151 / 58 and 146 / 146.
+static int tc_from(int box) { return box >= 4 ? 16 : box == 2 ? 48 : 128; }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
   const int bytes = there ? 16 : 0;  // the rest is filled with zeros
@@ -811,7 +815,7 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
   Choice x{};
   const int G = H / c->kv_heads, sms = device_sm_count() > 0 ? device_sm_count() : 148;
   const int64_t rows = (s->T + s->batch - 1) / s->batch * G;
-  x.kind = most == TC && rows <= TC_FROM ? MMA : most;
+  x.kind = most == TC && rows <= tc_from(cached_attn_tc_box(c)) ? MMA : most;
   x.dp = (c->dim + 31) / 32 * 32;
   x.hw = 1;
   x.cost = 2;

@@ -214,6 +214,12 @@ __device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key)
 }  // namespace cattn
 
 constexpr int CATTN_TC_ROWS = 128, CATTN_TC_KEYS = 64, CATTN_TC_BLOCKS = 2;  // rows of an item, keys of a tile, blocks of an SM
+// rows of a TMA box: the greatest common divisor of a tile's keys, a power of two, and a page's
+inline int cached_attn_tc_box(const mhc_kv_cache *c) {
+  int rows = CATTN_TC_KEYS;
+  while (c->page_size % rows) rows /= 2;
+  return rows;
+}
 bool cached_attn_tc_eligible(const mhc_kv_cache *c);
 cudaError_t launch_cached_attn_tc(const cattn::Args &a, const mhc_kv_cache *c, cudaStream_t stream);
 int read_cat_error(bool clear);

@@ -1,6 +1,5 @@
 // Attention over a paged cache on the 5th-generation tensor cores, for items of more rows
-// than the warp-wide products of mhc_cached_attn.cu take at once (bf16 / fp16; pages that
-// divide a tile of 64 keys or are made of such tiles).
+// than the warp-wide products of mhc_cached_attn.cu take at once (bf16 / fp16).
 //
 //   S = Q K^T    tcgen05.mma, M = 128, N = 64, K = D, both operands in shared memory
 //   P = exp2((S - m) c)                         c = scale log2(e), one thread per row
@@ -14,8 +13,9 @@
 // 1.5 us a tile and 14 us for an item's two ends.)  Scores are formed one tile ahead, into the
 // other of two buffers.
 //
-// K and V come by TMA, one box for each page and 64 columns of a tile of 64 keys, the lanes
-// of a warp one page each, across the ends of items too.  V rows that do
+// K and V come by TMA, a box for the rows that lie in one page wherever a tile begins (of 64
+// keys and pages of 48, 16; of pages of 17, each by itself) and 64 columns, the lanes of a
+// warp one or two boxes each, across the ends of items too.  V rows that do
 // not exist are zeroed in shared memory (a P of 0 times a NaN would be NaN), and so are
 // infinities and NaN of new tokens' V, which some rows of the item do not see: the rows
 // that see one add it in the end.  The softmax threads do that, a row each, before they hand
@@ -83,11 +83,12 @@ __device__ __forceinline__ void mma_product(uint32_t d, uint32_t p, uint32_t v, 
   }
 }
 
-// Tensor maps of keys and values: (D, slots and heads by their strides, pages) in boxes of one page's rows (64 at most) x 64
+// Tensor maps of keys and values: (D, slots and heads by their strides, pages) in boxes of the rows that pages and tiles have in common x 64
 // columns; head_first: the second axis is the head.
 struct Maps {
   CUtensorMap k, v;
   int k_head_first, v_head_first;
+  int rows;  // of a box: they lie in one page wherever a tile begins
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *tmap, int x, int y, int z, int w, uint32_t bar) {
@@ -179,26 +180,34 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
   const uint32_t tmem = uniform(tmem_slot);
 
   if (warp == W_TMA) {
-    // ---------------- TMA: a lane for each page of a tile ----------------
+    // ---------------- TMA: the lanes have a box or two of a tile each ----------------
     bool ok = true;
     int t = 0, nk = 0, nv = 0;  // key tiles, K and V tiles asked for so far
-    const int rows = min(a.c.size, TN), boxes = TN / rows;  // of a box, in a tile
+    const int rows = maps.rows, boxes = TN / rows;  // of a box, in a tile
     walk<M>(a, near, [&](const Segment &g, int) {
       if (!ok) return;
       for (int j = g.k0; j < g.k1; ++j, ++t) {
-        const int s = t % ST, key = j * TN + lane * rows;
+        const int s = t % ST;
         const uint32_t free_par = ((uint32_t)(t / ST) & 1u) ^ 1u;
-        int page = lane < boxes ? page_of(a, g, key) : -1;
-        if (page >= a.c.pages) page = -1;
-        const int slot = page >= 0 ? key - cache::page_index(a.c, key) * a.c.size : 0;
-        const uint32_t bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, page >= 0)) * rows * 128) * C::FULL;
-        auto load = [&](uint32_t dst, const CUtensorMap &map, int head_first, uint32_t bar) {
-          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-          __syncwarp();
-          if (page >= 0)
+        int page[2], slot[2], count = 0;  // a lane's boxes
 #pragma unroll
-            for (int b = 0; b < C::FULL; ++b)
-              tma_load_4d(dst + b * KBLK + lane * rows * 128, &map, b * 64, head_first ? g.hk : slot, head_first ? slot : g.hk, page, bar);
+        for (int u = 0; u < 2; ++u) {
+          const int box = lane + 32 * u, key = j * TN + box * rows;
+          page[u] = box < boxes ? page_of(a, g, key) : -1;
+          if (page[u] >= a.c.pages) page[u] = -1;
+          slot[u] = page[u] >= 0 ? key - cache::page_index(a.c, key) * a.c.size : 0;
+          count += __popc(__ballot_sync(0xffffffffu, page[u] >= 0));
+        }
+        auto load = [&](uint32_t dst, const CUtensorMap &map, int head_first, uint32_t bar) {
+          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * rows * 128) * C::FULL);
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (page[u] >= 0)
+#pragma unroll
+              for (int b = 0; b < C::FULL; ++b)
+                tma_load_4d(dst + b * KBLK + (lane + 32 * u) * rows * 128, &map, b * 64, head_first ? g.hk : slot[u],
+                            head_first ? slot[u] : g.hk, page[u], bar);
         };
         if (!wait_warp_parity(BAR(B_KE + s), free_par, abort_flag)) { ok = false; break; }
         load(ks + s * C::TILE, maps.k, maps.k_head_first, BAR(B_KF + s));
@@ -262,7 +271,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const uint32_t s_addr = tmem + lanes + S_COL, o_addr = tmem + lanes + O_COL;
     const uint64_t c2 = f2_pack(a.c2, a.c2), lift2 = f2_pack(LIFT, LIFT);
-    const int psize = min(a.c.size, TN), boxes = TN / psize;
+    const int rows = maps.rows, boxes = TN / rows;
     bool ok = true;
     int sf[2] = {0, 0}, of[2] = {0, 0}, tile0 = 0, items = 0;  // score tiles taken from and products asked of each buffer; key tiles of earlier items
     walk<M>(a, near, [&](const Segment &g, int slot) {
@@ -296,8 +305,12 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
       for (int i = 0; i < n; ++i) {
         const int k0 = (g.k0 + i) * TN, s = i & 1;
         // which of the tile's pages there are
-        const int page = lane < boxes ? page_of(a, g, k0 + lane * psize) : 0;
-        const unsigned missing = __ballot_sync(0xffffffffu, lane < boxes && k0 + lane * psize < g.keys && (page < 0 || page >= a.c.pages));
+        uint64_t missing = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int box = lane + 32 * u, key = k0 + box * rows, page = box < boxes ? page_of(a, g, key) : 0;
+          missing |= (uint64_t)__ballot_sync(0xffffffffu, box < boxes && key < g.keys && (page < 0 || page >= a.c.pages)) << (32 * u);
+        }
         if (!wait_warp_parity(BAR(B_SF + s), (uint32_t)sf[s] & 1u, abort_flag)) { ok = false; break; }
         ++sf[s];
         tc_fence_after();
@@ -319,7 +332,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
               if (missing) {
 #pragma unroll 1
                 for (int e = 0; e < 32; ++e)
-                  if ((missing >> ((q * 32 + e) / psize)) & 1) seen &= ~(1u << e);
+                  if ((missing >> ((q * 32 + e) / rows)) & 1) seen &= ~(1u << e);
               }
               some = some || seen;
 #pragma unroll
@@ -378,7 +391,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
         if (missing || fresh || k0 + TN > g.keys) {  // thread r looks after half of V's row r / 2
           const int tile = tile0 + i, st = tile % ST, vr = r >> 1, at = k0 + vr;
           if (!wait_warp_parity(BAR(B_VF + st), (uint32_t)(tile / ST) & 1u, abort_flag)) { ok = false; break; }
-          const bool gone = at >= g.keys || ((missing >> (vr / psize)) & 1);
+          const bool gone = at >= g.keys || ((missing >> (vr / rows)) & 1);
           if (gone || (fresh && at >= g.s.len)) {
             uint8_t *row = gen + (vs - base) + st * C::TILE + vr * 128;
 #pragma unroll
@@ -509,10 +522,9 @@ bool axes_ok(const mhc_kv_cache *c, const Axes &x) {
   return x.slot % 8 == 0 && x.head % 8 == 0 && x.page % 8 == 0 && x.slot >= c->dim && x.head >= c->dim && x.page >= x.slot && x.page >= x.head &&
          x.page < most;
 }
-bool make_map(CUtensorMap *map, const mhc_kv_cache *c, void *p, const Axes &x) {
+bool make_map(CUtensorMap *map, const mhc_kv_cache *c, void *p, const Axes &x, cuuint32_t rows) {
   auto enc = encode_fn();
   if (!enc) return false;
-  const cuuint32_t rows = c->page_size < TN ? c->page_size : TN;
   const cuuint64_t dims[4] = {(cuuint64_t)c->dim, (cuuint64_t)(x.head_first ? c->kv_heads : c->page_size),
                               (cuuint64_t)(x.head_first ? c->page_size : c->kv_heads), (cuuint64_t)c->pages};
   const cuuint64_t strides[3] = {(cuuint64_t)(x.head_first ? x.head : x.slot) * 2, (cuuint64_t)(x.head_first ? x.slot : x.head) * 2,
@@ -536,18 +548,17 @@ cudaError_t run(const Args &a, const Maps &maps, cudaStream_t stream) {
 }  // namespace
 }  // namespace cattn
 
-// What TMA asks of the cache: rows of 16-byte multiples that do not overlap, in pages of which a tile of 64 keys has a
-// whole number, or the other way round.
+// What TMA asks of the cache: rows of 16-byte multiples that do not overlap.
 bool cached_attn_tc_eligible(const mhc_kv_cache *c) {
-  if (c->dtype == MHC_F32 || c->dim % 8 || c->page_size % 8 || (CATTN_TC_KEYS % c->page_size && c->page_size % CATTN_TC_KEYS)) return false;
-  if ((uintptr_t)c->keys % 16 || (uintptr_t)c->values % 16) return false;
+  if (c->dtype == MHC_F32 || c->dim % 8 || (uintptr_t)c->keys % 16 || (uintptr_t)c->values % 16) return false;
   return cattn::axes_ok(c, cattn::axes_of(c, c->strides)) && cattn::axes_ok(c, cattn::axes_of(c, c->strides + 4));
 }
 
 cudaError_t launch_cached_attn_tc(const cattn::Args &a, const mhc_kv_cache *c, cudaStream_t stream) {
   cattn::Maps maps;
   const cattn::Axes k = cattn::axes_of(c, c->strides), v = cattn::axes_of(c, c->strides + 4);
-  if (!cattn::make_map(&maps.k, c, c->keys, k) || !cattn::make_map(&maps.v, c, c->values, v)) return cudaErrorNotSupported;
+  maps.rows = cached_attn_tc_box(c);
+  if (!cattn::make_map(&maps.k, c, c->keys, k, maps.rows) || !cattn::make_map(&maps.v, c, c->values, v, maps.rows)) return cudaErrorNotSupported;
   maps.k_head_first = k.head_first;
   maps.v_head_first = v.head_first;
   auto go = [&](auto tag) -> cudaError_t {
