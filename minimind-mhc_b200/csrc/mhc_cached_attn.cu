@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
 
 template <int DP>
 struct CoreShape {
-  static constexpr int KP = DP + 8, VP = DP + 4;  // floats of a row of K (two lanes to a key: no conflicts) and of V
+  static constexpr int KP = DP + 8, VP = DP;  // floats of a row of K (two lanes to a key: no conflicts) and of V
   static constexpr int STAGE = CHUNK * (KP + VP);
   static constexpr int BLOCKS = DP >= 128 ? 1 : DP >= 64 ? 2 : 3;  // of an SM
   static constexpr int STAGES = DP >= 128 ? 3 : DP >= 96 ? 2 : DP >= 64 ? 2 : 3;

@@ -49,7 +49,7 @@ __device__ __forceinline__ int keys_of(const cache::View &v, const cache::Seq &s
 }
 
 // The step's offsets and lengths in shared memory, where they are few: every warp looks them up for every item.
-constexpr int NEAR = 128;
+constexpr int NEAR = 96;
 struct Near {
   int cu[NEAR + 1], len[NEAR];
   // by all threads of the block; a barrier has to follow
