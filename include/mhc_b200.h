@@ -627,7 +627,8 @@ int mhc_last_path(void);
  * the single-read forward kernel, 31..37 = the producer / MMA / row /
  * coefficient / pre-aggregate / Sinkhorn / merge role of the fused merge +
  * coefficient kernel, 41..43 and 51..53 = the TMA / MMA / softmax
- * role of the attention forward and backward kernels, 11..14 = one of the producer / MMA /
+ * role of the attention forward and backward kernels, 61..63 = those of the
+ * attention over a paged cache, 11..14 = one of the producer / MMA /
  * epilogue / prep roles of the backward tensor-core kernel, 99 = the
  * self-test below).  A kernel whose wait runs out gives up
  * instead of hanging and overwrites the outputs it owns with NaN.

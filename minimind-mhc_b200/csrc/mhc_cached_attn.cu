@@ -5,19 +5,33 @@
 //
 // Few rows share a long row of keys: the bound is reading keys and values once.  All
 // query heads of a key head and all new tokens of a sequence are rows of one item (see
-// the header for the cut), so a key is read once for up to 16 or 32 rows.
+// the header for the cut), so a key is read once for up to 8, 16 or 32 rows; more rows go to
+// mhc_cached_attn_tc.cu.
 //
-// A warp works alone: of every tile of 64 keys it takes 16, brings their K and V rows into
-// a ring of its own with cp.async, three to eight chunks ahead, forms the scores, keeps its
-// own running reference and sums, and adds up O in registers.  No barrier stands between
-// the warps until an item ends; then their four sums are joined through shared memory.
-// Page numbers are fetched one chunk ahead of the rows that they lead to.
+// A warp works alone: it takes 16 keys at a time, brings their K and V rows into a ring of
+// its own with cp.async, forms the scores, keeps its own running reference and sums, and
+// adds up O in registers.  The four warps of a block take neighbouring key heads of the same
+// keys, whose rows lie side by side in memory, or, where there are fewer, neighbouring
+// keys.  No barrier stands between the warps until an item ends; then those of one head
+// join their sums through shared memory.  Page numbers are fetched one chunk ahead of the
+// rows that they lead to; where pages are multiples of 16 keys a chunk has one page and a
+// lane's addresses are a base and steps.
 //
-// 16-bit types: mma.sync m16n8k16, S = Q K^T with Q in registers, O += P V with P from the
-// scores' registers.  The matrix unit is not what bounds these few rows (16 rows of 128 need
-// 104 TFLOP/s at the copy rate); the rows are few for the 128 of tcgen05.mma.
+// 16-bit types: mma.sync m16n8k16 with the queries as the narrow operand, S^T = K Q^T and
+// O^T += V^T P^T, so that 8 rows waste nothing and O takes 32 registers a lane at heads of
+// 128 (with the queries as the 16 rows: twice that, two blocks an SM for four, and 123 us
+// where this takes 67).  P goes from the scores' registers to the second operand's by
+// movmatrix.  The matrix unit is not what bounds these few rows (16 rows of 128 need 104
+// TFLOP/s at the copy rate); they are few for the 128 of tcgen05.mma.
 // fp32 and what 16-byte copies cannot fetch (odd head sizes, strides, alignment): CUDA cores,
 // the same structure on fp32 copies of the rows, two lanes to a key.
+//
+// Measured (with the join): 64 sequences of one token, 239,000 keys in all, 8 / 4 heads of
+// 96, bf16: 74 us, 5.0 TB/s; one token over 200 keys 9.2 us; fp32, 16 sequences, 67,000 keys:
+// 57 us, 3.6 TB/s, and with trees of 16 over 16,000 keys 72 us (instructions: 4 FMA for
+// every shared-memory read of 16 bytes).  Bringing the rows by bulk copies (one a row)
+// measured 4.5 TB/s at rows of 128 bytes and 1.8 at 64 against 6.2 and 5.2 by cp.async, and 6.7
+// against 6.4 at 256.
 //
 // The reference m of a row is moved (and O and the sum rescaled) only when a score passes it
 // by 2^8 (fp16: 2^4, and P is held times 2^10, so that what is 2^-34 of the largest still

@@ -21,6 +21,12 @@
 // that see one add it in the end.  The softmax threads do that, a row each, before they hand
 // over P.
 //
+// What bounds it: a tile takes a block 1.0 to 1.2 us (two of them an SM: 32 KB of K and V each,
+// at 128 rows the softmax's chain and 2^x, at 32 rows HBM: 1.5 us a tile is the copy rate); an item's
+// two ends about 10 us, half of it instructions that have not run before.  Measured (with the
+// join): 16 sequences with trees of up to 64, 127,000 keys in all, 8 / 2 heads of 128, 256 rows:
+// 55 us; 16 tokens over 131,072 keys, 8 / 4 heads of 128: 57 us, 4.7 TB/s.
+//
 // Warps 0-3: softmax, a row each; 4: TMA; 5: MMA issue.  Every wait is bounded; a block whose
 // wait runs out writes NaN over its share.
 #include <cfloat>

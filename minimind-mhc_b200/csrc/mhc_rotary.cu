@@ -21,7 +21,10 @@
 //
 // Neighbouring threads take neighbouring places and heads: with a token's angles in the
 // registers of a thread that walks over its heads the instructions are a third, but a
-// warp's accesses lie 1.5 KB apart, and 16384 tokens of 12 heads of 96 took 27 us for 19.
+// warp's accesses lie 1.5 KB apart, and 16384 tokens of 12 heads of 96 took 27 us for 15.
+// Measured: those 14.7 us (75 MB, 5.1 TB/s), 8191 tokens of 10 heads of 128 in fp32 14.4 us
+// (84 MB, 5.8 TB/s); into a cache 24 prompts, 17,900 tokens, 24 us (110 MB, 4.5 TB/s), one token of
+// each of 16 sequences 3.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < tokens * a.half; i += THREADS) {
+  for (int i = tid; i < tokens * a.half; i += blockDim.x) {
     const int t = i / a.half, p = i - t * a.half, place = p / VEC;
     table[t * a.half + (p - place * VEC) * a.pair_items + place] = angle(a.turns[p], at_pos[t], a.gain, a.sign);
   }
@@ -247,7 +250,10 @@ static cudaError_t launch(Args a, int dtype, bool ilv, bool with_cache, cudaStre
   const int vec = usable(wide) ? wide : usable(wide / 2) ? wide / 2 : 1;
   a.pair_items = a.half / vec;
   a.items = a.pair_items + (a.D - a.part) / vec;
-  a.rows_at_once = THREADS / a.items;
+  // half blocks where a few tokens fit them: the last ones end nearer together (16384 tokens of 12 heads of 96, both
+  // directions: 30.5 us with whole ones, 29.4 with half; 8191 of 10 heads of 128, fp32: 15.2, 14.4)
+  const int threads = a.items <= THREADS / 4 ? THREADS / 2 : THREADS;
+  a.rows_at_once = threads / a.items;
   if (a.rows_at_once < 1) return cudaErrorInvalidValue;
   const int heads = a.H + a.Hk + a.Hv;
   a.twos = (heads + 1) / 2;
@@ -265,7 +271,7 @@ static cudaError_t launch(Args a, int dtype, bool ilv, bool with_cache, cudaStre
     using T = decltype(tag);
     constexpr int W = 16 / (int)sizeof(T);
     auto go = [&](auto v, auto i, auto c) -> cudaError_t {
-      rotary_kernel<T, decltype(v)::value, decltype(i)::value != 0, decltype(c)::value != 0><<<(unsigned)blocks, THREADS, smem, st>>>(a);
+      rotary_kernel<T, decltype(v)::value, decltype(i)::value != 0, decltype(c)::value != 0><<<(unsigned)blocks, threads, smem, st>>>(a);
       return cudaGetLastError();
     };
     auto by_vec = [&](auto i, auto c) -> cudaError_t {

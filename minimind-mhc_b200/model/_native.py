@@ -223,7 +223,8 @@ ERROR_ROLES = {1: "forward TMA producer", 2: "forward MMA issuer", 3: "forward r
                41: "attention forward TMA warp", 42: "attention forward MMA issuer",
                43: "attention forward softmax warps",
                51: "attention backward TMA warp", 52: "attention backward MMA issuer",
-               53: "attention backward softmax warps", 99: "bounded-wait self-test"}
+               53: "attention backward softmax warps", 61: "cached attention TMA warp",
+               62: "cached attention MMA issuer", 63: "cached attention softmax warps", 99: "bounded-wait self-test"}
 
 _flag_tensor = None   # pinned int32 host tensor registered with the library
 _flag_word = None     # ctypes view of its first element
