@@ -496,7 +496,7 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
  *   kept    if random[x] * mass * draft(x) < rest(x)   (draft(x) = 1 without a draft);
  *           then rest = x's target row, mass = 1;
  *   refused otherwise: rest = max(rest - mass * draft, 0), mass = sum of rest; without a
- *           draft mass -= rest(x), rest(x) = 0.
+ *           draft mass = max(mass - rest(x), 0), rest(x) = 0.
  * In the end next[b] is drawn from rest: the first token whose cumulative sum passes
  * random[row 0] * sum.  If nothing is left of rest, it is drawn from the node's target
  * row; if that holds nothing positive and finite either, next[b] is -1.  NaN and negative entries

@@ -173,6 +173,7 @@ struct Joined {
 template <typename T, int M, int DP>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   grid_dep_wait();
+  grid_dep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int first_row[JOIN_PIECES + 1];  // rows of the cut items that begin in blocks before c
   __shared__ int parts[JOIN_PIECES];
@@ -358,6 +359,7 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
   const float ahead = fminf(AHEAD / a.c2, FLT_MAX);
   if (D < DP)
     for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+  grid_dep_wait();
   near.fill(a);
   clear_rest<T>(a);
   __syncthreads();
@@ -633,6 +635,7 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.D;
   const float ahead = fminf(8.f / a.c2, FLT_MAX);
   for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
+  grid_dep_wait();
   near.fill(a);
   clear_rest<T>(a);
   __syncthreads();
@@ -859,28 +862,17 @@ static Choice choose(const mhc_kv_cache *c, const mhc_cache_step *s, int H, Kind
 
 template <typename K>
 static cudaError_t start(K kernel, const Args &a, int blocks, int smem, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  kernel<<<blocks, THREADS, smem, st>>>(a);
-  return cudaGetLastError();
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e != cudaSuccess ? e : launch_early(kernel, dim3((unsigned)blocks), THREADS, smem, st, a);
 }
 
 // the join begins while the last blocks of the first kernel still run, and waits for them on the device
 template <typename T, int M, int DP>
 static cudaError_t join(const Args &a, cudaStream_t st) {
   if (a.whole) return cudaSuccess;
-  cudaLaunchConfig_t cfg{};
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
   const int64_t rows = (int64_t)a.c.T * a.H;
-  cfg.gridDim = dim3((unsigned)(rows < 4 * sms ? rows : 4 * sms));
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, M, DP>, a);
+  return launch_early(join_kernel<T, M, DP>, dim3((unsigned)(rows < 4 * sms ? rows : 4 * sms)), JOIN_THREADS, 0, st, a);
 }
 
 template <typename F>

@@ -211,6 +211,23 @@ __device__ __forceinline__ int page_of(const Args &a, const Segment &g, int key)
   return key < g.keys ? a.c.table[g.b * a.c.pitch + cache::page_index(a.c, key)] : -1;
 }
 
+// Launches a kernel that may begin before the one in front of it in the stream has ended (where that one allows it) and
+// that waits on the device (grid_dep_wait) before it touches any memory that others write.
+template <typename K, typename... A>
+inline cudaError_t launch_early(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace cattn
 
 constexpr int CATTN_TC_ROWS = 128, CATTN_TC_KEYS = 64, CATTN_TC_BLOCKS = 2;  // rows of an item, keys of a tile, blocks of an SM

@@ -178,6 +178,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
     tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
+  grid_dep_wait();
   near.fill(a);
   clear_rest<T>(a);
   tc_fence_before();
@@ -547,8 +548,7 @@ cudaError_t run(const Args &a, const Maps &maps, cudaStream_t stream) {
   auto kern = cached_attn_tc_kernel<T, DP>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
   if (e != cudaSuccess) return e;
-  kern<<<a.pieces, NTHREADS, C::SMEM, stream>>>(maps, a);
-  return cudaGetLastError();
+  return launch_early(kern, dim3((unsigned)a.pieces), NTHREADS, C::SMEM, stream, maps, a);
 }
 
 }  // namespace

@@ -139,6 +139,7 @@ template <typename T, int VEC, bool ILV, bool CACHE>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
   extern __shared__ Cs table[];  // of token t: pair i of place p at t half + i (half / VEC) + p
   __shared__ int64_t at_k[MAX_TOKENS], at_v[MAX_TOKENS], at_pos[MAX_TOKENS];
+  grid_dep_launch();  // the attention behind an append sets itself up meanwhile
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int tokens = (int)min((int64_t)a.tokens, a.T - t0);

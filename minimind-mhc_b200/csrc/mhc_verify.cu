@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(THREADS, 2) verify_kernel(const Args a) {
         r.gone += mass;
         mass = sum_rest();
       } else {
-        mass -= left;
+        mass = fmax(mass - left, 0.0);  // a row may sum to a little more than 1
         __syncthreads();
         if (tid == 0) sh.refused[r.refused] = sh.token[x];
         ++r.refused;

@@ -33,7 +33,7 @@ def verify_drafts(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.
 
     The children x of the last kept row are tested in their order.  With rest the target's row and mass 1 at first, x is
     kept if ``random * mass * draft(x) < rest(x)`` (draft(x) = 1 without a draft).  If not, rest becomes
-    max(rest - mass * draft, 0), mass its sum; without a draft mass loses rest(x) and rest(x) becomes 0.  The next token
+    max(rest - mass * draft, 0), mass its sum; without a draft mass loses rest(x), down to 0, and rest(x) becomes 0.  The next token
     is the first whose cumulative sum of rest exceeds the first row's random number times the sum.  Where nothing of
     rest is left it is drawn from the target's row; -1 if that has no positive finite sum, and for empty sequences.
     Sums are fp64.  NaN and negative probabilities count as 0; tokens outside the vocabulary, parents that do not come

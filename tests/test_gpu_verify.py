@@ -39,7 +39,7 @@ def by_hand(tokens, parents, cu, target, draft, random, limit=1024):
                 rest = (rest - mass * off).clamp(min=0)
                 mass = float(rest.sum())
             else:
-                mass -= left
+                mass = max(mass - left, 0.0)
                 rest = rest.clone()
                 rest[x] = 0
         if not (0 < float(rest.sum()) < torch.inf):
@@ -134,6 +134,16 @@ def test_refusals_one_after_another():
     check(torch.full_like(tokens, 5), parents, cu, target, draft, random)
     check(torch.full_like(tokens, 5), parents, cu, target, None, random)
     check(torch.arange(n, device="cuda"), parents, cu, target, None, random)
+
+
+def test_children_that_use_the_row_up():
+    """Without a draft: a row that sums to a little more than 1, all of it refused: a token that it does not hold is not kept."""
+    target = torch.zeros(5, 9, device="cuda")
+    target[:, 2], target[:, 4] = 0.6, 0.40000004
+    cu, parents = torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.tensor([-1, 0, 0, 0, 0], dtype=torch.int32, device="cuda")
+    random = torch.tensor([0.3, 1.0, 1.0, 1.0, 1.0], device="cuda")  # (1 refuses all that it can; the draw stays off the borders)
+    got = check(torch.tensor([0, 2, 4, 7, 7], device="cuda"), parents, cu, target, None, random)
+    assert got.kept.tolist() == [1] or got.path[1] == 2   # the second one may be kept: what is left is less than it
 
 
 def test_empty_sequences_and_rows_of_none():
