@@ -129,7 +129,10 @@ __device__ __forceinline__ void join_warps(const Args &a, const Segment &g, int 
 // Joins the blocks that had part of a cut item.  Every block lists the cut items (one entry for each block of the first
 // kernel); a warp takes one row at a time and goes through its parts, AT_ONCE of them under way.  Where a row has more
 // than a few the block's warps share them and join what they have through shared memory.
-constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_PIECES = 1024;
+// Blocks of eight warps where rows have few parts, of sixteen where they have many (us for the whole call with blocks of 4 /
+// 8 / 16 warps: 64 sequences of one token, nine parts a row, 76 / 74 / 80; trees of 64, five parts, 58 / 55 / 62; one token
+// over 131,072 keys, 592 parts, - / 56 / 51).
+constexpr int JOIN_PIECES = 1024;
 constexpr int JOIN_ALONE = 16;  // parts that a warp goes through by itself
 
 template <int DP>
@@ -170,8 +173,9 @@ struct Joined {
   }
 };
 
-template <typename T, int M, int DP>
+template <typename T, int M, int DP, int JOIN_THREADS>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
+  constexpr int JOIN_WARPS = JOIN_THREADS / 32;
   grid_dep_wait();
   grid_dep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -591,9 +595,9 @@ __global__ void __launch_bounds__(THREADS, MmaShape<DP, R>::BLOCKS) mma_kernel(c
     __syncthreads();
     join_warps<T, M, DP>(a, g, slot, rows, reinterpret_cast<const float *>(smem), S::OP, S::RING / 4, ml, fac, true);
     __syncthreads();
-    if (D < DP) {  // columns past D are zeros again
-      for (int i = tid; i < S::SMEM / 16; i += THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
+    if (D < DP) {  // columns past D, where O lay, are zeros again
+      for (int i = lane; i < M * S::OP / 4; i += 32) reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
     }
   });
   grid_dep_launch();
@@ -810,9 +814,9 @@ __global__ void __launch_bounds__(THREADS) core_kernel(const Args a) {
     __syncthreads();
     join_warps<T, R, DP>(a, g, slot, rows, fsm, S::OP, S::RING, ml, fac, a.c.D % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0);
     __syncthreads();
-    if (D < DP)  // columns past D are zeros again
-      for (int i = tid; i < WARPS * S::RING; i += THREADS) fsm[i] = 0.f;
-    __syncthreads();
+    if (D < DP)  // columns past D, where O lay, are zeros again
+      for (int i = lane; i < R * S::OP; i += 32) ring[i] = 0.f;
+    __syncwarp();
   });
   grid_dep_launch();
 }
@@ -872,7 +876,9 @@ static cudaError_t join(const Args &a, cudaStream_t st) {
   if (a.whole) return cudaSuccess;
   const int sms = device_sm_count() > 0 ? device_sm_count() : 148;
   const int64_t rows = (int64_t)a.c.T * a.H;
-  return launch_early(join_kernel<T, M, DP>, dim3((unsigned)(rows < 4 * sms ? rows : 4 * sms)), JOIN_THREADS, 0, st, a);
+  const int64_t items = (int64_t)a.c.batch * a.groups;  // one tile of rows each, at least
+  if (a.pieces > JOIN_ALONE * items) return launch_early(join_kernel<T, M, DP, 512>, dim3((unsigned)(rows < 2 * sms ? rows : 2 * sms)), 512, 0, st, a);
+  return launch_early(join_kernel<T, M, DP, 256>, dim3((unsigned)(rows < 4 * sms ? rows : 4 * sms)), 256, 0, st, a);
 }
 
 template <typename F>
