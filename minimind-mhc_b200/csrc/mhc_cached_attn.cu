@@ -27,8 +27,8 @@
 // the same structure on fp32 copies of the rows, two lanes to a key.
 //
 // Measured (with the join): 64 sequences of one token, 239,000 keys in all, 8 / 4 heads of
-// 96, bf16: 74 us, 5.0 TB/s; one token over 200 keys 9.2 us; fp32, 16 sequences, 67,000 keys:
-// 57 us, 3.6 TB/s, and with trees of 16 over 16,000 keys 72 us (instructions: 4 FMA for
+// 96, bf16: 75 us, 4.9 TB/s; one token over 200 keys 8.9 us; fp32, 16 sequences, 67,000 keys:
+// 56 us, 3.7 TB/s, and with trees of 16 over 16,000 keys 73 us (instructions: 4 FMA for
 // every shared-memory read of 16 bytes).  Bringing the rows by bulk copies (one a row)
 // measured 4.5 TB/s at rows of 128 bytes and 1.8 at 64 against 6.2 and 5.2 by cp.async, and 6.7
 // against 6.4 at 256.

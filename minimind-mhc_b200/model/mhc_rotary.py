@@ -18,17 +18,16 @@ import torch
 
 from . import _native as nat
 
-# 2^320 / (2 pi): a frequency's turns need the bits behind a double's last
-_TURNS_BITS = 320
+# 2^192 / (2 pi): a frequency's turns need the bits behind a double's last
 _TURNS = (159154943091895335768883763372514362034459645740456448747667344058896797634226535090113802766253085956072842726757958
-          << _TURNS_BITS) // 10 ** 117
+          << 192) // 10 ** 117
 
 
 def _turns_of(f: float) -> int:
     """round(f / (2 pi) * 2^64) modulo 2^64."""
-    n, d = f.as_integer_ratio()  # d is a power of two
-    shift = _TURNS_BITS - 64
-    return (((n * _TURNS // d) + (1 << (shift - 1))) >> shift) & ((1 << 64) - 1)
+    n, d = f.as_integer_ratio()
+    shift = 127 + d.bit_length()  # d is a power of two
+    return ((n * _TURNS + (1 << (shift - 1))) >> shift) & 0xFFFFFFFFFFFFFFFF
 
 
 class Rotary:
