@@ -85,16 +85,17 @@ def keep_drafts(keys: torch.Tensor, values: torch.Tensor, step: CacheStep, path:
 def tree_mask(parents: torch.Tensor, cu_tokens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(mask, depth) of drafted trees: for every row the bits of itself and its ancestors, and how many ancestors it has.
 
-    ``parents`` (T,) is the index of a row's parent within its sequence, below its own; -1 for the first.  Trees of up to
-    64 rows.  Plain torch operations, on the tensors' device and without waiting for it: a tree that stays the same is
+    ``parents`` (T,) is the index of a row's parent within its sequence, below its own; -1 for the first.  (A row whose
+    parent is none of that, rows of no sequence among them, is taken for a first one.)  Trees of up to 64 rows.  Plain torch operations, on the tensors' device and without waiting for it: a tree that stays the same is
     done once.
     """
     t = parents.shape[0]
     at = torch.arange(t, device=parents.device)
     start = cu_tokens.long()[torch.searchsorted(cu_tokens[1:].long().contiguous(), at, right=True).clamp(max=cu_tokens.numel() - 2)]
-    up = torch.where(parents >= 0, start + parents.long(), at)  # a root is its own parent
+    child = (parents >= 0) & (parents < at - start)
+    up = torch.where(child, start + parents.long(), at)  # a root is its own parent
     mask = torch.ones_like(at) << (at - start).clamp(0, 63)
-    depth = (parents >= 0).long()
+    depth = child.long()
     for _ in range(6):  # the ancestors at twice the distance
         mask, depth, up = mask | mask[up], depth + depth[up], up[up]
     return mask, depth

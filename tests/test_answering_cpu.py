@@ -190,3 +190,8 @@ def test_tree_mask():
     parents = torch.tensor([-1, 0, 0, 1, 3, -1, -1, 0, 1], dtype=torch.int32)
     mask, depth = tree_mask(parents, torch.tensor([0, 5, 6, 6, 9], dtype=torch.int32))
     assert mask.tolist() == [1, 3, 5, 11, 27, 1, 1, 3, 7] and depth.tolist() == [0, 1, 1, 2, 3, 0, 0, 1, 2]
+    # rows of no sequence, parents that do not come before their row
+    parents = torch.tensor([7, -1, 0, 5, 1, 2 ** 31 - 1, 1, -9], dtype=torch.int32)
+    mask, depth = tree_mask(parents, torch.tensor([1, 5], dtype=torch.int32))
+    assert mask[1:5].tolist() == [1, 3, 4, 11] and depth.tolist()[:5] == [0, 0, 1, 0, 2] and depth.tolist()[7] == 0
+    assert tree_mask(parents[:0], torch.tensor([0], dtype=torch.int32))[0].numel() == 0
