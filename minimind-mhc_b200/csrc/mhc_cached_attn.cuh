@@ -5,8 +5,9 @@
 // units more, for its beginning and end.  The lengths are known on the device only, so
 // every block sums the units of all sequences itself (a few loads and one warp's scan) and
 // takes its share of the row of all units, W / N of them and the first W % N blocks one more:
-// equal work whatever the lengths.  An item that lies in one block is finished there; of one that is cut the blocks
-// leave their sums, references and rows, which a second kernel joins, in the blocks' order.
+// equal work whatever the lengths.  An item that lies in one block is finished there; of one
+// that is cut the blocks leave their sums, references and rows, which a second kernel joins,
+// in the blocks' order.
 #pragma once
 
 #include "mhc_cache.cuh"
@@ -75,16 +76,20 @@ struct Cut {
   __device__ __forceinline__ Cut(const Args &args, const Near &steps) : a(args), near(steps) {
     const int lane = threadIdx.x & 31;
     per = (a.c.batch + 31) / 32;
-    sum = 0;
-    for (int i = 0; i < per; ++i) sum += units(lane * per + i);
-    int inc = sum;
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) mine += units(lane * per + i);
+    int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += up;
     }
-    first = inc - sum;
-    total = __shfl_sync(0xffffffffu, inc, 31);
+    // the host has seen to it that 32 bits hold the units of any lengths; of offsets that are none (they decrease, and
+    // the sequences have more rows than there are) nothing is done
+    const int64_t all = __shfl_sync(0xffffffffu, inc, 31);
+    total = all > 0x7fffffff ? 0 : (int)all;
+    first = (int)(inc - mine);
+    sum = (int)mine;
   }
   __device__ __forceinline__ int tiles(int keys) const { return max(1, (keys + a.tile - 1) / a.tile); }
   __device__ __forceinline__ int row_tiles(int n) const { return (int)(((int64_t)n * a.G + M - 1) / M); }
@@ -112,7 +117,6 @@ struct Cut {
 template <int M, typename F>
 __device__ __forceinline__ void walk(const Args &a, const Near &near, F &&work) {
   const Cut<M> cut(a, near);
-  // (the host has seen to it that 32 bits hold the units of any lengths)
   const int W = cut.total, N = min(a.pieces, W), piece = blockIdx.x;
   int4 entry = make_int4(0, 0, 0, 0);
   if (piece < N) {
@@ -120,7 +124,7 @@ __device__ __forceinline__ void walk(const Args &a, const Near &near, F &&work) 
     const int w1 = each * (piece + 1) + min(piece + 1, more);
     int w = each * piece + min(piece, more), at, b;
     cut.find(w, b, at);
-    while (w < w1) {
+    while (w < w1 && b < a.c.batch) {
       Segment g;
       g.b = b;
       g.s = near.at(a, b);

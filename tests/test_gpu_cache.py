@@ -575,6 +575,30 @@ def test_decode_workload():
     assert line["value"] > 0 and 1 <= line["config"]["kept_per_step_and_sequence"] <= 16
 
 
+def test_offsets_and_lengths_that_are_none():
+    """Nothing is said of what comes out, only that every access stays inside: the cache keeps its bits where no place is, and
+    later calls are as ever."""
+    g = torch.Generator().manual_seed(5)
+    for new, columns in ((1, 2), (9, 80), (40, 80)):
+        q, keys, values, step, k, v = make([40, 9, 100], [new] * 3, 4, 2, 64, 16, torch.bfloat16, columns=columns)
+        want = cached_attention(q, keys, values, step)
+        t = q.shape[0]
+        kk, vv = (torch.randn(t, 2, 64, device="cuda").bfloat16() for _ in range(2))
+        for _ in range(12):
+            cu = torch.randint(-2 ** 31, 2 ** 31 - 1, (4,), generator=g)
+            cu = (cu if _ % 2 else cu % (2 * t + 1)).to(torch.int32).cuda()
+            lengths = torch.randint(-2 ** 31, 2 ** 31 - 1, (3,), generator=g).to(torch.int32).cuda() if _ % 3 else step.lengths
+            table = torch.randint(-2 ** 31, 2 ** 31 - 1, step.page_table.shape, generator=g).to(torch.int32).cuda() if _ % 4 else step.page_table
+            bad = CacheStep(table, lengths, cu)
+            mask = torch.randint(-2 ** 63, 2 ** 63 - 1, (t,), generator=g).cuda()
+            cached_attention(q, keys, values, bad, mask=mask if new < 64 and _ % 2 else None)
+            spare = keys.clone(), values.clone()
+            append_kv(*spare, bad, kk, vv, q=q, rotary=Rotary(64))
+            keep_drafts(*spare, bad, torch.randint(-2 ** 31, 2 ** 31 - 1, (t,), generator=g).to(torch.int32).cuda(),
+                        torch.randint(-2 ** 31, 2 ** 31 - 1, (3,), generator=g).to(torch.int32).cuda())
+        assert torch.equal(cached_attention(q, keys, values, step), want)
+
+
 def test_refused():
     q, keys, values, step, k, v = make([9, 3], [2, 1], 4, 2, 32, 8, torch.bfloat16)
     kk, vv = torch.zeros(3, 2, 32, device="cuda").bfloat16(), torch.zeros(3, 2, 32, device="cuda").bfloat16()
