@@ -412,7 +412,7 @@ int mhc_rotate(const mhc_rotary *rotary, const void *q, void *q_out, int H, cons
 
 /* Keys and values of `layers` layers in pages of page_size tokens: element (layer,
  * page, slot, head, d) of keys at the sum of its indexes times strides[0..3], plus d;
- * of values with strides[4..7] (in elements). */
+ * of values with strides[4..7] (in elements).  Up to 16384 heads. */
 typedef struct {
   void *keys, *values;
   int64_t pages, strides[8];
@@ -425,7 +425,7 @@ typedef struct {
  * page_size of page page_table[b * table_pitch + p / page_size].  All three arrays are
  * on the device and only read there: places past table_width * page_size, negative
  * ones and pages outside [0, pages) do not exist, nothing is read or written there.
- * cu_tokens is non-decreasing; rows of no sequence (behind cu_tokens[batch]) get 0
+ * cu_tokens is non-decreasing, batch up to 2^30; rows of no sequence (behind cu_tokens[batch]) get 0
  * where a call has an output for them. */
 typedef struct {
   const int32_t *page_table, *lengths, *cu_tokens;
@@ -467,7 +467,8 @@ size_t mhc_cached_attn_workspace(const mhc_kv_cache *cache, const mhc_cache_step
  *   mask == NULL: itself and those before it;
  *   else:         new token c of its sequence if bit c of mask[t] is set (c < 64).
  * q (T, H, dim) with token and head strides q_strides, out (T, H, dim) contiguous, both
- * in the cache's type; H a multiple of kv_heads, dim up to 128.  Scores, softmax and
+ * in the cache's type; H a multiple of kv_heads, dim up to 128, T (H / kv_heads) below
+ * 2^31 - 4096.  Scores, softmax and
  * sums are fp32.  A token that sees nothing gets 0.  What it does not see, NaN
  * included, does not touch it.  The same bits every time.
  *

@@ -408,6 +408,7 @@ std::optional<Tensor> adamw(const std::vector<Group> &groups, int bits, std::opt
 // ---- rotary positions -------------------------------------------------------------
 
 using Maybe = std::optional<Tensor>;
+constexpr int64_t MOST_HEADS = 16384;  // of the C entries, which count them in 32 bits
 
 // a dimension's stride; of one element none is needed, and whatever stands there must not cost the wide copies
 int64_t step_of(const Tensor &x, int64_t dim) { return x.size(dim) > 1 ? x.stride(dim) : 0; }
@@ -494,6 +495,8 @@ std::tuple<Tensor, Tensor> rotate(const Tensor &q, const Tensor &k, const Maybe 
                     k.sizes());
   bool same = q.size(-1) == k.size(-1) && q.size(0) == k.size(0) && (n == 3 || q.size(1) == k.size(1));
   TORCH_CHECK_VALUE(same && q.size(-2) >= 1 && k.size(-2) >= 1, who, ": shapes do not match: ", q.sizes(), ", ", k.sizes());
+  TORCH_CHECK_VALUE(q.size(-2) <= MOST_HEADS && k.size(-2) <= MOST_HEADS, who, ": up to ", MOST_HEADS, " heads are supported, got ", q.size(-2), " and ",
+                    k.size(-2));
   TORCH_CHECK_VALUE(q.device() == k.device() && turns.device() == q.device(), who, ": q, k and the frequencies must be on one device");
   const int64_t d = q.size(-1), part = 2 * turns.numel();
   TORCH_CHECK_VALUE(part <= d && d <= 256, who, ": heads of ", part, " (what is rotated) to 256 elements are wanted, got ", d);
@@ -540,6 +543,8 @@ Step step_of_cache(const char *who, const Tensor &keys, const Tensor &values, co
   TORCH_CHECK_VALUE(keys.device() == values.device(), who, ": keys and values must be on one device");
   const int64_t d = keys.size(f + 3);
   TORCH_CHECK_VALUE(keys.size(f + 1) >= 1 && keys.size(f + 2) >= 1 && d >= 1 && d <= 256, who, ": bad cache shape ", keys.sizes());
+  TORCH_CHECK_VALUE(keys.size(f + 1) <= 0x7fffffff && keys.size(f + 2) <= MOST_HEADS && keys.size(0) <= 0x7fffffff, who, ": a cache of ", keys.sizes(),
+                    " is more than 32 bits count");
   TORCH_CHECK_VALUE((keys.stride(f + 3) == 1 && values.stride(f + 3) == 1) || d == 1, who, ": the cache's heads must be contiguous");
   require_index(table, who, "page_table", at::kInt, keys);
   require_index(lengths, who, "lengths", at::kInt, keys);
@@ -548,6 +553,7 @@ Step step_of_cache(const char *who, const Tensor &keys, const Tensor &values, co
                     who, ": page_table (B, pages), lengths (B,) and cu_tokens (B + 1,) are wanted, got ", table.sizes(), ", ", lengths.sizes(), ", ",
                     cu.sizes());
   TORCH_CHECK_VALUE(table.size(1) * keys.size(f + 1) < ((int64_t)1 << 31) - 4096, who, ": a sequence of ", table.size(1), " pages is too long");
+  TORCH_CHECK_VALUE(lengths.size(0) <= (int64_t)1 << 30, who, ": ", lengths.size(0), " sequences are too many");
   s.table = table.size(1) > 1 && table.stride(1) != 1 ? table.contiguous() : table;
   s.lengths = lengths.contiguous();
   s.cu = cu.contiguous();
@@ -601,6 +607,7 @@ Maybe append_kv(const Tensor &keys, const Tensor &values, const Tensor &table, c
     TORCH_CHECK_TYPE(q.scalar_type() == keys.scalar_type(), who, ": q and the cache must have one type, got ", q.scalar_type(), ", ", keys.scalar_type());
     TORCH_CHECK_VALUE(q.device() == keys.device() && q.dim() == 3 && q.size(0) == k.size(0) && q.size(1) >= 1 && q.size(2) == k.size(2), who,
                       ": q (T, heads, D) on the cache's device is wanted, got ", q.sizes(), " for k ", k.sizes());
+    TORCH_CHECK_VALUE(q.size(1) <= MOST_HEADS, who, ": up to ", MOST_HEADS, " query heads are supported, got ", q.size(1));
   }
   if (positions.has_value()) {
     require_cuda(*positions);
@@ -641,6 +648,8 @@ Tensor cached_attention(const Tensor &q, const Tensor &keys, const Tensor &value
   TORCH_CHECK_VALUE(d == s.cache.dim && h >= 1 && h % s.cache.kv_heads == 0, who, ": ", h, " query heads of ", d, " cannot share ", s.cache.kv_heads,
                     " key heads of ", s.cache.dim);
   TORCH_CHECK_VALUE(d <= 128, who, ": head sizes up to 128 are supported, got ", d);
+  TORCH_CHECK_VALUE(h <= 0x7fffffff && t <= 0x7fffffff && t * (h / s.cache.kv_heads) <= 0x7fffffff - 4096, who, ": ", t, " tokens of ", h / s.cache.kv_heads,
+                    " heads for a key head are more rows than one call takes");
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)d);
   TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale), who, ": scale must be positive and finite, got ", scale);
   Tensor bits;
@@ -701,6 +710,7 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor &tokens, const Ten
   for (const Tensor *x : {&tokens, &parents, &random})
     TORCH_CHECK_VALUE(x->dim() == 1 && x->size(0) == t, who, ": tokens, parents and random of ", t, " rows are wanted, got ", x->sizes());
   TORCH_CHECK_VALUE(cu.dim() == 1 && cu.size(0) >= 1, who, ": cu_tokens (B + 1,) is wanted, got ", cu.sizes());
+  TORCH_CHECK_VALUE(cu.size(0) - 1 <= 0x7fffffff, who, ": ", cu.size(0) - 1, " sequences are too many");
   ready();
   const c10::cuda::CUDAGuard guard(target.device());
   auto whole = [](const Tensor &x) { return (x.stride(1) == 1 || x.size(1) == 1) && (x.size(0) <= 1 || x.stride(0) >= x.size(1)) ? x : x.contiguous(); };

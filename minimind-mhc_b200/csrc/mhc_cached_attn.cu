@@ -961,6 +961,10 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
   if (int st = cache_view(who, cache, step, a.c)) return st;
   if (cache->dim > 128) return fail(MHC_ERR_SHAPE, "%s: head sizes up to 128 are supported (got %d)", who, cache->dim);
   if (H < 1 || H % cache->kv_heads) return fail(MHC_ERR_SHAPE, "%s: %d query heads cannot share %d key heads", who, H, cache->kv_heads);
+  // a sequence's rows (new tokens x heads of a group) are counted in 32 bits
+  if (step->T * (H / cache->kv_heads) > 0x7fffffff - 4096)
+    return fail(MHC_ERR_SHAPE, "%s: %lld tokens of %d heads for a key head are more rows than one call takes", who, (long long)step->T,
+                H / cache->kv_heads);
   a.c2 = (float)((double)scale * 1.4426950408889634);
   if (!(scale > 0.f) || !(a.c2 < INFINITY)) return fail(MHC_ERR_SHAPE, "%s: scale must be positive and finite (got %g)", who, scale);
   if (step->T == 0) return MHC_OK;

@@ -304,10 +304,11 @@ static int check_positions(const char *who, const void *p, int bytes) {
 int cache_view(const char *who, const mhc_kv_cache *c, const mhc_cache_step *s, cache::View &v) {
   if (!c || !s) return fail(MHC_ERR_NULL, "%s: cache or step is NULL", who);
   if (c->dtype != MHC_F32 && c->dtype != MHC_BF16 && c->dtype != MHC_F16) return fail(MHC_ERR_DTYPE, "%s: bad dtype code %d", who, c->dtype);
-  if (c->pages < 0 || c->pages > 0x7fffffff || c->page_size < 1 || c->kv_heads < 1 || c->dim < 1 || c->dim > rotary::MAX_D || c->layers < 0)
+  if (c->pages < 0 || c->pages > 0x7fffffff || c->page_size < 1 || c->kv_heads < 1 || c->kv_heads > 16384 || c->dim < 1 ||
+      c->dim > rotary::MAX_D || c->layers < 0)
     return fail(MHC_ERR_SHAPE, "%s: bad cache: %lld pages of %d, %d heads of %d, %d layers", who, (long long)c->pages, c->page_size,
                 c->kv_heads, c->dim, c->layers);
-  if (s->T < 0 || s->T > 0x7fffffff - 4096 || s->batch < 0 || s->table_width < 0 || (int64_t)s->table_width * c->page_size > 0x7fffffff - 4096)
+  if (s->T < 0 || s->T > 0x7fffffff - 4096 || s->batch < 0 || s->batch > 1 << 30 || s->table_width < 0 || (int64_t)s->table_width * c->page_size > 0x7fffffff - 4096)
     return fail(MHC_ERR_SHAPE, "%s: bad step: %lld rows, %d sequences, a table of %d pages of %d", who, (long long)s->T, s->batch,
                 s->table_width, c->page_size);
   if (s->batch > 0 && (!s->lengths || !s->cu_tokens || (s->table_width > 0 && !s->page_table)))
@@ -378,7 +379,7 @@ int mhc_append_kv(const mhc_kv_cache *cache, const mhc_cache_step *step, const v
   if (int st = cache_view(who, cache, step, a.c)) return st;
   if (!strides) return fail(MHC_ERR_NULL, "%s: strides is NULL", who);
   const int D = cache->dim;
-  if (H < 0 || H > 16384 || cache->kv_heads > 16384) return fail(MHC_ERR_SHAPE, "%s: %d query heads, %d key heads", who, H, cache->kv_heads);
+  if (H < 0 || H > 16384) return fail(MHC_ERR_SHAPE, "%s: %d query heads", who, H);
   if (r) {
     if (int st = rotary::check_rotary(who, r, D)) return st;
   } else {

@@ -195,3 +195,16 @@ def test_tree_mask():
     mask, depth = tree_mask(parents, torch.tensor([1, 5], dtype=torch.int32))
     assert mask[1:5].tolist() == [1, 3, 4, 11] and depth.tolist()[:5] == [0, 0, 1, 0, 2] and depth.tolist()[7] == 0
     assert tree_mask(parents[:0], torch.tensor([0], dtype=torch.int32))[0].numel() == 0
+
+
+def test_sizes_that_32_bits_do_not_hold(lib):
+    """Rows of an item are counted in 32 bits, and so are sequences and heads: what they do not hold is refused, where every
+    other limit of the call would let it pass."""
+    small = dict(kv_heads=1, dim=8)
+    for tokens, heads in ((1 << 27, 32), (1 << 26, 32), (1 << 20, 1 << 12)):
+        assert attend(lib, c=cache(**small), s=step(T=tokens, table_width=4), H=heads, n=1 << 50) == -3
+        assert b"rows" in lib.mhc_last_error()
+    wide = cache(kv_heads=16385)
+    assert append(lib, c=wide) == -3 and attend(lib, c=wide, H=16385, n=1 << 50) == -3 and lib.mhc_keep_drafts(wide, step(), P, P, None) == -3
+    many = step(batch=(1 << 30) + 1)
+    assert append(lib, s=many) == -3 and attend(lib, s=many, n=1 << 50) == -3 and lib.mhc_keep_drafts(cache(), many, P, P, None) == -3

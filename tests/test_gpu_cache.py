@@ -637,3 +637,19 @@ def test_refused():
             bad()
     with torch.no_grad():
         cached_attention(q.clone().requires_grad_(True), keys, values, step)
+
+
+def test_sizes_that_32_bits_do_not_hold():
+    """(Tensors of one element's memory: nothing is allocated before the refusal.)"""
+    one = torch.zeros(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+    keys = torch.zeros(4, 16, 1, 8, device="cuda", dtype=torch.bfloat16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    step = CacheStep(i32(0, 1)[None], i32(5), i32(0, 1))
+    for t, h in ((1 << 27, 32), (1 << 20, 1 << 12), (1, (1 << 32) + 1)):
+        with pytest.raises(ValueError, match="rows"):
+            cached_attention(one.expand(t, h, 8), keys, keys, step)
+    many = one.expand(1, (1 << 32) + 1, 8)
+    for bad in (lambda: rotate(Rotary(8), many, one), lambda: rotate(Rotary(8), one, many), lambda: append_kv(keys, keys, step, one, one, q=many, rotary=Rotary(8)),
+                lambda: append_kv(keys.expand(4, 16, (1 << 32) + 1, 8), keys.expand(4, 16, (1 << 32) + 1, 8), step, many, many)):
+        with pytest.raises(ValueError):
+            bad()
