@@ -17,9 +17,11 @@
 // keys and pages of 48, 16; of pages of 17, each by itself) and 64 columns, the lanes of a
 // warp one or two boxes each, across the ends of items too.  V rows that do
 // not exist are zeroed in shared memory (a P of 0 times a NaN would be NaN), and so are
-// infinities and NaN of new tokens' V, which some rows of the item do not see: the rows
-// that see one add it in the end.  The softmax threads do that, a row each, before they hand
-// over P.
+// infinities and NaN of those new tokens' V that some rows of the item do not see: the rows
+// that see one add it in the end.  (Without a mask those are the item's own tokens but the
+// first and what lies behind them, with one the sequence's first 64: however long a piece
+// of a prompt, a row looks through 128 keys at most.)  The softmax threads do that, half a row
+// of V each, before they hand over P.
 //
 // What bounds it: a tile takes a block 1.0 to 1.2 us (two of them an SM: 32 KB of K and V each,
 // at 128 rows the softmax's chain and 2^x, at 32 rows HBM: 1.5 us a tile is the copy rate); an item's
@@ -308,6 +310,7 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
       }
       const bool any_rows = warp * 32 < g.rows;
       const int n = g.k1 - g.k0;
+      const int shared = a.mask ? 0 : g.row0 / a.G + 1;  // new tokens that every row sees
       float ref = -INFINITY, sum = 0.f;
       for (int i = 0; i < n; ++i) {
         const int k0 = (g.k0 + i) * TN, s = i & 1;
@@ -394,12 +397,12 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
           f2_unpack(f2_add(acc[0], acc[1]), y, z);
           sum += y + z;
         }
-        const bool fresh = (g.s.n > 1 || a.mask) && k0 + TN > g.s.len;  // new tokens' V: not every row sees it
+        const bool fresh = k0 + TN - g.s.len > shared;  // V that not every row sees
         if (missing || fresh || k0 + TN > g.keys) {  // thread r looks after half of V's row r / 2
           const int tile = tile0 + i, st = tile % ST, vr = r >> 1, at = k0 + vr;
           if (!wait_warp_parity(BAR(B_VF + st), (uint32_t)(tile / ST) & 1u, abort_flag)) { ok = false; break; }
           const bool gone = at >= g.keys || ((missing >> (vr / rows)) & 1);
-          if (gone || (fresh && at >= g.s.len)) {
+          if (gone || (fresh && at - g.s.len >= shared)) {
             uint8_t *row = gen + (vs - base) + st * C::TILE + vr * 128;
 #pragma unroll
             for (int c = 0; c < C::FULL * 4; ++c) {
@@ -455,19 +458,26 @@ cached_attn_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__
       tc_fence_before();
       // (the next item's is set only after all have come to its queries)
       if (odd_item == items && x.j >= 0) {  // a row adds what it sees of the infinities and NaN that were taken out of V
-        for (int key = max(g.s.len, g.k0 * TN); key < min(g.keys, g.k1 * TN); ++key) {
+        const int first = max(g.s.len + shared, g.k0 * TN), end = min(min(g.keys, g.k1 * TN), g.s.len + (a.mask ? 64 : x.j + 1));
+        for (int key = first; key < end; ++key) {
           const int page = page_of(a, g, key);
           if (!sees(a.mask != nullptr, x.bits, x.j, key - g.s.len) || page < 0 || page >= a.c.pages) continue;
           const T *v = static_cast<const T *>(a.c.values) + page * a.c.vp + (key - cache::page_index(a.c, key) * a.c.size) * a.c.vs +
                        g.hk * a.c.vh;
-          for (int d = 0; d < a.c.D; ++d) {
-            const T y = v[d];
-            if (finite16<T>(*reinterpret_cast<const uint16_t *>(&y))) continue;
-            if (slot >= 0) {
-              a.part_o[((int64_t)slot * M + r) * DP + d] += to_f(y);
-            } else {
-              T *out = static_cast<T *>(a.out) + out_at(a, g, x, g.hk) + d;
-              *out = from_f<T>(to_f(*out) + to_f(y));
+          for (int d = 0; d < a.c.D; d += 8) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(v + d);
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint16_t bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+              if (finite16<T>(bits)) continue;
+              const float add = to_f(*reinterpret_cast<const T *>(&bits));
+              if (slot >= 0) {
+                a.part_o[((int64_t)slot * M + r) * DP + d + e] += add;
+              } else {
+                T *out = static_cast<T *>(a.out) + out_at(a, g, x, g.hk) + d + e;
+                *out = from_f<T>(to_f(*out) + add);
+              }
             }
           }
         }

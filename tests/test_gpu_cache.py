@@ -270,6 +270,40 @@ def test_infinite_values_that_are_seen(dtype, page, new, columns):
     assert torch.equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("dtype,group,new,lens", ((torch.bfloat16, 2, 8000, 0), (torch.float16, 1, 4000, 37), (torch.bfloat16, 4, 3000, 1000)))
+def test_one_infinity_in_a_long_piece(dtype, group, new, lens):
+    """One overflowed value among thousands of new tokens: it reaches its column of the rows that see it, and costs what its
+    neighbourhood costs, not a search of the whole piece by every row (that took 36 times as long with 2048 tokens, 146 with
+    8192, and with longer pieces more than the kernel's other warps wait)."""
+    q, keys, values, step, k, v = make([lens], [new], group, 1, 64, 64, dtype, columns=9)
+
+    def timed():
+        best = math.inf
+        for _ in range(4):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            out = cached_attention(q, keys, values, step)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        return out, best
+
+    clean, usual = timed()
+    for bit in (3, new // 2 + 1, new - 1):
+        at = lens + bit
+        where = step.page_table[0, at // 64], at % 64, 0, 5
+        was = values[where].clone()
+        values[where] = math.inf
+        got, took = timed()
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[bit:, :, 5] = True
+        assert (got[hit] == math.inf).all()
+        assert torch.equal(got[~hit], clean[~hit])
+        assert took < 8 * usual
+        values[where] = was
+    assert torch.equal(cached_attention(q, keys, values, step), clean)
+
+
 @pytest.mark.parametrize("dtype,page,new", ((torch.bfloat16, 16, 1), (torch.bfloat16, 17, 9), (torch.bfloat16, 16, 30), (torch.float32, 16, 3)))
 @pytest.mark.parametrize("columns", (2, 90))
 def test_scores_at_the_ends(dtype, page, new, columns):
