@@ -86,13 +86,16 @@ def tree_mask(parents: torch.Tensor, cu_tokens: torch.Tensor) -> tuple[torch.Ten
     """(mask, depth) of drafted trees: for every row the bits of itself and its ancestors, and how many ancestors it has.
 
     ``parents`` (T,) is the index of a row's parent within its sequence, below its own; -1 for the first.  (A row whose
-    parent is none of that, rows of no sequence among them, is taken for a first one.)  Trees of up to 64 rows.  Plain torch operations, on the tensors' device and without waiting for it: a tree that stays the same is
-    done once.
+    parent is none of that is taken for a first one, and so are all rows of no sequence.)  Trees of up to 64 rows.  Plain
+    torch operations, on the tensors' device and without waiting for it: a tree that stays the same is done once.
     """
+    if parents.dim() != 1 or cu_tokens.dim() != 1 or cu_tokens.numel() < 1:
+        raise ValueError(f"tree_mask: parents (T,) and cu_tokens (B + 1,) are wanted, got {tuple(parents.shape)}, {tuple(cu_tokens.shape)}")
     t = parents.shape[0]
     at = torch.arange(t, device=parents.device)
     start = cu_tokens.long()[torch.searchsorted(cu_tokens[1:].long().contiguous(), at, right=True).clamp(max=cu_tokens.numel() - 2)]
-    child = (parents >= 0) & (parents < at - start)
+    start = torch.where(at < cu_tokens[-1], start, at)  # rows behind the last sequence are their own first ones
+    child = (parents >= 0) & (parents < at - start) & (start >= 0)
     up = torch.where(child, start + parents.long(), at)  # a root is its own parent
     mask = torch.ones_like(at) << (at - start).clamp(0, 63)
     depth = child.long()

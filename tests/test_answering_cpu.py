@@ -208,3 +208,21 @@ def test_sizes_that_32_bits_do_not_hold(lib):
     assert append(lib, c=wide) == -3 and attend(lib, c=wide, H=16385, n=1 << 50) == -3 and lib.mhc_keep_drafts(wide, step(), P, P, None) == -3
     many = step(batch=(1 << 30) + 1)
     assert append(lib, s=many) == -3 and attend(lib, s=many, n=1 << 50) == -3 and lib.mhc_keep_drafts(cache(), many, P, P, None) == -3
+
+
+def test_tree_mask_of_rows_of_no_sequence():
+    """They are first ones, whatever their parents look like; offsets that are none index nothing."""
+    from model.mhc_cache import tree_mask
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    mask, depth = tree_mask(i32(-1, 0, 1, 0, 1, 2), i32(0, 3))
+    assert mask.tolist() == [1, 3, 7, 1, 1, 1] and depth.tolist() == [0, 1, 2, 0, 0, 0]
+    mask, depth = tree_mask(i32(0, 0, -1, 0, 1, 0, 2), i32(2, 2, 4, 4))
+    assert mask.tolist() == [1, 1, 1, 3, 1, 1, 1] and depth.tolist() == [0, 0, 0, 1, 0, 0, 0]
+    mask, depth = tree_mask(i32(0, 0, 1), i32(0))
+    assert mask.tolist() == [1, 1, 1] and depth.tolist() == [0, 0, 0]
+    for cu in (i32(-2 ** 31, 2 ** 31 - 1), i32(-9, -5, 2), i32(2 ** 31 - 1, -7, 3), i32(5, 1, 0)):
+        mask, depth = tree_mask(i32(0, 1, 2, 0), cu)
+        assert mask.shape == depth.shape == (4,) and (depth >= 0).all() and (depth < 4).all()
+    for bad in (lambda: tree_mask(i32(-1, 0), i32()), lambda: tree_mask(i32(-1, 0)[None], i32(0, 2)), lambda: tree_mask(i32(-1, 0), i32(0, 2)[None])):
+        with pytest.raises(ValueError):
+            bad()
