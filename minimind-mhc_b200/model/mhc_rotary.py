@@ -77,9 +77,10 @@ class Rotary:
         self.dim, self.interleaved, self.gain = dim, bool(interleaved), 1.0 if gain is None else float(gain)
         if not math.isfinite(self.gain):
             raise ValueError(f"Rotary: gain must be finite, got {gain}")
-        self.inv_freq = torch.tensor(inv, dtype=torch.float64)
         turns = [_turns_of(f) for f in inv]
-        self._host = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
+        with torch.inference_mode(False):  # a later training step keeps them for its backward pass
+            self.inv_freq = torch.tensor(inv, dtype=torch.float64)
+            self._host = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
         self._on = {}
         if device is not None or torch.cuda.is_available():
             self.turns(torch.device("cuda" if device is None else device))
@@ -91,7 +92,8 @@ class Rotary:
             device = torch.device("cuda", torch.cuda.current_device())
         got = self._on.get(device)
         if got is None:
-            got = self._on[device] = self._host.to(device)
+            with torch.inference_mode(False):
+                got = self._on[device] = self._host.to(device)
         return got
 
 

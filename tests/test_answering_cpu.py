@@ -226,3 +226,15 @@ def test_tree_mask_of_rows_of_no_sequence():
     for bad in (lambda: tree_mask(i32(-1, 0), i32()), lambda: tree_mask(i32(-1, 0)[None], i32(0, 2)), lambda: tree_mask(i32(-1, 0), i32(0, 2)[None])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_frequencies_made_in_inference_mode():
+    """An evaluation that is a rotation's first use leaves frequencies that a training step can keep for its backward pass."""
+    from model.mhc_rotary import Rotary
+    outside = Rotary(16, device="cpu")
+    with torch.inference_mode():
+        inside = Rotary(16, device="cpu")
+        late = outside.turns("meta")
+    for x in (inside.turns("cpu"), inside._host, inside.inv_freq, late):
+        assert not x.is_inference()
+    assert torch.equal(inside.turns("cpu"), outside.turns("cpu"))

@@ -257,3 +257,14 @@ def test_positions_changed_before_the_backward_pass():
     pos += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         a.sum().backward()
+
+
+def test_made_in_inference_mode():
+    with torch.inference_mode():
+        rotary = Rotary(32)
+        q = torch.randn(9, 4, 32, device="cuda")
+        check(rotate(rotary, q, q)[0], rotary, q, torch.arange(9, device="cuda"))
+    q = torch.randn(9, 4, 32, device="cuda", requires_grad=True)
+    g = torch.randn(9, 4, 32, device="cuda")
+    d, = torch.autograd.grad(rotate(rotary, q, q.detach())[0], q, g)
+    check(d, rotary, g, torch.arange(9, device="cuda"), -1.0)
