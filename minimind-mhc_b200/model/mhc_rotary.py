@@ -79,8 +79,8 @@ class Rotary:
             raise ValueError(f"Rotary: gain must be finite, got {gain}")
         turns = [_turns_of(f) for f in inv]
         with torch.inference_mode(False):  # a later training step keeps them for its backward pass
-            self.inv_freq = torch.tensor(inv, dtype=torch.float64)
-            self._host = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
+            self.inv_freq = torch.tensor(inv, dtype=torch.float64, device="cpu")
+            self._host = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device="cpu")
         self._on = {}
         if device is not None or torch.cuda.is_available():
             self.turns(torch.device("cuda" if device is None else device))

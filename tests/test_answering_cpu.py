@@ -238,3 +238,13 @@ def test_frequencies_made_in_inference_mode():
     for x in (inside.turns("cpu"), inside._host, inside.inv_freq, late):
         assert not x.is_inference()
     assert torch.equal(inside.turns("cpu"), outside.turns("cpu"))
+
+
+@pytest.mark.parametrize("device", ("meta", "cpu"))
+def test_frequencies_under_another_default_device(device):
+    """A model whose parameters are laid out later is built under a default device that holds no values."""
+    from model.mhc_rotary import Rotary
+    with torch.device(device):
+        r = Rotary(16, device="cpu")
+    assert r._host.device.type == r.inv_freq.device.type == "cpu"
+    assert torch.equal(r.turns("cpu"), Rotary(16, device="cpu").turns("cpu"))
