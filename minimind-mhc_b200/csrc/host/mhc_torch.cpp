@@ -577,6 +577,13 @@ Step step_of_cache(const char *who, const Tensor &keys, const Tensor &values, co
   s.step.T = t;
   return s;
 }
+// what is written to must not be expanded: two places would be one memory, and which of them comes last is nobody's choice
+void require_own_places(const char *who, std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    for (int64_t i = 0; i < t->dim(); ++i)
+      TORCH_CHECK_VALUE(t->size(i) <= 1 || t->stride(i) != 0, who, ": keys and values are written to and must not be expanded, got sizes ", t->sizes(),
+                        " with strides ", t->strides());
+}
 void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -592,6 +599,7 @@ Maybe append_kv(const Tensor &keys, const Tensor &values, const Tensor &table, c
   require_cuda(v);
   TORCH_CHECK_VALUE(k.dim() == 3 && k.sizes() == v.sizes(), who, ": k and v (T, heads, D) are wanted, got ", k.sizes(), ", ", v.sizes());
   Step s = step_of_cache(who, keys, values, table, lengths, cu, k.size(0), false);
+  require_own_places(who, {&keys, &values});
   TORCH_CHECK_VALUE(k.size(1) == s.cache.kv_heads && k.size(2) == s.cache.dim, who, ": k and v ", k.sizes(), " do not fit the cache ", keys.sizes());
   TORCH_CHECK_TYPE(k.scalar_type() == keys.scalar_type() && v.scalar_type() == keys.scalar_type(), who, ": k, v and the cache must have one type, got ",
                    k.scalar_type(), ", ", v.scalar_type(), ", ", keys.scalar_type());
@@ -676,6 +684,7 @@ void keep_drafts(const Tensor &keys, const Tensor &values, const Tensor &table, 
   require_no_grad(who, {&keys, &values});
   TORCH_CHECK_VALUE(path.dim() == 1, who, ": path (T,) is wanted, got ", path.sizes());
   Step s = step_of_cache(who, keys, values, table, lengths, cu, path.size(0), true);
+  require_own_places(who, {&keys, &values});
   require_index(path, who, "path", at::kInt, keys);
   require_index(kept, who, "kept", at::kInt, keys);
   TORCH_CHECK_VALUE(kept.sizes() == lengths.sizes(), who, ": a number of kept tokens for every sequence is wanted, got ", kept.sizes());

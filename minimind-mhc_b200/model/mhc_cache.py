@@ -26,7 +26,8 @@ from .mhc_rotary import Rotary
 class PagedCache:
     """Keys and values of all layers in pages of ``page_size`` tokens: ``keys`` and ``values`` are (layers, pages,
     page_size, kv_heads, dim).  Which page belongs to whom is the caller's bookkeeping.  The functions below take any
-    tensors of that shape (one layer: without the first dimension), whatever their strides, with contiguous heads."""
+    tensors of that shape (one layer: without the first dimension), whatever their strides, with contiguous heads; those
+    that write to them no expanded ones."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, dim: int, dtype=torch.bfloat16, device="cuda"):
         shape = (layers, pages, page_size, kv_heads, dim)

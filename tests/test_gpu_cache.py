@@ -687,3 +687,22 @@ def test_sizes_that_32_bits_do_not_hold():
                 lambda: append_kv(keys.expand(4, 16, (1 << 32) + 1, 8), keys.expand(4, 16, (1 << 32) + 1, 8), step, many, many)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_expanded_caches():
+    """They can be read (one layer's pages for all, one head for all) and not written to."""
+    q, keys, values, step, k, v = make([9, 3], [2, 1], 4, 1, 32, 8, torch.bfloat16)
+    heads = keys.expand(-1, -1, 2, -1), values.expand(-1, -1, 2, -1)
+    got = cached_attention(q, *heads, step)
+    want = cached_attention(q, *(x.repeat(1, 1, 2, 1) for x in (keys, values)), step)
+    assert err(got, want.double()) <= U[torch.bfloat16]
+    kk = torch.zeros(3, 2, 32, device="cuda").bfloat16()
+    path, kept = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    layers = keys.expand(3, -1, -1, -1, -1), values.expand(3, -1, -1, -1, -1)
+    before = keys.clone(), values.clone()
+    for bad in (lambda: append_kv(*heads, step, kk, kk), lambda: append_kv(heads[0], values.repeat(1, 1, 2, 1), step, kk, kk),
+                lambda: keep_drafts(*heads, step, path, kept), lambda: keep_drafts(*layers, step, path, kept),
+                lambda: append_kv(keys[:1].expand(6, -1, -1, -1), values[:1].expand(6, -1, -1, -1), step, kk[:, :1], kk[:, :1])):
+        with pytest.raises(ValueError, match="expanded"):
+            bad()
+    assert all(torch.equal(x.nan_to_num(), y.nan_to_num()) for x, y in zip(before, (keys, values)))
