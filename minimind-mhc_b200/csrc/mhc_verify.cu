@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(THREADS, 2) verify_kernel(const Args a) {
         r.gone += mass;
         mass = sum_rest();
       } else {
-        mass = fmax(mass - left, 0.0);  // a row may sum to a little more than 1
+        // (only numbers of 1 and more refuse what has more than the mass; below 0 a token that the row does not hold would pass)
+        mass = fmax(mass - left, 0.0);
         __syncthreads();
         if (tid == 0) sh.refused[r.refused] = sh.token[x];
         ++r.refused;

@@ -256,3 +256,15 @@ def test_refused():
             verify_drafts(*({"tokens": tokens, "parents": parents, "cu": cu, "target": target, "draft": draft, "random": random} | bad).values())
     with pytest.raises(RuntimeError, match="CUDA"):
         verify_drafts(tokens, parents, cu, target, draft, random.cpu())
+
+
+def test_numbers_outside_their_range():
+    """Without a draft: 3 refuses a child that has more than is left of the mass, which would fall below 0 then, and 2 times
+    that is less than the 0 of a token that the row does not hold: it must not be kept for it.  (With numbers below 1 a
+    refused child never has more than the mass.)"""
+    target = torch.zeros(4, 9, device="cuda")
+    target[:, 2], target[:, 4] = 0.75, 0.5  # a row that sums to more than 1
+    cu, parents = torch.tensor([0, 4], dtype=torch.int32, device="cuda"), torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
+    random = torch.tensor([0.3, 1.0, 3.0, 2.0], device="cuda")
+    got = check(torch.tensor([0, 2, 4, 7], device="cuda"), parents, cu, target, None, random)
+    assert got.path.tolist() == [0, -1, -1, -1] and got.kept.tolist() == [1] and got.next.tolist() == [2]
