@@ -37,9 +37,10 @@ class Rotary:
     2 i with 2 i + 1.  Pair i turns by ``theta ** (-2 i / dim)`` radians a position.  ``factor`` above 1 stretches the
     positions for longer contexts: by itself all frequencies are divided by it; with ``original_length``, the trained
     length, only the slow ones: those that turn less than ``slow`` times within it are divided, those that turn more than
-    ``fast`` times left, with a ramp between (the reference's ``rope_scaling``), and cosines and sines are multiplied by
-    ``gain``, 0.1 log(factor) + 1 if it is not given (1 without ``original_length``).  ``inv_freq`` sets the dim / 2
-    frequencies (radians a position) in place of all that.
+    ``fast`` times left, with a ramp over the pairs between.  Cosines and sines are multiplied by ``gain``: with
+    ``original_length`` and a factor above 1 it is 0.1 log(factor) + 1 if it is not given, else 1.  It belongs to the
+    weights like the frequencies do: a model whose scaled positions leave cosines and sines as they are (an attention
+    factor of 1) needs ``gain=1.0``.  ``inv_freq`` sets the dim / 2 frequencies (radians a position) in place of all that.
 
     The frequencies lie on ``device`` (the current CUDA device) and are copied to another device at the first call
     there, which a CUDA graph cannot capture."""

@@ -248,3 +248,30 @@ def test_frequencies_under_another_default_device(device):
         r = Rotary(16, device="cpu")
     assert r._host.device.type == r.inv_freq.device.type == "cpu"
     assert torch.equal(r.turns("cpu"), Rotary(16, device="cpu").turns("cpu"))
+
+
+@pytest.mark.parametrize("dim,theta,factor,length,fast,slow", ((96, 1e6, 16.0, 2048, 32.0, 1.0), (128, 1e4, 4.0, 4096, 32.0, 1.0), (64, 1e6, 8.0, 512, 4.0, 0.5)))
+def test_scaled_tables(dim, theta, factor, length, fast, slow):
+    """Pair by pair, and the tables that a model with an attention factor of 1, or of its own, multiplies with: pair i turns
+    length theta^(-2i/dim) / 2 pi times within the trained length; the pairs at which that is `fast` and `slow`, rounded
+    outwards, are the ramp's ends."""
+    import math
+
+    from model.mhc_rotary import Rotary
+    lo = max(math.floor(dim / 2 * math.log(length / (2 * math.pi * fast), theta)), 0)
+    hi = min(math.ceil(dim / 2 * math.log(length / (2 * math.pi * slow), theta)), dim // 2 - 1)
+    assert 0 <= lo < hi
+    position = torch.arange(0, 4 * length, 97, dtype=torch.float64)[:, None]
+    for gain in (1.0, 1.5):
+        r = Rotary(dim, theta, factor=factor, original_length=length, fast=fast, slow=slow, gain=gain)
+        assert r.gain == gain
+        want = []
+        for i in range(dim // 2):
+            f = theta ** (-2 * i / dim)
+            part = 0.0 if i <= lo else 1.0 if i >= hi else (i - lo) / (hi - lo)
+            want.append(f * (1 - part) + f / factor * part)
+        want = torch.tensor(want, dtype=torch.float64)
+        assert torch.allclose(r.inv_freq, want, rtol=1e-14, atol=0)
+        # angles up to 4 length, off by 1e-14 of themselves
+        assert torch.allclose((position * r.inv_freq).cos() * r.gain, (position * want).cos() * gain, rtol=0, atol=4 * length * 1e-14 * gain + 1e-15)
+    assert Rotary(dim, theta, factor=1.0, original_length=length).gain == 1.0
