@@ -488,7 +488,9 @@ int mhc_cached_attn(const mhc_kv_cache *cache, const mhc_cache_step *step, const
  * are a tree in which a parent comes before its children: row 0 its last token,
  * the others drafted ones with tokens[t] and parents[t] (index within the sequence).
  * Row t of target (T, V) holds the target's probabilities behind node t, of draft
- * those that the children of t were drawn from (NULL: the children were not drawn).
+ * those that the children of t were drawn from, independently of each other and with
+ * replacement (NULL: the children were not drawn).  Children drawn without replacement
+ * leave answers of another distribution than the target's.
  * Rows of probabilities are target_stride and draft_stride elements apart, of type
  * `dtype`, and taken to sum to 1.  random (T) fp32 in [0, 1).
  *

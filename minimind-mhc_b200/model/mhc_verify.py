@@ -4,6 +4,10 @@
 
 decides which of a step's drafted tokens are kept, so that the answer is distributed as if the target had drawn every
 token itself, and draws the next one.  The random numbers are the caller's.  CUDA tensors only.
+
+That holds where the children of a row are drawn from its row of ``draft`` independently of each other, with replacement
+(the same token may come twice), or, without ``draft``, are chosen without chance.  Children drawn without replacement, as
+``torch.multinomial`` draws several unless told otherwise, give another distribution.
 """
 
 from __future__ import annotations
@@ -28,7 +32,7 @@ def verify_drafts(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.
     Sequence b's rows are ``[cu_tokens[b], cu_tokens[b + 1])``: its last token, then the drafted ones, each behind its
     parent; ``parents`` (T,) int32 index within the sequence, -1 for the first row.  ``tokens`` (T,) int64.  Row t of
     ``target`` (T, V) holds the target's probabilities of the token behind row t, row t of ``draft`` those that the
-    children of t were drawn from; ``None`` where they were not drawn (the draft's best, for one).  Both fp32, bf16 or
+    children of t were drawn from, each by itself; ``None`` where they were not drawn (the draft's best, for one).  Both fp32, bf16 or
     fp16, alike, rows that sum to one.  ``random`` (T,) fp32 in [0, 1).
 
     The children x of the last kept row are tested in their order.  With rest the target's row and mass 1 at first, x is
