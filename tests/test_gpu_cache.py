@@ -304,6 +304,35 @@ def test_one_infinity_in_a_long_piece(dtype, group, new, lens):
     assert torch.equal(cached_attention(q, keys, values, step), clean)
 
 
+@pytest.mark.parametrize("dtype,page", ((torch.bfloat16, 16), (torch.float16, 17), (torch.bfloat16, 64), (torch.float32, 16)))
+@pytest.mark.parametrize("group,lens", ((1, 0), (3, 70), (8, 5)))
+@pytest.mark.parametrize("columns", (1, 90))
+def test_lost_tokens_of_a_piece(dtype, page, group, lens, columns):
+    """No mask, several tiles of rows: a new token of nothing but NaN is lost with those behind it, one infinity of V reaches
+    its column of these rows, and the rows before are as they were, wherever in a tile it lies."""
+    new = 300
+    q, keys, values, step, k, v = make([lens, 3], [new, 2], 2 * group, 2, 64, page, dtype, columns=columns)
+    clean = cached_attention(q, keys, values, step)
+    for bit in (0, 1, 63, 64, 127, 128, 130, new - 1):
+        at = lens + bit
+        where = step.page_table[0, at // page], at % page
+        kept = keys[where].clone(), values[where].clone()
+        values[where + (1, 7)] = -math.inf
+        got = cached_attention(q, keys, values, step)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[bit:new, group:, 7] = True
+        assert (got[hit] == -math.inf).all()
+        assert torch.equal(got[~hit], clean[~hit])
+        keys[where], values[where] = NAN, NAN
+        got = cached_attention(q, keys, values, step)
+        assert got[bit:new].isnan().all()
+        seen = torch.cat((got[:bit], got[new:])), torch.cat((clean[:bit], clean[new:]))
+        # (the references that the sums go by may be other ones)
+        assert err(seen[0], seen[1].double()) < 2 * OUT[dtype] * U[dtype]
+        keys[where], values[where] = kept
+    assert torch.equal(cached_attention(q, keys, values, step), clean)
+
+
 @pytest.mark.parametrize("dtype,page,new", ((torch.bfloat16, 16, 1), (torch.bfloat16, 17, 9), (torch.bfloat16, 16, 30), (torch.float32, 16, 3)))
 @pytest.mark.parametrize("columns", (2, 90))
 def test_scores_at_the_ends(dtype, page, new, columns):
