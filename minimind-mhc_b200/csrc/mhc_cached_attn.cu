@@ -62,12 +62,18 @@ constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int CHUNK = 16;           // keys that a warp takes at a time
 constexpr int KT = CHUNK * WARPS;   // keys of a tile
-// Where the page table has room for so few keys, an item is one block's: nothing is cut and nothing joined.
+// Where the page table has room for so few keys, an item is one block's: nothing is cut and nothing joined.  8 / 4 heads of
+// 96, bf16, every table full, us, whole items / cut ones: one new token in each of 1, 16 and 64 sequences of 256 keys
+// 9.1 / 10.5, 10.9 / 13.0 and 13.0 / 18.6; of 512 keys 12.2 / 9.5, 14.0 / 11.7 and 19.3 / 20.6; of 1024 keys 17.9 / 9.9, 20.7 /
+// 13.5 and 29.6 / 28.7; with 16 new tokens of 512 keys 15.4 / 13.1, 16.9 / 18.9 and 18.0 / 29.1, of 1024 22.4 / 14.9, 24.1 / 20.7
+// and 27.8 / 39.8.
 constexpr int WHOLE = 512;
 // Rows of an item above which the tcgen05 kernel takes over, by the rows of a TMA box: small boxes are many copies for a
 // tile.  16 sequences, up to 8192 keys, 8 / 4 heads of 96, trees of 16 (32 rows) and of 64 (128 rows), us, tcgen05 / warps:
 // pages of 16 (boxes of 16) 38 / 60 and 38 / 145; of 100 (boxes of 4) 57 / 60 and 58 / 145; of 34 (2) 87 / 61 and 86 / 146;
-// of 17 (1) 151 / 58 and 146 / 146.
+// of 17 (1) 151 / 58 and 146 / 146.  Other shapes in pages of 64, with 8, 16 and 32 rows: 64 sequences up to 4096 keys, 8 / 2
+// heads of 128, 42 / 41, 41 / 46 and 42 / 67; one sequence of 65,536, 8 / 4 heads of 128, 34 / 39, 34 / 43 and 35 / 55; 4 up to
+// 16,384, 8 / 1 heads of 64, 14 / 17, 15 / 19 and 14 / 16.
 static int tc_from(int box) { return box >= 4 ? 16 : box == 2 ? 48 : 128; }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {

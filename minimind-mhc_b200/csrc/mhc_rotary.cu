@@ -23,7 +23,7 @@
 // registers of a thread that walks over its heads the instructions are a third, but a
 // warp's accesses lie 1.5 KB apart, and 16384 tokens of 12 heads of 96 took 27 us for 15.
 // Measured: those 14.7 us (75 MB, 5.1 TB/s), 8191 tokens of 10 heads of 128 in fp32 14.4 us
-// (84 MB, 5.8 TB/s); into a cache 24 prompts, 17,900 tokens, 24 us (110 MB, 4.5 TB/s), one token of
+// (84 MB, 5.8 TB/s); into a cache 24 prompts, 17,900 tokens, 24 us (110 MB, 4.5 TB/s; fp32 40 us, 5.4), one token of
 // each of 16 sequences 3.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

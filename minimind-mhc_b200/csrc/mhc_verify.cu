@@ -25,7 +25,8 @@
 // Measured: 32 sequences with trees of up to 32 rows, 100,003 tokens: 29 us, of which a pass over
 // both rows takes 4.6 (26 MB for all sequences, HBM or L2) and the slowest sequence has three; a
 // chain of six over 6400 tokens 8 us: launch, two chains of loads (rows, then their probabilities)
-// and one pass.
+// and one pass.  The trees without a draft take 30 us (every element is held against the refused
+// tokens), with 16-bit probabilities 25 where fp32 ones that L2 holds take 24.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
