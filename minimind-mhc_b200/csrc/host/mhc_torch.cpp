@@ -468,6 +468,10 @@ struct RotateFn : torch::autograd::Function<RotateFn> {
     ctx->saved_data["gain"] = gain;
     ctx->set_materialize_grads(false);
     const Turned out = turn(q, k, pos, period, turns, interleaved, gain, false);
+    variable_list frozen;
+    if (!q.requires_grad()) frozen.push_back(out.q);
+    if (!k.requires_grad()) frozen.push_back(out.k);
+    ctx->mark_non_differentiable(frozen);
     return {out.q, out.k};
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {

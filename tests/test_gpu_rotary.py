@@ -268,3 +268,26 @@ def test_made_in_inference_mode():
     g = torch.randn(9, 4, 32, device="cuda")
     d, = torch.autograd.grad(rotate(rotary, q, q.detach())[0], q, g)
     check(d, rotary, g, torch.arange(9, device="cuda"), -1.0)
+
+
+def test_what_is_frozen_wants_no_gradient():
+    """As with torch's operators: the turned keys of frozen keys are no part of the graph, so that attention behind them
+    computes no gradient for them and a cache takes them."""
+    rotary = Rotary(32)
+    q, k = torch.randn(9, 4, 32, device="cuda"), torch.randn(9, 2, 32, device="cuda")
+    g = torch.randn(9, 4, 32, device="cuda")
+    at = torch.arange(9, device="cuda")
+    a, b = rotate(rotary, q.clone().requires_grad_(True), k)
+    assert a.requires_grad and not b.requires_grad and b.grad_fn is None
+    check(b, rotary, k, at)
+    leaf = k.clone().requires_grad_(True)
+    a, b = rotate(rotary, q, leaf)
+    assert b.requires_grad and not a.requires_grad
+    check(a, rotary, q, at)
+    check(torch.autograd.grad(b, leaf, g[:, :2])[0], rotary, g[:, :2], at, -1.0)
+    leaf = q.clone().requires_grad_(True)
+    both = rotate(rotary, leaf, leaf)
+    assert all(x.requires_grad for x in both)
+    d, = torch.autograd.grad(both, leaf, (g, g))
+    want = reference(rotary, g, at, -1.0)[0] * 2
+    assert (d.double() - want).abs().max() <= 32 * U[torch.float32] * 2 * g.abs().max().item() * math.sqrt(2)
